@@ -1020,6 +1020,58 @@ int pa_conv_rope_norm_append_rows(const void* d_in, int64_t in_stride, int in_of
                                   const int32_t* d_items, int num_items, int item_tokens, int64_t rows, int elem, pa_stream_t stream);
 int pa_conv_append_in_words(int units, int columns, int num_items, int64_t rows);
 
+/* ---- verifying trees of drafted tokens (no reference implementation) ------------------------------------------------
+ * Sequence b brings the drafted nodes d_node_start[b] .. d_node_start[b + 1] - 1 (rows of all arrays below), numbered parents
+ * first; node i's K/V rows stand at position d_ctx_lens[b] + i of table row d_beam_ids[b] (NULL: b).  At most
+ * PA_TREE_MOST_NODES nodes a sequence (more: PA_ERR_UNSUPPORTED); most_nodes bounds them.
+ *
+ * pa_tree_attention: row r of d_q ([heads][head_dim], rows q_stride elements apart) attends, with head h on kv head
+ *   h / (heads / kv_heads), the positions below d_ctx_lens[b] and the position d_ctx_lens[b] + j of every bit j of its mask
+ *   (d_mask [rows][mask_words], bit j & 31 of word j >> 5; bits of nodes that the sequence has not are ignored):
+ *     s = q . k / temperature, p = exp(s - max) / (sum + 1e-6), out[r] = sum p v        (as pa_paged_decode_*)
+ *   Keys that a row does not see, or on pages that are unmapped or out of range, contribute nothing, whatever they hold; a row
+ *   that sees nothing is zero.  d_out [rows][heads][head_dim] of the queries' type.  Types (q, pools): f32 with f16, i8, f32;
+ *   f16 with f16, i8; bf16 with bf16.  i8 pools have a scale per row and are read as q / scale.  head_dim <= 256.
+ *   The workspace holds the partial results of keys that were split; d_workspace may be NULL where the function of its size
+ *   returns 0.
+ * pa_adjust_logits: row r of d_logits (rows `stride` elements apart; type PA_TYPE_F32, _F16 or _BF16) belongs to sequence
+ *   d_row_seq[r] (NULL: r).  With c the number of times a token v stands in d_history[d_history_start[b] ..
+ *   d_history_start[b + 1] - 1] and, where d_tokens is given, on the way from the root to row r's node (itself included):
+ *     c > 0: x = x > 0 ? x / repetition : x * repetition, x -= presence, x -= frequency * c;   x += bias;
+ *     a bit of d_allowed that is 0: x = -inf
+ *   penalties per sequence (device arrays), or one value where the array is NULL.  Biases of sequence b are the entries
+ *   d_bias_start[b] .. of (d_bias_ids, d_bias); of entries for the same token the last counts.  d_allowed: rows of
+ *   allowed_stride 32-bit words, row d_allowed_rows[r] (NULL: r; negative: everything is allowed).  Tokens outside the
+ *   vocabulary are ignored.  d_out (NULL: not wanted; may be d_logits) gets the logits in their type, d_ids (NULL: not wanted)
+ *   the lowest index of the largest float before it is rounded (NaN never wins; 0 where nothing does).
+ * pa_tree_accept: from node 0 to the child whose token is the one chosen at the node (d_ids[row]; of several the lowest) as
+ *   long as there is one.  d_counts[b]: nodes on that path (0 for a sequence without nodes); d_nodes, d_out_tokens
+ *   [num_seqs][depth]: the nodes and what was chosen at them, -1 behind them; d_new_lens[b] = d_ctx_lens[b] + d_counts[b].
+ *   The K/V rows of path node d move from position ctx + node to ctx + d in each of num_caches caches of one geometry
+ *   (caches: HOST array of num_caches x {keys, values, key scales, value scales, table}, the middle three may be NULL;
+ *   key_bytes / value_bytes of a row); rows on unmapped pages stay. */
+#define PA_TYPE_F32 0
+#define PA_TYPE_F16 1
+#define PA_TYPE_BF16 2
+#define PA_TYPE_I8 3
+#define PA_TREE_MOST_NODES 1024
+size_t pa_tree_attention_workspace_bytes(int rows, int num_seqs, int most_nodes, int heads, int kv_heads, int head_dim);
+int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void* d_out, const void* d_k_pool, const void* d_v_pool,
+                      const float* d_k_scales, const float* d_v_scales, int kv_type, const int32_t* d_table, int num_beams, int kv_heads,
+                      int num_tiles, int total_pages, const int32_t* d_beam_ids, const int32_t* d_ctx_lens, const int32_t* d_node_start,
+                      const int32_t* d_mask, int mask_words, int rows, int num_seqs, int most_nodes, int heads, int head_dim,
+                      int tile_size, float temperature, void* d_workspace, size_t workspace_bytes, pa_stream_t stream);
+int pa_adjust_logits(const void* d_logits, int type, int64_t stride, int rows, int vocab, void* d_out, int64_t out_stride,
+                     int32_t* d_ids, const int32_t* d_row_seq, const int32_t* d_history, const int32_t* d_history_start,
+                     const float* d_repetition, const float* d_presence, const float* d_frequency, float repetition, float presence,
+                     float frequency, const int32_t* d_bias_ids, const float* d_bias, const int32_t* d_bias_start,
+                     const int32_t* d_allowed, int64_t allowed_stride, const int32_t* d_allowed_rows, const int32_t* d_tokens,
+                     const int32_t* d_parents, const int32_t* d_node_start, pa_stream_t stream);
+int pa_tree_accept(const int32_t* d_ids, const int32_t* d_tokens, const int32_t* d_parents, const int32_t* d_node_start, int num_seqs,
+                   int most_nodes, int depth, const int32_t* d_ctx_lens, const int32_t* d_beam_ids, int num_beams, int kv_heads,
+                   int num_tiles, int total_pages, int tile_size, int key_bytes, int value_bytes, int num_caches, void* const* caches,
+                   int32_t* d_counts, int32_t* d_out_tokens, int32_t* d_nodes, int32_t* d_new_lens, pa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

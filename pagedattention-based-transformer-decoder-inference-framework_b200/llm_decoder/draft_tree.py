@@ -1,0 +1,203 @@
+"""Verifying trees of drafted tokens: one step of a model over several guesses of what comes next, instead of one step per token.
+
+    tree = DraftTree(parents, tokens, device)                   # per sequence: node 0 the pending token, then guesses, parents first
+    kv.append(k, v, tree.positions(ctx_lens), tree.row_seq)     # per layer: the nodes' rows behind the context ...
+    out = paged_tree_attention(q, kv, tree, ctx_lens, T)        # ... and attention of every node to the context and its ancestors
+    ids = sampling.adjusted_argmax(logits, tree=tree, ...)      # what the model chooses at every node
+    done = tree_accept(ids, tree, TreeCaches(layers), ctx_lens) # the path that it agrees with; its rows move to their places
+
+`done.tokens[b, :done.counts[b]]` are the tokens that the model itself would have given one by one; the last of them is the next
+pending token (it has no row in the caches yet), `done.ctx_lens` the next context lengths."""
+import collections
+import ctypes
+
+import numpy as np
+import torch
+
+from . import _cabi
+from .host_stage import to_device
+
+MOST_NODES = 1024               # PA_TREE_MOST_NODES
+TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}      # PA_TYPE_*
+_PAIRS = {(torch.float32, "f16"), (torch.float32, "i8"), (torch.float32, "f32"), (torch.float16, "f16"), (torch.float16, "i8"),
+          (torch.bfloat16, "bf16")}
+
+
+def _on(device):
+    device = torch.device(device) if device is not None else torch.device("cuda")
+    return torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
+
+
+class DraftTree:
+    """The drafted nodes of a batch of sequences, on the device.  parents: per sequence the parent of every node as a number within the
+    sequence, -1 for node 0 and a lower node for every other (a sequence without nodes sits the step out); tokens: per
+    sequence the nodes' tokens, where ids are to be adjusted or accepted.
+
+    rows (nodes of all sequences), num_seqs, sizes, most (nodes of the largest), depth (nodes on the longest path); int32 tensors
+    node_start [num_seqs + 1], row_seq, parents, depths (0 at the root), nodes (the node's number), tokens [rows] or None, and
+    mask [rows, words], bit j of which says that node j is on the row's path."""
+
+    def __init__(self, parents, tokens=None, device=None):
+        parents = [np.asarray(p, dtype=np.int64).reshape(-1) for p in parents]
+        sizes = np.array([len(p) for p in parents], dtype=np.int64)
+        B, R, most = len(parents), int(sizes.sum()), int(sizes.max(initial=0))
+        if most > MOST_NODES:
+            raise ValueError(f"DraftTree: at most {MOST_NODES} nodes a sequence")
+        start = np.zeros(B + 1, dtype=np.int64)
+        np.cumsum(sizes, out=start[1:])
+        flat = np.concatenate(parents) if R else np.zeros(0, dtype=np.int64)
+        seq, node = np.repeat(np.arange(B), sizes), np.arange(R) - np.repeat(start[:-1], sizes)
+        if not np.all(np.where(node == 0, flat == -1, (flat >= 0) & (flat < node))):
+            raise ValueError("DraftTree: node 0 has parent -1, every other node a lower one of its sequence")
+        words = max(1, -(-most // 32))
+        mask, depths = np.zeros((R, words), dtype=np.uint32), np.zeros(R, dtype=np.int64)
+        order = np.argsort(node, kind="stable")             # node by node, all sequences at a time: parents are done first
+        ends = np.searchsorted(node[order], np.arange(most + 1))
+        for i in range(most):
+            r = order[ends[i]:ends[i + 1]]
+            if i:
+                up = start[seq[r]] + flat[r]
+                mask[r], depths[r] = mask[up], depths[up] + 1
+            mask[r, i >> 5] |= np.uint32(1 << (i & 31))
+        per_row = [seq, flat, depths, node]
+        if tokens is not None:
+            tokens = [np.asarray(t, dtype=np.int64).reshape(-1) for t in tokens]
+            if [len(t) for t in tokens] != sizes.tolist():
+                raise ValueError("DraftTree: a token for every node")
+            per_row.append(np.concatenate(tokens) if R else flat)
+        self.rows, self.num_seqs, self.sizes, self.most = R, B, sizes.tolist(), most
+        self.depth = int(depths.max(initial=-1)) + 1
+        self.device = _on(device)
+        host = np.concatenate([start] + per_row).astype(np.int32)
+        host = torch.from_numpy(np.concatenate([host, mask.view(np.int32).reshape(-1)]))    # one copy
+        dev = to_device(host, self.device)
+        self.node_start, at = dev[:B + 1], B + 1
+        self.row_seq, self.parents, self.depths, self.nodes = (dev[at + i * R:at + (i + 1) * R] for i in range(4))
+        at += 4 * R
+        self.tokens = None
+        if tokens is not None:
+            self.tokens, at = dev[at:at + R], at + R
+        self.mask = dev[at:].view(R, words)
+
+    def positions(self, ctx_lens):
+        """Where the nodes' K/V rows go in the caches (`KVTileCache.append`): behind the context, in node order."""
+        return ctx_lens[self.row_seq] + self.nodes
+
+
+def _vector(x, n, device, what):
+    if not isinstance(x, torch.Tensor):
+        x = to_device(torch.as_tensor(np.asarray(x), dtype=torch.int32), device)
+    if x.dtype != torch.int32 or x.dim() != 1 or x.numel() != n or x.device != device or not x.is_contiguous():
+        raise ValueError(f"{what}: a contiguous int32 vector of {n} on {device}")
+    return x
+
+
+def paged_tree_attention(q, kv_cache, tree, ctx_lens, temperature=1.0, beam_ids=None, out=None):
+    """Attention of the nodes of `tree` over the pages of `kv_cache` (pa_tree_attention): q [rows, heads, D] (rows may be a view of a
+    wider projection); row r of sequence b sees the first ctx_lens[b] cached tokens and, of the nodes behind them, those of its mask.
+    heads is a multiple of the cache's heads.  beam_ids: table row per sequence (None: b).  ctx_lens, beam_ids: int32 device tensors,
+    or sequences of ints.  out: [rows, heads, D] like q, contiguous."""
+    pt, dev = kv_cache.page_table_, kv_cache.key_buffer_.device
+    KVH, D = pt.num_heads_, kv_cache.head_dim_
+    if q.dim() != 3 or q.shape[0] != tree.rows or q.shape[2] != D or q.shape[1] % KVH or q.shape[1] == 0:
+        raise ValueError(f"paged_tree_attention: q is [{tree.rows}, a multiple of {KVH}, {D}], not {list(q.shape)}")
+    if kv_cache.value_dim_ != D:
+        raise ValueError("paged_tree_attention: keys and values of one width")
+    if (q.dtype, kv_cache.dtype) not in _PAIRS:
+        raise ValueError(f"paged_tree_attention: {q.dtype} queries on '{kv_cache.dtype}' pages")
+    if q.device != dev or tree.device != dev:
+        raise ValueError("paged_tree_attention: q, tree and cache on one device")
+    if not temperature:
+        raise ValueError("paged_tree_attention: temperature 0")
+    R, H = tree.rows, q.shape[1]
+    if R and (q.stride(2) != 1 or q.stride(1) != D or (R > 1 and q.stride(0) < H * D)):
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty((R, H, D), dtype=q.dtype, device=dev)
+    elif out.shape != (R, H, D) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError("paged_tree_attention: out is contiguous, of q's shape, type and device")
+    ctx_lens = _vector(ctx_lens, tree.num_seqs, dev, "ctx_lens")
+    if beam_ids is not None:
+        beam_ids = _vector(beam_ids, tree.num_seqs, dev, "beam_ids")
+    if R == 0:
+        return out
+    lib = _cabi.lib()
+    table = pt.device_data()
+    with _cabi.on_device(dev):
+        stream = _cabi.stream()
+        need = lib.pa_tree_attention_workspace_bytes(R, tree.num_seqs, tree.most, H, KVH, D)
+        ws = kv_cache._ws.get(("tree", stream))
+        if need and (ws is None or ws.numel() < need):
+            ws = kv_cache._ws[("tree", stream)] = torch.empty(need, dtype=torch.uint8, device=dev)
+        _cabi.check(lib.pa_tree_attention(
+            q.data_ptr(), q.stride(0) if R > 1 else H * D, TYPES[q.dtype], out.data_ptr(), kv_cache.key_buffer_.data_ptr(),
+            kv_cache.value_buffer_.data_ptr(), _cabi.ptr(kv_cache.k_scales_), _cabi.ptr(kv_cache.v_scales_),
+            TYPES[kv_cache.key_buffer_.dtype], table.data_ptr(), pt.num_beams_, KVH, pt.num_tiles_, kv_cache.total_pages_, _cabi.ptr(beam_ids),
+            ctx_lens.data_ptr(), tree.node_start.data_ptr(), tree.mask.data_ptr(), tree.mask.shape[1], R, tree.num_seqs, tree.most, H, D,
+            kv_cache.tile_size_, float(temperature), _cabi.ptr(ws) if need else None, need, stream), "pa_tree_attention")
+    return out
+
+
+class TreeCaches:
+    """The caches of a model's layers, for tree_accept: KVTileCaches of one geometry (each with a table of its own, or one shared).
+    Holds their addresses: made anew after a cache's init, resize, configure_table or adopt_buffers."""
+
+    def __init__(self, kv_caches):
+        self.caches = list(kv_caches)
+
+        def kind(k):
+            pt = k.page_table_
+            return (k.key_buffer_.device, k.dtype, k.single_rows_, k.head_dim_, k.value_dim_, k.tile_size_, k.total_pages_, pt.num_beams_,
+                    pt.num_heads_, pt.num_tiles_)
+        if len({kind(k) for k in self.caches}) > 1:
+            raise ValueError("TreeCaches: caches of one device, type and geometry")
+        self.tables = list({id(k.page_table_): k.page_table_ for k in self.caches}.values())
+        ptrs = []
+        for k in self.caches:
+            ptrs += [_cabi.ptr(k.key_buffer_), _cabi.ptr(k.value_buffer_), _cabi.ptr(k.k_scales_), _cabi.ptr(k.v_scales_),
+                     k.page_table_.d_table_.data_ptr()]
+        self._array = (ctypes.c_void_p * max(1, len(ptrs)))(*ptrs)
+        self._geometry = (0, 0, 0, 0, 0, 0, 0)
+        if self.caches:
+            k, pt = self.caches[0], self.caches[0].page_table_
+            e = k.key_buffer_.element_size()
+            self._geometry = (pt.num_beams_, pt.num_heads_, pt.num_tiles_, k.total_pages_, k.tile_size_, k.head_dim_ * e,
+                              0 if k.single_rows_ else k.value_dim_ * e)
+
+
+Accepted = collections.namedtuple("Accepted", "counts tokens nodes ctx_lens")
+
+
+def tree_accept(ids, tree, caches, ctx_lens, beam_ids=None):
+    """What the model agrees with: from node 0 on to the child whose token is the one chosen at the node (ids [rows] int32), as long
+    as there is one, and the K/V rows of that path to positions ctx_lens[b] + 0, 1, 2, ... of every cache (pa_tree_accept).
+    Accepted(counts [B], tokens [B, depth], nodes [B, depth], ctx_lens [B]): nodes on the path, what was chosen at them and their
+    numbers (-1 behind them), the new context lengths; int32 on the device."""
+    if tree.tokens is None:
+        raise ValueError("tree_accept: a tree with tokens")
+    if not isinstance(caches, TreeCaches):
+        caches = TreeCaches(caches)
+    dev, B = tree.device, tree.num_seqs
+    if caches.caches and caches.caches[0].key_buffer_.device != dev:
+        raise ValueError("tree_accept: tree and caches on one device")
+    ids = _vector(ids, tree.rows, dev, "ids")
+    ctx_lens = _vector(ctx_lens, B, dev, "ctx_lens")
+    if beam_ids is not None:
+        beam_ids = _vector(beam_ids, B, dev, "beam_ids")
+    out = torch.empty(2 * B + 2 * B * tree.depth, dtype=torch.int32, device=dev)
+    counts, lens = out[:B], out[B:2 * B]
+    tokens, nodes = out[2 * B:].view(2, B, tree.depth)
+    if B == 0:
+        return Accepted(counts, tokens, nodes, lens)
+    if tree.rows == 0:
+        counts.zero_()
+        lens.copy_(ctx_lens)
+        return Accepted(counts, tokens, nodes, lens)
+    for t in caches.tables:
+        t.flush()
+    with _cabi.on_device(dev):
+        _cabi.check(_cabi.lib().pa_tree_accept(
+            ids.data_ptr(), tree.tokens.data_ptr(), tree.parents.data_ptr(), tree.node_start.data_ptr(), B, tree.most, tree.depth,
+            ctx_lens.data_ptr(), _cabi.ptr(beam_ids), *caches._geometry, len(caches.caches), caches._array, counts.data_ptr(),
+            tokens.data_ptr(), nodes.data_ptr(), lens.data_ptr(), _cabi.stream()), "pa_tree_accept")
+    return Accepted(counts, tokens, nodes, lens)

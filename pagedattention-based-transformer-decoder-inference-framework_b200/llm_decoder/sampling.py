@@ -77,3 +77,100 @@ def sample(logits, temperature=1.0, top_k=0, top_p=1.0, eos_token_id=-1, eos_thr
     apply_topk_topp_filter(probs, top_k, top_p, eos_token_id, eos_thresh)
     u = torch.rand(probs.shape[0], device=probs.device, generator=generator)
     return sample_from_probs(probs, u)
+
+
+def _rules(logits, out, ids, history, history_start, repetition, presence, frequency, bias, allowed, allowed_rows, row_seq, tree):
+    dev, types = logits.device, {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    if logits.dim() != 2 or logits.dtype not in types or not logits.is_cuda:
+        raise ValueError("logits: [rows, vocab] of float32, float16 or bfloat16 on the GPU")
+    rows, V = logits.shape
+    if V == 0 or (rows and (logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < V))):
+        raise ValueError("logits: a vocabulary, and rows of consecutive elements that do not overlap")
+    if (history is None) != (history_start is None):
+        raise ValueError("history and history_start come together")
+
+    def of(x, dtype, what, n=None):
+        if not isinstance(x, torch.Tensor) or x.dtype != dtype or x.device != dev or x.dim() != 1 or not x.is_contiguous() or \
+                (n is not None and x.numel() != n):
+            raise ValueError(f"{what}: a contiguous {dtype} vector{'' if n is None else f' of {n}'} on {dev}")
+        return x
+    if tree is not None:
+        if tree.tokens is None or tree.rows != rows or tree.device != dev or row_seq is not None:
+            raise ValueError("tree: one with tokens, a node for every row, on the logits' device (and then no row_seq)")
+        seqs, row_seq = tree.num_seqs, tree.row_seq
+    elif row_seq is not None:
+        of(row_seq, torch.int32, "row_seq", rows)
+        seqs = None             # as many as the other arguments say
+    else:
+        seqs = rows
+    if history is not None:
+        of(history, torch.int32, "history")
+        of(history_start, torch.int32, "history_start", None if seqs is None else seqs + 1)
+        seqs = history_start.numel() - 1
+    arrays, values = [], []
+    for x, what in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")):
+        if isinstance(x, torch.Tensor):
+            arrays.append(of(x, torch.float32, what, seqs))
+            seqs = x.numel()
+            values.append(0.0)
+        else:
+            arrays.append(None)
+            values.append(float(x))
+    if arrays[0] is None and not values[0] > 0:
+        raise ValueError("repetition: above 0 (1 changes nothing)")
+    b_ids = b_val = b_start = None
+    if bias is not None:
+        b_ids, b_val, b_start = bias
+        of(b_ids, torch.int32, "bias tokens")
+        of(b_val, torch.float32, "bias values", b_ids.numel())
+        of(b_start, torch.int32, "bias starts", None if seqs is None else seqs + 1)
+    if allowed is not None:
+        if allowed.dim() != 2 or allowed.dtype != torch.int32 or allowed.device != dev or allowed.shape[1] * 32 < V or \
+                (allowed.numel() and allowed.stride(1) != 1) or (allowed_rows is None and allowed.shape[0] != rows):
+            raise ValueError("allowed: int32 [rows, words], 32 tokens a word, the logits' vocabulary")
+        if allowed_rows is not None:
+            of(allowed_rows, torch.int32, "allowed_rows", rows)
+    if rows == 0:
+        return
+    # (stride(0) of a single row may be anything)
+    with torch.cuda.device(dev):
+        _cabi.check(_cabi.lib().pa_adjust_logits(
+            logits.data_ptr(), types[logits.dtype], logits.stride(0) if rows > 1 else V, rows, V, _cabi.ptr(out),
+            0 if out is None else out.stride(0) if rows > 1 else V, _cabi.ptr(ids), _cabi.ptr(row_seq), _cabi.ptr(history), _cabi.ptr(history_start),
+            *(_cabi.ptr(a) for a in arrays), *values, _cabi.ptr(b_ids), _cabi.ptr(b_val), _cabi.ptr(b_start), _cabi.ptr(allowed),
+            0 if allowed is None else allowed.stride(0) if allowed.shape[0] > 1 else allowed.shape[1], _cabi.ptr(allowed_rows),
+            *((tree.tokens.data_ptr(), tree.parents.data_ptr(), tree.node_start.data_ptr()) if tree is not None else (None, None, None)),
+            _cabi.stream()), "pa_adjust_logits")
+
+
+def adjust_logits(logits, history=None, history_start=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None,
+                  allowed_rows=None, row_seq=None, tree=None, out=None, ids=False):
+    """What the requests of a batch ask of their logits [rows, vocab] (pa_adjust_logits), in their type; with ids=True also the greedy
+    ids, (logits, ids).  For a token that stands c times in the history of the row's sequence (c > 0):
+        x = x / repetition if x > 0 else x * repetition;  x -= presence;  x -= frequency * c
+    then x += bias, and -inf for what is not allowed.
+
+    history, history_start: the sequences' tokens one after the other, and where each begins [sequences + 1] (int32).
+    repetition, presence, frequency: a number, or a float32 tensor per sequence.
+    bias: (tokens, values, start [sequences + 1]); of two entries for a token the last counts.
+    allowed: int32 [rows, words], bit v & 31 of word v >> 5 for token v; with allowed_rows, the mask of row r is allowed[allowed_rows[r]],
+    and a negative one allows everything.
+    row_seq: the sequence of every row (None: row r is sequence r).  tree: the rows are the nodes of a DraftTree with tokens; the
+    tokens on a node's path, its own among them, count as history.
+    out: a tensor like logits (also logits itself)."""
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or (out.numel() and out.stride(1) != 1) or \
+            (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
+        raise ValueError("out: of the logits' shape, type and device, rows of consecutive elements")
+    chosen = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device) if ids else None
+    _rules(logits, out, chosen, history, history_start, repetition, presence, frequency, bias, allowed, allowed_rows, row_seq, tree)
+    return (out, chosen) if ids else out
+
+
+def adjusted_argmax(logits, history=None, history_start=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None,
+                    allowed_rows=None, row_seq=None, tree=None):
+    """The greedy ids [rows] int32 of adjust_logits' result (the lowest index of the largest), which is not written."""
+    ids = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
+    _rules(logits, None, ids, history, history_start, repetition, presence, frequency, bias, allowed, allowed_rows, row_seq, tree)
+    return ids
