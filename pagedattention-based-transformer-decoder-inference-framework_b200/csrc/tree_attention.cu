@@ -7,6 +7,7 @@
 //
 // The form for every page size, head size up to 256 and element type: one CTA per (row, head), its warps take the keys in turns, a
 // lane holds dim / 32 columns; softmax with a running maximum and sum in float, joined over the warps at the end.
+#include "tcgen05_utils.cuh"
 #include "tree_attention.cuh"
 
 namespace pa {
@@ -94,8 +95,15 @@ static int launch_rows(const TreeParams& p, cudaStream_t st) {
 using namespace pa;
 
 PA_API size_t pa_tree_attention_workspace_bytes(int rows, int num_seqs, int most_nodes, int heads, int kv_heads, int head_dim) {
-    (void)rows; (void)num_seqs; (void)most_nodes; (void)heads; (void)kv_heads; (void)head_dim;
-    return 0;
+    if (rows <= 0 || num_seqs <= 0 || num_seqs > kTreeMostSeqs || heads <= 0 || kv_heads <= 0 || heads % kv_heads || (head_dim != 64 && head_dim != 128))
+        return 0;
+    // whichever kernel serves: it goes by the types too
+    size_t most = 0;
+    for (int block : {16, 32, 128, 256}) {
+        const size_t n = tree_work_bytes(num_seqs, block <= 32 ? tree_stream_workers() : tree_tc_workers(block), block, head_dim);
+        if (n > most) most = n;
+    }
+    return most;
 }
 
 PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void* d_out, const void* d_k_pool, const void* d_v_pool,
@@ -114,8 +122,17 @@ PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void
     const TreeParams p{d_q, q_stride, d_out, d_k_pool, d_v_pool, d_k_scales, d_v_scales, d_table, d_beam_ids, d_ctx_lens, d_node_start,
                        reinterpret_cast<const uint32_t*>(d_mask), q_type, kv_type, num_beams, kv_heads, num_tiles, total_pages, mask_words,
                        rows, num_seqs, most_nodes, heads, head_dim, tile_size, temperature};
-    (void)d_workspace; (void)workspace_bytes;
     cudaStream_t st = as_stream(stream);
+    const int tc_block = tree_tc_block(p), block = tc_block ? tc_block : tree_stream_block(p);
+    if (block) {
+        const int workers = tc_block ? tree_tc_workers(block) : tree_stream_workers();
+        if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < tree_work_bytes(num_seqs, workers, block, head_dim)) return PA_ERR_WORKSPACE;
+        const TreeWork w{p, workers, kTreeLeast, block, tc_block ? 64 : 16, total_pages * tile_size, kTreeStreamScale, tc::kPolls, static_cast<int*>(d_workspace),
+                         reinterpret_cast<float*>(static_cast<char*>(d_workspace) + shares::pre_bytes(num_seqs))};
+        int rc = tc_block ? tree_tc_launch(w, st) : tree_stream_launch(w, st);
+        if (rc == PA_OK) rc = tree_join_launch(w, st);
+        if (rc != PA_ERR_UNSUPPORTED) return rc;
+    }
 #define PA_TREE(QT, QC, KT, KC) if (q_type == QT && kv_type == KT) return launch_rows<QC, KC>(p, st);
     PA_TREE(PA_TYPE_F32, float, PA_TYPE_F16, __half)
     PA_TREE(PA_TYPE_F32, float, PA_TYPE_I8, int8_t)

@@ -1,5 +1,13 @@
-// tree_attention.cuh -- what the kernels of attention over drafted trees share (tree_attention.cu, tree_attention_tc.cu).
+// tree_attention.cuh -- what the kernels of attention over drafted trees share (tree_attention.cu, tree_stream.cu).
+//
+// The rows of a sequence that share a kv head are its nodes' query heads: row rr = node * G + head of the group, G = heads / kv_heads.
+// An item is a block of `block` such rows of one (sequence, kv head) with the keys that its sequence has, in steps of `unit` keys.  The
+// list of all items' steps, sequence by sequence, kv head by kv head, block by block, is cut into equal contiguous shares
+// (decode_shares.cuh: as many as follow from the lengths alone).  A share that holds all of an item writes its rows' results; otherwise
+// it leaves reference, sum and weighted sums of its piece in a slot, and a second kernel joins the pieces: an item's first piece is in slot
+// 2 w + 1 of share w unless the share begins with it, every other one is the beginning of its share, in slot 2 w.
 #pragma once
+#include "decode_shares.cuh"
 #include "seq_common.cuh"
 
 namespace pa {
@@ -34,5 +42,58 @@ __device__ __forceinline__ int tree_seq_of(const int32_t* node_start, int num_se
     }
     return lo;
 }
+
+// ---- the shares
+constexpr int kTreeMostSeqs = 1024;     // sequences that the streaming kernels take: their step counts stand in shared memory
+constexpr int kTreeLeast = 2;           // steps of a share, where there are that many
+
+struct TreeSeq {
+    int r0, n, ctx, keys, blocks, steps;
+    __device__ __forceinline__ int units() const { return blocks * steps; }     // of one kv head
+};
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b, int block, int unit) {
+    TreeSeq s;
+    s.r0 = __ldg(p.node_start + b);
+    s.n = max(min(__ldg(p.node_start + b + 1), p.rows) - s.r0, 0);
+    s.ctx = max(__ldg(p.ctx_lens + b), 0);
+    const int64_t cap = min((int64_t)p.num_tiles * p.tile_size, (int64_t)0x7fffff00);
+    s.keys = s.n > 0 ? (int)min((int64_t)s.ctx + s.n, cap) : 0;
+    s.blocks = (s.n * (p.heads / p.kv_heads) + block - 1) / block;
+    s.steps = (s.keys + unit - 1) / unit;
+    return s;
+}
+// Bits 0 .. width - 1: which of the keys at ctx + off .. a row sees (off < 0: the first -off are context).  word: of the row's mask
+template <typename W>
+__device__ __forceinline__ uint32_t tree_visible(int off, int words, W word) {
+    if (off <= -32) return 0xffffffffu;
+    if (off < 0) return ((1u << -off) - 1u) | (word(0) << -off);
+    const int i = off >> 5;
+    const uint32_t lo = i < words ? word(i) : 0u, hi = i + 1 < words ? word(i + 1) : 0u;
+    return __funnelshift_r(lo, hi, off & 31);
+}
+
+struct TreeWork {
+    TreeParams p;
+    int workers, least, block, unit, total_rows;
+    float p_scale;                      // the partial sums are times this (softmax weights enter products so that small halves keep their bits)
+    uint32_t polls;                     // of a wait
+    int* pre;                           // [num_seqs + 1] steps of one kv head of every sequence, summed up
+    float* part;                        // [2 * workers][block][dim + 4]: weighted sums, reference (log2), sum, largest score, -
+};
+
+static inline size_t tree_work_bytes(int num_seqs, int workers, int block, int dim) {
+    return shares::pre_bytes(num_seqs) + (size_t)2 * workers * block * (dim + 4) * sizeof(float);
+}
+
+// tree_stream.cu: few query rows; the join of pieces
+constexpr float kTreeStreamScale = 128.f;
+int tree_stream_workers();
+int tree_stream_block(const TreeParams& p);                     // rows of a block, 0: not served
+int tree_stream_launch(const TreeWork& w, cudaStream_t st);
+int tree_join_launch(const TreeWork& w, cudaStream_t st);
+// tree_tc.cu: many query rows of 16-bit types
+int tree_tc_workers(int block);
+int tree_tc_block(const TreeParams& p);
+int tree_tc_launch(const TreeWork& w, cudaStream_t st);
 
 }  // namespace pa

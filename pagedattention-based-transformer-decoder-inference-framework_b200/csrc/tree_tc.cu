@@ -1,0 +1,603 @@
+// tree_tc.cu -- attention of drafted trees with many query rows on the 5th-generation tensor cores (tcgen05.mma kind::f16, operands of one
+// 16-bit type, float accumulators in TMEM); tree_attention.cuh has the work list, tree_stream.cu the join.
+//
+// One CTA = NQ tiles of 128 query rows (node, head of the group) of one kv head, which share every staged key and value.  Persistent over
+// its share of the list: barriers and ring run on from piece to piece.  Keys come in tiles of 64:
+//   warps 0-3 (4-7)  softmax of query tile 0 (1), one thread per row = TMEM lane: its 64 scores, the mask of its node where the tile has
+//                    drafted keys, running reference and sum in float, P back to TMEM over the scores it came from
+//   next NQ warps    one elected thread each:  S = Q K^T of tile i + 1  and  O += P V  of tile i (A operand from TMEM)
+//   last warp        TMA boxes of 16 keys x 64 columns into a ring, SWIZZLE_128B, page ids a tile ahead
+// The reference of a row is raised only when a score exceeds it by more than 2^8; weights are 2^(s - reference + 7), so that halves
+// hold them down to 2^-31 of the largest.
+//
+// Drafted rows whose values are not finite may be hidden from some rows, and zero times them is no zero: the softmax threads look
+// through the values of tiles with drafted keys, and a piece that has such values is computed again row by row, from the keys that
+// each row sees alone.
+#include "softmax_tile.cuh"
+#include "tcgen05_utils.cuh"
+#include "tree_attention.cuh"
+
+namespace pa {
+namespace ttc {
+
+using namespace tc;
+
+constexpr int QT = 128, KT = 64;
+constexpr float kShift = 7.f;           // weights times 2^7
+
+__device__ int g_errors;
+
+__host__ __device__ constexpr int q_bytes(int D) { return D * QT * 2; }
+__host__ __device__ constexpr int stage_bytes(int D) { return 2 * D * KT * 2; }
+__host__ __device__ constexpr int stages_for(int D, int nq) { return nq == 2 ? (D == 128 ? 4 : 8) : D == 128 ? 2 : 4; }
+__host__ __device__ constexpr int threads_for(int nq) { return (5 * nq + 1) * 32; }
+// kv_full, kv_empty [stage]; per query tile s_full, p_full, o_full [2], q_ready
+__host__ __device__ constexpr int nbar_for(int D, int nq) { return 2 * stages_for(D, nq) + 7 * nq; }
+constexpr size_t smem_for(int D, int nq, int seqs) {
+    return (size_t)nq * q_bytes(D) + stages_for(D, nq) * stage_bytes(D) + nbar_for(D, nq) * 8 + 64 + stages_for(D, nq) * 4 + (seqs + 1) * 4 + 1024;
+}
+
+// Pieces of a share, in order.  Every role walks them for itself.
+struct Walk {
+    const TreeWork& a;
+    const int* pre;
+    int64_t f, f_hi;
+    int b, item;                        // item within the sequence
+    TreeSeq sq;
+    int g, rr0, i0, i1;                 // the piece: kv head, first row, steps [i0, i1)
+    int64_t slot;                       // of its partial sums, -1: it is a whole item
+    int64_t f_lo;
+    __device__ __forceinline__ Walk(const TreeWork& w, const int* pre_) : a(w), pre(pre_), b(-1) {
+        const int64_t total = (int64_t)pre[w.p.num_seqs] * w.p.kv_heads, ns = shares::count(total, w.workers, w.least);
+        f_lo = f = blockIdx.x < ns ? total * blockIdx.x / ns : 0;
+        f_hi = blockIdx.x < ns ? total * (blockIdx.x + 1) / ns : 0;
+    }
+    __device__ __forceinline__ bool next() {
+        if (f >= f_hi) return false;
+        const TreeParams& p = a.p;
+        if (b < 0 || f >= (int64_t)pre[b + 1] * p.kv_heads) {
+            b = shares::find_token(pre, p.num_seqs, f, p.kv_heads);
+            sq = tree_seq(p, b, a.block, a.unit);
+        }
+        const int64_t rem = f - (int64_t)pre[b] * p.kv_heads;
+        item = (int)(rem / sq.steps);
+        i0 = (int)(rem - (int64_t)item * sq.steps);
+        g = item / sq.blocks;
+        rr0 = (item - g * sq.blocks) * a.block;
+        const int64_t left = f_hi - f;
+        i1 = left < sq.steps - i0 ? i0 + (int)left : sq.steps;
+        slot = i0 == 0 && i1 == sq.steps ? -1 : 2 * (int64_t)blockIdx.x + (f - i0 > f_lo ? 1 : 0);
+        f += i1 - i0;
+        return true;
+    }
+};
+
+template <bool BF> struct Elem { typedef __half T; };
+template <> struct Elem<true> { typedef bf16_t T; };
+
+// Row by row, keys [k0, k1) that the row sees and no others (see above): by a warp, lanes over columns
+template <int D, bool BF>
+__device__ __noinline__ void piece_by_rows(const TreeWork& a, const Walk& w, int row_in_block, int rows) {
+    typedef typename Elem<BF>::T T;
+    constexpr int NC = D / 32;
+    const TreeParams& p = a.p;
+    const int lane = threadIdx.x & 31, G = p.heads / p.kv_heads;
+    const int trow = p.beam_ids ? __ldg(p.beam_ids + w.b) : w.b;
+    const float fe = 1.4426950408889634f / p.temperature;
+    for (int x = 0; x < rows; ++x) {
+        const int rr = w.rr0 + row_in_block + x;
+        if (rr >= w.sq.n * G) break;
+        const int node = rr / G, h = w.g * G + rr % G, r = w.sq.r0 + node;
+        const T* q = static_cast<const T*>(p.q) + (int64_t)r * p.q_stride + (int64_t)h * D;
+        const uint32_t* mask = p.mask + (int64_t)r * p.mask_words;
+        float qf[NC], o[NC], m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            qf[c] = tree_widen<T>(q[lane + 32 * c]);
+            o[c] = 0.f;
+        }
+        for (int t = w.i0 * KT; t < min(w.i1 * KT, w.sq.keys); ++t) {
+            const int j = t - w.sq.ctx;
+            if (j >= 0 && (j >= p.mask_words * 32 || !((__ldg(mask + (j >> 5)) >> (j & 31)) & 1u))) continue;
+            const int tile = t / p.tile_size;
+            if ((unsigned)trow >= (unsigned)p.num_beams || tile >= p.num_tiles) continue;
+            const int page = __ldg(p.table + ((int64_t)trow * p.kv_heads + w.g) * p.num_tiles + tile);
+            if ((unsigned)page >= (unsigned)p.total_pages) continue;
+            const int64_t at = ((int64_t)page * p.tile_size + (t - tile * p.tile_size)) * D + lane;
+            float s = 0.f, v[NC];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s = fmaf(qf[c], tree_widen<T>(static_cast<const T*>(p.k)[at + 32 * c]), s);
+                v[c] = tree_widen<T>(static_cast<const T*>(p.v)[at + 32 * c]);
+            }
+            s = warp_sum(s) * fe;
+            const float mn = fmaxf(m, s);
+            const float f = m == mn ? 1.f : fast_exp2(m - mn), e = s == mn ? 1.f : fast_exp2(s - mn);
+            m = mn;
+            l = l * f + e;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) o[c] = fmaf(e, v[c], o[c] * f);
+        }
+        if (w.slot < 0) {
+            T* out = static_cast<T*>(p.out) + ((int64_t)r * p.heads + h) * D;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) out[lane + 32 * c] = tree_narrow<T>(o[c] / (l + 1e-6f));
+        } else {
+            float* dst = a.part + (w.slot * a.block + row_in_block + x) * (D + 4);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) dst[lane + 32 * c] = o[c] * a.p_scale;
+            if (lane == 0) *reinterpret_cast<float4*>(dst + D) = make_float4(m, l * a.p_scale, m, 0.f);
+        }
+    }
+}
+
+template <int D, int NQ, bool BF>
+__global__ void __launch_bounds__(threads_for(NQ), NQ == 1 ? 2 : 1)
+tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeWork a) {
+    typedef typename Elem<BF>::T T;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    constexpr int ST = stages_for(D, NQ), NBAR = nbar_for(D, NQ), TMEM_COLS = NQ * 256, KB = D / 64;
+    constexpr int Q_BYTES = q_bytes(D), K_BYTES = D * KT * 2, STAGE = stage_bytes(D);
+    constexpr int W_MMA = 4 * NQ, W_PROD = 5 * NQ;
+    const TreeParams& p = a.p;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t kv_sm = base + NQ * Q_BYTES, bar0 = kv_sm + ST * STAGE;
+    auto kv_full = [&](int s) { return bar0 + s * 8; };
+    auto kv_empty = [&](int s) { return bar0 + (ST + s) * 8; };
+    auto s_full = [&](int x, int i) { return bar0 + (2 * ST + 7 * x + i) * 8; };
+    auto p_full = [&](int x, int i) { return bar0 + (2 * ST + 7 * x + 2 + i) * 8; };
+    auto o_full = [&](int x, int i) { return bar0 + (2 * ST + 7 * x + 4 + i) * 8; };
+    auto q_ready = [&](int x) { return bar0 + (2 * ST + 7 * x + 6) * 8; };
+    const uint32_t tmem_slot = bar0 + NBAR * 8, fail_sm = tmem_slot + 8, odd_sm = fail_sm + 4, meta_sm = odd_sm + 8;
+    int* pre = reinterpret_cast<int*>(smem_raw + (meta_sm + ST * 4 - smem_u32(smem_raw)));
+    auto failed = [&] { return tc_failed(fail_sm); };
+    auto wait = [&](uint32_t bar, uint32_t parity) { tc_wait(bar, parity, fail_sm, a.polls); };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.heads / p.kv_heads;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(kv_full(s), 1);
+            mbar_init(kv_empty(s), NQ);
+        }
+        for (int x = 0; x < NQ; ++x) {
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(s_full(x, i), 1);
+                mbar_init(p_full(x, i), QT);
+                mbar_init(o_full(x, i), 1);
+            }
+            mbar_init(q_ready(x), 1);
+        }
+        asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(fail_sm), "r"(0u) : "memory");
+        asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(odd_sm), "r"(0u) : "memory");
+        asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(odd_sm + 4), "r"(0u) : "memory");
+        mbar_fence_init();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmK));
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmV));
+    }
+    if (warp == W_MMA) tmem_alloc(tmem_slot, TMEM_COLS);
+    shares::count_units(pre, p.num_seqs, [&](int b) { return tree_seq(p, b, a.block, a.unit).units(); });
+    if (blockIdx.x == 0)
+        for (int b = threadIdx.x; b <= p.num_seqs; b += blockDim.x) a.pre[b] = pre[b];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem_base;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
+    Walk w(a, pre);
+    // which query tiles of the piece have rows, and its tiles of keys
+    auto has_rows = [&](int x) { return w.rr0 + x * QT < w.sq.n * G; };
+
+    if (warp == W_PROD) {
+        if (elect_one()) {
+            int s = 0;
+            uint32_t ph = 1;
+            bool ok = true;
+            while (ok && w.next()) {
+                const int row = p.beam_ids ? __ldg(p.beam_ids + w.b) : w.b;
+                const int32_t* trow = p.table + ((int64_t)row * p.kv_heads + w.g) * p.num_tiles;
+                const bool row_ok = (unsigned)row < (unsigned)p.num_beams;
+                int pgn[4];
+                auto load_pages = [&](int i) {
+#pragma unroll
+                    for (int uu = 0; uu < 4; ++uu) {
+                        const int t0 = (i * 4 + uu) * 16, t = t0 / p.tile_size;
+                        const int page = row_ok && t0 < w.sq.keys && t < p.num_tiles ? __ldg(trow + t) : -1;
+                        pgn[uu] = (unsigned)page < (unsigned)p.total_pages ? page * p.tile_size + (t0 - t * p.tile_size) : -1;
+                    }
+                };
+                load_pages(w.i0);
+                for (int i = w.i0; i < w.i1; ++i) {
+                    int r[4];
+                    uint32_t mask = 0;
+#pragma unroll
+                    for (int uu = 0; uu < 4; ++uu) {
+                        r[uu] = pgn[uu] >= 0 ? pgn[uu] : a.total_rows;          // no page: zeros, and its scores are masked
+                        mask |= (pgn[uu] >= 0 ? 1u : 0u) << uu;
+                    }
+                    if (i + 1 < w.i1) load_pages(i + 1);
+                    wait(kv_empty(s), ph);
+                    if (failed()) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t st = kv_sm + s * STAGE;
+                    asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(meta_sm + s * 4), "r"(mask) : "memory");
+                    mbar_arrive_expect_tx(kv_full(s), STAGE);
+#pragma unroll
+                    for (int uu = 0; uu < 4; ++uu)
+#pragma unroll
+                        for (int kb = 0; kb < KB; ++kb) tma_load_2d(st + kb * 8192 + uu * 2048, &tmK, kb * 64, r[uu], kv_full(s));
+#pragma unroll
+                    for (int uu = 0; uu < 4; ++uu)
+#pragma unroll
+                        for (int kb = 0; kb < KB; ++kb) tma_load_2d(st + K_BYTES + kb * 8192 + uu * 2048, &tmV, kb * 64, r[uu], kv_full(s));
+                    if (++s == ST) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            if (failed())       // let the copies in flight land before the CTA's shared memory goes away
+                for (int i = 0; i < ST; ++i) tc_let_land(kv_full(i), i < s ? ph ^ 1u : ph);
+        }
+    } else if (warp >= W_MMA) {
+        constexpr uint32_t kIdescS = idesc_f16(QT, KT, 0, 0, BF), kIdescO = idesc_f16(QT, D, 0, 1, BF);
+        const int x = warp - W_MMA;
+        int s = 0, n = 0, qn = 0;           // stage; key tiles and pieces of this query tile so far
+        uint32_t kv_ph = 0;
+        while (w.next()) {
+            const bool mine = has_rows(x);
+            auto issue_S = [&](int i, int stage) {
+                if (elect_one()) {
+                    const uint32_t st = kv_sm + stage * STAGE, qx = base + x * Q_BYTES;
+                    const int sb = (n + i) & 1;
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        const uint64_t da = make_desc(qx + (ks >> 2) * (QT * 128) + (ks & 3) * 32, 16, 1024);
+                        const uint64_t db = make_desc(st + (ks >> 2) * (KT * 128) + (ks & 3) * 32, 16, 1024);
+                        umma_f16(tmem_base + x * 2 * KT + sb * KT, da, db, kIdescS, ks > 0 ? 1u : 0u);
+                    }
+                    umma_commit(s_full(x, sb));
+                }
+                __syncwarp();
+            };
+            const int nt = w.i1 - w.i0;
+            wait(kv_full(s), kv_ph);
+            if (mine) {
+                wait(q_ready(x), (uint32_t)qn & 1u);
+                tc_fence_after();
+                issue_S(0, s);
+            }
+            for (int i = 0; i < nt; ++i) {
+                const int s_next = (s + 1 == ST) ? 0 : s + 1;
+                if (i + 1 < nt) {           // every issuer waits for every stage: its arrival on kv_empty belongs to THIS use of it
+                    wait(kv_full(s_next), (s + 1 == ST) ? (kv_ph ^ 1u) : kv_ph);
+                    tc_fence_after();
+                    if (mine) issue_S(i + 1, s_next);
+                }
+                if (mine) {
+                    const uint32_t st = kv_sm + s * STAGE;
+                    const int sb = (n + i) & 1, nvalid = min(KT, w.sq.keys - (w.i0 + i) * KT);
+                    if (nvalid & 15) {
+                        // value rows past the last key may hold anything (0 x NaN = NaN): zeros (both issuers write the same)
+                        const int r1 = (nvalid + 15) & ~15;
+                        for (int idx = lane; idx < (r1 - nvalid) * (D / 8); idx += 32) {
+                            const int r = nvalid + idx / (D / 8), c = idx % (D / 8);
+                            const uint32_t addr = st + K_BYTES + (c >> 3) * 8192 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(addr), "r"(0u) : "memory");
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                    // every row's thread has also read the last piece's O by the time it hands over a piece's first P
+                    wait(p_full(x, sb), (uint32_t)((n + i) >> 1) & 1u);
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const int ksteps = (nvalid + 15) >> 4;
+                        for (int ks = 0; ks < ksteps; ++ks) {
+                            const uint32_t ta = tmem_base + x * 2 * KT + sb * KT + ks * 8;
+                            const uint64_t db = make_desc(st + K_BYTES + ks * 2048, 8192, 1024);
+                            umma_f16_ts(tmem_base + NQ * 2 * KT + x * D, ta, db, kIdescO, (i > 0 || ks > 0) ? 1u : 0u);
+                        }
+                        umma_commit(o_full(x, sb));
+                    }
+                    __syncwarp();
+                }
+                if (elect_one()) umma_commit(kv_empty(s));
+                __syncwarp();
+                if (++s == ST) {
+                    s = 0;
+                    kv_ph ^= 1u;
+                }
+            }
+            if (mine) {
+                n += nt;
+                ++qn;
+            }
+        }
+    } else {
+        // ---- softmax: one thread per query row
+        const int x = warp >> 2, qtr = warp & 3, row_in_block = x * QT + qtr * 32;
+        const uint32_t lane_base = (uint32_t)(qtr * 32) << 16;
+        const uint32_t s_addr = tmem_base + lane_base + x * 2 * KT;
+        const uint32_t o_addr = tmem_base + lane_base + NQ * 2 * KT + x * D;
+        const float f0 = 1.4426950408889634f / p.temperature, fe = fmaxf(fabsf(f0), 1e-30f);
+        const bool flip = f0 < 0.f;
+        auto group_sync = [&] {
+            if (x == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+            else asm volatile("bar.sync 2, 128;" ::: "memory");
+        };
+        // P.V(t) is complete.  Unambiguous without consuming every phase: S(n) follows P.V(n - 2) on the pipe, so by the time a
+        // thread works on tile n the barrier of P.V(n - 1) is in the phase asked for or just past it.
+        auto pv_done = [&](int t) { wait(o_full(x, t & 1), (uint32_t)((t >> 1) & 1)); };
+        int st_i = 0, n = 0;
+        uint32_t st_ph = 0;
+        auto next_stage = [&] {
+            if (++st_i == ST) {
+                st_i = 0;
+                st_ph ^= 1u;
+            }
+        };
+        while (w.next()) {
+            const int nt = w.i1 - w.i0, all = w.sq.n * G;
+            if (!has_rows(x)) {
+                for (int i = 0; i < nt; ++i) next_stage();
+                continue;
+            }
+            const int rr = w.rr0 + row_in_block + lane, rows = min(32, all - w.rr0 - row_in_block);       // rows of this warp, may be negative
+            const int node = rr < all ? rr / G : -1, head = w.g * G + rr % G;
+            if (rows > 0) {
+                // the warp's query rows into the swizzled K-major A tile, whose last products this thread has seen complete
+                const uint32_t qx = base + x * Q_BYTES;
+                constexpr int CH = D / 8, PER = 8;      // 16-byte pieces of a row; loads in flight per lane
+#pragma unroll 1
+                for (int c0 = 0; c0 < 32 * CH; c0 += 32 * PER) {
+                    uint4 v[PER];
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) {
+                        const int idx = c0 + j * 32 + lane, r = idx / CH, c = idx % CH, q = w.rr0 + row_in_block + r;
+                        v[j] = make_uint4(0u, 0u, 0u, 0u);
+                        if (r < rows)
+                            v[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(w.sq.r0 + q / G) * p.q_stride +
+                                                                        (int64_t)(w.g * G + q % G) * D) + c);
+                    }
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) {
+                        const int idx = c0 + j * 32 + lane, r = idx / CH, c = idx % CH, at = qtr * 32 + r;
+                        const uint32_t addr = qx + (c >> 3) * (QT * 128) + at * 128 + (((c & 7) ^ (at & 7)) << 4);
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v[j].x), "r"(v[j].y), "r"(v[j].z), "r"(v[j].w) : "memory");
+                    }
+                }
+            }
+            fence_proxy_async();
+            group_sync();
+            if (qtr == 0 && lane == 0) mbar_arrive_cnt(q_ready(x));
+            const uint32_t* mask = p.mask + (int64_t)(w.sq.r0 + max(node, 0)) * p.mask_words;
+            float m_ref = -INFINITY, l_run = 0.f;
+            bool odd = false;
+#pragma unroll 1
+            for (int i = 0; i < nt; ++i) {
+                const int sb = (n + i) & 1, kp0 = (w.i0 + i) * KT;
+                const bool drafts = kp0 + KT > w.sq.ctx;
+                wait(s_full(x, sb), (uint32_t)((n + i) >> 1) & 1u);
+                tc_fence_after();
+                if (drafts) {       // values that are not finite (the keys past the last one were looked at or are zeros)
+                    wait(kv_full(st_i), st_ph);
+                    const uint32_t vt = kv_sm + st_i * STAGE + K_BYTES;
+                    const int mine = threadIdx.x & 127, r = mine >> 1;
+                    if (kp0 + r < w.sq.keys) {
+#pragma unroll
+                        for (int c = 0; c < D / 16; ++c) {
+                            const uint4 v = lds_128(vt + ((mine & 1) * (D / 16) + c) / 8 * 8192 + r * 128 + ((((mine & 1) * (D / 16) + c) & 7) << 4));
+                            constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+                            const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) odd |= (q[e] & E) == E || (q[e] >> 16 & E) == E;
+                        }
+                    }
+                }
+                if (rows <= 0) {    // nothing of this warp's: it only keeps the barriers' count
+                    mbar_arrive_cnt(p_full(x, sb));
+                    next_stage();
+                    continue;
+                }
+                uint32_t mapped;    // the producer's note about this stage, older than the scores
+                asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(mapped) : "r"(meta_sm + st_i * 4) : "memory");
+                uint32_t sr[2][32];
+                tmem_ld32(s_addr + sb * KT, sr[0]);
+                tmem_ld32(s_addr + sb * KT + 32, sr[1]);
+                tmem_wait_ld();
+                if (flip) {
+#pragma unroll
+                    for (int k = 0; k < KT; ++k) sr[k >> 5][k & 31] ^= 0x80000000u;
+                }
+                const bool full = !drafts && mapped == 15u;
+                if (!full) {
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const int k0 = kp0 + 32 * hf, valid = w.sq.keys - k0;
+                        uint32_t vis = 0xffffffffu;
+                        if (drafts) {
+                            vis = tree_visible(k0 - w.sq.ctx, p.mask_words, [&](int j) { return __ldg(mask + j); });
+                            if (valid < 32) vis &= valid > 0 ? (1u << valid) - 1u : 0u;
+                        }
+                        if (!(mapped >> 2 * hf & 1u)) vis &= 0xffff0000u;
+                        if (!(mapped >> 2 * hf & 2u)) vis &= 0x0000ffffu;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (!(vis >> k & 1u)) sr[hf][k] = 0xff800000u;
+                    }
+                }
+                // A row's reference rarely moves, so a tile that all rows of the warp see whole takes the exponentials with the one at
+                // hand, without waiting for the maximum, and the scores' first half is on its way to TMEM under the second's exponentials
+                auto pack = [](float lo, float hi) {
+                    if constexpr (BF) return pack_bf16x2(lo, hi);
+                    else return pack_half2(lo, hi);
+                };
+                uint32_t w0[16], w1[16];
+                uint64_t acc[2] = {0ull, 0ull};
+                if (__all_sync(0xffffffffu, full && m_ref > -INFINITY)) {
+                    smx::exp_half(sr[0], fe, m_ref - kShift, w0, acc, pack);
+                    tmem_st16(s_addr + sb * KT, w0);
+                    const float mx = smx::row_max(sr) * fe;
+                    smx::exp_half(sr[1], fe, m_ref - kShift, w1, acc, pack);
+                    if (!__any_sync(0xffffffffu, mx > m_ref + 8.f)) {
+                        tmem_st16(s_addr + sb * KT + 16, w1);
+                        l_run += smx::sum_of(acc);
+                        tmem_wait_st();
+                        tc_fence_before();
+                        mbar_arrive_cnt(p_full(x, sb));
+                        next_stage();
+                        continue;
+                    }
+                    acc[0] = acc[1] = 0ull;
+                    tmem_wait_st();
+                }
+                const float mx = smx::row_max(sr) * fe;
+                const bool raise = mx > m_ref + 8.f || (m_ref == -INFINITY && mx > -INFINITY);
+                const float m_new = raise ? mx : m_ref;
+                const float corr = raise && m_ref != -INFINITY ? fast_exp2(m_ref - m_new) : 1.f;
+                m_ref = m_new;
+                smx::exp_half(sr[0], fe, m_ref - kShift, w0, acc, pack);
+                smx::exp_half(sr[1], fe, m_ref - kShift, w1, acc, pack);
+                const bool dead = m_ref == -INFINITY;       // nothing visible yet: the exponents above are NaN
+                if (__any_sync(0xffffffffu, corr != 1.f)) {
+                    if (i > 0) pv_done(n + i - 1);
+                    tc_fence_after();
+#pragma unroll
+                    for (int c4 = 0; c4 < D / 32; ++c4) {
+                        uint32_t orr[32];
+                        tmem_ld32(o_addr + c4 * 32, orr);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) orr[j] = __float_as_uint(__uint_as_float(orr[j]) * corr);
+                        tmem_st32(o_addr + c4 * 32, orr);
+                    }
+                    l_run *= corr;
+                }
+                if (dead) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) w0[k] = w1[k] = 0u;
+                } else {
+                    l_run += smx::sum_of(acc);
+                }
+                tmem_st16(s_addr + sb * KT, w0);
+                tmem_st16(s_addr + sb * KT + 16, w1);
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive_cnt(p_full(x, sb));
+                next_stage();
+            }
+            n += nt;
+            pv_done(n - 1);
+            tc_fence_after();
+            if (w.i1 * KT > w.sq.ctx) {         // the piece had drafted keys
+                if (odd) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(odd_sm + 4 * x), "r"(1u) : "memory");
+                group_sync();
+                uint32_t any;
+                asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(any) : "r"(odd_sm + 4 * x) : "memory");
+                group_sync();
+                odd = any != 0;
+                if (odd && qtr == 0 && lane == 0) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(odd_sm + 4 * x), "r"(0u) : "memory");
+            }
+            if (odd && !failed()) {
+                piece_by_rows<D, BF>(a, w, row_in_block, 32);
+                continue;
+            }
+            if (rows <= 0) continue;
+            // every thread writes its own row: the stores leave while the next piece's scores come
+            float inv = 1.f / (l_run + 1e-6f * 128.f);
+            if (m_ref == -INFINITY) inv = 0.f;              // saw nothing
+            if (failed()) inv = m_ref = l_run = __int_as_float(0x7fc00000);
+            T* out = static_cast<T*>(p.out) + ((int64_t)(w.sq.r0 + max(node, 0)) * p.heads + head) * D;
+            float* part = a.part + (w.slot * a.block + row_in_block + lane) * (D + 4);
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+                uint32_t o[32];
+                tmem_ld32(o_addr + c0, o);
+                tmem_wait_ld();
+                if (node >= 0 && w.slot < 0) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float lo = m_ref == -INFINITY ? 0.f : __uint_as_float(o[j * 8 + 2 * e]) * inv;
+                            const float hi = m_ref == -INFINITY ? 0.f : __uint_as_float(o[j * 8 + 2 * e + 1]) * inv;
+                            if constexpr (BF) v[e] = pack_bf16x2(lo, hi);
+                            else v[e] = pack_half2(lo, hi);
+                        }
+                        reinterpret_cast<uint4*>(out + c0)[j] = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+                } else if (node >= 0) {
+                    const float k = a.p_scale / 128.f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        float v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = m_ref == -INFINITY ? 0.f : __uint_as_float(o[4 * j + e]) * k;
+                        reinterpret_cast<float4*>(part + c0)[j] = make_float4(v[0], v[1], v[2], v[3]);
+                    }
+                }
+                __syncwarp();
+            }
+            if (node >= 0 && w.slot >= 0) *reinterpret_cast<float4*>(part + D) = make_float4(m_ref, l_run * (a.p_scale / 128.f), m_ref, 0.f);
+        }
+        tc_fence_before();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == W_MMA) {
+        tc_fence_after();
+        if (failed()) {
+            __nanosleep(1000000);       // products in flight write TMEM for microseconds at most
+            if (lane == 0) atomicAdd(&g_errors, 1);
+        }
+        tmem_dealloc(tmem_base, TMEM_COLS);
+    }
+}
+
+template <int D, int NQ, bool BF>
+static int launch(const TreeWork& a, cudaStream_t st) {
+    const TreeParams& p = a.p;
+    const size_t smem = smem_for(D, NQ, p.num_seqs);
+    if (smem > (size_t)device_info().max_smem_optin) return PA_ERR_UNSUPPORTED;
+    auto kern = tree_tc_kernel<D, NQ, BF>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    CUtensorMap k, v;                   // boxes move bits: one map type for both 16-bit types
+    if (!make_bf16_map(&k, p.k, a.total_rows, D, D, 16) || !make_bf16_map(&v, p.v, a.total_rows, D, D, 16)) return PA_ERR_UNSUPPORTED;
+    kern<<<a.workers, threads_for(NQ), smem, st>>>(k, v, a);
+    PA_RETURN_LAUNCH_STATUS();
+}
+
+}  // namespace ttc
+
+int tree_tc_workers(int block) { return device_info().sm_count * (block == 128 ? 2 : 1); }
+
+// Rows of a block, 0 where this kernel does not serve or the streaming one is faster
+int tree_tc_block(const TreeParams& p) {
+    const int G = p.heads / p.kv_heads, rows = p.most * G;
+    if (!((p.q_type == PA_TYPE_F16 && p.kv_type == PA_TYPE_F16) || (p.q_type == PA_TYPE_BF16 && p.kv_type == PA_TYPE_BF16)) || rows <= 32) return 0;
+    if ((p.dim != 64 && p.dim != 128) || p.tile_size % 16 || p.num_seqs > kTreeMostSeqs) return 0;
+    if ((int64_t)p.total_pages * p.tile_size >= 0x7fffff00ll || ((uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.q | (uintptr_t)p.out) % 16 || p.q_stride % 8) return 0;
+    const int block = rows <= 128 ? 128 : 256;
+    const int64_t steps = ((int64_t)p.num_tiles * p.tile_size + ttc::KT - 1) / ttc::KT;
+    return ((int64_t)p.rows * G / block + p.num_seqs) * steps < 0x7fffffff ? block : 0;     // the list's sums are 32 bits
+}
+
+int tree_tc_launch(const TreeWork& a, cudaStream_t st) {
+    using namespace ttc;
+    const bool bf = a.p.q_type == PA_TYPE_BF16;
+    if (a.p.dim == 64) {
+        if (a.block == 128) return bf ? launch<64, 1, true>(a, st) : launch<64, 1, false>(a, st);
+        return bf ? launch<64, 2, true>(a, st) : launch<64, 2, false>(a, st);
+    }
+    if (a.block == 128) return bf ? launch<128, 1, true>(a, st) : launch<128, 1, false>(a, st);
+    return bf ? launch<128, 2, true>(a, st) : launch<128, 2, false>(a, st);
+}
+
+int tree_tc_errors(int* host_count) { return (int)cudaMemcpyFromSymbol(host_count, ttc::g_errors, sizeof(int)); }
+
+}  // namespace pa
