@@ -127,8 +127,8 @@ PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void
     if (block) {
         const int workers = tc_block ? tree_tc_workers(block) : tree_stream_workers();
         if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < tree_work_bytes(num_seqs, workers, block, head_dim)) return PA_ERR_WORKSPACE;
-        const TreeWork w{p, workers, kTreeLeast, block, tc_block ? 64 : 16, total_pages * tile_size, kTreeStreamScale, tc::kPolls, static_cast<int*>(d_workspace),
-                         reinterpret_cast<float*>(static_cast<char*>(d_workspace) + shares::pre_bytes(num_seqs))};
+        const TreeWork w{p, workers, kTreeLeast, block, tc_block ? 64 : 16, total_pages * tile_size, kTreeStreamScale, tc::kPolls, static_cast<TreeNote*>(d_workspace),
+                         reinterpret_cast<float*>(static_cast<TreeNote*>(d_workspace) + workers)};
         int rc = tc_block ? tree_tc_launch(w, st) : tree_stream_launch(w, st);
         if (rc == PA_OK) rc = tree_join_launch(w, st);
         if (rc != PA_ERR_UNSUPPORTED) return rc;

@@ -4,8 +4,9 @@
 // An item is a block of `block` such rows of one (sequence, kv head) with the keys that its sequence has, in steps of `unit` keys.  The
 // list of all items' steps, sequence by sequence, kv head by kv head, block by block, is cut into equal contiguous shares
 // (decode_shares.cuh: as many as follow from the lengths alone).  A share that holds all of an item writes its rows' results; otherwise
-// it leaves reference, sum and weighted sums of its piece in a slot, and a second kernel joins the pieces: an item's first piece is in slot
-// 2 w + 1 of share w unless the share begins with it, every other one is the beginning of its share, in slot 2 w.
+// it leaves reference, sum and weighted sums of its piece in a slot, and a second kernel joins the pieces: the share in which such an
+// item begins notes it (TreeNote); the item's first piece is in slot 2 w + 1 of that share w unless the share begins with it, every other one
+// is the beginning of its share, in slot 2 w.
 #pragma once
 #include "decode_shares.cuh"
 #include "seq_common.cuh"
@@ -72,17 +73,40 @@ __device__ __forceinline__ uint32_t tree_visible(int off, int words, W word) {
     return __funnelshift_r(lo, hi, off & 31);
 }
 
+// The item that begins in a share and does not end there
+struct __align__(16) TreeNote {
+    int rows;                           // of the item's block; 0: there is none
+    int first_row, g, rr0;              // the sequence's first row, kv head, the block's first row within the group
+    int last;                           // the share in which it ends
+    int slot;                           // of its first piece
+    int pad[2];
+};
+
 struct TreeWork {
     TreeParams p;
     int workers, least, block, unit, total_rows;
     float p_scale;                      // the partial sums are times this (softmax weights enter products so that small halves keep their bits)
     uint32_t polls;                     // of a wait
-    int* pre;                           // [num_seqs + 1] steps of one kv head of every sequence, summed up
+    TreeNote* notes;                    // [workers]
     float* part;                        // [2 * workers][block][dim + 4]: weighted sums, reference (log2), sum, largest score, -
 };
 
 static inline size_t tree_work_bytes(int num_seqs, int workers, int block, int dim) {
-    return shares::pre_bytes(num_seqs) + (size_t)2 * workers * block * (dim + 4) * sizeof(float);
+    (void)num_seqs;
+    return (size_t)workers * sizeof(TreeNote) + (size_t)2 * workers * block * (dim + 4) * sizeof(float);
+}
+// by one thread of a worker: what it notes of the last piece of its share, steps [i0, i1) of an item that begins at step f_item of the list
+__device__ __forceinline__ TreeNote tree_note(const TreeWork& a, const TreeSeq& s, int g, int rr0, int i0, int i1, int64_t f_item, int64_t total, int64_t ns, int64_t slot) {
+    TreeNote t{};
+    if (i0 == 0 && i1 < s.steps) {
+        t.rows = min(a.block, s.n * (a.p.heads / a.p.kv_heads) - rr0);
+        t.first_row = s.r0;
+        t.g = g;
+        t.rr0 = rr0;
+        t.last = (int)(((f_item + s.steps) * ns - 1) / total);
+        t.slot = (int)slot;
+    }
+    return t;
 }
 
 // tree_stream.cu: few query rows; the join of pieces

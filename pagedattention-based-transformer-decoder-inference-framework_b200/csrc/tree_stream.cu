@@ -70,15 +70,16 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
     }
     if (threadIdx.x == 0) fail_word = 0;
     shares::count_units(pre, p.num_seqs, [&](int b) { return tree_seq(p, b, MT * 16, kUnit).units(); });
-    if (blockIdx.x == 0)
-        for (int b = threadIdx.x; b <= p.num_seqs; b += blockDim.x) a.pre[b] = pre[b];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int w = warp * gridDim.x + blockIdx.x, G = p.heads / p.kv_heads;
     const int64_t total = (int64_t)pre[p.num_seqs] * p.kv_heads;
     const int64_t ns = shares::count(total, a.workers, a.least);
     const int64_t f_lo = w < ns ? total * w / ns : 0, f_hi = w < ns ? total * (w + 1) / ns : 0;
-    if (f_lo >= f_hi) return;
+    if (f_lo >= f_hi) {
+        if (lane == 0) a.notes[w] = TreeNote{};
+        return;
+    }
 
     // ---- the copies: unit f's rows in the pools, 32 units at a time
     auto rows_of = [&](int64_t f) -> int {
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
         item = (int)(rem / sq.steps);
         u = (int)(rem % sq.steps);
     }
-    bool from_start = u == 0;           // the piece at hand begins its item
+    int u0 = u;                         // the piece at hand begins with it
     uint32_t qf[MT][TERMS][KS][4];
     float o[MT][NT][4], m[MT][2], l[MT][2], fe[MT][2], top[MT][2];     // reference, sum, factor of the scores, largest score
     int node[MT][2];                    // of a row, -1: no row
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
                 s += __shfl_xor_sync(0xffffffffu, s, 2);
                 if (node[mt][i] < 0) continue;
                 const int rl = mt * 16 + lr + 8 * i, rr = rr0 + rl;
-                if (from_start && to_end) {
+                if (u0 == 0 && to_end) {
                     const float eps = 1e-6f * kTreeStreamScale * (TWO && m[mt][i] != -INFINITY ? fast_exp2(top[mt][i] - m[mt][i]) : 1.f);
                     const float inv = 1.f / (s + eps);
                     const int64_t at = ((int64_t)(sq.r0 + rr / G) * p.heads + g * G + rr % G) * D;
@@ -253,8 +254,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
             }
     };
     auto next_item = [&] {
-        u = 0;
-        from_start = true;
+        u = u0 = 0;
         if (++item == p.kv_heads * sq.blocks) {
             item = 0;
             do ++b; while (pre[b + 1] == pre[b]);       // a sequence without nodes has no items
@@ -573,69 +573,145 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
         u = (int)(sq.steps - (f - f_hi));
     }
     close_item(u == sq.steps);
+    if (lane == 0) {
+        const int64_t f_item = (int64_t)pre[b] * p.kv_heads + (int64_t)item * sq.steps;
+        a.notes[w] = tree_note(a, sq, item / sq.blocks, item % sq.blocks * (MT * 16), u0, u, f_item, total, ns, 2 * (int64_t)w + (f_item > f_lo ? 1 : 0));
+    }
 }
 
-// One warp per (row, head); a lane has D / 32 neighbouring columns.  A row whose item was in one share is there already.
-template <typename Q>
-__global__ void __launch_bounds__(128) tree_join_kernel(const TreeWork a) {
+// The rows of items whose keys were in several shares.  blockIdx.x: the share that noted the item (where items are few and their pieces many,
+// the number of the note among all), blockIdx.y: kJoinWarps / SPLIT of its rows, SPLIT warps each that share the row's pieces; a lane has
+// D / 32 neighbouring columns.  A warp's pieces come in order, FLIGHT at a time with all their loads in flight, under a running maximum.
+constexpr int kJoinWarps = 8;
+template <typename Q, int NV, int SPLIT>
+__global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeWork a) {
+    constexpr int D = NV * 32, LD = D + 4, ROWS = kJoinWarps / SPLIT, FLIGHT = SPLIT > 1 ? 8 : 4;
+    __shared__ float s_acc[SPLIT > 1 ? kJoinWarps : 1][D], s_ml[SPLIT > 1 ? kJoinWarps : 1][3];
     const TreeParams& p = a.p;
-    const int lane = threadIdx.x & 31, G = p.heads / p.kv_heads, D = p.dim;
-    const int64_t wid = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.heads / p.kv_heads;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (wid >= (int64_t)p.rows * p.heads) return;
-    const int r = (int)(wid / p.heads), h = (int)(wid % p.heads);
-    const int b = tree_seq_of(p.node_start, p.num_seqs, r);
-    const TreeSeq sq = tree_seq(p, b, a.block, a.unit);
-    const int rr = (r - sq.r0) * G + h % G, rl = rr % a.block;
-    if (r >= sq.r0 + sq.n) return;
-    const int64_t total = (int64_t)a.pre[p.num_seqs] * p.kv_heads, ns = shares::count(total, a.workers, a.least);
-    const int64_t f0 = (int64_t)a.pre[b] * p.kv_heads + ((int64_t)(h / G) * sq.blocks + rr / a.block) * sq.steps, f1 = f0 + sq.steps - 1;
-    const int64_t w0 = ((f0 + 1) * ns - 1) / total, w1 = ((f1 + 1) * ns - 1) / total;
-    if (w0 == w1) return;
-    const int ld = D + 4, nv = D / 32;  // 2 or 4 columns
-    const int64_t step = (int64_t)2 * a.block * ld;
-    const float* first = a.part + ((2 * w0 + (f0 > total * w0 / ns ? 1 : 0)) * a.block + rl) * ld;
-    const float* rest = a.part + (2 * w0 * a.block + rl) * ld;         // share w's piece, w > w0
-    auto piece = [&](int64_t w) { return w == w0 ? first : rest + (w - w0) * step; };
-    float mx = -INFINITY, top = -INFINITY;
-    for (int64_t w = w0 + lane; w <= w1; w += 32) {
-        mx = fmaxf(mx, piece(w)[D]);
-        top = fmaxf(top, piece(w)[D + 2]);
-    }
-    mx = warp_max(mx);
-    top = warp_max(top);
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    // pieces in order, four at a time so that their loads are in flight together
-    for (int64_t w = w0; w <= w1; w += 4) {
-        float c[4];
-        float4 v[4];
+    int w0 = blockIdx.x;
+    if constexpr (SPLIT > 1) {
+        __shared__ int s_count[kJoinWarps], s_found;
+        const int per = (a.workers + kJoinWarps * 32 - 1) / (kJoinWarps * 32);
+        int mine = 0;
+        for (int i = 0; i < per; ++i) {
+            const int w = threadIdx.x * per + i;
+            mine += w < a.workers && __ldcg(&a.notes[w].rows) > 0;
+        }
+        int before = mine;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float* s = piece(w + k < w1 ? w + k : w1);
-            const float2 ml = *reinterpret_cast<const float2*>(s + D);
-            const bool in = w + k <= w1 && !(ml.x == -INFINITY && ml.y == 0.f);         // 0 x infinity = NaN
-            c[k] = in ? exp2f(ml.x - ref) : 0.f;
-            l = in ? fmaf(c[k], ml.y, l) : l;
-            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (in && nv == 4) v[k] = *reinterpret_cast<const float4*>(s + lane * 4);
-            else if (in) {
-                const float2 x = *reinterpret_cast<const float2*>(s + lane * 2);
-                v[k].x = x.x;
-                v[k].y = x.y;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += x;
+        }
+        if (lane == 31) s_count[warp] = before;
+        if (threadIdx.x == 0) s_found = -1;
+        __syncthreads();
+        before -= mine;
+        for (int k = 0; k < warp; ++k) before += s_count[k];
+        if ((int)blockIdx.x >= before && (int)blockIdx.x < before + mine) {
+            int left = blockIdx.x - before, w = threadIdx.x * per;
+            for (;; ++w)
+                if (__ldcg(&a.notes[w].rows) > 0 && left-- == 0) break;
+            s_found = w;
+        }
+        __syncthreads();
+        w0 = s_found;
+        if (w0 < 0) return;
+    }
+    const int4* note = reinterpret_cast<const int4*>(a.notes + w0);
+    const int4 n0 = __ldcg(note), n1 = __ldcg(note + 1);
+    if ((int)blockIdx.y * ROWS >= n0.x) return;
+    const int w1 = n1.x, rl = blockIdx.y * ROWS + warp / SPLIT, rr = n0.w + rl;
+    const bool real = rl < n0.x;
+    const int64_t step = (int64_t)2 * a.block * LD;
+    const float* rest = a.part + ((int64_t)2 * w0 * a.block + rl) * LD;         // share w's piece, w > w0
+    const float* first = a.part + ((int64_t)n1.y * a.block + rl) * LD;
+    float mx = -INFINITY, top = -INFINITY, l = 0.f, acc[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) acc[i] = 0.f;
+    for (int w = w0 + warp % SPLIT; real && w <= w1; w += FLIGHT * SPLIT) {
+        float4 ml[FLIGHT];
+        float v[FLIGHT][NV];
+#pragma unroll
+        for (int k = 0; k < FLIGHT; ++k) {
+            const int wk = w + k * SPLIT;
+            if (wk > w1) continue;
+            const float* s = wk == w0 ? first : rest + (wk - w0) * step;
+            ml[k] = __ldcg(reinterpret_cast<const float4*>(s + D));
+            if constexpr (NV == 4) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(s) + lane);
+                v[k][0] = x.x; v[k][1] = x.y; v[k][NV - 2] = x.z; v[k][NV - 1] = x.w;
+            } else {
+                const float2 x = __ldcg(reinterpret_cast<const float2*>(s) + lane);
+                v[k][0] = x.x; v[k][1] = x.y;
             }
         }
+        float mn = mx;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            acc[0] = fmaf(c[k], v[k].x, acc[0]);
-            acc[1] = fmaf(c[k], v[k].y, acc[1]);
-            acc[2] = fmaf(c[k], v[k].z, acc[2]);
-            acc[3] = fmaf(c[k], v[k].w, acc[3]);
+        for (int k = 0; k < FLIGHT; ++k)
+            if (w + k * SPLIT <= w1) {
+                mn = fmaxf(mn, ml[k].x);
+                top = fmaxf(top, ml[k].z);
+            }
+        const float ref = mn == -INFINITY ? 0.f : mn, f = exp2f(mx - ref);
+        mx = mn;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) acc[i] *= f;
+#pragma unroll
+        for (int k = 0; k < FLIGHT; ++k) {
+            if (w + k * SPLIT > w1 || (ml[k].x == -INFINITY && ml[k].y == 0.f)) continue;       // saw nothing: 0 x infinity = NaN
+            const float c = exp2f(ml[k].x - ref);
+            l = fmaf(c, ml[k].y, l);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) acc[i] = fmaf(c, v[k][i], acc[i]);
         }
     }
+    if constexpr (SPLIT > 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) s_acc[warp][lane * NV + i] = acc[i];
+        if (lane == 0) {
+            s_ml[warp][0] = mx;
+            s_ml[warp][1] = l;
+            s_ml[warp][2] = top;
+        }
+        __syncthreads();
+        if (warp % SPLIT) return;
+        float all = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < SPLIT; ++k) {
+            all = fmaxf(all, s_ml[warp + k][0]);
+            top = fmaxf(top, s_ml[warp + k][2]);
+        }
+        l = 0.f;
+        mx = all;
+        const float ref = all == -INFINITY ? 0.f : all;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < SPLIT; ++k) {
+            const float m = s_ml[warp + k][0];
+            if (m == -INFINITY && s_ml[warp + k][1] == 0.f) continue;
+            const float c = exp2f(m - ref);
+            l = fmaf(c, s_ml[warp + k][1], l);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) acc[i] = fmaf(c, s_acc[warp + k][lane * NV + i], acc[i]);
+        }
+    }
+    if (!real) return;
     const float inv = 1.f / (l + 1e-6f * a.p_scale * (mx == -INFINITY ? 1.f : exp2f(top - mx)));     // the formula's sum is relative to the largest score
-    Q* out = static_cast<Q*>(p.out) + ((int64_t)r * p.heads + h) * D + lane * nv;
-    for (int i = 0; i < nv; ++i) out[i] = tree_narrow<Q>(acc[i] * inv);
+    Q* out = static_cast<Q*>(p.out) + ((int64_t)(n0.y + rr / G) * p.heads + n0.z * G + rr % G) * D + lane * NV;
+#pragma unroll
+    for (int i = 0; i < NV; i += 2) {
+        if constexpr (sizeof(Q) == 4) {
+            *reinterpret_cast<float2*>(out + i) = make_float2(acc[i] * inv, acc[i + 1] * inv);
+        } else {
+            Q two[2] = {tree_narrow<Q>(acc[i] * inv), tree_narrow<Q>(acc[i + 1] * inv)};
+            *reinterpret_cast<uint32_t*>(out + i) = *reinterpret_cast<uint32_t*>(two);
+        }
+    }
 }
 
 template <int D, int MT, int QT, int KT>
@@ -656,21 +732,39 @@ static int launch(const TreeWork& a, cudaStream_t st) {
 
 }  // namespace tstream
 
-// resident before the shares' kernel ends (programmatic dependent launch)
-int tree_join_launch(const TreeWork& a, cudaStream_t st) {
-    using namespace tstream;
+namespace tstream {
+
+template <typename Q, int NV, int SPLIT>
+static int join(const TreeWork& a, int64_t items, cudaStream_t st) {
+    const int rows = (int)((int64_t)a.p.most * (a.p.heads / a.p.kv_heads) < a.block ? a.p.most * (a.p.heads / a.p.kv_heads) : a.block);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(((int64_t)a.p.rows * a.p.heads + 3) / 4));
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3((unsigned)(SPLIT > 1 ? items : a.workers), (unsigned)((rows * SPLIT + kJoinWarps - 1) / kJoinWarps));
+    cfg.blockDim = dim3(kJoinWarps * 32);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // resident before the shares' kernel ends
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    if (a.p.q_type == F32) return (int)cudaLaunchKernelEx(&cfg, tree_join_kernel<float>, a);
-    if (a.p.q_type == F16) return (int)cudaLaunchKernelEx(&cfg, tree_join_kernel<__half>, a);
-    return (int)cudaLaunchKernelEx(&cfg, tree_join_kernel<bf16_t>, a);
+    return (int)cudaLaunchKernelEx(&cfg, tree_join_kernel<Q, NV, SPLIT>, a);
+}
+
+}  // namespace tstream
+
+int tree_join_launch(const TreeWork& a, cudaStream_t st) {
+    using namespace tstream;
+    const TreeParams& p = a.p;
+    // pieces of an item, were all items alike: from 16 (64) on a row's pieces are shared by four (eight) warps
+    const int64_t items = p.kv_heads * ((int64_t)p.rows * (p.heads / p.kv_heads) / a.block + p.num_seqs);       // at most
+    const int split = a.workers >= 64 * items ? 8 : a.workers >= 16 * items ? 4 : 1;
+#define PA_TJ(QT, Q)                                                                                                   \
+    if (p.q_type == QT) {                                                                                              \
+        if (p.dim == 64) return split == 8 ? join<Q, 2, 8>(a, items, st) : split == 4 ? join<Q, 2, 4>(a, items, st) : join<Q, 2, 1>(a, items, st);                                   \
+        return split == 8 ? join<Q, 4, 8>(a, items, st) : split == 4 ? join<Q, 4, 4>(a, items, st) : join<Q, 4, 1>(a, items, st);                                                    \
+    }
+    PA_TJ(F32, float) PA_TJ(F16, __half) PA_TJ(BF16, bf16_t)
+#undef PA_TJ
+    return PA_ERR_UNSUPPORTED;
 }
 
 int tree_stream_workers() { return tstream::kWarps * device_info().sm_count; }

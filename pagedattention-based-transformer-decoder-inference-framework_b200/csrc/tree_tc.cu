@@ -28,13 +28,15 @@ constexpr float kShift = 7.f;           // weights times 2^7
 __device__ int g_errors;
 
 __host__ __device__ constexpr int q_bytes(int D) { return D * QT * 2; }
-__host__ __device__ constexpr int stage_bytes(int D) { return 2 * D * KT * 2; }
-__host__ __device__ constexpr int stages_for(int D, int nq) { return nq == 2 ? (D == 128 ? 4 : 8) : D == 128 ? 2 : 4; }
+// the ring: tiles of keys and of values, each of 64 rows
+__host__ __device__ constexpr int tile_bytes(int D) { return D * KT * 2; }
+__host__ __device__ constexpr int ring_for(int D, int nq) { return nq == 2 ? (D == 128 ? 9 : 18) : D == 128 ? 4 : 10; }
+constexpr int kNotes = 32;              // of the producer on its tiles; more than it can be ahead
 __host__ __device__ constexpr int threads_for(int nq) { return (5 * nq + 1) * 32; }
-// kv_full, kv_empty [stage]; per query tile s_full, p_full, o_full [2], q_ready
-__host__ __device__ constexpr int nbar_for(int D, int nq) { return 2 * stages_for(D, nq) + 7 * nq; }
+// full, empty [ring]; per query tile s_full, p_full, o_full [2], q_ready
+__host__ __device__ constexpr int nbar_for(int D, int nq) { return 2 * ring_for(D, nq) + 7 * nq; }
 constexpr size_t smem_for(int D, int nq, int seqs) {
-    return (size_t)nq * q_bytes(D) + stages_for(D, nq) * stage_bytes(D) + nbar_for(D, nq) * 8 + 64 + stages_for(D, nq) * 4 + (seqs + 1) * 4 + 1024;
+    return (size_t)nq * q_bytes(D) + ring_for(D, nq) * tile_bytes(D) + nbar_for(D, nq) * 8 + 64 + kNotes * 4 + (seqs + 1) * 4 + 1024;
 }
 
 // Pieces of a share, in order.  Every role walks them for itself.
@@ -46,9 +48,10 @@ struct Walk {
     TreeSeq sq;
     int g, rr0, i0, i1;                 // the piece: kv head, first row, steps [i0, i1)
     int64_t slot;                       // of its partial sums, -1: it is a whole item
-    int64_t f_lo;
+    int64_t f_lo, total, ns;
     __device__ __forceinline__ Walk(const TreeWork& w, const int* pre_) : a(w), pre(pre_), b(-1) {
-        const int64_t total = (int64_t)pre[w.p.num_seqs] * w.p.kv_heads, ns = shares::count(total, w.workers, w.least);
+        total = (int64_t)pre[w.p.num_seqs] * w.p.kv_heads;
+        ns = shares::count(total, w.workers, w.least);
         f_lo = f = blockIdx.x < ns ? total * blockIdx.x / ns : 0;
         f_hi = blockIdx.x < ns ? total * (blockIdx.x + 1) / ns : 0;
     }
@@ -136,26 +139,26 @@ __global__ void __launch_bounds__(threads_for(NQ), NQ == 1 ? 2 : 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeWork a) {
     typedef typename Elem<BF>::T T;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    constexpr int ST = stages_for(D, NQ), NBAR = nbar_for(D, NQ), TMEM_COLS = NQ * 256, KB = D / 64;
-    constexpr int Q_BYTES = q_bytes(D), K_BYTES = D * KT * 2, STAGE = stage_bytes(D);
+    constexpr int RING = ring_for(D, NQ), NBAR = nbar_for(D, NQ), TMEM_COLS = NQ * 256, KB = D / 64;
+    constexpr int Q_BYTES = q_bytes(D), TILE = tile_bytes(D);
     constexpr int W_MMA = 4 * NQ, W_PROD = 5 * NQ;
     const TreeParams& p = a.p;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t kv_sm = base + NQ * Q_BYTES, bar0 = kv_sm + ST * STAGE;
+    const uint32_t kv_sm = base + NQ * Q_BYTES, bar0 = kv_sm + RING * TILE;
     auto kv_full = [&](int s) { return bar0 + s * 8; };
-    auto kv_empty = [&](int s) { return bar0 + (ST + s) * 8; };
-    auto s_full = [&](int x, int i) { return bar0 + (2 * ST + 7 * x + i) * 8; };
-    auto p_full = [&](int x, int i) { return bar0 + (2 * ST + 7 * x + 2 + i) * 8; };
-    auto o_full = [&](int x, int i) { return bar0 + (2 * ST + 7 * x + 4 + i) * 8; };
-    auto q_ready = [&](int x) { return bar0 + (2 * ST + 7 * x + 6) * 8; };
+    auto kv_empty = [&](int s) { return bar0 + (RING + s) * 8; };
+    auto s_full = [&](int x, int i) { return bar0 + (2 * RING + 7 * x + i) * 8; };
+    auto p_full = [&](int x, int i) { return bar0 + (2 * RING + 7 * x + 2 + i) * 8; };
+    auto o_full = [&](int x, int i) { return bar0 + (2 * RING + 7 * x + 4 + i) * 8; };
+    auto q_ready = [&](int x) { return bar0 + (2 * RING + 7 * x + 6) * 8; };
     const uint32_t tmem_slot = bar0 + NBAR * 8, fail_sm = tmem_slot + 8, odd_sm = fail_sm + 4, meta_sm = odd_sm + 8;
-    int* pre = reinterpret_cast<int*>(smem_raw + (meta_sm + ST * 4 - smem_u32(smem_raw)));
+    int* pre = reinterpret_cast<int*>(smem_raw + (meta_sm + kNotes * 4 - smem_u32(smem_raw)));
     auto failed = [&] { return tc_failed(fail_sm); };
     auto wait = [&](uint32_t bar, uint32_t parity) { tc_wait(bar, parity, fail_sm, a.polls); };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.heads / p.kv_heads;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < ST; ++s) {
+        for (int s = 0; s < RING; ++s) {
             mbar_init(kv_full(s), 1);
             mbar_init(kv_empty(s), NQ);
         }
@@ -176,8 +179,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     }
     if (warp == W_MMA) tmem_alloc(tmem_slot, TMEM_COLS);
     shares::count_units(pre, p.num_seqs, [&](int b) { return tree_seq(p, b, a.block, a.unit).units(); });
-    if (blockIdx.x == 0)
-        for (int b = threadIdx.x; b <= p.num_seqs; b += blockDim.x) a.pre[b] = pre[b];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tc_fence_before();
     __syncthreads();
@@ -185,72 +186,83 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     uint32_t tmem_base;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
     Walk w(a, pre);
-    // which query tiles of the piece have rows, and its tiles of keys
+    // Tiles go through the ring in the order of their products: K(0), K(1), V(0), K(2), V(1), ..., K(n - 1), V(n - 2), V(n - 1); the ring's
+    // count `at` runs on through the pieces
+    auto k_at = [&](uint32_t at, int i) { return at + (uint32_t)(i == 0 ? 0 : 2 * i - 1); };
+    auto v_at = [&](uint32_t at, int i, int nt) { return at + (uint32_t)(i + 1 < nt ? 2 * i + 2 : 2 * nt - 1); };
+    auto slot_of = [&](uint32_t c) { return (int)(c % RING); };
+    auto phase_of = [&](uint32_t c) { return c / RING & 1u; };
+    // which query tiles of the piece have rows
     auto has_rows = [&](int x) { return w.rr0 + x * QT < w.sq.n * G; };
 
     if (warp == W_PROD) {
         if (elect_one()) {
-            int s = 0;
-            uint32_t ph = 1;
+            uint32_t c = 0, tiles = 0;              // requests and tiles of keys so far
+            if (w.f >= w.f_hi) a.notes[blockIdx.x] = TreeNote{};
             bool ok = true;
+            auto request = [&](const CUtensorMap* map, const int (&r)[4]) {
+                const int s = (int)(c % RING);
+                wait(kv_empty(s), (c / RING & 1u) ^ 1u);
+                if (failed()) {
+                    ok = false;
+                    return;
+                }
+                const uint32_t st = kv_sm + s * TILE;
+                mbar_arrive_expect_tx(kv_full(s), TILE);
+#pragma unroll
+                for (int uu = 0; uu < 4; ++uu)
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb) tma_load_2d(st + kb * 8192 + uu * 2048, map, kb * 64, r[uu], kv_full(s));
+                ++c;
+            };
             while (ok && w.next()) {
+                if (w.f >= w.f_hi) a.notes[blockIdx.x] = tree_note(a, w.sq, w.g, w.rr0, w.i0, w.i1, w.f - w.i1, w.total, w.ns, w.slot);
                 const int row = p.beam_ids ? __ldg(p.beam_ids + w.b) : w.b;
                 const int32_t* trow = p.table + ((int64_t)row * p.kv_heads + w.g) * p.num_tiles;
                 const bool row_ok = (unsigned)row < (unsigned)p.num_beams;
-                int pgn[4];
+                int page[4], r[4], prev[4] = {0, 0, 0, 0};
                 auto load_pages = [&](int i) {
 #pragma unroll
                     for (int uu = 0; uu < 4; ++uu) {
                         const int t0 = (i * 4 + uu) * 16, t = t0 / p.tile_size;
-                        const int page = row_ok && t0 < w.sq.keys && t < p.num_tiles ? __ldg(trow + t) : -1;
-                        pgn[uu] = (unsigned)page < (unsigned)p.total_pages ? page * p.tile_size + (t0 - t * p.tile_size) : -1;
+                        const int pg = row_ok && t0 < w.sq.keys && t < p.num_tiles ? __ldg(trow + t) : -1;
+                        page[uu] = (unsigned)pg < (unsigned)p.total_pages ? pg * p.tile_size + (t0 - t * p.tile_size) : -1;
                     }
                 };
                 load_pages(w.i0);
-                for (int i = w.i0; i < w.i1; ++i) {
-                    int r[4];
-                    uint32_t mask = 0;
+                for (int i = w.i0; i <= w.i1 && ok; ++i) {          // K(i) and V(i - 1)
+                    if (i < w.i1) {
+                        uint32_t mask = 0;
 #pragma unroll
-                    for (int uu = 0; uu < 4; ++uu) {
-                        r[uu] = pgn[uu] >= 0 ? pgn[uu] : a.total_rows;          // no page: zeros, and its scores are masked
-                        mask |= (pgn[uu] >= 0 ? 1u : 0u) << uu;
+                        for (int uu = 0; uu < 4; ++uu) {
+                            r[uu] = page[uu] >= 0 ? page[uu] : a.total_rows;        // no page: zeros, and its scores are masked
+                            mask |= (page[uu] >= 0 ? 1u : 0u) << uu;
+                        }
+                        if (i + 1 < w.i1) load_pages(i + 1);
+                        asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(meta_sm + tiles++ % kNotes * 4), "r"(mask) : "memory");
+                        request(&tmK, r);
                     }
-                    if (i + 1 < w.i1) load_pages(i + 1);
-                    wait(kv_empty(s), ph);
-                    if (failed()) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t st = kv_sm + s * STAGE;
-                    asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(meta_sm + s * 4), "r"(mask) : "memory");
-                    mbar_arrive_expect_tx(kv_full(s), STAGE);
+                    if (i > w.i0 && ok) request(&tmV, prev);
 #pragma unroll
-                    for (int uu = 0; uu < 4; ++uu)
-#pragma unroll
-                        for (int kb = 0; kb < KB; ++kb) tma_load_2d(st + kb * 8192 + uu * 2048, &tmK, kb * 64, r[uu], kv_full(s));
-#pragma unroll
-                    for (int uu = 0; uu < 4; ++uu)
-#pragma unroll
-                        for (int kb = 0; kb < KB; ++kb) tma_load_2d(st + K_BYTES + kb * 8192 + uu * 2048, &tmV, kb * 64, r[uu], kv_full(s));
-                    if (++s == ST) {
-                        s = 0;
-                        ph ^= 1u;
-                    }
+                    for (int uu = 0; uu < 4; ++uu) prev[uu] = r[uu];
                 }
             }
             if (failed())       // let the copies in flight land before the CTA's shared memory goes away
-                for (int i = 0; i < ST; ++i) tc_let_land(kv_full(i), i < s ? ph ^ 1u : ph);
+                for (uint32_t i = c > RING ? c - RING : 0; i < c; ++i) tc_let_land(kv_full((int)(i % RING)), i / RING & 1u);
         }
     } else if (warp >= W_MMA) {
         constexpr uint32_t kIdescS = idesc_f16(QT, KT, 0, 0, BF), kIdescO = idesc_f16(QT, D, 0, 1, BF);
         const int x = warp - W_MMA;
-        int s = 0, n = 0, qn = 0;           // stage; key tiles and pieces of this query tile so far
-        uint32_t kv_ph = 0;
+        int n = 0, qn = 0;                  // key tiles and pieces of this query tile so far
+        uint32_t at = 0;
         while (w.next()) {
             const bool mine = has_rows(x);
-            auto issue_S = [&](int i, int stage) {
-                if (elect_one()) {
-                    const uint32_t st = kv_sm + stage * STAGE, qx = base + x * Q_BYTES;
+            auto issue_S = [&](int i) {     // every issuer waits for every tile: its arrival at the empty barrier belongs to THIS use of it
+                const int s = slot_of(k_at(at, i));
+                wait(kv_full(s), phase_of(k_at(at, i)));
+                tc_fence_after();
+                if (mine && elect_one()) {
+                    const uint32_t st = kv_sm + s * TILE, qx = base + x * Q_BYTES;
                     const int sb = (n + i) & 1;
 #pragma unroll
                     for (int ks = 0; ks < D / 16; ++ks) {
@@ -261,30 +273,25 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                     umma_commit(s_full(x, sb));
                 }
                 __syncwarp();
+                if (elect_one()) umma_commit(kv_empty(s));
+                __syncwarp();
             };
             const int nt = w.i1 - w.i0;
-            wait(kv_full(s), kv_ph);
-            if (mine) {
-                wait(q_ready(x), (uint32_t)qn & 1u);
-                tc_fence_after();
-                issue_S(0, s);
-            }
+            if (mine) wait(q_ready(x), (uint32_t)qn & 1u);
+            issue_S(0);
             for (int i = 0; i < nt; ++i) {
-                const int s_next = (s + 1 == ST) ? 0 : s + 1;
-                if (i + 1 < nt) {           // every issuer waits for every stage: its arrival on kv_empty belongs to THIS use of it
-                    wait(kv_full(s_next), (s + 1 == ST) ? (kv_ph ^ 1u) : kv_ph);
-                    tc_fence_after();
-                    if (mine) issue_S(i + 1, s_next);
-                }
+                if (i + 1 < nt) issue_S(i + 1);
+                const int s = slot_of(v_at(at, i, nt));
+                wait(kv_full(s), phase_of(v_at(at, i, nt)));
                 if (mine) {
-                    const uint32_t st = kv_sm + s * STAGE;
+                    const uint32_t st = kv_sm + s * TILE;
                     const int sb = (n + i) & 1, nvalid = min(KT, w.sq.keys - (w.i0 + i) * KT);
                     if (nvalid & 15) {
                         // value rows past the last key may hold anything (0 x NaN = NaN): zeros (both issuers write the same)
                         const int r1 = (nvalid + 15) & ~15;
                         for (int idx = lane; idx < (r1 - nvalid) * (D / 8); idx += 32) {
                             const int r = nvalid + idx / (D / 8), c = idx % (D / 8);
-                            const uint32_t addr = st + K_BYTES + (c >> 3) * 8192 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                            const uint32_t addr = st + (c >> 3) * 8192 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
                             asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(addr), "r"(0u) : "memory");
                         }
                         fence_proxy_async();
@@ -297,7 +304,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         const int ksteps = (nvalid + 15) >> 4;
                         for (int ks = 0; ks < ksteps; ++ks) {
                             const uint32_t ta = tmem_base + x * 2 * KT + sb * KT + ks * 8;
-                            const uint64_t db = make_desc(st + K_BYTES + ks * 2048, 8192, 1024);
+                            const uint64_t db = make_desc(st + ks * 2048, 8192, 1024);
                             umma_f16_ts(tmem_base + NQ * 2 * KT + x * D, ta, db, kIdescO, (i > 0 || ks > 0) ? 1u : 0u);
                         }
                         umma_commit(o_full(x, sb));
@@ -306,11 +313,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 }
                 if (elect_one()) umma_commit(kv_empty(s));
                 __syncwarp();
-                if (++s == ST) {
-                    s = 0;
-                    kv_ph ^= 1u;
-                }
             }
+            at += 2 * nt;
             if (mine) {
                 n += nt;
                 ++qn;
@@ -331,18 +335,14 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         // P.V(t) is complete.  Unambiguous without consuming every phase: S(n) follows P.V(n - 2) on the pipe, so by the time a
         // thread works on tile n the barrier of P.V(n - 1) is in the phase asked for or just past it.
         auto pv_done = [&](int t) { wait(o_full(x, t & 1), (uint32_t)((t >> 1) & 1)); };
-        int st_i = 0, n = 0;
-        uint32_t st_ph = 0;
-        auto next_stage = [&] {
-            if (++st_i == ST) {
-                st_i = 0;
-                st_ph ^= 1u;
-            }
-        };
+        int n = 0;
+        uint32_t tiles = 0;                 // of keys, of all pieces
+        uint32_t at = 0;
         while (w.next()) {
             const int nt = w.i1 - w.i0, all = w.sq.n * G;
             if (!has_rows(x)) {
-                for (int i = 0; i < nt; ++i) next_stage();
+                at += 2 * nt;
+                tiles += nt;
                 continue;
             }
             const int rr = w.rr0 + row_in_block + lane, rows = min(32, all - w.rr0 - row_in_block);       // rows of this warp, may be negative
@@ -383,8 +383,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 wait(s_full(x, sb), (uint32_t)((n + i) >> 1) & 1u);
                 tc_fence_after();
                 if (drafts) {       // values that are not finite (the keys past the last one were looked at or are zeros)
-                    wait(kv_full(st_i), st_ph);
-                    const uint32_t vt = kv_sm + st_i * STAGE + K_BYTES;
+                    const uint32_t c = v_at(at, i, nt);
+                    wait(kv_full(slot_of(c)), phase_of(c));
+                    const uint32_t vt = kv_sm + slot_of(c) * TILE;
                     const int mine = threadIdx.x & 127, r = mine >> 1;
                     if (kp0 + r < w.sq.keys) {
 #pragma unroll
@@ -399,11 +400,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 }
                 if (rows <= 0) {    // nothing of this warp's: it only keeps the barriers' count
                     mbar_arrive_cnt(p_full(x, sb));
-                    next_stage();
                     continue;
                 }
-                uint32_t mapped;    // the producer's note about this stage, older than the scores
-                asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(mapped) : "r"(meta_sm + st_i * 4) : "memory");
+                uint32_t mapped;    // the producer's note about this tile, older than the scores
+                asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(mapped) : "r"(meta_sm + (tiles + i) % kNotes * 4) : "memory");
                 uint32_t sr[2][32];
                 tmem_ld32(s_addr + sb * KT, sr[0]);
                 tmem_ld32(s_addr + sb * KT + 32, sr[1]);
@@ -448,7 +448,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         tmem_wait_st();
                         tc_fence_before();
                         mbar_arrive_cnt(p_full(x, sb));
-                        next_stage();
                         continue;
                     }
                     acc[0] = acc[1] = 0ull;
@@ -487,9 +486,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive_cnt(p_full(x, sb));
-                next_stage();
             }
             n += nt;
+            at += 2 * nt;
+            tiles += nt;
             pv_done(n - 1);
             tc_fence_after();
             if (w.i1 * KT > w.sq.ctx) {         // the piece had drafted keys
@@ -579,7 +579,7 @@ int tree_tc_workers(int block) { return device_info().sm_count * (block == 128 ?
 // Rows of a block, 0 where this kernel does not serve or the streaming one is faster
 int tree_tc_block(const TreeParams& p) {
     const int G = p.heads / p.kv_heads, rows = p.most * G;
-    if (!((p.q_type == PA_TYPE_F16 && p.kv_type == PA_TYPE_F16) || (p.q_type == PA_TYPE_BF16 && p.kv_type == PA_TYPE_BF16)) || rows <= 32) return 0;
+    if (!((p.q_type == PA_TYPE_F16 && p.kv_type == PA_TYPE_F16) || (p.q_type == PA_TYPE_BF16 && p.kv_type == PA_TYPE_BF16)) || rows <= 16) return 0;
     if ((p.dim != 64 && p.dim != 128) || p.tile_size % 16 || p.num_seqs > kTreeMostSeqs) return 0;
     if ((int64_t)p.total_pages * p.tile_size >= 0x7fffff00ll || ((uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.q | (uintptr_t)p.out) % 16 || p.q_stride % 8) return 0;
     const int block = rows <= 128 ? 128 : 256;
