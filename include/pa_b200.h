@@ -1036,14 +1036,17 @@ int pa_conv_append_in_words(int units, int columns, int num_items, int64_t rows)
  *   returns 0.
  * pa_adjust_logits: row r of d_logits (rows `stride` elements apart; type PA_TYPE_F32, _F16 or _BF16) belongs to sequence
  *   d_row_seq[r] (NULL: r).  With c the number of times a token v stands in d_history[d_history_start[b] ..
- *   d_history_start[b + 1] - 1] and, where d_tokens is given, on the way from the root to row r's node (itself included):
+ *   d_history_start[b + 1] - 1] and, where d_tokens is given, on the way to row r's node: the tokens
+ *   of the sequence's nodes (d_node_start) whose bits d_path [rows][path_words] has (pa_tree_attention's mask; at most
+ *   PA_TREE_MOST_NODES):
  *     c > 0: x = x > 0 ? x / repetition : x * repetition, x -= presence, x -= frequency * c;   x += bias;
  *     a bit of d_allowed that is 0: x = -inf
  *   penalties per sequence (device arrays), or one value where the array is NULL.  Biases of sequence b are the entries
  *   d_bias_start[b] .. of (d_bias_ids, d_bias); of entries for the same token the last counts.  d_allowed: rows of
  *   allowed_stride 32-bit words, row d_allowed_rows[r] (NULL: r; negative: everything is allowed).  Tokens outside the
  *   vocabulary are ignored.  d_out (NULL: not wanted; may be d_logits) gets the logits in their type, d_ids (NULL: not wanted)
- *   the lowest index of the largest float before it is rounded (NaN never wins; 0 where nothing does).
+ *   the lowest index of the largest float before it is rounded (NaN never wins; 0 where nothing does); d_ids take a workspace
+ *   that is zero before the first call and left so by every call.
  * pa_tree_accept: from node 0 to the child whose token is the one chosen at the node (d_ids[row]; of several the lowest) as
  *   long as there is one.  d_counts[b]: nodes on that path (0 for a sequence without nodes); d_nodes, d_out_tokens
  *   [num_seqs][depth]: the nodes and what was chosen at them, -1 behind them; d_new_lens[b] = d_ctx_lens[b] + d_counts[b].
@@ -1061,12 +1064,14 @@ int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void* d_out
                       int num_tiles, int total_pages, const int32_t* d_beam_ids, const int32_t* d_ctx_lens, const int32_t* d_node_start,
                       const int32_t* d_mask, int mask_words, int rows, int num_seqs, int most_nodes, int heads, int head_dim,
                       int tile_size, float temperature, void* d_workspace, size_t workspace_bytes, pa_stream_t stream);
+size_t pa_adjust_logits_workspace_bytes(int rows);
 int pa_adjust_logits(const void* d_logits, int type, int64_t stride, int rows, int vocab, void* d_out, int64_t out_stride,
                      int32_t* d_ids, const int32_t* d_row_seq, const int32_t* d_history, const int32_t* d_history_start,
                      const float* d_repetition, const float* d_presence, const float* d_frequency, float repetition, float presence,
                      float frequency, const int32_t* d_bias_ids, const float* d_bias, const int32_t* d_bias_start,
                      const int32_t* d_allowed, int64_t allowed_stride, const int32_t* d_allowed_rows, const int32_t* d_tokens,
-                     const int32_t* d_parents, const int32_t* d_node_start, pa_stream_t stream);
+                     const int32_t* d_path, int path_words, const int32_t* d_node_start, void* d_workspace, size_t workspace_bytes,
+                     pa_stream_t stream);
 int pa_tree_accept(const int32_t* d_ids, const int32_t* d_tokens, const int32_t* d_parents, const int32_t* d_node_start, int num_seqs,
                    int most_nodes, int depth, const int32_t* d_ctx_lens, const int32_t* d_beam_ids, int num_beams, int kv_heads,
                    int num_tiles, int total_pages, int tile_size, int key_bytes, int value_bytes, int num_caches, void* const* caches,

@@ -6,19 +6,31 @@
 //     x = logits[r][v];   c > 0:  x = x > 0 ? x / repetition : x * repetition,  x -= presence;   x -= frequency c
 //     x += bias[b][v];    not allowed[r][v]:  x = -inf;       id[r] = the lowest v of the largest x
 // each operation rounded by itself (IEEE float, no contraction), 16-bit logits widened first and the result rounded once.
+//
+// One CTA has a chunk of one row.  A bulk copy brings the chunk into shared memory while the CTA counts the tokens of its chunk that the
+// sequence's history and the node's way have (32-bit counts by integer atomics: no order), with a bit for every token that a rule touches:
+// some percent of the vocabulary, scattered over it.  Those are done first, one per thread, in shared memory; then the chunk streams out
+// through the mask.  (Rules in the stream took three times as long: nearly every warp has a touched token among its 128.  CTAs that stay and
+// keep counts for several rows took longer too: 126 against 103 us, for their chain of small loads.)  Several small CTAs per SM cover each
+// other's chain: bounds of the history, its tokens, the counts.
+// Greedy ids: the largest (value, lowest index) of a chunk as one 64-bit word, joined over the chunks by an atomic maximum that nobody waits
+// for; a second kernel (programmatic dependent launch) turns the words into ids and zeroes them.  (Counting the CTAs at a row, so that the last
+// one does that, held every CTA's place for two trips to L2 more: 61 us for 256 x 128000 logits.)
 #include "seq_common.cuh"
 
 namespace pa {
 namespace rules {
 
-constexpr int kThreads = 512, kChunk = 4096;
+constexpr int kThreads = 256, kMostBytes = 16384, kBiases = 512, kList = 1024;
+constexpr uint32_t kPolls = 1u << 25;           // of the wait for a copy
+constexpr uint32_t kBiased = 0x80000000u;
 
 struct Args {
     const void* logits;
     void* out;                  // null: only ids
     int32_t* ids;               // null: only logits
     int64_t stride, out_stride;
-    int rows, vocab;
+    int rows, vocab, chunk, chunks;                        // tokens of a chunk, chunks of a row
     const int32_t *history, *history_start, *row_seq;
     const float *repetition, *presence, *frequency;        // per sequence; null: the value beside it
     float repetition1, presence1, frequency1;
@@ -27,7 +39,10 @@ struct Args {
     const uint32_t* allowed;
     int64_t allowed_stride;
     const int32_t* allowed_rows;
-    const int32_t *tokens, *parents, *node_start;          // drafted trees, or null
+    const int32_t *tokens, *node_start;                    // drafted trees, or null
+    const uint32_t* path;                                  // [rows, path_words]: nodes on a row's way
+    int path_words;
+    unsigned long long* best;                              // [rows], zero
 };
 
 template <typename T> __device__ __forceinline__ float widen(T v) { return to_f32<T>(v); }
@@ -35,74 +50,276 @@ template <> __device__ __forceinline__ float widen<__half>(__half v) { return __
 template <typename T> __device__ __forceinline__ T narrow(float v) { return from_f32<T>(v); }
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 
-__device__ __forceinline__ float adjust(float x, uint32_t c, float rep, float pres, float freq) {
-    if (c) {
-        x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-        x = __fsub_rn(x, pres);
-        x = __fsub_rn(x, __fmul_rn(freq, (float)c));
-    }
-    return x;
+// 16 bytes of a row
+template <typename T> struct __align__(16) Word {
+    static constexpr int N = 16 / (int)sizeof(T);
+    T v[N];
+};
+__device__ __forceinline__ unsigned long long key_of(float f, int v) {
+    const uint32_t u = __float_as_uint(f + 0.f), o = u & 0x80000000u ? ~u : u | 0x80000000u;       // ordered as the numbers, -0 as 0
+    return (unsigned long long)o << 32 | (uint32_t)~v;
 }
 
-// One CTA per row, kChunk tokens at a time: counts and bias places in shared memory, then one pass over the chunk's logits.
+// shared memory: the chunk (its ends widened to whole words), counts, a bit per touched token, the mask, a list of touched tokens, biases
+template <typename T> __host__ __device__ constexpr int data_bytes(int chunk) { return chunk * (int)sizeof(T) + 32; }
+template <typename T>
+static size_t shared_bytes(const Args& a) {
+    return data_bytes<T>(a.chunk) + a.chunk * 4 + 2 * (a.chunk / 32 + 4) * 4 + kList * 2 + (a.bias ? kBiases * 8 : 0);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
-    __shared__ uint32_t count[kChunk], place[kChunk];
-    __shared__ float sv[kThreads / 32];
-    __shared__ int si[kThreads / 32];
-    const int r = blockIdx.x, b = a.row_seq ? a.row_seq[r] : r;
-    const T* x = static_cast<const T*>(a.logits) + (int64_t)r * a.stride;
-    T* out = a.out ? static_cast<T*>(a.out) + (int64_t)r * a.out_stride : nullptr;
-    const int64_t mrow = a.allowed_rows ? a.allowed_rows[r] : r;
-    const uint32_t* allowed = a.allowed && mrow >= 0 ? a.allowed + mrow * a.allowed_stride : nullptr;
-    const float rep = a.repetition ? a.repetition[b] : a.repetition1, pres = a.presence ? a.presence[b] : a.presence1;
-    const float freq = a.frequency ? a.frequency[b] : a.frequency1;
-    float best = -INFINITY;
-    int bi = 0x7fffffff;
-    for (int v0 = 0; v0 < a.vocab; v0 += kChunk) {
-        const int nv = min(kChunk, a.vocab - v0);
-        for (int i = threadIdx.x; i < nv; i += kThreads) count[i] = place[i] = 0;
-        __syncthreads();
-        if (a.history)
-            for (int i = a.history_start[b] + threadIdx.x; i < a.history_start[b + 1]; i += kThreads) {
-                const int v = a.history[i] - v0;
-                if ((unsigned)v < (unsigned)nv) atomicAdd(&count[v], 1u);
-            }
-        if (a.tokens && threadIdx.x == 0) {
-            const int s0 = a.node_start[b];
-            for (int i = r - s0; i >= 0; i = a.parents[s0 + i] < i ? a.parents[s0 + i] : -1) {
-                const int v = a.tokens[s0 + i] - v0;
-                if ((unsigned)v < (unsigned)nv) atomicAdd(&count[v], 1u);
-            }
-        }
-        if (a.bias)
-            for (int i = a.bias_start[b] + threadIdx.x; i < a.bias_start[b + 1]; i += kThreads) {
-                const int v = a.bias_ids[i] - v0;
-                if ((unsigned)v < (unsigned)nv) atomicMax(&place[v], (uint32_t)i + 1u);
-            }
-        __syncthreads();
-        for (int i = threadIdx.x; i < nv; i += kThreads) {
-            const int v = v0 + i;
-            float f = adjust(widen<T>(x[v]), count[i], rep, pres, freq);
-            if (place[i]) f = __fadd_rn(f, a.bias[place[i] - 1]);
-            if (allowed && !((allowed[v >> 5] >> (v & 31)) & 1u)) f = -INFINITY;
-            if (out) out[v] = narrow<T>(f);
-            if (f > best || (f == best && v < bi)) { best = f; bi = v; }
-        }
-        __syncthreads();
+    constexpr int N = Word<T>::N;
+    extern __shared__ __align__(16) uint8_t smem[];
+    T* data = reinterpret_cast<T*>(smem);
+    uint32_t *count = reinterpret_cast<uint32_t*>(smem + data_bytes<T>(a.chunk)), *touched = count + a.chunk, *mask = touched + a.chunk / 32 + 4;
+    uint16_t* list = reinterpret_cast<uint16_t*>(mask + a.chunk / 32 + 4);
+    int *bias_v = reinterpret_cast<int*>(list + kList), *bias_i = bias_v + kBiases;
+    __shared__ int s_biases, s_sum[kThreads / 32];
+    __shared__ unsigned long long s_key[kThreads / 32];
+    __shared__ __align__(8) uint64_t s_bar;
+    const int r = blockIdx.x / a.chunks, v0 = (blockIdx.x - r * a.chunks) * a.chunk, nv = min(a.chunk, a.vocab - v0), tid = threadIdx.x;
+    const T* x = static_cast<const T*>(a.logits) + (int64_t)r * a.stride + v0;
+    // ---- the chunk, from the 16-byte word that it begins in to the one that it ends in
+    const int off = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+    const uint32_t bar = smem_u32(&s_bar);
+    if (tid == 0) {
+        mbar_init(bar, 1);
+        mbar_fence_init();
+        const uint32_t bytes = (uint32_t)((off + nv) * (int)sizeof(T) + 15) & ~15u;
+        mbar_arrive_expect_tx(bar, bytes);
+        bulk_g2s_nohint(smem_u32(data), x - off, bytes, bar);
+        s_biases = 0;
     }
-    if (!a.ids) return;
-    auto join = [&](float ov, int oi) {
-        if (ov > best || (ov == best && oi < bi)) { best = ov; bi = oi; }
-    };
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) join(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, bi, o));
-    if ((threadIdx.x & 31) == 0) { sv[threadIdx.x >> 5] = best; si[threadIdx.x >> 5] = bi; }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // ---- bounds and bits that nothing waits for yet
+    const int b = a.row_seq ? __ldg(a.row_seq + r) : r;
+    int h0 = 0, h1 = 0, i0 = 0, i1 = 0, s0 = 0;
+    uint32_t way = 0;
+    if (a.history) {
+        h0 = __ldg(a.history_start + b);
+        h1 = __ldg(a.history_start + b + 1);
+    }
+    if (a.bias) {
+        i0 = __ldg(a.bias_start + b);
+        i1 = __ldg(a.bias_start + b + 1);
+    }
+    if (a.tokens) {             // thread j has word j of the node's way, the first 32 nodes are everyone's
+        s0 = __ldg(a.node_start + b);
+        way = tid < a.path_words ? __ldg(a.path + (int64_t)r * a.path_words + tid) : 0u;
+    }
+    const int64_t mrow = a.allowed_rows ? __ldg(a.allowed_rows + r) : r;
+    const uint32_t* allowed = a.allowed && mrow >= 0 ? a.allowed + mrow * a.allowed_stride + (v0 >> 5) : nullptr;
+    const float rep = a.repetition ? __ldg(a.repetition + b) : a.repetition1, pres = a.presence ? __ldg(a.presence + b) : a.presence1;
+    const float freq = a.frequency ? __ldg(a.frequency + b) : a.frequency1;
+    for (int i = tid; i < a.chunk / 4; i += kThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
+    const int mwords = (nv + 31) >> 5;
+    for (int i = tid; i < a.chunk / 32 + 4; i += kThreads) {
+        touched[i] = 0u;
+        if (a.allowed) mask[i] = i >= mwords ? 0u : allowed ? __ldg(allowed + i) : 0xffffffffu;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kThreads / 32; ++w) join(sv[w], si[w]);
-        a.ids[r] = bi == 0x7fffffff ? 0 : bi;
+    // ---- the touched tokens
+    auto note = [&](int v) { atomicOr(&touched[v >> 5], 1u << (v & 31)); };
+    auto add = [&](int token) {
+        const int v = token - v0;
+        if ((unsigned)v < (unsigned)nv) {
+            atomicAdd(&count[v], 1u);
+            note(v);
+        }
+    };
+    if (a.history) {
+        const int q0 = min(h1, h0 + (int)((16 - ((uintptr_t)(a.history + h0) & 15)) & 15) / 4), q1 = h1 > q0 ? q0 + ((h1 - q0) & ~3) : q0;
+        if (tid < q0 - h0) add(__ldg(a.history + h0 + tid));
+        if (tid >= 32 && tid - 32 < h1 - q1) add(__ldg(a.history + q1 + tid - 32));
+        for (int i = q0 + 4 * tid; i < q1; i += 16 * kThreads) {
+            int4 t[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                t[k] = i + 4 * k * kThreads < q1 ? __ldg(reinterpret_cast<const int4*>(a.history + i + 4 * k * kThreads)) : make_int4(-1, -1, -1, -1);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                add(t[k].x);
+                add(t[k].y);
+                add(t[k].z);
+                add(t[k].w);
+            }
+        }
     }
+    for (uint32_t m = way; m; m &= m - 1) add(__ldg(a.tokens + s0 + tid * 32 + __ffs(m) - 1));
+    if (a.bias)
+        for (int i = i0 + tid; i < i1; i += kThreads) {
+            const int v = __ldg(a.bias_ids + i) - v0;
+            if ((unsigned)v >= (unsigned)nv) continue;
+            atomicOr(&count[v], kBiased);
+            note(v);
+            const int place = atomicAdd(&s_biases, 1);
+            if (place < kBiases) {
+                bias_v[place] = v;
+                bias_i[place] = i;
+            }
+        }
+    __syncthreads();
+    // thread j numbers the touched tokens of word j
+    const uint32_t mine = tid < a.chunk / 32 ? touched[tid] : 0u;
+    int before = __popc(mine), total = 0;
+    {
+        const int own = before;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, before, o);
+            if ((tid & 31) >= o) before += u;
+        }
+        if ((tid & 31) == 31) s_sum[tid >> 5] = before;
+        before -= own;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kThreads / 32; ++k) {
+        before += k < (tid >> 5) ? s_sum[k] : 0;
+        total += s_sum[k];
+    }
+    bool here = true;
+    for (uint32_t polls = 0; !mbar_try_wait(bar, 0); ++polls)
+        if (polls > kPolls) {
+            here = false;
+            break;
+        }
+    // ---- their rules, in place
+    auto is_allowed = [&](int i) { return !a.allowed || (mask[i >> 5] >> (i & 31) & 1u); };
+    float best = -INFINITY;
+    int bi = -1;
+    auto offer = [&](float f, int i) {          // of equal ones the lowest, in whatever order they come
+        if (f > best || (f == best && bi >= 0 && v0 + i < bi)) {
+            best = f;
+            bi = v0 + i;
+        }
+    };
+    for (int from = 0; from < total; from += kList) {
+        int n = before - from;
+        for (uint32_t m = mine; m; m &= m - 1, ++n)
+            if ((unsigned)n < (unsigned)kList) list[n] = (uint16_t)(tid * 32 + __ffs(m) - 1);
+        __syncthreads();
+        for (int k = tid; k < min(kList, total - from); k += kThreads) {
+            const int i = list[k];
+        const uint32_t raw = count[i], c = raw & ~kBiased;
+        float f = widen<T>(data[off + i]);
+        if (c) {
+            f = f > 0.f ? __fdiv_rn(f, rep) : __fmul_rn(f, rep);
+            f = __fsub_rn(f, pres);
+            f = __fsub_rn(f, __fmul_rn(freq, (float)c));
+        }
+        if (raw & kBiased) {
+            int last = -1;
+            if (s_biases <= kBiases) {
+                for (int q = 0; q < s_biases; ++q)
+                    if (bias_v[q] == i) last = max(last, bias_i[q]);
+            } else {            // more than were kept: the last entry of them all
+                for (int q = i1 - 1; last < 0; --q)
+                    if (__ldg(a.bias_ids + q) == v0 + i) last = q;
+            }
+            f = __fadd_rn(f, __ldg(a.bias + last));
+        }
+        if (a.ids && is_allowed(i)) offer(f, i);        // before it is rounded
+        data[off + i] = narrow<T>(f);
+        }
+        __syncthreads();
+    }
+    // ---- the stream: words of the result
+    T* out = a.out ? static_cast<T*>(a.out) + (int64_t)r * a.out_stride + v0 : nullptr;
+    const T* edge = out ? out : x;
+    const int head = min(nv, (int)((16 - ((uintptr_t)edge & 15)) & 15) / (int)sizeof(T)), words = (nv - head) / N, tail = head + words * N;
+    const bool whole = (off + head) % N == 0;           // they are words of the chunk as well
+    if (!here) bi = -1;
+    auto single = [&](int i) {                          // a place outside the words
+        float f = widen<T>(data[off + i]);
+        if (!is_allowed(i)) f = -INFINITY;
+        if (a.ids && !(touched[i >> 5] >> (i & 31) & 1u)) offer(f, i);
+        if (out) out[i] = here ? narrow<T>(f) : narrow<T>(__int_as_float(0x7fc00000));
+    };
+    if (tid < head) single(tid);
+    for (int k = tid; k < words; k += kThreads) {
+        const int i = head + k * N;
+        Word<T> w;
+        if (whole) w = *reinterpret_cast<const Word<T>*>(data + off + i);
+        else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) w.v[e] = data[off + i + e];
+        }
+        if (a.allowed) {
+            const uint32_t ok = __funnelshift_r(mask[i >> 5], mask[(i >> 5) + 1], i & 31);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (!(ok >> e & 1u)) w.v[e] = narrow<T>(-INFINITY);
+        }
+        if (!here) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) w.v[e] = narrow<T>(__int_as_float(0x7fc00000));
+        }
+        if (out) *reinterpret_cast<Word<T>*>(out + i) = w;
+        if (a.ids) {
+            const uint32_t t = __funnelshift_r(touched[i >> 5], touched[(i >> 5) + 1], i & 31);
+            float f[N], top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                f[e] = t >> e & 1u ? -INFINITY : widen<T>(w.v[e]);
+                top = fmaxf(top, f[e]);
+            }
+            if (top > best || (top == best && bi > v0 + i)) {
+#pragma unroll
+                for (int e = N - 1; e >= 0; --e)
+                    if (f[e] == top && top > -INFINITY) bi = v0 + i + e;
+                best = top;
+            }
+        }
+    }
+    if (tail + tid < nv) single(tail + tid);
+    if (!a.ids) return;
+    unsigned long long key = bi >= 0 ? key_of(best, bi) : 0ull;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+    if ((tid & 31) == 0) s_key[tid >> 5] = key;
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int k = 1; k < kThreads / 32; ++k) key = max(key, s_key[k]);
+        if (key) atomicMax(a.best + r, key);
+    }
+}
+
+__global__ void __launch_bounds__(128) rules_ids_kernel(unsigned long long* best, int rows, int32_t* ids) {
+    const int r = blockIdx.x * 128 + threadIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (r >= rows) return;
+    const unsigned long long key = __ldcg(best + r);
+    ids[r] = key ? (int32_t)~(uint32_t)key : 0;
+    best[r] = 0ull;
+}
+
+template <typename T>
+static int launch(Args a, cudaStream_t st) {
+    // few rows: smaller chunks, until every SM has one
+    a.chunk = kMostBytes / (int)sizeof(T);
+    while (a.chunk > 1024 && (int64_t)a.rows * ((a.vocab + a.chunk - 1) / a.chunk) < device_info().sm_count) a.chunk /= 2;
+    a.chunks = (a.vocab + a.chunk - 1) / a.chunk;
+    const int64_t ctas = (int64_t)a.rows * a.chunks;
+    if (ctas > 0x7fffffff) return PA_ERR_UNSUPPORTED;
+    const size_t smem = shared_bytes<T>(a);
+    cudaError_t e = cudaFuncSetAttribute(rules_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    rules_kernel<T><<<(unsigned)ctas, kThreads, smem, st>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || !a.ids) return (int)e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((a.rows + 127) / 128));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, rules_ids_kernel, a.best, a.rows, a.ids);
 }
 
 }  // namespace rules
@@ -110,24 +327,33 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
 
 using namespace pa;
 
+PA_API size_t pa_adjust_logits_workspace_bytes(int rows) { return rows > 0 ? (size_t)rows * 8 : 0; }
+
 PA_API int pa_adjust_logits(const void* d_logits, int type, int64_t stride, int rows, int vocab, void* d_out, int64_t out_stride,
                             int32_t* d_ids, const int32_t* d_row_seq, const int32_t* d_history, const int32_t* d_history_start,
                             const float* d_repetition, const float* d_presence, const float* d_frequency, float repetition, float presence,
                             float frequency, const int32_t* d_bias_ids, const float* d_bias, const int32_t* d_bias_start,
                             const int32_t* d_allowed, int64_t allowed_stride, const int32_t* d_allowed_rows, const int32_t* d_tokens,
-                            const int32_t* d_parents, const int32_t* d_node_start, pa_stream_t stream) {
+                            const int32_t* d_path, int path_words, const int32_t* d_node_start, void* d_workspace, size_t workspace_bytes,
+                            pa_stream_t stream) {
     using namespace pa::rules;
     PA_CHECK_ARG(rows >= 0 && vocab > 0 && stride >= vocab && (!d_out || out_stride >= vocab) && (d_out || d_ids));
     if (rows == 0) return PA_OK;
     PA_CHECK_ARG(d_logits && (!d_history || d_history_start) && (!d_bias || (d_bias_ids && d_bias_start)));
-    PA_CHECK_ARG((!d_allowed || allowed_stride >= ((int64_t)vocab + 31) / 32) && (!d_tokens || (d_parents && d_node_start && d_row_seq)));
-    const Args a{d_logits, d_out, d_ids, stride, out_stride, rows, vocab, d_history, d_history_start, d_row_seq, d_repetition, d_presence,
-                 d_frequency, repetition, presence, frequency, d_bias_ids, d_bias_start, d_bias, reinterpret_cast<const uint32_t*>(d_allowed),
-                 allowed_stride, d_allowed_rows, d_tokens, d_parents, d_node_start};
+    PA_CHECK_ARG((!d_allowed || allowed_stride >= ((int64_t)vocab + 31) / 32) && (!d_tokens || (d_path && path_words > 0 && d_node_start && d_row_seq)));
+    if (d_ids && (!d_workspace || (uintptr_t)d_workspace % 8 || workspace_bytes < pa_adjust_logits_workspace_bytes(rows))) return PA_ERR_WORKSPACE;
+    Args a{};
+    a.logits = d_logits; a.out = d_out; a.ids = d_ids; a.stride = stride; a.out_stride = out_stride; a.rows = rows; a.vocab = vocab;
+    a.history = d_history; a.history_start = d_history_start; a.row_seq = d_row_seq;
+    a.repetition = d_repetition; a.presence = d_presence; a.frequency = d_frequency;
+    a.repetition1 = repetition; a.presence1 = presence; a.frequency1 = frequency;
+    a.bias_ids = d_bias_ids; a.bias_start = d_bias_start; a.bias = d_bias;
+    a.allowed = reinterpret_cast<const uint32_t*>(d_allowed); a.allowed_stride = allowed_stride; a.allowed_rows = d_allowed_rows;
+    a.tokens = d_tokens; a.node_start = d_node_start; a.path = reinterpret_cast<const uint32_t*>(d_path); a.path_words = path_words;
+    a.best = static_cast<unsigned long long*>(d_workspace);
     cudaStream_t st = as_stream(stream);
-    if (type == PA_TYPE_F32) rules_kernel<float><<<rows, kThreads, 0, st>>>(a);
-    else if (type == PA_TYPE_F16) rules_kernel<__half><<<rows, kThreads, 0, st>>>(a);
-    else if (type == PA_TYPE_BF16) rules_kernel<bf16_t><<<rows, kThreads, 0, st>>>(a);
-    else return PA_ERR_UNSUPPORTED;
-    PA_RETURN_LAUNCH_STATUS();
+    if (type == PA_TYPE_F32) return launch<float>(a, st);
+    if (type == PA_TYPE_F16) return launch<__half>(a, st);
+    if (type == PA_TYPE_BF16) return launch<bf16_t>(a, st);
+    return PA_ERR_UNSUPPORTED;
 }

@@ -79,6 +79,9 @@ def sample(logits, temperature=1.0, top_k=0, top_p=1.0, eos_token_id=-1, eos_thr
     return sample_from_probs(probs, u)
 
 
+_rule_words = {}        # (device, stream) -> workspace of pa_adjust_logits
+
+
 def _rules(logits, out, ids, history, history_start, repetition, presence, frequency, bias, allowed, allowed_rows, row_seq, tree):
     dev, types = logits.device, {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
     if logits.dim() != 2 or logits.dtype not in types or not logits.is_cuda:
@@ -132,15 +135,22 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
             of(allowed_rows, torch.int32, "allowed_rows", rows)
     if rows == 0:
         return
-    # (stride(0) of a single row may be anything)
-    with torch.cuda.device(dev):
-        _cabi.check(_cabi.lib().pa_adjust_logits(
+    lib = _cabi.lib()
+    with _cabi.on_device(dev):
+        stream, ws, need = _cabi.stream(), None, 0
+        if ids is not None:     # words that every call leaves at zero, one buffer per stream
+            need = lib.pa_adjust_logits_workspace_bytes(rows)
+            ws = _rule_words.get((dev.index, stream))
+            if ws is None or ws.numel() < need:
+                ws = _rule_words[(dev.index, stream)] = torch.zeros(max(need, 1 << 14), dtype=torch.uint8, device=dev)
+        # (the stride of a single row may be anything)
+        _cabi.check(lib.pa_adjust_logits(
             logits.data_ptr(), types[logits.dtype], logits.stride(0) if rows > 1 else V, rows, V, _cabi.ptr(out),
             0 if out is None else out.stride(0) if rows > 1 else V, _cabi.ptr(ids), _cabi.ptr(row_seq), _cabi.ptr(history), _cabi.ptr(history_start),
             *(_cabi.ptr(a) for a in arrays), *values, _cabi.ptr(b_ids), _cabi.ptr(b_val), _cabi.ptr(b_start), _cabi.ptr(allowed),
             0 if allowed is None else allowed.stride(0) if allowed.shape[0] > 1 else allowed.shape[1], _cabi.ptr(allowed_rows),
-            *((tree.tokens.data_ptr(), tree.parents.data_ptr(), tree.node_start.data_ptr()) if tree is not None else (None, None, None)),
-            _cabi.stream()), "pa_adjust_logits")
+            *((tree.tokens.data_ptr(), tree.mask.data_ptr(), tree.mask.shape[1], tree.node_start.data_ptr()) if tree is not None else
+              (None, None, 0, None)), _cabi.ptr(ws), need, stream), "pa_adjust_logits")
 
 
 def adjust_logits(logits, history=None, history_start=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None,
