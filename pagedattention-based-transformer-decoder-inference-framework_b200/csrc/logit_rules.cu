@@ -8,20 +8,22 @@
 // each operation rounded by itself (IEEE float, no contraction), 16-bit logits widened first and the result rounded once.
 //
 // One CTA has a chunk of one row.  A bulk copy brings the chunk into shared memory while the CTA counts the tokens of its chunk that the
-// sequence's history and the node's way have (32-bit counts by integer atomics: no order), with a bit for every token that a rule touches:
-// some percent of the vocabulary, scattered over it.  Those are done first, one per thread, in shared memory; then the chunk streams out
+// sequence's history and the node's way have (32-bit counts by integer atomics: no order) and lists the tokens that a rule touches: some
+// percent of the vocabulary, scattered over it.  Those are done first, one per thread, in shared memory; then the chunk streams out
 // through the mask.  (Rules in the stream took three times as long: nearly every warp has a touched token among its 128.  CTAs that stay and
 // keep counts for several rows took longer too: 126 against 103 us, for their chain of small loads.)  Several small CTAs per SM cover each
 // other's chain: bounds of the history, its tokens, the counts.
 // Greedy ids: the largest (value, lowest index) of a chunk as one 64-bit word, joined over the chunks by an atomic maximum that nobody waits
 // for; a second kernel (programmatic dependent launch) turns the words into ids and zeroes them.  (Counting the CTAs at a row, so that the last
 // one does that, held every CTA's place for two trips to L2 more: 61 us for 256 x 128000 logits.)
+#include <type_traits>
+
 #include "seq_common.cuh"
 
 namespace pa {
 namespace rules {
 
-constexpr int kThreads = 256, kMostBytes = 16384, kBiases = 512, kList = 1024;
+constexpr int kThreads = 256, kChunk = 4096, kBiases = 512, kList = 1024;
 constexpr uint32_t kPolls = 1u << 25;           // of the wait for a copy
 constexpr uint32_t kBiased = 0x80000000u;
 
@@ -55,27 +57,28 @@ template <typename T> struct __align__(16) Word {
     static constexpr int N = 16 / (int)sizeof(T);
     T v[N];
 };
-__device__ __forceinline__ unsigned long long key_of(float f, int v) {
-    const uint32_t u = __float_as_uint(f + 0.f), o = u & 0x80000000u ? ~u : u | 0x80000000u;       // ordered as the numbers, -0 as 0
-    return (unsigned long long)o << 32 | (uint32_t)~v;
-}
+template <typename T> struct Pair { typedef float2 type; };
+template <> struct Pair<__half> { typedef __half2 type; };
+template <> struct Pair<bf16_t> { typedef __nv_bfloat162 type; };
 
-// shared memory: the chunk (its ends widened to whole words), counts, a bit per touched token, the mask, a list of touched tokens, biases
+// shared memory: the chunk (its ends widened to whole words), counts, the mask, for 16-bit logits a bit per touched token, a list of touched
+// tokens, biases
 template <typename T> __host__ __device__ constexpr int data_bytes(int chunk) { return chunk * (int)sizeof(T) + 32; }
 template <typename T>
 static size_t shared_bytes(const Args& a) {
-    return data_bytes<T>(a.chunk) + a.chunk * 4 + 2 * (a.chunk / 32 + 4) * 4 + kList * 2 + (a.bias ? kBiases * 8 : 0);
+    return data_bytes<T>(a.chunk) + a.chunk * 4 + (sizeof(T) < 4 ? 2 : 1) * (a.chunk / 32 + 4) * 4 + kList * 2 + (a.bias ? kBiases * 8 : 0);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
     constexpr int N = Word<T>::N;
+    constexpr bool ROUNDS = sizeof(T) < 4;              // a touched token's float may win before it is rounded, not after
     extern __shared__ __align__(16) uint8_t smem[];
     T* data = reinterpret_cast<T*>(smem);
-    uint32_t *count = reinterpret_cast<uint32_t*>(smem + data_bytes<T>(a.chunk)), *touched = count + a.chunk, *mask = touched + a.chunk / 32 + 4;
-    uint16_t* list = reinterpret_cast<uint16_t*>(mask + a.chunk / 32 + 4);
+    uint32_t *count = reinterpret_cast<uint32_t*>(smem + data_bytes<T>(a.chunk)), *mask = count + a.chunk, *touched = mask + a.chunk / 32 + 4;
+    uint16_t* list = reinterpret_cast<uint16_t*>(touched + (ROUNDS ? a.chunk / 32 + 4 : 0));
     int *bias_v = reinterpret_cast<int*>(list + kList), *bias_i = bias_v + kBiases;
-    __shared__ int s_biases, s_sum[kThreads / 32];
+    __shared__ int s_listed, s_biases;
     __shared__ unsigned long long s_key[kThreads / 32];
     __shared__ __align__(8) uint64_t s_bar;
     const int r = blockIdx.x / a.chunks, v0 = (blockIdx.x - r * a.chunks) * a.chunk, nv = min(a.chunk, a.vocab - v0), tid = threadIdx.x;
@@ -89,7 +92,7 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
         const uint32_t bytes = (uint32_t)((off + nv) * (int)sizeof(T) + 15) & ~15u;
         mbar_arrive_expect_tx(bar, bytes);
         bulk_g2s_nohint(smem_u32(data), x - off, bytes, bar);
-        s_biases = 0;
+        s_listed = s_biases = 0;
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // ---- bounds and bits that nothing waits for yet
@@ -104,7 +107,7 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
         i0 = __ldg(a.bias_start + b);
         i1 = __ldg(a.bias_start + b + 1);
     }
-    if (a.tokens) {             // thread j has word j of the node's way, the first 32 nodes are everyone's
+    if (a.tokens) {             // thread j has word j of the node's way
         s0 = __ldg(a.node_start + b);
         way = tid < a.path_words ? __ldg(a.path + (int64_t)r * a.path_words + tid) : 0u;
     }
@@ -112,21 +115,25 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
     const uint32_t* allowed = a.allowed && mrow >= 0 ? a.allowed + mrow * a.allowed_stride + (v0 >> 5) : nullptr;
     const float rep = a.repetition ? __ldg(a.repetition + b) : a.repetition1, pres = a.presence ? __ldg(a.presence + b) : a.presence1;
     const float freq = a.frequency ? __ldg(a.frequency + b) : a.frequency1;
-    for (int i = tid; i < a.chunk / 4; i += kThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
-    const int mwords = (nv + 31) >> 5;
-    for (int i = tid; i < a.chunk / 32 + 4; i += kThreads) {
-        touched[i] = 0u;
-        if (a.allowed) mask[i] = i >= mwords ? 0u : allowed ? __ldg(allowed + i) : 0xffffffffu;
+    if (a.history || a.tokens || a.bias)
+        for (int i = tid; i < a.chunk / 4; i += kThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (ROUNDS || a.allowed) {
+        const int mwords = (nv + 31) >> 5;
+        for (int i = tid; i < a.chunk / 32 + 4; i += kThreads) {
+            if (ROUNDS) touched[i] = 0u;
+            if (a.allowed) mask[i] = i >= mwords ? 0u : allowed ? __ldg(allowed + i) : 0xffffffffu;
+        }
     }
     __syncthreads();
     // ---- the touched tokens
-    auto note = [&](int v) { atomicOr(&touched[v >> 5], 1u << (v & 31)); };
+    auto note = [&](int v) {
+        if (ROUNDS) atomicOr(&touched[v >> 5], 1u << (v & 31));
+        const int at = atomicAdd(&s_listed, 1);
+        if (at < kList) list[at] = (uint16_t)v;
+    };
     auto add = [&](int token) {
         const int v = token - v0;
-        if ((unsigned)v < (unsigned)nv) {
-            atomicAdd(&count[v], 1u);
-            note(v);
-        }
+        if ((unsigned)v < (unsigned)nv && atomicAdd(&count[v], 1u) == 0u) note(v);
     };
     if (a.history) {
         const int q0 = min(h1, h0 + (int)((16 - ((uintptr_t)(a.history + h0) & 15)) & 15) / 4), q1 = h1 > q0 ? q0 + ((h1 - q0) & ~3) : q0;
@@ -139,46 +146,31 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
                 t[k] = i + 4 * k * kThreads < q1 ? __ldg(reinterpret_cast<const int4*>(a.history + i + 4 * k * kThreads)) : make_int4(-1, -1, -1, -1);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                add(t[k].x);
-                add(t[k].y);
-                add(t[k].z);
-                add(t[k].w);
+                const unsigned n = (unsigned)nv;
+                if ((unsigned)(t[k].x - v0) < n || (unsigned)(t[k].y - v0) < n || (unsigned)(t[k].z - v0) < n || (unsigned)(t[k].w - v0) < n) {
+                    add(t[k].x);
+                    add(t[k].y);
+                    add(t[k].z);
+                    add(t[k].w);
+                }
             }
         }
     }
     for (uint32_t m = way; m; m &= m - 1) add(__ldg(a.tokens + s0 + tid * 32 + __ffs(m) - 1));
-    if (a.bias)
+    if (a.bias) {
+        if (a.history || a.tokens) __syncthreads();     // a token is noted once
         for (int i = i0 + tid; i < i1; i += kThreads) {
             const int v = __ldg(a.bias_ids + i) - v0;
             if ((unsigned)v >= (unsigned)nv) continue;
-            atomicOr(&count[v], kBiased);
-            note(v);
+            if (atomicOr(&count[v], kBiased) == 0u) note(v);
             const int place = atomicAdd(&s_biases, 1);
             if (place < kBiases) {
                 bias_v[place] = v;
                 bias_i[place] = i;
             }
         }
-    __syncthreads();
-    // thread j numbers the touched tokens of word j
-    const uint32_t mine = tid < a.chunk / 32 ? touched[tid] : 0u;
-    int before = __popc(mine), total = 0;
-    {
-        const int own = before;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, before, o);
-            if ((tid & 31) >= o) before += u;
-        }
-        if ((tid & 31) == 31) s_sum[tid >> 5] = before;
-        before -= own;
     }
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kThreads / 32; ++k) {
-        before += k < (tid >> 5) ? s_sum[k] : 0;
-        total += s_sum[k];
-    }
     bool here = true;
     for (uint32_t polls = 0; !mbar_try_wait(bar, 0); ++polls)
         if (polls > kPolls) {
@@ -188,40 +180,38 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
     // ---- their rules, in place
     auto is_allowed = [&](int i) { return !a.allowed || (mask[i >> 5] >> (i & 31) & 1u); };
     float best = -INFINITY;
-    int bi = -1;
+    int bi = 0x7fffffff;
     auto offer = [&](float f, int i) {          // of equal ones the lowest, in whatever order they come
-        if (f > best || (f == best && bi >= 0 && v0 + i < bi)) {
+        if (f > best || (f == best && f > -INFINITY && i < bi)) {
             best = f;
-            bi = v0 + i;
+            bi = i;
         }
     };
-    for (int from = 0; from < total; from += kList) {
-        int n = before - from;
-        for (uint32_t m = mine; m; m &= m - 1, ++n)
-            if ((unsigned)n < (unsigned)kList) list[n] = (uint16_t)(tid * 32 + __ffs(m) - 1);
-        __syncthreads();
-        for (int k = tid; k < min(kList, total - from); k += kThreads) {
-            const int i = list[k];
-        const uint32_t raw = count[i], c = raw & ~kBiased;
-        float f = widen<T>(data[off + i]);
-        if (c) {
-            f = f > 0.f ? __fdiv_rn(f, rep) : __fmul_rn(f, rep);
-            f = __fsub_rn(f, pres);
-            f = __fsub_rn(f, __fmul_rn(freq, (float)c));
-        }
-        if (raw & kBiased) {
-            int last = -1;
-            if (s_biases <= kBiases) {
-                for (int q = 0; q < s_biases; ++q)
-                    if (bias_v[q] == i) last = max(last, bias_i[q]);
-            } else {            // more than were kept: the last entry of them all
-                for (int q = i1 - 1; last < 0; --q)
-                    if (__ldg(a.bias_ids + q) == v0 + i) last = q;
+    if (s_listed > 0) {
+        const bool kept = s_listed <= kList;            // else every token is looked at
+        for (int k = tid; k < (kept ? s_listed : nv); k += kThreads) {
+            const int i = kept ? list[k] : k;
+            const uint32_t raw = count[i], c = raw & ~kBiased;
+            if (!raw) continue;
+            float f = widen<T>(data[off + i]);
+            if (c) {
+                f = f > 0.f ? __fdiv_rn(f, rep) : __fmul_rn(f, rep);
+                f = __fsub_rn(f, pres);
+                f = __fsub_rn(f, __fmul_rn(freq, (float)c));
             }
-            f = __fadd_rn(f, __ldg(a.bias + last));
-        }
-        if (a.ids && is_allowed(i)) offer(f, i);        // before it is rounded
-        data[off + i] = narrow<T>(f);
+            if (raw & kBiased) {
+                int last = -1;
+                if (s_biases <= kBiases) {
+                    for (int q = 0; q < s_biases; ++q)
+                        if (bias_v[q] == i) last = max(last, bias_i[q]);
+                } else {        // more than were kept: the last entry of them all
+                    for (int q = i1 - 1; last < 0; --q)
+                        if (__ldg(a.bias_ids + q) == v0 + i) last = q;
+                }
+                f = __fadd_rn(f, __ldg(a.bias + last));
+            }
+            if (ROUNDS && a.ids && is_allowed(i)) offer(f, i);
+            data[off + i] = narrow<T>(f);
         }
         __syncthreads();
     }
@@ -230,16 +220,18 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
     const T* edge = out ? out : x;
     const int head = min(nv, (int)((16 - ((uintptr_t)edge & 15)) & 15) / (int)sizeof(T)), words = (nv - head) / N, tail = head + words * N;
     const bool whole = (off + head) % N == 0;           // they are words of the chunk as well
-    if (!here) bi = -1;
+    const T nan = narrow<T>(__int_as_float(0x7fc00000));
+    if (!here) {                        // the copy did not come: NaN
+        best = -INFINITY;
+        for (int i = tid; i < nv; i += kThreads) data[off + i] = nan;
+        __syncthreads();
+    }
     auto single = [&](int i) {                          // a place outside the words
-        float f = widen<T>(data[off + i]);
-        if (!is_allowed(i)) f = -INFINITY;
-        if (a.ids && !(touched[i >> 5] >> (i & 31) & 1u)) offer(f, i);
-        if (out) out[i] = here ? narrow<T>(f) : narrow<T>(__int_as_float(0x7fc00000));
+        const T v = is_allowed(i) ? data[off + i] : narrow<T>(-INFINITY);
+        if (a.ids && !(ROUNDS && (touched[i >> 5] >> (i & 31) & 1u))) offer(widen<T>(v), i);
+        if (out) out[i] = v;
     };
-    if (tid < head) single(tid);
-    for (int k = tid; k < words; k += kThreads) {
-        const int i = head + k * N;
+    auto word = [&](int i) {
         Word<T> w;
         if (whole) w = *reinterpret_cast<const Word<T>*>(data + off + i);
         else {
@@ -248,42 +240,77 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
         }
         if (a.allowed) {
             const uint32_t ok = __funnelshift_r(mask[i >> 5], mask[(i >> 5) + 1], i & 31);
+            if constexpr (ROUNDS) {
+                constexpr uint32_t NINF = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+                uint32_t* p = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (!(ok >> e & 1u)) w.v[e] = narrow<T>(-INFINITY);
-        }
-        if (!here) {
+                for (int e = 0; e < N / 2; ++e) {
+                    const uint32_t keep = (0u - (ok >> 2 * e & 1u)) & 0xffffu | (0u - (ok >> (2 * e + 1) & 1u)) << 16;
+                    p[e] = (p[e] & keep) | (NINF & ~keep);
+                }
+            } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e) w.v[e] = narrow<T>(__int_as_float(0x7fc00000));
+                for (int e = 0; e < N; ++e)
+                    if (!(ok >> e & 1u)) w.v[e] = narrow<T>(-INFINITY);
+            }
         }
+        return w;
+    };
+    // the numbers of a word, and the largest: touched tokens of 16-bit logits as -infinity
+    auto contest = [&](Word<T> w, int i, float (&f)[N]) {
+        const uint32_t t = ROUNDS ? __funnelshift_r(touched[i >> 5], touched[(i >> 5) + 1], i & 31) : 0u;
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = ROUNDS && (t >> e & 1u) ? -INFINITY : widen<T>(w.v[e]);
+    };
+    auto largest = [&](const Word<T>& w, int i) {
+        if constexpr (ROUNDS) {
+            if (!(__funnelshift_r(touched[i >> 5], touched[(i >> 5) + 1], i & 31) & ((1u << N) - 1u))) {
+                typedef typename Pair<T>::type P;
+                const P* p = reinterpret_cast<const P*>(&w);
+                const P m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+                return fmaxf(widen<T>(m.x), widen<T>(m.y));
+            }
+        }
+        float f[N];
+        contest(w, i, f);
+        float top = f[0];
+#pragma unroll
+        for (int e = 1; e < N; ++e) top = fmaxf(top, f[e]);
+        return top;
+    };
+    if (tid < head) single(tid);
+    if (tail + tid < nv) single(tail + tid);
+    float wbest = -INFINITY;
+    int wi = -1;                                        // the first word with the largest
+    for (int i = head + tid * N; i < tail; i += kThreads * N) {
+        const Word<T> w = word(i);
         if (out) *reinterpret_cast<Word<T>*>(out + i) = w;
         if (a.ids) {
-            const uint32_t t = __funnelshift_r(touched[i >> 5], touched[(i >> 5) + 1], i & 31);
-            float f[N], top = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                f[e] = t >> e & 1u ? -INFINITY : widen<T>(w.v[e]);
-                top = fmaxf(top, f[e]);
-            }
-            if (top > best || (top == best && bi > v0 + i)) {
-#pragma unroll
-                for (int e = N - 1; e >= 0; --e)
-                    if (f[e] == top && top > -INFINITY) bi = v0 + i + e;
-                best = top;
+            const float top = largest(w, i);
+            if (top > wbest) {
+                wbest = top;
+                wi = i;
             }
         }
     }
-    if (tail + tid < nv) single(tail + tid);
     if (!a.ids) return;
-    unsigned long long key = bi >= 0 ? key_of(best, bi) : 0ull;
+    if (wi >= 0) {
+        float f[N];
+        contest(word(wi), wi, f);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
-    if ((tid & 31) == 0) s_key[tid >> 5] = key;
+        for (int e = N - 1; e >= 0; --e)
+            if (f[e] == wbest) offer(wbest, wi + e);
+    }
+    // (value, lowest index) of the warp, then of the CTA
+    const uint32_t u = __float_as_uint(best + 0.f), o = best > -INFINITY ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;   // ordered as the numbers, -0 as 0
+    const uint32_t top = __reduce_max_sync(0xffffffffu, o), at = __reduce_min_sync(0xffffffffu, o == top ? (uint32_t)bi : 0xffffffffu);
+    if ((tid & 31) == 0) s_key[tid >> 5] = top ? (unsigned long long)top << 32 | (uint32_t)~(v0 + (int)at) : 0ull;
     __syncthreads();
-    if (tid == 0) {
-#pragma unroll
-        for (int k = 1; k < kThreads / 32; ++k) key = max(key, s_key[k]);
-        if (key) atomicMax(a.best + r, key);
+    if (tid < 32) {
+        unsigned long long key = tid < kThreads / 32 ? s_key[tid] : 0ull;
+        const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32));
+        const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32) == hi ? (uint32_t)key : 0u);
+        if (tid == 0 && hi) atomicMax(a.best + r, (unsigned long long)hi << 32 | lo);
     }
 }
 
@@ -299,7 +326,7 @@ __global__ void __launch_bounds__(128) rules_ids_kernel(unsigned long long* best
 template <typename T>
 static int launch(Args a, cudaStream_t st) {
     // few rows: smaller chunks, until every SM has one
-    a.chunk = kMostBytes / (int)sizeof(T);
+    a.chunk = kChunk;
     while (a.chunk > 1024 && (int64_t)a.rows * ((a.vocab + a.chunk - 1) / a.chunk) < device_info().sm_count) a.chunk /= 2;
     a.chunks = (a.vocab + a.chunk - 1) / a.chunk;
     const int64_t ctas = (int64_t)a.rows * a.chunks;
