@@ -649,6 +649,7 @@ int latent_decode_errors(int* host_count);
 // not in the core library
 int tree_stream_errors(int* host_count) __attribute__((weak));
 int tree_tc_errors(int* host_count) __attribute__((weak));
+int tree_terms_errors(int* host_count) __attribute__((weak));
 
 int masked_attention_tc_launch(const MaskAttnParams& p, int ntiles, int q_tiles, cudaStream_t st) {
     using namespace atc;
@@ -754,12 +755,13 @@ PA_API int pa_latent_attention_expanded(const void* d_q, int64_t q_stride, int q
 
 PA_API int pa_attention_tc_errors(int* host_count) {
     PA_CHECK_ARG(host_count);
-    int n = 0, masked = 0, latent = 0, tree = 0, tree_tc = 0;
+    int n = 0, masked = 0, latent = 0, tree = 0, tree_tc = 0, tree_terms = 0;
     int rc = (int)cudaMemcpyFromSymbol(&n, pa::atc::g_errors, sizeof(int));
     if (rc == PA_OK) rc = masked_decode_errors(&masked);
     if (rc == PA_OK) rc = latent_decode_errors(&latent);
     if (rc == PA_OK && pa::tree_stream_errors) rc = tree_stream_errors(&tree);
     if (rc == PA_OK && pa::tree_tc_errors) rc = tree_tc_errors(&tree_tc);
-    *host_count = n + masked + latent + tree + tree_tc;
+    if (rc == PA_OK && pa::tree_terms_errors) rc = tree_terms_errors(&tree_terms);
+    *host_count = n + masked + latent + tree + tree_tc + tree_terms;
     return rc;
 }

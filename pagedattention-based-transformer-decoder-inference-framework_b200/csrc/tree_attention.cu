@@ -99,8 +99,8 @@ PA_API size_t pa_tree_attention_workspace_bytes(int rows, int num_seqs, int most
         return 0;
     // whichever kernel serves: it goes by the types too
     size_t most = 0;
-    for (int block : {16, 32, 128, 256}) {
-        const size_t n = tree_work_bytes(num_seqs, block <= 32 ? tree_stream_workers() : tree_tc_workers(block), block, head_dim);
+    for (int block : {16, 32, 64, 128, 256}) {
+        const size_t n = tree_work_bytes(num_seqs, block <= 32 ? tree_stream_workers() : block == 64 ? tree_terms_workers() : tree_tc_workers(block), block, head_dim);
         if (n > most) most = n;
     }
     return most;
@@ -123,13 +123,19 @@ PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void
                        reinterpret_cast<const uint32_t*>(d_mask), q_type, kv_type, num_beams, kv_heads, num_tiles, total_pages, mask_words,
                        rows, num_seqs, most_nodes, heads, head_dim, tile_size, temperature};
     cudaStream_t st = as_stream(stream);
-    const int tc_block = tree_tc_block(p), block = tc_block ? tc_block : tree_stream_block(p);
-    if (block) {
-        const int workers = tc_block ? tree_tc_workers(block) : tree_stream_workers();
-        if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < tree_work_bytes(num_seqs, workers, block, head_dim)) return PA_ERR_WORKSPACE;
-        const TreeWork w{p, workers, kTreeLeast, block, tc_block ? 64 : 16, total_pages * tile_size, kTreeStreamScale, tc::kPolls, static_cast<TreeNote*>(d_workspace),
-                         reinterpret_cast<float*>(static_cast<TreeNote*>(d_workspace) + workers)};
-        int rc = tc_block ? tree_tc_launch(w, st) : tree_stream_launch(w, st);
+    struct Form {
+        int block, workers, unit;
+        int (*launch)(const TreeWork&, cudaStream_t);
+    };
+    Form f{tree_tc_block(p), 0, 64, tree_tc_launch};
+    f.workers = tree_tc_workers(f.block);
+    if (!f.block) f = Form{tree_terms_block(p), tree_terms_workers(), 128, tree_terms_launch};
+    if (!f.block) f = Form{tree_stream_block(p), tree_stream_workers(), 16, tree_stream_launch};
+    if (f.block) {
+        if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < tree_work_bytes(num_seqs, f.workers, f.block, head_dim)) return PA_ERR_WORKSPACE;
+        const TreeWork w{p, f.workers, kTreeLeast, f.block, f.unit, total_pages * tile_size, kTreeStreamScale, tc::kPolls, static_cast<TreeNote*>(d_workspace),
+                         reinterpret_cast<float*>(static_cast<TreeNote*>(d_workspace) + f.workers)};
+        int rc = f.launch(w, st);
         if (rc == PA_OK) rc = tree_join_launch(w, st);
         if (rc != PA_ERR_UNSUPPORTED) return rc;
     }

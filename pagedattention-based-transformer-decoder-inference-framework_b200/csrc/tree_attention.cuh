@@ -1,4 +1,5 @@
-// tree_attention.cuh -- what the kernels of attention over drafted trees share (tree_attention.cu, tree_stream.cu).
+// tree_attention.cuh -- what the kernels of attention over drafted trees share (tree_attention.cu, tree_stream.cu,
+// tree_tc.cu, tree_terms.cu).
 //
 // The rows of a sequence that share a kv head are its nodes' query heads: row rr = node * G + head of the group, G = heads / kv_heads.
 // An item is a block of `block` such rows of one (sequence, kv head) with the keys that its sequence has, in steps of `unit` keys.  The
@@ -119,5 +120,9 @@ int tree_join_launch(const TreeWork& w, cudaStream_t st);
 int tree_tc_workers(int block);
 int tree_tc_block(const TreeParams& p);
 int tree_tc_launch(const TreeWork& w, cudaStream_t st);
+// tree_terms.cu: float queries over half pages, int8 pages
+int tree_terms_workers();
+int tree_terms_block(const TreeParams& p);
+int tree_terms_launch(const TreeWork& w, cudaStream_t st);
 
 }  // namespace pa

@@ -15,7 +15,7 @@
 // each row sees alone.
 #include "softmax_tile.cuh"
 #include "tcgen05_utils.cuh"
-#include "tree_attention.cuh"
+#include "tree_pieces.cuh"
 
 namespace pa {
 namespace ttc {
@@ -39,100 +39,8 @@ constexpr size_t smem_for(int D, int nq, int seqs) {
     return (size_t)nq * q_bytes(D) + ring_for(D, nq) * tile_bytes(D) + nbar_for(D, nq) * 8 + 64 + kNotes * 4 + (seqs + 1) * 4 + 1024;
 }
 
-// Pieces of a share, in order.  Every role walks them for itself.
-struct Walk {
-    const TreeWork& a;
-    const int* pre;
-    int64_t f, f_hi;
-    int b, item;                        // item within the sequence
-    TreeSeq sq;
-    int g, rr0, i0, i1;                 // the piece: kv head, first row, steps [i0, i1)
-    int64_t slot;                       // of its partial sums, -1: it is a whole item
-    int64_t f_lo, total, ns;
-    __device__ __forceinline__ Walk(const TreeWork& w, const int* pre_) : a(w), pre(pre_), b(-1) {
-        total = (int64_t)pre[w.p.num_seqs] * w.p.kv_heads;
-        ns = shares::count(total, w.workers, w.least);
-        f_lo = f = blockIdx.x < ns ? total * blockIdx.x / ns : 0;
-        f_hi = blockIdx.x < ns ? total * (blockIdx.x + 1) / ns : 0;
-    }
-    __device__ __forceinline__ bool next() {
-        if (f >= f_hi) return false;
-        const TreeParams& p = a.p;
-        if (b < 0 || f >= (int64_t)pre[b + 1] * p.kv_heads) {
-            b = shares::find_token(pre, p.num_seqs, f, p.kv_heads);
-            sq = tree_seq(p, b, a.block, a.unit);
-        }
-        const int64_t rem = f - (int64_t)pre[b] * p.kv_heads;
-        item = (int)(rem / sq.steps);
-        i0 = (int)(rem - (int64_t)item * sq.steps);
-        g = item / sq.blocks;
-        rr0 = (item - g * sq.blocks) * a.block;
-        const int64_t left = f_hi - f;
-        i1 = left < sq.steps - i0 ? i0 + (int)left : sq.steps;
-        slot = i0 == 0 && i1 == sq.steps ? -1 : 2 * (int64_t)blockIdx.x + (f - i0 > f_lo ? 1 : 0);
-        f += i1 - i0;
-        return true;
-    }
-};
-
 template <bool BF> struct Elem { typedef __half T; };
 template <> struct Elem<true> { typedef bf16_t T; };
-
-// Row by row, keys [k0, k1) that the row sees and no others (see above): by a warp, lanes over columns
-template <int D, bool BF>
-__device__ __noinline__ void piece_by_rows(const TreeWork& a, const Walk& w, int row_in_block, int rows) {
-    typedef typename Elem<BF>::T T;
-    constexpr int NC = D / 32;
-    const TreeParams& p = a.p;
-    const int lane = threadIdx.x & 31, G = p.heads / p.kv_heads;
-    const int trow = p.beam_ids ? __ldg(p.beam_ids + w.b) : w.b;
-    const float fe = 1.4426950408889634f / p.temperature;
-    for (int x = 0; x < rows; ++x) {
-        const int rr = w.rr0 + row_in_block + x;
-        if (rr >= w.sq.n * G) break;
-        const int node = rr / G, h = w.g * G + rr % G, r = w.sq.r0 + node;
-        const T* q = static_cast<const T*>(p.q) + (int64_t)r * p.q_stride + (int64_t)h * D;
-        const uint32_t* mask = p.mask + (int64_t)r * p.mask_words;
-        float qf[NC], o[NC], m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            qf[c] = tree_widen<T>(q[lane + 32 * c]);
-            o[c] = 0.f;
-        }
-        for (int t = w.i0 * KT; t < min(w.i1 * KT, w.sq.keys); ++t) {
-            const int j = t - w.sq.ctx;
-            if (j >= 0 && (j >= p.mask_words * 32 || !((__ldg(mask + (j >> 5)) >> (j & 31)) & 1u))) continue;
-            const int tile = t / p.tile_size;
-            if ((unsigned)trow >= (unsigned)p.num_beams || tile >= p.num_tiles) continue;
-            const int page = __ldg(p.table + ((int64_t)trow * p.kv_heads + w.g) * p.num_tiles + tile);
-            if ((unsigned)page >= (unsigned)p.total_pages) continue;
-            const int64_t at = ((int64_t)page * p.tile_size + (t - tile * p.tile_size)) * D + lane;
-            float s = 0.f, v[NC];
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                s = fmaf(qf[c], tree_widen<T>(static_cast<const T*>(p.k)[at + 32 * c]), s);
-                v[c] = tree_widen<T>(static_cast<const T*>(p.v)[at + 32 * c]);
-            }
-            s = warp_sum(s) * fe;
-            const float mn = fmaxf(m, s);
-            const float f = m == mn ? 1.f : fast_exp2(m - mn), e = s == mn ? 1.f : fast_exp2(s - mn);
-            m = mn;
-            l = l * f + e;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) o[c] = fmaf(e, v[c], o[c] * f);
-        }
-        if (w.slot < 0) {
-            T* out = static_cast<T*>(p.out) + ((int64_t)r * p.heads + h) * D;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) out[lane + 32 * c] = tree_narrow<T>(o[c] / (l + 1e-6f));
-        } else {
-            float* dst = a.part + (w.slot * a.block + row_in_block + x) * (D + 4);
-#pragma unroll
-            for (int c = 0; c < NC; ++c) dst[lane + 32 * c] = o[c] * a.p_scale;
-            if (lane == 0) *reinterpret_cast<float4*>(dst + D) = make_float4(m, l * a.p_scale, m, 0.f);
-        }
-    }
-}
 
 template <int D, int NQ, bool BF>
 __global__ void __launch_bounds__(threads_for(NQ), NQ == 1 ? 2 : 1)
@@ -185,7 +93,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     tc_fence_after();
     uint32_t tmem_base;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
-    Walk w(a, pre);
+    TreeWalk w(a, pre);
     // Tiles go through the ring in the order of their products: K(0), K(1), V(0), K(2), V(1), ..., K(n - 1), V(n - 2), V(n - 1); the ring's
     // count `at` runs on through the pieces
     auto k_at = [&](uint32_t at, int i) { return at + (uint32_t)(i == 0 ? 0 : 2 * i - 1); };
@@ -196,60 +104,48 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     auto has_rows = [&](int x) { return w.rr0 + x * QT < w.sq.n * G; };
 
     if (warp == W_PROD) {
-        if (elect_one()) {
-            uint32_t c = 0, tiles = 0;              // requests and tiles of keys so far
-            if (w.f >= w.f_hi) a.notes[blockIdx.x] = TreeNote{};
-            bool ok = true;
-            auto request = [&](const CUtensorMap* map, const int (&r)[4]) {
-                const int s = (int)(c % RING);
-                wait(kv_empty(s), (c / RING & 1u) ^ 1u);
-                if (failed()) {
-                    ok = false;
-                    return;
-                }
+        uint32_t c = 0, tiles = 0;          // requests and tiles of keys so far
+        bool ok = true;
+        if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = TreeNote{};
+        auto request = [&](const CUtensorMap* map, const int (&r)[4]) {
+            const int s = (int)(c % RING);
+            wait(kv_empty(s), (c / RING & 1u) ^ 1u);
+            if (__any_sync(0xffffffffu, failed())) {
+                ok = false;
+                return;
+            }
+            if (elect_one()) {
                 const uint32_t st = kv_sm + s * TILE;
                 mbar_arrive_expect_tx(kv_full(s), TILE);
 #pragma unroll
                 for (int uu = 0; uu < 4; ++uu)
 #pragma unroll
-                    for (int kb = 0; kb < KB; ++kb) tma_load_2d(st + kb * 8192 + uu * 2048, map, kb * 64, r[uu], kv_full(s));
-                ++c;
-            };
-            while (ok && w.next()) {
-                if (w.f >= w.f_hi) a.notes[blockIdx.x] = tree_note(a, w.sq, w.g, w.rr0, w.i0, w.i1, w.f - w.i1, w.total, w.ns, w.slot);
-                const int row = p.beam_ids ? __ldg(p.beam_ids + w.b) : w.b;
-                const int32_t* trow = p.table + ((int64_t)row * p.kv_heads + w.g) * p.num_tiles;
-                const bool row_ok = (unsigned)row < (unsigned)p.num_beams;
-                int page[4], r[4], prev[4] = {0, 0, 0, 0};
-                auto load_pages = [&](int i) {
-#pragma unroll
-                    for (int uu = 0; uu < 4; ++uu) {
-                        const int t0 = (i * 4 + uu) * 16, t = t0 / p.tile_size;
-                        const int pg = row_ok && t0 < w.sq.keys && t < p.num_tiles ? __ldg(trow + t) : -1;
-                        page[uu] = (unsigned)pg < (unsigned)p.total_pages ? pg * p.tile_size + (t0 - t * p.tile_size) : -1;
-                    }
-                };
-                load_pages(w.i0);
-                for (int i = w.i0; i <= w.i1 && ok; ++i) {          // K(i) and V(i - 1)
-                    if (i < w.i1) {
-                        uint32_t mask = 0;
-#pragma unroll
-                        for (int uu = 0; uu < 4; ++uu) {
-                            r[uu] = page[uu] >= 0 ? page[uu] : a.total_rows;        // no page: zeros, and its scores are masked
-                            mask |= (page[uu] >= 0 ? 1u : 0u) << uu;
-                        }
-                        if (i + 1 < w.i1) load_pages(i + 1);
-                        asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(meta_sm + tiles++ % kNotes * 4), "r"(mask) : "memory");
-                        request(&tmK, r);
-                    }
-                    if (i > w.i0 && ok) request(&tmV, prev);
-#pragma unroll
-                    for (int uu = 0; uu < 4; ++uu) prev[uu] = r[uu];
-                }
+                    for (int kb = 0; kb < KB; ++kb)     // no page: zeros, and its scores are masked
+                        tma_load_2d(st + kb * 8192 + uu * 2048, map, kb * 64, r[uu] >= 0 ? r[uu] : a.total_rows, kv_full(s));
             }
-            if (failed())       // let the copies in flight land before the CTA's shared memory goes away
-                for (uint32_t i = c > RING ? c - RING : 0; i < c; ++i) tc_let_land(kv_full((int)(i % RING)), i / RING & 1u);
+            __syncwarp();
+            ++c;
+        };
+        TreePages pages(p);
+        while (ok && w.next()) {
+            if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = tree_note(a, w.sq, w.g, w.rr0, w.i0, w.i1, w.f - w.i1, w.total, w.ns, w.slot);
+            pages.open(w, 4);
+            int r[4] = {-1, -1, -1, -1}, prev[4] = {-1, -1, -1, -1};
+            for (int i = w.i0; i <= w.i1 && ok; ++i) {              // K(i) and V(i - 1)
+                if (i < w.i1) {
+                    const uint32_t mapped = pages.rows<4>((i - w.i0) * 4, r);
+                    if (lane == 0) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(meta_sm + tiles % kNotes * 4), "r"(mapped) : "memory");
+                    __syncwarp();
+                    ++tiles;
+                    request(&tmK, r);
+                }
+                if (i > w.i0 && ok) request(&tmV, prev);
+#pragma unroll
+                for (int uu = 0; uu < 4; ++uu) prev[uu] = r[uu];
+            }
         }
+        if (failed())           // let the copies in flight land before the CTA's shared memory goes away
+            for (uint32_t i = c > RING ? c - RING : 0; i < c; ++i) tc_let_land(kv_full((int)(i % RING)), i / RING & 1u);
     } else if (warp >= W_MMA) {
         constexpr uint32_t kIdescS = idesc_f16(QT, KT, 0, 0, BF), kIdescO = idesc_f16(QT, D, 0, 1, BF);
         const int x = warp - W_MMA;
@@ -346,21 +242,21 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 continue;
             }
             const int rr = w.rr0 + row_in_block + lane, rows = min(32, all - w.rr0 - row_in_block);       // rows of this warp, may be negative
-            const int node = rr < all ? rr / G : -1, head = w.g * G + rr % G;
+            const int div = rr / G, node = rr < all ? div : -1, head = w.g * G + rr - div * G;
             if (rows > 0) {
                 // the warp's query rows into the swizzled K-major A tile, whose last products this thread has seen complete
                 const uint32_t qx = base + x * Q_BYTES;
                 constexpr int CH = D / 8, PER = 8;      // 16-byte pieces of a row; loads in flight per lane
+                const int64_t own = node >= 0 ? (int64_t)(w.sq.r0 + node) * p.q_stride + (int64_t)head * D : 0;      // one division a row
 #pragma unroll 1
                 for (int c0 = 0; c0 < 32 * CH; c0 += 32 * PER) {
                     uint4 v[PER];
 #pragma unroll
                     for (int j = 0; j < PER; ++j) {
-                        const int idx = c0 + j * 32 + lane, r = idx / CH, c = idx % CH, q = w.rr0 + row_in_block + r;
+                        const int idx = c0 + j * 32 + lane, r = idx / CH, c = idx % CH;
+                        const int64_t from = __shfl_sync(0xffffffffu, own, r);
                         v[j] = make_uint4(0u, 0u, 0u, 0u);
-                        if (r < rows)
-                            v[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(w.sq.r0 + q / G) * p.q_stride +
-                                                                        (int64_t)(w.g * G + q % G) * D) + c);
+                        if (r < rows) v[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + from) + c);
                     }
 #pragma unroll
                     for (int j = 0; j < PER; ++j) {
@@ -502,7 +398,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 if (odd && qtr == 0 && lane == 0) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(odd_sm + 4 * x), "r"(0u) : "memory");
             }
             if (odd && !failed()) {
-                piece_by_rows<D, BF>(a, w, row_in_block, 32);
+                tree_piece_by_rows<D, T, T>(a, w, row_in_block, 32);
                 continue;
             }
             if (rows <= 0) continue;

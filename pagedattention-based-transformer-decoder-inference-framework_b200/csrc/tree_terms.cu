@@ -1,0 +1,705 @@
+// tree_terms.cu -- attention of drafted trees on the 5th-generation tensor cores with factors in several terms: float queries over half pages, and
+// int8 pages (tree_attention.cuh has the work list, tree_stream.cu the join).
+//
+// Keys are the rows of the products, query rows (and their terms) the columns: a tile is 128 keys whatever the number of query rows, and
+// staged keys and values are the A operands as they stand in their pages.
+//     S^T = K Q^T      [128 keys x terms R],   O^T = V^T P^T   [D x terms R],   R = 16, 32 or 64 query rows of a block
+//   half pages    two terms of half each for a query (its row scaled by a power of two first) and for a weight: 22 bits of every factor
+//   int8 pages    kind::i8 with three signed digits each: a query row as 23-bit integers relative to its largest, the weights times their
+//                 values' scales relative to the largest possible of a tile; products and their sums are exact integers, no byte is converted
+// The sums of a tile leave the tensor cores as they are and are added up in float registers (the tensor cores cut where float rounds: over a
+// long context that would add up).  A row's terms are neighbours in P^T, whose rows are keys: a thread stores four query rows at once.
+//   warps 0-7    softmax, one thread per key and half of the rows: its scores, one vote per tile whether a row's reference has to move (then
+//                the maxima by warp and through shared memory), weights to shared memory as the MN-major B operand
+//   warps 8-11   one thread per value column: the tile's sums into its R float sums, rescaled where a reference moved
+//   warp 12      issues  S^T of tile t + 1  and  O^T of tile t;  scores and sums are double-buffered in TMEM
+//   warp 13      TMA boxes of 16 keys into a ring (int8: and the rows' scales), page ids a tile ahead
+//   warps 14-15  the next piece's queries into the K-major B operand, their factors and masks
+#include "tcgen05_utils.cuh"
+#include "tree_pieces.cuh"
+
+namespace pa {
+namespace tterms {
+
+using namespace tc;
+
+constexpr int KT = 128, kSoftmax = 256, kThreads = 512, kNotes = 32;
+constexpr int W_SUMS = 8, W_MMA = 12, W_PROD = 13, W_LOAD = 14;
+constexpr float kDigits = 8.3e6f;       // the largest number of three signed digits, and some to spare
+
+__device__ int g_errors;
+
+// I8: int8 pages.  R: query rows of a block
+template <int D, bool I8, int R> struct Shape {
+    static constexpr int TERMS = I8 ? 3 : 2, N = TERMS * R;         // columns of the scores: term by term
+    static constexpr int NO = I8 ? 4 * R : 2 * R;                   // columns of the sums: row by row (int8: three digits and nothing)
+    static constexpr int TILE = KT * D * (I8 ? 1 : 2), SCALES = I8 ? KT * 8 : 0, SLOT = TILE + SCALES;     // of keys or values; both scales of a tile come with its values
+    static constexpr int Q_BYTES = N * 128 * (I8 ? 1 : D / 64), P_BYTES = KT * 128 * (R == 64 ? 2 : 1);
+    static constexpr int Q_BUFS = Q_BYTES > 16384 ? 1 : 2;
+    static constexpr int FREE = 200 * 1024 - Q_BUFS * Q_BYTES;
+    static constexpr int P_BUFS = (FREE - 2 * P_BYTES) / SLOT >= 4 ? 2 : 1;
+    static constexpr int RING = (FREE - P_BUFS * P_BYTES) / SLOT < 12 ? (FREE - P_BUFS * P_BYTES) / SLOT : 12;
+    static constexpr int COLS = 2 * N + 2 * NO, TMEM = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+    static constexpr int NBAR = 2 * RING + 16;      // full, empty [ring]; s_full, p_full, o_full, o_empty, q_ready, q_free [2]; piece_done [4]
+    static constexpr int FLOATS = 2 * R /*factors*/ + 2 * R /*references, thresholds*/ + 4 * R /*corrections*/ + 4 * R /*maxima*/ +
+                                  4 * 5 * R /*sums, references at the end*/ + R /*what the sums are multiplied by*/ + 2 * 8 * R /*rows*/ + 24;
+    static size_t smem(int seqs, int mask_words) {
+        return (size_t)RING * SLOT + Q_BUFS * Q_BYTES + P_BUFS * P_BYTES + NBAR * 8 + FLOATS * 4 + 2 * R * mask_words * 4 + kNotes * 4 + 64 + (seqs + 1) * 4 + 1024;
+    }
+};
+
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// kind::i8: c = S32 (2) [4,6), a and b signed (1) [7,10) [10,13), the rest as for kind::f16
+__host__ __device__ constexpr uint32_t idesc_i8(int M, int N, int a_mn_major, int b_mn_major) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn_major << 15) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(N >> 3) << 17) |
+           ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr));
+}
+template <int N> __device__ __forceinline__ void tmem_ldn(uint32_t taddr, uint32_t (&r)[N]) {
+    if constexpr (N == 8) tmem_ld8(taddr, r);
+    else tmem_ld16(taddr, r);
+}
+__device__ __forceinline__ uint32_t ordered(float f) {
+    const uint32_t u = __float_as_uint(f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+// three signed digits of x, the lowest in the lowest byte: x = d0 + 256 d1 + 65536 d2
+__device__ __forceinline__ uint32_t digits(int x) { return (uint32_t)(x + 0x808080) ^ 0x808080u; }
+// their sums of products: the upper one is below 2^22 (128 x 127 x 127), so that a float's mantissa holds it
+__device__ __forceinline__ float from_digits(uint32_t d0, uint32_t d1, uint32_t d2) {
+    const float hi = __uint_as_float(d2 + 0x4b400000u) - 12582912.f;
+    return fmaf(hi, 65536.f, (float)((int)d1 * 256 + (int)d0));
+}
+
+template <int D, bool I8, int R, typename Q>
+__global__ void __launch_bounds__(kThreads, 1) tree_terms_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeWork a) {
+    typedef Shape<D, I8, R> C;
+    constexpr int N = C::N, TERMS = C::TERMS, RING = C::RING, CB = I8 ? 1 : D / 64, RH = R / 2;       // CB: column blocks of a tile
+    constexpr float kRaise = I8 ? 1.f : 2.f, kShift = I8 ? 0.f : 10.f;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const TreeParams& p = a.p;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t q_sm = base + RING * C::TILE, p_sm = q_sm + C::Q_BUFS * C::Q_BYTES, sc_sm = p_sm + C::P_BUFS * C::P_BYTES, bar0 = sc_sm + RING * C::SCALES;
+    auto kv_full = [&](int s) { return bar0 + s * 8; };
+    auto kv_empty = [&](int s) { return bar0 + (RING + s) * 8; };
+    auto s_full = [&](int i) { return bar0 + (2 * RING + i) * 8; };
+    auto p_full = [&](int i) { return bar0 + (2 * RING + 2 + i) * 8; };
+    auto o_full = [&](int i) { return bar0 + (2 * RING + 4 + i) * 8; };
+    auto o_empty = [&](int i) { return bar0 + (2 * RING + 6 + i) * 8; };
+    auto q_ready = [&](uint32_t piece) { return bar0 + (2 * RING + 8 + piece % C::Q_BUFS) * 8; };
+    auto q_free = [&](uint32_t piece) { return bar0 + (2 * RING + 10 + piece % C::Q_BUFS) * 8; };
+    auto q_phase = [&](uint32_t piece) { return piece / C::Q_BUFS & 1u; };
+    auto piece_done = [&](uint32_t piece) { return bar0 + (2 * RING + 12 + (piece & 3)) * 8; };
+    const uint32_t tmem_slot = bar0 + C::NBAR * 8, fail_sm = tmem_slot + 8, meta_sm = fail_sm + 8;
+    // factors of the scores [2 pieces], references (less kShift) and what a score may exceed them by, corrections of the last four tiles, maxima
+    // by warp, sums by warp and references of the last four pieces, what a piece's sums are multiplied by; nodes and heads of the last eight
+    // pieces' rows (node -1: no row); scales of the last four tiles, largest scale by warp of the last two;
+    // whether references moved in the last four tiles, whether the last four pieces are computed by rows
+    float* fl = reinterpret_cast<float*>(smem_raw + (meta_sm + kNotes * 4 - smem_u32(smem_raw)));
+    float *s_fe = fl, *s_ref = fl + 2 * R, *s_thr = fl + 3 * R, *s_corr = fl + 4 * R, *s_max = fl + 8 * R, *s_end = fl + 12 * R, *s_inv = fl + 32 * R, *s_scale = fl + 49 * R,
+          *s_big = s_scale + 4;
+    int *s_node = reinterpret_cast<int*>(fl + 33 * R), *s_head = s_node + 8 * R;         // (seven pieces at most are on their way)
+    int *s_moved = reinterpret_cast<int*>(s_big + 8), *s_odd = s_moved + 4, *pre = s_odd + 4;
+    uint32_t* s_mask = reinterpret_cast<uint32_t*>(pre + p.num_seqs + 1);      // [2 pieces][R][mask_words]
+    auto failed = [&] { return tc_failed(fail_sm); };
+    auto wait = [&](uint32_t bar, uint32_t parity) { tc_wait(bar, parity, fail_sm, a.polls); };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.heads / p.kv_heads;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < RING; ++s) {
+            mbar_init(kv_full(s), I8 ? 33 : 1);     // int8: a warp's copies of scales, too
+            mbar_init(kv_empty(s), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full(i), 1);
+            mbar_init(p_full(i), kSoftmax);
+            mbar_init(o_full(i), 1);
+            mbar_init(o_empty(i), 128);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(q_ready(i), 64);
+            mbar_init(q_free(i), 1 + kSoftmax / 32);
+        }
+        for (uint32_t i = 0; i < 4; ++i) mbar_init(piece_done(i), kSoftmax / 32);
+        asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(fail_sm), "r"(0u) : "memory");
+        mbar_fence_init();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmK));
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmV));
+    }
+    if (warp == W_MMA) tmem_alloc(tmem_slot, C::TMEM);
+    shares::count_units(pre, p.num_seqs, [&](int b) { return tree_seq(p, b, a.block, a.unit).units(); });
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem_base;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
+    // columns of TMEM: scores [2][N], sums [2][NO]
+    auto s_col = [&](int i) { return tmem_base + i * N; };
+    auto o_col = [&](int i) { return tmem_base + 2 * N + i * C::NO; };
+    TreeWalk w(a, pre);
+    // Tiles go through the ring in the order of their products: K(0), K(1), V(0), K(2), V(1), ..., K(n - 1), V(n - 2), V(n - 1); the ring's
+    // count `at` runs on through the pieces, as do the tiles' parities
+    auto k_at = [&](uint32_t at, int i) { return at + (uint32_t)(i == 0 ? 0 : 2 * i - 1); };
+    auto v_at = [&](uint32_t at, int i, int nt) { return at + (uint32_t)(i + 1 < nt ? 2 * i + 2 : 2 * nt - 1); };
+    auto slot_of = [&](uint32_t c) { return (int)(c % RING); };
+    auto phase_of = [&](uint32_t c) { return c / RING & 1u; };
+    uint32_t at = 0, n = 0, pieces = 0;     // requests to the ring, tiles, pieces so far
+
+    if (warp == W_PROD) {
+        uint32_t c = 0, tiles = 0;          // requests and tiles of keys so far
+        bool ok = true;
+        if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = TreeNote{};
+        auto request = [&](const CUtensorMap* map, bool scales, const int (&r)[8]) {
+            const int s = (int)(c % RING);
+            wait(kv_empty(s), (c / RING & 1u) ^ 1u);
+            if (__any_sync(0xffffffffu, failed())) {
+                ok = false;
+                return;
+            }
+            if (elect_one()) {
+                const uint32_t st = base + s * C::TILE;
+                mbar_arrive_expect_tx(kv_full(s), C::TILE);
+#pragma unroll
+                for (int uu = 0; uu < 8; ++uu)
+#pragma unroll
+                    for (int cb = 0; cb < CB; ++cb)     // no page: zeros, and its scores are masked
+                        tma_load_2d(st + cb * 16384 + uu * (I8 ? 16 * D : 2048), map, cb * 64, r[uu] >= 0 ? r[uu] : a.total_rows, kv_full(s));
+            }
+            __syncwarp();
+            if (I8 && scales) {                         // a lane: 16 bytes of a unit's 64, of keys and of values
+                int row = -1;
+#pragma unroll
+                for (int uu = 0; uu < 8; ++uu) row = lane >> 2 == uu ? r[uu] : row;
+                if (row >= 0) {
+                    const uint32_t to = sc_sm + s * C::SCALES + lane * 16;
+                    cp_async_16(to, p.k_scales + row + (lane & 3) * 4, true);
+                    cp_async_16(to + 512, p.v_scales + row + (lane & 3) * 4, true);
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(kv_full(s)) : "memory");
+            } else if (I8) {
+                mbar_arrive(kv_full(s));
+            }
+            ++c;
+        };
+        TreePages pages(p);
+        while (ok && w.next()) {
+            if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = tree_note(a, w.sq, w.g, w.rr0, w.i0, w.i1, w.f - w.i1, w.total, w.ns, w.slot);
+            pages.open(w, 8);
+            int r[8], prev[8];
+#pragma unroll
+            for (int uu = 0; uu < 8; ++uu) r[uu] = prev[uu] = -1;
+            for (int i = w.i0; i <= w.i1 && ok; ++i) {              // K(i) and V(i - 1)
+                if (i < w.i1) {
+                    const uint32_t mapped = pages.rows<8>((i - w.i0) * 8, r);
+                    if (lane == 0) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(meta_sm + tiles % kNotes * 4), "r"(mapped) : "memory");
+                    __syncwarp();
+                    ++tiles;
+                    request(&tmK, false, r);
+                }
+                if (i > w.i0 && ok) request(&tmV, true, prev);
+#pragma unroll
+                for (int uu = 0; uu < 8; ++uu) prev[uu] = r[uu];
+            }
+        }
+        if (failed())           // let the copies in flight land before the CTA's shared memory goes away
+            for (uint32_t i = c > RING ? c - RING : 0; i < c; ++i) tc_let_land(kv_full((int)(i % RING)), i / RING & 1u);
+    } else if (warp == W_MMA) {
+        constexpr uint32_t kIdescS = I8 ? idesc_i8(128, N, 0, 0) : idesc_f16(128, N, 0, 0, 0);
+        constexpr uint32_t kIdescO = I8 ? idesc_i8(128, C::NO, 1, 1) : idesc_f16(128, C::NO, 1, 1, 0);
+        while (w.next()) {
+            const int nt = w.i1 - w.i0;
+            auto issue_S = [&](int i) {
+                const int s = slot_of(k_at(at, i)), sb = (int)(n + i) & 1;
+                wait(kv_full(s), phase_of(k_at(at, i)));
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t st = base + s * C::TILE, qb = q_sm + pieces % C::Q_BUFS * C::Q_BYTES;
+                    if constexpr (I8) {
+#pragma unroll
+                        for (int ks = 0; ks < D / 32; ++ks)
+                            umma_i8(s_col(sb), make_desc(st + ks * 32, 16, 1024), make_desc(qb + ks * 32, 16, 1024), kIdescS, ks > 0 ? 1u : 0u);
+                    } else {
+#pragma unroll
+                        for (int ks = 0; ks < D / 16; ++ks)
+                            umma_f16(s_col(sb), make_desc(st + (ks >> 2) * 16384 + (ks & 3) * 32, 16, 1024),
+                                     make_desc(qb + (ks >> 2) * (N * 128) + (ks & 3) * 32, 16, 1024), kIdescS, ks > 0 ? 1u : 0u);
+                    }
+                    umma_commit(s_full(sb));
+                    umma_commit(kv_empty(s));
+                    if (i + 1 == nt) umma_commit(q_free(pieces));
+                }
+                __syncwarp();
+            };
+            wait(q_ready(pieces), q_phase(pieces));
+            issue_S(0);
+            for (int i = 0; i < nt; ++i) {
+                if (i + 1 < nt) issue_S(i + 1);
+                const uint32_t t = n + i;
+                const int s = slot_of(v_at(at, i, nt)), sb = (int)t & 1, nvalid = min(KT, w.sq.keys - (w.i0 + i) * KT);
+                const uint32_t st = base + s * C::TILE;
+                wait(kv_full(s), phase_of(v_at(at, i, nt)));
+                if (!I8 && (nvalid & 15)) {         // value rows past the last key may hold anything (0 x NaN = NaN): zeros
+                    const int r1 = (nvalid + 15) & ~15;
+                    for (int idx = lane; idx < (r1 - nvalid) * (D / 8); idx += 32) {
+                        const int r = nvalid + idx / (D / 8), c = idx % (D / 8);
+                        const uint32_t addr = st + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(addr), "r"(0u) : "memory");
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                wait(p_full(sb), t >> 1 & 1u);
+                wait(o_empty(sb), (t >> 1 & 1u) ^ 1u);          // the sums of tile t - 2 are taken
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t pb = p_sm + (C::P_BUFS == 2 ? sb : 0) * C::P_BYTES;
+                    if constexpr (I8) {
+                        const int ksteps = (nvalid + 31) >> 5;
+                        for (int ks = 0; ks < ksteps; ++ks)
+                            umma_i8(o_col(sb), make_desc(st + ks * 32 * 128, 16, 1024), make_desc(pb + ks * 32 * 128, 16, 1024), kIdescO, ks > 0 ? 1u : 0u);
+                    } else {
+                        const int ksteps = (nvalid + 15) >> 4;
+                        for (int ks = 0; ks < ksteps; ++ks)     // 64 value columns twice where there are no more
+                            umma_f16(o_col(sb), make_desc(st + ks * 2048, D == 128 ? 16384 : 0, 1024),
+                                     make_desc(pb + ks * 2048, 16384, 1024), kIdescO, ks > 0 ? 1u : 0u);
+                    }
+                    umma_commit(o_full(sb));
+                    umma_commit(kv_empty(s));
+                }
+                __syncwarp();
+            }
+            at += 2 * nt;
+            n += nt;
+            ++pieces;
+        }
+    } else if (warp >= W_LOAD) {
+        // ---- queries: a warp per row, eight rows at a time
+        constexpr int PER = D / 32;         // columns of a lane
+        const float f0 = 1.4426950408889634f / p.temperature;
+        const int c0 = lane * PER;
+        while (w.next()) {
+            const int all = w.sq.n * G, buf = (int)(pieces % C::Q_BUFS);
+            const uint32_t qb = q_sm + buf * C::Q_BYTES;
+            wait(q_free(pieces), q_phase(pieces) ^ 1u);
+            int *nodes = s_node + (pieces & 7) * R, *heads = s_head + (pieces & 7) * R;
+            const int mine = threadIdx.x - W_LOAD * 32;
+            if (mine < R) {                 // one division a row, for everyone
+                const int rr = w.rr0 + mine, node = rr / G;
+                nodes[mine] = rr < all ? w.sq.r0 + node : -1;
+                heads[mine] = w.g * G + rr - node * G;
+            }
+            asm volatile("bar.sync 2, 64;" ::: "memory");
+#pragma unroll 1
+            for (int r0 = (warp - W_LOAD) * 8; r0 < R; r0 += 16) {
+                float x[8][PER], big[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int node = nodes[r0 + k];
+                    const Q* q = static_cast<const Q*>(p.q) + (node >= 0 ? (int64_t)node * p.q_stride + (int64_t)heads[r0 + k] * D : 0) + c0;
+#pragma unroll
+                    for (int c = 0; c < PER; ++c) x[k][c] = node >= 0 ? tree_widen<Q>(q[c]) : 0.f;
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    big[k] = 0.f;
+#pragma unroll
+                    for (int c = 0; c < PER; ++c) big[k] = fmaxf(big[k], fabsf(x[k][c]));
+                    big[k] = warp_max(big[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int r = r0 + k;
+                    if constexpr (I8) {
+                        // a row with numbers that are not finite: its scores are not, through their factor
+                        const float up = big[k] > 0.f && big[k] < INFINITY ? kDigits / big[k] : 0.f;
+                        uint32_t word[3] = {0u, 0u, 0u};
+                        bool odd = false;
+#pragma unroll
+                        for (int c = 0; c < PER; ++c) {
+                            odd |= !(fabsf(x[k][c]) < INFINITY);
+                            const uint32_t d = digits(odd ? 0 : __float2int_rn(x[k][c] * up));
+#pragma unroll
+                            for (int t = 0; t < 3; ++t) word[t] |= (d >> 8 * t & 255u) << 8 * c;
+                        }
+#pragma unroll
+                        for (int t = 0; t < 3; ++t) {
+                            const int row = t * R + r;
+                            const uint32_t addr = qb + row * 128 + (((c0 >> 4) ^ (row & 7)) << 4) + (c0 & 15);
+                            if (PER == 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(word[t]) : "memory");
+                            else asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"((uint16_t)word[t]) : "memory");
+                        }
+                        odd = __any_sync(0xffffffffu, odd);
+                        if (lane == 0) s_fe[buf * R + r] = odd ? __int_as_float(0x7fc00000) : f0 * (big[k] / kDigits);
+                    } else {
+                        // the row's largest between 2^10 and 2^11: halves hold hi, and lo down to 2^-35 of it
+                        const int e = big[k] > 0.f && big[k] < INFINITY ? max(-100, min(100, 10 - ilogbf(big[k]))) : 0;
+                        const float up = exp2f((float)e);
+#pragma unroll
+                        for (int c = 0; c < PER; c += 2) {
+                            const uint32_t hi = pack_half2(x[k][c] * up, x[k][c + 1] * up);
+                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                            const uint32_t v[2] = {hi, pack_half2(x[k][c] * up - back.x, x[k][c + 1] * up - back.y)};
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+                                const int row = t * R + r, col = c0 + c;
+                                const uint32_t addr = qb + (col >> 6) * (N * 128) + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2;
+                                asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v[t]) : "memory");
+                            }
+                        }
+                        if (lane == 0) s_fe[buf * R + r] = f0 * exp2f((float)-e);
+                    }
+                }
+            }
+            if (mine < R)
+                for (int x = 0; x < p.mask_words; ++x)
+                    s_mask[(buf * R + mine) * p.mask_words + x] = nodes[mine] >= 0 ? __ldg(p.mask + (int64_t)nodes[mine] * p.mask_words + x) : 0u;
+            fence_proxy_async();
+            mbar_arrive_cnt(q_ready(pieces));
+            ++pieces;
+        }
+    } else if (warp < W_SUMS) {
+        // ---- softmax: one thread per key and half of the rows
+        const int kk = threadIdx.x & 127, quarter = warp & 3, h0 = (warp >> 2) * RH;
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        auto group_sync = [&] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        auto group_any = [&](bool x) {
+            int any;
+            asm volatile(
+                "{\n\t.reg .pred p, q;\n\t"
+                "setp.ne.b32 p, %1, 0;\n\t"
+                "barrier.cta.red.or.pred q, 1, 256, p;\n\t"
+                "selp.b32 %0, 1, 0, q;\n\t}"
+                : "=r"(any) : "r"((int)x) : "memory");
+            return any != 0;
+        };
+        auto four = [&](const float* f) { return *reinterpret_cast<const float4*>(f); };
+        auto fresh = [&] {                  // no reference yet: any score sets one
+            if (threadIdx.x < R) {
+                s_ref[threadIdx.x] = 0.f;
+                s_thr[threadIdx.x] = -3e38f;
+            }
+        };
+        fresh();
+        while (w.next()) {
+            const int nt = w.i1 - w.i0, buf = (int)(pieces % C::Q_BUFS);
+            wait(q_ready(pieces), q_phase(pieces));
+            group_sync();                   // fresh references
+            const float* fes = s_fe + buf * R + h0;
+            float l[RH];
+#pragma unroll
+            for (int r = 0; r < RH; ++r) l[r] = 0.f;
+            bool odd = false;
+#pragma unroll 1
+            for (int i = 0; i < nt; ++i) {
+                const uint32_t t = n + i;
+                const int sb = (int)t & 1, ring4 = (int)t & 3, kp = (w.i0 + i) * KT + kk;
+                const bool drafts = (w.i0 + i + 1) * KT > w.sq.ctx;
+                wait(s_full(sb), t >> 1 & 1u);
+                tc_fence_after();
+                uint32_t mapped;            // the producer's note about this tile, older than the scores
+                asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(mapped) : "r"(meta_sm + t % kNotes * 4) : "memory");
+                const bool here = kp < w.sq.keys && (mapped >> (kk >> 4) & 1u);
+                float ksc = 1.f, vsc = 0.f;
+                if (I8) {
+                    const uint32_t c = v_at(at, i, nt), sc = sc_sm + slot_of(c) * C::SCALES + kk * 4;
+                    wait(kv_full(slot_of(c)), phase_of(c));
+                    float ks, vs;
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(ks) : "r"(sc) : "memory");
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vs) : "r"(sc + 512) : "memory");
+                    ksc = here ? __frcp_rn(ks) : 1.f;
+                    vsc = here ? __frcp_rn(vs) : 0.f;
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, ordered(vsc));
+                    if (lane == 0) s_big[sb * 4 + quarter] = unordered(top);       // both halves the same
+                } else if (drafts) {        // values that are not finite (rows past the last key: zeros, or looked at in vain)
+                    const uint32_t c = v_at(at, i, nt);
+                    wait(kv_full(slot_of(c)), phase_of(c));
+                    if (kp < w.sq.keys && h0 == 0) {
+                        const uint32_t vt = base + slot_of(c) * C::TILE + kk * 128;
+#pragma unroll
+                        for (int x = 0; x < D / 8; ++x) {
+                            const uint4 v = lds_128(vt + (x >> 3) * 16384 + ((x & 7) << 4));
+                            const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) odd |= (q[e] & 0x7c00u) == 0x7c00u || (q[e] >> 16 & 0x7c00u) == 0x7c00u;
+                        }
+                    }
+                }
+                // ---- scores, less their references; does one exceed its threshold?
+                constexpr int CH = RH < 16 ? RH : 16;
+                const int bit = kp - w.sq.ctx;              // of the rows' masks, where it is not negative
+                const bool masked = drafts && here && bit >= 0, hidden = !here || (masked && (bit >> 5) >= p.mask_words);
+                float s[RH];
+                bool over = false;
+#pragma unroll
+                for (int c = 0; c < RH / CH; ++c) {
+                    uint32_t x[TERMS][CH];
+#pragma unroll
+                    for (int term = 0; term < TERMS; ++term) tmem_ldn<CH>(s_col(sb) + lane_base + term * R + h0 + c * CH, x[term]);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < CH; j += 4) {
+                        const int r = c * CH + j;
+                        const float4 fe = four(fes + r), ref = four(s_ref + h0 + r), thr = four(s_thr + h0 + r);
+                        const float f[4] = {fe.x, fe.y, fe.z, fe.w}, o[4] = {ref.x, ref.y, ref.z, ref.w}, h[4] = {thr.x, thr.y, thr.z, thr.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float v;
+                            if constexpr (I8) v = fmaf(from_digits(x[0][j + e], x[1][j + e], x[TERMS - 1][j + e]), f[e] * ksc, -o[e]);
+                            else v = fmaf(__uint_as_float(x[0][j + e]) + __uint_as_float(x[1][j + e]), f[e], -o[e]);
+                            s[r + e] = hidden ? -INFINITY : v;
+                            over |= s[r + e] > h[e];
+                        }
+                    }
+                }
+                if (drafts) {
+                    const uint32_t* mw = s_mask + (buf * R + h0) * p.mask_words + (masked && !hidden ? bit >> 5 : 0);
+                    over = false;
+#pragma unroll
+                    for (int r = 0; r < RH; ++r) {
+                        if (masked && !(mw[r * p.mask_words] >> (bit & 31) & 1u)) s[r] = -INFINITY;
+                        over |= s[r] > s_thr[h0 + r];
+                    }
+                }
+                const bool any = group_any(over);
+                if (any) {
+#pragma unroll
+                    for (int r = 0; r < RH; ++r) {
+                        const uint32_t top = __reduce_max_sync(0xffffffffu, ordered(s[r] == s[r] ? s[r] : -INFINITY));
+                        if (lane == 0) s_max[quarter * R + h0 + r] = unordered(top);
+                    }
+                    group_sync();
+                    if (threadIdx.x < R) {
+                        const int r = threadIdx.x;
+                        const float top = fmaxf(fmaxf(s_max[r], s_max[R + r]), fmaxf(s_max[2 * R + r], s_max[3 * R + r]));
+                        const bool raise = top > s_thr[r];
+                        const float by = raise ? top - kShift : 0.f;
+                        // a first reference has no sums to correct
+                        s_corr[ring4 * R + r] = s_thr[r] < -1e38f ? 1.f : exp2f(-by);
+                        s_max[r] = by;
+                        s_ref[r] += by;
+                        if (raise) s_thr[r] = kRaise + kShift;
+                    }
+                    group_sync();
+#pragma unroll
+                    for (int r = 0; r < RH; ++r) {
+                        l[r] *= s_corr[ring4 * R + h0 + r];
+                        s[r] -= s_max[h0 + r];
+                    }
+                }
+                float unit = 0.f;           // int8: weights per value scale, as integers
+                if (I8) {
+                    const float4 b4 = four(s_big + sb * 4);
+                    const float big = fmaxf(fmaxf(b4.x, b4.y), fmaxf(b4.z, b4.w));
+                    unit = big > 0.f ? vsc / big * (kDigits / 2.f) : 0.f;
+                    if (threadIdx.x == 0) s_scale[ring4] = big * (2.f / kDigits);
+                }
+                if (threadIdx.x == 0) s_moved[ring4] = any;
+                // ---- weights: four rows' terms a 16-byte word
+                const uint32_t pb = p_sm + (uint32_t)((C::P_BUFS == 2 ? sb : 0) * C::P_BYTES) + kk * 128;
+                if (C::P_BUFS == 1 && t > 0) wait(o_full((t - 1) & 1), (t - 1) >> 1 & 1u);      // their place is read
+#pragma unroll
+                for (int r = 0; r < RH; r += 4) {
+                    float e[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        e[k] = fast_exp2(s[r + k]);
+                        l[r + k] += e[k];
+                    }
+                    uint32_t v[4];
+                    if constexpr (I8) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)         // a float between 2^23 and 2^24 holds the integer in its mantissa
+                            v[k] = (__float_as_uint(fmaf(e[k], unit, 8388608.f)) + (0x808080u - 0x4b000000u)) ^ 0x808080u;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            v[2 * k] = pack_half2(e[2 * k], e[2 * k + 1]);
+                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&v[2 * k]));
+                            v[2 * k + 1] = pack_half2(e[2 * k] - back.x, e[2 * k + 1] - back.y);
+                        }
+                    }
+                    const int c = (h0 + r) >> 2;
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(pb + (c >> 3) * 16384 + (((c & 7) ^ (kk & 7)) << 4)), "r"(v[0]), "r"(v[1]),
+                                 "r"(v[2]), "r"(v[3]) : "memory");
+                }
+                fence_proxy_async();
+                tc_fence_before();
+                mbar_arrive_cnt(p_full(sb));
+            }
+            n += nt;
+            at += 2 * nt;
+            // ---- the piece's end: sums over the warps' keys, references, whether it has to be computed by rows
+            odd = group_any(odd);           // everyone is through with the references, too
+            float* end = s_end + (pieces & 3) * 5 * R;
+#pragma unroll
+            for (int r = 0; r < RH; ++r) {
+                const float sum = warp_sum(l[r]);
+                if (lane == 0) end[quarter * R + h0 + r] = sum;
+            }
+            if (threadIdx.x < R) end[4 * R + threadIdx.x] = s_thr[threadIdx.x] < -1e38f ? -INFINITY : s_ref[threadIdx.x] + kShift;
+            if (threadIdx.x == 0) s_odd[pieces & 3] = odd;
+            fresh();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive_cnt(piece_done(pieces));
+                mbar_arrive_cnt(q_free(pieces));
+            }
+            if (!I8 && odd && !failed()) tree_piece_by_rows<D, Q, __half>(a, w, warp * (R / 8), R / 8);
+            ++pieces;
+        }
+    } else {
+        // ---- sums: one thread per value column (64 columns: the upper half of the threads has them a second time)
+        const int d = threadIdx.x - kSoftmax;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        while (w.next()) {
+            const int nt = w.i1 - w.i0;
+            float o[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) o[r] = 0.f;
+#pragma unroll 1
+            for (int i = 0; i < nt; ++i) {
+                const uint32_t t = n + i;
+                const int sb = (int)t & 1, ring4 = (int)t & 3;
+                wait(o_full(sb), t >> 1 & 1u);
+                tc_fence_after();
+                if (s_moved[ring4])
+#pragma unroll
+                    for (int r = 0; r < R; ++r) o[r] *= s_corr[ring4 * R + r];
+                const float unit = I8 ? s_scale[ring4] : 1.f;
+#pragma unroll
+                for (int c = 0; c < C::NO / 32; ++c) {
+                    uint32_t x[32];
+                    tmem_ld32(o_col(sb) + lane_base + c * 32, x);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        if constexpr (I8) {                 // a row's digits, and nothing
+                            const int r = c * 8 + j / 4;
+                            o[r] = fmaf(from_digits(x[j], x[j + 1], x[j + 2]), unit, o[r]);
+                        } else {                            // two rows' large terms, and their small ones
+                            const int r = c * 16 + j / 2;
+                            o[r] += __uint_as_float(x[j]) + __uint_as_float(x[j + 2]);
+                            o[r + 1] += __uint_as_float(x[j + 1]) + __uint_as_float(x[j + 3]);
+                        }
+                    }
+                }
+                tc_fence_before();
+                mbar_arrive_cnt(o_empty(sb));
+            }
+            n += nt;
+            wait(piece_done(pieces), pieces >> 2 & 1u);
+            const float* end = s_end + (pieces & 3) * 5 * R;
+            const bool skip = !I8 && s_odd[pieces & 3];
+            ++pieces;
+            const int* nodes = s_node + ((pieces - 1) & 7) * R;
+            const int* heads = s_head + ((pieces - 1) & 7) * R;
+            constexpr float scale = I8 ? 1.f : 1.f / 1024.f;    // 2^-kShift
+            const float bad = failed() ? __int_as_float(0x7fc00000) : 0.f;
+            if (d < R) {
+                const float sum = (end[d] + end[R + d] + end[2 * R + d] + end[3 * R + d]) * scale, ref = end[4 * R + d];
+                s_inv[d] = (w.slot < 0 ? scale / (sum + 1e-6f) : scale * a.p_scale) + bad;
+                if (w.slot >= 0 && !skip && nodes[d] >= 0)
+                    *reinterpret_cast<float4*>(a.part + (w.slot * a.block + d) * (D + 4) + D) = make_float4(ref + bad, sum * a.p_scale + bad, ref, 0.f);
+            }
+            asm volatile("bar.sync 3, 128;" ::: "memory");
+            if (!skip && d < D) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float x = o[r] * s_inv[r];
+                    if (nodes[r] < 0) continue;
+                    if (w.slot < 0) static_cast<Q*>(p.out)[((int64_t)nodes[r] * p.heads + heads[r]) * D + d] = tree_narrow<Q>(x);
+                    else a.part[(w.slot * a.block + r) * (D + 4) + d] = x;
+                }
+            }
+            asm volatile("bar.sync 3, 128;" ::: "memory");      // s_inv is read
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == W_MMA) {
+        tc_fence_after();
+        if (failed()) {
+            __nanosleep(1000000);       // products in flight write TMEM for microseconds at most
+            if (lane == 0) atomicAdd(&g_errors, 1);
+        }
+        tmem_dealloc(tmem_base, C::TMEM);
+    }
+}
+
+// [rows][D] bytes, boxes of 16 rows, SWIZZLE_128B
+static bool make_byte_map(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t cols) {
+    EncodeTiledFnG fn = encode_fn_g();
+    if (!fn || rows == 0) return false;
+    cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols};
+    cuuint32_t box[2] = {(cuuint32_t)cols, 16}, estr[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool I8, int R, typename Q>
+static int launch(const TreeWork& a, cudaStream_t st) {
+    const TreeParams& p = a.p;
+    typedef Shape<D, I8, R> C;
+    static_assert(C::COLS <= 512 && C::RING >= 4, "TMEM or shared memory");
+    const size_t smem = C::smem(p.num_seqs, p.mask_words);
+    if (smem > (size_t)device_info().max_smem_optin) return PA_ERR_UNSUPPORTED;
+    auto kern = tree_terms_kernel<D, I8, R, Q>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    CUtensorMap k, v;
+    const bool ok = I8 ? make_byte_map(&k, p.k, a.total_rows, D) && make_byte_map(&v, p.v, a.total_rows, D)
+                       : make_bf16_map(&k, p.k, a.total_rows, D, D, 16) && make_bf16_map(&v, p.v, a.total_rows, D, D, 16);     // boxes move bits
+    if (!ok) return PA_ERR_UNSUPPORTED;
+    kern<<<a.workers, kThreads, smem, st>>>(k, v, a);
+    PA_RETURN_LAUNCH_STATUS();
+}
+
+}  // namespace tterms
+
+int tree_terms_workers() { return device_info().sm_count; }
+
+// Rows of a block, 0 where this kernel does not serve or the streaming one is faster
+int tree_terms_block(const TreeParams& p) {
+    const int G = p.heads / p.kv_heads, rows = p.most * G;
+    const bool half = p.q_type == PA_TYPE_F32 && p.kv_type == PA_TYPE_F16, bytes = p.kv_type == PA_TYPE_I8 && p.dim == 128;
+    if ((!half && !bytes) || (p.dim != 64 && p.dim != 128) || p.tile_size % 16 || p.num_seqs > kTreeMostSeqs) return 0;
+    if ((int64_t)p.total_pages * p.tile_size >= 0x7fffff00ll || ((uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.k_scales | (uintptr_t)p.v_scales) % 16) return 0;
+    if (half && rows <= 16) return 0;
+    const int block = bytes ? (rows <= 16 ? 16 : 32) : rows <= 32 ? 32 : 64;
+    const int64_t steps = ((int64_t)p.num_tiles * p.tile_size + tterms::KT - 1) / tterms::KT;
+    return ((int64_t)p.rows * G / block + p.num_seqs) * steps < 0x7fffffff ? block : 0;     // the list's sums are 32 bits
+}
+
+int tree_terms_launch(const TreeWork& a, cudaStream_t st) {
+    using namespace tterms;
+    const TreeParams& p = a.p;
+    if (p.kv_type == PA_TYPE_I8) {
+        if (p.q_type == PA_TYPE_F32) return a.block == 16 ? launch<128, true, 16, float>(a, st) : launch<128, true, 32, float>(a, st);
+        return a.block == 16 ? launch<128, true, 16, __half>(a, st) : launch<128, true, 32, __half>(a, st);
+    }
+    if (p.dim == 64) return a.block == 32 ? launch<64, false, 32, float>(a, st) : launch<64, false, 64, float>(a, st);
+    return a.block == 32 ? launch<128, false, 32, float>(a, st) : launch<128, false, 64, float>(a, st);
+}
+
+int tree_terms_errors(int* host_count) { return (int)cudaMemcpyFromSymbol(host_count, tterms::g_errors, sizeof(int)); }
+
+}  // namespace pa
