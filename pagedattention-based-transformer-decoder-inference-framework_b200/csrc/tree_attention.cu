@@ -100,7 +100,7 @@ PA_API size_t pa_tree_attention_workspace_bytes(int rows, int num_seqs, int most
     // whichever kernel serves: it goes by the types too
     size_t most = 0;
     for (int block : {16, 32, 64, 128, 256}) {
-        const size_t n = tree_work_bytes(num_seqs, block <= 32 ? tree_stream_workers() : block == 64 ? tree_terms_workers() : tree_tc_workers(block), block, head_dim);
+        const size_t n = tree_work_bytes(num_seqs, block <= 32 ? tree_stream_workers() : block == 64 ? tree_terms_workers(block) : tree_tc_workers(block), block, head_dim);
         if (n > most) most = n;
     }
     return most;
@@ -129,7 +129,10 @@ PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void
     };
     Form f{tree_tc_block(p), 0, 64, tree_tc_launch};
     f.workers = tree_tc_workers(f.block);
-    if (!f.block) f = Form{tree_terms_block(p), tree_terms_workers(), 128, tree_terms_launch};
+    if (!f.block) {
+        f = Form{tree_terms_block(p), 0, 128, tree_terms_launch};
+        f.workers = tree_terms_workers(f.block);
+    }
     if (!f.block) f = Form{tree_stream_block(p), tree_stream_workers(), 16, tree_stream_launch};
     if (f.block) {
         if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < tree_work_bytes(num_seqs, f.workers, f.block, head_dim)) return PA_ERR_WORKSPACE;

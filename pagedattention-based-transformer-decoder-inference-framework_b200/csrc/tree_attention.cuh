@@ -121,7 +121,7 @@ int tree_tc_workers(int block);
 int tree_tc_block(const TreeParams& p);
 int tree_tc_launch(const TreeWork& w, cudaStream_t st);
 // tree_terms.cu: float queries over half pages, int8 pages
-int tree_terms_workers();
+int tree_terms_workers(int block);
 int tree_terms_block(const TreeParams& p);
 int tree_terms_launch(const TreeWork& w, cudaStream_t st);
 

@@ -13,6 +13,7 @@
 //
 // A value that is not finite in a drafted row does not reach the rows that do not see it: a unit of drafted keys with such values takes
 // them out of the product and adds them for the rows that see them.
+#include "f32x2.cuh"
 #include "mma_utils.cuh"
 #include "tcgen05_utils.cuh"
 #include "tree_attention.cuh"
@@ -32,6 +33,21 @@ template <bool BF>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (BF) mma_bf16_16816(d, a, b0, b1);
     else mma_16816_full(d, a[0], a[1], a[2], a[3], b0, b1);
+}
+// the product alone: d = a b
+template <bool BF>
+__device__ __forceinline__ void mma_from_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// to += x, two at a time
+__device__ __forceinline__ void add_four(float (&to)[4], const float (&x)[4]) {
+#pragma unroll
+    for (int c = 0; c < 4; c += 2) f32x2::unpack2(f32x2::add2(f32x2::pack2(to[c], to[c + 1]), f32x2::pack2(x[c], x[c + 1])), to[c], to[c + 1]);
 }
 template <bool BF> __device__ __forceinline__ uint32_t pack(float x, float y) {
     if constexpr (BF) return pack_bf16x2(x, y);
@@ -307,11 +323,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
 #pragma unroll
                     for (int c = 0; c < 4; ++c) s[mt][n][c] = s_lo[mt][n][c] = 0.f;
             auto add_to = [&](float (&to)[4], const uint32_t (&q0)[4], const uint32_t (&q1)[4], uint32_t b00, uint32_t b01, uint32_t b10, uint32_t b11) {
-                float t[4] = {0.f, 0.f, 0.f, 0.f};
-                mma<BF>(t, q0, b00, b01);
+                float t[4];
+                mma_from_zero<BF>(t, q0, b00, b01);
                 mma<BF>(t, q1, b10, b11);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) to[c] += t[c];
+                add_four(to, t);
             };
             if constexpr (KT == I8) {
 #pragma unroll
@@ -441,11 +456,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
             }
             auto weigh = [&](int mt, int n, uint32_t b0, uint32_t b1) {
                 if constexpr (TWO) {
-                    float t[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma<BF>(t, pf[mt][1], b0, b1);
+                    float t[4];
+                    mma_from_zero<BF>(t, pf[mt][1], b0, b1);
                     mma<BF>(t, pf[mt][0], b0, b1);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) o[mt][n][c] += t[c];
+                    add_four(o[mt][n], t);
                 } else {
                     mma<BF>(o[mt][n], pf[mt][0], b0, b1);
                 }

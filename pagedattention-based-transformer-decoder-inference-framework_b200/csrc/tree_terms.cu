@@ -9,12 +9,12 @@
 //                 values' scales relative to the largest possible of a tile; products and their sums are exact integers, no byte is converted
 // The sums of a tile leave the tensor cores as they are and are added up in float registers (the tensor cores cut where float rounds: over a
 // long context that would add up).  A row's terms are neighbours in P^T, whose rows are keys: a thread stores four query rows at once.
-//   warps 0-7    softmax, one thread per key and half of the rows: its scores, one vote per tile whether a row's reference has to move (then
+//   warps 0-7    (0-3: two CTAs an SM) softmax, one thread per key and half of (all) the rows: its scores, one vote per tile whether a row's reference has to move (then
 //                the maxima by warp and through shared memory), weights to shared memory as the MN-major B operand
-//   warps 8-11   one thread per value column: the tile's sums into its R float sums, rescaled where a reference moved
-//   warp 12      issues  S^T of tile t + 1  and  O^T of tile t;  scores and sums are double-buffered in TMEM
-//   warp 13      TMA boxes of 16 keys into a ring (int8: and the rows' scales), page ids a tile ahead
-//   warps 14-15  the next piece's queries into the K-major B operand, their factors and masks
+//   next four    one thread per value column: the tile's sums into its R float sums, rescaled where a reference moved
+//   next         issues  S^T of tile t + 1  and  O^T of tile t;  scores and sums are double-buffered in TMEM
+//   next         TMA boxes of 16 keys into a ring (int8: and the rows' scales), page ids a tile ahead
+//   last two     the next piece's queries into the K-major B operand, their factors and masks
 #include "tcgen05_utils.cuh"
 #include "tree_pieces.cuh"
 
@@ -23,26 +23,27 @@ namespace tterms {
 
 using namespace tc;
 
-constexpr int KT = 128, kSoftmax = 256, kThreads = 512, kNotes = 32;
-constexpr int W_SUMS = 8, W_MMA = 12, W_PROD = 13, W_LOAD = 14;
+constexpr int KT = 128, kNotes = 32;
 constexpr float kDigits = 8.3e6f;       // the largest number of three signed digits, and some to spare
 
 __device__ int g_errors;
 
-// I8: int8 pages.  R: query rows of a block
+// I8: int8 pages.  R: query rows of a block.  Blocks of 16 rows need so little that two CTAs share an SM and cover each other's beginnings and ends
 template <int D, bool I8, int R> struct Shape {
+    static constexpr int HALVES = R == 16 ? 1 : 2, CTAS = R == 16 ? 2 : 1, SOFTMAX = 128 * HALVES;     // threads
+    static constexpr int W_SUMS = 4 * HALVES, W_MMA = W_SUMS + 4, W_PROD = W_MMA + 1, W_LOAD = W_PROD + 1, THREADS = (W_LOAD + 2) * 32;
     static constexpr int TERMS = I8 ? 3 : 2, N = TERMS * R;         // columns of the scores: term by term
     static constexpr int NO = I8 ? 4 * R : 2 * R;                   // columns of the sums: row by row (int8: three digits and nothing)
     static constexpr int TILE = KT * D * (I8 ? 1 : 2), SCALES = I8 ? KT * 8 : 0, SLOT = TILE + SCALES;     // of keys or values; both scales of a tile come with its values
     static constexpr int Q_BYTES = N * 128 * (I8 ? 1 : D / 64), P_BYTES = KT * 128 * (R == 64 ? 2 : 1);
     static constexpr int Q_BUFS = Q_BYTES > 16384 ? 1 : 2;
-    static constexpr int FREE = 200 * 1024 - Q_BUFS * Q_BYTES;
+    static constexpr int FREE = (CTAS == 2 ? 106 : 200) * 1024 - Q_BUFS * Q_BYTES;
     static constexpr int P_BUFS = (FREE - 2 * P_BYTES) / SLOT >= 4 ? 2 : 1;
     static constexpr int RING = (FREE - P_BUFS * P_BYTES) / SLOT < 12 ? (FREE - P_BUFS * P_BYTES) / SLOT : 12;
     static constexpr int COLS = 2 * N + 2 * NO, TMEM = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int NBAR = 2 * RING + 16;      // full, empty [ring]; s_full, p_full, o_full, o_empty, q_ready, q_free [2]; piece_done [4]
     static constexpr int FLOATS = 2 * R /*factors*/ + 2 * R /*references, thresholds*/ + 4 * R /*corrections*/ + 4 * R /*maxima*/ +
-                                  4 * 5 * R /*sums, references at the end*/ + R /*what the sums are multiplied by*/ + 2 * 8 * R /*rows*/ + 24;
+                                  4 * 5 * R /*sums, references at the end*/ + 2 * R /*what becomes of the sums*/ + 2 * 8 * R /*rows*/ + 24;
     static size_t smem(int seqs, int mask_words) {
         return (size_t)RING * SLOT + Q_BUFS * Q_BYTES + P_BUFS * P_BYTES + NBAR * 8 + FLOATS * 4 + 2 * R * mask_words * 4 + kNotes * 4 + 64 + (seqs + 1) * 4 + 1024;
     }
@@ -90,9 +91,10 @@ __device__ __forceinline__ float from_digits(uint32_t d0, uint32_t d1, uint32_t 
 }
 
 template <int D, bool I8, int R, typename Q>
-__global__ void __launch_bounds__(kThreads, 1) tree_terms_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeWork a) {
+__global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTAS) tree_terms_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeWork a) {
     typedef Shape<D, I8, R> C;
-    constexpr int N = C::N, TERMS = C::TERMS, RING = C::RING, CB = I8 ? 1 : D / 64, RH = R / 2;       // CB: column blocks of a tile
+    constexpr int N = C::N, TERMS = C::TERMS, RING = C::RING, CB = I8 ? 1 : D / 64, RH = R / C::HALVES;       // CB: column blocks of a tile
+    constexpr int W_SUMS = C::W_SUMS, W_MMA = C::W_MMA, W_PROD = C::W_PROD, W_LOAD = C::W_LOAD, kSoftmax = C::SOFTMAX;
     constexpr float kRaise = I8 ? 1.f : 2.f, kShift = I8 ? 0.f : 10.f;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const TreeParams& p = a.p;
@@ -110,13 +112,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_terms_kernel(const __grid_co
     auto piece_done = [&](uint32_t piece) { return bar0 + (2 * RING + 12 + (piece & 3)) * 8; };
     const uint32_t tmem_slot = bar0 + C::NBAR * 8, fail_sm = tmem_slot + 8, meta_sm = fail_sm + 8;
     // factors of the scores [2 pieces], references (less kShift) and what a score may exceed them by, corrections of the last four tiles, maxima
-    // by warp, sums by warp and references of the last four pieces, what a piece's sums are multiplied by; nodes and heads of the last eight
+    // by warp, sums by warp and references of the last four pieces, a piece's rows of the output and what their sums are
+    // multiplied by; nodes and heads of the last eight
     // pieces' rows (node -1: no row); scales of the last four tiles, largest scale by warp of the last two;
     // whether references moved in the last four tiles, whether the last four pieces are computed by rows
     float* fl = reinterpret_cast<float*>(smem_raw + (meta_sm + kNotes * 4 - smem_u32(smem_raw)));
-    float *s_fe = fl, *s_ref = fl + 2 * R, *s_thr = fl + 3 * R, *s_corr = fl + 4 * R, *s_max = fl + 8 * R, *s_end = fl + 12 * R, *s_inv = fl + 32 * R, *s_scale = fl + 49 * R,
+    float *s_fe = fl, *s_ref = fl + 2 * R, *s_thr = fl + 3 * R, *s_corr = fl + 4 * R, *s_max = fl + 8 * R, *s_end = fl + 12 * R, *s_scale = fl + 50 * R,
           *s_big = s_scale + 4;
-    int *s_node = reinterpret_cast<int*>(fl + 33 * R), *s_head = s_node + 8 * R;         // (seven pieces at most are on their way)
+    int2* s_fin = reinterpret_cast<int2*>(fl + 32 * R);
+    int *s_node = reinterpret_cast<int*>(fl + 34 * R), *s_head = s_node + 8 * R;         // (seven pieces at most are on their way)
     int *s_moved = reinterpret_cast<int*>(s_big + 8), *s_odd = s_moved + 4, *pre = s_odd + 4;
     uint32_t* s_mask = reinterpret_cast<uint32_t*>(pre + p.num_seqs + 1);      // [2 pieces][R][mask_words]
     auto failed = [&] { return tc_failed(fail_sm); };
@@ -314,45 +318,52 @@ __global__ void __launch_bounds__(kThreads, 1) tree_terms_kernel(const __grid_co
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const int node = nodes[r0 + k];
-                    const Q* q = static_cast<const Q*>(p.q) + (node >= 0 ? (int64_t)node * p.q_stride + (int64_t)heads[r0 + k] * D : 0) + c0;
-#pragma unroll
-                    for (int c = 0; c < PER; ++c) x[k][c] = node >= 0 ? tree_widen<Q>(q[c]) : 0.f;
+                    const Q* q = static_cast<const Q*>(p.q) + (int64_t)node * p.q_stride + (int64_t)heads[r0 + k] * D + c0;
+                    if constexpr (sizeof(Q) == 4 && PER == 4) {
+                        const float4 v = node >= 0 ? __ldg(reinterpret_cast<const float4*>(q)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x[k][0] = v.x; x[k][1] = v.y; x[k][PER - 2] = v.z; x[k][PER - 1] = v.w;
+                    } else if constexpr (sizeof(Q) == 4) {
+                        const float2 v = node >= 0 ? __ldg(reinterpret_cast<const float2*>(q)) : make_float2(0.f, 0.f);
+                        x[k][0] = v.x; x[k][1] = v.y;
+                    } else {
+                        const uint2 v = node >= 0 ? __ldg(reinterpret_cast<const uint2*>(q)) : make_uint2(0u, 0u);
+                        const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+                        x[k][0] = lo.x; x[k][1] = lo.y; x[k][PER - 2] = hi.x; x[k][PER - 1] = hi.y;
+                    }
                 }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     big[k] = 0.f;
 #pragma unroll
                     for (int c = 0; c < PER; ++c) big[k] = fmaxf(big[k], fabsf(x[k][c]));
-                    big[k] = warp_max(big[k]);
                 }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) big[k] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big[k])));
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const int r = r0 + k;
                     if constexpr (I8) {
-                        // a row with numbers that are not finite: its scores are not, through their factor
-                        const float up = big[k] > 0.f && big[k] < INFINITY ? kDigits / big[k] : 0.f;
-                        uint32_t word[3] = {0u, 0u, 0u};
+                        // a row with numbers that are not finite: no digits, and its scores are not finite through their factor
                         bool odd = false;
 #pragma unroll
-                        for (int c = 0; c < PER; ++c) {
-                            odd |= !(fabsf(x[k][c]) < INFINITY);
-                            const uint32_t d = digits(odd ? 0 : __float2int_rn(x[k][c] * up));
+                        for (int c = 0; c < PER; ++c) odd |= !(fabsf(x[k][c]) < INFINITY);
+                        odd = __any_sync(0xffffffffu, odd);
+                        const float up = big[k] > 0.f && !odd ? __fdividef(kDigits, big[k]) : 0.f;
+                        uint32_t z[4];
 #pragma unroll
-                            for (int t = 0; t < 3; ++t) word[t] |= (d >> 8 * t & 255u) << 8 * c;
-                        }
+                        for (int c = 0; c < 4; ++c) z[c] = digits(__float2int_rn(x[k][c < PER ? c : 0] * up));
 #pragma unroll
                         for (int t = 0; t < 3; ++t) {
                             const int row = t * R + r;
-                            const uint32_t addr = qb + row * 128 + (((c0 >> 4) ^ (row & 7)) << 4) + (c0 & 15);
-                            if (PER == 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(word[t]) : "memory");
-                            else asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"((uint16_t)word[t]) : "memory");
+                            const uint32_t sel = (uint32_t)t | (uint32_t)(4 + t) << 4;
+                            const uint32_t word = __byte_perm(__byte_perm(z[0], z[1], sel), __byte_perm(z[2], z[3], sel), 0x5410);
+                            asm volatile("st.shared.u32 [%0], %1;" ::"r"(qb + row * 128 + (((c0 >> 4) ^ (row & 7)) << 4) + (c0 & 15)), "r"(word) : "memory");
                         }
-                        odd = __any_sync(0xffffffffu, odd);
-                        if (lane == 0) s_fe[buf * R + r] = odd ? __int_as_float(0x7fc00000) : f0 * (big[k] / kDigits);
+                        if (lane == 0) s_fe[buf * R + r] = odd ? __int_as_float(0x7fc00000) : up > 0.f ? __fdiv_rn(f0, up) : 0.f;
                     } else {
                         // the row's largest between 2^10 and 2^11: halves hold hi, and lo down to 2^-35 of it
-                        const int e = big[k] > 0.f && big[k] < INFINITY ? max(-100, min(100, 10 - ilogbf(big[k]))) : 0;
-                        const float up = exp2f((float)e);
+                        const int e = max(-100, min(100, 137 - (int)(__float_as_uint(big[k]) >> 23)));
+                        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
                         for (int c = 0; c < PER; c += 2) {
                             const uint32_t hi = pack_half2(x[k][c] * up, x[k][c + 1] * up);
@@ -365,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_terms_kernel(const __grid_co
                                 asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v[t]) : "memory");
                             }
                         }
-                        if (lane == 0) s_fe[buf * R + r] = f0 * exp2f((float)-e);
+                        if (lane == 0) s_fe[buf * R + r] = f0 * __uint_as_float((uint32_t)(127 - e) << 23);
                     }
                 }
             }
@@ -380,15 +391,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_terms_kernel(const __grid_co
         // ---- softmax: one thread per key and half of the rows
         const int kk = threadIdx.x & 127, quarter = warp & 3, h0 = (warp >> 2) * RH;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        auto group_sync = [&] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        auto group_sync = [&] { asm volatile("bar.sync 1, %0;" ::"n"(kSoftmax) : "memory"); };
         auto group_any = [&](bool x) {
             int any;
             asm volatile(
                 "{\n\t.reg .pred p, q;\n\t"
                 "setp.ne.b32 p, %1, 0;\n\t"
-                "barrier.cta.red.or.pred q, 1, 256, p;\n\t"
+                "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
                 "selp.b32 %0, 1, 0, q;\n\t}"
-                : "=r"(any) : "r"((int)x) : "memory");
+                : "=r"(any) : "r"((int)x), "n"(kSoftmax) : "memory");
             return any != 0;
         };
         auto four = [&](const float* f) { return *reinterpret_cast<const float4*>(f); };
@@ -444,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_terms_kernel(const __grid_co
                     }
                 }
                 // ---- scores, less their references; does one exceed its threshold?
-                constexpr int CH = RH < 16 ? RH : 16;
+                constexpr int CH = C::HALVES == 1 || RH < 16 ? 8 : 16;
                 const int bit = kp - w.sq.ctx;              // of the rows' masks, where it is not negative
                 const bool masked = drafts && here && bit >= 0, hidden = !here || (masked && (bit >> 5) >= p.mask_words);
                 float s[RH];
@@ -563,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_terms_kernel(const __grid_co
                 mbar_arrive_cnt(piece_done(pieces));
                 mbar_arrive_cnt(q_free(pieces));
             }
-            if (!I8 && odd && !failed()) tree_piece_by_rows<D, Q, __half>(a, w, warp * (R / 8), R / 8);
+            if (!I8 && odd && !failed()) tree_piece_by_rows<D, Q, __half>(a, w, warp * (R / W_SUMS), R / W_SUMS);
             ++pieces;
         }
     } else {
@@ -616,21 +627,26 @@ __global__ void __launch_bounds__(kThreads, 1) tree_terms_kernel(const __grid_co
             const float bad = failed() ? __int_as_float(0x7fc00000) : 0.f;
             if (d < R) {
                 const float sum = (end[d] + end[R + d] + end[2 * R + d] + end[3 * R + d]) * scale, ref = end[4 * R + d];
-                s_inv[d] = (w.slot < 0 ? scale / (sum + 1e-6f) : scale * a.p_scale) + bad;
-                if (w.slot >= 0 && !skip && nodes[d] >= 0)
+                const bool row = nodes[d] >= 0 && !skip;
+                s_fin[d] = make_int2(row ? (w.slot < 0 ? nodes[d] * p.heads + heads[d] : d) : -1,
+                                     __float_as_int((w.slot < 0 ? __fdiv_rn(scale, sum + 1e-6f) : scale * a.p_scale) + bad));
+                if (w.slot >= 0 && row)
                     *reinterpret_cast<float4*>(a.part + (w.slot * a.block + d) * (D + 4) + D) = make_float4(ref + bad, sum * a.p_scale + bad, ref, 0.f);
             }
             asm volatile("bar.sync 3, 128;" ::: "memory");
             if (!skip && d < D) {
+                float* part = a.part + w.slot * a.block * (D + 4) + d;
+                Q* out = static_cast<Q*>(p.out) + d;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const float x = o[r] * s_inv[r];
-                    if (nodes[r] < 0) continue;
-                    if (w.slot < 0) static_cast<Q*>(p.out)[((int64_t)nodes[r] * p.heads + heads[r]) * D + d] = tree_narrow<Q>(x);
-                    else a.part[(w.slot * a.block + r) * (D + 4) + d] = x;
+                    const int2 f = s_fin[r];
+                    const float x = o[r] * __int_as_float(f.y);
+                    if (f.x < 0) continue;
+                    if (w.slot < 0) out[(int64_t)f.x * D] = tree_narrow<Q>(x);
+                    else part[r * (D + 4)] = x;
                 }
             }
-            asm volatile("bar.sync 3, 128;" ::: "memory");      // s_inv is read
+            asm volatile("bar.sync 3, 128;" ::: "memory");      // s_fin is read
         }
     }
     tc_fence_before();
@@ -669,13 +685,13 @@ static int launch(const TreeWork& a, cudaStream_t st) {
     const bool ok = I8 ? make_byte_map(&k, p.k, a.total_rows, D) && make_byte_map(&v, p.v, a.total_rows, D)
                        : make_bf16_map(&k, p.k, a.total_rows, D, D, 16) && make_bf16_map(&v, p.v, a.total_rows, D, D, 16);     // boxes move bits
     if (!ok) return PA_ERR_UNSUPPORTED;
-    kern<<<a.workers, kThreads, smem, st>>>(k, v, a);
+    kern<<<a.workers, C::THREADS, smem, st>>>(k, v, a);
     PA_RETURN_LAUNCH_STATUS();
 }
 
 }  // namespace tterms
 
-int tree_terms_workers() { return device_info().sm_count; }
+int tree_terms_workers(int block) { return device_info().sm_count * (block == 16 ? 2 : 1); }
 
 // Rows of a block, 0 where this kernel does not serve or the streaming one is faster
 int tree_terms_block(const TreeParams& p) {
@@ -684,6 +700,7 @@ int tree_terms_block(const TreeParams& p) {
     if ((!half && !bytes) || (p.dim != 64 && p.dim != 128) || p.tile_size % 16 || p.num_seqs > kTreeMostSeqs) return 0;
     if ((int64_t)p.total_pages * p.tile_size >= 0x7fffff00ll || ((uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.k_scales | (uintptr_t)p.v_scales) % 16) return 0;
     if (half && rows <= 16) return 0;
+    if ((uintptr_t)p.q % 16 || p.q_stride % 4) return 0;
     const int block = bytes ? (rows <= 16 ? 16 : 32) : rows <= 32 ? 32 : 64;
     const int64_t steps = ((int64_t)p.num_tiles * p.tile_size + tterms::KT - 1) / tterms::KT;
     return ((int64_t)p.rows * G / block + p.num_seqs) * steps < 0x7fffffff ? block : 0;     // the list's sums are 32 bits
