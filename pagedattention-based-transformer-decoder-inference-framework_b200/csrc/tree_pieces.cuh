@@ -72,6 +72,14 @@ struct TreePages {
         cur = look_up(u0 + lane);
         nxt = look_up(u0 + 32 + lane);
     }
+    // lane k: the row of the k-th unit from `at`
+    __device__ __forceinline__ int lane_row(int at) {
+        if (at && (at & 31) == 0) {
+            cur = nxt;
+            nxt = look_up(u0 + at + 32 + (threadIdx.x & 31));
+        }
+        return __shfl_sync(0xffffffffu, cur, ((at & 31) + (threadIdx.x & 31)) & 31);
+    }
     // rows of the N units from `at` (a multiple of N, counted from the piece's first; in rising order), -1: no page; returns which have one
     template <int N>
     __device__ __forceinline__ uint32_t rows(int at, int (&r)[N]) {

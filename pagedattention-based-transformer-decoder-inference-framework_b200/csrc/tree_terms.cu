@@ -5,8 +5,11 @@
 // staged keys and values are the A operands as they stand in their pages.
 //     S^T = K Q^T      [128 keys x terms R],   O^T = V^T P^T   [D x terms R],   R = 16, 32 or 64 query rows of a block
 //   half pages    two terms of half each for a query (its row scaled by a power of two first) and for a weight: 22 bits of every factor
-//   int8 pages    kind::i8 with three signed digits each: a query row as 23-bit integers relative to its largest, the weights times their
-//                 values' scales relative to the largest possible of a tile; products and their sums are exact integers, no byte is converted
+//   int8 pages    kind::i8 with signed digits: a query row as 23-bit integers relative to its largest (three digits), the weights times their
+//                 values' scales as 31-bit ones relative to the largest possible of a tile (four); products and their sums are exact
+//                 integers, no byte is converted
+// A row's reference moves only when a score exceeds it by more than 2^8, which the terms leave room for: after a piece's first tile
+// hardly ever.
 // The sums of a tile leave the tensor cores as they are and are added up in float registers (the tensor cores cut where float rounds: over a
 // long context that would add up).  A row's terms are neighbours in P^T, whose rows are keys: a thread stores four query rows at once.
 //   warps 0-7    (0-3: two CTAs an SM) softmax, one thread per key and half of (all) the rows: its scores, one vote per tile whether a row's reference has to move (then
@@ -24,7 +27,8 @@ namespace tterms {
 using namespace tc;
 
 constexpr int KT = 128, kNotes = 32;
-constexpr float kDigits = 8.3e6f;       // the largest number of three signed digits, and some to spare
+constexpr float kDigits = 8.3e6f, kDigits4 = 2.1e9f;      // the largest number of three and of four signed digits, and some to spare
+constexpr float kRaise = 8.f;
 
 __device__ int g_errors;
 
@@ -33,7 +37,7 @@ template <int D, bool I8, int R> struct Shape {
     static constexpr int HALVES = R == 16 ? 1 : 2, CTAS = R == 16 ? 2 : 1, SOFTMAX = 128 * HALVES;     // threads
     static constexpr int W_SUMS = 4 * HALVES, W_MMA = W_SUMS + 4, W_PROD = W_MMA + 1, W_LOAD = W_PROD + 1, THREADS = (W_LOAD + 2) * 32;
     static constexpr int TERMS = I8 ? 3 : 2, N = TERMS * R;         // columns of the scores: term by term
-    static constexpr int NO = I8 ? 4 * R : 2 * R;                   // columns of the sums: row by row (int8: three digits and nothing)
+    static constexpr int NO = I8 ? 4 * R : 2 * R;                   // columns of the sums: row by row
     static constexpr int TILE = KT * D * (I8 ? 1 : 2), SCALES = I8 ? KT * 8 : 0, SLOT = TILE + SCALES;     // of keys or values; both scales of a tile come with its values
     static constexpr int Q_BYTES = N * 128 * (I8 ? 1 : D / 64), P_BYTES = KT * 128 * (R == 64 ? 2 : 1);
     static constexpr int Q_BUFS = Q_BYTES > 16384 ? 1 : 2;
@@ -43,7 +47,7 @@ template <int D, bool I8, int R> struct Shape {
     static constexpr int COLS = 2 * N + 2 * NO, TMEM = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int NBAR = 2 * RING + 16;      // full, empty [ring]; s_full, p_full, o_full, o_empty, q_ready, q_free [2]; piece_done [4]
     static constexpr int FLOATS = 2 * R /*factors*/ + 2 * R /*references, thresholds*/ + 4 * R /*corrections*/ + 4 * R /*maxima*/ +
-                                  4 * 5 * R /*sums, references at the end*/ + 2 * R /*what becomes of the sums*/ + 2 * 8 * R /*rows*/ + 24;
+                                  4 * 5 * R /*sums, references at the end*/ + 2 * R /*what becomes of the sums*/ + 2 * 8 * R /*rows*/ + 28;
     static size_t smem(int seqs, int mask_words) {
         return (size_t)RING * SLOT + Q_BUFS * Q_BYTES + P_BUFS * P_BYTES + NBAR * 8 + FLOATS * 4 + 2 * R * mask_words * 4 + kNotes * 4 + 64 + (seqs + 1) * 4 + 1024;
     }
@@ -89,13 +93,18 @@ __device__ __forceinline__ float from_digits(uint32_t d0, uint32_t d1, uint32_t 
     const float hi = __uint_as_float(d2 + 0x4b400000u) - 12582912.f;
     return fmaf(hi, 65536.f, (float)((int)d1 * 256 + (int)d0));
 }
+// and of four
+__device__ __forceinline__ uint32_t digits4(int x) { return (uint32_t)(x + 0x80808080) ^ 0x80808080u; }
+__device__ __forceinline__ float from_digits4(uint32_t d0, uint32_t d1, uint32_t d2, uint32_t d3) {
+    return fmaf((float)((int)d3 * 256 + (int)d2), 65536.f, (float)((int)d1 * 256 + (int)d0));
+}
 
 template <int D, bool I8, int R, typename Q>
 __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTAS) tree_terms_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeWork a) {
     typedef Shape<D, I8, R> C;
     constexpr int N = C::N, TERMS = C::TERMS, RING = C::RING, CB = I8 ? 1 : D / 64, RH = R / C::HALVES;       // CB: column blocks of a tile
     constexpr int W_SUMS = C::W_SUMS, W_MMA = C::W_MMA, W_PROD = C::W_PROD, W_LOAD = C::W_LOAD, kSoftmax = C::SOFTMAX;
-    constexpr float kRaise = I8 ? 1.f : 2.f, kShift = I8 ? 0.f : 10.f;
+    constexpr float kShift = I8 ? 0.f : 7.f;                     // half weights times 2^7: up to 2^15
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const TreeParams& p = a.p;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -111,17 +120,18 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
     auto q_phase = [&](uint32_t piece) { return piece / C::Q_BUFS & 1u; };
     auto piece_done = [&](uint32_t piece) { return bar0 + (2 * RING + 12 + (piece & 3)) * 8; };
     const uint32_t tmem_slot = bar0 + C::NBAR * 8, fail_sm = tmem_slot + 8, meta_sm = fail_sm + 8;
-    // factors of the scores [2 pieces], references (less kShift) and what a score may exceed them by, corrections of the last four tiles, maxima
+    // factors of the scores [2 pieces], references (less kShift) and whether rows have one, corrections of the last four tiles, maxima
     // by warp, sums by warp and references of the last four pieces, a piece's rows of the output and what their sums are
     // multiplied by; nodes and heads of the last eight
     // pieces' rows (node -1: no row); scales of the last four tiles, largest scale by warp of the last two;
-    // whether references moved in the last four tiles, whether the last four pieces are computed by rows
+    // whether references moved in the last four tiles, whether the last four pieces are computed by rows,
+    // whether a row has no reference yet
     float* fl = reinterpret_cast<float*>(smem_raw + (meta_sm + kNotes * 4 - smem_u32(smem_raw)));
-    float *s_fe = fl, *s_ref = fl + 2 * R, *s_thr = fl + 3 * R, *s_corr = fl + 4 * R, *s_max = fl + 8 * R, *s_end = fl + 12 * R, *s_scale = fl + 50 * R,
+    float *s_fe = fl, *s_ref = fl + 2 * R, *s_set = fl + 3 * R, *s_corr = fl + 4 * R, *s_max = fl + 8 * R, *s_end = fl + 12 * R, *s_scale = fl + 50 * R,
           *s_big = s_scale + 4;
     int2* s_fin = reinterpret_cast<int2*>(fl + 32 * R);
     int *s_node = reinterpret_cast<int*>(fl + 34 * R), *s_head = s_node + 8 * R;         // (seven pieces at most are on their way)
-    int *s_moved = reinterpret_cast<int*>(s_big + 8), *s_odd = s_moved + 4, *pre = s_odd + 4;
+    int *s_moved = reinterpret_cast<int*>(s_big + 8), *s_odd = s_moved + 4, *s_pending = s_odd + 4, *pre = s_pending + 4;
     uint32_t* s_mask = reinterpret_cast<uint32_t*>(pre + p.num_seqs + 1);      // [2 pieces][R][mask_words]
     auto failed = [&] { return tc_failed(fail_sm); };
     auto wait = [&](uint32_t bar, uint32_t parity) { tc_wait(bar, parity, fail_sm, a.polls); };
@@ -172,27 +182,29 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
         uint32_t c = 0, tiles = 0;          // requests and tiles of keys so far
         bool ok = true;
         if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = TreeNote{};
-        auto request = [&](const CUtensorMap* map, bool scales, const int (&r)[8]) {
+        auto request = [&](const CUtensorMap* map, bool scales, int rows) {         // lane u < 8: of unit u
             const int s = (int)(c % RING);
             wait(kv_empty(s), (c / RING & 1u) ^ 1u);
             if (__any_sync(0xffffffffu, failed())) {
                 ok = false;
                 return;
             }
-            if (elect_one()) {
-                const uint32_t st = base + s * C::TILE;
-                mbar_arrive_expect_tx(kv_full(s), C::TILE);
+            const uint32_t st = base + s * C::TILE;
+            if (elect_one()) mbar_arrive_expect_tx(kv_full(s), C::TILE);
+            int r[8];
+#pragma unroll
+            for (int uu = 0; uu < 8; ++uu) {
+                r[uu] = __shfl_sync(0xffffffffu, rows, uu);
+                if (r[uu] < 0) r[uu] = a.total_rows;    // no page: zeros, and its scores are masked
+            }
+            if (elect_one())
 #pragma unroll
                 for (int uu = 0; uu < 8; ++uu)
 #pragma unroll
-                    for (int cb = 0; cb < CB; ++cb)     // no page: zeros, and its scores are masked
-                        tma_load_2d(st + cb * 16384 + uu * (I8 ? 16 * D : 2048), map, cb * 64, r[uu] >= 0 ? r[uu] : a.total_rows, kv_full(s));
-            }
+                    for (int cb = 0; cb < CB; ++cb) tma_load_2d(st + cb * 16384 + uu * 2048, map, cb * 64, r[uu], kv_full(s));
             __syncwarp();
             if (I8 && scales) {                         // a lane: 16 bytes of a unit's 64, of keys and of values
-                int row = -1;
-#pragma unroll
-                for (int uu = 0; uu < 8; ++uu) row = lane >> 2 == uu ? r[uu] : row;
+                const int row = __shfl_sync(0xffffffffu, rows, lane >> 2);
                 if (row >= 0) {
                     const uint32_t to = sc_sm + s * C::SCALES + lane * 16;
                     cp_async_16(to, p.k_scales + row + (lane & 3) * 4, true);
@@ -208,20 +220,19 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
         while (ok && w.next()) {
             if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = tree_note(a, w.sq, w.g, w.rr0, w.i0, w.i1, w.f - w.i1, w.total, w.ns, w.slot);
             pages.open(w, 8);
-            int r[8], prev[8];
-#pragma unroll
-            for (int uu = 0; uu < 8; ++uu) r[uu] = prev[uu] = -1;
+            int rows = -1, before = -1;
+#pragma unroll 1
             for (int i = w.i0; i <= w.i1 && ok; ++i) {              // K(i) and V(i - 1)
                 if (i < w.i1) {
-                    const uint32_t mapped = pages.rows<8>((i - w.i0) * 8, r);
+                    rows = pages.lane_row((i - w.i0) * 8);
+                    const uint32_t mapped = __ballot_sync(0xffffffffu, rows >= 0) & 255u;
                     if (lane == 0) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(meta_sm + tiles % kNotes * 4), "r"(mapped) : "memory");
                     __syncwarp();
                     ++tiles;
-                    request(&tmK, false, r);
                 }
-                if (i > w.i0 && ok) request(&tmV, true, prev);
-#pragma unroll
-                for (int uu = 0; uu < 8; ++uu) prev[uu] = r[uu];
+#pragma unroll 1
+                for (int v = i < w.i1 ? 0 : 1; v < (i > w.i0 ? 2 : 1) && ok; ++v) request(v ? &tmV : &tmK, v, v ? before : rows);
+                before = rows;
             }
         }
         if (failed())           // let the copies in flight land before the CTA's shared memory goes away
@@ -403,11 +414,9 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
             return any != 0;
         };
         auto four = [&](const float* f) { return *reinterpret_cast<const float4*>(f); };
-        auto fresh = [&] {                  // no reference yet: any score sets one
-            if (threadIdx.x < R) {
-                s_ref[threadIdx.x] = 0.f;
-                s_thr[threadIdx.x] = -3e38f;
-            }
+        auto fresh = [&] {                  // no references yet
+            if (threadIdx.x < R) s_ref[threadIdx.x] = s_set[threadIdx.x] = 0.f;
+            if (threadIdx.x == 0) *s_pending = 1;
         };
         fresh();
         while (w.next()) {
@@ -454,7 +463,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                         }
                     }
                 }
-                // ---- scores, less their references; does one exceed its threshold?
+                // ---- scores, less their references; does one exceed its own?
                 constexpr int CH = C::HALVES == 1 || RH < 16 ? 8 : 16;
                 const int bit = kp - w.sq.ctx;              // of the rows' masks, where it is not negative
                 const bool masked = drafts && here && bit >= 0, hidden = !here || (masked && (bit >> 5) >= p.mask_words);
@@ -469,15 +478,15 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
 #pragma unroll
                     for (int j = 0; j < CH; j += 4) {
                         const int r = c * CH + j;
-                        const float4 fe = four(fes + r), ref = four(s_ref + h0 + r), thr = four(s_thr + h0 + r);
-                        const float f[4] = {fe.x, fe.y, fe.z, fe.w}, o[4] = {ref.x, ref.y, ref.z, ref.w}, h[4] = {thr.x, thr.y, thr.z, thr.w};
+                        const float4 fe = four(fes + r), ref = four(s_ref + h0 + r);
+                        const float f[4] = {fe.x, fe.y, fe.z, fe.w}, o[4] = {ref.x, ref.y, ref.z, ref.w};
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             float v;
                             if constexpr (I8) v = fmaf(from_digits(x[0][j + e], x[1][j + e], x[TERMS - 1][j + e]), f[e] * ksc, -o[e]);
                             else v = fmaf(__uint_as_float(x[0][j + e]) + __uint_as_float(x[1][j + e]), f[e], -o[e]);
                             s[r + e] = hidden ? -INFINITY : v;
-                            over |= s[r + e] > h[e];
+                            over |= s[r + e] > kRaise + kShift;
                         }
                     }
                 }
@@ -487,10 +496,11 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
 #pragma unroll
                     for (int r = 0; r < RH; ++r) {
                         if (masked && !(mw[r * p.mask_words] >> (bit & 31) & 1u)) s[r] = -INFINITY;
-                        over |= s[r] > s_thr[h0 + r];
+                        over |= s[r] > kRaise + kShift;
                     }
                 }
-                const bool any = group_any(over);
+                const bool any = group_any(over || *s_pending);
+                if (threadIdx.x == 0) s_moved[ring4] = any;
                 if (any) {
 #pragma unroll
                     for (int r = 0; r < RH; ++r) {
@@ -501,13 +511,13 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                     if (threadIdx.x < R) {
                         const int r = threadIdx.x;
                         const float top = fmaxf(fmaxf(s_max[r], s_max[R + r]), fmaxf(s_max[2 * R + r], s_max[3 * R + r]));
-                        const bool raise = top > s_thr[r];
+                        const bool has = s_set[r] != 0.f, raise = has ? top > kRaise + kShift : top > -INFINITY;
                         const float by = raise ? top - kShift : 0.f;
-                        // a first reference has no sums to correct
-                        s_corr[ring4 * R + r] = s_thr[r] < -1e38f ? 1.f : exp2f(-by);
+                        s_corr[ring4 * R + r] = has ? exp2f(-by) : 1.f;         // a first reference has no sums to correct
                         s_max[r] = by;
                         s_ref[r] += by;
-                        if (raise) s_thr[r] = kRaise + kShift;
+                        if (raise) s_set[r] = 1.f;
+                        else if (!has && s_node[(pieces & 7) * R + r] >= 0) s_moved[ring4] = 2;        // still none
                     }
                     group_sync();
 #pragma unroll
@@ -515,15 +525,15 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                         l[r] *= s_corr[ring4 * R + h0 + r];
                         s[r] -= s_max[h0 + r];
                     }
+                    if (threadIdx.x == 0) *s_pending = s_moved[ring4] == 2;
                 }
                 float unit = 0.f;           // int8: weights per value scale, as integers
                 if (I8) {
                     const float4 b4 = four(s_big + sb * 4);
                     const float big = fmaxf(fmaxf(b4.x, b4.y), fmaxf(b4.z, b4.w));
-                    unit = big > 0.f ? vsc / big * (kDigits / 2.f) : 0.f;
-                    if (threadIdx.x == 0) s_scale[ring4] = big * (2.f / kDigits);
+                    unit = big > 0.f ? __fdividef(vsc, big) * (kDigits4 / 256.f) : 0.f;         // weights are 2^8 at most
+                    if (threadIdx.x == 0) s_scale[ring4] = big * (256.f / kDigits4);
                 }
-                if (threadIdx.x == 0) s_moved[ring4] = any;
                 // ---- weights: four rows' terms a 16-byte word
                 const uint32_t pb = p_sm + (uint32_t)((C::P_BUFS == 2 ? sb : 0) * C::P_BYTES) + kk * 128;
                 if (C::P_BUFS == 1 && t > 0) wait(o_full((t - 1) & 1), (t - 1) >> 1 & 1u);      // their place is read
@@ -538,8 +548,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                     uint32_t v[4];
                     if constexpr (I8) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)         // a float between 2^23 and 2^24 holds the integer in its mantissa
-                            v[k] = (__float_as_uint(fmaf(e[k], unit, 8388608.f)) + (0x808080u - 0x4b000000u)) ^ 0x808080u;
+                        for (int k = 0; k < 4; ++k) v[k] = digits4(__float2int_rn(e[k] * unit));
                     } else {
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
@@ -566,7 +575,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                 const float sum = warp_sum(l[r]);
                 if (lane == 0) end[quarter * R + h0 + r] = sum;
             }
-            if (threadIdx.x < R) end[4 * R + threadIdx.x] = s_thr[threadIdx.x] < -1e38f ? -INFINITY : s_ref[threadIdx.x] + kShift;
+            if (threadIdx.x < R) end[4 * R + threadIdx.x] = s_set[threadIdx.x] != 0.f ? s_ref[threadIdx.x] + kShift : -INFINITY;
             if (threadIdx.x == 0) s_odd[pieces & 3] = odd;
             fresh();
             __syncwarp();
@@ -603,9 +612,9 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                     tmem_wait_ld();
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
-                        if constexpr (I8) {                 // a row's digits, and nothing
+                        if constexpr (I8) {                 // a row's digits
                             const int r = c * 8 + j / 4;
-                            o[r] = fmaf(from_digits(x[j], x[j + 1], x[j + 2]), unit, o[r]);
+                            o[r] = fmaf(from_digits4(x[j], x[j + 1], x[j + 2], x[j + 3]), unit, o[r]);
                         } else {                            // two rows' large terms, and their small ones
                             const int r = c * 16 + j / 2;
                             o[r] += __uint_as_float(x[j]) + __uint_as_float(x[j + 2]);
@@ -623,7 +632,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
             ++pieces;
             const int* nodes = s_node + ((pieces - 1) & 7) * R;
             const int* heads = s_head + ((pieces - 1) & 7) * R;
-            constexpr float scale = I8 ? 1.f : 1.f / 1024.f;    // 2^-kShift
+            constexpr float scale = I8 ? 1.f : 1.f / 128.f;     // 2^-kShift
             const float bad = failed() ? __int_as_float(0x7fc00000) : 0.f;
             if (d < R) {
                 const float sum = (end[d] + end[R + d] + end[2 * R + d] + end[3 * R + d]) * scale, ref = end[4 * R + d];
