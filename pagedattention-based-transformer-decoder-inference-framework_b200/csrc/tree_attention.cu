@@ -118,7 +118,10 @@ PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void
     PA_CHECK_ARG(d_q && d_out && d_k_pool && d_v_pool && d_table && d_ctx_lens && d_node_start && d_mask);
     PA_CHECK_ARG(q_stride >= (int64_t)heads * head_dim && mask_words > 0 && (int64_t)mask_words * 32 >= most_nodes);
     PA_CHECK_ARG((kv_type == PA_TYPE_I8) == (d_k_scales != nullptr) && (kv_type == PA_TYPE_I8) == (d_v_scales != nullptr));
-    if (most_nodes > PA_TREE_MOST_NODES) return PA_ERR_UNSUPPORTED;
+    const bool pair = q_type == PA_TYPE_F32    ? kv_type == PA_TYPE_F16 || kv_type == PA_TYPE_I8 || kv_type == PA_TYPE_F32
+                      : q_type == PA_TYPE_F16 ? kv_type == PA_TYPE_F16 || kv_type == PA_TYPE_I8
+                                              : q_type == PA_TYPE_BF16 && kv_type == PA_TYPE_BF16;
+    if (most_nodes > PA_TREE_MOST_NODES || !pair) return PA_ERR_UNSUPPORTED;
     const TreeParams p{d_q, q_stride, d_out, d_k_pool, d_v_pool, d_k_scales, d_v_scales, d_table, d_beam_ids, d_ctx_lens, d_node_start,
                        reinterpret_cast<const uint32_t*>(d_mask), q_type, kv_type, num_beams, kv_heads, num_tiles, total_pages, mask_words,
                        rows, num_seqs, most_nodes, heads, head_dim, tile_size, temperature};

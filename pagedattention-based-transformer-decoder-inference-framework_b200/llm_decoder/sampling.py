@@ -93,8 +93,8 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
         raise ValueError("history and history_start come together")
 
     def of(x, dtype, what, n=None):
-        if not isinstance(x, torch.Tensor) or x.dtype != dtype or x.device != dev or x.dim() != 1 or not x.is_contiguous() or \
-                (n is not None and x.numel() != n):
+        if not isinstance(x, torch.Tensor) or x.dtype is not dtype or x.device != dev or x.dim() != 1 or not x.is_contiguous() or \
+                (n is not None and len(x) != n):
             raise ValueError(f"{what}: a contiguous {dtype} vector{'' if n is None else f' of {n}'} on {dev}")
         return x
     if tree is not None:
@@ -113,8 +113,8 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
     arrays, values = [], []
     for x, what in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")):
         if isinstance(x, torch.Tensor):
-            arrays.append(of(x, torch.float32, what, seqs))
-            seqs = x.numel()
+            arrays.append(of(x, torch.float32, what, seqs).data_ptr())
+            seqs = len(x)
             values.append(0.0)
         else:
             arrays.append(None)
@@ -147,7 +147,7 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
         _cabi.check(lib.pa_adjust_logits(
             logits.data_ptr(), types[logits.dtype], logits.stride(0) if rows > 1 else V, rows, V, _cabi.ptr(out),
             0 if out is None else out.stride(0) if rows > 1 else V, _cabi.ptr(ids), _cabi.ptr(row_seq), _cabi.ptr(history), _cabi.ptr(history_start),
-            *(_cabi.ptr(a) for a in arrays), *values, _cabi.ptr(b_ids), _cabi.ptr(b_val), _cabi.ptr(b_start), _cabi.ptr(allowed),
+            *arrays, *values, _cabi.ptr(b_ids), _cabi.ptr(b_val), _cabi.ptr(b_start), _cabi.ptr(allowed),
             0 if allowed is None else allowed.stride(0) if allowed.shape[0] > 1 else allowed.shape[1], _cabi.ptr(allowed_rows),
             *((tree.tokens.data_ptr(), tree.mask.data_ptr(), tree.mask.shape[1], tree.node_start.data_ptr()) if tree is not None else
               (None, None, 0, None)), _cabi.ptr(ws), need, stream), "pa_adjust_logits")
