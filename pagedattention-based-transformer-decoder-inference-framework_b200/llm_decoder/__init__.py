@@ -13,7 +13,7 @@ from .int8_quant import (batch_dequantize, batch_minmax_scale, batch_quantize, c
 from .kv_tile_cache import KVTileCache  # noqa: F401
 from .page_table import PageTable  # noqa: F401
 from . import sampling  # noqa: F401
-from .draft_tree import Accepted, DraftTree, TreeCaches, paged_tree_attention, tree_accept  # noqa: F401
+from .draft_tree import Accepted, DraftTree, TreeCaches, lookup_drafts, paged_tree_attention, tree_accept  # noqa: F401
 
 from .decoders import CUDADecoder, INT8Decoder  # noqa: F401
 

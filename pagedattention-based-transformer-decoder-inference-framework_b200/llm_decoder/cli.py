@@ -2,7 +2,11 @@
 
     python -m llm_decoder.cli generate --model DIR --prompt 5,17,3 [--prompt ...] --max-new-tokens 16
                                        [--dtype bfloat16|float32] [--temperature T --top-k K --top-p P --seed S]
+                                       [--drafts N --repetition-penalty R --presence-penalty P --frequency-penalty F]
     python -m llm_decoder.cli trace    --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N   (bin/trace_run)
+
+--drafts and the penalties are for CUDADecoder and INT8Decoder, greedily: up to N guesses of the next tokens, looked up in the sequence
+itself, are verified in every step (decoders.generate_drafted).
 
 `trace` replays a schedule from standard input, one JSON object per line:
     {"step": 0, "entries": [{"id": "a", "tokens": [5, 17, 3], "want": [0, 2]}], "end": []}
@@ -81,12 +85,25 @@ def generate_main(argv=None):
     ap.add_argument("--top-k", type=int, default=0)
     ap.add_argument("--top-p", type=float, default=1.0)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--drafts", type=int, default=0)
+    ap.add_argument("--repetition-penalty", type=float, default=1.0)
+    ap.add_argument("--presence-penalty", type=float, default=0.0)
+    ap.add_argument("--frequency-penalty", type=float, default=0.0)
     a = ap.parse_args(argv)
+    rules = dict(repetition=a.repetition_penalty, presence=a.presence_penalty, frequency=a.frequency_penalty)
+    drafted = a.drafts != 0 or rules != dict(repetition=1.0, presence=0.0, frequency=0.0)
+    if drafted and (a.temperature != 1.0 or a.top_k > 0 or a.top_p < 1.0):
+        ap.error("--drafts and the penalties go with greedy generation")
     _ensure_library()
     from .registry import load_model
     prompts = [[int(t) for t in p.split(",") if t.strip()] for p in a.prompt]
     model = load_model(a.model, a.dtype, max_tokens=a.max_tokens, max_seqs=a.max_seqs)
-    if hasattr(model, "states"):
+    if drafted:
+        if not hasattr(model, "generate_drafted"):
+            print("this architecture does not verify drafts", file=sys.stderr)
+            return 4
+        outs = [model.generate_drafted([p], a.max_new_tokens, drafts=a.drafts, **rules)[0] for p in prompts]
+    elif hasattr(model, "states"):
         from .engine import generate
         outs = generate(model, prompts, a.max_new_tokens, max_batch_tokens=a.max_batch_tokens,
                         temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, seed=a.seed)

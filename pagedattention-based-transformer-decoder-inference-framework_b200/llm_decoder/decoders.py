@@ -30,6 +30,7 @@ tcgen05 GEMM (pa_gemm_i8_dequant) with the LN1 output quantised per row.  Files 
 Every step runs on the device through libpa_b200.so (no host math, no per-step
 synchronisation); the steady-state step is captured in a CUDA graph.
 """
+import copy
 import json
 import os
 
@@ -37,6 +38,9 @@ import numpy as np
 import torch
 
 from . import _cabi
+from . import sampling
+from .draft_tree import DraftTree, TreeCaches, lookup_drafts, paged_tree_attention, tree_accept
+from .host_stage import to_device
 from .kv_tile_cache import KVTileCache
 
 _LAYER_FILES = ("ln1.bin", "ln2.bin", "mlp_fc1.bin", "mlp_fc2.bin", "mlp_biases.bin")  # int8_decoder.cpp:66-70
@@ -73,6 +77,12 @@ class _Bufs:
         self.hs = torch.ones(R, **f32)
         self.ws = None  # GEMM / linear scratch for R rows (owned here, never by the library; _DecoderBase._scratch)
         self.qp = self.kp = self.vp = None  # q / k / v projections [R, hid] f32, allocated when a layer has them
+
+    def first(self, R):
+        """The buffers of the first R rows."""
+        few = copy.copy(self)
+        few.__dict__.update({k: v[:R] for k, v in self.__dict__.items() if isinstance(v, torch.Tensor) and k != "ws"}, R=R)
+        return few
 
 
 class _DecoderBase:
@@ -153,10 +163,14 @@ class _DecoderBase:
                 self._graph = None
         return bf.ws.data_ptr(), bf.ws.numel()
 
-    def _attention(self, layer_idx, q, out, R, ctx_lens, beam_ids, ws, prefill_shape=None):
+    def _attention(self, layer_idx, q, out, R, ctx_lens, beam_ids, ws, prefill_shape=None, tree=None):
         kvc = self.kv_caches[layer_idx]
         pt = kvc.page_table_
         lib = self._lib
+        if tree is not None:
+            shape = (R, self.num_heads_, self.head_dim_)
+            paged_tree_attention(q.view(shape), kvc, tree, ctx_lens, self.attn_temperature, out=out.view(shape))
+            return
         if prefill_shape is not None and self.head_dim_ in (64, 128):
             # prompt pass: the tcgen05 flash-attention prefill kernel ([B, H, n, D] layout)
             from .attention import paged_prefill
@@ -191,10 +205,11 @@ class _DecoderBase:
                     kvc.k_scales_.data_ptr(), kvc.v_scales_.data_ptr(), *common)
         self._chk(st, "pa_paged_decode")
 
-    def _layers(self, bf, ids, positions, ctx_lens, beam_ids, ws, prefill_shape=None):
+    def _layers(self, bf, ids, positions, ctx_lens, beam_ids, ws, prefill_shape=None, tree=None):
         """The decoder stack (decoder_block.hpp:41-62) for bf.R rows: row r is token ids[r] at position
         positions[r] of table row beam_ids[r] (None: r) attending ctx_lens[r] cached tokens (its own K/V
-        included).  Leaves the final hidden states in bf.x."""
+        included).  tree: the rows are the nodes of a DraftTree, ctx_lens the cached tokens of its sequences before them.  Leaves the
+        final hidden states in bf.x."""
         lib, R, hid, s = self._lib, bf.R, self.hidden_dim_, _cabi.stream()
         self._embed(bf, ids)
         for li, L in enumerate(self.layers):
@@ -204,13 +219,13 @@ class _DecoderBase:
             if getattr(L, "wq", None) is None:
                 nview = bf.n.view(R, H, D)
                 self.kv_caches[li].append(nview, nview, positions, beam_ids)  # K = V = LN1 output (see module doc)
-                self._attention(li, bf.n, bf.a, R, ctx_lens, beam_ids, ws, prefill_shape)
+                self._attention(li, bf.n, bf.a, R, ctx_lens, beam_ids, ws, prefill_shape, tree)
             else:
                 if bf.qp is None:
                     bf.qp, bf.kp, bf.vp = (torch.empty((R, hid), dtype=torch.float32, device=self.device) for _ in range(3))
                 self._qkv_proj(bf, L)                                   # bf.n -> bf.qp, bf.kp, bf.vp
                 self.kv_caches[li].append(bf.kp.view(R, H, D), bf.vp.view(R, H, D), positions, beam_ids)
-                self._attention(li, bf.qp, bf.kp, R, ctx_lens, beam_ids, ws, prefill_shape)   # kp reused as the output
+                self._attention(li, bf.qp, bf.kp, R, ctx_lens, beam_ids, ws, prefill_shape, tree)   # kp reused as the output
                 self._o_proj(bf, L, bf.kp, bf.a)                        # attention output . Wo -> bf.a
             self._ln2_mlp(bf, L)
 
@@ -233,7 +248,6 @@ class _DecoderBase:
                                                  self.ids.data_ptr(), _cabi.stream()), "pa_logits_argmax")
             return
         self._logits(x_rows)
-        from . import sampling
         # CUDADecoder scales logits by 1/T (cuda_decoder.cu:10-13), INT8Decoder by T (int8_decoder.cpp:100)
         t_eff = self._temperature if self.ARGMAX_DIVIDE else 1.0 / self._temperature
         probs = sampling.softmax_temperature(self.logits, t_eff)
@@ -249,11 +263,11 @@ class _DecoderBase:
         self._chk(self._lib.pa_advance_positions(self.positions.data_ptr(), self.ctx_lens.data_ptr(), self._batch,
                                                  _cabi.stream()), "pa_advance_positions")
 
-    def _prefill(self, prompt):
+    def _prefill(self, prompt, head=True):
         """All prompt tokens of all sequences in ONE pass through the stack: row
         (b, t) appends its K/V at position t of table row b and attends causally (ctx = t + 1) through
         the beam indirection of the decode kernels; LayerNorm and the MLP GEMMs run on B*n rows.
-        Leaves the first sampled token in self.ids and positions = n."""
+        Leaves the first sampled token in self.ids (head) and positions = n."""
         B, n = prompt.shape
         dev = self.device
         R = B * n
@@ -265,8 +279,8 @@ class _DecoderBase:
         ws = torch.empty(self._lib.pa_decode_workspace_bytes(R, self.num_heads_, self.head_dim_, self._num_tiles,
                                                              self.tile_size_), dtype=torch.uint8, device=dev)
         self._layers(bf, prompt.reshape(-1).contiguous(), positions, ctx, beam, ws, prefill_shape=(B, n))
-        last = bf.x.view(B, n, self.hidden_dim_)[:, n - 1, :].contiguous()
-        self._head(last)
+        if head:
+            self._head(bf.x.view(B, n, self.hidden_dim_)[:, n - 1, :].contiguous())
         self.positions.fill_(n)
         self.ctx_lens.fill_(n + 1)
 
@@ -350,6 +364,79 @@ class _DecoderBase:
                     self._step_or_replay()
             gen_host = gen.t().cpu().tolist()  # the only synchronisation of the call
         return [list(p) + g for p, g in zip(prompts, gen_host)]
+
+    def generate_drafted(self, prompts, max_len, drafts=16, branches=2, draft=None, repetition=1.0, presence=0.0, frequency=0.0,
+                         bias=None, allowed=None):
+        """generate_batch's greedy tokens in fewer steps: every step runs the pending token of each sequence and up to `drafts` guesses
+        of what follows it, and keeps the guesses that the model itself would have given (draft_tree.py).  What the guesses are
+        changes the number of steps (`drafted_steps_` afterwards) and not the tokens, up to ties within the rounding of the logits.
+
+        draft(tokens, most, depth) -> (parents, tokens) of a sequence's tree, at most `most` nodes in paths of at most `depth`, whose node 0 is
+        the last of `tokens`; the default looks for what followed when the last tokens came up before (lookup_drafts).
+        repetition, presence, frequency: sampling.adjust_logits' penalties for tokens of the prompt and those generated (a number, or one
+        per sequence); bias: (tokens, values, start [sequences + 1]); allowed: a mask [sequences, words] of int32, both as there."""
+        B, n = len(prompts), len(prompts[0]) if prompts else 0
+        if n == 0 or any(len(p) != n for p in prompts):
+            raise ValueError("prompts must be non-empty and of equal length")
+        if n + max_len - 1 > self.max_seq_len_:
+            raise ValueError("prompt + max_len exceeds max_seq_len")
+        if drafts < 0:
+            raise ValueError("drafts must not be negative")
+        if max_len <= 0:
+            return [list(p) for p in prompts]
+        draft = draft or (lambda tokens, most, depth: lookup_drafts(tokens, most, depth, branches))
+        self._setup_batch(B)
+        self.reset()
+        self._sampling = None
+        dev, self.drafted_steps_ = self.device, 0
+        with torch.cuda.device(dev):
+            def on_device(x, dtype):
+                return x if isinstance(x, torch.Tensor) else to_device(torch.as_tensor(np.asarray(x), dtype=dtype), dev)
+            per_seq = [x if isinstance(x, (int, float)) else on_device(x, torch.float32) for x in (repetition, presence, frequency)]
+            if bias is not None:
+                bias = [on_device(x, t) for x, t in zip(bias, (torch.int32, torch.float32, torch.int32))]
+            if allowed is not None:
+                allowed = on_device(allowed, torch.int32)
+            plain = all(isinstance(x, (int, float)) for x in per_seq) and (*per_seq,) == (1, 0, 0)
+            seqs = [np.asarray(p, dtype=np.int32) for p in prompts]
+            if n > 1:       # all but the last token of a prompt, which is the first pending one
+                self._prefill(to_device(torch.from_numpy(np.stack(seqs)[:, :-1].copy()), dev), head=False)
+            ctx = torch.full((B,), n - 1, dtype=torch.int32, device=dev)
+            caches, bufs = TreeCaches(self.kv_caches), None
+            while any(len(s) < n + max_len for s in seqs):
+                parents, tokens = [], []
+                for s in seqs:
+                    left, room = n + max_len - len(s), self.max_seq_len_ - len(s) + 1        # tokens to come; rows that the cache takes
+                    if left == 0:
+                        p, t = [], []           # this one is done
+                    elif left == 1 or drafts == 0:
+                        p, t = [-1], s[-1:]
+                    else:
+                        p, t = draft(s, min(1 + drafts, room), left)
+                        if not 1 <= len(p) <= min(1 + drafts, room) or len(t) != len(p) or int(t[0]) != int(s[-1]):
+                            raise ValueError("draft: between one and `most` nodes, the first of them the sequence's last token")
+                    parents.append(p)
+                    tokens.append(t)
+                tree = DraftTree(parents, tokens, dev)
+                if bufs is None or bufs.R < tree.rows:
+                    bufs = _Bufs(max(tree.rows, B * (1 + drafts)), self.hidden_dim_, self.inter_dim_, dev)
+                bf = bufs.first(tree.rows)
+                self._layers(bf, tree.tokens, tree.positions(ctx), ctx, tree.row_seq, None, tree=tree)
+                history = start = None
+                if not plain:       # the tokens before the pending one; a node's path counts by itself
+                    history = to_device(torch.from_numpy(np.concatenate([s[:-1] for s in seqs] + [np.zeros(1, np.int32)])), dev)
+                    start = to_device(torch.from_numpy(np.cumsum([0] + [len(s) - 1 for s in seqs], dtype=np.int32)), dev)
+                ids = sampling.adjusted_argmax(self._node_logits(bf), history, start, *per_seq, bias=bias, allowed=allowed,
+                                               allowed_rows=None if allowed is None else tree.row_seq, tree=tree)
+                done = tree_accept(ids, tree, caches, ctx)
+                ctx = done.ctx_lens
+                got = torch.cat((done.counts[:, None], done.tokens), 1).cpu().numpy()       # the step's synchronisation
+                seqs = [np.concatenate((s, g[1:1 + g[0]]))[:n + max_len] for s, g in zip(seqs, got)]
+                self.drafted_steps_ += 1
+            self.positions.copy_(ctx)
+            self.ctx_lens.copy_(ctx + 1)
+            self.ids.copy_(to_device(torch.from_numpy(np.array([s[-1] for s in seqs], dtype=np.int32)), dev))
+        return [s.tolist() for s in seqs]
 
     def forward_tokens(self, token_ids, temperature=1.0):
         """One eager decode step for `token_ids` ([B] ints) at the current positions: appends their K/V,
@@ -495,13 +582,25 @@ class CUDADecoder(_DecoderBase):
         B = self._batch
         if B <= 8 or getattr(self, "_sampling", None) is not None:
             return super()._head(x_rows)
+        self._linear_logits(self.bufs, x_rows, self.logits)
+        self._chk(self._lib.pa_argmax_f32(self.logits.data_ptr(), B, self.vocab_size_, self._temperature,
+                                          self.ARGMAX_DIVIDE, self.ids.data_ptr(), _cabi.stream()), "pa_argmax_f32")
+
+    def _linear_logits(self, bf, x_rows, logits):
         if getattr(self, "_emb_T", None) is None or self._emb_T.shape != (self.hidden_dim_, self.vocab_size_):
             self._emb_T = self.embedding.t().contiguous()
-        lib, s = self._lib, _cabi.stream()
-        wp, wb = self._scratch(self.bufs, lib.pa_linear_workspace_bytes(B, self.hidden_dim_, self.vocab_size_))
-        self._linear(x_rows, self._emb_T, None, B, self.hidden_dim_, self.vocab_size_, "", self.logits, wp, wb)
-        self._chk(lib.pa_argmax_f32(self.logits.data_ptr(), B, self.vocab_size_, self._temperature,
-                                    self.ARGMAX_DIVIDE, self.ids.data_ptr(), s), "pa_argmax_f32")
+        wp, wb = self._scratch(bf, self._lib.pa_linear_workspace_bytes(bf.R, self.hidden_dim_, self.vocab_size_))
+        self._linear(x_rows, self._emb_T, None, bf.R, self.hidden_dim_, self.vocab_size_, "", logits, wp, wb)
+
+    def _node_logits(self, bf):
+        """Logits [bf.R, vocab] of the hidden states in bf.x."""
+        logits = torch.empty((bf.R, self.vocab_size_), dtype=torch.float32, device=self.device)
+        if bf.R > 8:
+            self._linear_logits(bf, bf.x, logits)
+        else:
+            self._chk(self._lib.pa_logits_f32(bf.x.data_ptr(), self.embedding.data_ptr(), bf.R, self.hidden_dim_, self.vocab_size_,
+                                              logits.data_ptr(), _cabi.stream()), "pa_logits_f32")
+        return logits
 
     def _embed(self, bf, ids):
         self._chk(self._lib.pa_embedding_f32(self.embedding.data_ptr(), ids.data_ptr(), bf.R, self.hidden_dim_,
@@ -649,35 +748,49 @@ class INT8Decoder(_DecoderBase):
         B = self._batch
         if B < self.GEMM_LOGITS_MIN_ROWS:
             return super()._head(x_rows)
-        V, hid, dev = self.vocab_size_, self.hidden_dim_, self.device
-        Vp = (V + 15) // 16 * 16
+        V, Vp = self.vocab_size_, (self.vocab_size_ + 15) // 16 * 16
+        if getattr(self, "_logits_pad", None) is None or self._logits_pad.shape != (B, Vp):
+            self._logits_pad = torch.empty((B, Vp), dtype=torch.float32, device=self.device)
+        self._gemm_logits(self.bufs, x_rows, self._logits_pad)
+        self.logits = self._logits_pad[:, :V]
+        sp = getattr(self, "_sampling", None)
+        if sp is None:
+            self._chk(self._lib.pa_argmax_f32(self._logits_pad.data_ptr(), B, Vp, self._temperature, self.ARGMAX_DIVIDE,
+                                              self.ids.data_ptr(), _cabi.stream()), "pa_argmax_f32")
+            return
+        probs = sampling.softmax_temperature(self.logits.contiguous(), 1.0 / self._temperature)
+        sampling.apply_topk_topp_filter(probs, sp["top_k"], sp["top_p"], sp["eos_token_id"], sp["eos_thresh"])
+        u = torch.rand(B, device=self.device, generator=sp["generator"])
+        sampling.sample_from_probs(probs, u, out=self.ids)
+
+    def _gemm_logits(self, bf, x_rows, out):
+        """Logits of bf.R rows as an int8 GEMM -> out [bf.R, vocab rounded up to 16], -inf in the padding."""
+        V, Vp, hid, dev, lib, R = self.vocab_size_, out.shape[1], self.hidden_dim_, self.device, self._lib, bf.R
         if getattr(self, "_emb_T", None) is None or self._emb_T.shape != (hid, Vp):
             self._emb_T = torch.zeros((hid, Vp), dtype=torch.int8, device=dev)
             self._emb_T[:, :V] = self.embedding.t()
             self._pad_bias = torch.zeros(Vp, dtype=torch.float32, device=dev)
             self._pad_bias[V:] = float("-inf")  # padded columns never win the argmax
-        if getattr(self, "_logits_pad", None) is None or self._logits_pad.shape != (B, Vp):
-            self._logits_pad = torch.empty((B, Vp), dtype=torch.float32, device=dev)
-            self._lq = torch.empty((B, hid), dtype=torch.int8, device=dev)
-            self._ls = torch.empty(B, dtype=torch.float32, device=dev)
-        lib, s = self._lib, _cabi.stream()
-        self._quant_rows(x_rows, self._lq, self._ls, B, hid)
-        wp, wb = self._scratch(self.bufs, lib.pa_gemm_i8_workspace_bytes(1, B, Vp, hid))
-        self._chk(lib.pa_gemm_i8_dequant(self._lq.data_ptr(), self._emb_T.data_ptr(), self._logits_pad.data_ptr(), 1,
-                                         B, Vp, hid, self._ls.data_ptr(), 1.0 / float(self.emb_qscale),
-                                         self._pad_bias.data_ptr(), _cabi.ACT[""], wp, wb, s), "pa_gemm_i8_dequant")
-        self.logits = self._logits_pad[:, :V]
-        sp = getattr(self, "_sampling", None)
-        if sp is None:
-            self._chk(lib.pa_argmax_f32(self._logits_pad.data_ptr(), B, Vp, self._temperature, self.ARGMAX_DIVIDE,
-                                        self.ids.data_ptr(), s), "pa_argmax_f32")
-            return
-        from . import sampling
-        probs = sampling.softmax_temperature(self.logits.contiguous(), 1.0 / self._temperature)
-        sampling.apply_topk_topp_filter(probs, sp["top_k"], sp["top_p"], sp["eos_token_id"], sp["eos_thresh"])
-        u = torch.rand(B, device=dev, generator=sp["generator"])
-        sampling.sample_from_probs(probs, u, out=self.ids)
+        if getattr(bf, "lq", None) is None:
+            bf.lq = torch.empty((R, hid), dtype=torch.int8, device=dev)
+            bf.ls = torch.empty(R, dtype=torch.float32, device=dev)
+        self._quant_rows(x_rows, bf.lq, bf.ls, R, hid)
+        wp, wb = self._scratch(bf, lib.pa_gemm_i8_workspace_bytes(1, R, Vp, hid))
+        self._chk(lib.pa_gemm_i8_dequant(bf.lq.data_ptr(), self._emb_T.data_ptr(), out.data_ptr(), 1, R, Vp, hid, bf.ls.data_ptr(),
+                                         1.0 / float(self.emb_qscale), self._pad_bias.data_ptr(), _cabi.ACT[""], wp, wb,
+                                         _cabi.stream()), "pa_gemm_i8_dequant")
 
+    def _node_logits(self, bf):
+        """Logits [bf.R, vocab] of the hidden states in bf.x, computed as the decode steps of this batch compute theirs."""
+        V, dev = self.vocab_size_, self.device
+        if self._batch >= self.GEMM_LOGITS_MIN_ROWS:
+            logits = torch.empty((bf.R, (V + 15) // 16 * 16), dtype=torch.float32, device=dev)
+            self._gemm_logits(bf, bf.x, logits)
+            return logits[:, :V]
+        logits = torch.empty((bf.R, V), dtype=torch.float32, device=dev)
+        self._chk(self._lib.pa_logits_i8(bf.x.data_ptr(), self.embedding.data_ptr(), float(self.emb_qscale), bf.R, self.hidden_dim_, V,
+                                         logits.data_ptr(), _cabi.stream()), "pa_logits_i8")
+        return logits
     def _embed(self, bf, ids):
         self._chk(self._lib.pa_embedding_i8(self.embedding.data_ptr(), float(self.emb_qscale), ids.data_ptr(), bf.R,
                                             self.hidden_dim_, self.vocab_size_, bf.x.data_ptr(), _cabi.stream()),

@@ -78,16 +78,48 @@ class DraftTree:
         if tokens is not None:
             self.tokens, at = dev[at:at + R], at + R
         self.mask = dev[at:].view(R, words)
+        self._space = {}                # (heads, kv heads, D) -> bytes of workspace that pa_tree_attention wants for this tree
 
     def positions(self, ctx_lens):
         """Where the nodes' K/V rows go in the caches (`KVTileCache.append`): behind the context, in node order."""
         return ctx_lens[self.row_seq] + self.nodes
 
 
+def lookup_drafts(tokens, most, depth, branches=2, longest=3):
+    """A tree of guesses from the sequence itself: (parents, tokens) of at most `most` nodes in paths of at most `depth`, node 0 being the
+    last of `tokens`.  Where the last `longest` tokens (then one fewer, ... then the last one) came up before, what followed is a guess, the
+    latest first, up to `branches` of them; guesses that begin alike share their nodes."""
+    tokens = np.asarray(tokens)
+    parents, out, child, found = [-1], [int(tokens[-1])], {}, 0
+    before = tokens[:-1] == tokens[-1]          # the places of the last k tokens' ends
+    matches = [before]
+    for k in range(1, min(longest, len(tokens) - 1)):
+        before = before.copy()
+        before[:k] = False
+        before[k:] &= tokens[:-1 - k] == tokens[-1 - k]
+        matches.append(before)
+    for ends in reversed(matches):
+        for end in np.flatnonzero(ends)[::-1]:
+            node, new = 0, False
+            for t in tokens[end + 1:end + depth].tolist():
+                if (node, t) not in child:
+                    if len(out) >= most:
+                        break
+                    child[node, t] = len(out)
+                    parents.append(node)
+                    out.append(t)
+                    new = True
+                node = child[node, t]
+            found += new
+            if found == branches or len(out) >= most:
+                return parents, out
+    return parents, out
+
+
 def _vector(x, n, device, what):
     if not isinstance(x, torch.Tensor):
         x = to_device(torch.as_tensor(np.asarray(x), dtype=torch.int32), device)
-    if x.dtype != torch.int32 or x.dim() != 1 or x.numel() != n or x.device != device or not x.is_contiguous():
+    if x.dtype is not torch.int32 or x.shape != (n,) or x.device != device or not x.is_contiguous():
         raise ValueError(f"{what}: a contiguous int32 vector of {n} on {device}")
     return x
 
@@ -110,7 +142,7 @@ def paged_tree_attention(q, kv_cache, tree, ctx_lens, temperature=1.0, beam_ids=
     if not temperature:
         raise ValueError("paged_tree_attention: temperature 0")
     R, H = tree.rows, q.shape[1]
-    if R and (q.stride(2) != 1 or q.stride(1) != D or (R > 1 and q.stride(0) < H * D)):
+    if not q.is_contiguous() and (q.stride(2) != 1 or q.stride(1) != D or (R > 1 and q.stride(0) < H * D)):
         q = q.contiguous()
     if out is None:
         out = torch.empty((R, H, D), dtype=q.dtype, device=dev)
@@ -125,7 +157,9 @@ def paged_tree_attention(q, kv_cache, tree, ctx_lens, temperature=1.0, beam_ids=
     table = pt.device_data()
     with _cabi.on_device(dev):
         stream = _cabi.stream()
-        need = lib.pa_tree_attention_workspace_bytes(R, tree.num_seqs, tree.most, H, KVH, D)
+        need = tree._space.get((H, KVH, D))
+        if need is None:
+            need = tree._space[(H, KVH, D)] = lib.pa_tree_attention_workspace_bytes(R, tree.num_seqs, tree.most, H, KVH, D)
         ws = kv_cache._ws.get(("tree", stream))
         if need and (ws is None or ws.numel() < need):
             ws = kv_cache._ws[("tree", stream)] = torch.empty(need, dtype=torch.uint8, device=dev)
@@ -184,9 +218,7 @@ def tree_accept(ids, tree, caches, ctx_lens, beam_ids=None):
     ctx_lens = _vector(ctx_lens, B, dev, "ctx_lens")
     if beam_ids is not None:
         beam_ids = _vector(beam_ids, B, dev, "beam_ids")
-    out = torch.empty(2 * B + 2 * B * tree.depth, dtype=torch.int32, device=dev)
-    counts, lens = out[:B], out[B:2 * B]
-    tokens, nodes = out[2 * B:].view(2, B, tree.depth)
+    (counts, lens), (tokens, nodes) = (torch.empty(s, dtype=torch.int32, device=dev).unbind(0) for s in ((2, B), (2, B, tree.depth)))
     if B == 0:
         return Accepted(counts, tokens, nodes, lens)
     if tree.rows == 0:
