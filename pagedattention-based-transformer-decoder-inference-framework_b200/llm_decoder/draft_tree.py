@@ -160,9 +160,12 @@ def paged_tree_attention(q, kv_cache, tree, ctx_lens, temperature=1.0, beam_ids=
         need = tree._space.get((H, KVH, D))
         if need is None:
             need = tree._space[(H, KVH, D)] = lib.pa_tree_attention_workspace_bytes(R, tree.num_seqs, tree.most, H, KVH, D)
-        ws = kv_cache._ws.get(("tree", stream))
-        if need and (ws is None or ws.numel() < need):
-            ws = kv_cache._ws[("tree", stream)] = torch.empty(need, dtype=torch.uint8, device=dev)
+        if torch._C._cuda_isCurrentStreamCapturing():           # a graph has a workspace of its own: its replays may run beside other calls
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        else:
+            ws = kv_cache._ws.get(("tree", stream))
+            if need and (ws is None or ws.numel() < need):
+                ws = kv_cache._ws[("tree", stream)] = torch.empty(need, dtype=torch.uint8, device=dev)
         _cabi.check(lib.pa_tree_attention(
             q.data_ptr(), q.stride(0) if R > 1 else H * D, TYPES[q.dtype], out.data_ptr(), kv_cache.key_buffer_.data_ptr(),
             kv_cache.value_buffer_.data_ptr(), _cabi.ptr(kv_cache.k_scales_), _cabi.ptr(kv_cache.v_scales_),

@@ -79,41 +79,46 @@ def sample(logits, temperature=1.0, top_k=0, top_p=1.0, eos_token_id=-1, eos_thr
     return sample_from_probs(probs, u)
 
 
+_LOGIT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # PA_TYPE_*
 _rule_words = {}        # (device, stream) -> workspace of pa_adjust_logits
 
 
 def _rules(logits, out, ids, history, history_start, repetition, presence, frequency, bias, allowed, allowed_rows, row_seq, tree):
-    dev, types = logits.device, {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    if logits.dim() != 2 or logits.dtype not in types or not logits.is_cuda:
+    dev, at, kind = logits.device, logits.get_device(), _LOGIT_TYPES.get(logits.dtype)
+    if logits.dim() != 2 or kind is None or not logits.is_cuda:
         raise ValueError("logits: [rows, vocab] of float32, float16 or bfloat16 on the GPU")
-    rows, V = logits.shape
-    if V == 0 or (rows and (logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < V))):
+    (rows, V), (stride, one) = logits.shape, logits.stride()
+    if V == 0 or (rows and (one != 1 or (rows > 1 and stride < V))):
         raise ValueError("logits: a vocabulary, and rows of consecutive elements that do not overlap")
     if (history is None) != (history_start is None):
         raise ValueError("history and history_start come together")
 
     def of(x, dtype, what, n=None):
-        if not isinstance(x, torch.Tensor) or x.dtype is not dtype or x.device != dev or x.dim() != 1 or not x.is_contiguous() or \
+        """The address of a vector."""
+        if not isinstance(x, torch.Tensor) or x.dtype is not dtype or x.get_device() != at or x.dim() != 1 or not x.is_contiguous() or \
                 (n is not None and len(x) != n):
             raise ValueError(f"{what}: a contiguous {dtype} vector{'' if n is None else f' of {n}'} on {dev}")
-        return x
+        return x.data_ptr()
+    i32, f32, p_seq, p_history, p_start, p_ids, p_val, p_bias, p_rows = torch.int32, torch.float32, None, None, None, None, None, None, None
+    paths = (None, None, 0, None)
     if tree is not None:
         if tree.tokens is None or tree.rows != rows or tree.device != dev or row_seq is not None:
             raise ValueError("tree: one with tokens, a node for every row, on the logits' device (and then no row_seq)")
-        seqs, row_seq = tree.num_seqs, tree.row_seq
+        seqs, p_seq = tree.num_seqs, tree.row_seq.data_ptr()
+        paths = (tree.tokens.data_ptr(), tree.mask.data_ptr(), tree.mask.shape[1], tree.node_start.data_ptr())
     elif row_seq is not None:
-        of(row_seq, torch.int32, "row_seq", rows)
+        p_seq = of(row_seq, i32, "row_seq", rows)
         seqs = None             # as many as the other arguments say
     else:
         seqs = rows
     if history is not None:
-        of(history, torch.int32, "history")
-        of(history_start, torch.int32, "history_start", None if seqs is None else seqs + 1)
-        seqs = history_start.numel() - 1
+        p_history = of(history, i32, "history")
+        p_start = of(history_start, i32, "history_start", None if seqs is None else seqs + 1)
+        seqs = len(history_start) - 1
     arrays, values = [], []
     for x, what in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")):
         if isinstance(x, torch.Tensor):
-            arrays.append(of(x, torch.float32, what, seqs).data_ptr())
+            arrays.append(of(x, f32, what, seqs))
             seqs = len(x)
             values.append(0.0)
         else:
@@ -121,18 +126,16 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
             values.append(float(x))
     if arrays[0] is None and not values[0] > 0:
         raise ValueError("repetition: above 0 (1 changes nothing)")
-    b_ids = b_val = b_start = None
     if bias is not None:
         b_ids, b_val, b_start = bias
-        of(b_ids, torch.int32, "bias tokens")
-        of(b_val, torch.float32, "bias values", b_ids.numel())
-        of(b_start, torch.int32, "bias starts", None if seqs is None else seqs + 1)
+        p_ids, p_val = of(b_ids, i32, "bias tokens"), of(b_val, f32, "bias values", len(b_ids))
+        p_bias = of(b_start, i32, "bias starts", None if seqs is None else seqs + 1)
     if allowed is not None:
         if allowed.dim() != 2 or allowed.dtype != torch.int32 or allowed.device != dev or allowed.shape[1] * 32 < V or \
                 (allowed.numel() and allowed.stride(1) != 1) or (allowed_rows is None and allowed.shape[0] != rows):
             raise ValueError("allowed: int32 [rows, words], 32 tokens a word, the logits' vocabulary")
         if allowed_rows is not None:
-            of(allowed_rows, torch.int32, "allowed_rows", rows)
+            p_rows = of(allowed_rows, i32, "allowed_rows", rows)
     if rows == 0:
         return
     lib = _cabi.lib()
@@ -140,17 +143,18 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
         stream, ws, need = _cabi.stream(), None, 0
         if ids is not None:     # words that every call leaves at zero, one buffer per stream
             need = lib.pa_adjust_logits_workspace_bytes(rows)
-            ws = _rule_words.get((dev.index, stream))
-            if ws is None or ws.numel() < need:
-                ws = _rule_words[(dev.index, stream)] = torch.zeros(max(need, 1 << 14), dtype=torch.uint8, device=dev)
+            if torch._C._cuda_isCurrentStreamCapturing():       # a graph has words of its own: its replays may run beside other calls
+                ws = torch.zeros(need, dtype=torch.uint8, device=dev)
+            else:
+                ws = _rule_words.get((dev.index, stream))
+                if ws is None or ws.numel() < need:
+                    ws = _rule_words[(dev.index, stream)] = torch.zeros(max(need, 1 << 14), dtype=torch.uint8, device=dev)
         # (the stride of a single row may be anything)
         _cabi.check(lib.pa_adjust_logits(
-            logits.data_ptr(), types[logits.dtype], logits.stride(0) if rows > 1 else V, rows, V, _cabi.ptr(out),
-            0 if out is None else out.stride(0) if rows > 1 else V, _cabi.ptr(ids), _cabi.ptr(row_seq), _cabi.ptr(history), _cabi.ptr(history_start),
-            *arrays, *values, _cabi.ptr(b_ids), _cabi.ptr(b_val), _cabi.ptr(b_start), _cabi.ptr(allowed),
-            0 if allowed is None else allowed.stride(0) if allowed.shape[0] > 1 else allowed.shape[1], _cabi.ptr(allowed_rows),
-            *((tree.tokens.data_ptr(), tree.mask.data_ptr(), tree.mask.shape[1], tree.node_start.data_ptr()) if tree is not None else
-              (None, None, 0, None)), _cabi.ptr(ws), need, stream), "pa_adjust_logits")
+            logits.data_ptr(), kind, stride if rows > 1 else V, rows, V, _cabi.ptr(out), 0 if out is None else out.stride(0) if rows > 1 else V,
+            _cabi.ptr(ids), p_seq, p_history, p_start, *arrays, *values, p_ids, p_val, p_bias, _cabi.ptr(allowed),
+            0 if allowed is None else allowed.stride(0) if allowed.shape[0] > 1 else allowed.shape[1], p_rows, *paths, _cabi.ptr(ws), need,
+            stream), "pa_adjust_logits")
 
 
 def adjust_logits(logits, history=None, history_start=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None,

@@ -145,3 +145,47 @@ def test_refusals(tmp_path):
             dec.generate_drafted(*args, **kw)
     assert dec.generate_drafted([[1, 2, 3]], 0) == [[1, 2, 3]]
     assert dec.generate_drafted([[1, 2, 3]], 30) == dec.generate_drafted([[1, 2, 3]], 30, drafts=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pool", ["f16", "i8"])
+def test_the_step_replays_as_a_graph(pool):
+    """Attention, rules and acceptance in a graph, replayed next to launched calls on the stream of the capture: equal bits."""
+    import llm_decoder as ld
+    rng = np.random.default_rng(12)
+    B, H, D, V, tile = 3, 4, 128, 1000, 16
+    dev = torch.device("cuda", torch.cuda.current_device())
+    kv = ld.KVTileCache(pool, device=dev)
+    kv.init(B * H * 40, tile, D)
+    kv.configure_table(B, H, 40)
+    kv.page_table_.load_host_table(rng.permutation(B * H * 40).astype(np.int32).reshape(B, H, 40))
+    lens = [600, 30, 0]
+    for b, n in enumerate(lens):
+        x = torch.from_numpy(rng.standard_normal((max(n, 1) + 20, H, D)).astype(np.float32)).to(dev)
+        kv.append(x, -x, torch.arange(len(x), dtype=torch.int32, device=dev), torch.full((len(x),), b, dtype=torch.int32, device=dev))
+    tokens = [rng.integers(0, V, n).tolist() for n in (18, 5, 20)]
+    tree = ld.DraftTree([[-1] + [int(rng.integers(0, i)) for i in range(1, len(t))] for t in tokens], tokens, dev)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=dev)
+    q = torch.from_numpy(rng.standard_normal((tree.rows, H, D)).astype(np.float32)).to(dev)
+    logits = torch.from_numpy(rng.standard_normal((tree.rows, V)).astype(np.float32)).to(dev)
+    history = torch.from_numpy(rng.integers(0, V, 90).astype(np.int32)).to(dev)
+    start = torch.tensor([0, 40, 40, 90], dtype=torch.int32, device=dev)
+
+    def step():
+        return (ld.paged_tree_attention(q, kv, tree, ctx), ld.sampling.adjusted_argmax(logits, history, start, 1.3, 0.2, 0.1, tree=tree))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        want = [x.clone() for x in step()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = step()
+    for _ in range(3):
+        graph.replay()
+        with torch.cuda.stream(side):
+            launched = step()
+        torch.cuda.synchronize()
+        for w, g, x in zip(want, got, launched):
+            assert torch.equal(w, g) and torch.equal(w, x)
+            g.zero_()
