@@ -30,21 +30,29 @@ __device__ int g_errors;
 __host__ __device__ constexpr int q_bytes(int D) { return D * QT * 2; }
 // the ring: tiles of keys and of values, each of 64 rows
 __host__ __device__ constexpr int tile_bytes(int D) { return D * KT * 2; }
-__host__ __device__ constexpr int ring_for(int D, int nq) { return nq == 2 ? (D == 128 ? 9 : 18) : D == 128 ? 4 : 10; }
+__host__ __device__ constexpr int ring_for(int D, int nq) { return nq == 2 ? (D == 128 ? 8 : 18) : D == 128 ? 4 : 10; }
 constexpr int kNotes = 32;              // of the producer on its tiles; more than it can be ahead
 __host__ __device__ constexpr int threads_for(int nq) { return (5 * nq + 1) * 32; }
 // full, empty [ring]; per query tile s_full, p_full, o_full [2], q_ready
 __host__ __device__ constexpr int nbar_for(int D, int nq) { return 2 * ring_for(D, nq) + 7 * nq; }
+constexpr int kStage = 2048;            // of a warp: 32 columns of its rows' results
 constexpr size_t smem_for(int D, int nq, int seqs) {
-    return (size_t)nq * q_bytes(D) + ring_for(D, nq) * tile_bytes(D) + nbar_for(D, nq) * 8 + 64 + kNotes * 4 + (seqs + 1) * 4 + 1024;
+    return (size_t)nq * q_bytes(D) + ring_for(D, nq) * tile_bytes(D) + nq * 4 * kStage + nbar_for(D, nq) * 8 + 64 + kNotes * 4 + (seqs + 1) * 4 + 1024;
 }
 
 template <bool BF> struct Elem { typedef __half T; };
 template <> struct Elem<true> { typedef bf16_t T; };
 
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map),
+                 "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+
+// q_boxes: tmQ has boxes of a query tile, else the softmax warps gather its rows
 template <int D, int NQ, bool BF>
 __global__ void __launch_bounds__(threads_for(NQ), NQ == 1 ? 2 : 1)
-tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeWork a) {
+tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmQ,
+               const bool q_boxes, const TreeWork a) {
     typedef typename Elem<BF>::T T;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     constexpr int RING = ring_for(D, NQ), NBAR = nbar_for(D, NQ), TMEM_COLS = NQ * 256, KB = D / 64;
@@ -52,7 +60,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     constexpr int W_MMA = 4 * NQ, W_PROD = 5 * NQ;
     const TreeParams& p = a.p;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t kv_sm = base + NQ * Q_BYTES, bar0 = kv_sm + RING * TILE;
+    const uint32_t kv_sm = base + NQ * Q_BYTES, stage_sm = kv_sm + RING * TILE, bar0 = stage_sm + NQ * 4 * kStage;
     auto kv_full = [&](int s) { return bar0 + s * 8; };
     auto kv_empty = [&](int s) { return bar0 + (RING + s) * 8; };
     auto s_full = [&](int x, int i) { return bar0 + (2 * RING + 7 * x + i) * 8; };
@@ -100,8 +108,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     auto v_at = [&](uint32_t at, int i, int nt) { return at + (uint32_t)(i + 1 < nt ? 2 * i + 2 : 2 * nt - 1); };
     auto slot_of = [&](uint32_t c) { return (int)(c % RING); };
     auto phase_of = [&](uint32_t c) { return c / RING & 1u; };
-    // which query tiles of the piece have rows
-    auto has_rows = [&](int x) { return w.rr0 + x * QT < w.sq.n * G; };
+    // which query tiles of a piece have rows
+    auto rows_of = [&](const TreeWalk& piece, int x) { return piece.rr0 + x * QT < piece.sq.n * G; };
+    auto has_rows = [&](int x) { return rows_of(w, x); };
 
     if (warp == W_PROD) {
         uint32_t c = 0, tiles = 0;          // requests and tiles of keys so far
@@ -149,10 +158,26 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     } else if (warp >= W_MMA) {
         constexpr uint32_t kIdescS = idesc_f16(QT, KT, 0, 0, BF), kIdescO = idesc_f16(QT, D, 0, 1, BF);
         const int x = warp - W_MMA;
-        int n = 0, qn = 0;                  // key tiles and pieces of this query tile so far
+        int n = 0, qn = 0, asked = 0;       // key tiles and pieces of this query tile so far; its boxes asked for
         uint32_t at = 0;
+        // the queries of the piece after this one, as soon as the products with this one's are done; rows behind the sequence's are others' or
+        // zeros, and nobody looks at what becomes of them
+        TreeWalk ahead(a, pre);
+        auto fetch_q = [&] {
+            if (!q_boxes || !ahead.next() || !rows_of(ahead, x) || __any_sync(0xffffffffu, failed())) return;
+            ++asked;
+            if (elect_one()) {
+                mbar_arrive_expect_tx(q_ready(x), Q_BYTES);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+                    tma_load_3d(base + x * Q_BYTES + kb * (QT * 128), &tmQ, kb * 64, ahead.g * G, ahead.sq.r0 + (ahead.rr0 + x * QT) / G, q_ready(x));
+            }
+            __syncwarp();
+        };
+        fetch_q();
         while (w.next()) {
             const bool mine = has_rows(x);
+            if (!mine) fetch_q();
             auto issue_S = [&](int i) {     // every issuer waits for every tile: its arrival at the empty barrier belongs to THIS use of it
                 const int s = slot_of(k_at(at, i));
                 wait(kv_full(s), phase_of(k_at(at, i)));
@@ -209,6 +234,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 }
                 if (elect_one()) umma_commit(kv_empty(s));
                 __syncwarp();
+                if (mine && i + 1 == nt) fetch_q();         // (its scores were read: the products with the queries are done)
             }
             at += 2 * nt;
             if (mine) {
@@ -216,6 +242,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 ++qn;
             }
         }
+        if (failed() && asked > 0) tc_let_land(q_ready(x), (uint32_t)(asked - 1) & 1u);
     } else {
         // ---- softmax: one thread per query row
         const int x = warp >> 2, qtr = warp & 3, row_in_block = x * QT + qtr * 32;
@@ -243,7 +270,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             }
             const int rr = w.rr0 + row_in_block + lane, rows = min(32, all - w.rr0 - row_in_block);       // rows of this warp, may be negative
             const int div = rr / G, node = rr < all ? div : -1, head = w.g * G + rr - div * G;
-            if (rows > 0) {
+            if (!q_boxes && rows > 0) {
                 // the warp's query rows into the swizzled K-major A tile, whose last products this thread has seen complete
                 const uint32_t qx = base + x * Q_BYTES;
                 constexpr int CH = D / 8, PER = 8;      // 16-byte pieces of a row; loads in flight per lane
@@ -266,9 +293,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                     }
                 }
             }
-            fence_proxy_async();
-            group_sync();
-            if (qtr == 0 && lane == 0) mbar_arrive_cnt(q_ready(x));
+            if (!q_boxes) {
+                fence_proxy_async();
+                group_sync();
+                if (qtr == 0 && lane == 0) mbar_arrive_cnt(q_ready(x));
+            }
             const uint32_t* mask = p.mask + (int64_t)(w.sq.r0 + max(node, 0)) * p.mask_words;
             float m_ref = -INFINITY, l_run = 0.f;
             bool odd = false;
@@ -402,18 +431,23 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 continue;
             }
             if (rows <= 0) continue;
-            // every thread writes its own row: the stores leave while the next piece's scores come
+            // a share's own piece: every thread its row; a whole item: 32 columns of the warp's rows at a time through shared memory, so that
+            // four lanes write 64 bytes of a row (each lane its own row: 32 half sectors a store, half of a short piece's time)
             float inv = 1.f / (l_run + 1e-6f * 128.f);
             if (m_ref == -INFINITY) inv = 0.f;              // saw nothing
             if (failed()) inv = m_ref = l_run = __int_as_float(0x7fc00000);
-            T* out = static_cast<T*>(p.out) + ((int64_t)(w.sq.r0 + max(node, 0)) * p.heads + head) * D;
+            const int64_t own_row = node >= 0 ? ((int64_t)(w.sq.r0 + node) * p.heads + head) * D : -1;
+            int64_t out_row[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out_row[j] = __shfl_sync(0xffffffffu, own_row, 8 * j + (lane >> 2));
+            const uint32_t stage = stage_sm + warp * kStage;
             float* part = a.part + (w.slot * a.block + row_in_block + lane) * (D + 4);
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
                 uint32_t o[32];
                 tmem_ld32(o_addr + c0, o);
                 tmem_wait_ld();
-                if (node >= 0 && w.slot < 0) {
+                if (w.slot < 0) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t v[4];
@@ -424,7 +458,15 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                             if constexpr (BF) v[e] = pack_bf16x2(lo, hi);
                             else v[e] = pack_half2(lo, hi);
                         }
-                        reinterpret_cast<uint4*>(out + c0)[j] = make_uint4(v[0], v[1], v[2], v[3]);
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)), "r"(v[0]), "r"(v[1]),
+                                     "r"(v[2]), "r"(v[3]) : "memory");
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = 8 * j + (lane >> 2);
+                        const uint4 v = lds_128(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4));
+                        if (out_row[j] >= 0) reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row[j] + c0)[lane & 3] = v;
                     }
                 } else if (node >= 0) {
                     const float k = a.p_scale / 128.f;
@@ -454,6 +496,16 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     }
 }
 
+// [rows][heads][dim], box = (128 / G) rows x G heads x 64 columns
+static bool make_q_map(CUtensorMap* map, const TreeParams& p, int G) {
+    EncodeTiledFnG fn = encode_fn_g();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)p.dim, (cuuint64_t)p.heads, (cuuint64_t)p.rows}, strides[2] = {(cuuint64_t)p.dim * 2, (cuuint64_t)p.q_stride * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(QT / G)}, estr[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, int NQ, bool BF>
 static int launch(const TreeWork& a, cudaStream_t st) {
     const TreeParams& p = a.p;
@@ -462,9 +514,12 @@ static int launch(const TreeWork& a, cudaStream_t st) {
     auto kern = tree_tc_kernel<D, NQ, BF>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    CUtensorMap k, v;                   // boxes move bits: one map type for both 16-bit types
+    CUtensorMap k, v, q{};              // boxes move bits: one map type for both 16-bit types
     if (!make_bf16_map(&k, p.k, a.total_rows, D, D, 16) || !make_bf16_map(&v, p.v, a.total_rows, D, D, 16)) return PA_ERR_UNSUPPORTED;
-    kern<<<a.workers, threads_for(NQ), smem, st>>>(k, v, a);
+    // queries: boxes of 128 rows = 128 / G nodes' heads of a group
+    const int G = p.heads / p.kv_heads;
+    const bool q_boxes = QT % G == 0 && make_q_map(&q, p, G);
+    kern<<<a.workers, threads_for(NQ), smem, st>>>(k, v, q, q_boxes, a);
     PA_RETURN_LAUNCH_STATUS();
 }
 
