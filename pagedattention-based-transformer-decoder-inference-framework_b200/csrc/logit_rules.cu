@@ -97,8 +97,7 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // ---- bounds and bits that nothing waits for yet
     const int b = a.row_seq ? __ldg(a.row_seq + r) : r;
-    int h0 = 0, h1 = 0, i0 = 0, i1 = 0, s0 = 0;
-    uint32_t way = 0;
+    int h0 = 0, h1 = 0, i0 = 0, i1 = 0, s0 = 0, s1 = 0;
     if (a.history) {
         h0 = __ldg(a.history_start + b);
         h1 = __ldg(a.history_start + b + 1);
@@ -107,9 +106,9 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
         i0 = __ldg(a.bias_start + b);
         i1 = __ldg(a.bias_start + b + 1);
     }
-    if (a.tokens) {             // thread j has word j of the node's way
+    if (a.tokens) {
         s0 = __ldg(a.node_start + b);
-        way = tid < a.path_words ? __ldg(a.path + (int64_t)r * a.path_words + tid) : 0u;
+        s1 = min(__ldg(a.node_start + b + 1), s0 + 32 * a.path_words);
     }
     const int64_t mrow = a.allowed_rows ? __ldg(a.allowed_rows + r) : r;
     const uint32_t* allowed = a.allowed && mrow >= 0 ? a.allowed + mrow * a.allowed_stride + (v0 >> 5) : nullptr;
@@ -156,7 +155,8 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
             }
         }
     }
-    for (uint32_t m = way; m; m &= m - 1) add(__ldg(a.tokens + s0 + tid * 32 + __ffs(m) - 1));
+    for (int j = tid; j < s1 - s0; j += kThreads)       // thread j has node j
+        if (__ldg(a.path + (int64_t)r * a.path_words + (j >> 5)) >> (j & 31) & 1u) add(__ldg(a.tokens + s0 + j));
     if (a.bias) {
         if (a.history || a.tokens) __syncthreads();     // a token is noted once
         for (int i = i0 + tid; i < i1; i += kThreads) {

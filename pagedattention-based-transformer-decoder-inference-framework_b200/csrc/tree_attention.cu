@@ -124,7 +124,7 @@ PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void
     if (most_nodes > PA_TREE_MOST_NODES || !pair) return PA_ERR_UNSUPPORTED;
     const TreeParams p{d_q, q_stride, d_out, d_k_pool, d_v_pool, d_k_scales, d_v_scales, d_table, d_beam_ids, d_ctx_lens, d_node_start,
                        reinterpret_cast<const uint32_t*>(d_mask), q_type, kv_type, num_beams, kv_heads, num_tiles, total_pages, mask_words,
-                       rows, num_seqs, most_nodes, heads, head_dim, tile_size, temperature};
+                       rows, num_seqs, most_nodes, heads, head_dim, tile_size, temperature, heads / kv_heads};
     cudaStream_t st = as_stream(stream);
     struct Form {
         int block, workers, unit;

@@ -25,6 +25,7 @@ struct TreeParams {
     const uint32_t* mask;           // [rows, mask_words]
     int q_type, kv_type, num_beams, kv_heads, num_tiles, total_pages, mask_words, rows, num_seqs, most, heads, dim, tile_size;
     float temperature;
+    int group;                      // heads / kv_heads
 };
 
 template <typename T> __device__ __forceinline__ float tree_widen(T v) { return (float)v; }
@@ -60,8 +61,8 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b, int bloc
     s.ctx = max(__ldg(p.ctx_lens + b), 0);
     const int64_t cap = min((int64_t)p.num_tiles * p.tile_size, (int64_t)0x7fffff00);
     s.keys = s.n > 0 ? (int)min((int64_t)s.ctx + s.n, cap) : 0;
-    s.blocks = (s.n * (p.heads / p.kv_heads) + block - 1) / block;
-    s.steps = (s.keys + unit - 1) / unit;
+    s.blocks = (s.n * p.group + block - 1) >> (31 - __clz(block));      // powers of two, both
+    s.steps = (s.keys + unit - 1) >> (31 - __clz(unit));
     return s;
 }
 // Bits 0 .. width - 1: which of the keys at ctx + off .. a row sees (off < 0: the first -off are context).  word: of the row's mask
@@ -100,7 +101,7 @@ static inline size_t tree_work_bytes(int num_seqs, int workers, int block, int d
 __device__ __forceinline__ TreeNote tree_note(const TreeWork& a, const TreeSeq& s, int g, int rr0, int i0, int i1, int64_t f_item, int64_t total, int64_t ns, int64_t slot) {
     TreeNote t{};
     if (i0 == 0 && i1 < s.steps) {
-        t.rows = min(a.block, s.n * (a.p.heads / a.p.kv_heads) - rr0);
+        t.rows = min(a.block, s.n * a.p.group - rr0);
         t.first_row = s.r0;
         t.g = g;
         t.rr0 = rr0;

@@ -5,7 +5,8 @@
 
 namespace pa {
 
-// Pieces of a CTA's share, in order.  Every role walks them for itself.
+// Pieces of a CTA's share, in order.  Every role walks them for itself, from the first one, which is found before the roles part: that takes
+// divisions, and the roles' instructions share the SM's caches.
 struct TreeWalk {
     const TreeWork& a;
     const int* pre;
@@ -13,36 +14,37 @@ struct TreeWalk {
     int b, rb;                          // sequence, block within the kv head
     TreeSeq sq;
     int g, rr0, i0, i1;                 // the piece: kv head, first row, steps [i0, i1)
+    bool first;
     int64_t slot;                       // of its partial sums, -1: it is a whole item
     int64_t f_lo, total, ns;
-    __device__ __forceinline__ TreeWalk(const TreeWork& w, const int* pre_) : a(w), pre(pre_), b(-1) {
+    __device__ __forceinline__ TreeWalk(const TreeWork& w, const int* pre_) : a(w), pre(pre_), first(true) {
         total = (int64_t)pre[w.p.num_seqs] * w.p.kv_heads;
         ns = shares::count(total, w.workers, w.least);
         f_lo = f = blockIdx.x < ns ? total * blockIdx.x / ns : 0;
         f_hi = blockIdx.x < ns ? total * (blockIdx.x + 1) / ns : 0;
+        if (f >= f_hi) return;
+        b = shares::find_token(pre, w.p.num_seqs, f, w.p.kv_heads);
+        sq = tree_seq(w.p, b, w.block, w.unit);
+        const int64_t rem = f - (int64_t)pre[b] * w.p.kv_heads;
+        const int item = (int)(rem / sq.steps);
+        i0 = (int)(rem - (int64_t)item * sq.steps);
+        g = item / sq.blocks;
+        rb = item - g * sq.blocks;
     }
     __device__ __forceinline__ bool next() {
         if (f >= f_hi) return false;
-        const TreeParams& p = a.p;
-        if (b < 0) {                        // the first piece may begin anywhere; the ones behind it begin their items, without a division
-            b = shares::find_token(pre, p.num_seqs, f, p.kv_heads);
-            sq = tree_seq(p, b, a.block, a.unit);
-            const int64_t rem = f - (int64_t)pre[b] * p.kv_heads;
-            const int item = (int)(rem / sq.steps);
-            i0 = (int)(rem - (int64_t)item * sq.steps);
-            g = item / sq.blocks;
-            rb = item - g * sq.blocks;
-        } else {
+        if (!first) {                       // the pieces behind the first begin their items
             i0 = 0;
             if (++rb == sq.blocks) {
                 rb = 0;
-                if (++g == p.kv_heads) {
+                if (++g == a.p.kv_heads) {
                     g = 0;
                     do ++b; while (pre[b + 1] == pre[b]);       // a sequence without nodes has no items
-                    sq = tree_seq(p, b, a.block, a.unit);
+                    sq = tree_seq(a.p, b, a.block, a.unit);
                 }
             }
         }
+        first = false;
         rr0 = rb * a.block;
         const int64_t left = f_hi - f;
         i1 = left < sq.steps - i0 ? i0 + (int)left : sq.steps;
@@ -102,7 +104,7 @@ template <int D, typename Q, typename KV>
 __device__ __noinline__ void tree_piece_by_rows(const TreeWork& a, const TreeWalk& w, int row_in_block, int rows) {
     constexpr int NC = D / 32;
     const TreeParams& p = a.p;
-    const int lane = threadIdx.x & 31, G = p.heads / p.kv_heads;
+    const int lane = threadIdx.x & 31, G = p.group;
     const int trow = p.beam_ids ? __ldg(p.beam_ids + w.b) : w.b;
     const float fe = 1.4426950408889634f / p.temperature;
     for (int x = 0; x < rows; ++x) {

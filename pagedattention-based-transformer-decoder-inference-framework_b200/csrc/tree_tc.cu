@@ -72,7 +72,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     auto failed = [&] { return tc_failed(fail_sm); };
     auto wait = [&](uint32_t bar, uint32_t parity) { tc_wait(bar, parity, fail_sm, a.polls); };
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.heads / p.kv_heads;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group;
     if (threadIdx.x == 0) {
         for (int s = 0; s < RING; ++s) {
             mbar_init(kv_full(s), 1);
@@ -162,7 +162,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         uint32_t at = 0;
         // the queries of the piece after this one, as soon as the products with this one's are done; rows behind the sequence's are others' or
         // zeros, and nobody looks at what becomes of them
-        TreeWalk ahead(a, pre);
+        TreeWalk ahead = w;
         auto fetch_q = [&] {
             if (!q_boxes || !ahead.next() || !rows_of(ahead, x) || __any_sync(0xffffffffu, failed())) return;
             ++asked;

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
     auto failed = [&] { return tc_failed(fail_sm); };
     auto wait = [&](uint32_t bar, uint32_t parity) { tc_wait(bar, parity, fail_sm, a.polls); };
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.heads / p.kv_heads;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group;
     if (threadIdx.x == 0) {
         for (int s = 0; s < RING; ++s) {
             mbar_init(kv_full(s), I8 ? 33 : 1);     // int8: a warp's copies of scales, too
