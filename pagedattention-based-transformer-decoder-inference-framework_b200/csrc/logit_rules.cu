@@ -18,6 +18,7 @@
 // one does that, held every CTA's place for two trips to L2 more: 61 us for 256 x 128000 logits.)
 #include <type_traits>
 
+#include "dynamic_smem.cuh"
 #include "seq_common.cuh"
 
 namespace pa {
@@ -332,7 +333,7 @@ static int launch(Args a, cudaStream_t st) {
     const int64_t ctas = (int64_t)a.rows * a.chunks;
     if (ctas > 0x7fffffff) return PA_ERR_UNSUPPORTED;
     const size_t smem = shared_bytes<T>(a);
-    cudaError_t e = cudaFuncSetAttribute(rules_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = allow_dynamic_smem<rules_kernel<T>>(smem);
     if (e != cudaSuccess) return (int)e;
     rules_kernel<T><<<(unsigned)ctas, kThreads, smem, st>>>(a);
     e = cudaGetLastError();

@@ -10,6 +10,7 @@
 // is the beginning of its share, in slot 2 w.
 #pragma once
 #include "decode_shares.cuh"
+#include "dynamic_smem.cuh"
 #include "seq_common.cuh"
 
 namespace pa {

@@ -734,7 +734,7 @@ static int launch(const TreeWork& a, cudaStream_t st) {
     constexpr int ST = stages<D, KT>(), STAGE = stage_bytes<D, KT>();
     const size_t smem = (size_t)kWarps * ST * (STAGE + 8) + (p.num_seqs + 1) * 4 + 1024;
     auto kern = tree_stream_kernel<D, MT, QT, KT>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = allow_dynamic_smem<tree_stream_kernel<D, MT, QT, KT>>(smem);
     if (e != cudaSuccess) return (int)e;
     CUtensorMap k{}, v{};
     if constexpr (KT != I8) {           // boxes move bits: one map type for both 16-bit types

@@ -512,7 +512,7 @@ static int launch(const TreeWork& a, cudaStream_t st) {
     const size_t smem = smem_for(D, NQ, p.num_seqs);
     if (smem > (size_t)device_info().max_smem_optin) return PA_ERR_UNSUPPORTED;
     auto kern = tree_tc_kernel<D, NQ, BF>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = allow_dynamic_smem<tree_tc_kernel<D, NQ, BF>>(smem);
     if (e != cudaSuccess) return (int)e;
     CUtensorMap k, v, q{};              // boxes move bits: one map type for both 16-bit types
     if (!make_bf16_map(&k, p.k, a.total_rows, D, D, 16) || !make_bf16_map(&v, p.v, a.total_rows, D, D, 16)) return PA_ERR_UNSUPPORTED;

@@ -688,7 +688,7 @@ static int launch(const TreeWork& a, cudaStream_t st) {
     const size_t smem = C::smem(p.num_seqs, p.mask_words);
     if (smem > (size_t)device_info().max_smem_optin) return PA_ERR_UNSUPPORTED;
     auto kern = tree_terms_kernel<D, I8, R, Q>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = allow_dynamic_smem<tree_terms_kernel<D, I8, R, Q>>(smem);
     if (e != cudaSuccess) return (int)e;
     CUtensorMap k, v;
     const bool ok = I8 ? make_byte_map(&k, p.k, a.total_rows, D) && make_byte_map(&v, p.v, a.total_rows, D)

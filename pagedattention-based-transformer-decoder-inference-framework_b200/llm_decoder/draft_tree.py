@@ -145,7 +145,7 @@ def paged_tree_attention(q, kv_cache, tree, ctx_lens, temperature=1.0, beam_ids=
     if not q.is_contiguous() and (q.stride(2) != 1 or q.stride(1) != D or (R > 1 and q.stride(0) < H * D)):
         q = q.contiguous()
     if out is None:
-        out = torch.empty((R, H, D), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != (R, H, D) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError("paged_tree_attention: out is contiguous, of q's shape, type and device")
     ctx_lens = _vector(ctx_lens, tree.num_seqs, dev, "ctx_lens")
@@ -221,7 +221,9 @@ def tree_accept(ids, tree, caches, ctx_lens, beam_ids=None):
     ctx_lens = _vector(ctx_lens, B, dev, "ctx_lens")
     if beam_ids is not None:
         beam_ids = _vector(beam_ids, B, dev, "beam_ids")
-    (counts, lens), (tokens, nodes) = (torch.empty(s, dtype=torch.int32, device=dev).unbind(0) for s in ((2, B), (2, B, tree.depth)))
+    paths = B * tree.depth
+    counts, lens, tokens, nodes = torch.empty(2 * (B + paths), dtype=torch.int32, device=dev).split_with_sizes((B, B, paths, paths))
+    tokens, nodes = tokens.view(B, tree.depth), nodes.view(B, tree.depth)
     if B == 0:
         return Accepted(counts, tokens, nodes, lens)
     if tree.rows == 0:

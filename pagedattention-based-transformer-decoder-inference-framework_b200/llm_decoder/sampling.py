@@ -96,7 +96,7 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
     def of(x, dtype, what, n=None):
         """The address of a vector."""
         if not isinstance(x, torch.Tensor) or x.dtype is not dtype or x.get_device() != at or x.dim() != 1 or not x.is_contiguous() or \
-                (n is not None and len(x) != n):
+                (n is not None and x.numel() != n):
             raise ValueError(f"{what}: a contiguous {dtype} vector{'' if n is None else f' of {n}'} on {dev}")
         return x.data_ptr()
     i32, f32, p_seq, p_history, p_start, p_ids, p_val, p_bias, p_rows = torch.int32, torch.float32, None, None, None, None, None, None, None
@@ -114,12 +114,12 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
     if history is not None:
         p_history = of(history, i32, "history")
         p_start = of(history_start, i32, "history_start", None if seqs is None else seqs + 1)
-        seqs = len(history_start) - 1
+        seqs = history_start.numel() - 1
     arrays, values = [], []
     for x, what in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")):
         if isinstance(x, torch.Tensor):
             arrays.append(of(x, f32, what, seqs))
-            seqs = len(x)
+            seqs = x.numel()
             values.append(0.0)
         else:
             arrays.append(None)
@@ -128,7 +128,7 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
         raise ValueError("repetition: above 0 (1 changes nothing)")
     if bias is not None:
         b_ids, b_val, b_start = bias
-        p_ids, p_val = of(b_ids, i32, "bias tokens"), of(b_val, f32, "bias values", len(b_ids))
+        p_ids, p_val = of(b_ids, i32, "bias tokens"), of(b_val, f32, "bias values", b_ids.numel())
         p_bias = of(b_start, i32, "bias starts", None if seqs is None else seqs + 1)
     if allowed is not None:
         if allowed.dim() != 2 or allowed.dtype != torch.int32 or allowed.device != dev or allowed.shape[1] * 32 < V or \
@@ -173,7 +173,7 @@ def adjust_logits(logits, history=None, history_start=None, repetition=1.0, pres
     tokens on a node's path, its own among them, count as history.
     out: a tensor like logits (also logits itself)."""
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or (out.numel() and out.stride(1) != 1) or \
             (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
         raise ValueError("out: of the logits' shape, type and device, rows of consecutive elements")
