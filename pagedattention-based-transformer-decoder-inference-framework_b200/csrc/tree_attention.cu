@@ -127,19 +127,19 @@ PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void
                        rows, num_seqs, most_nodes, heads, head_dim, tile_size, temperature, heads / kv_heads};
     cudaStream_t st = as_stream(stream);
     struct Form {
-        int block, workers, unit;
+        int block, workers, unit, extra;
         int (*launch)(const TreeWork&, cudaStream_t);
     };
-    Form f{tree_tc_block(p), 0, 64, tree_tc_launch};
+    Form f{tree_tc_block(p), 0, 64, kTreeTcExtra, tree_tc_launch};
     f.workers = tree_tc_workers(f.block);
     if (!f.block) {
-        f = Form{tree_terms_block(p), 0, 128, tree_terms_launch};
+        f = Form{tree_terms_block(p), 0, 128, kTreeTermsExtra, tree_terms_launch};
         f.workers = tree_terms_workers(f.block);
     }
-    if (!f.block) f = Form{tree_stream_block(p), tree_stream_workers(), 16, tree_stream_launch};
+    if (!f.block) f = Form{tree_stream_block(p), tree_stream_workers(), 16, 0, tree_stream_launch};
     if (f.block) {
         if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < tree_work_bytes(num_seqs, f.workers, f.block, head_dim)) return PA_ERR_WORKSPACE;
-        const TreeWork w{p, f.workers, kTreeLeast, f.block, f.unit, total_pages * tile_size, kTreeStreamScale, tc::kPolls, static_cast<TreeNote*>(d_workspace),
+        const TreeWork w{p, f.workers, kTreeLeast, f.block, f.unit, total_pages * tile_size, f.extra, kTreeStreamScale, tc::kPolls, static_cast<TreeNote*>(d_workspace),
                          reinterpret_cast<float*>(static_cast<TreeNote*>(d_workspace) + f.workers)};
         int rc = f.launch(w, st);
         if (rc == PA_OK) rc = tree_join_launch(w, st);

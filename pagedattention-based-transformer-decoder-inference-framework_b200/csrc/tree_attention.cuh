@@ -49,11 +49,15 @@ __device__ __forceinline__ int tree_seq_of(const int32_t* node_start, int num_se
 
 // ---- the shares
 constexpr int kTreeMostSeqs = 1024;     // sequences that the streaming kernels take: their step counts stand in shared memory
-constexpr int kTreeLeast = 2;           // steps of a share, where there are that many
+constexpr int kTreeLeast = 2;           // units of a share, where there are that many
+// Beginning and ending an item takes the tcgen05 kernels as long as this many of their steps (of 64 and 128 keys); where shares are cut by steps
+// alone, the ones with many short items end last.  48 sequences of 1 to 2048 keys, 32 heads: 32 bf16 rows 331 -> 188 us (5 units: 192, 3: 210), int8 pages
+// 182 -> 131 us (3: 137, 8: 131), 32 float rows 312 -> 200 us (8: 196).
+constexpr int kTreeTcExtra = 8, kTreeTermsExtra = 6;
 
 struct TreeSeq {
     int r0, n, ctx, keys, blocks, steps;
-    __device__ __forceinline__ int units() const { return blocks * steps; }     // of one kv head
+    __device__ __forceinline__ int units(int extra) const { return steps > 0 ? blocks * (steps + extra) : 0; }     // of one kv head
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b, int block, int unit) {
     TreeSeq s;
@@ -88,6 +92,7 @@ struct __align__(16) TreeNote {
 struct TreeWork {
     TreeParams p;
     int workers, least, block, unit, total_rows;
+    int extra;                          // units before an item's steps in the list: what beginning and ending an item costs
     float p_scale;                      // the partial sums are times this (softmax weights enter products so that small halves keep their bits)
     uint32_t polls;                     // of a wait
     TreeNote* notes;                    // [workers]
@@ -106,7 +111,7 @@ __device__ __forceinline__ TreeNote tree_note(const TreeWork& a, const TreeSeq& 
         t.first_row = s.r0;
         t.g = g;
         t.rr0 = rr0;
-        t.last = (int)(((f_item + s.steps) * ns - 1) / total);
+        t.last = (int)(((f_item + a.extra + s.steps) * ns - 1) / total);
         t.slot = (int)slot;
     }
     return t;

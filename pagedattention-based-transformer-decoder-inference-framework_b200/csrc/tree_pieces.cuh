@@ -14,27 +14,28 @@ struct TreeWalk {
     int b, rb;                          // sequence, block within the kv head
     TreeSeq sq;
     int g, rr0, i0, i1;                 // the piece: kv head, first row, steps [i0, i1)
-    bool first;
+    int u, pieces;                      // its first unit within the item; pieces before it
     int64_t slot;                       // of its partial sums, -1: it is a whole item
-    int64_t f_lo, total, ns;
-    __device__ __forceinline__ TreeWalk(const TreeWork& w, const int* pre_) : a(w), pre(pre_), first(true) {
+    int64_t total, ns;
+    __device__ __forceinline__ TreeWalk(const TreeWork& w, const int* pre_) : a(w), pre(pre_), pieces(-1) {
         total = (int64_t)pre[w.p.num_seqs] * w.p.kv_heads;
         ns = shares::count(total, w.workers, w.least);
-        f_lo = f = blockIdx.x < ns ? total * blockIdx.x / ns : 0;
+        f = blockIdx.x < ns ? total * blockIdx.x / ns : 0;
         f_hi = blockIdx.x < ns ? total * (blockIdx.x + 1) / ns : 0;
         if (f >= f_hi) return;
         b = shares::find_token(pre, w.p.num_seqs, f, w.p.kv_heads);
         sq = tree_seq(w.p, b, w.block, w.unit);
         const int64_t rem = f - (int64_t)pre[b] * w.p.kv_heads;
-        const int item = (int)(rem / sq.steps);
-        i0 = (int)(rem - (int64_t)item * sq.steps);
+        const int each = sq.steps + w.extra, item = (int)(rem / each);
+        u = (int)(rem - (int64_t)item * each);
         g = item / sq.blocks;
         rb = item - g * sq.blocks;
+        if (u + (f_hi - f) <= w.extra) f = f_hi;            // no step of the item is this share's
     }
     __device__ __forceinline__ bool next() {
         if (f >= f_hi) return false;
-        if (!first) {                       // the pieces behind the first begin their items
-            i0 = 0;
+        if (++pieces > 0) {                 // the pieces behind the first begin their items
+            u = 0;
             if (++rb == sq.blocks) {
                 rb = 0;
                 if (++g == a.p.kv_heads) {
@@ -44,14 +45,18 @@ struct TreeWalk {
                 }
             }
         }
-        first = false;
         rr0 = rb * a.block;
         const int64_t left = f_hi - f;
-        i1 = left < sq.steps - i0 ? i0 + (int)left : sq.steps;
-        slot = i0 == 0 && i1 == sq.steps ? -1 : 2 * (int64_t)blockIdx.x + (f - i0 > f_lo ? 1 : 0);
-        f += i1 - i0;
+        const int all = sq.steps + a.extra, end = left < all - u ? u + (int)left : all;
+        i0 = max(u - a.extra, 0);
+        i1 = end - a.extra;
+        slot = i0 == 0 && i1 == sq.steps ? -1 : 2 * (int64_t)blockIdx.x + (pieces > 0 ? 1 : 0);
+        f += end - u;
+        if (f_hi - f <= a.extra) f = f_hi;                  // nothing but units before the steps of the next item
         return true;
     }
+    // where the item that the share's last piece began stands in the list
+    __device__ __forceinline__ int64_t item_at() const { return f_hi - a.extra - i1; }
 };
 
 // The pool rows of a piece's 16-key units, by a whole warp: 32 of them looked up at a time, the next 32 on their way (every lane divides and waits

@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
         mbar_fence_init();
     }
     if (threadIdx.x == 0) fail_word = 0;
-    shares::count_units(pre, p.num_seqs, [&](int b) { return tree_seq(p, b, MT * 16, kUnit).units(); });
+    shares::count_units(pre, p.num_seqs, [&](int b) { return tree_seq(p, b, MT * 16, kUnit).units(0); });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int w = warp * gridDim.x + blockIdx.x, G = p.heads / p.kv_heads;
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
         const int b = shares::find_token(pre, p.num_seqs, f, p.kv_heads);
         const TreeSeq q = tree_seq(p, b, MT * 16, kUnit);
         const int64_t rem = f - (int64_t)pre[b] * p.kv_heads;
-        const int g = (int)(rem / q.units()), j = (int)(rem % q.steps) * kUnit, t = j / p.tile_size;
+        const int g = (int)(rem / q.units(0)), j = (int)(rem % q.steps) * kUnit, t = j / p.tile_size;
         const int row = p.beam_ids ? __ldg(p.beam_ids + b) : b;
         if ((unsigned)row >= (unsigned)p.num_beams || t >= p.num_tiles) return -1;
         const int page = __ldg(p.table + ((int64_t)row * p.kv_heads + g) * p.num_tiles + t);

@@ -94,7 +94,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tmV));
     }
     if (warp == W_MMA) tmem_alloc(tmem_slot, TMEM_COLS);
-    shares::count_units(pre, p.num_seqs, [&](int b) { return tree_seq(p, b, a.block, a.unit).units(); });
+    shares::count_units(pre, p.num_seqs, [&](int b) { return tree_seq(p, b, a.block, a.unit).units(a.extra); });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tc_fence_before();
     __syncthreads();
@@ -137,7 +137,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         };
         TreePages pages(p);
         while (ok && w.next()) {
-            if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = tree_note(a, w.sq, w.g, w.rr0, w.i0, w.i1, w.f - w.i1, w.total, w.ns, w.slot);
+            if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = tree_note(a, w.sq, w.g, w.rr0, w.i0, w.i1, w.item_at(), w.total, w.ns, w.slot);
             pages.open(w, 4);
             int r[4] = {-1, -1, -1, -1}, prev[4] = {-1, -1, -1, -1};
             for (int i = w.i0; i <= w.i1 && ok; ++i) {              // K(i) and V(i - 1)
@@ -535,7 +535,7 @@ int tree_tc_block(const TreeParams& p) {
     if ((int64_t)p.total_pages * p.tile_size >= 0x7fffff00ll || ((uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.q | (uintptr_t)p.out) % 16 || p.q_stride % 8) return 0;
     const int block = rows <= 128 ? 128 : 256;
     const int64_t steps = ((int64_t)p.num_tiles * p.tile_size + ttc::KT - 1) / ttc::KT;
-    return ((int64_t)p.rows * G / block + p.num_seqs) * steps < 0x7fffffff ? block : 0;     // the list's sums are 32 bits
+    return ((int64_t)p.rows * G / block + p.num_seqs) * (steps + kTreeTcExtra) < 0x7fffffff ? block : 0;     // the list's sums are 32 bits
 }
 
 int tree_tc_launch(const TreeWork& a, cudaStream_t st) {

@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tmV));
     }
     if (warp == W_MMA) tmem_alloc(tmem_slot, C::TMEM);
-    shares::count_units(pre, p.num_seqs, [&](int b) { return tree_seq(p, b, a.block, a.unit).units(); });
+    shares::count_units(pre, p.num_seqs, [&](int b) { return tree_seq(p, b, a.block, a.unit).units(a.extra); });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tc_fence_before();
     __syncthreads();
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
         };
         TreePages pages(p);
         while (ok && w.next()) {
-            if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = tree_note(a, w.sq, w.g, w.rr0, w.i0, w.i1, w.f - w.i1, w.total, w.ns, w.slot);
+            if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = tree_note(a, w.sq, w.g, w.rr0, w.i0, w.i1, w.item_at(), w.total, w.ns, w.slot);
             pages.open(w, 8);
             int rows = -1, before = -1;
 #pragma unroll 1
@@ -712,7 +712,7 @@ int tree_terms_block(const TreeParams& p) {
     if ((uintptr_t)p.q % 16 || p.q_stride % 4) return 0;
     const int block = bytes ? (rows <= 16 ? 16 : 32) : rows <= 32 ? 32 : 64;
     const int64_t steps = ((int64_t)p.num_tiles * p.tile_size + tterms::KT - 1) / tterms::KT;
-    return ((int64_t)p.rows * G / block + p.num_seqs) * steps < 0x7fffffff ? block : 0;     // the list's sums are 32 bits
+    return ((int64_t)p.rows * G / block + p.num_seqs) * (steps + kTreeTermsExtra) < 0x7fffffff ? block : 0;     // the list's sums are 32 bits
 }
 
 int tree_terms_launch(const TreeWork& a, cudaStream_t st) {
