@@ -136,7 +136,7 @@ PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void
         f = Form{tree_terms_block(p), 0, 128, kTreeTermsExtra, tree_terms_launch};
         f.workers = tree_terms_workers(f.block);
     }
-    if (!f.block) f = Form{tree_stream_block(p), tree_stream_workers(), 16, 0, tree_stream_launch};
+    if (!f.block) f = Form{tree_stream_block(p), tree_stream_workers(), 16, kTreeStreamExtra, tree_stream_launch};
     if (f.block) {
         if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < tree_work_bytes(num_seqs, f.workers, f.block, head_dim)) return PA_ERR_WORKSPACE;
         const TreeWork w{p, f.workers, kTreeLeast, f.block, f.unit, total_pages * tile_size, f.extra, kTreeStreamScale, tc::kPolls, static_cast<TreeNote*>(d_workspace),

@@ -50,10 +50,11 @@ __device__ __forceinline__ int tree_seq_of(const int32_t* node_start, int num_se
 // ---- the shares
 constexpr int kTreeMostSeqs = 1024;     // sequences that the streaming kernels take: their step counts stand in shared memory
 constexpr int kTreeLeast = 2;           // units of a share, where there are that many
-// Beginning and ending an item takes the tcgen05 kernels as long as this many of their steps (of 64 and 128 keys); where shares are cut by steps
+// Beginning and ending an item takes as long as this many steps (of 64 and 128 keys; 16 in the streaming kernel); where shares are cut by steps
 // alone, the ones with many short items end last.  48 sequences of 1 to 2048 keys, 32 heads: 32 bf16 rows 331 -> 188 us (5 units: 192, 3: 210), int8 pages
-// 182 -> 131 us (3: 137, 8: 131), 32 float rows 312 -> 200 us (8: 196).
-constexpr int kTreeTcExtra = 8, kTreeTermsExtra = 6;
+// 182 -> 131 us (3: 137, 8: 131), 32 float rows 312 -> 200 us (8: 196),
+// 8 bf16 rows 188 -> 161 us (8: 164, 16: 168).
+constexpr int kTreeTcExtra = 8, kTreeTermsExtra = 6, kTreeStreamExtra = 4;
 
 struct TreeSeq {
     int r0, n, ctx, keys, blocks, steps;

@@ -85,13 +85,25 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
         mbar_fence_init();
     }
     if (threadIdx.x == 0) fail_word = 0;
+    int* cut = pre + p.num_seqs + 1;
     shares::count_units(pre, p.num_seqs, [&](int b) { return tree_seq(p, b, MT * 16, kUnit).units(0); });
+    shares::count_units(cut, p.num_seqs, [&](int b) { return tree_seq(p, b, MT * 16, kUnit).units(a.extra); });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int w = warp * gridDim.x + blockIdx.x, G = p.heads / p.kv_heads;
-    const int64_t total = (int64_t)pre[p.num_seqs] * p.kv_heads;
+    // the list is cut with what items take to begin and end (`cut`), and walked by its units of keys (`pre`)
+    const int64_t total = (int64_t)cut[p.num_seqs] * p.kv_heads;
     const int64_t ns = shares::count(total, a.workers, a.least);
-    const int64_t f_lo = w < ns ? total * w / ns : 0, f_hi = w < ns ? total * (w + 1) / ns : 0;
+    auto unit_at = [&](int64_t c) -> int64_t {
+        if (c >= total) return (int64_t)pre[p.num_seqs] * p.kv_heads;
+        const int b = shares::find_token(cut, p.num_seqs, c, p.kv_heads);
+        const TreeSeq q = tree_seq(p, b, MT * 16, kUnit);
+        const int64_t rem = c - (int64_t)cut[b] * p.kv_heads;
+        const int each = q.steps + a.extra, item = (int)(rem / each);
+        return (int64_t)pre[b] * p.kv_heads + (int64_t)item * q.steps + max((int)(rem - (int64_t)item * each) - a.extra, 0);
+    };
+    const int64_t at = w < ns ? unit_at(total * (w + (lane & 1)) / ns) : 0;         // even lanes: the beginning, odd ones: the end
+    const int64_t f_lo = __shfl_sync(0xffffffffu, at, 0), f_hi = __shfl_sync(0xffffffffu, at, 1);
     if (f_lo >= f_hi) {
         if (lane == 0) a.notes[w] = TreeNote{};
         return;
@@ -589,7 +601,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
     close_item(u == sq.steps);
     if (lane == 0) {
         const int64_t f_item = (int64_t)pre[b] * p.kv_heads + (int64_t)item * sq.steps;
-        a.notes[w] = tree_note(a, sq, item / sq.blocks, item % sq.blocks * (MT * 16), u0, u, f_item, total, ns, 2 * (int64_t)w + (f_item > f_lo ? 1 : 0));
+        const int64_t c_item = (int64_t)cut[b] * p.kv_heads + (int64_t)item * (sq.steps + a.extra);
+        a.notes[w] = tree_note(a, sq, item / sq.blocks, item % sq.blocks * (MT * 16), u0, u, c_item, total, ns, 2 * (int64_t)w + (f_item > f_lo ? 1 : 0));
     }
 }
 
@@ -732,7 +745,7 @@ template <int D, int MT, int QT, int KT>
 static int launch(const TreeWork& a, cudaStream_t st) {
     const TreeParams& p = a.p;
     constexpr int ST = stages<D, KT>(), STAGE = stage_bytes<D, KT>();
-    const size_t smem = (size_t)kWarps * ST * (STAGE + 8) + (p.num_seqs + 1) * 4 + 1024;
+    const size_t smem = (size_t)kWarps * ST * (STAGE + 8) + 2 * (p.num_seqs + 1) * 4 + 1024;
     auto kern = tree_stream_kernel<D, MT, QT, KT>;
     const cudaError_t e = allow_dynamic_smem<tree_stream_kernel<D, MT, QT, KT>>(smem);
     if (e != cudaSuccess) return (int)e;
@@ -791,7 +804,7 @@ int tree_stream_block(const TreeParams& p) {
     if ((uintptr_t)p.q % 8 || (uintptr_t)p.out % 8 || p.q_stride % 2) return 0;
     const int G = p.heads / p.kv_heads, block = p.q_type == PA_TYPE_F32 || p.most * G <= 16 ? 16 : 32;
     const int64_t steps = ((int64_t)p.num_tiles * p.tile_size + kUnit - 1) / kUnit;
-    return ((int64_t)p.rows * G / block + p.num_seqs) * steps < 0x7fffffff ? block : 0;     // the list's sums are 32 bits
+    return ((int64_t)p.rows * G / block + p.num_seqs) * (steps + kTreeStreamExtra) < 0x7fffffff ? block : 0;     // the list's sums are 32 bits
 }
 
 int tree_stream_launch(const TreeWork& a, cudaStream_t st) {
