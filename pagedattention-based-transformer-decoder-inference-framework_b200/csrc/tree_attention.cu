@@ -100,7 +100,7 @@ PA_API size_t pa_tree_attention_workspace_bytes(int rows, int num_seqs, int most
     // whichever kernel serves: it goes by the types too
     size_t most = 0;
     for (int block : {16, 32, 64, 128, 256}) {
-        const size_t n = tree_work_bytes(num_seqs, block <= 32 ? tree_stream_workers() : block == 64 ? tree_terms_workers(block) : tree_tc_workers(block), block, head_dim);
+        const size_t n = tree_work_bytes(num_seqs, block <= 32 ? (head_dim == 64 && block == 16 ? 16 : 8) * device_info().sm_count : block == 64 ? tree_terms_workers(block) : tree_tc_workers(block), block, head_dim);
         if (n > most) most = n;
     }
     return most;
@@ -136,7 +136,10 @@ PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void
         f = Form{tree_terms_block(p), 0, 128, kTreeTermsExtra, tree_terms_launch};
         f.workers = tree_terms_workers(f.block);
     }
-    if (!f.block) f = Form{tree_stream_block(p), tree_stream_workers(), 16, kTreeStreamExtra, tree_stream_launch};
+    if (!f.block) {
+        f = Form{tree_stream_block(p), 0, 16, kTreeStreamExtra, tree_stream_launch};
+        if (f.block) f.workers = tree_stream_warps(p, f.block) * device_info().sm_count;
+    }
     if (f.block) {
         if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < tree_work_bytes(num_seqs, f.workers, f.block, head_dim)) return PA_ERR_WORKSPACE;
         const TreeWork w{p, f.workers, kTreeLeast, f.block, f.unit, total_pages * tile_size, f.extra, kTreeStreamScale, tc::kPolls, static_cast<TreeNote*>(d_workspace),

@@ -120,7 +120,7 @@ __device__ __forceinline__ TreeNote tree_note(const TreeWork& a, const TreeSeq& 
 
 // tree_stream.cu: few query rows; the join of pieces
 constexpr float kTreeStreamScale = 128.f;
-int tree_stream_workers();
+int tree_stream_warps(const TreeParams& p, int block);          // workers of an SM
 int tree_stream_block(const TreeParams& p);                     // rows of a block, 0: not served
 int tree_stream_launch(const TreeWork& w, cudaStream_t st);
 int tree_join_launch(const TreeWork& w, cudaStream_t st);

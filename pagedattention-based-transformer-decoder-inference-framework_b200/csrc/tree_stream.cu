@@ -21,13 +21,13 @@
 namespace pa {
 namespace tstream {
 
-constexpr int kWarps = 8, kUnit = 16;
+constexpr int kUnit = 16;
 enum { F32 = PA_TYPE_F32, F16 = PA_TYPE_F16, BF16 = PA_TYPE_BF16, I8 = PA_TYPE_I8 };
 
 __device__ int g_errors;
 
 template <int D, int KT> __host__ __device__ constexpr int stage_bytes() { return KT == I8 ? 2 * kUnit * D + 2 * kUnit * 4 : 2 * kUnit * D * 2; }
-template <int D, int KT> __host__ __device__ constexpr int stages() { return KT == I8 ? (D == 128 ? 5 : 8) : D == 128 ? 3 : 6; }
+template <int D, int W, int KT> __host__ __device__ constexpr int stages() { return W == 16 ? (KT == I8 ? 5 : 3) : KT == I8 ? (D == 128 ? 5 : 8) : D == 128 ? 3 : 6; }
 
 template <bool BF>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -67,11 +67,11 @@ __device__ __forceinline__ uint32_t byte_of_both(uint32_t x, uint32_t y, int j) 
     return bytes_to_half2(w, 0x5140);
 }
 
-template <int D, int MT, int QT, int KT>
+template <int D, int MT, int QT, int KT, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                                                      const TreeWork a) {
     constexpr bool BF = KT == BF16, TWO = QT == F32;
-    constexpr int ST = stages<D, KT>(), STAGE = stage_bytes<D, KT>(), NT = D / 8, KS = D / 16, TERMS = TWO ? 2 : 1, CB = D / 64;
+    constexpr int ST = stages<D, kWarps, KT>(), STAGE = stage_bytes<D, KT>(), NT = D / 8, KS = D / 16, TERMS = TWO ? 2 : 1, CB = D / 64;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ int fail_word;
     const TreeParams& p = a.p;
@@ -621,11 +621,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeWo
     if constexpr (SPLIT > 1) {
         __shared__ int s_count[kJoinWarps], s_found;
         const int per = (a.workers + kJoinWarps * 32 - 1) / (kJoinWarps * 32);
-        int mine = 0;
-        for (int i = 0; i < per; ++i) {
-            const int w = threadIdx.x * per + i;
-            mine += w < a.workers && __ldcg(&a.notes[w].rows) > 0;
+        uint32_t noted = 0;             // a thread has `per` shares, at most 32 (a trip to L2 each, eight under way at a time)
+        for (int i0 = 0; i0 < per; i0 += 8) {
+            int rows[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int w = threadIdx.x * per + i0 + i;
+                rows[i] = i0 + i < per && w < a.workers ? __ldcg(&a.notes[w].rows) : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) noted |= rows[i] > 0 ? 1u << (i0 + i) : 0u;
         }
+        const int mine = __popc(noted);
         int before = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -638,10 +645,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeWo
         before -= mine;
         for (int k = 0; k < warp; ++k) before += s_count[k];
         if ((int)blockIdx.x >= before && (int)blockIdx.x < before + mine) {
-            int left = blockIdx.x - before, w = threadIdx.x * per;
-            for (;; ++w)
-                if (__ldcg(&a.notes[w].rows) > 0 && left-- == 0) break;
-            s_found = w;
+            for (int left = blockIdx.x - before; left > 0; --left) noted &= noted - 1;
+            s_found = threadIdx.x * per + __ffs(noted) - 1;
         }
         __syncthreads();
         w0 = s_found;
@@ -741,13 +746,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeWo
     }
 }
 
-template <int D, int MT, int QT, int KT>
+template <int D, int MT, int QT, int KT, int kWarps>
 static int launch(const TreeWork& a, cudaStream_t st) {
     const TreeParams& p = a.p;
-    constexpr int ST = stages<D, KT>(), STAGE = stage_bytes<D, KT>();
+    constexpr int ST = stages<D, kWarps, KT>(), STAGE = stage_bytes<D, KT>();
     const size_t smem = (size_t)kWarps * ST * (STAGE + 8) + 2 * (p.num_seqs + 1) * 4 + 1024;
-    auto kern = tree_stream_kernel<D, MT, QT, KT>;
-    const cudaError_t e = allow_dynamic_smem<tree_stream_kernel<D, MT, QT, KT>>(smem);
+    auto kern = tree_stream_kernel<D, MT, QT, KT, kWarps>;
+    const cudaError_t e = allow_dynamic_smem<tree_stream_kernel<D, MT, QT, KT, kWarps>>(smem);
     if (e != cudaSuccess) return (int)e;
     CUtensorMap k{}, v{};
     if constexpr (KT != I8) {           // boxes move bits: one map type for both 16-bit types
@@ -783,7 +788,7 @@ int tree_join_launch(const TreeWork& a, cudaStream_t st) {
     const TreeParams& p = a.p;
     // pieces of an item, were all items alike: from 16 (64) on a row's pieces are shared by four (eight) warps
     const int64_t items = p.kv_heads * ((int64_t)p.rows * (p.heads / p.kv_heads) / a.block + p.num_seqs);       // at most
-    const int split = a.workers >= 64 * items ? 8 : a.workers >= 16 * items ? 4 : 1;
+    const int split = a.workers > 32 * kJoinWarps * 32 ? 1 : a.workers >= 64 * items ? 8 : a.workers >= 16 * items ? 4 : 1;
 #define PA_TJ(QT, Q)                                                                                                   \
     if (p.q_type == QT) {                                                                                              \
         if (p.dim == 64) return split == 8 ? join<Q, 2, 8>(a, items, st) : split == 4 ? join<Q, 2, 4>(a, items, st) : join<Q, 2, 1>(a, items, st);                                   \
@@ -794,7 +799,13 @@ int tree_join_launch(const TreeWork& a, cudaStream_t st) {
     return PA_ERR_UNSUPPORTED;
 }
 
-int tree_stream_workers() { return tstream::kWarps * device_info().sm_count; }
+// Warps of a CTA.  16 rows of 64 columns leave registers for 16 warps, which cover each other's waits (16 sequences of 4K keys, 12 heads, float
+// queries: 59 us, with 8 warps 67); where a warp would have a unit or two all the same, a warp alone is through sooner with more registers and the
+// join finds room beside 8 warps (one sequence of 333 keys: 14.5 us, with 16 warps 16.8).
+int tree_stream_warps(const TreeParams& p, int block) {
+    const int64_t units = p.kv_heads * ((int64_t)p.rows * (p.heads / p.kv_heads) / block + p.num_seqs) * (((int64_t)p.num_tiles * p.tile_size + tstream::kUnit - 1) / tstream::kUnit);
+    return p.dim == 64 && block == 16 && units >= 4 * 16 * (int64_t)device_info().sm_count ? 16 : 8;
+}
 
 // Rows of a block, 0 where these kernels do not serve.  Float queries have twice the fragments: 16 rows of them fill the registers.
 int tree_stream_block(const TreeParams& p) {
@@ -810,8 +821,11 @@ int tree_stream_block(const TreeParams& p) {
 int tree_stream_launch(const TreeWork& a, cudaStream_t st) {
     using namespace tstream;
     const TreeParams& p = a.p;
-#define PA_TS(D, MT, QT, KT) if (p.dim == D && a.block == MT * 16 && p.q_type == QT && p.kv_type == KT) return launch<D, MT, QT, KT>(a, st);
-#define PA_TSD(MT, QT, KT) PA_TS(64, MT, QT, KT) PA_TS(128, MT, QT, KT)
+    const int warps = a.workers / device_info().sm_count;
+#define PA_TS(D, MT, QT, KT, W) if (p.dim == D && a.block == MT * 16 && p.q_type == QT && p.kv_type == KT && warps == W) return launch<D, MT, QT, KT, W>(a, st);
+#define PA_TSD(MT, QT, KT) PA_TS(64, MT, QT, KT, 8) PA_TS(128, MT, QT, KT, 8)
+    PA_TS(64, 1, F32, F16, 16) PA_TS(64, 1, F32, I8, 16)
+    PA_TS(64, 1, F16, F16, 16) PA_TS(64, 1, F16, I8, 16) PA_TS(64, 1, BF16, BF16, 16)
     PA_TSD(1, F32, F16) PA_TSD(1, F32, I8)
     PA_TSD(1, F16, F16) PA_TSD(1, F16, I8) PA_TSD(1, BF16, BF16)
     PA_TSD(2, F16, F16) PA_TSD(2, F16, I8) PA_TSD(2, BF16, BF16)
