@@ -1047,6 +1047,9 @@ int pa_conv_append_in_words(int units, int columns, int num_items, int64_t rows)
  *   vocabulary are ignored.  d_out (NULL: not wanted; may be d_logits) gets the logits in their type, d_ids (NULL: not wanted)
  *   the lowest index of the largest float before it is rounded (NaN never wins; 0 where nothing does); d_ids take a workspace
  *   that is zero before the first call and left so by every call.
+ * pa_draft_trees (host arrays): from the nodes' parents (numbers within the sequence; -1 for node 0, a lower node for every other, else
+ *   PA_ERR_INVALID_ARG) of sequences at node_start [num_seqs + 1]: per row its sequence, parent, depth (0 at the root), number and mask
+ *   [rows][mask_words], and the nodes on the longest path.
  * pa_tree_accept: from node 0 to the child whose token is the one chosen at the node (d_ids[row]; of several the lowest) as
  *   long as there is one.  d_counts[b]: nodes on that path (0 for a sequence without nodes); d_nodes, d_out_tokens
  *   [num_seqs][depth]: the nodes and what was chosen at them, -1 behind them; d_new_lens[b] = d_ctx_lens[b] + d_counts[b].
@@ -1072,6 +1075,8 @@ int pa_adjust_logits(const void* d_logits, int type, int64_t stride, int rows, i
                      const int32_t* d_allowed, int64_t allowed_stride, const int32_t* d_allowed_rows, const int32_t* d_tokens,
                      const int32_t* d_path, int path_words, const int32_t* d_node_start, void* d_workspace, size_t workspace_bytes,
                      pa_stream_t stream);
+int pa_draft_trees(const int64_t* parents, const int32_t* node_start, int num_seqs, int mask_words, int32_t* row_seq,
+                   int32_t* row_parents, int32_t* depths, int32_t* nodes, int32_t* mask, int32_t* longest);
 int pa_tree_accept(const int32_t* d_ids, const int32_t* d_tokens, const int32_t* d_parents, const int32_t* d_node_start, int num_seqs,
                    int most_nodes, int depth, const int32_t* d_ctx_lens, const int32_t* d_beam_ids, int num_beams, int kv_heads,
                    int num_tiles, int total_pages, int tile_size, int key_bytes, int value_bytes, int num_caches, void* const* caches,

@@ -10,6 +10,7 @@
 pending token (it has no row in the caches yet), `done.ctx_lens` the next context lengths."""
 import collections
 import ctypes
+import itertools
 
 import numpy as np
 import torch
@@ -38,46 +39,29 @@ class DraftTree:
     mask [rows, words], bit j of which says that node j is on the row's path."""
 
     def __init__(self, parents, tokens=None, device=None):
-        parents = [np.asarray(p, dtype=np.int64).reshape(-1) for p in parents]
-        sizes = np.array([len(p) for p in parents], dtype=np.int64)
-        B, R, most = len(parents), int(sizes.sum()), int(sizes.max(initial=0))
+        sizes = [len(p) for p in parents]
+        B, R, most = len(sizes), sum(sizes), max(sizes, default=0)
         if most > MOST_NODES:
             raise ValueError(f"DraftTree: at most {MOST_NODES} nodes a sequence")
-        start = np.zeros(B + 1, dtype=np.int64)
-        np.cumsum(sizes, out=start[1:])
-        flat = np.concatenate(parents) if R else np.zeros(0, dtype=np.int64)
-        seq, node = np.repeat(np.arange(B), sizes), np.arange(R) - np.repeat(start[:-1], sizes)
-        if not np.all(np.where(node == 0, flat == -1, (flat >= 0) & (flat < node))):
+        if tokens is not None and [len(t) for t in tokens] != sizes:
+            raise ValueError("DraftTree: a token for every node")
+        words, rows = max(1, -(-most // 32)), 4 if tokens is None else 5
+        flat = np.fromiter(itertools.chain.from_iterable(parents), np.int64, R)
+        host = np.zeros(B + 1 + R * (rows + words) + 1, dtype=np.int32)         # one copy; the last word stays here
+        np.cumsum(sizes, out=host[1:B + 1])
+        if tokens is not None:
+            host[B + 1 + 4 * R:B + 1 + 5 * R] = np.fromiter(itertools.chain.from_iterable(tokens), np.int64, R)
+        at = host.ctypes.data
+        row = [at + 4 * (B + 1 + i * R) for i in range(rows + 1)]               # sequences, parents, depths, nodes, (tokens,) masks
+        if _cabi.lib().pa_draft_trees(flat.ctypes.data, at, B, words, *row[:4], row[rows], at + 4 * (len(host) - 1)) != _cabi.PA_OK:
             raise ValueError("DraftTree: node 0 has parent -1, every other node a lower one of its sequence")
-        words = max(1, -(-most // 32))
-        mask, depths = np.zeros((R, words), dtype=np.uint32), np.zeros(R, dtype=np.int64)
-        order = np.argsort(node, kind="stable")             # node by node, all sequences at a time: parents are done first
-        ends = np.searchsorted(node[order], np.arange(most + 1))
-        for i in range(most):
-            r = order[ends[i]:ends[i + 1]]
-            if i:
-                up = start[seq[r]] + flat[r]
-                mask[r], depths[r] = mask[up], depths[up] + 1
-            mask[r, i >> 5] |= np.uint32(1 << (i & 31))
-        per_row = [seq, flat, depths, node]
-        if tokens is not None:
-            tokens = [np.asarray(t, dtype=np.int64).reshape(-1) for t in tokens]
-            if [len(t) for t in tokens] != sizes.tolist():
-                raise ValueError("DraftTree: a token for every node")
-            per_row.append(np.concatenate(tokens) if R else flat)
-        self.rows, self.num_seqs, self.sizes, self.most = R, B, sizes.tolist(), most
-        self.depth = int(depths.max(initial=-1)) + 1
+        self.rows, self.num_seqs, self.sizes, self.most, self.depth = R, B, sizes, most, int(host[-1])
         self.device = _on(device)
-        host = np.concatenate([start] + per_row).astype(np.int32)
-        host = torch.from_numpy(np.concatenate([host, mask.view(np.int32).reshape(-1)]))    # one copy
-        dev = to_device(host, self.device)
-        self.node_start, at = dev[:B + 1], B + 1
-        self.row_seq, self.parents, self.depths, self.nodes = (dev[at + i * R:at + (i + 1) * R] for i in range(4))
-        at += 4 * R
-        self.tokens = None
-        if tokens is not None:
-            self.tokens, at = dev[at:at + R], at + R
-        self.mask = dev[at:].view(R, words)
+        dev = to_device(torch.from_numpy(host[:-1]), self.device)
+        self.node_start, *parts = dev.split_with_sizes([B + 1] + [R] * rows + [R * words])
+        self.row_seq, self.parents, self.depths, self.nodes = parts[:4]
+        self.tokens = None if tokens is None else parts[4]
+        self.mask = parts[-1].view(R, words)
         self._space = {}                # (heads, kv heads, D) -> bytes of workspace that pa_tree_attention wants for this tree
 
     def positions(self, ctx_lens):
