@@ -307,52 +307,47 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
             ++pieces;
         }
     } else if (warp >= W_LOAD) {
-        // ---- queries: a warp per row, eight rows at a time
-        constexpr int PER = D / 32;         // columns of a lane
+        // ---- queries: half of the rows a warp, one row at a time over its lanes, up to 16 rows under way together
+        constexpr int PER = D / 32, HALF = R / 2, LB = HALF < 16 ? HALF : 16;       // columns of a lane, rows of a warp, rows under way
         const float f0 = 1.4426950408889634f / p.temperature;
-        const int c0 = lane * PER;
+        const int c0 = lane * PER, mine = (warp - W_LOAD) * HALF + lane;            // the row that this lane knows about
         while (w.next()) {
-            const int all = w.sq.n * G, buf = (int)(pieces % C::Q_BUFS);
+            const int all = w.sq.n * G, buf = (int)(pieces % C::Q_BUFS), rr = w.rr0 + mine, div = rr / G;
             const uint32_t qb = q_sm + buf * C::Q_BYTES;
-            wait(q_free(pieces), q_phase(pieces) ^ 1u);
-            int *nodes = s_node + (pieces & 7) * R, *heads = s_head + (pieces & 7) * R;
-            const int mine = threadIdx.x - W_LOAD * 32;
-            if (mine < R) {                 // one division a row, for everyone
-                const int rr = w.rr0 + mine, node = rr / G;
-                nodes[mine] = rr < all ? w.sq.r0 + node : -1;
-                heads[mine] = w.g * G + rr - node * G;
-            }
-            asm volatile("bar.sync 2, 64;" ::: "memory");
+            const int node = lane < HALF && rr < all ? w.sq.r0 + div : -1, head = w.g * G + rr - div * G;
+            const int64_t own = node >= 0 ? (int64_t)node * p.q_stride + (int64_t)head * D : -1;
+            const uint32_t mask0 = node >= 0 ? __ldg(p.mask + (int64_t)node * p.mask_words) : 0u;
 #pragma unroll 1
-            for (int r0 = (warp - W_LOAD) * 8; r0 < R; r0 += 16) {
-                float x[8][PER], big[8];
+            for (int b0 = 0; b0 < HALF; b0 += LB) {
+                float x[LB][PER], big[LB];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int node = nodes[r0 + k];
-                    const Q* q = static_cast<const Q*>(p.q) + (int64_t)node * p.q_stride + (int64_t)heads[r0 + k] * D + c0;
+                for (int k = 0; k < LB; ++k) {
+                    const int64_t from = __shfl_sync(0xffffffffu, own, b0 + k);
+                    const Q* q = static_cast<const Q*>(p.q) + from + c0;
                     if constexpr (sizeof(Q) == 4 && PER == 4) {
-                        const float4 v = node >= 0 ? __ldg(reinterpret_cast<const float4*>(q)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        const float4 v = from >= 0 ? __ldg(reinterpret_cast<const float4*>(q)) : make_float4(0.f, 0.f, 0.f, 0.f);
                         x[k][0] = v.x; x[k][1] = v.y; x[k][PER - 2] = v.z; x[k][PER - 1] = v.w;
                     } else if constexpr (sizeof(Q) == 4) {
-                        const float2 v = node >= 0 ? __ldg(reinterpret_cast<const float2*>(q)) : make_float2(0.f, 0.f);
+                        const float2 v = from >= 0 ? __ldg(reinterpret_cast<const float2*>(q)) : make_float2(0.f, 0.f);
                         x[k][0] = v.x; x[k][1] = v.y;
                     } else {
-                        const uint2 v = node >= 0 ? __ldg(reinterpret_cast<const uint2*>(q)) : make_uint2(0u, 0u);
+                        const uint2 v = from >= 0 ? __ldg(reinterpret_cast<const uint2*>(q)) : make_uint2(0u, 0u);
                         const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
                         x[k][0] = lo.x; x[k][1] = lo.y; x[k][PER - 2] = hi.x; x[k][PER - 1] = hi.y;
                     }
                 }
+                if (b0 == 0) wait(q_free(pieces), q_phase(pieces) ^ 1u);        // their place is read; the rows are on their way by then
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
+                for (int k = 0; k < LB; ++k) {
                     big[k] = 0.f;
 #pragma unroll
                     for (int c = 0; c < PER; ++c) big[k] = fmaxf(big[k], fabsf(x[k][c]));
                 }
 #pragma unroll
-                for (int k = 0; k < 8; ++k) big[k] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big[k])));
+                for (int k = 0; k < LB; ++k) big[k] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big[k])));
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int r = r0 + k;
+                for (int k = 0; k < LB; ++k) {
+                    const int r = (warp - W_LOAD) * HALF + b0 + k;
                     if constexpr (I8) {
                         // a row with numbers that are not finite: no digits, and its scores are not finite through their factor
                         bool odd = false;
@@ -375,25 +370,33 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                         // the row's largest between 2^10 and 2^11: halves hold hi, and lo down to 2^-35 of it
                         const int e = max(-100, min(100, 137 - (int)(__float_as_uint(big[k]) >> 23)));
                         const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+                        uint32_t v[2][PER / 2];
 #pragma unroll
                         for (int c = 0; c < PER; c += 2) {
-                            const uint32_t hi = pack_half2(x[k][c] * up, x[k][c + 1] * up);
-                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                            const uint32_t v[2] = {hi, pack_half2(x[k][c] * up - back.x, x[k][c + 1] * up - back.y)};
+                            v[0][c / 2] = pack_half2(x[k][c] * up, x[k][c + 1] * up);
+                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&v[0][c / 2]));
+                            v[1][c / 2] = pack_half2(x[k][c] * up - back.x, x[k][c + 1] * up - back.y);
+                        }
 #pragma unroll
-                            for (int t = 0; t < 2; ++t) {
-                                const int row = t * R + r, col = c0 + c;
-                                const uint32_t addr = qb + (col >> 6) * (N * 128) + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2;
-                                asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v[t]) : "memory");
-                            }
+                        for (int t = 0; t < 2; ++t) {
+                            const int row = t * R + r;
+                            const uint32_t addr = qb + (c0 >> 6) * (N * 128) + row * 128 + ((((c0 & 63) >> 3) ^ (row & 7)) << 4) + (c0 & 7) * 2;
+                            if constexpr (PER == 4)
+                                asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(addr), "r"(v[t][0]), "r"(v[t][PER / 2 - 1]) : "memory");
+                            else
+                                asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v[t][0]) : "memory");
                         }
                         if (lane == 0) s_fe[buf * R + r] = f0 * __uint_as_float((uint32_t)(127 - e) << 23);
                     }
                 }
             }
-            if (mine < R)
-                for (int x = 0; x < p.mask_words; ++x)
-                    s_mask[(buf * R + mine) * p.mask_words + x] = nodes[mine] >= 0 ? __ldg(p.mask + (int64_t)nodes[mine] * p.mask_words + x) : 0u;
+            if (lane < HALF) {
+                s_node[(pieces & 7) * R + mine] = node;
+                s_head[(pieces & 7) * R + mine] = head;
+                uint32_t* mask = s_mask + (buf * R + mine) * p.mask_words;
+                mask[0] = mask0;
+                for (int x = 1; x < p.mask_words; ++x) mask[x] = node >= 0 ? __ldg(p.mask + (int64_t)node * p.mask_words + x) : 0u;
+            }
             fence_proxy_async();
             mbar_arrive_cnt(q_ready(pieces));
             ++pieces;
