@@ -13,6 +13,8 @@
 //
 // A value that is not finite in a drafted row does not reach the rows that do not see it: a unit of drafted keys with such values takes
 // them out of the product and adds them for the rows that see them.
+#include <algorithm>
+
 #include "f32x2.cuh"
 #include "mma_utils.cuh"
 #include "tcgen05_utils.cuh"
@@ -607,15 +609,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
 }
 
 // The rows of items whose keys were in several shares.  blockIdx.x: the share that noted the item (where items are few and their pieces many,
-// the number of the note among all), blockIdx.y: kJoinWarps / SPLIT of its rows, SPLIT warps each that share the row's pieces; a lane has
-// D / 32 neighbouring columns.  A warp's pieces come in order, FLIGHT at a time with all their loads in flight, under a running maximum.
+// the number of the note among all), blockIdx.y: its share of the item's rows.  A warp has RW rows at a time, or SPLIT warps one row whose pieces they
+// share; a lane has D / 32 neighbouring columns.  Pieces come in order, FLIGHT of a warp at a time with the loads of all its rows in flight, under a running
+// maximum.  It is bound by trips to L2: waiting for the shares, note, pieces.  (One row a warp and a CTA for every eight of them took 19 of 128 us
+// behind 32 sequences of 128 rows and 8 kv heads.)
 constexpr int kJoinWarps = 8;
-template <typename Q, int NV, int SPLIT>
+template <typename Q, int NV, int SPLIT, int RW>
 __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeWork a) {
-    constexpr int D = NV * 32, LD = D + 4, ROWS = kJoinWarps / SPLIT, FLIGHT = SPLIT > 1 ? 8 : 4;
+    constexpr int D = NV * 32, LD = D + 4, ROWS = kJoinWarps / SPLIT * RW, FLIGHT = 8 / RW;
     __shared__ float s_acc[SPLIT > 1 ? kJoinWarps : 1][D], s_ml[SPLIT > 1 ? kJoinWarps : 1][3];
     const TreeParams& p = a.p;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.heads / p.kv_heads;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.group;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int w0 = blockIdx.x;
     if constexpr (SPLIT > 1) {
@@ -654,94 +658,113 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeWo
     }
     const int4* note = reinterpret_cast<const int4*>(a.notes + w0);
     const int4 n0 = __ldcg(note), n1 = __ldcg(note + 1);
-    if ((int)blockIdx.y * ROWS >= n0.x) return;
-    const int w1 = n1.x, rl = blockIdx.y * ROWS + warp / SPLIT, rr = n0.w + rl;
-    const bool real = rl < n0.x;
+    const int w1 = n1.x;
     const int64_t step = (int64_t)2 * a.block * LD;
-    const float* rest = a.part + ((int64_t)2 * w0 * a.block + rl) * LD;         // share w's piece, w > w0
-    const float* first = a.part + ((int64_t)n1.y * a.block + rl) * LD;
-    float mx = -INFINITY, top = -INFINITY, l = 0.f, acc[NV];
+    const float *rest = a.part + (int64_t)2 * w0 * a.block * LD, *first = a.part + (int64_t)n1.y * a.block * LD;       // share w's piece, w > w0; the first
+#pragma unroll 1
+    for (int r0 = blockIdx.y * ROWS; r0 < n0.x; r0 += gridDim.y * ROWS) {
+        const int rl = r0 + warp / SPLIT * RW;          // the warp's rows: rl .. rl + RW - 1
+        float mx[RW], top[RW], l[RW], acc[RW][NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) acc[i] = 0.f;
-    for (int w = w0 + warp % SPLIT; real && w <= w1; w += FLIGHT * SPLIT) {
-        float4 ml[FLIGHT];
-        float v[FLIGHT][NV];
+        for (int x = 0; x < RW; ++x) {
+            mx[x] = top[x] = -INFINITY;
+            l[x] = 0.f;
 #pragma unroll
-        for (int k = 0; k < FLIGHT; ++k) {
-            const int wk = w + k * SPLIT;
-            if (wk > w1) continue;
-            const float* s = wk == w0 ? first : rest + (wk - w0) * step;
-            ml[k] = __ldcg(reinterpret_cast<const float4*>(s + D));
-            if constexpr (NV == 4) {
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(s) + lane);
-                v[k][0] = x.x; v[k][1] = x.y; v[k][NV - 2] = x.z; v[k][NV - 1] = x.w;
-            } else {
-                const float2 x = __ldcg(reinterpret_cast<const float2*>(s) + lane);
-                v[k][0] = x.x; v[k][1] = x.y;
+            for (int i = 0; i < NV; ++i) acc[x][i] = 0.f;
+        }
+#pragma unroll 1
+        for (int w = w0 + warp % SPLIT; rl < n0.x && w <= w1; w += FLIGHT * SPLIT) {
+            float4 ml[FLIGHT][RW];
+            float v[FLIGHT][RW][NV];
+#pragma unroll
+            for (int k = 0; k < FLIGHT; ++k)
+#pragma unroll
+                for (int x = 0; x < RW; ++x) {
+                    const int wk = w + k * SPLIT;
+                    ml[k][x] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+                    if (wk > w1 || rl + x >= n0.x) continue;
+                    const float* s = (wk == w0 ? first : rest + (wk - w0) * step) + (rl + x) * LD;
+                    ml[k][x] = __ldcg(reinterpret_cast<const float4*>(s + D));
+                    if constexpr (NV == 4) {
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(s) + lane);
+                        v[k][x][0] = y.x; v[k][x][1] = y.y; v[k][x][NV - 2] = y.z; v[k][x][NV - 1] = y.w;
+                    } else {
+                        const float2 y = __ldcg(reinterpret_cast<const float2*>(s) + lane);
+                        v[k][x][0] = y.x; v[k][x][1] = y.y;
+                    }
+                }
+#pragma unroll
+            for (int x = 0; x < RW; ++x) {
+                float mn = mx[x];
+#pragma unroll
+                for (int k = 0; k < FLIGHT; ++k) {
+                    mn = fmaxf(mn, ml[k][x].x);
+                    top[x] = fmaxf(top[x], ml[k][x].z);
+                }
+                const float ref = mn == -INFINITY ? 0.f : mn, f = exp2f(mx[x] - ref);
+                mx[x] = mn;
+                l[x] *= f;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) acc[x][i] *= f;
+#pragma unroll
+                for (int k = 0; k < FLIGHT; ++k) {
+                    if (ml[k][x].x == -INFINITY && ml[k][x].y == 0.f) continue;       // no piece, or it saw nothing: 0 x infinity = NaN
+                    const float c = exp2f(ml[k][x].x - ref);
+                    l[x] = fmaf(c, ml[k][x].y, l[x]);
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) acc[x][i] = fmaf(c, v[k][x][i], acc[x][i]);
+                }
             }
         }
-        float mn = mx;
+        if constexpr (SPLIT > 1) {                      // RW is 1
 #pragma unroll
-        for (int k = 0; k < FLIGHT; ++k)
-            if (w + k * SPLIT <= w1) {
-                mn = fmaxf(mn, ml[k].x);
-                top = fmaxf(top, ml[k].z);
+            for (int i = 0; i < NV; ++i) s_acc[warp][lane * NV + i] = acc[0][i];
+            if (lane == 0) {
+                s_ml[warp][0] = mx[0];
+                s_ml[warp][1] = l[0];
+                s_ml[warp][2] = top[0];
             }
-        const float ref = mn == -INFINITY ? 0.f : mn, f = exp2f(mx - ref);
-        mx = mn;
-        l *= f;
+            __syncthreads();
+            if (warp % SPLIT == 0) {
+                float all = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) acc[i] *= f;
+                for (int k = 0; k < SPLIT; ++k) {
+                    all = fmaxf(all, s_ml[warp + k][0]);
+                    top[0] = fmaxf(top[0], s_ml[warp + k][2]);
+                }
+                l[0] = 0.f;
+                mx[0] = all;
+                const float ref = all == -INFINITY ? 0.f : all;
 #pragma unroll
-        for (int k = 0; k < FLIGHT; ++k) {
-            if (w + k * SPLIT > w1 || (ml[k].x == -INFINITY && ml[k].y == 0.f)) continue;       // saw nothing: 0 x infinity = NaN
-            const float c = exp2f(ml[k].x - ref);
-            l = fmaf(c, ml[k].y, l);
+                for (int i = 0; i < NV; ++i) acc[0][i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) acc[i] = fmaf(c, v[k][i], acc[i]);
+                for (int k = 0; k < SPLIT; ++k) {
+                    const float m = s_ml[warp + k][0];
+                    if (m == -INFINITY && s_ml[warp + k][1] == 0.f) continue;
+                    const float c = exp2f(m - ref);
+                    l[0] = fmaf(c, s_ml[warp + k][1], l[0]);
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) acc[0][i] = fmaf(c, s_acc[warp + k][lane * NV + i], acc[0][i]);
+                }
+            }
+            __syncthreads();
+            if (warp % SPLIT) continue;
         }
-    }
-    if constexpr (SPLIT > 1) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) s_acc[warp][lane * NV + i] = acc[i];
-        if (lane == 0) {
-            s_ml[warp][0] = mx;
-            s_ml[warp][1] = l;
-            s_ml[warp][2] = top;
-        }
-        __syncthreads();
-        if (warp % SPLIT) return;
-        float all = -INFINITY;
+        for (int x = 0; x < RW; ++x) {
+            if (rl + x >= n0.x) continue;
+            const int rr = n0.w + rl + x;
+            const float inv = 1.f / (l[x] + 1e-6f * a.p_scale * (mx[x] == -INFINITY ? 1.f : exp2f(top[x] - mx[x])));     // the formula's sum is relative to the largest score
+            Q* out = static_cast<Q*>(p.out) + ((int64_t)(n0.y + rr / G) * p.heads + n0.z * G + rr % G) * D + lane * NV;
 #pragma unroll
-        for (int k = 0; k < SPLIT; ++k) {
-            all = fmaxf(all, s_ml[warp + k][0]);
-            top = fmaxf(top, s_ml[warp + k][2]);
-        }
-        l = 0.f;
-        mx = all;
-        const float ref = all == -INFINITY ? 0.f : all;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) acc[i] = 0.f;
-#pragma unroll
-        for (int k = 0; k < SPLIT; ++k) {
-            const float m = s_ml[warp + k][0];
-            if (m == -INFINITY && s_ml[warp + k][1] == 0.f) continue;
-            const float c = exp2f(m - ref);
-            l = fmaf(c, s_ml[warp + k][1], l);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) acc[i] = fmaf(c, s_acc[warp + k][lane * NV + i], acc[i]);
-        }
-    }
-    if (!real) return;
-    const float inv = 1.f / (l + 1e-6f * a.p_scale * (mx == -INFINITY ? 1.f : exp2f(top - mx)));     // the formula's sum is relative to the largest score
-    Q* out = static_cast<Q*>(p.out) + ((int64_t)(n0.y + rr / G) * p.heads + n0.z * G + rr % G) * D + lane * NV;
-#pragma unroll
-    for (int i = 0; i < NV; i += 2) {
-        if constexpr (sizeof(Q) == 4) {
-            *reinterpret_cast<float2*>(out + i) = make_float2(acc[i] * inv, acc[i + 1] * inv);
-        } else {
-            Q two[2] = {tree_narrow<Q>(acc[i] * inv), tree_narrow<Q>(acc[i + 1] * inv)};
-            *reinterpret_cast<uint32_t*>(out + i) = *reinterpret_cast<uint32_t*>(two);
+            for (int i = 0; i < NV; i += 2) {
+                if constexpr (sizeof(Q) == 4) {
+                    *reinterpret_cast<float2*>(out + i) = make_float2(acc[x][i] * inv, acc[x][i + 1] * inv);
+                } else {
+                    Q two[2] = {tree_narrow<Q>(acc[x][i] * inv), tree_narrow<Q>(acc[x][i + 1] * inv)};
+                    *reinterpret_cast<uint32_t*>(out + i) = *reinterpret_cast<uint32_t*>(two);
+                }
+            }
         }
     }
 }
@@ -766,11 +789,12 @@ static int launch(const TreeWork& a, cudaStream_t st) {
 
 namespace tstream {
 
-template <typename Q, int NV, int SPLIT>
+template <typename Q, int NV, int SPLIT, int RW>
 static int join(const TreeWork& a, int64_t items, cudaStream_t st) {
-    const int rows = (int)((int64_t)a.p.most * (a.p.heads / a.p.kv_heads) < a.block ? a.p.most * (a.p.heads / a.p.kv_heads) : a.block);
+    const int64_t rows = std::min<int64_t>((int64_t)a.p.most * a.p.group, a.block), groups = (rows * SPLIT + kJoinWarps * RW - 1) / (kJoinWarps * RW);
+    const int64_t x = SPLIT > 1 ? items : a.workers, most = 4 * device_info().sm_count / x;     // a few CTAs an SM walk the rest
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(SPLIT > 1 ? items : a.workers), (unsigned)((rows * SPLIT + kJoinWarps - 1) / kJoinWarps));
+    cfg.gridDim = dim3((unsigned)x, (unsigned)std::max<int64_t>(1, std::min(groups, most)));
     cfg.blockDim = dim3(kJoinWarps * 32);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -778,7 +802,7 @@ static int join(const TreeWork& a, int64_t items, cudaStream_t st) {
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, tree_join_kernel<Q, NV, SPLIT>, a);
+    return (int)cudaLaunchKernelEx(&cfg, tree_join_kernel<Q, NV, SPLIT, RW>, a);
 }
 
 }  // namespace tstream
@@ -787,15 +811,19 @@ int tree_join_launch(const TreeWork& a, cudaStream_t st) {
     using namespace tstream;
     const TreeParams& p = a.p;
     // pieces of an item, were all items alike: from 16 (64) on a row's pieces are shared by four (eight) warps
-    const int64_t items = p.kv_heads * ((int64_t)p.rows * (p.heads / p.kv_heads) / a.block + p.num_seqs);       // at most
+    const int64_t items = p.kv_heads * (((int64_t)p.rows * p.group + (int64_t)p.num_seqs * (a.block - 1)) / a.block);       // at most
     const int split = a.workers > 32 * kJoinWarps * 32 ? 1 : a.workers >= 64 * items ? 8 : a.workers >= 16 * items ? 4 : 1;
+#define PA_TJN(Q, NV)                                                                                                  \
+    return split == 8 ? join<Q, NV, 8, 1>(a, items, st) : split == 4 ? join<Q, NV, 4, 1>(a, items, st)                 \
+         : a.block <= 32 ? join<Q, NV, 1, 2>(a, items, st) : join<Q, NV, 1, 4>(a, items, st);
 #define PA_TJ(QT, Q)                                                                                                   \
     if (p.q_type == QT) {                                                                                              \
-        if (p.dim == 64) return split == 8 ? join<Q, 2, 8>(a, items, st) : split == 4 ? join<Q, 2, 4>(a, items, st) : join<Q, 2, 1>(a, items, st);                                   \
-        return split == 8 ? join<Q, 4, 8>(a, items, st) : split == 4 ? join<Q, 4, 4>(a, items, st) : join<Q, 4, 1>(a, items, st);                                                    \
+        if (p.dim == 64) PA_TJN(Q, 2)                                                                                  \
+        PA_TJN(Q, 4)                                                                                                   \
     }
     PA_TJ(F32, float) PA_TJ(F16, __half) PA_TJ(BF16, bf16_t)
 #undef PA_TJ
+#undef PA_TJN
     return PA_ERR_UNSUPPORTED;
 }
 
