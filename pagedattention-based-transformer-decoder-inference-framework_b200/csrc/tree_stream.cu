@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
 constexpr int kJoinWarps = 8;
 template <typename Q, int NV, int SPLIT, int RW>
 __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeWork a) {
-    constexpr int D = NV * 32, LD = D + 4, ROWS = kJoinWarps / SPLIT * RW, FLIGHT = 8 / RW;
+    constexpr int D = NV * 32, LD = D + 4, ROWS = kJoinWarps / SPLIT * RW, FLIGHT = SPLIT > 1 ? 8 : RW == 1 ? 4 : 8 / RW;
     __shared__ float s_acc[SPLIT > 1 ? kJoinWarps : 1][D], s_ml[SPLIT > 1 ? kJoinWarps : 1][3];
     const TreeParams& p = a.p;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.group;
@@ -792,7 +792,7 @@ namespace tstream {
 template <typename Q, int NV, int SPLIT, int RW>
 static int join(const TreeWork& a, int64_t items, cudaStream_t st) {
     const int64_t rows = std::min<int64_t>((int64_t)a.p.most * a.p.group, a.block), groups = (rows * SPLIT + kJoinWarps * RW - 1) / (kJoinWarps * RW);
-    const int64_t x = SPLIT > 1 ? items : a.workers, most = 4 * device_info().sm_count / x;     // a few CTAs an SM walk the rest
+    const int64_t x = SPLIT > 1 ? items : a.workers, most = SPLIT == 1 && RW == 1 ? groups : 4 * device_info().sm_count / x;      // a few CTAs an SM walk the rest
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)x, (unsigned)std::max<int64_t>(1, std::min(groups, most)));
     cfg.blockDim = dim3(kJoinWarps * 32);
@@ -815,7 +815,7 @@ int tree_join_launch(const TreeWork& a, cudaStream_t st) {
     const int split = a.workers > 32 * kJoinWarps * 32 ? 1 : a.workers >= 64 * items ? 8 : a.workers >= 16 * items ? 4 : 1;
 #define PA_TJN(Q, NV)                                                                                                  \
     return split == 8 ? join<Q, NV, 8, 1>(a, items, st) : split == 4 ? join<Q, NV, 4, 1>(a, items, st)                 \
-         : a.block <= 32 ? join<Q, NV, 1, 2>(a, items, st) : join<Q, NV, 1, 4>(a, items, st);
+         : a.block <= 32 ? join<Q, NV, 1, 1>(a, items, st) : join<Q, NV, 1, 4>(a, items, st);
 #define PA_TJ(QT, Q)                                                                                                   \
     if (p.q_type == QT) {                                                                                              \
         if (p.dim == 64) PA_TJN(Q, 2)                                                                                  \
