@@ -5,8 +5,11 @@
 // over t < ctx and t = ctx + j with bit j of the row's mask set; keys on unmapped pages contribute nothing, a row that sees nothing
 // is zero.
 //
-// The form for every page size, head size up to 256 and element type: one CTA per (row, head), its warps take the keys in turns, a
-// lane holds dim / 32 columns; softmax with a running maximum and sum in float, joined over the warps at the end.
+// The form for every page size, head size up to 256 and element type: one CTA per (row, head), its warps take the keys in turns, a lane holds dim /
+// 32 columns; softmax with a running maximum and sum in float, joined over the warps at the end.  It reads a sequence's keys and values once per row
+// and is bound by that and by the chain from key to key: 16 sequences of 4096 keys, 12 float heads of 64 columns, float pages, 8 nodes 1.8 ms, 224
+// GB/s of the bytes there are.  The kernels of tree_stream.cu, tree_tc.cu and tree_terms.cu take half, bfloat16 and int8 pages of 16 rows (or
+// multiples), head sizes 64 and 128 and up to 1024 sequences.
 #include "tcgen05_utils.cuh"
 #include "tree_attention.cuh"
 

@@ -9,15 +9,24 @@
 //                 values' scales as 31-bit ones relative to the largest possible of a tile (four); products and their sums are exact
 //                 integers, no byte is converted
 // A row's reference moves only when a score exceeds it by more than 2^8, which the terms leave room for: after a piece's first tile
-// hardly ever.
+// hardly ever.  (So the formula's 1e-6 stands beside a sum that may be up to 2^8 times the one relative to the largest score: 1e-6 of a result.)
 // The sums of a tile leave the tensor cores as they are and are added up in float registers (the tensor cores cut where float rounds: over a
 // long context that would add up).  A row's terms are neighbours in P^T, whose rows are keys: a thread stores four query rows at once.
-//   warps 0-7    (0-3: two CTAs an SM) softmax, one thread per key and half of (all) the rows: its scores, one vote per tile whether a row's reference has to move (then
-//                the maxima by warp and through shared memory), weights to shared memory as the MN-major B operand
+//   warps 0-7    softmax, one thread per key and half of the rows (blocks of 16 rows: warps 0-3 and all rows, two CTAs an SM): its scores, one vote
+//                per tile whether a row's reference has to move (then the maxima by warp and through shared memory), weights to shared memory
+//                as the MN-major B operand
 //   next four    one thread per value column: the tile's sums into its R float sums, rescaled where a reference moved
 //   next         issues  S^T of tile t + 1  and  O^T of tile t;  scores and sums are double-buffered in TMEM
 //   next         TMA boxes of 16 keys into a ring (int8: and the rows' scales), page ids a tile ahead
 //   last two     the next piece's queries into the K-major B operand, their factors and masks
+//
+// What bounds it: the latency of a tile's chain (scores, vote, weights, products, sums) at one or two softmax warps for each quarter of an SM, and
+// of a piece's beginning and end, some 6 us.  12 sequences of 4K keys, 32 heads: half pages and 32 float rows 152 us, 5.3 TB/s; int8 pages and 16
+// float rows 87 us, 4.8 TB/s; 48 sequences of 1 to 2K keys, int8 pages 126 us, 3.5 TB/s; 16 sequences of 4K keys, 128 rows a kv head (blocks of 64)
+// 131 us, 262 TFLOP/s of the formula's operations.  Rows as the columns of the products keep the tile at 128 keys for any number of rows: as rows
+// they would fill 128 lanes with 16.  Digits and terms instead of tf32 or a conversion to half: int8 pages stay as they are, and float results keep
+// 22 bits.  Reading a tile's maximum before its exponentials for every tile took 223 us where votes on 2^8 take 192 (before the shares counted
+// beginnings and ends: 126 now).
 #include "tcgen05_utils.cuh"
 #include "tree_pieces.cuh"
 
@@ -705,7 +714,11 @@ static int launch(const TreeWork& a, cudaStream_t st) {
 
 int tree_terms_workers(int block) { return device_info().sm_count * (block == 16 ? 2 : 1); }
 
-// Rows of a block, 0 where this kernel does not serve or the streaming one is faster
+// Rows of a block, 0 where this kernel does not serve or the streaming one is faster.  us, this kernel against the streaming one: int8 pages, 16
+// rows: 1000 keys 111 against 206, 4K keys 87 against 194, ragged 126 against 207, 100 keys 38 against 52; half pages, 32 float rows: 4K keys 153
+// against 294, 1000 keys 189 against 307, 90 keys 92 against 72 (the host does not know how long contexts are); 16 float rows 205 against 209, and
+// of 64 columns 65 against 58: from 17 on.  int8 rows of 64 bytes have no tile here.  Blocks: int8, 256 rows in 32s 317, in 16s 370, 16 rows in a
+// block of 32 194 instead of 111; half, 128 rows in 64s 131, in 32s 196; 32 rows in a block of 64 177 instead of 153.
 int tree_terms_block(const TreeParams& p) {
     const int G = p.heads / p.kv_heads, rows = p.most * G;
     const bool half = p.q_type == PA_TYPE_F32 && p.kv_type == PA_TYPE_F16, bytes = p.kv_type == PA_TYPE_I8 && p.dim == 128;
