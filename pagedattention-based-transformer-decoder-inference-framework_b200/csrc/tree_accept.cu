@@ -15,11 +15,12 @@
 namespace pa {
 namespace accept {
 
-constexpr int kThreads = 128, kMostCaches = 64, kBatch = 4;
+constexpr int kThreads = 128, kBatch = 4;
 
-struct Caches {
-    void* p[kMostCaches][4];            // keys, values, their scales (or null)
-    const int32_t* table[kMostCaches];
+// of a launch: as many as its arguments hold (issuing 64 caches' addresses takes longer than 16's)
+template <int MOST> struct Caches {
+    void* p[MOST][4];                   // keys, values, their scales (or null)
+    const int32_t* table[MOST];
 };
 
 struct Args {
@@ -62,7 +63,8 @@ __device__ __forceinline__ void move_rows(uint8_t* pool, int row_bytes, const in
     }
 }
 
-__global__ void __launch_bounds__(kThreads) tree_accept_kernel(const Args a, const __grid_constant__ Caches caches) {
+template <int MOST>
+__global__ void __launch_bounds__(kThreads) tree_accept_kernel(const Args a, const __grid_constant__ Caches<MOST> caches) {
     extern __shared__ int sm[];
     __shared__ int s_len;
     const int b = blockIdx.x, r0 = a.node_start[b], n = min(a.node_start[b + 1] - r0, a.most);
@@ -122,6 +124,22 @@ __global__ void __launch_bounds__(kThreads) tree_accept_kernel(const Args a, con
     }
 }
 
+// caches c0 .. of the call; the first launch also writes what was accepted
+template <int MOST>
+static cudaError_t launch(Args a, void* const* caches, int c0, int num_caches, cudaStream_t st) {
+    Caches<MOST> cs;
+    a.num_caches = num_caches - c0 < MOST ? num_caches - c0 : MOST;
+    if (c0 > 0) a.counts = nullptr;
+    for (int c = 0; c < a.num_caches; ++c) {
+        for (int k = 0; k < 4; ++k) cs.p[c][k] = caches[5 * (c0 + c) + k];
+        cs.table[c] = static_cast<const int32_t*>(caches[5 * (c0 + c) + 4]);
+    }
+    const int items = a.num_caches * a.kv_heads * 2, per = kThreads / 32;
+    const int y = items <= per ? 1 : (items + per - 1) / per;
+    tree_accept_kernel<MOST><<<dim3((unsigned)a.num_seqs, (unsigned)(y < 65535 ? y : 65535)), kThreads, (size_t)4 * a.most * sizeof(int), st>>>(a, cs);
+    return cudaGetLastError();
+}
+
 }  // namespace accept
 }  // namespace pa
 
@@ -141,21 +159,9 @@ PA_API int pa_tree_accept(const int32_t* d_ids, const int32_t* d_tokens, const i
     Args a{d_ids, d_tokens, d_parents, d_node_start, d_ctx_lens, d_beam_ids, num_seqs, most_nodes, depth, num_beams, kv_heads, num_tiles,
            total_pages, tile_size, {key_bytes, value_bytes}, 0, d_counts, d_out_tokens, d_nodes, d_new_lens};
     for (int c = 0; c < num_caches; ++c) PA_CHECK_ARG(caches[5 * c] && caches[5 * c + 4]);
-    int c0 = 0;
-    do {
-        Caches cs;
-        a.num_caches = num_caches - c0 < kMostCaches ? num_caches - c0 : kMostCaches;
-        for (int c = 0; c < a.num_caches; ++c) {
-            for (int k = 0; k < 4; ++k) cs.p[c][k] = caches[5 * (c0 + c) + k];
-            cs.table[c] = static_cast<const int32_t*>(caches[5 * (c0 + c) + 4]);
-        }
-        const int items = a.num_caches * kv_heads * 2, per = kThreads / 32;
-        const int y = items <= per ? 1 : (items + per - 1) / per;
-        tree_accept_kernel<<<dim3((unsigned)num_seqs, (unsigned)(y < 65535 ? y : 65535)), kThreads, (size_t)4 * most_nodes * sizeof(int), as_stream(stream)>>>(a, cs);
-        const cudaError_t e = cudaGetLastError();
+    for (int c0 = 0; c0 == 0 || c0 < num_caches; c0 += 64) {
+        const cudaError_t e = num_caches - c0 <= 16 ? launch<16>(a, caches, c0, num_caches, as_stream(stream)) : launch<64>(a, caches, c0, num_caches, as_stream(stream));
         if (e != cudaSuccess) return (int)e;
-        a.counts = nullptr;
-        c0 += a.num_caches;
-    } while (c0 < num_caches);
+    }
     return PA_OK;
 }

@@ -333,6 +333,18 @@ def on_device(device):
     return torch.cuda.device(device)
 
 
+def stream_on(device):
+    """Raw handle of the current stream of a tensor's device."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def capturing(raw_stream):
+    """Whether the current stream, whose handle this is, records a graph.  The legacy stream cannot."""
+    import torch
+    return raw_stream != 0 and torch._C._cuda_isCurrentStreamCapturing()
+
+
 def device_info():
     sm, maj, mnr = _i32(), _i32(), _i32()
     check(lib().pa_device_info(C.byref(sm), C.byref(maj), C.byref(mnr)), "pa_device_info")

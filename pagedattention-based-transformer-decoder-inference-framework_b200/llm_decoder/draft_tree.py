@@ -139,12 +139,12 @@ def paged_tree_attention(q, kv_cache, tree, ctx_lens, temperature=1.0, beam_ids=
         return out
     lib = _cabi.lib()
     table = pt.device_data()
+    need = tree._space.get((H, KVH, D))
     with _cabi.on_device(dev):
-        stream = _cabi.stream()
-        need = tree._space.get((H, KVH, D))
+        stream = _cabi.stream_on(dev)
         if need is None:
             need = tree._space[(H, KVH, D)] = lib.pa_tree_attention_workspace_bytes(R, tree.num_seqs, tree.most, H, KVH, D)
-        if torch._C._cuda_isCurrentStreamCapturing():           # a graph has a workspace of its own: its replays may run beside other calls
+        if _cabi.capturing(stream):     # a graph has a workspace of its own: its replays may run beside other calls
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
         else:
             ws = kv_cache._ws.get(("tree", stream))
@@ -220,5 +220,5 @@ def tree_accept(ids, tree, caches, ctx_lens, beam_ids=None):
         _cabi.check(_cabi.lib().pa_tree_accept(
             ids.data_ptr(), tree.tokens.data_ptr(), tree.parents.data_ptr(), tree.node_start.data_ptr(), B, tree.most, tree.depth,
             ctx_lens.data_ptr(), _cabi.ptr(beam_ids), *caches._geometry, len(caches.caches), caches._array, counts.data_ptr(),
-            tokens.data_ptr(), nodes.data_ptr(), lens.data_ptr(), _cabi.stream()), "pa_tree_accept")
+            tokens.data_ptr(), nodes.data_ptr(), lens.data_ptr(), _cabi.stream_on(dev)), "pa_tree_accept")
     return Accepted(counts, tokens, nodes, lens)

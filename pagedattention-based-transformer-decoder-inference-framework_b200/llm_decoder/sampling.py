@@ -140,10 +140,10 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
         return
     lib = _cabi.lib()
     with _cabi.on_device(dev):
-        stream, ws, need = _cabi.stream(), None, 0
+        stream, ws, need = _cabi.stream_on(dev), None, 0
         if ids is not None:     # words that every call leaves at zero, one buffer per stream
             need = lib.pa_adjust_logits_workspace_bytes(rows)
-            if torch._C._cuda_isCurrentStreamCapturing():       # a graph has words of its own: its replays may run beside other calls
+            if _cabi.capturing(stream):         # a graph has words of its own: its replays may run beside other calls
                 ws = torch.zeros(need, dtype=torch.uint8, device=dev)
             else:
                 ws = _rule_words.get((dev.index, stream))
