@@ -628,8 +628,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeWo
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.group;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int w0 = blockIdx.x;
+    int4 n0, n1;
     if constexpr (SPLIT > 1) {
         __shared__ int s_count[kJoinWarps], s_found;
+        __shared__ int4 s_note[2];
         const int per = (a.workers + kJoinWarps * 32 - 1) / (kJoinWarps * 32);
         uint32_t noted = 0;             // a thread has `per` shares, at most 32 (a trip to L2 each, eight under way at a time)
         for (int i0 = 0; i0 < per; i0 += 8) {
@@ -641,6 +643,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeWo
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) noted |= rows[i] > 0 ? 1u << (i0 + i) : 0u;
+        }
+        // the first note of a thread comes along: one is all that most have
+        const int4* mine0 = reinterpret_cast<const int4*>(a.notes + threadIdx.x * per + max(__ffs(noted) - 1, 0));
+        int4 a0 = make_int4(0, 0, 0, 0), a1 = a0;
+        if (noted) {
+            a0 = __ldcg(mine0);
+            a1 = __ldcg(mine0 + 1);
         }
         const int mine = __popc(noted);
         int before = mine;
@@ -655,15 +664,27 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeWo
         before -= mine;
         for (int k = 0; k < warp; ++k) before += s_count[k];
         if ((int)blockIdx.x >= before && (int)blockIdx.x < before + mine) {
-            for (int left = blockIdx.x - before; left > 0; --left) noted &= noted - 1;
-            s_found = threadIdx.x * per + __ffs(noted) - 1;
+            const int left = blockIdx.x - before;
+            for (int k = left; k > 0; --k) noted &= noted - 1;
+            const int w = threadIdx.x * per + __ffs(noted) - 1;
+            if (left > 0) {
+                a0 = __ldcg(reinterpret_cast<const int4*>(a.notes + w));
+                a1 = __ldcg(reinterpret_cast<const int4*>(a.notes + w) + 1);
+            }
+            s_found = w;
+            s_note[0] = a0;
+            s_note[1] = a1;
         }
         __syncthreads();
         w0 = s_found;
         if (w0 < 0) return;
+        n0 = s_note[0];
+        n1 = s_note[1];
+    } else {
+        const int4* note = reinterpret_cast<const int4*>(a.notes + w0);
+        n0 = __ldcg(note);
+        n1 = __ldcg(note + 1);
     }
-    const int4* note = reinterpret_cast<const int4*>(a.notes + w0);
-    const int4 n0 = __ldcg(note), n1 = __ldcg(note + 1);
     const int w1 = n1.x;
     const int64_t step = (int64_t)2 * a.block * LD;
     const float *rest = a.part + (int64_t)2 * w0 * a.block * LD, *first = a.part + (int64_t)n1.y * a.block * LD;       // share w's piece, w > w0; the first
