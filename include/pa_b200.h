@@ -1043,8 +1043,9 @@ int pa_conv_append_in_words(int units, int columns, int num_items, int64_t rows)
  *     a bit of d_allowed that is 0: x = -inf
  *   penalties per sequence (device arrays), or one value where the array is NULL.  Biases of sequence b are the entries
  *   d_bias_start[b] .. of (d_bias_ids, d_bias); of entries for the same token the last counts.  d_allowed: rows of
- *   allowed_stride 32-bit words, row d_allowed_rows[r] (NULL: r; negative: everything is allowed).  Tokens outside the
- *   vocabulary are ignored.  d_out (NULL: not wanted; may be d_logits) gets the logits in their type, d_ids (NULL: not wanted)
+ *   allowed_stride 32-bit words, row d_allowed_rows[r] (NULL: r; outside [0, mask_rows): everything is allowed).  Tokens outside
+ *   the vocabulary are ignored; a row whose sequence is outside [0, num_seqs) has no history and no biases, and starts reach no further than
+ *   history_tokens and bias_entries.  d_out (NULL: not wanted; may be d_logits) gets the logits in their type, d_ids (NULL: not wanted)
  *   the lowest index of the largest float before it is rounded (NaN never wins; 0 where nothing does); d_ids take a workspace
  *   that is zero before the first call and left so by every call.
  * pa_draft_trees (host arrays): from the nodes' parents (numbers within the sequence; -1 for node 0, a lower node for every other, else
@@ -1069,10 +1070,11 @@ int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void* d_out
                       int tile_size, float temperature, void* d_workspace, size_t workspace_bytes, pa_stream_t stream);
 size_t pa_adjust_logits_workspace_bytes(int rows);
 int pa_adjust_logits(const void* d_logits, int type, int64_t stride, int rows, int vocab, void* d_out, int64_t out_stride,
-                     int32_t* d_ids, const int32_t* d_row_seq, const int32_t* d_history, const int32_t* d_history_start,
+                     int32_t* d_ids, const int32_t* d_row_seq, int num_seqs, const int32_t* d_history, int history_tokens,
+                     const int32_t* d_history_start,
                      const float* d_repetition, const float* d_presence, const float* d_frequency, float repetition, float presence,
-                     float frequency, const int32_t* d_bias_ids, const float* d_bias, const int32_t* d_bias_start,
-                     const int32_t* d_allowed, int64_t allowed_stride, const int32_t* d_allowed_rows, const int32_t* d_tokens,
+                     float frequency, const int32_t* d_bias_ids, const float* d_bias, int bias_entries, const int32_t* d_bias_start,
+                     const int32_t* d_allowed, int mask_rows, int64_t allowed_stride, const int32_t* d_allowed_rows, const int32_t* d_tokens,
                      const int32_t* d_path, int path_words, const int32_t* d_node_start, void* d_workspace, size_t workspace_bytes,
                      pa_stream_t stream);
 int pa_draft_trees(const int64_t* parents, const int32_t* node_start, int num_seqs, int mask_words, int32_t* row_seq,

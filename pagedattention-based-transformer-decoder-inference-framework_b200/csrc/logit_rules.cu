@@ -39,6 +39,7 @@ struct Args {
     int32_t* ids;               // null: only logits
     int64_t stride, out_stride;
     int rows, vocab, chunk, chunks;                        // tokens of a chunk, chunks of a row
+    int num_seqs, history_tokens, bias_entries, mask_rows;  // bounds of what the device arrays below may name
     const int32_t *history, *history_start, *row_seq;
     const float *repetition, *presence, *frequency;        // per sequence; null: the value beside it
     float repetition1, presence1, frequency1;
@@ -103,23 +104,24 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // ---- bounds and bits that nothing waits for yet
     const int b = a.row_seq ? __ldg(a.row_seq + r) : r;
+    const bool known = (unsigned)b < (unsigned)a.num_seqs;  // no sequence of the call: no history and no biases
     int h0 = 0, h1 = 0, i0 = 0, i1 = 0, s0 = 0, s1 = 0;
-    if (a.history) {
-        h0 = __ldg(a.history_start + b);
-        h1 = __ldg(a.history_start + b + 1);
+    if (a.history && known) {
+        h0 = max(__ldg(a.history_start + b), 0);
+        h1 = min(__ldg(a.history_start + b + 1), a.history_tokens);
     }
-    if (a.bias) {
-        i0 = __ldg(a.bias_start + b);
-        i1 = __ldg(a.bias_start + b + 1);
+    if (a.bias && known) {
+        i0 = max(__ldg(a.bias_start + b), 0);
+        i1 = min(__ldg(a.bias_start + b + 1), a.bias_entries);
     }
-    if (a.tokens) {
-        s0 = __ldg(a.node_start + b);
-        s1 = min(__ldg(a.node_start + b + 1), s0 + 32 * a.path_words);
+    if (a.tokens && known) {
+        s0 = max(__ldg(a.node_start + b), 0);
+        s1 = min(min(__ldg(a.node_start + b + 1), a.rows), s0 + 32 * a.path_words);
     }
     const int64_t mrow = a.allowed_rows ? __ldg(a.allowed_rows + r) : r;
-    const uint32_t* allowed = a.allowed && mrow >= 0 ? a.allowed + mrow * a.allowed_stride + (v0 >> 5) : nullptr;
-    const float rep = a.repetition ? __ldg(a.repetition + b) : a.repetition1, pres = a.presence ? __ldg(a.presence + b) : a.presence1;
-    const float freq = a.frequency ? __ldg(a.frequency + b) : a.frequency1;
+    const uint32_t* allowed = a.allowed && mrow >= 0 && mrow < a.mask_rows ? a.allowed + mrow * a.allowed_stride + (v0 >> 5) : nullptr;
+    const float rep = a.repetition && known ? __ldg(a.repetition + b) : a.repetition1, pres = a.presence && known ? __ldg(a.presence + b) : a.presence1;
+    const float freq = a.frequency && known ? __ldg(a.frequency + b) : a.frequency1;
     if (a.history || a.tokens || a.bias)
         for (int i = tid; i < a.chunk / 4; i += kThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
     if (ROUNDS || a.allowed) {
@@ -364,20 +366,22 @@ using namespace pa;
 PA_API size_t pa_adjust_logits_workspace_bytes(int rows) { return rows > 0 ? (size_t)rows * 8 : 0; }
 
 PA_API int pa_adjust_logits(const void* d_logits, int type, int64_t stride, int rows, int vocab, void* d_out, int64_t out_stride,
-                            int32_t* d_ids, const int32_t* d_row_seq, const int32_t* d_history, const int32_t* d_history_start,
+                            int32_t* d_ids, const int32_t* d_row_seq, int num_seqs, const int32_t* d_history, int history_tokens, const int32_t* d_history_start,
                             const float* d_repetition, const float* d_presence, const float* d_frequency, float repetition, float presence,
-                            float frequency, const int32_t* d_bias_ids, const float* d_bias, const int32_t* d_bias_start,
-                            const int32_t* d_allowed, int64_t allowed_stride, const int32_t* d_allowed_rows, const int32_t* d_tokens,
+                            float frequency, const int32_t* d_bias_ids, const float* d_bias, int bias_entries, const int32_t* d_bias_start,
+                            const int32_t* d_allowed, int mask_rows, int64_t allowed_stride, const int32_t* d_allowed_rows, const int32_t* d_tokens,
                             const int32_t* d_path, int path_words, const int32_t* d_node_start, void* d_workspace, size_t workspace_bytes,
                             pa_stream_t stream) {
     using namespace pa::rules;
     PA_CHECK_ARG(rows >= 0 && vocab > 0 && stride >= vocab && (!d_out || out_stride >= vocab) && (d_out || d_ids));
     if (rows == 0) return PA_OK;
+    PA_CHECK_ARG(num_seqs >= 0 && history_tokens >= 0 && bias_entries >= 0 && mask_rows >= 0);
     PA_CHECK_ARG(d_logits && (!d_history || d_history_start) && (!d_bias || (d_bias_ids && d_bias_start)));
     PA_CHECK_ARG((!d_allowed || allowed_stride >= ((int64_t)vocab + 31) / 32) && (!d_tokens || (d_path && path_words > 0 && d_node_start && d_row_seq)));
     if (d_ids && (!d_workspace || (uintptr_t)d_workspace % 8 || workspace_bytes < pa_adjust_logits_workspace_bytes(rows))) return PA_ERR_WORKSPACE;
     Args a{};
     a.logits = d_logits; a.out = d_out; a.ids = d_ids; a.stride = stride; a.out_stride = out_stride; a.rows = rows; a.vocab = vocab;
+    a.num_seqs = num_seqs; a.history_tokens = history_tokens; a.bias_entries = bias_entries; a.mask_rows = mask_rows;
     a.history = d_history; a.history_start = d_history_start; a.row_seq = d_row_seq;
     a.repetition = d_repetition; a.presence = d_presence; a.frequency = d_frequency;
     a.repetition1 = repetition; a.presence1 = presence; a.frequency1 = frequency;

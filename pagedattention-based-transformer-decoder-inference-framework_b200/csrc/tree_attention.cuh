@@ -62,7 +62,7 @@ struct TreeSeq {
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b, int block, int unit) {
     TreeSeq s;
-    s.r0 = __ldg(p.node_start + b);
+    s.r0 = max(__ldg(p.node_start + b), 0);
     s.n = max(min(__ldg(p.node_start + b + 1), p.rows) - s.r0, 0);
     s.ctx = max(__ldg(p.ctx_lens + b), 0);
     const int64_t cap = min((int64_t)p.num_tiles * p.tile_size, (int64_t)0x7fffff00);

@@ -130,12 +130,15 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
         b_ids, b_val, b_start = bias
         p_ids, p_val = of(b_ids, i32, "bias tokens"), of(b_val, f32, "bias values", b_ids.numel())
         p_bias = of(b_start, i32, "bias starts", None if seqs is None else seqs + 1)
+        seqs = b_start.numel() - 1
+    masks = (0, 0)              # rows of masks, words from one to the next
     if allowed is not None:
         if allowed.dim() != 2 or allowed.dtype != torch.int32 or allowed.device != dev or allowed.shape[1] * 32 < V or \
                 (allowed.numel() and allowed.stride(1) != 1) or (allowed_rows is None and allowed.shape[0] != rows):
             raise ValueError("allowed: int32 [rows, words], 32 tokens a word, the logits' vocabulary")
         if allowed_rows is not None:
             p_rows = of(allowed_rows, i32, "allowed_rows", rows)
+        masks = (allowed.shape[0], allowed.stride(0) if allowed.shape[0] > 1 else allowed.shape[1])
     if rows == 0:
         return
     lib = _cabi.lib()
@@ -152,9 +155,8 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
         # (the stride of a single row may be anything)
         _cabi.check(lib.pa_adjust_logits(
             logits.data_ptr(), kind, stride if rows > 1 else V, rows, V, _cabi.ptr(out), 0 if out is None else out.stride(0) if rows > 1 else V,
-            _cabi.ptr(ids), p_seq, p_history, p_start, *arrays, *values, p_ids, p_val, p_bias, _cabi.ptr(allowed),
-            0 if allowed is None else allowed.stride(0) if allowed.shape[0] > 1 else allowed.shape[1], p_rows, *paths, _cabi.ptr(ws), need,
-            stream), "pa_adjust_logits")
+            _cabi.ptr(ids), p_seq, seqs or 0, p_history, history.numel() if p_history else 0, p_start, *arrays, *values, p_ids, p_val,
+            b_ids.numel() if p_ids else 0, p_bias, _cabi.ptr(allowed), *masks, p_rows, *paths, _cabi.ptr(ws), need, stream), "pa_adjust_logits")
 
 
 def adjust_logits(logits, history=None, history_start=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None,
@@ -168,7 +170,7 @@ def adjust_logits(logits, history=None, history_start=None, repetition=1.0, pres
     repetition, presence, frequency: a number, or a float32 tensor per sequence.
     bias: (tokens, values, start [sequences + 1]); of two entries for a token the last counts.
     allowed: int32 [rows, words], bit v & 31 of word v >> 5 for token v; with allowed_rows, the mask of row r is allowed[allowed_rows[r]],
-    and a negative one allows everything.
+    and a number that there is no mask for allows everything.
     row_seq: the sequence of every row (None: row r is sequence r).  tree: the rows are the nodes of a DraftTree with tokens; the
     tokens on a node's path, its own among them, count as history.
     out: a tensor like logits (also logits itself)."""

@@ -203,3 +203,26 @@ def test_refusals():
     for bad in (x.double(), x[0], x.cpu(), x.t(), x[:1].expand(3, 64)):
         with pytest.raises(ValueError):
             sampling.adjust_logits(bad)
+
+
+@pytest.mark.gpu
+def test_numbers_outside_the_arrays_read_nothing():
+    """Rows of sequences that the call has not, mask rows that there are not and starts behind the lists: as without the rule."""
+    import llm_decoder as ld
+    V = 500
+    x = torch.from_numpy(np.random.default_rng(14).standard_normal((6, V)).astype(np.float32)).cuda()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    history, start = i32([3, 4, 5, 6]), i32([0, 2, 900])
+    rep = torch.tensor([2.0, 2.0], device="cuda")
+    masks = torch.zeros((2, 16), dtype=torch.int32, device="cuda")
+    seq, rows = i32([0, 1, 2, -1, 1 << 30, 0]), i32([-1, 2, 1 << 30, -(1 << 31), 5, 0])
+    bias = (i32([7, 8]), torch.tensor([1.5, -2.5], device="cuda"), i32([0, 1, 1 << 20]))
+    got = ld.sampling.adjust_logits(x, history, start, rep, 0.25, 0.0, bias=bias, allowed=masks, allowed_rows=rows, row_seq=seq)
+    want = x.clone()
+    for r, (tokens, b) in enumerate([([3, 4], (7, 1.5)), ([5, 6], (8, -2.5)), ([], None), ([], None), ([], None)]):
+        for t in tokens:
+            want[r, t] = (want[r, t] / 2 if want[r, t] > 0 else want[r, t] * 2) - 0.25
+        if b:
+            want[r, b[0]] += b[1]
+    want[5] = -math.inf
+    assert torch.equal(got, want)
