@@ -15,7 +15,7 @@
 // rows: 208 us, 5.3 TB/s), narrower ones and int8 pages the chain of a unit, wait, products, softmax, products, that one to four warps of an SM's
 // quarter cover for each other (16 sequences of 4K keys, 12 heads of 64, float queries: 58 us, 3.5 TB/s; instructions issue half of the time).  Keys
 // come by the warp because few rows give no tile to share, and units of 16 because a page is that long; a smaller unit is the finest cut of a long
-// context (one sequence of 333 keys, 12 heads: 14.5 us, of which 6 are the join and its launch).
+// context (one sequence of 333 keys, 12 heads: 14.0 us, of which 5 are the join and its launch).
 //
 // A value that is not finite in a drafted row does not reach the rows that do not see it: a unit of drafted keys with such values takes
 // them out of the product and adds them for the rows that see them.

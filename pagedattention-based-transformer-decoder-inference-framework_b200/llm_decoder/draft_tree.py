@@ -215,7 +215,8 @@ def tree_accept(ids, tree, caches, ctx_lens, beam_ids=None):
         lens.copy_(ctx_lens)
         return Accepted(counts, tokens, nodes, lens)
     for t in caches.tables:
-        t.flush()
+        if t._pending:
+            t.flush()
     with _cabi.on_device(dev):
         _cabi.check(_cabi.lib().pa_tree_accept(
             ids.data_ptr(), tree.tokens.data_ptr(), tree.parents.data_ptr(), tree.node_start.data_ptr(), B, tree.most, tree.depth,
