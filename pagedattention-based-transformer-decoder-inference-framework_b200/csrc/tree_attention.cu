@@ -145,10 +145,11 @@ PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void
     }
     if (f.block) {
         if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < tree_work_bytes(num_seqs, f.workers, f.block, head_dim)) return PA_ERR_WORKSPACE;
-        const TreeWork w{p, f.workers, kTreeLeast, f.block, f.unit, total_pages * tile_size, f.extra, kTreeStreamScale, tc::kPolls, static_cast<TreeNote*>(d_workspace),
+        const bool whole = (int64_t)num_tiles * tile_size <= (f.unit == 16 ? kTreeWholeStream : kTreeWhole) && tree_items(p, f.block) <= f.workers;
+        const TreeWork w{p, f.workers, kTreeLeast, f.block, f.unit, total_pages * tile_size, f.extra, whole, kTreeStreamScale, tc::kPolls, static_cast<TreeNote*>(d_workspace),
                          reinterpret_cast<float*>(static_cast<TreeNote*>(d_workspace) + f.workers)};
         int rc = f.launch(w, st);
-        if (rc == PA_OK) rc = tree_join_launch(w, st);
+        if (rc == PA_OK && !whole) rc = tree_join_launch(w, st);
         if (rc != PA_ERR_UNSUPPORTED) return rc;
     }
 #define PA_TREE(QT, QC, KT, KC) if (q_type == QT && kv_type == KT) return launch_rows<QC, KC>(p, st);

@@ -56,6 +56,11 @@ constexpr int kTreeLeast = 2;           // units of a share, where there are tha
 // 8 bf16 rows 188 -> 161 us (8: 164, 16: 168).
 constexpr int kTreeTcExtra = 8, kTreeTermsExtra = 6, kTreeStreamExtra = 4;
 
+// Items are left whole, and nothing is joined, where the page table has room for no more than this many keys and every worker has an item at most: a
+// warp that streams 16 keys at a time passes 6 such units in the time of the join, the tcgen05 kernels 512 keys.  us, whole against cut: 2 sequences of 57 keys, 16 rows,
+// 9.9 against 12.8; 4 of 181 in the streaming kernel 23.9 against 15.7; 45 of up to 309 on tcgen05 18 against 25, 9 of 116 18 against 24; 4 of 554 20 against 16.
+constexpr int kTreeWholeStream = 96, kTreeWhole = 512;
+
 struct TreeSeq {
     int r0, n, ctx, keys, blocks, steps;
     __device__ __forceinline__ int units(int extra) const { return steps > 0 ? blocks * (steps + extra) : 0; }     // of one kv head
@@ -94,6 +99,7 @@ struct TreeWork {
     TreeParams p;
     int workers, least, block, unit, total_rows;
     int extra;                          // units before an item's steps in the list: what beginning and ending an item costs
+    bool whole;                         // shares end with items: no item is cut, and nothing is joined
     float p_scale;                      // the partial sums are times this (softmax weights enter products so that small halves keep their bits)
     uint32_t polls;                     // of a wait
     TreeNote* notes;                    // [workers]
@@ -116,6 +122,11 @@ __device__ __forceinline__ TreeNote tree_note(const TreeWork& a, const TreeSeq& 
         t.slot = (int)slot;
     }
     return t;
+}
+
+// items of a call, at most
+static inline int64_t tree_items(const TreeParams& p, int block) {
+    return p.kv_heads * (((int64_t)p.rows * p.group + (int64_t)p.num_seqs * (block - 1)) / block);
 }
 
 // tree_stream.cu: few query rows; the join of pieces

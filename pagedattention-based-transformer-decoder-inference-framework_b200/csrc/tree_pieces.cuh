@@ -30,6 +30,15 @@ struct TreeWalk {
         u = (int)(rem - (int64_t)item * each);
         g = item / sq.blocks;
         rb = item - g * sq.blocks;
+        if (w.whole) {                      // both ends back to where their items begin
+            f -= u;
+            u = 0;
+            if (f_hi < total) {
+                const int b1 = shares::find_token(pre, w.p.num_seqs, f_hi, w.p.kv_heads);
+                f_hi -= (f_hi - (int64_t)pre[b1] * w.p.kv_heads) % (tree_seq(w.p, b1, w.block, w.unit).steps + w.extra);
+            }
+            if (f >= f_hi) return;
+        }
         if (u + (f_hi - f) <= w.extra) f = f_hi;            // no step of the item is this share's
     }
     __device__ __forceinline__ bool next() {

@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
         const TreeSeq q = tree_seq(p, b, MT * 16, kUnit);
         const int64_t rem = c - (int64_t)cut[b] * p.kv_heads;
         const int each = q.steps + a.extra, item = (int)(rem / each);
-        return (int64_t)pre[b] * p.kv_heads + (int64_t)item * q.steps + max((int)(rem - (int64_t)item * each) - a.extra, 0);
+        return (int64_t)pre[b] * p.kv_heads + (int64_t)item * q.steps + (a.whole ? 0 : max((int)(rem - (int64_t)item * each) - a.extra, 0));
     };
     const int64_t at = w < ns ? unit_at(total * (w + (lane & 1)) / ns) : 0;         // even lanes: the beginning, odd ones: the end
     const int64_t f_lo = __shfl_sync(0xffffffffu, at, 0), f_hi = __shfl_sync(0xffffffffu, at, 1);
@@ -838,7 +838,7 @@ int tree_join_launch(const TreeWork& a, cudaStream_t st) {
     using namespace tstream;
     const TreeParams& p = a.p;
     // pieces of an item, were all items alike: from 16 (64) on a row's pieces are shared by four (eight) warps
-    const int64_t items = p.kv_heads * (((int64_t)p.rows * p.group + (int64_t)p.num_seqs * (a.block - 1)) / a.block);       // at most
+    const int64_t items = tree_items(p, a.block);
     const int split = a.workers > 32 * kJoinWarps * 32 ? 1 : a.workers >= 64 * items ? 8 : a.workers >= 16 * items ? 4 : 1;
 #define PA_TJN(Q, NV)                                                                                                  \
     return split == 8 ? join<Q, NV, 8, 1>(a, items, st) : split == 4 ? join<Q, NV, 4, 1>(a, items, st)                 \

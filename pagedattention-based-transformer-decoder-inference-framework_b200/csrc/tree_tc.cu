@@ -536,14 +536,14 @@ int tree_tc_workers(int block) { return device_info().sm_count * (block == 128 ?
 
 // Rows of a block, 0 where this kernel does not serve or the streaming one is faster.  us, this kernel against the streaming one: 64 rows a head (32
 // sequences, 4K keys, 8 kv heads) 113 against 235, 32 rows 106 against 132, 16 rows 104 against 106, 8 rows and 32 kv heads 191 against 189, ragged
-// contexts 168 against 161: from 17 on. Blocks of 128 rows against 256: 128 rows a head 126 against 142, 64 rows 113 against 135; 256 rows a head
-// read everything once in one block (89 us against 94).
+// contexts 168 against 161: from 17 on.  Blocks of 128 rows against 256: 128 rows a head 126 against 142, 64 rows 113 against 135; 160 rows (2K
+// keys) 121 against 99, 256 rows 130 against 112; 384 rows 102 against 104, 448 rows 80 against 83, 800 rows 45 against 47.
 int tree_tc_block(const TreeParams& p) {
     const int G = p.heads / p.kv_heads, rows = p.most * G;
     if (!((p.q_type == PA_TYPE_F16 && p.kv_type == PA_TYPE_F16) || (p.q_type == PA_TYPE_BF16 && p.kv_type == PA_TYPE_BF16)) || rows <= 16) return 0;
     if ((p.dim != 64 && p.dim != 128) || p.tile_size % 16 || p.num_seqs > kTreeMostSeqs) return 0;
     if ((int64_t)p.total_pages * p.tile_size >= 0x7fffff00ll || ((uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.q | (uintptr_t)p.out) % 16 || p.q_stride % 8) return 0;
-    const int block = rows <= 128 ? 128 : 256;
+    const int block = rows <= 128 || rows > 256 ? 128 : 256;
     const int64_t steps = ((int64_t)p.num_tiles * p.tile_size + ttc::KT - 1) / ttc::KT;
     return ((int64_t)p.rows * G / block + p.num_seqs) * (steps + kTreeTcExtra) < 0x7fffffff ? block : 0;     // the list's sums are 32 bits
 }
