@@ -22,11 +22,11 @@
 //
 // What bounds it: the latency of a tile's chain (scores, vote, weights, products, sums) at one or two softmax warps for each quarter of an SM, and
 // of a piece's beginning and end, some 6 us.  12 sequences of 4K keys, 32 heads: half pages and 32 float rows 152 us, 5.3 TB/s; int8 pages and 16
-// float rows 87 us, 4.8 TB/s; 48 sequences of 1 to 2K keys, int8 pages 126 us, 3.5 TB/s; 16 sequences of 4K keys, 128 rows a kv head (blocks of 64)
-// 131 us, 262 TFLOP/s of the formula's operations.  Rows as the columns of the products keep the tile at 128 keys for any number of rows: as rows
+// float rows 87 us, 4.8 TB/s; 48 sequences of 1 to 2K keys, int8 pages 124 us, 3.6 TB/s; 16 sequences of 4K keys, 128 rows a kv head (blocks of 64)
+// 133 us, 258 TFLOP/s of the formula's operations.  Rows as the columns of the products keep the tile at 128 keys for any number of rows: as rows
 // they would fill 128 lanes with 16.  Digits and terms instead of tf32 or a conversion to half: int8 pages stay as they are, and float results keep
 // 22 bits.  Reading a tile's maximum before its exponentials for every tile took 223 us where votes on 2^8 take 192 (before the shares counted
-// beginnings and ends: 126 now).
+// beginnings and ends: 124 now).
 #include "tcgen05_utils.cuh"
 #include "tree_pieces.cuh"
 
@@ -51,14 +51,13 @@ template <int D, bool I8, int R> struct Shape {
     static constexpr int Q_BYTES = N * 128 * (I8 ? 1 : D / 64), P_BYTES = KT * 128 * (R == 64 ? 2 : 1);
     static constexpr int Q_BUFS = Q_BYTES > 16384 ? 1 : 2;
     static constexpr int FREE = (CTAS == 2 ? 106 : 200) * 1024 - Q_BUFS * Q_BYTES;
-    static constexpr int P_BUFS = (FREE - 2 * P_BYTES) / SLOT >= 4 ? 2 : 1;
-    static constexpr int RING = (FREE - P_BUFS * P_BYTES) / SLOT < 12 ? (FREE - P_BUFS * P_BYTES) / SLOT : 12;
+    static constexpr int RING = (FREE - 2 * P_BYTES) / SLOT < 12 ? (FREE - 2 * P_BYTES) / SLOT : 12;       // weights are double-buffered
     static constexpr int COLS = 2 * N + 2 * NO, TMEM = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int NBAR = 2 * RING + 16;      // full, empty [ring]; s_full, p_full, o_full, o_empty, q_ready, q_free [2]; piece_done [4]
     static constexpr int FLOATS = 2 * R /*factors*/ + 2 * R /*references, thresholds*/ + 4 * R /*corrections*/ + 4 * R /*maxima*/ +
                                   4 * 5 * R /*sums, references at the end*/ + 2 * R /*what becomes of the sums*/ + 2 * 8 * R /*rows*/ + 28;
     static size_t smem(int seqs, int mask_words) {
-        return (size_t)RING * SLOT + Q_BUFS * Q_BYTES + P_BUFS * P_BYTES + NBAR * 8 + FLOATS * 4 + 2 * R * mask_words * 4 + kNotes * 4 + 64 + (seqs + 1) * 4 + 1024;
+        return (size_t)RING * SLOT + Q_BUFS * Q_BYTES + 2 * P_BYTES + NBAR * 8 + FLOATS * 4 + 2 * R * mask_words * 4 + kNotes * 4 + 64 + (seqs + 1) * 4 + 1024;
     }
 };
 
@@ -117,7 +116,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const TreeParams& p = a.p;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t q_sm = base + RING * C::TILE, p_sm = q_sm + C::Q_BUFS * C::Q_BYTES, sc_sm = p_sm + C::P_BUFS * C::P_BYTES, bar0 = sc_sm + RING * C::SCALES;
+    const uint32_t q_sm = base + RING * C::TILE, p_sm = q_sm + C::Q_BUFS * C::Q_BYTES, sc_sm = p_sm + 2 * C::P_BYTES, bar0 = sc_sm + RING * C::SCALES;
     auto kv_full = [&](int s) { return bar0 + s * 8; };
     auto kv_empty = [&](int s) { return bar0 + (RING + s) * 8; };
     auto s_full = [&](int i) { return bar0 + (2 * RING + i) * 8; };
@@ -295,7 +294,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                 wait(o_empty(sb), (t >> 1 & 1u) ^ 1u);          // the sums of tile t - 2 are taken
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t pb = p_sm + (C::P_BUFS == 2 ? sb : 0) * C::P_BYTES;
+                    const uint32_t pb = p_sm + sb * C::P_BYTES;
                     if constexpr (I8) {
                         const int ksteps = (nvalid + 31) >> 5;
                         for (int ks = 0; ks < ksteps; ++ks)
@@ -547,8 +546,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                     if (threadIdx.x == 0) s_scale[ring4] = big * (256.f / kDigits4);
                 }
                 // ---- weights: four rows' terms a 16-byte word
-                const uint32_t pb = p_sm + (uint32_t)((C::P_BUFS == 2 ? sb : 0) * C::P_BYTES) + kk * 128;
-                if (C::P_BUFS == 1 && t > 0) wait(o_full((t - 1) & 1), (t - 1) >> 1 & 1u);      // their place is read
+                const uint32_t pb = p_sm + (uint32_t)(sb * C::P_BYTES) + kk * 128;
 #pragma unroll
                 for (int r = 0; r < RH; r += 4) {
                     float e[4];
@@ -696,7 +694,7 @@ template <int D, bool I8, int R, typename Q>
 static int launch(const TreeWork& a, cudaStream_t st) {
     const TreeParams& p = a.p;
     typedef Shape<D, I8, R> C;
-    static_assert(C::COLS <= 512 && C::RING >= 4, "TMEM or shared memory");
+    static_assert(C::COLS <= 512 && C::RING >= 3, "TMEM or shared memory");
     const size_t smem = C::smem(p.num_seqs, p.mask_words);
     if (smem > (size_t)device_info().max_smem_optin) return PA_ERR_UNSUPPORTED;
     auto kern = tree_terms_kernel<D, I8, R, Q>;
@@ -715,10 +713,10 @@ static int launch(const TreeWork& a, cudaStream_t st) {
 int tree_terms_workers(int block) { return device_info().sm_count * (block == 16 ? 2 : 1); }
 
 // Rows of a block, 0 where this kernel does not serve or the streaming one is faster.  us, this kernel against the streaming one: int8 pages, 16
-// rows: 1000 keys 111 against 206, 4K keys 87 against 194, ragged 126 against 207, 100 keys 38 against 52; half pages, 32 float rows: 4K keys 153
+// rows: 1000 keys 107 against 206, 4K keys 87 against 194, ragged 124 against 207, 100 keys 38 against 52; half pages, 32 float rows: 4K keys 153
 // against 294, 1000 keys 189 against 307, 90 keys 92 against 72 (the host does not know how long contexts are); 16 float rows 205 against 209, and
 // of 64 columns 65 against 58: from 17 on.  int8 rows of 64 bytes have no tile here.  Blocks: int8, 256 rows in 32s 317, in 16s 370, 16 rows in a
-// block of 32 194 instead of 111; half, 128 rows in 64s 131, in 32s 196; 32 rows in a block of 64 177 instead of 153.
+// block of 32 194 instead of 107; half, 128 rows in 64s 133, in 32s 196; 32 rows in a block of 64 177 instead of 153.
 int tree_terms_block(const TreeParams& p) {
     const int G = p.heads / p.kv_heads, rows = p.most * G;
     const bool half = p.q_type == PA_TYPE_F32 && p.kv_type == PA_TYPE_F16, bytes = p.kv_type == PA_TYPE_I8 && p.dim == 128;
