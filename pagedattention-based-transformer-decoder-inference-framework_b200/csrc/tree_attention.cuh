@@ -3,8 +3,9 @@
 //
 // The rows of a sequence that share a kv head are its nodes' query heads: row rr = node * G + head of the group, G = heads / kv_heads.
 // An item is a block of `block` such rows of one (sequence, kv head) with the keys that its sequence has, in steps of `unit` keys.  The
-// list of all items' steps, sequence by sequence, kv head by kv head, block by block, is cut into equal contiguous shares
-// (decode_shares.cuh: as many as follow from the lengths alone).  A share that holds all of an item writes its rows' results; otherwise
+// list of all items' steps, sequence by sequence, kv head by kv head, block by block, `extra` units before each item's, is cut into equal
+// contiguous shares (decode_shares.cuh: their number follows from the lengths and the workers of the call).  A cut before an item's steps
+// is one at its beginning.  A share that holds all of an item writes its rows' results; otherwise
 // it leaves reference, sum and weighted sums of its piece in a slot, and a second kernel joins the pieces: the share in which such an
 // item begins notes it (TreeNote); the item's first piece is in slot 2 w + 1 of that share w unless the share begins with it, every other one
 // is the beginning of its share, in slot 2 w.
@@ -110,7 +111,7 @@ static inline size_t tree_work_bytes(int num_seqs, int workers, int block, int d
     (void)num_seqs;
     return (size_t)workers * sizeof(TreeNote) + (size_t)2 * workers * block * (dim + 4) * sizeof(float);
 }
-// by one thread of a worker: what it notes of the last piece of its share, steps [i0, i1) of an item that begins at step f_item of the list
+// by one thread of a worker: what it notes of the last piece of its share, steps [i0, i1) of an item that begins at unit f_item of the list
 __device__ __forceinline__ TreeNote tree_note(const TreeWork& a, const TreeSeq& s, int g, int rr0, int i0, int i1, int64_t f_item, int64_t total, int64_t ns, int64_t slot) {
     TreeNote t{};
     if (i0 == 0 && i1 < s.steps) {
