@@ -9,7 +9,8 @@
 //                   sums; twice the products, which the copies still cover
 //   int8 pools      bytes become halves in registers (1024 + 128 + b as a half, minus 1152: exact); the order of the summed columns and
 //                   keys is free as long as both factors have it, so every lane reads 16 bytes of a row at a time; a
-//                   key's scale goes to its scores, a value's to its weights
+//                   key's scale goes to its scores, a value's to its weights, which a row's power of two then brings between 2^14 and 2^15
+//                   unit by unit: halves hold the largest product of weight and 1 / scale, whatever it is, and all others to 2^-39 of it
 //
 // What bounds it: 16-bit pages of 128 columns the copies (32 sequences of 4K keys, 32 heads, 8 rows a head: 189 us, 5.7 TB/s; float queries, 16
 // rows: 208 us, 5.3 TB/s), narrower ones and int8 pages the chain of a unit, wait, products, softmax, products, that one to four warps of an SM's
@@ -51,6 +52,12 @@ __device__ __forceinline__ void mma_from_zero(float (&d)[4], const uint32_t (&a)
     else
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// to += x * by[row], two at a time
+__device__ __forceinline__ void add_four_times(float (&to)[4], const float (&x)[4], const float (&by)[2]) {
+#pragma unroll
+    for (int c = 0; c < 4; c += 2)
+        f32x2::unpack2(f32x2::fma2(f32x2::pack2(x[c], x[c + 1]), f32x2::pack2(by[c >> 1], by[c >> 1]), f32x2::pack2(to[c], to[c + 1])), to[c], to[c + 1]);
 }
 // to += x, two at a time
 __device__ __forceinline__ void add_four(float (&to)[4], const float (&x)[4]) {
@@ -418,6 +425,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
                 }
             }
             uint32_t pf[MT][TERMS][4];
+            float down[MT][2];              // int8: what a row's products are times
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 float mx[2] = {-INFINITY, -INFINITY};
@@ -464,6 +472,21 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
                         if constexpr (KT == I8) e = e != 0.f ? e * vsc[2 * n + (c & 1)] : 0.f;      // a key that nobody sees may have any scale
                         s[mt][n][c] = e;
                     }
+                if constexpr (KT == I8) {       // a row's largest between 2^14 and 2^15, see above
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float big = fmaxf(fmaxf(fabsf(s[mt][0][2 * i]), fabsf(s[mt][0][2 * i + 1])), fmaxf(fabsf(s[mt][1][2 * i]), fabsf(s[mt][1][2 * i + 1])));
+                        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                        const uint32_t e = max(__float_as_uint(big) >> 23, 15u);
+                        const float up = __uint_as_float((268u - e) << 23);
+                        down[mt][i] = __uint_as_float((e - 14u) << 23);
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) s[mt][n][2 * i + c] *= up;
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float x = s[mt][j >> 1][2 * (j & 1)], y = s[mt][j >> 1][2 * (j & 1) + 1];
@@ -475,11 +498,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
                 }
             }
             auto weigh = [&](int mt, int n, uint32_t b0, uint32_t b1) {
-                if constexpr (TWO) {
+                if constexpr (TWO || KT == I8) {
                     float t[4];
-                    mma_from_zero<BF>(t, pf[mt][1], b0, b1);
-                    mma<BF>(t, pf[mt][0], b0, b1);
-                    add_four(o[mt][n], t);
+                    mma_from_zero<BF>(t, pf[mt][TERMS - 1], b0, b1);
+                    if constexpr (TWO) mma<BF>(t, pf[mt][0], b0, b1);
+                    if constexpr (KT == I8) add_four_times(o[mt][n], t, down[mt]);
+                    else add_four(o[mt][n], t);
                 } else {
                     mma<BF>(o[mt][n], pf[mt][0], b0, b1);
                 }
