@@ -6,8 +6,9 @@
 //     S^T = K Q^T      [128 keys x terms R],   O^T = V^T P^T   [D x terms R],   R = 16, 32 or 64 query rows of a block
 //   half pages    two terms of half each for a query (its row scaled by a power of two first) and for a weight: 22 bits of every factor
 //   int8 pages    kind::i8 with signed digits: a query row as 23-bit integers relative to its largest (three digits), the weights times their
-//                 values' scales as 31-bit ones relative to the largest possible of a tile (four); products and their sums are exact
-//                 integers, no byte is converted
+//                 values' scales as 31-bit ones (four) relative to the largest possible, where a tile's values have scales alike; where they
+//                 have not, relative to the row's largest in the tile, so that a key which a row does not see, or hardly weighs, takes no bits from
+//                 the others.  Products and their sums are exact integers, no byte is converted
 // A row's reference moves only when a score exceeds it by more than 2^8, which the terms leave room for: after a piece's first tile
 // hardly ever.  (So the formula's 1e-6 stands beside a sum that may be up to 2^8 times the one relative to the largest score: 1e-6 of a result.)
 // The sums of a tile leave the tensor cores as they are and are added up in float registers (the tensor cores cut where float rounds: over a
@@ -38,6 +39,9 @@ using namespace tc;
 constexpr int KT = 128, kNotes = 32;
 constexpr float kDigits = 8.3e6f, kDigits4 = 2.1e9f;      // the largest number of three and of four signed digits, and some to spare
 constexpr float kRaise = 8.f;
+// Scales (1 / scale of a value) of a tile are alike within a factor of 8.  They are taken relative to twice the largest of the last such tile as long as
+// they lie within a factor of 16 below: weights have 23 bits at that scale and 19 at the far end.
+constexpr float kAlike = 8.f;
 
 __device__ int g_errors;
 
@@ -55,7 +59,7 @@ template <int D, bool I8, int R> struct Shape {
     static constexpr int COLS = 2 * N + 2 * NO, TMEM = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int NBAR = 2 * RING + 16;      // full, empty [ring]; s_full, p_full, o_full, o_empty, q_ready, q_free [2]; piece_done [4]
     static constexpr int FLOATS = 2 * R /*factors*/ + 2 * R /*references, thresholds*/ + 4 * R /*corrections*/ + 4 * R /*maxima*/ +
-                                  4 * 5 * R /*sums, references at the end*/ + 2 * R /*what becomes of the sums*/ + 2 * 8 * R /*rows*/ + 28;
+                                  4 * 5 * R /*sums, references at the end*/ + 2 * R /*what becomes of the sums*/ + 2 * 8 * R /*rows*/ + (I8 ? 8 * R : 0) /*units, largest products*/ + 28;
     static size_t smem(int seqs, int mask_words) {
         return (size_t)RING * SLOT + Q_BUFS * Q_BYTES + 2 * P_BYTES + NBAR * 8 + FLOATS * 4 + 2 * R * mask_words * 4 + kNotes * 4 + 64 + (seqs + 1) * 4 + 1024;
     }
@@ -107,6 +111,42 @@ __device__ __forceinline__ float from_digits4(uint32_t d0, uint32_t d1, uint32_t
     return fmaf((float)((int)d3 * 256 + (int)d2), 65536.f, (float)((int)d1 * 256 + (int)d0));
 }
 
+// Weights of a tile whose values have scales that are not alike, by all softmax threads, each a key's RH rows from h0 on: from floats in the place of the digits
+// (a word a row, see the softmax) to digits relative to the row's largest product of weight and scale; units: what the rows' sums are times.  A product that
+// is not finite makes its row's sums NaN.  Row by row through shared memory and out of line, since instructions are what the kernel's caches are short of
+// (48 sequences of 1 to 2K keys: 129 us, inline and in registers 138, without any of this 123).
+template <int R, int RH, int SOFTMAX>
+__device__ __noinline__ void digits_apart(uint32_t pb, int h0, float vsc, uint32_t* s_top, float* units) {
+    const int lane = threadIdx.x & 31, kk = threadIdx.x & 127, quarter = threadIdx.x >> 5 & 3;
+    auto group_sync = [&] { asm volatile("bar.sync 1, %0;" ::"n"(SOFTMAX) : "memory"); };
+    auto word = [&](int r) { return pb + (((h0 + r) >> 2 ^ (kk & 7)) << 4) + (r & 3) * 4; };
+#pragma unroll 1
+    for (int r = 0; r < RH; ++r) {
+        float e;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(e) : "r"(word(r)) : "memory");
+        e = e != 0.f ? e * vsc : 0.f;
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(word(r)), "f"(e) : "memory");
+        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(e) & 0x7fffffffu);
+        if (lane == 0) s_top[quarter * R + h0 + r] = top;
+    }
+    group_sync();
+    if (threadIdx.x < R) {
+        const int r = threadIdx.x;
+        const uint32_t top = max(max(s_top[r], s_top[R + r]), max(s_top[2 * R + r], s_top[3 * R + r]));
+        const bool finite = top < 0x7f800000u;
+        const float most = fmaxf(__uint_as_float(top), 1e-28f);
+        units[r] = finite ? __fdiv_rn(most, kDigits4) : __int_as_float(0x7fc00000);
+        s_top[r] = __float_as_uint(finite ? __fdiv_rn(kDigits4, most) : 0.f);
+    }
+    group_sync();
+#pragma unroll 1
+    for (int r = 0; r < RH; ++r) {
+        float y;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(word(r)) : "memory");
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(word(r)), "r"(digits4(__float2int_rn(y * __uint_as_float(s_top[h0 + r])))) : "memory");
+    }
+}
+
 template <int D, bool I8, int R, typename Q>
 __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTAS) tree_terms_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeWork a) {
     typedef Shape<D, I8, R> C;
@@ -131,15 +171,17 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
     // factors of the scores [2 pieces], references (less kShift) and whether rows have one, corrections of the last four tiles, maxima
     // by warp, sums by warp and references of the last four pieces, a piece's rows of the output and what their sums are
     // multiplied by; nodes and heads of the last eight
-    // pieces' rows (node -1: no row); scales of the last four tiles, largest scale by warp of the last two;
+    // pieces' rows (node -1: no row); int8: what the last four tiles' sums are times, largest products of weights and scales by warp;
+    // the unit of the scales and what gives integers of it, bits of the largest and the smallest scale by warp;
     // whether references moved in the last four tiles, whether the last four pieces are computed by rows,
     // whether a row has no reference yet
     float* fl = reinterpret_cast<float*>(smem_raw + (meta_sm + kNotes * 4 - smem_u32(smem_raw)));
-    float *s_fe = fl, *s_ref = fl + 2 * R, *s_set = fl + 3 * R, *s_corr = fl + 4 * R, *s_max = fl + 8 * R, *s_end = fl + 12 * R, *s_scale = fl + 50 * R,
-          *s_big = s_scale + 4;
+    float *s_fe = fl, *s_ref = fl + 2 * R, *s_set = fl + 3 * R, *s_corr = fl + 4 * R, *s_max = fl + 8 * R, *s_end = fl + 12 * R, *s_unit = fl + 50 * R;
+    uint32_t *s_top = reinterpret_cast<uint32_t*>(s_unit + (I8 ? 4 * R : 0)), *s_big = s_top + (I8 ? 4 * R : 0), *s_small = s_big + 4;
+    float* s_scale = reinterpret_cast<float*>(s_small + 4);
     int2* s_fin = reinterpret_cast<int2*>(fl + 32 * R);
     int *s_node = reinterpret_cast<int*>(fl + 34 * R), *s_head = s_node + 8 * R;         // (seven pieces at most are on their way)
-    int *s_moved = reinterpret_cast<int*>(s_big + 8), *s_odd = s_moved + 4, *s_pending = s_odd + 4, *pre = s_pending + 4;
+    int *s_moved = reinterpret_cast<int*>(s_scale + 8), *s_odd = s_moved + 4, *s_pending = s_odd + 4, *pre = s_pending + 4;
     uint32_t* s_mask = reinterpret_cast<uint32_t*>(pre + p.num_seqs + 1);      // [2 pieces][R][mask_words]
     auto failed = [&] { return tc_failed(fail_sm); };
     auto wait = [&](uint32_t bar, uint32_t parity) { tc_wait(bar, parity, fail_sm, a.polls); };
@@ -428,6 +470,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
         auto fresh = [&] {                  // no references yet
             if (threadIdx.x < R) s_ref[threadIdx.x] = s_set[threadIdx.x] = 0.f;
             if (threadIdx.x == 0) *s_pending = 1;
+            if (I8 && threadIdx.x == 0) s_scale[0] = s_scale[1] = 0.f;
         };
         fresh();
         while (w.next()) {
@@ -458,8 +501,6 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vs) : "r"(sc + 512) : "memory");
                     ksc = here ? __frcp_rn(ks) : 1.f;
                     vsc = here ? __frcp_rn(vs) : 0.f;
-                    const uint32_t top = __reduce_max_sync(0xffffffffu, ordered(vsc));
-                    if (lane == 0) s_big[sb * 4 + quarter] = unordered(top);       // both halves the same
                 } else if (drafts) {        // values that are not finite (rows past the last key: zeros, or looked at in vain)
                     const uint32_t c = v_at(at, i, nt);
                     wait(kv_full(slot_of(c)), phase_of(c));
@@ -479,6 +520,9 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                 const int bit = kp - w.sq.ctx;              // of the rows' masks, where it is not negative
                 const bool masked = drafts && here && bit >= 0, hidden = !here || (masked && (bit >> 5) >= p.mask_words);
                 float s[RH];
+                // a value's scale that lies outside the range of the unit (or is not finite) is a reason, too
+                const float by = I8 ? s_scale[0] : 0.f;
+                const bool strange = I8 && here && !(fabsf(vsc) <= by && 16.f * fabsf(vsc) >= by);
                 bool over = false;
 #pragma unroll
                 for (int c = 0; c < RH / CH; ++c) {
@@ -510,9 +554,19 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                         over |= s[r] > kRaise + kShift;
                     }
                 }
-                const bool any = group_any(over || *s_pending);
+                const bool any = group_any(over || strange || *s_pending);
                 if (threadIdx.x == 0) s_moved[ring4] = any;
+                const uint32_t pb = p_sm + (uint32_t)(sb * C::P_BYTES) + kk * 128;
+                if (I8 && threadIdx.x < R) s_unit[ring4 * R + threadIdx.x] = by * (256.f / kDigits4);
                 if (any) {
+                    if (I8) {
+                        const uint32_t bits = __float_as_uint(vsc) & 0x7fffffffu;       // what is not a number is above infinity
+                        const uint32_t most = __reduce_max_sync(0xffffffffu, bits), least = __reduce_min_sync(0xffffffffu, here ? bits : 0x7f7fffffu);
+                        if (lane == 0) {                                                // both halves the same
+                            s_big[quarter] = most;
+                            s_small[quarter] = least;
+                        }
+                    }
 #pragma unroll
                     for (int r = 0; r < RH; ++r) {
                         const uint32_t top = __reduce_max_sync(0xffffffffu, ordered(s[r] == s[r] ? s[r] : -INFINITY));
@@ -530,6 +584,16 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                         if (raise) s_set[r] = 1.f;
                         else if (!has && s_node[(pieces & 7) * R + r] >= 0) s_moved[ring4] = 2;        // still none
                     }
+                    float big = 0.f;            // int8: the tile's largest scale, if all are alike; infinity, if they are not
+                    if constexpr (I8) {
+                        const uint4 b4 = *reinterpret_cast<const uint4*>(s_big), s4 = *reinterpret_cast<const uint4*>(s_small);
+                        big = __uint_as_float(max(max(b4.x, b4.y), max(b4.z, b4.w)));
+                        if (!(big < 1e36f && (big == 0.f || big > 1e-28f) && big <= kAlike * __uint_as_float(min(min(s4.x, s4.y), min(s4.z, s4.w))))) big = INFINITY;
+                        if (threadIdx.x == 0 && big > 0.f && big < INFINITY) {
+                            s_scale[0] = 2.f * big;
+                            s_scale[1] = __fdiv_rn(kDigits4 / 256.f, 2.f * big);
+                        }
+                    }
                     group_sync();
 #pragma unroll
                     for (int r = 0; r < RH; ++r) {
@@ -537,16 +601,31 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                         s[r] -= s_max[h0 + r];
                     }
                     if (threadIdx.x == 0) *s_pending = s_moved[ring4] == 2;
+                    if constexpr (I8) {
+                        if (big < INFINITY) {
+                            if (threadIdx.x < R) s_unit[ring4 * R + threadIdx.x] = s_scale[0] * (256.f / kDigits4);
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < RH; r += 4) {
+                                float e[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    e[k] = fast_exp2(s[r + k]);
+                                    l[r + k] += e[k];
+                                }
+                                asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(pb + (((h0 + r) >> 2 ^ (kk & 7)) << 4)), "f"(e[0]), "f"(e[1]), "f"(e[2]),
+                                             "f"(e[3]) : "memory");
+                            }
+                            digits_apart<R, RH, kSoftmax>(pb, h0, vsc, s_top, s_unit + ring4 * R);
+                            fence_proxy_async();
+                            tc_fence_before();
+                            mbar_arrive_cnt(p_full(sb));
+                            continue;
+                        }
+                    }
                 }
-                float unit = 0.f;           // int8: weights per value scale, as integers
-                if (I8) {
-                    const float4 b4 = four(s_big + sb * 4);
-                    const float big = fmaxf(fmaxf(b4.x, b4.y), fmaxf(b4.z, b4.w));
-                    unit = big > 0.f ? __fdividef(vsc, big) * (kDigits4 / 256.f) : 0.f;         // weights are 2^8 at most
-                    if (threadIdx.x == 0) s_scale[ring4] = big * (256.f / kDigits4);
-                }
-                // ---- weights: four rows' terms a 16-byte word
-                const uint32_t pb = p_sm + (uint32_t)(sb * C::P_BYTES) + kk * 128;
+                // ---- weights
+                const float unit = I8 ? vsc * s_scale[1] : 0.f;            // per value's scale, as integers: weights are 2^8 at most
 #pragma unroll
                 for (int r = 0; r < RH; r += 4) {
                     float e[4];
@@ -614,7 +693,6 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                 if (s_moved[ring4])
 #pragma unroll
                     for (int r = 0; r < R; ++r) o[r] *= s_corr[ring4 * R + r];
-                const float unit = I8 ? s_scale[ring4] : 1.f;
 #pragma unroll
                 for (int c = 0; c < C::NO / 32; ++c) {
                     uint32_t x[32];
@@ -624,7 +702,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                     for (int j = 0; j < 32; j += 4) {
                         if constexpr (I8) {                 // a row's digits
                             const int r = c * 8 + j / 4;
-                            o[r] = fmaf(from_digits4(x[j], x[j + 1], x[j + 2], x[j + 3]), unit, o[r]);
+                            o[r] = fmaf(from_digits4(x[j], x[j + 1], x[j + 2], x[j + 3]), s_unit[ring4 * R + r], o[r]);
                         } else {                            // two rows' large terms, and their small ones
                             const int r = c * 16 + j / 2;
                             o[r] += __uint_as_float(x[j]) + __uint_as_float(x[j + 2]);
