@@ -355,7 +355,9 @@ static int launch(Args a, cudaStream_t st) {
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, rules_ids_kernel, a.best, a.rows, a.ids);
+    e = cudaLaunchKernelEx(&cfg, rules_ids_kernel, a.best, a.rows, a.ids);
+    if (e != cudaSuccess) (void)cudaMemsetAsync(a.best, 0, (size_t)a.rows * 8, st);         // as every call leaves them
+    return (int)e;
 }
 
 }  // namespace rules

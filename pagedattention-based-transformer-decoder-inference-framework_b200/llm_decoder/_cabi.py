@@ -6,6 +6,7 @@ fallback: a missing or unloadable library raises at first use.
 """
 import ctypes as C
 import os
+import threading
 
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG, "libpa_b200.so")
@@ -337,6 +338,14 @@ def stream_on(device):
     """Raw handle of the current stream of a tensor's device."""
     import torch
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class PerThread(threading.local):
+    """Buffers that a call of the library uses from its first kernel to its last, by (device index, raw stream).  One set per host thread: the
+    library is called without the interpreter's lock, so that two threads' calls on one stream may be issued kernel by kernel in turn."""
+
+    def __init__(self):
+        self.of = {}
 
 
 def capturing(raw_stream):

@@ -80,7 +80,7 @@ def sample(logits, temperature=1.0, top_k=0, top_p=1.0, eos_token_id=-1, eos_thr
 
 
 _LOGIT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # PA_TYPE_*
-_rule_words = {}        # (device, stream) -> workspace of pa_adjust_logits
+_rule_words = _cabi.PerThread()         # workspaces of pa_adjust_logits
 
 
 def _rules(logits, out, ids, history, history_start, repetition, presence, frequency, bias, allowed, allowed_rows, row_seq, tree):
@@ -144,19 +144,22 @@ def _rules(logits, out, ids, history, history_start, repetition, presence, frequ
     lib = _cabi.lib()
     with _cabi.on_device(dev):
         stream, ws, need = _cabi.stream_on(dev), None, 0
-        if ids is not None:     # words that every call leaves at zero, one buffer per stream
+        if ids is not None:     # words that every call leaves at zero
             need = lib.pa_adjust_logits_workspace_bytes(rows)
             if _cabi.capturing(stream):         # a graph has words of its own: its replays may run beside other calls
                 ws = torch.zeros(need, dtype=torch.uint8, device=dev)
             else:
-                ws = _rule_words.get((dev.index, stream))
+                ws = _rule_words.of.get((dev.index, stream))
                 if ws is None or ws.numel() < need:
-                    ws = _rule_words[(dev.index, stream)] = torch.zeros(max(need, 1 << 14), dtype=torch.uint8, device=dev)
+                    ws = _rule_words.of[(dev.index, stream)] = torch.zeros(max(need, 1 << 14), dtype=torch.uint8, device=dev)
         # (the stride of a single row may be anything)
-        _cabi.check(lib.pa_adjust_logits(
+        status = lib.pa_adjust_logits(
             logits.data_ptr(), kind, stride if rows > 1 else V, rows, V, _cabi.ptr(out), 0 if out is None else out.stride(0) if rows > 1 else V,
             _cabi.ptr(ids), p_seq, seqs or 0, p_history, history.numel() if p_history else 0, p_start, *arrays, *values, p_ids, p_val,
-            b_ids.numel() if p_ids else 0, p_bias, _cabi.ptr(allowed), *masks, p_rows, *paths, _cabi.ptr(ws), need, stream), "pa_adjust_logits")
+            b_ids.numel() if p_ids else 0, p_bias, _cabi.ptr(allowed), *masks, p_rows, *paths, _cabi.ptr(ws), need, stream)
+        if status != _cabi.PA_OK:               # what the words hold now nobody knows
+            _rule_words.of.pop((dev.index, stream), None)
+        _cabi.check(status, "pa_adjust_logits")
 
 
 def adjust_logits(logits, history=None, history_start=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None,

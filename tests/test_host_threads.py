@@ -1,0 +1,83 @@
+"""Operators of drafted trees called from two host threads: the library is called without the interpreter's lock, so that two calls may be
+issued at the same time, on one stream too.  Where a case would be a matter of luck, a stand-in for the library holds both calls until the other
+one is under way."""
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+
+class Library:
+    """The library, with calls of `name` answered by `answer`."""
+
+    def __init__(self, real, name, answer):
+        self.__dict__.update(real=real, name=name, answer=answer)
+
+    def __getattr__(self, name):
+        return self.answer if name == self.name else getattr(self.real, name)
+
+
+def in_threads(n, work):
+    out, errors = [None] * n, []
+
+    def run(i):
+        try:
+            out[i] = work(i)
+        except BaseException as e:      # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(n)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    return out
+
+
+@pytest.mark.gpu
+def test_rules_in_two_threads_have_words_of_their_own(monkeypatch):
+    from llm_decoder import _cabi, sampling
+    real, gate, words = _cabi.lib(), threading.Barrier(2, timeout=60), []
+
+    def answer(*args):
+        gate.wait()
+        words.append(args[-3])
+        return 0
+    logits = torch.zeros(3, 100, device="cuda")
+    monkeypatch.setattr(_cabi, "lib", lambda: Library(real, "pa_adjust_logits", answer))
+    in_threads(2, lambda i: sampling.adjusted_argmax(logits))
+    assert len(set(words)) == 2 and None not in words
+
+
+@pytest.mark.gpu
+def test_rules_in_threads_give_their_own_ids():
+    from llm_decoder import sampling
+    g = torch.Generator(device="cuda").manual_seed(1)
+    logits = [torch.randn(40, 5000, device="cuda", generator=g) for _ in range(4)]
+    want = [x.argmax(1).to(torch.int32) for x in logits]
+    torch.cuda.synchronize()
+    got = in_threads(4, lambda i: [sampling.adjusted_argmax(logits[i]) for _ in range(200)])
+    torch.cuda.synchronize()
+    for w, ids in zip(want, got):
+        assert all(torch.equal(w, x) for x in ids)
+
+
+@pytest.mark.gpu
+def test_rules_after_a_call_that_failed(monkeypatch):
+    """Its words may hold anything; the next call's ids are right all the same."""
+    from llm_decoder import _cabi, sampling
+    real = _cabi.lib()
+    logits = torch.from_numpy(np.random.default_rng(2).standard_normal((5, 700)).astype(np.float32)).cuda()
+    want = sampling.adjusted_argmax(logits)
+    assert torch.equal(want, logits.argmax(1).to(torch.int32))
+
+    def answer(*_args):
+        for words in sampling._rule_words.of.values():
+            words.fill_(255)
+        return 2
+    with monkeypatch.context() as m:
+        m.setattr(_cabi, "lib", lambda: Library(real, "pa_adjust_logits", answer))
+        with pytest.raises(Exception):
+            sampling.adjusted_argmax(logits)
+    assert torch.equal(sampling.adjusted_argmax(logits), want)
