@@ -100,6 +100,9 @@ def lookup_drafts(tokens, most, depth, branches=2, longest=3):
     return parents, out
 
 
+_workspaces = _cabi.PerThread()         # of pa_tree_attention: one for the caches of all layers, whose calls on a stream come one after the other
+
+
 def _vector(x, n, device, what):
     if not isinstance(x, torch.Tensor):
         x = to_device(torch.as_tensor(np.asarray(x), dtype=torch.int32), device)
@@ -147,9 +150,9 @@ def paged_tree_attention(q, kv_cache, tree, ctx_lens, temperature=1.0, beam_ids=
         if _cabi.capturing(stream):     # a graph has a workspace of its own: its replays may run beside other calls
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
         else:
-            ws = kv_cache._ws.get(("tree", stream))
+            ws = _workspaces.of.get((dev.index, stream))
             if need and (ws is None or ws.numel() < need):
-                ws = kv_cache._ws[("tree", stream)] = torch.empty(need, dtype=torch.uint8, device=dev)
+                ws = _workspaces.of[(dev.index, stream)] = torch.empty(need, dtype=torch.uint8, device=dev)
         _cabi.check(lib.pa_tree_attention(
             q.data_ptr(), q.stride(0) if R > 1 else H * D, TYPES[q.dtype], out.data_ptr(), kv_cache.key_buffer_.data_ptr(),
             kv_cache.value_buffer_.data_ptr(), _cabi.ptr(kv_cache.k_scales_), _cabi.ptr(kv_cache.v_scales_),

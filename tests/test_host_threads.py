@@ -81,3 +81,39 @@ def test_rules_after_a_call_that_failed(monkeypatch):
         with pytest.raises(Exception):
             sampling.adjusted_argmax(logits)
     assert torch.equal(sampling.adjusted_argmax(logits), want)
+
+
+def small_cache(seed):
+    import llm_decoder as ld
+    kv = ld.KVTileCache("f16")
+    kv.init(2 * 2 * 8, 16, 64)
+    kv.configure_table(2, 2, 8)
+    kv.page_table_.load_host_table(np.arange(32, dtype=np.int32).reshape(2, 2, 8))
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    kv.key_buffer_.normal_(generator=g)
+    kv.value_buffer_.normal_(generator=g)
+    return kv
+
+
+@pytest.mark.gpu
+def test_tree_attention_has_a_workspace_per_thread_and_none_per_cache(monkeypatch):
+    import llm_decoder as ld
+    from llm_decoder import _cabi
+    real, gate, used = _cabi.lib(), threading.Barrier(2, timeout=60), []
+    caches = [small_cache(i) for i in range(3)]
+    trees = [ld.DraftTree([[-1, 0, 0], [-1, 0]], device="cuda") for _ in range(2)]
+    q, ctx = torch.randn(5, 2, 64, device="cuda"), torch.tensor([100, 30], dtype=torch.int32, device="cuda")
+    for c in caches:
+        c.page_table_.device_data()
+
+    def answer(*args):
+        gate.wait()
+        used.append((threading.get_ident(), args[-3]))
+        return 0
+    monkeypatch.setattr(_cabi, "lib", lambda: Library(real, "pa_tree_attention", answer))
+    in_threads(2, lambda i: [ld.paged_tree_attention(q, c, trees[i], ctx) for c in (caches[0], caches[i + 1])])
+    spaces = {}
+    for thread, space in used:
+        spaces.setdefault(thread, set()).add(space)
+    assert len(used) == 4 and [len(s) for s in spaces.values()] == [1, 1] and len(set.union(*spaces.values())) == 2
+    assert None not in set.union(*spaces.values())
