@@ -38,9 +38,9 @@
 
 #include <cstdlib>
 #include <cstring>
-#include <mutex>
 
 #include "pa_common.cuh"
+#include "tensor_map.cuh"
 
 namespace pa {
 namespace tf32x3 {
@@ -529,21 +529,6 @@ __global__ void __launch_bounds__(256) linear_streamk_reduce_kernel(const float*
     }
 }
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult qres;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qres) == cudaSuccess &&
-            qres == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-    });
-    return fn;
-}
 // 2-D f32 tensor [rows][cols] (cols contiguous), box [box_rows][box_cols], zero fill out of range.
 static bool make_map_f32(CUtensorMap* map, const void* ptr, uint64_t cols, uint64_t rows, uint32_t box_cols,
                          uint32_t box_rows, CUtensorMapSwizzle swizzle) {

@@ -6,7 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <mutex>
+#include "tensor_map.cuh"
 
 namespace pa {
 
@@ -45,24 +45,9 @@ __device__ __forceinline__ void mma_16816_full(float (&d)[4], uint32_t a0, uint3
 }
 
 // ---- host: tensor maps for the group kernel ------------------------------------------------
-typedef CUresult (*EncodeTiledFnG)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static inline EncodeTiledFnG encode_fn_g() {
-    static EncodeTiledFnG fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult qres;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qres) == cudaSuccess &&
-            qres == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFnG>(p);
-    });
-    return fn;
-}
 // fp16 pool viewed as [total_tokens][head_dim]; box = 16 tokens x 64 dims (128 B), SWIZZLE_128B.
 static inline bool make_pool_map(CUtensorMap* map, const void* pool, uint64_t total_tokens, int head_dim = 128) {
-    EncodeTiledFnG fn = encode_fn_g();
+    EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
     cuuint64_t dims[2] = {(cuuint64_t)head_dim, total_tokens};
     cuuint64_t strides[1] = {(cuuint64_t)head_dim * 2};

@@ -110,7 +110,7 @@ __device__ __forceinline__ void tc_let_land(uint32_t bar, uint32_t parity) {
 
 // [rows][cols] bfloat16, rows `stride` elements apart; box = box_rows x 64 columns (128 bytes), SWIZZLE_128B
 static inline bool make_bf16_map(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t cols, uint64_t stride, uint32_t box_rows) {
-    EncodeTiledFnG fn = encode_fn_g();
+    EncodeTiledFn fn = encode_fn();
     if (!fn || rows == 0) return false;
     cuuint64_t dims[2] = {cols, rows}, strides[1] = {stride * 2};
     cuuint32_t box[2] = {64, box_rows}, estr[2] = {1, 1};

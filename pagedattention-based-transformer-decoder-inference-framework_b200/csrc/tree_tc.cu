@@ -505,7 +505,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 
 // [rows][heads][dim], box = (128 / G) rows x G heads x 64 columns
 static bool make_q_map(CUtensorMap* map, const TreeParams& p, int G) {
-    EncodeTiledFnG fn = encode_fn_g();
+    EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
     cuuint64_t dims[3] = {(cuuint64_t)p.dim, (cuuint64_t)p.heads, (cuuint64_t)p.rows}, strides[2] = {(cuuint64_t)p.dim * 2, (cuuint64_t)p.q_stride * 2};
     cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(QT / G)}, estr[3] = {1, 1, 1};

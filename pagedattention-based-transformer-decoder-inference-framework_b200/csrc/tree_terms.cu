@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
 
 // [rows][D] bytes, boxes of 16 rows, SWIZZLE_128B
 static bool make_byte_map(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t cols) {
-    EncodeTiledFnG fn = encode_fn_g();
+    EncodeTiledFn fn = encode_fn();
     if (!fn || rows == 0) return false;
     cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols};
     cuuint32_t box[2] = {(cuuint32_t)cols, 16}, estr[2] = {1, 1};

@@ -117,3 +117,39 @@ def test_tree_attention_has_a_workspace_per_thread_and_none_per_cache(monkeypatc
         spaces.setdefault(thread, set()).add(space)
     assert len(used) == 4 and [len(s) for s in spaces.values()] == [1, 1] and len(set.union(*spaces.values())) == 2
     assert None not in set.union(*spaces.values())
+
+
+@pytest.mark.gpu
+def test_tree_attention_in_threads_on_one_cache():
+    import llm_decoder as ld
+    kv = small_cache(7)
+    ctx = torch.tensor([100, 30], dtype=torch.int32, device="cuda")
+    trees = [ld.DraftTree([[-1] + [0] * (3 + i), [-1, 0]], device="cuda") for i in range(4)]
+    qs = [torch.randn(t.rows, 2, 64, device="cuda") for t in trees]
+    want = [ld.paged_tree_attention(q, kv, t, ctx) for q, t in zip(qs, trees)]
+    torch.cuda.synchronize()
+    got = in_threads(4, lambda i: [ld.paged_tree_attention(qs[i], kv, trees[i], ctx) for _ in range(100)])
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, x) for x in outs)
+
+
+@pytest.mark.gpu
+def test_the_first_call_of_a_thread_is_served_as_any_other():
+    """By a thread that has not called CUDA before, into memory that is there: the same bits."""
+    import llm_decoder as ld
+    from llm_decoder import draft_tree
+    kv = small_cache(9)
+    ctx = torch.tensor([100, 30], dtype=torch.int32, device="cuda")
+    tree = ld.DraftTree([[-1, 0, 0, 1], [-1, 0]], device="cuda")
+    q = torch.randn(tree.rows, 2, 64, device="cuda")
+    want = ld.paged_tree_attention(q, kv, tree, ctx)
+    outs, spaces = [torch.empty_like(want) for _ in range(8)], dict(draft_tree._workspaces.of)
+
+    def first(i):
+        draft_tree._workspaces.of.update(spaces)
+        return ld.paged_tree_attention(q, kv, tree, ctx, out=outs[i])
+    for i in range(8):              # one thread after the other
+        in_threads(1, lambda _k, i=i: first(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(want, x) for x in outs)
