@@ -153,3 +153,44 @@ def test_the_first_call_of_a_thread_is_served_as_any_other():
         in_threads(1, lambda _k, i=i: first(i))
     torch.cuda.synchronize()
     assert all(torch.equal(want, x) for x in outs)
+
+
+def test_host_stage_gives_threads_regions_of_their_own(monkeypatch):
+    """Two threads in the middle of a step's description: neither writes where the other's copy still reads."""
+    from llm_decoder.host_stage import _PinnedStage
+
+    class Stage(_PinnedStage):
+        def __init__(self):
+            monkeypatch.setattr(torch.Tensor, "pin_memory", lambda self: self)
+            super().__init__()
+
+    class View:
+        """A region of the stage; its copy takes as long as the other thread needs to come here, where it may."""
+
+        def __init__(self, view):
+            self.view_ = view
+
+        def view(self, shape):
+            return self
+
+        def copy_(self, t):
+            self.view_.copy_(t)
+            try:
+                meet.wait(timeout=0.3)
+            except threading.BrokenBarrierError:
+                pass
+
+        def to(self, device, non_blocking):
+            return self.view_.clone()
+
+    class Buffer:
+        def __init__(self, t):
+            self.t = t
+
+        def __getitem__(self, key):
+            return View(self.t[key])
+
+    meet, stage = threading.Barrier(2), Stage()
+    stage.buf = Buffer(stage.buf)
+    got = in_threads(2, lambda i: stage.put(torch.full((100,), i, dtype=torch.int32), torch.device("cpu")))
+    assert [x.tolist() for x in got] == [[0] * 100, [1] * 100]
