@@ -898,8 +898,8 @@ int pa_streams_add_norm(const float* d_src, int src_streams, float* d_dst, int64
  *   q_tiles)), first row of the sequence in the key buffers, position.  d_out [rows][heads * vdim].
  * pa_latent_gather: d_items [n][3] = slot, tokens (at most `longest`), first output row: the cached rows of whole sequences
  *   from a latent pool into d_out [rows][row_bytes].
- * pa_attention_tc_errors: how often one of these kernels, pa_masked_decode or pa_latent_decode gave up on a wait since the library was
- *   loaded (0 unless something is broken; the rows of that CTA or share hold NaN).  Synchronises.  pa_moe_tc_errors: the same for the grouped expert products on tcgen05. */
+ * pa_attention_tc_errors: how often one of these kernels, pa_masked_decode, pa_latent_decode, pa_tree_attention or pa_adjust_logits gave up on a
+ *   wait since the library was loaded (0 unless something is broken; the rows of that CTA or share hold NaN).  Synchronises.  pa_moe_tc_errors: the same for the grouped expert products on tcgen05. */
 int pa_masked_attention_tc_tile_tokens(int heads, int kv_heads, int dim, int vdim, int elem, int q_tiles);
 int pa_masked_attention_tc_units(int heads, int kv_heads, int q_tiles);
 int pa_latent_attention_expanded(const void* d_q, int64_t q_stride, int q_off, const void* d_k, int64_t k_stride,
@@ -1047,7 +1047,9 @@ int pa_conv_append_in_words(int units, int columns, int num_items, int64_t rows)
  *   the vocabulary are ignored; a row whose sequence is outside [0, num_seqs) has no history and no biases, and starts reach no further than
  *   history_tokens and bias_entries.  d_out (NULL: not wanted; may be d_logits) gets the logits in their type, d_ids (NULL: not wanted)
  *   the lowest index of the largest float before it is rounded (NaN never wins; 0 where nothing does); d_ids take a workspace
- *   that is zero before the first call and left so by every call.
+ *   that is zero before the first call and left so by every call.  Where the kernel gave up on a wait (pa_attention_tc_errors) the row's
+ *   logits hold NaN and its id is -1.  pa_adjust_logits_polls: the same with a limit of the kernel's waits (0: nothing is requested, so that
+ *   all of them run out).
  * pa_draft_trees (host arrays): from the nodes' parents (numbers within the sequence; -1 for node 0, a lower node for every other, else
  *   PA_ERR_INVALID_ARG) of sequences at node_start [num_seqs + 1]: per row its sequence, parent, depth (0 at the root), number and mask
  *   [rows][mask_words], and the nodes on the longest path.
@@ -1077,6 +1079,13 @@ int pa_adjust_logits(const void* d_logits, int type, int64_t stride, int rows, i
                      const int32_t* d_allowed, int mask_rows, int64_t allowed_stride, const int32_t* d_allowed_rows, const int32_t* d_tokens,
                      const int32_t* d_path, int path_words, const int32_t* d_node_start, void* d_workspace, size_t workspace_bytes,
                      pa_stream_t stream);
+int pa_adjust_logits_polls(const void* d_logits, int type, int64_t stride, int rows, int vocab, void* d_out, int64_t out_stride,
+                           int32_t* d_ids, const int32_t* d_row_seq, int num_seqs, const int32_t* d_history, int history_tokens,
+                           const int32_t* d_history_start, const float* d_repetition, const float* d_presence, const float* d_frequency,
+                           float repetition, float presence, float frequency, const int32_t* d_bias_ids, const float* d_bias, int bias_entries,
+                           const int32_t* d_bias_start, const int32_t* d_allowed, int mask_rows, int64_t allowed_stride,
+                           const int32_t* d_allowed_rows, const int32_t* d_tokens, const int32_t* d_path, int path_words,
+                           const int32_t* d_node_start, void* d_workspace, size_t workspace_bytes, int polls, pa_stream_t stream);
 int pa_draft_trees(const int64_t* parents, const int32_t* node_start, int num_seqs, int mask_words, int32_t* row_seq,
                    int32_t* row_parents, int32_t* depths, int32_t* nodes, int32_t* mask, int32_t* longest);
 int pa_tree_accept(const int32_t* d_ids, const int32_t* d_tokens, const int32_t* d_parents, const int32_t* d_node_start, int num_seqs,

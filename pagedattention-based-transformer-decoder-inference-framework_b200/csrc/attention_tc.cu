@@ -646,6 +646,7 @@ static void plan(int hpg, int q_tiles, int& tb, int& hg) {
 
 int masked_decode_errors(int* host_count);
 int latent_decode_errors(int* host_count);
+int logit_rules_errors(int* host_count);
 // not in the core library
 int tree_stream_errors(int* host_count) __attribute__((weak));
 int tree_tc_errors(int* host_count) __attribute__((weak));
@@ -755,13 +756,14 @@ PA_API int pa_latent_attention_expanded(const void* d_q, int64_t q_stride, int q
 
 PA_API int pa_attention_tc_errors(int* host_count) {
     PA_CHECK_ARG(host_count);
-    int n = 0, masked = 0, latent = 0, tree = 0, tree_tc = 0, tree_terms = 0;
+    int n = 0, masked = 0, latent = 0, rules = 0, tree = 0, tree_tc = 0, tree_terms = 0;
     int rc = (int)cudaMemcpyFromSymbol(&n, pa::atc::g_errors, sizeof(int));
     if (rc == PA_OK) rc = masked_decode_errors(&masked);
     if (rc == PA_OK) rc = latent_decode_errors(&latent);
+    if (rc == PA_OK) rc = logit_rules_errors(&rules);
     if (rc == PA_OK && pa::tree_stream_errors) rc = tree_stream_errors(&tree);
     if (rc == PA_OK && pa::tree_tc_errors) rc = tree_tc_errors(&tree_tc);
     if (rc == PA_OK && pa::tree_terms_errors) rc = tree_terms_errors(&tree_terms);
-    *host_count = n + masked + latent + tree + tree_tc + tree_terms;
+    *host_count = n + masked + latent + rules + tree + tree_tc + tree_terms;
     return rc;
 }

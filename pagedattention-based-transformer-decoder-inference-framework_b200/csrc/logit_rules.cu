@@ -24,14 +24,17 @@
 #include <type_traits>
 
 #include "dynamic_smem.cuh"
+#include "tcgen05_utils.cuh"
 #include "seq_common.cuh"
 
 namespace pa {
 namespace rules {
 
 constexpr int kThreads = 256, kChunk = 4096, kBiases = 512, kList = 1024;
-constexpr uint32_t kPolls = 1u << 25;           // of the wait for a copy
+constexpr uint32_t kNothing = 0xffffffffu;      // above every number, as ordered words: a chunk that did not come
 constexpr uint32_t kBiased = 0x80000000u;
+
+__device__ int g_errors;
 
 struct Args {
     const void* logits;
@@ -52,6 +55,7 @@ struct Args {
     const uint32_t* path;                                  // [rows, path_words]: nodes on a row's way
     int path_words;
     unsigned long long* best;                              // [rows], zero
+    uint32_t polls;                                        // of the wait for a copy
 };
 
 template <typename T> __device__ __forceinline__ float widen(T v) { return to_f32<T>(v); }
@@ -85,7 +89,7 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
     uint32_t *count = reinterpret_cast<uint32_t*>(smem + data_bytes<T>(a.chunk)), *mask = count + a.chunk, *touched = mask + a.chunk / 32 + 4;
     uint16_t* list = reinterpret_cast<uint16_t*>(touched + (ROUNDS ? a.chunk / 32 + 4 : 0));
     int *bias_v = reinterpret_cast<int*>(list + kList), *bias_i = bias_v + kBiases;
-    __shared__ int s_listed, s_biases;
+    __shared__ int s_listed, s_biases, s_lost, s_counted;
     __shared__ unsigned long long s_key[kThreads / 32];
     __shared__ __align__(8) uint64_t s_bar;
     const int r = blockIdx.x / a.chunks, v0 = (blockIdx.x - r * a.chunks) * a.chunk, nv = min(a.chunk, a.vocab - v0), tid = threadIdx.x;
@@ -97,9 +101,11 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
         mbar_init(bar, 1);
         mbar_fence_init();
         const uint32_t bytes = (uint32_t)((off + nv) * (int)sizeof(T) + 15) & ~15u;
-        mbar_arrive_expect_tx(bar, bytes);
-        bulk_g2s_nohint(smem_u32(data), x - off, bytes, bar);
-        s_listed = s_biases = 0;
+        if (a.polls) {                                      // 0: a wait that is to run out
+            mbar_arrive_expect_tx(bar, bytes);
+            bulk_g2s_nohint(smem_u32(data), x - off, bytes, bar);
+        }
+        s_listed = s_biases = s_lost = s_counted = 0;
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // ---- bounds and bits that nothing waits for yet
@@ -179,12 +185,9 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
         }
     }
     __syncthreads();
-    bool here = true;
-    for (uint32_t polls = 0; !mbar_try_wait(bar, 0); ++polls)
-        if (polls > kPolls) {
-            here = false;
-            break;
-        }
+    bool here = true;               // of this thread; of all, where they changed one another's tokens
+    for (uint32_t polls = 0; here && !mbar_try_wait(bar, 0); ++polls) here = polls < a.polls;
+    if (!here) s_lost = 1;
     // ---- their rules, in place
     auto is_allowed = [&](int i) { return !a.allowed || (mask[i >> 5] >> (i & 31) & 1u); };
     float best = -INFINITY;
@@ -197,7 +200,7 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
     };
     if (s_listed > 0) {
         const bool kept = s_listed <= kList;            // else every token is looked at
-        for (int k = tid; k < (kept ? s_listed : nv); k += kThreads) {
+        for (int k = tid; here && k < (kept ? s_listed : nv); k += kThreads) {
             const int i = kept ? list[k] : k;
             const uint32_t raw = count[i], c = raw & ~kBiased;
             if (!raw) continue;
@@ -222,18 +225,13 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
             data[off + i] = narrow<T>(f);
         }
         __syncthreads();
+        here = !s_lost;
     }
     // ---- the stream: words of the result
     T* out = a.out ? static_cast<T*>(a.out) + (int64_t)r * a.out_stride + v0 : nullptr;
     const T* edge = out ? out : x;
     const int head = min(nv, (int)((16 - ((uintptr_t)edge & 15)) & 15) / (int)sizeof(T)), words = (nv - head) / N, tail = head + words * N;
     const bool whole = (off + head) % N == 0;           // they are words of the chunk as well
-    const T nan = narrow<T>(__int_as_float(0x7fc00000));
-    if (!here) {                        // the copy did not come: NaN
-        best = -INFINITY;
-        for (int i = tid; i < nv; i += kThreads) data[off + i] = nan;
-        __syncthreads();
-    }
     auto single = [&](int i) {                          // a place outside the words
         const T v = is_allowed(i) ? data[off + i] : narrow<T>(-INFINITY);
         if (a.ids && !(ROUNDS && (touched[i >> 5] >> (i & 31) & 1u))) offer(widen<T>(v), i);
@@ -286,11 +284,24 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
         for (int e = 1; e < N; ++e) top = fmaxf(top, f[e]);
         return top;
     };
-    if (tid < head) single(tid);
-    if (tail + tid < nv) single(tail + tid);
+    if (!here) {                        // the copy did not come: NaN in the thread's places, and no id for the row
+        if (out) {
+            const T nan = narrow<T>(__int_as_float(0x7fc00000));
+            if (tid < head) out[tid] = nan;
+            if (tail + tid < nv) out[tail + tid] = nan;
+            for (int i = head + tid * N; i < tail; i += kThreads * N)
+                for (int e = 0; e < N; ++e) out[i + e] = nan;
+        }
+        if (a.ids) atomicMax(a.best + r, (unsigned long long)kNothing << 32);
+        if (atomicExch(&s_counted, 1) == 0) atomicAdd(&g_errors, 1);
+        if (a.polls) tc::tc_let_land(bar, 0);               // the CTA's shared memory outlives the copy
+    } else {
+        if (tid < head) single(tid);
+        if (tail + tid < nv) single(tail + tid);
+    }
     float wbest = -INFINITY;
     int wi = -1;                                        // the first word with the largest
-    for (int i = head + tid * N; i < tail; i += kThreads * N) {
+    for (int i = head + tid * N; here && i < tail; i += kThreads * N) {
         const Word<T> w = word(i);
         if (out) *reinterpret_cast<Word<T>*>(out + i) = w;
         if (a.ids) {
@@ -310,7 +321,7 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
             if (f[e] == wbest) offer(wbest, wi + e);
     }
     // (value, lowest index) of the warp, then of the CTA
-    const uint32_t u = __float_as_uint(best + 0.f), o = best > -INFINITY ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;   // ordered as the numbers, -0 as 0
+    const uint32_t u = __float_as_uint(best + 0.f), o = here && best > -INFINITY ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;   // ordered as the numbers, -0 as 0
     const uint32_t top = __reduce_max_sync(0xffffffffu, o), at = __reduce_min_sync(0xffffffffu, o == top ? (uint32_t)bi : 0xffffffffu);
     if ((tid & 31) == 0) s_key[tid >> 5] = top ? (unsigned long long)top << 32 | (uint32_t)~(v0 + (int)at) : 0ull;
     __syncthreads();
@@ -327,7 +338,7 @@ __global__ void __launch_bounds__(128) rules_ids_kernel(unsigned long long* best
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (r >= rows) return;
     const unsigned long long key = __ldcg(best + r);
-    ids[r] = key ? (int32_t)~(uint32_t)key : 0;
+    ids[r] = key ? (int32_t)~(uint32_t)key : 0;             // (kNothing, 0): -1
     best[r] = 0ull;
 }
 
@@ -361,20 +372,24 @@ static int launch(Args a, cudaStream_t st) {
 }
 
 }  // namespace rules
+
+int logit_rules_errors(int* host_count) { return (int)cudaMemcpyFromSymbol(host_count, rules::g_errors, sizeof(int)); }
+
 }  // namespace pa
 
 using namespace pa;
 
 PA_API size_t pa_adjust_logits_workspace_bytes(int rows) { return rows > 0 ? (size_t)rows * 8 : 0; }
 
-PA_API int pa_adjust_logits(const void* d_logits, int type, int64_t stride, int rows, int vocab, void* d_out, int64_t out_stride,
+PA_API int pa_adjust_logits_polls(const void* d_logits, int type, int64_t stride, int rows, int vocab, void* d_out, int64_t out_stride,
                             int32_t* d_ids, const int32_t* d_row_seq, int num_seqs, const int32_t* d_history, int history_tokens, const int32_t* d_history_start,
                             const float* d_repetition, const float* d_presence, const float* d_frequency, float repetition, float presence,
                             float frequency, const int32_t* d_bias_ids, const float* d_bias, int bias_entries, const int32_t* d_bias_start,
                             const int32_t* d_allowed, int mask_rows, int64_t allowed_stride, const int32_t* d_allowed_rows, const int32_t* d_tokens,
                             const int32_t* d_path, int path_words, const int32_t* d_node_start, void* d_workspace, size_t workspace_bytes,
-                            pa_stream_t stream) {
+                            int polls, pa_stream_t stream) {
     using namespace pa::rules;
+    PA_CHECK_ARG(polls >= 0);
     PA_CHECK_ARG(rows >= 0 && vocab > 0 && stride >= vocab && (!d_out || out_stride >= vocab) && (d_out || d_ids));
     if (rows == 0) return PA_OK;
     PA_CHECK_ARG(num_seqs >= 0 && history_tokens >= 0 && bias_entries >= 0 && mask_rows >= 0);
@@ -391,9 +406,23 @@ PA_API int pa_adjust_logits(const void* d_logits, int type, int64_t stride, int 
     a.allowed = reinterpret_cast<const uint32_t*>(d_allowed); a.allowed_stride = allowed_stride; a.allowed_rows = d_allowed_rows;
     a.tokens = d_tokens; a.node_start = d_node_start; a.path = reinterpret_cast<const uint32_t*>(d_path); a.path_words = path_words;
     a.best = static_cast<unsigned long long*>(d_workspace);
+    a.polls = (uint32_t)polls;
     cudaStream_t st = as_stream(stream);
     if (type == PA_TYPE_F32) return launch<float>(a, st);
     if (type == PA_TYPE_F16) return launch<__half>(a, st);
     if (type == PA_TYPE_BF16) return launch<bf16_t>(a, st);
     return PA_ERR_UNSUPPORTED;
+}
+
+PA_API int pa_adjust_logits(const void* d_logits, int type, int64_t stride, int rows, int vocab, void* d_out, int64_t out_stride,
+                            int32_t* d_ids, const int32_t* d_row_seq, int num_seqs, const int32_t* d_history, int history_tokens, const int32_t* d_history_start,
+                            const float* d_repetition, const float* d_presence, const float* d_frequency, float repetition, float presence,
+                            float frequency, const int32_t* d_bias_ids, const float* d_bias, int bias_entries, const int32_t* d_bias_start,
+                            const int32_t* d_allowed, int mask_rows, int64_t allowed_stride, const int32_t* d_allowed_rows, const int32_t* d_tokens,
+                            const int32_t* d_path, int path_words, const int32_t* d_node_start, void* d_workspace, size_t workspace_bytes,
+                            pa_stream_t stream) {
+    return pa_adjust_logits_polls(d_logits, type, stride, rows, vocab, d_out, out_stride, d_ids, d_row_seq, num_seqs, d_history, history_tokens,
+                                  d_history_start, d_repetition, d_presence, d_frequency, repetition, presence, frequency, d_bias_ids, d_bias,
+                                  bias_entries, d_bias_start, d_allowed, mask_rows, allowed_stride, d_allowed_rows, d_tokens, d_path, path_words,
+                                  d_node_start, d_workspace, workspace_bytes, tc::kPolls, stream);
 }

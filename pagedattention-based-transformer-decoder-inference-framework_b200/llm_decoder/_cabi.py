@@ -236,6 +236,8 @@ _SIGS = {
     "pa_adjust_logits_workspace_bytes": ([_i32], _sz),
     "pa_adjust_logits": ([_vp, _i32, _i64, _i32, _i32, _vp, _i64, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _vp, _vp,
                           _i32, _vp, _vp, _i32, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _sz, _vp], _i32),
+    "pa_adjust_logits_polls": ([_vp, _i32, _i64, _i32, _i32, _vp, _i64, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _vp, _vp,
+                          _i32, _vp, _vp, _i32, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _sz, _i32, _vp], _i32),
     "pa_draft_trees": ([_vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp], _i32),
     "pa_tree_accept": ([_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, C.POINTER(_vp),
                         _vp, _vp, _vp, _vp, _vp], _i32),
