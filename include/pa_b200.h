@@ -1033,7 +1033,8 @@ int pa_conv_append_in_words(int units, int columns, int num_items, int64_t rows)
  *   that sees nothing is zero.  d_out [rows][heads][head_dim] of the queries' type.  Types (q, pools): f32 with f16, i8, f32;
  *   f16 with f16, i8; bf16 with bf16.  i8 pools have a scale per row and are read as q / scale.  head_dim <= 256.
  *   The workspace holds the partial results of keys that were split; d_workspace may be NULL where the function of its size
- *   returns 0.
+ *   returns 0.  Rows of a share whose kernel gave up on a wait hold NaN (pa_attention_tc_errors).  pa_tree_attention_polls: the same with
+ *   a limit of the kernels' waits (0: nothing is requested, so that all of them run out; the general kernel has none).
  * pa_adjust_logits: row r of d_logits (rows `stride` elements apart; type PA_TYPE_F32, _F16 or _BF16) belongs to sequence
  *   d_row_seq[r] (NULL: r).  With c the number of times a token v stands in d_history[d_history_start[b] ..
  *   d_history_start[b + 1] - 1] and, where d_tokens is given, on the way to row r's node: the tokens
@@ -1070,6 +1071,11 @@ int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void* d_out
                       int num_tiles, int total_pages, const int32_t* d_beam_ids, const int32_t* d_ctx_lens, const int32_t* d_node_start,
                       const int32_t* d_mask, int mask_words, int rows, int num_seqs, int most_nodes, int heads, int head_dim,
                       int tile_size, float temperature, void* d_workspace, size_t workspace_bytes, pa_stream_t stream);
+int pa_tree_attention_polls(const void* d_q, int64_t q_stride, int q_type, void* d_out, const void* d_k_pool, const void* d_v_pool,
+                            const float* d_k_scales, const float* d_v_scales, int kv_type, const int32_t* d_table, int num_beams, int kv_heads,
+                            int num_tiles, int total_pages, const int32_t* d_beam_ids, const int32_t* d_ctx_lens, const int32_t* d_node_start,
+                            const int32_t* d_mask, int mask_words, int rows, int num_seqs, int most_nodes, int heads, int head_dim,
+                            int tile_size, float temperature, void* d_workspace, size_t workspace_bytes, int polls, pa_stream_t stream);
 size_t pa_adjust_logits_workspace_bytes(int rows);
 int pa_adjust_logits(const void* d_logits, int type, int64_t stride, int rows, int vocab, void* d_out, int64_t out_stride,
                      int32_t* d_ids, const int32_t* d_row_seq, int num_seqs, const int32_t* d_history, int history_tokens,

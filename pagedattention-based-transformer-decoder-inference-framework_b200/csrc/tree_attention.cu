@@ -109,12 +109,13 @@ PA_API size_t pa_tree_attention_workspace_bytes(int rows, int num_seqs, int most
     return most;
 }
 
-PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void* d_out, const void* d_k_pool, const void* d_v_pool,
+PA_API int pa_tree_attention_polls(const void* d_q, int64_t q_stride, int q_type, void* d_out, const void* d_k_pool, const void* d_v_pool,
                              const float* d_k_scales, const float* d_v_scales, int kv_type, const int32_t* d_table, int num_beams, int kv_heads,
                              int num_tiles, int total_pages, const int32_t* d_beam_ids, const int32_t* d_ctx_lens, const int32_t* d_node_start,
                              const int32_t* d_mask, int mask_words, int rows, int num_seqs, int most_nodes, int heads, int head_dim,
-                             int tile_size, float temperature, void* d_workspace, size_t workspace_bytes, pa_stream_t stream) {
+                             int tile_size, float temperature, void* d_workspace, size_t workspace_bytes, int polls, pa_stream_t stream) {
     using namespace pa::tree;
+    PA_CHECK_ARG(polls >= 0);
     PA_CHECK_ARG(rows >= 0 && num_seqs >= 0 && most_nodes >= 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && head_dim > 0);
     PA_CHECK_ARG(num_beams > 0 && num_tiles > 0 && total_pages > 0 && tile_size > 0 && temperature != 0.f && (num_seqs > 0 || rows == 0));
     if (rows == 0) return PA_OK;
@@ -146,7 +147,7 @@ PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void
     if (f.block) {
         if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < tree_work_bytes(num_seqs, f.workers, f.block, head_dim)) return PA_ERR_WORKSPACE;
         const bool whole = (int64_t)num_tiles * tile_size <= (f.unit == 16 ? kTreeWholeStream : kTreeWhole) && tree_items(p, f.block) <= f.workers;
-        const TreeWork w{p, f.workers, kTreeLeast, f.block, f.unit, total_pages * tile_size, f.extra, whole, kTreeStreamScale, tc::kPolls, static_cast<TreeNote*>(d_workspace),
+        const TreeWork w{p, f.workers, kTreeLeast, f.block, f.unit, total_pages * tile_size, f.extra, whole, kTreeStreamScale, (uint32_t)polls, static_cast<TreeNote*>(d_workspace),
                          reinterpret_cast<float*>(static_cast<TreeNote*>(d_workspace) + f.workers)};
         int rc = f.launch(w, st);
         if (rc == PA_OK && !whole) rc = tree_join_launch(w, st);
@@ -161,4 +162,14 @@ PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void
     PA_TREE(PA_TYPE_BF16, bf16_t, PA_TYPE_BF16, bf16_t)
 #undef PA_TREE
     return PA_ERR_UNSUPPORTED;
+}
+
+PA_API int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void* d_out, const void* d_k_pool, const void* d_v_pool,
+                             const float* d_k_scales, const float* d_v_scales, int kv_type, const int32_t* d_table, int num_beams, int kv_heads,
+                             int num_tiles, int total_pages, const int32_t* d_beam_ids, const int32_t* d_ctx_lens, const int32_t* d_node_start,
+                             const int32_t* d_mask, int mask_words, int rows, int num_seqs, int most_nodes, int heads, int head_dim,
+                             int tile_size, float temperature, void* d_workspace, size_t workspace_bytes, pa_stream_t stream) {
+    return pa_tree_attention_polls(d_q, q_stride, q_type, d_out, d_k_pool, d_v_pool, d_k_scales, d_v_scales, kv_type, d_table, num_beams, kv_heads,
+                                   num_tiles, total_pages, d_beam_ids, d_ctx_lens, d_node_start, d_mask, mask_words, rows, num_seqs, most_nodes, heads,
+                                   head_dim, tile_size, temperature, d_workspace, workspace_bytes, tc::kPolls, stream);
 }

@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_stream_kernel(const __gri
         }
     }
     if (f < f_hi) {                     // a wait ran out: the copies that were requested land, and the pieces from here on are NaN
-        for (int64_t i = f; i < f_is; ++i) {
+        for (int64_t i = a.polls ? f : f_is; i < f_is; ++i) {
             const int at = stage + (int)(i - f);
             tc::tc_let_land(bar0 + at % ST * 8, at < ST ? phase : phase ^ 1u);
         }

@@ -121,7 +121,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 
     if (warp == W_PROD) {
         uint32_t c = 0, tiles = 0;          // requests and tiles of keys so far
-        bool ok = true;
+        bool ok = a.polls > 0;              // 0: nothing is requested, so that all waits run out
         if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = TreeNote{};
         auto request = [&](const CUtensorMap* map, const int (&r)[4]) {
             const int s = (int)(c % RING);
@@ -143,8 +143,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             ++c;
         };
         TreePages pages(p);
-        while (ok && w.next()) {
+        while (w.next()) {                  // to the end, also where a wait ran out: the join goes by the last piece's note
             if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = tree_note(a, w.sq, w.g, w.rr0, w.i0, w.i1, w.item_at(), w.total, w.ns, w.slot);
+            if (!ok) continue;
             pages.open(w, 4);
             int r[4] = {-1, -1, -1, -1}, prev[4] = {-1, -1, -1, -1};
             for (int i = w.i0; i <= w.i1 && ok; ++i) {              // K(i) and V(i - 1)
@@ -171,7 +172,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         // zeros, and nobody looks at what becomes of them
         TreeWalk ahead = w;
         auto fetch_q = [&] {
-            if (!q_boxes || !ahead.next() || !rows_of(ahead, x) || __any_sync(0xffffffffu, failed())) return;
+            if (!q_boxes || !a.polls || !ahead.next() || !rows_of(ahead, x) || __any_sync(0xffffffffu, failed())) return;
             ++asked;
             if (elect_one()) {
                 mbar_arrive_expect_tx(q_ready(x), Q_BYTES);

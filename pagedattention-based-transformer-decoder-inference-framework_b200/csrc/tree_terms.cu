@@ -59,7 +59,7 @@ template <int D, bool I8, int R> struct Shape {
     static constexpr int COLS = 2 * N + 2 * NO, TMEM = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int NBAR = 2 * RING + 16;      // full, empty [ring]; s_full, p_full, o_full, o_empty, q_ready, q_free [2]; piece_done [4]
     static constexpr int FLOATS = 2 * R /*factors*/ + 2 * R /*references, thresholds*/ + 4 * R /*corrections*/ + 4 * R /*maxima*/ +
-                                  4 * 5 * R /*sums, references at the end*/ + 2 * R /*what becomes of the sums*/ + 2 * 8 * R /*rows*/ + (I8 ? 8 * R : 0) /*units, largest products*/ + 28;
+                                  4 * 5 * R /*sums, references at the end*/ + 2 * R /*what becomes of the sums*/ + (I8 ? 8 * R : 0) /*units, largest products*/ + 28;
     static size_t smem(int seqs, int mask_words) {
         return (size_t)RING * SLOT + Q_BUFS * Q_BYTES + 2 * P_BYTES + NBAR * 8 + FLOATS * 4 + 2 * R * mask_words * 4 + kNotes * 4 + 64 + (seqs + 1) * 4 + 1024;
     }
@@ -170,17 +170,15 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
     const uint32_t tmem_slot = bar0 + C::NBAR * 8, fail_sm = tmem_slot + 8, meta_sm = fail_sm + 8;
     // factors of the scores [2 pieces], references (less kShift) and whether rows have one, corrections of the last four tiles, maxima
     // by warp, sums by warp and references of the last four pieces, a piece's rows of the output and what their sums are
-    // multiplied by; nodes and heads of the last eight
-    // pieces' rows (node -1: no row); int8: what the last four tiles' sums are times, largest products of weights and scales by warp;
+    // multiplied by; int8: what the last four tiles' sums are times, largest products of weights and scales by warp;
     // the unit of the scales and what gives integers of it, bits of the largest and the smallest scale by warp;
     // whether references moved in the last four tiles, whether the last four pieces are computed by rows,
     // whether a row has no reference yet
     float* fl = reinterpret_cast<float*>(smem_raw + (meta_sm + kNotes * 4 - smem_u32(smem_raw)));
-    float *s_fe = fl, *s_ref = fl + 2 * R, *s_set = fl + 3 * R, *s_corr = fl + 4 * R, *s_max = fl + 8 * R, *s_end = fl + 12 * R, *s_unit = fl + 50 * R;
+    float *s_fe = fl, *s_ref = fl + 2 * R, *s_set = fl + 3 * R, *s_corr = fl + 4 * R, *s_max = fl + 8 * R, *s_end = fl + 12 * R, *s_unit = fl + 34 * R;
     uint32_t *s_top = reinterpret_cast<uint32_t*>(s_unit + (I8 ? 4 * R : 0)), *s_big = s_top + (I8 ? 4 * R : 0), *s_small = s_big + 4;
     float* s_scale = reinterpret_cast<float*>(s_small + 4);
     int2* s_fin = reinterpret_cast<int2*>(fl + 32 * R);
-    int *s_node = reinterpret_cast<int*>(fl + 34 * R), *s_head = s_node + 8 * R;         // (seven pieces at most are on their way)
     int *s_moved = reinterpret_cast<int*>(s_scale + 8), *s_odd = s_moved + 4, *s_pending = s_odd + 4, *pre = s_pending + 4;
     uint32_t* s_mask = reinterpret_cast<uint32_t*>(pre + p.num_seqs + 1);      // [2 pieces][R][mask_words]
     auto failed = [&] { return tc_failed(fail_sm); };
@@ -230,7 +228,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
 
     if (warp == W_PROD) {
         uint32_t c = 0, tiles = 0;          // requests and tiles of keys so far
-        bool ok = true;
+        bool ok = a.polls > 0;              // 0: nothing is requested, so that all waits run out
         if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = TreeNote{};
         auto request = [&](const CUtensorMap* map, bool scales, int rows) {         // lane u < 8: of unit u
             const int s = (int)(c % RING);
@@ -268,7 +266,6 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
         };
         TreePages pages(p);
         while (ok && w.next()) {
-            if (w.f >= w.f_hi && lane == 0) a.notes[blockIdx.x] = tree_note(a, w.sq, w.g, w.rr0, w.i0, w.i1, w.item_at(), w.total, w.ns, w.slot);
             pages.open(w, 8);
             int rows = -1, before = -1;
 #pragma unroll 1
@@ -441,8 +438,6 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                 }
             }
             if (lane < HALF) {
-                s_node[(pieces & 7) * R + mine] = node;
-                s_head[(pieces & 7) * R + mine] = head;
                 uint32_t* mask = s_mask + (buf * R + mine) * p.mask_words;
                 mask[0] = mask0;
                 for (int x = 1; x < p.mask_words; ++x) mask[x] = node >= 0 ? __ldg(p.mask + (int64_t)node * p.mask_words + x) : 0u;
@@ -450,6 +445,8 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
             fence_proxy_async();
             mbar_arrive_cnt(q_ready(pieces));
             ++pieces;
+            // (these warps come to the share's end whatever runs out: the join goes by the note)
+            if (w.f >= w.f_hi && threadIdx.x == W_LOAD * 32) a.notes[blockIdx.x] = tree_note(a, w.sq, w.g, w.rr0, w.i0, w.i1, w.item_at(), w.total, w.ns, w.slot);
         }
     } else if (warp < W_SUMS) {
         // ---- softmax: one thread per key and half of the rows
@@ -582,7 +579,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                         s_max[r] = by;
                         s_ref[r] += by;
                         if (raise) s_set[r] = 1.f;
-                        else if (!has && s_node[(pieces & 7) * R + r] >= 0) s_moved[ring4] = 2;        // still none
+                        else if (!has && w.rr0 + r < w.sq.n * G) s_moved[ring4] = 2;        // still none
                     }
                     float big = 0.f;            // int8: the tile's largest scale, if all are alike; infinity, if they are not
                     if constexpr (I8) {
@@ -672,7 +669,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                 mbar_arrive_cnt(piece_done(pieces));
                 mbar_arrive_cnt(q_free(pieces));
             }
-            if (!I8 && odd && !failed()) tree_piece_by_rows<D, Q, __half>(a, w, warp * (R / W_SUMS), R / W_SUMS);
+            if (!I8 && odd) tree_piece_by_rows<D, Q, __half>(a, w, warp * (R / W_SUMS), R / W_SUMS);
             ++pieces;
         }
     } else {
@@ -716,20 +713,20 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
             n += nt;
             wait(piece_done(pieces), pieces >> 2 & 1u);
             const float* end = s_end + (pieces & 3) * 5 * R;
-            const bool skip = !I8 && s_odd[pieces & 3];
-            ++pieces;
-            const int* nodes = s_node + ((pieces - 1) & 7) * R;
-            const int* heads = s_head + ((pieces - 1) & 7) * R;
+            // a wait ran out: what the others left here may be of another piece
+            const bool lost = failed(), skip = !I8 && !lost && s_odd[pieces & 3];
             constexpr float scale = I8 ? 1.f : 1.f / 128.f;     // 2^-kShift
-            const float bad = failed() ? __int_as_float(0x7fc00000) : 0.f;
+            const float bad = lost ? __int_as_float(0x7fc00000) : 0.f;
             if (d < R) {
                 const float sum = (end[d] + end[R + d] + end[2 * R + d] + end[3 * R + d]) * scale, ref = end[4 * R + d];
-                const bool row = nodes[d] >= 0 && !skip;
-                s_fin[d] = make_int2(row ? (w.slot < 0 ? nodes[d] * p.heads + heads[d] : d) : -1,
+                const int rr = w.rr0 + d, node = rr / G;
+                const bool row = rr < w.sq.n * G && !skip;
+                s_fin[d] = make_int2(row ? (w.slot < 0 ? (w.sq.r0 + node) * p.heads + w.g * G + rr - node * G : d) : -1,
                                      __float_as_int((w.slot < 0 ? __fdiv_rn(scale, sum + 1e-6f) : scale * a.p_scale) + bad));
                 if (w.slot >= 0 && row)
                     *reinterpret_cast<float4*>(a.part + (w.slot * a.block + d) * (D + 4) + D) = make_float4(ref + bad, sum * a.p_scale + bad, ref, 0.f);
             }
+            ++pieces;
             asm volatile("bar.sync 3, 128;" ::: "memory");
             if (!skip && d < D) {
                 float* part = a.part + w.slot * a.block * (D + 4) + d;

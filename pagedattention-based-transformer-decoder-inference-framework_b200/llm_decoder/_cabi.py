@@ -233,6 +233,8 @@ _SIGS = {
     "pa_tree_attention_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32], _sz),
     "pa_tree_attention": ([_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32,
                            _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp], _i32),
+    "pa_tree_attention_polls": ([_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32,
+                           _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _i32, _vp], _i32),
     "pa_adjust_logits_workspace_bytes": ([_i32], _sz),
     "pa_adjust_logits": ([_vp, _i32, _i64, _i32, _i32, _vp, _i64, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _vp, _vp,
                           _i32, _vp, _vp, _i32, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _sz, _vp], _i32),
