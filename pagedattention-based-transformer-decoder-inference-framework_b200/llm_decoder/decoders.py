@@ -39,7 +39,7 @@ import torch
 
 from . import _cabi
 from . import sampling
-from .draft_tree import DraftTree, TreeCaches, lookup_drafts, paged_tree_attention, tree_accept
+from .draft_tree import DraftTree, TreeCaches, longest_path, lookup_drafts, paged_tree_attention, tree_accept
 from .host_stage import to_device
 from .kv_tile_cache import KVTileCache
 
@@ -384,7 +384,7 @@ class _DecoderBase:
             raise ValueError("drafts must not be negative")
         if max_len <= 0:
             return [list(p) for p in prompts]
-        draft = draft or (lambda tokens, most, depth: lookup_drafts(tokens, most, depth, branches))
+        given, draft = draft, draft or (lambda tokens, most, depth: lookup_drafts(tokens, most, depth, branches))
         self._setup_batch(B)
         self.reset()
         self._sampling = None
@@ -415,6 +415,8 @@ class _DecoderBase:
                         p, t = draft(s, min(1 + drafts, room), left)
                         if not 1 <= len(p) <= min(1 + drafts, room) or len(t) != len(p) or int(t[0]) != int(s[-1]):
                             raise ValueError("draft: between one and `most` nodes, the first of them the sequence's last token")
+                        if given and longest_path(p) > left:
+                            raise ValueError("draft: paths of at most `depth` nodes")
                     parents.append(p)
                     tokens.append(t)
                 tree = DraftTree(parents, tokens, dev)

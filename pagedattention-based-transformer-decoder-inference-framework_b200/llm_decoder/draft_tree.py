@@ -69,6 +69,14 @@ class DraftTree:
         return ctx_lens[self.row_seq] + self.nodes
 
 
+def longest_path(parents):
+    """Nodes on the longest path of one sequence's tree (its parents as for DraftTree)."""
+    depths = []
+    for up in parents:
+        depths.append(1 if up < 0 or up >= len(depths) else depths[up] + 1)
+    return max(depths, default=0)
+
+
 def lookup_drafts(tokens, most, depth, branches=2, longest=3):
     """A tree of guesses from the sequence itself: (parents, tokens) of at most `most` nodes in paths of at most `depth`, node 0 being the
     last of `tokens`.  Where the last `longest` tokens (then one fewer, ... then the last one) came up before, what followed is a guess, the
