@@ -390,6 +390,7 @@ class _DecoderBase:
         self._sampling = None
         dev, self.drafted_steps_ = self.device, 0
         with torch.cuda.device(dev):
+            lost = _cabi.lost_waits()
             def on_device(x, dtype):
                 return x if isinstance(x, torch.Tensor) else to_device(torch.as_tensor(np.asarray(x), dtype=dtype), dev)
             per_seq = [x if isinstance(x, (int, float)) else on_device(x, torch.float32) for x in (repetition, presence, frequency)]
@@ -435,6 +436,8 @@ class _DecoderBase:
                 got = torch.cat((done.counts[:, None], done.tokens), 1).cpu().numpy()       # the step's synchronisation
                 seqs = [np.concatenate((s, g[1:1 + g[0]]))[:n + max_len] for s, g in zip(seqs, got)]
                 self.drafted_steps_ += 1
+            if _cabi.lost_waits() != lost:      # asked before tokens are handed out
+                raise RuntimeError("a kernel gave up on a wait: logits of this call are not valid")
             self.positions.copy_(ctx)
             self.ctx_lens.copy_(ctx + 1)
             self.ids.copy_(to_device(torch.from_numpy(np.array([s[-1] for s in seqs], dtype=np.int32)), dev))

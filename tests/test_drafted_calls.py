@@ -23,3 +23,14 @@ def test_paths_that_are_too_long_are_refused(tmp_path):
     assert len(got) == len(prompt) + n and dec.positions.tolist() == [len(prompt) + n - 1]
     with pytest.raises(ValueError):
         dec.generate_drafted([prompt], n, draft=lambda *a: draft(*a, 1))
+
+
+@pytest.mark.gpu
+def test_no_tokens_where_a_wait_ran_out(tmp_path, monkeypatch):
+    from llm_decoder import decoders
+    dec = decoder("CUDADecoder", tmp_path, 12, 60, 2, 64, max_len=64)
+    assert len(dec.generate_drafted([[1, 2]], 5)[0]) == 7
+    counts = [3, 4]
+    monkeypatch.setattr(decoders._cabi, "lost_waits", lambda: counts.pop(0))
+    with pytest.raises(RuntimeError):
+        dec.generate_drafted([[1, 2]], 5)
