@@ -1046,7 +1046,7 @@ int pa_conv_append_in_words(int units, int columns, int num_items, int64_t rows)
  *   d_bias_start[b] .. of (d_bias_ids, d_bias); of entries for the same token the last counts.  d_allowed: rows of
  *   allowed_stride 32-bit words, row d_allowed_rows[r] (NULL: r; outside [0, mask_rows): everything is allowed).  Tokens outside
  *   the vocabulary are ignored; a row whose sequence is outside [0, num_seqs) has no history and no biases, and starts reach no further than
- *   history_tokens and bias_entries.  d_out (NULL: not wanted; may be d_logits) gets the logits in their type, d_ids (NULL: not wanted)
+ *   history_tokens and bias_entries.  d_out (NULL: not wanted; may be d_logits with its stride, rows that overlap otherwise are PA_ERR_INVALID_ARG) gets the logits in their type, d_ids (NULL: not wanted)
  *   the lowest index of the largest float before it is rounded (NaN never wins; 0 where nothing does); d_ids take a workspace
  *   that is zero before the first call and left so by every call.  Where the kernel gave up on a wait (pa_attention_tc_errors) the row's
  *   logits hold NaN and its id is -1.  pa_adjust_logits_polls: the same with a limit of the kernel's waits (0: nothing is requested, so that

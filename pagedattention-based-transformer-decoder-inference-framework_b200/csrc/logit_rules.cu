@@ -21,6 +21,7 @@
 // both results: 23 us, 1.8 TB/s), nearer to the copies where rows are written and no history is long (256 x 128000 floats: 41 us without
 // rules, 6.4 TB/s; with histories of 4096 tokens, 64 biases and masks 76 us, 3.5 TB/s).  Two, four or eight rows of a tree per CTA, which would
 // share the counts of their history, took 66, 62 and 70 us instead of 53: fewer CTAs cover each other.
+#include <algorithm>
 #include <type_traits>
 
 #include "dynamic_smem.cuh"
@@ -371,6 +372,18 @@ static int launch(Args a, cudaStream_t st) {
     return (int)e;
 }
 
+// Whether one of `rows` rows of `width` bytes from b on, `db` apart, shares a byte with one from a on, `da` apart
+static bool overlap(uintptr_t a, int64_t da, uintptr_t b, int64_t db, int rows, int64_t width) {
+    const int64_t off = (int64_t)(b - a), span_a = (rows - 1) * da + width, span_b = (rows - 1) * db + width;
+    if (off >= span_a || -off >= span_b) return false;
+    for (int r = 0; r < rows; ++r) {
+        const int64_t at = off + r * db;                    // the last row of a that begins before this one ends
+        const int64_t k = std::min<int64_t>(rows - 1, at + width > 0 ? (at + width - 1) / da : -1);
+        if (k >= 0 && k * da + width > at) return true;
+    }
+    return false;
+}
+
 }  // namespace rules
 
 int logit_rules_errors(int* host_count) { return (int)cudaMemcpyFromSymbol(host_count, rules::g_errors, sizeof(int)); }
@@ -395,6 +408,9 @@ PA_API int pa_adjust_logits_polls(const void* d_logits, int type, int64_t stride
     PA_CHECK_ARG(num_seqs >= 0 && history_tokens >= 0 && bias_entries >= 0 && mask_rows >= 0);
     PA_CHECK_ARG(d_logits && (!d_history || d_history_start) && (!d_bias || (d_bias_ids && d_bias_start)));
     PA_CHECK_ARG((!d_allowed || allowed_stride >= ((int64_t)vocab + 31) / 32) && (!d_tokens || (d_path && path_words > 0 && d_node_start && d_row_seq)));
+    const int64_t elem = type == PA_TYPE_F32 ? 4 : 2;
+    PA_CHECK_ARG(!d_out || (d_out == d_logits && (out_stride == stride || rows == 1)) ||
+                 !overlap((uintptr_t)d_logits, stride * elem, (uintptr_t)d_out, out_stride * elem, rows, vocab * elem));
     if (d_ids && (!d_workspace || (uintptr_t)d_workspace % 8 || workspace_bytes < pa_adjust_logits_workspace_bytes(rows))) return PA_ERR_WORKSPACE;
     Args a{};
     a.logits = d_logits; a.out = d_out; a.ids = d_ids; a.stride = stride; a.out_stride = out_stride; a.rows = rows; a.vocab = vocab;

@@ -176,7 +176,7 @@ def adjust_logits(logits, history=None, history_start=None, repetition=1.0, pres
     and a number that there is no mask for allows everything.
     row_seq: the sequence of every row (None: row r is sequence r).  tree: the rows are the nodes of a DraftTree with tokens; the
     tokens on a node's path, its own among them, count as history.
-    out: a tensor like logits (also logits itself)."""
+    out: a tensor like logits (also logits itself, no other rows that overlap them)."""
     if out is None:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or (out.numel() and out.stride(1) != 1) or \
