@@ -79,7 +79,7 @@ int pa_kv_gather(const void* d_pool, void* d_dense, const int32_t* d_table, int 
  * write the caller performs: row (d_positions[r] % tile_size) of page
  * (beam, head, d_positions[r] / tile_size) := new_k/new_v[r, head, :].
  * Unmapped pages are skipped.  new_k/new_v are [R, H, D].
- *   _f16      : new rows already fp16, byte copy.
+ *   _f16      : new rows already fp16 (or bf16 rows for bf16 pools), byte copy.
  *   _f32_f16  : new rows fp32, rounded to nearest-even fp16 on write.
  *   _f32_i8   : new rows fp32; per (row, head) scale = compute_minmax_scale
  *               (int8_quant.cpp:59-64), q = batch_quantize (int8_quant.cpp:15-28);

@@ -327,7 +327,7 @@ class KVTileCache:
 
     # ---- hot path: append (get_write_ptr + row write, hpp:29-34) -------------------------
     def append(self, new_k, new_v, positions, beam_ids=None):
-        """new_k/new_v: [R, H, D] device tensors (f16 or f32), or page-locked host tensors (uploaded on the copy
+        """new_k/new_v: [R, H, D] device tensors (f16 or f32; bf16 for bf16 pools), or page-locked host tensors (uploaded on the copy
         stream, attention.HostPipe); positions: [R] int32 device."""
         pt = self.page_table_
         table = pt.device_data()
@@ -341,7 +341,7 @@ class KVTileCache:
                 new_v, rv = pipe.upload(new_v, "new_v")
             releases = [rk, rv]
         R = new_k.shape[0]
-        assert self.value_dim_ == self.head_dim_ and self.dtype != "bf16", "append(): equal K/V widths, f16/f32/i8 pools"
+        assert self.value_dim_ == self.head_dim_, "append(): equal K/V widths"
         assert new_k.is_contiguous() and new_v.is_contiguous() and new_k.shape == new_v.shape
         assert new_k.shape[1] == pt.num_heads_ and new_k.shape[2] == self.head_dim_
         lib = _cabi.lib()
@@ -356,7 +356,8 @@ class KVTileCache:
                 assert new_k.dtype == torch.float32
                 st = lib.pa_kv_append_f32_i8(self.key_buffer_.data_ptr(), self.value_buffer_.data_ptr(),
                                              self.k_scales_.data_ptr(), self.v_scales_.data_ptr(), *common)
-            elif new_k.dtype == torch.float16:
+            elif self.dtype == "bf16" or new_k.dtype == torch.float16:     # 16-bit rows as they are
+                assert new_k.dtype == self.key_buffer_.dtype
                 st = lib.pa_kv_append_f16(self.key_buffer_.data_ptr(), self.value_buffer_.data_ptr(), *common)
             else:
                 assert new_k.dtype == torch.float32

@@ -1,5 +1,7 @@
 """What generation with drafted trees refuses, and what it does when something under it goes wrong."""
+import numpy as np
 import pytest
+import torch
 
 from test_generate_drafted import decoder
 
@@ -34,3 +36,39 @@ def test_no_tokens_where_a_wait_ran_out(tmp_path, monkeypatch):
     monkeypatch.setattr(decoders._cabi, "lost_waits", lambda: counts.pop(0))
     with pytest.raises(RuntimeError):
         dec.generate_drafted([[1, 2]], 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pool,dtype", [("f32", torch.float32), ("f16", torch.float32), ("f16", torch.float16), ("bf16", torch.bfloat16), ("i8", torch.float32)])
+def test_a_step_as_it_is_written_down(pool, dtype):
+    """Rows of all nodes by append, attention, acceptance, for every type of pages: the rows are where they should be."""
+    import llm_decoder as ld
+    rng = np.random.default_rng(4)
+    B, H, D, tiles = 2, 3, 64, 6
+    kv = ld.KVTileCache(pool)
+    kv.init(B * H * tiles, 16, D)
+    kv.configure_table(B, H, tiles)
+    table = rng.permutation(B * H * tiles).astype(np.int32).reshape(B, H, tiles)
+    kv.page_table_.load_host_table(table)
+    kv.key_buffer_.zero_()
+    kv.value_buffer_.zero_()
+    tree = ld.DraftTree([[-1, 0, 0, 2], [-1, 0]], [[5, 6, 7, 8], [9, 1]], "cuda")
+    ctx = torch.tensor([14, 40], dtype=torch.int32, device="cuda")
+    k, v = (torch.from_numpy(rng.standard_normal((tree.rows, H, D)).astype(np.float32)).to(dtype).cuda() for _ in "kv")
+    kv.append(k, v, tree.positions(ctx), tree.row_seq)
+
+    def row(x, b, h, pos):
+        x, s = (kv.key_buffer_, kv.k_scales_) if x == "k" else (kv.value_buffer_, kv.v_scales_)
+        at = int(table[b, h, pos // 16]), pos % 16
+        return x[at].float() if s is None else x[at].float() / s[at]
+    near = {"f32": 0.0, "f16": 2.0 ** -11 if dtype is torch.float32 else 0.0, "bf16": 0.0, "i8": 0.5 / 127 * 1.01}[pool]       # rounding to the pool's type
+    place = [(0, 14 + i) for i in range(4)] + [(1, 40), (1, 41)]
+    for x, new in (("k", k), ("v", v)):
+        for r, (b, pos) in enumerate(place):
+            for h in range(H):
+                assert float((row(x, b, h, pos) - new[r, h].float()).abs().max()) <= near * float(new[r, h].abs().max())
+    q = torch.randn(tree.rows, H, D, device="cuda").to({"f16": torch.float32, "i8": torch.float32}.get(pool, dtype))
+    assert bool(ld.paged_tree_attention(q, kv, tree, ctx, 8.0).isfinite().all())
+    want = row("k", 0, 1, 17)
+    done = ld.tree_accept(torch.tensor([7, 1, 8, 3, 2, 1], dtype=torch.int32, device="cuda"), tree, [kv], ctx)
+    assert done.counts.tolist() == [3, 1] and torch.equal(row("k", 0, 1, 16), want)
