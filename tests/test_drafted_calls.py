@@ -72,3 +72,30 @@ def test_a_step_as_it_is_written_down(pool, dtype):
     want = row("k", 0, 1, 17)
     done = ld.tree_accept(torch.tensor([7, 1, 8, 3, 2, 1], dtype=torch.int32, device="cuda"), tree, [kv], ctx)
     assert done.counts.tolist() == [3, 1] and torch.equal(row("k", 0, 1, 16), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", ["CUDADecoder", "INT8Decoder"])
+def test_the_command(tmp_path, capsys, cls):
+    """bin/generate with drafts and penalties: what generate_drafted gives; without them what it gave before."""
+    import json
+
+    from llm_decoder import cli
+    dec = decoder(cls, tmp_path, 13, 97, 2, 64, max_len=128)
+    config = dict(architecture=cls, num_layers=2, num_heads=2, head_dim=64, hidden_dim=128, vocab_size=97, max_seq_len=128,
+                  weights="q" if cls == "INT8Decoder" else "w")
+    (tmp_path / "config.json").write_text(json.dumps(config))
+
+    def run(*args):
+        assert cli.main(["generate", "--model", str(tmp_path), "--prompt", "5,17,3", "--prompt", "9,9", "--max-new-tokens", "30", *args]) == 0
+        return [[int(t) for t in line.split(",")] for line in capsys.readouterr().out.splitlines() if line[:1].isdigit()]
+    prompts = [[5, 17, 3], [9, 9]]
+    assert run("--drafts", "12") == [dec.generate_drafted([p], 30, drafts=12)[0] for p in prompts]
+    rules = dict(repetition=1.3, presence=0.2, frequency=0.1)
+    want = [dec.generate_drafted([p], 30, drafts=4, **rules)[0] for p in prompts]
+    assert run("--drafts", "4", "--repetition-penalty", "1.3", "--presence-penalty", "0.2", "--frequency-penalty", "0.1") == want
+    assert run("--repetition-penalty", "1.3") == [dec.generate_drafted([p], 30, drafts=0, repetition=1.3)[0] for p in prompts]
+    assert run() == [dec.generate(p, 30) for p in prompts]
+    for args in (["--drafts", "4", "--temperature", "0.7"], ["--presence-penalty", "1", "--top-k", "3"], ["--drafts", "4", "--top-p", "0.5"]):
+        with pytest.raises(SystemExit):
+            run(*args)
