@@ -200,30 +200,43 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const Args a) {
         }
     };
     if (s_listed > 0) {
-        const bool kept = s_listed <= kList;            // else every token is looked at
-        for (int k = tid; here && k < (kept ? s_listed : nv); k += kThreads) {
-            const int i = kept ? list[k] : k;
+        // one touched token; last(i): of the entries for its bias the last
+        auto apply = [&](int i, auto last) {
             const uint32_t raw = count[i], c = raw & ~kBiased;
-            if (!raw) continue;
+            if (!raw) return;
             float f = widen<T>(data[off + i]);
             if (c) {
                 f = f > 0.f ? __fdiv_rn(f, rep) : __fmul_rn(f, rep);
                 f = __fsub_rn(f, pres);
                 f = __fsub_rn(f, __fmul_rn(freq, (float)c));
             }
-            if (raw & kBiased) {
-                int last = -1;
-                if (s_biases <= kBiases) {
-                    for (int q = 0; q < s_biases; ++q)
-                        if (bias_v[q] == i) last = max(last, bias_i[q]);
-                } else {        // more than were kept: the last entry of them all
-                    for (int q = i1 - 1; last < 0; --q)
-                        if (__ldg(a.bias_ids + q) == v0 + i) last = q;
-                }
-                f = __fadd_rn(f, __ldg(a.bias + last));
-            }
+            if (raw & kBiased) f = __fadd_rn(f, __ldg(a.bias + last(i)));
             if (ROUNDS && a.ids && is_allowed(i)) offer(f, i);
             data[off + i] = narrow<T>(f);
+        };
+        if (s_biases <= kBiases) {
+            const bool kept = s_listed <= kList;        // else every token is looked at
+            for (int k = tid; here && k < (kept ? s_listed : nv); k += kThreads)
+                apply(kept ? list[k] : k, [&](int i) {
+                    int last = -1;
+                    for (int q = 0; q < s_biases; ++q)
+                        if (bias_v[q] == i) last = max(last, bias_i[q]);
+                    return last;
+                });
+        } else {
+            // more entries than were kept: the last one of every token, for some tokens at a time, from a pass over the sequence's list each (16 x 128000
+            // logits with as many biases 0.46 ms; a search of the list per token 146)
+            for (int t0 = 0; t0 < nv; t0 += kBiases) {
+                __syncthreads();
+                for (int k = tid; k < kBiases; k += kThreads) bias_i[k] = -1;
+                __syncthreads();
+                for (int q = i0 + tid; q < i1; q += kThreads) {
+                    const unsigned k = (unsigned)(__ldg(a.bias_ids + q) - v0 - t0);
+                    if (k < (unsigned)kBiases) atomicMax(&bias_i[k], q);
+                }
+                __syncthreads();
+                for (int k = tid; here && k < min(kBiases, nv - t0); k += kThreads) apply(t0 + k, [&](int i) { return bias_i[i - t0]; });
+            }
         }
         __syncthreads();
         here = !s_lost;
