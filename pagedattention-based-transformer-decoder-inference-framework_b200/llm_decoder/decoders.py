@@ -77,12 +77,23 @@ class _Bufs:
         self.hs = torch.ones(R, **f32)
         self.ws = None  # GEMM / linear scratch for R rows (owned here, never by the library; _DecoderBase._scratch)
         self.qp = self.kp = self.vp = None  # q / k / v projections [R, hid] f32, allocated when a layer has them
+        self.whole = self   # where what is allocated on demand stays: first()'s results share it
 
     def first(self, R):
         """The buffers of the first R rows."""
         few = copy.copy(self)
         few.__dict__.update({k: v[:R] for k, v in self.__dict__.items() if isinstance(v, torch.Tensor) and k != "ws"}, R=R)
         return few
+
+    def on_demand(self, name, make):
+        """The buffer `name`, made once by make(rows) for the rows of all."""
+        if getattr(self.whole, name, None) is None:
+            setattr(self.whole, name, make(self.whole.R))
+        x = getattr(self.whole, name)
+        if self.whole is not self:
+            x = x[:self.R]
+            setattr(self, name, x)
+        return x
 
 
 class _DecoderBase:
@@ -157,6 +168,7 @@ class _DecoderBase:
         request that does not fit re-allocates AND drops the captured graph."""
         if need == 0:
             return None, 0
+        bf = bf.whole
         if bf.ws is None or bf.ws.numel() < need:
             bf.ws = torch.empty(need, dtype=torch.uint8, device=self.device)
             if bf is getattr(self, "bufs", None):
@@ -222,7 +234,8 @@ class _DecoderBase:
                 self._attention(li, bf.n, bf.a, R, ctx_lens, beam_ids, ws, prefill_shape, tree)
             else:
                 if bf.qp is None:
-                    bf.qp, bf.kp, bf.vp = (torch.empty((R, hid), dtype=torch.float32, device=self.device) for _ in range(3))
+                    for name in ("qp", "kp", "vp"):
+                        bf.on_demand(name, lambda rows: torch.empty((rows, hid), dtype=torch.float32, device=self.device))
                 self._qkv_proj(bf, L)                                   # bf.n -> bf.qp, bf.kp, bf.vp
                 self.kv_caches[li].append(bf.kp.view(R, H, D), bf.vp.view(R, H, D), positions, beam_ids)
                 self._attention(li, bf.qp, bf.kp, R, ctx_lens, beam_ids, ws, prefill_shape, tree)   # kp reused as the output
@@ -776,12 +789,11 @@ class INT8Decoder(_DecoderBase):
             self._emb_T[:, :V] = self.embedding.t()
             self._pad_bias = torch.zeros(Vp, dtype=torch.float32, device=dev)
             self._pad_bias[V:] = float("-inf")  # padded columns never win the argmax
-        if getattr(bf, "lq", None) is None:
-            bf.lq = torch.empty((R, hid), dtype=torch.int8, device=dev)
-            bf.ls = torch.empty(R, dtype=torch.float32, device=dev)
-        self._quant_rows(x_rows, bf.lq, bf.ls, R, hid)
+        lq = bf.on_demand("lq", lambda rows: torch.empty((rows, hid), dtype=torch.int8, device=dev))
+        ls = bf.on_demand("ls", lambda rows: torch.empty(rows, dtype=torch.float32, device=dev))
+        self._quant_rows(x_rows, lq, ls, R, hid)
         wp, wb = self._scratch(bf, lib.pa_gemm_i8_workspace_bytes(1, R, Vp, hid))
-        self._chk(lib.pa_gemm_i8_dequant(bf.lq.data_ptr(), self._emb_T.data_ptr(), out.data_ptr(), 1, R, Vp, hid, bf.ls.data_ptr(),
+        self._chk(lib.pa_gemm_i8_dequant(lq.data_ptr(), self._emb_T.data_ptr(), out.data_ptr(), 1, R, Vp, hid, ls.data_ptr(),
                                          1.0 / float(self.emb_qscale), self._pad_bias.data_ptr(), _cabi.ACT[""], wp, wb,
                                          _cabi.stream()), "pa_gemm_i8_dequant")
 

@@ -99,3 +99,14 @@ def test_the_command(tmp_path, capsys, cls):
     for args in (["--drafts", "4", "--temperature", "0.7"], ["--presence-penalty", "1", "--top-k", "3"], ["--drafts", "4", "--top-p", "0.5"]):
         with pytest.raises(SystemExit):
             run(*args)
+
+
+@pytest.mark.gpu
+def test_steps_of_other_sizes_share_their_scratch(tmp_path):
+    from llm_decoder.decoders import _Bufs
+    dec = decoder("INT8Decoder", tmp_path, 14, 97, 2, 64, attn=True, batch_size=10)
+    bufs = _Bufs(12, 128, 512, dec.device)
+    few, fewer = bufs.first(9), bufs.first(4)
+    assert dec._scratch(few, 1000) == dec._scratch(fewer, 900) == dec._scratch(bufs, 1000)
+    made = [b.on_demand("lq", lambda rows: torch.empty((rows, 128), dtype=torch.int8, device=dec.device)) for b in (few, fewer, bufs, bufs.first(7))]
+    assert [len(x) for x in made] == [9, 4, 12, 7] and len({x.data_ptr() for x in made}) == 1
