@@ -9,7 +9,7 @@
 //                 values' scales as 31-bit ones (four) relative to the largest possible, where a tile's values have scales alike; where they
 //                 have not, relative to the row's largest in the tile, so that a key which a row does not see, or hardly weighs, takes no bits from
 //                 the others.  Products and their sums are exact integers, no byte is converted
-// A row's reference moves only when a score exceeds it by more than 2^8, which the terms leave room for: after a piece's first tile
+// A row's reference moves only when a score exceeds it by more than 2^8 (int8: 2^7), which the terms leave room for: after a piece's first tile
 // hardly ever.  (So the formula's 1e-6 stands beside a sum that may be up to 2^8 times the one relative to the largest score: 1e-6 of a result.)
 // The sums of a tile leave the tensor cores as they are and are added up in float registers (the tensor cores cut where float rounds: over a
 // long context that would add up).  A row's terms are neighbours in P^T, whose rows are keys: a thread stores four query rows at once.
@@ -38,10 +38,9 @@ using namespace tc;
 
 constexpr int KT = 128, kNotes = 32;
 constexpr float kDigits = 8.3e6f, kDigits4 = 2.1e9f;      // the largest number of three and of four signed digits, and some to spare
-constexpr float kRaise = 8.f;
-// Scales (1 / scale of a value) of a tile are alike within a factor of 8.  They are taken relative to twice the largest of the last such tile as long as
-// they lie within a factor of 16 below: weights have 23 bits at that scale and 19 at the far end.
-constexpr float kAlike = 8.f;
+// Scales (1 / scale of a value) of a tile are alike within a factor of 8.  They are taken relative to 1.25 times the largest of the last such tile as long
+// as they lie within a factor of 16 below: weights have 24 bits at that scale and 20 at the far end.
+constexpr float kAlike = 8.f, kRoom = 1.25f, kLeast = 1.f / 16.f;
 
 __device__ int g_errors;
 
@@ -152,7 +151,8 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
     typedef Shape<D, I8, R> C;
     constexpr int N = C::N, TERMS = C::TERMS, RING = C::RING, CB = I8 ? 1 : D / 64, RH = R / C::HALVES;       // CB: column blocks of a tile
     constexpr int W_SUMS = C::W_SUMS, W_MMA = C::W_MMA, W_PROD = C::W_PROD, W_LOAD = C::W_LOAD, kSoftmax = C::SOFTMAX;
-    constexpr float kShift = I8 ? 0.f : 7.f;                     // half weights times 2^7: up to 2^15
+    constexpr float kRaise = I8 ? 7.f : 8.f, kShift = I8 ? 0.f : 7.f;      // half weights times 2^7: up to 2^15; int8: up to 2^7, a bit more for the rest
+    constexpr float kWeight = kDigits4 / 128.f;                  // int8: integers of a weight
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const TreeParams& p = a.p;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                 float s[RH];
                 // a value's scale that lies outside the range of the unit (or is not finite) is a reason, too
                 const float by = I8 ? s_scale[0] : 0.f;
-                const bool strange = I8 && here && !(fabsf(vsc) <= by && 16.f * fabsf(vsc) >= by);
+                const bool strange = I8 && here && !(fabsf(vsc) <= by && fabsf(vsc) >= kLeast * by);
                 bool over = false;
 #pragma unroll
                 for (int c = 0; c < RH / CH; ++c) {
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                 const bool any = group_any(over || strange || *s_pending);
                 if (threadIdx.x == 0) s_moved[ring4] = any;
                 const uint32_t pb = p_sm + (uint32_t)(sb * C::P_BYTES) + kk * 128;
-                if (I8 && threadIdx.x < R) s_unit[ring4 * R + threadIdx.x] = by * (256.f / kDigits4);
+                if (I8 && threadIdx.x < R) s_unit[ring4 * R + threadIdx.x] = by * (1.f / kWeight);
                 if (any) {
                     if (I8) {
                         const uint32_t bits = __float_as_uint(vsc) & 0x7fffffffu;       // what is not a number is above infinity
@@ -587,8 +587,8 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                         big = __uint_as_float(max(max(b4.x, b4.y), max(b4.z, b4.w)));
                         if (!(big < 1e36f && (big == 0.f || big > 1e-28f) && big <= kAlike * __uint_as_float(min(min(s4.x, s4.y), min(s4.z, s4.w))))) big = INFINITY;
                         if (threadIdx.x == 0 && big > 0.f && big < INFINITY) {
-                            s_scale[0] = 2.f * big;
-                            s_scale[1] = __fdiv_rn(kDigits4 / 256.f, 2.f * big);
+                            s_scale[0] = kRoom * big;
+                            s_scale[1] = __fdiv_rn(kWeight, kRoom * big);
                         }
                     }
                     group_sync();
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                     if (threadIdx.x == 0) *s_pending = s_moved[ring4] == 2;
                     if constexpr (I8) {
                         if (big < INFINITY) {
-                            if (threadIdx.x < R) s_unit[ring4 * R + threadIdx.x] = s_scale[0] * (256.f / kDigits4);
+                            if (threadIdx.x < R) s_unit[ring4 * R + threadIdx.x] = s_scale[0] * (1.f / kWeight);
                         } else {
 #pragma unroll
                             for (int r = 0; r < RH; r += 4) {
@@ -622,7 +622,7 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                     }
                 }
                 // ---- weights
-                const float unit = I8 ? vsc * s_scale[1] : 0.f;            // per value's scale, as integers: weights are 2^8 at most
+                const float unit = I8 ? vsc * s_scale[1] : 0.f;            // per value's scale, as integers: weights are 2^7 at most
 #pragma unroll
                 for (int r = 0; r < RH; r += 4) {
                     float e[4];
