@@ -17,9 +17,9 @@
 // for; a second kernel (programmatic dependent launch) turns the words into ids and zeroes them.  (Counting the CTAs at a row, so that the last
 // one does that, held every CTA's place for two trips to L2 more: 61 us for 256 x 128000 logits.)
 //
-// What bounds it: the instructions of a chunk, 75 % of the issue slots (512 rows x 50257 floats, ids only: 53 us, 2.0 TB/s; 100 x 100003 bfloat16,
-// both results: 23 us, 1.8 TB/s), nearer to the copies where rows are written and no history is long (256 x 128000 floats: 41 us without
-// rules, 6.4 TB/s; with histories of 4096 tokens, 64 biases and masks 76 us, 3.5 TB/s).  Two, four or eight rows of a tree per CTA, which would
+// What bounds it: the instructions of a chunk, 75 % of the issue slots (512 rows x 50257 floats, ids only: 54 us, 2.0 TB/s; 100 x 100003 bfloat16,
+// both results: 24 us, 1.7 TB/s), nearer to the copies where rows are written and no history is long (256 x 128000 floats: 41 us without
+// rules, 6.4 TB/s; with histories of 4096 tokens, 64 biases and masks 78 us, 3.5 TB/s).  Two, four or eight rows of a tree per CTA, which would
 // share the counts of their history, took 66, 62 and 70 us instead of 53: fewer CTAs cover each other.
 #include <algorithm>
 #include <type_traits>

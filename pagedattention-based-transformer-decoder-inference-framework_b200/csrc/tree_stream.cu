@@ -12,9 +12,11 @@
 //                   key's scale goes to its scores, a value's to its weights, which a row's power of two then brings between 2^14 and 2^15
 //                   unit by unit: halves hold the largest product of weight and 1 / scale, whatever it is, and all others to 2^-39 of it
 //
-// What bounds it: 16-bit pages of 128 columns the copies (32 sequences of 4K keys, 32 heads, 8 rows a head: 189 us, 5.7 TB/s; float queries, 16
-// rows: 208 us, 5.3 TB/s), narrower ones and int8 pages the chain of a unit, wait, products, softmax, products, that one to four warps of an SM's
-// quarter cover for each other (16 sequences of 4K keys, 12 heads of 64, float queries: 58 us, 3.5 TB/s; instructions issue half of the time).  Keys
+// What bounds it: 16-bit pages of 128 columns the copies (32 sequences of 2K keys, 32 heads, 8 rows a head: 189 us, 5.7 TB/s; float queries, 16
+// rows: 207 us, 5.3 TB/s), narrower ones and int8 pages the chain of a unit, wait, products, softmax, products, that one to four warps of an SM's
+// quarter cover for each other (16 sequences of 4K keys, 12 heads of 64, float queries: 58 us, 3.5 TB/s; instructions issue half of the time; int8
+// pages: 72 us, 1.5 TB/s, of which the scaling of the weights takes 2.5).  Softmax weights of 16-bit queries enter the second product in the pages' type,
+// since both factors of one are of a type (2.3e-3 of a bfloat16 result where rounding it alone takes 1.7e-3); their sum is of the float ones.  Keys
 // come by the warp because few rows give no tile to share, and units of 16 because a page is that long; a smaller unit is the finest cut of a long
 // context (one sequence of 333 keys, 12 heads: 14.0 us, of which 5 are the join and its launch).
 //

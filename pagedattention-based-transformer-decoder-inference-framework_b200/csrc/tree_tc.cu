@@ -8,10 +8,11 @@
 //   next NQ warps    one elected thread each:  S = Q K^T of tile i + 1  and  O += P V  of tile i (A operand from TMEM)
 //   last warp        TMA boxes of 16 keys x 64 columns into a ring, SWIZZLE_128B, page ids a tile ahead
 // The reference of a row is raised only when a score exceeds it by more than 2^8; weights are 2^(s - reference + 7), so that halves
-// hold them down to 2^-31 of the largest.
+// hold them down to 2^-31 of the largest.  They enter the second product in the values' type, since its factors have one type (bfloat16: 2.3e-3 from
+// float64, where rounding the result alone takes 1.7e-3); their sum is taken of the float ones.
 //
 // What bounds it: the hand-over between tensor pipe and exponentials, one thread per row as in prefill attention (131072 keys, 64 nodes, 16 heads on
-// 4: 89 us, 3.0 TB/s, 770 TFLOP/s; the tensor pipe is busy 42 % of the time), with fewer rows the copies (64 rows a head, 4K keys: 156 us, 5.3
+// 4: 89 us, 3.0 TB/s, 770 TFLOP/s; the tensor pipe is busy 42 % of the time), with fewer rows the copies (12 sequences of 4K keys, 32 heads, 64 rows a head: 156 us, 5.2
 // TB/s), and where contexts are short what a piece takes to begin and end, some 7 us (60 keys: 72 us for 1536 pieces on 296 CTAs).  So the next
 // piece's queries come as boxes under the last products of this one, and results leave through shared memory: 93 us before.  A CTA per 128 rows, two
 // an SM, covers one's softmax with the other's products; 256 rows in one CTA share what is staged, which pays where a kv head has more than 128 of
@@ -536,7 +537,7 @@ static int launch(const TreeWork& a, cudaStream_t st) {
 int tree_tc_workers(int block) { return device_info().sm_count * (block == 128 ? 2 : 1); }
 
 // Rows of a block, 0 where this kernel does not serve or the streaming one is faster.  us, this kernel against the streaming one: 64 rows a head (32
-// sequences, 4K keys, 8 kv heads) 113 against 235, 32 rows 106 against 132, 16 rows 104 against 106, 8 rows and 32 kv heads 191 against 189, ragged
+// sequences, 4K keys, 8 kv heads) 113 against 235, 32 rows 106 against 132, 16 rows 104 against 106, 8 rows and 32 kv heads of 2K keys 191 against 189, ragged
 // contexts 168 against 161: from 17 on.  Blocks of 128 rows against 256: 128 rows a head 126 against 142, 64 rows 113 against 135; 160 rows (2K
 // keys) 121 against 99, 256 rows 130 against 112; 384 rows 102 against 104, 448 rows 80 against 83, 800 rows 45 against 47.
 int tree_tc_block(const TreeParams& p) {

@@ -23,11 +23,12 @@
 //
 // What bounds it: the latency of a tile's chain (scores, vote, weights, products, sums) at one or two softmax warps for each quarter of an SM, and
 // of a piece's beginning and end, some 6 us.  12 sequences of 4K keys, 32 heads: half pages and 32 float rows 152 us, 5.3 TB/s; int8 pages and 16
-// float rows 87 us, 4.8 TB/s; 48 sequences of 1 to 2K keys, int8 pages 124 us, 3.6 TB/s; 16 sequences of 4K keys, 128 rows a kv head (blocks of 64)
-// 133 us, 258 TFLOP/s of the formula's operations.  Rows as the columns of the products keep the tile at 128 keys for any number of rows: as rows
+// float rows 87 us, 4.8 TB/s; 48 sequences of 1 to 2K keys, int8 pages 130 us, 3.4 TB/s (values' scales that differ by more than 8 in every tile:
+// 256); 16 sequences of 4K keys, 128 rows a kv head (blocks of 64) 134 us, 257 TFLOP/s of the formula's operations.  Rows as the columns of the products keep the tile at 128 keys for any number of rows: as rows
 // they would fill 128 lanes with 16.  Digits and terms instead of tf32 or a conversion to half: int8 pages stay as they are, and float results keep
-// 22 bits.  Reading a tile's maximum before its exponentials for every tile took 223 us where votes on 2^8 take 192 (before the shares counted
-// beginnings and ends: 124 now).
+// 22 bits.  Reading a tile's maximum before its exponentials for every tile took 223 us where votes on 2^8 took 192 (before the shares counted
+// beginnings and ends).  Instructions are what its caches are short of: a branch more in the softmax, never taken, took 14 of 107 us where pieces are
+// short.
 #include "tcgen05_utils.cuh"
 #include "tree_pieces.cuh"
 
@@ -788,10 +789,10 @@ static int launch(const TreeWork& a, cudaStream_t st) {
 int tree_terms_workers(int block) { return device_info().sm_count * (block == 16 ? 2 : 1); }
 
 // Rows of a block, 0 where this kernel does not serve or the streaming one is faster.  us, this kernel against the streaming one: int8 pages, 16
-// rows: 1000 keys 107 against 206, 4K keys 87 against 194, ragged 124 against 207, 100 keys 38 against 52; half pages, 32 float rows: 4K keys 153
-// against 294, 1000 keys 189 against 307, 90 keys 92 against 72 (the host does not know how long contexts are); 16 float rows 205 against 209, and
-// of 64 columns 65 against 58: from 17 on.  int8 rows of 64 bytes have no tile here.  Blocks: int8, 256 rows in 32s 317, in 16s 370, 16 rows in a
-// block of 32 194 instead of 107; half, 128 rows in 64s 133, in 32s 196; 32 rows in a block of 64 177 instead of 153.
+// rows: 1000 keys 114 against 214, 4K keys 87 against 204, ragged 130 against 216, 100 keys 38 against 52; half pages, 32 float rows: 4K keys 153
+// against 292, 1000 keys 186 against 305, 90 keys 96 against 71 (the host does not know how long contexts are); 16 float rows 205 against 209, and
+// of 64 columns 65 against 58: from 17 on.  int8 rows of 64 bytes have no tile here.  Blocks: int8, 256 rows in 32s 332, in 16s 365, 16 rows in a
+// block of 32 (ragged) 229 instead of 130; half, 128 rows in 64s 133, in 32s 196; 32 rows in a block of 64 177 instead of 153.
 int tree_terms_block(const TreeParams& p) {
     const int G = p.heads / p.kv_heads, rows = p.most * G;
     const bool half = p.q_type == PA_TYPE_F32 && p.kv_type == PA_TYPE_F16, bytes = p.kv_type == PA_TYPE_I8 && p.dim == 128;

@@ -123,7 +123,10 @@ def paged_tree_attention(q, kv_cache, tree, ctx_lens, temperature=1.0, beam_ids=
     """Attention of the nodes of `tree` over the pages of `kv_cache` (pa_tree_attention): q [rows, heads, D] (rows may be a view of a
     wider projection); row r of sequence b sees the first ctx_lens[b] cached tokens and, of the nodes behind them, those of its mask.
     heads is a multiple of the cache's heads.  beam_ids: table row per sequence (None: b).  ctx_lens, beam_ids: int32 device tensors,
-    or sequences of ints.  out: [rows, heads, D] like q, contiguous."""
+    or sequences of ints.  out: [rows, heads, D] like q, contiguous.
+
+    Up to 1024 sequences, heads of 64 or 128, pages of 16 rows (or multiples) that are not float; what is beyond goes through the general kernel, some
+    forty times as slow where contexts are long.  Partial results are kept in a workspace per host thread and stream."""
     pt, dev = kv_cache.page_table_, kv_cache.key_buffer_.device
     KVH, D = pt.num_heads_, kv_cache.head_dim_
     if q.dim() != 3 or q.shape[0] != tree.rows or q.shape[2] != D or q.shape[1] % KVH or q.shape[1] == 0:
