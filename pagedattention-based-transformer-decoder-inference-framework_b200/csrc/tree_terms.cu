@@ -23,8 +23,8 @@
 //
 // What bounds it: the latency of a tile's chain (scores, vote, weights, products, sums) at one or two softmax warps for each quarter of an SM, and
 // of a piece's beginning and end, some 6 us.  12 sequences of 4K keys, 32 heads: half pages and 32 float rows 152 us, 5.3 TB/s; int8 pages and 16
-// float rows 87 us, 4.8 TB/s; 48 sequences of 1 to 2K keys, int8 pages 130 us, 3.4 TB/s (values' scales that differ by more than 8 in every tile:
-// 256); 16 sequences of 4K keys, 128 rows a kv head (blocks of 64) 134 us, 257 TFLOP/s of the formula's operations.  Rows as the columns of the products keep the tile at 128 keys for any number of rows: as rows
+// float rows 87 us, 4.8 TB/s; 48 sequences of 1 to 2K keys, int8 pages 128 us, 3.5 TB/s (values' scales that differ by more than 8 in every tile:
+// 255); 16 sequences of 4K keys, 128 rows a kv head (blocks of 64) 134 us, 257 TFLOP/s of the formula's operations.  Rows as the columns of the products keep the tile at 128 keys for any number of rows: as rows
 // they would fill 128 lanes with 16.  Digits and terms instead of tf32 or a conversion to half: int8 pages stay as they are, and float results keep
 // 22 bits.  Reading a tile's maximum before its exponentials for every tile took 223 us where votes on 2^8 took 192 (before the shares counted
 // beginnings and ends).  Instructions are what its caches are short of: a branch more in the softmax, never taken, took 14 of 107 us where pieces are
@@ -114,7 +114,7 @@ __device__ __forceinline__ float from_digits4(uint32_t d0, uint32_t d1, uint32_t
 // Weights of a tile whose values have scales that are not alike, by all softmax threads, each a key's RH rows from h0 on: from floats in the place of the digits
 // (a word a row, see the softmax) to digits relative to the row's largest product of weight and scale; units: what the rows' sums are times.  A product that
 // is not finite makes its row's sums NaN.  Row by row through shared memory and out of line, since instructions are what the kernel's caches are short of
-// (48 sequences of 1 to 2K keys: 129 us, inline and in registers 138, without any of this 123).
+// (48 sequences of 1 to 2K keys: 128 us, inline and in registers 138, without any of this 123).
 template <int R, int RH, int SOFTMAX>
 __device__ __noinline__ void digits_apart(uint32_t pb, int h0, float vsc, uint32_t* s_top, float* units) {
     const int lane = threadIdx.x & 31, kk = threadIdx.x & 127, quarter = threadIdx.x >> 5 & 3;
@@ -695,12 +695,19 @@ __global__ void __launch_bounds__(Shape<D, I8, R>::THREADS, Shape<D, I8, R>::CTA
                 for (int c = 0; c < C::NO / 32; ++c) {
                     uint32_t x[32];
                     tmem_ld32(o_col(sb) + lane_base + c * 32, x);
+                    float unit[8] = {};         // int8: of the rows' digits
+                    if constexpr (I8) {
+                        const float4* u = reinterpret_cast<const float4*>(s_unit + ring4 * R + c * 8);
+                        const float4 a = u[0], b = u[1];
+                        unit[0] = a.x; unit[1] = a.y; unit[2] = a.z; unit[3] = a.w;
+                        unit[4] = b.x; unit[5] = b.y; unit[6] = b.z; unit[7] = b.w;
+                    }
                     tmem_wait_ld();
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
                         if constexpr (I8) {                 // a row's digits
                             const int r = c * 8 + j / 4;
-                            o[r] = fmaf(from_digits4(x[j], x[j + 1], x[j + 2], x[j + 3]), s_unit[ring4 * R + r], o[r]);
+                            o[r] = fmaf(from_digits4(x[j], x[j + 1], x[j + 2], x[j + 3]), unit[j / 4], o[r]);
                         } else {                            // two rows' large terms, and their small ones
                             const int r = c * 16 + j / 2;
                             o[r] += __uint_as_float(x[j]) + __uint_as_float(x[j + 2]);
@@ -789,10 +796,10 @@ static int launch(const TreeWork& a, cudaStream_t st) {
 int tree_terms_workers(int block) { return device_info().sm_count * (block == 16 ? 2 : 1); }
 
 // Rows of a block, 0 where this kernel does not serve or the streaming one is faster.  us, this kernel against the streaming one: int8 pages, 16
-// rows: 1000 keys 114 against 214, 4K keys 87 against 204, ragged 130 against 216, 100 keys 38 against 52; half pages, 32 float rows: 4K keys 153
+// rows: 1000 keys 112 against 214, 4K keys 87 against 204, ragged 128 against 216, 100 keys 38 against 52; half pages, 32 float rows: 4K keys 153
 // against 292, 1000 keys 186 against 305, 90 keys 96 against 71 (the host does not know how long contexts are); 16 float rows 205 against 209, and
 // of 64 columns 65 against 58: from 17 on.  int8 rows of 64 bytes have no tile here.  Blocks: int8, 256 rows in 32s 332, in 16s 365, 16 rows in a
-// block of 32 (ragged) 229 instead of 130; half, 128 rows in 64s 133, in 32s 196; 32 rows in a block of 64 177 instead of 153.
+// block of 32 (ragged) 229 instead of 128; half, 128 rows in 64s 133, in 32s 196; 32 rows in a block of 64 177 instead of 153.
 int tree_terms_block(const TreeParams& p) {
     const int G = p.heads / p.kv_heads, rows = p.most * G;
     const bool half = p.q_type == PA_TYPE_F32 && p.kv_type == PA_TYPE_F16, bytes = p.kv_type == PA_TYPE_I8 && p.dim == 128;
