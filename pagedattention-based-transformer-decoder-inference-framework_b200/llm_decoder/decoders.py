@@ -77,23 +77,22 @@ class _Bufs:
         self.hs = torch.ones(R, **f32)
         self.ws = None  # GEMM / linear scratch for R rows (owned here, never by the library; _DecoderBase._scratch)
         self.qp = self.kp = self.vp = None  # q / k / v projections [R, hid] f32, allocated when a layer has them
-        self.whole = self   # where what is allocated on demand stays: first()'s results share it
+        self.whole = None   # of first()'s results: the buffers that they are rows of, where what is allocated on demand stays
 
     def first(self, R):
         """The buffers of the first R rows."""
         few = copy.copy(self)
-        few.__dict__.update({k: v[:R] for k, v in self.__dict__.items() if isinstance(v, torch.Tensor) and k != "ws"}, R=R)
+        few.__dict__.update({k: v[:R] for k, v in self.__dict__.items() if isinstance(v, torch.Tensor) and k != "ws"}, R=R, whole=self.whole or self)
         return few
 
     def on_demand(self, name, make):
         """The buffer `name`, made once by make(rows) for the rows of all."""
-        if getattr(self.whole, name, None) is None:
-            setattr(self.whole, name, make(self.whole.R))
-        x = getattr(self.whole, name)
-        if self.whole is not self:
-            x = x[:self.R]
-            setattr(self, name, x)
-        return x
+        whole = self.whole or self
+        if getattr(whole, name, None) is None:
+            setattr(whole, name, make(whole.R))
+        if whole is not self:
+            setattr(self, name, getattr(whole, name)[:self.R])
+        return getattr(self, name)
 
 
 class _DecoderBase:
@@ -168,7 +167,7 @@ class _DecoderBase:
         request that does not fit re-allocates AND drops the captured graph."""
         if need == 0:
             return None, 0
-        bf = bf.whole
+        bf = bf.whole or bf
         if bf.ws is None or bf.ws.numel() < need:
             bf.ws = torch.empty(need, dtype=torch.uint8, device=self.device)
             if bf is getattr(self, "bufs", None):

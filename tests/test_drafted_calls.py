@@ -1,4 +1,6 @@
 """What generation with drafted trees refuses, and what it does when something under it goes wrong."""
+import weakref
+
 import numpy as np
 import pytest
 import torch
@@ -110,3 +112,6 @@ def test_steps_of_other_sizes_share_their_scratch(tmp_path):
     assert dec._scratch(few, 1000) == dec._scratch(fewer, 900) == dec._scratch(bufs, 1000)
     made = [b.on_demand("lq", lambda rows: torch.empty((rows, 128), dtype=torch.int8, device=dec.device)) for b in (few, fewer, bufs, bufs.first(7))]
     assert [len(x) for x in made] == [9, 4, 12, 7] and len({x.data_ptr() for x in made}) == 1
+    gone = weakref.ref(bufs)
+    del bufs, few, fewer, made
+    assert gone() is None           # and it goes with the buffers, at once
