@@ -1099,6 +1099,69 @@ int pa_tree_accept(const int32_t* d_ids, const int32_t* d_tokens, const int32_t*
                    int num_tiles, int total_pages, int tile_size, int key_bytes, int value_bytes, int num_caches, void* const* caches,
                    int32_t* d_counts, int32_t* d_out_tokens, int32_t* d_nodes, int32_t* d_new_lens, pa_stream_t stream);
 
+/* Sampling with drafted tokens (draw_tokens.cu): the distribution that a token is drawn from, draws from it by given numbers, drafted tokens
+ * kept or replaced.  No counterpart in the reference but its temperature / top-k / top-p filters (attention_cpu/softmax_lut.cpp:203-256).
+ *
+ * Row r of d_logits (rows `stride` elements apart; type PA_TYPE_F32, _F16 or _BF16) belongs to sequence d_row_seq[r] (NULL: r), whose rules
+ * are the entries of the device arrays [num_seqs], or the value where an array is NULL (a row whose sequence is outside [0, num_seqs):
+ * temperature 1 and nothing left out).  With x the row's logits (NaN as -inf, +inf as the type's largest value), top the largest of them:
+ *     w = exp((x - top) / temperature)       (temperature not above 0: only the lowest index of the largest)
+ *     a token stays if fewer than top_k tokens are above it (top_k <= 0: all do), if the w above it, of those that stay so far, sum up to
+ *     less than top_p of theirs (top_p not below 1: all do), and if its w is at least min_p; the largest always stays, tokens of one
+ *     value stay or go together;       p = w / (sum of the w that stay)
+ * Weights and sums are in 64 bits.  Vocabularies up to 1.5 million bytes of logits a row (more: PA_ERR_UNSUPPORTED).
+ *
+ * pa_truncated_softmax: p as floats [rows][vocab], rows probs_stride apart (zeros where every logit is -inf), in memory that the logits do not
+ *   share (PA_ERR_INVALID_ARG).
+ * pa_draw_tokens: d_ids[r][i] = the first v up to which the sum of p, without the tokens d_ids[r][0 .. i - 1], exceeds
+ *   d_uniform[r][i] times all of it (numbers below 0 and NaN as 0; from 1 on: the last token that stays); -1 where no token is left.
+ *   d_logprobs (NULL: not wanted): log p of it, -inf for -1.
+ * pa_verify_drafts: rows are nodes of drafted trees (pa_draft_trees; d_node_start [num_seqs + 1], d_row_seq not NULL).  The children of node r, in
+ *   order, were drawn from q = row d_draft_rows[r] (NULL: r) of d_draft (of draft_type, rows draft_stride apart): each from all of it, or
+ *   with `distinct` from what the ones before it left.  One after the other a child c is kept, where d_uniform[c][0] q(c) S < max(p(c) -
+ *   a q(c), 0) (1 - Q), or refused (a += S / (1 - Q), S = sum max(p - a q, 0), with `distinct` Q += q(c); from a = 0, S = 1, Q = 0).
+ *   d_ids[r]: the token of the child that is kept, else one drawn by d_uniform[r][1] from max(p - a q, 0) (from p, where nothing is left of it);
+ *   of a node without children, or without a row of d_draft: from p.  -1 where every logit is -inf.  So the tokens along the path that
+ *   pa_tree_accept takes by these ids are distributed as those drawn one by one.  Children outside the vocabulary are passed over.
+ *   d_logprobs (NULL: not wanted): log p of the id. */
+typedef struct {
+    const int32_t* d_row_seq;
+    int num_seqs;
+    const float* d_temperature;
+    const int32_t* d_top_k;
+    const float* d_top_p;
+    const float* d_min_p;
+    float temperature;
+    int top_k;
+    float top_p, min_p;
+} pa_draw_rules;
+int pa_truncated_softmax(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, float* d_probs,
+                         int64_t probs_stride, pa_stream_t stream);
+int pa_draw_tokens(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, const float* d_uniform, int count,
+                   int32_t* d_ids, float* d_logprobs, pa_stream_t stream);
+int pa_verify_drafts(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, const float* d_uniform,
+                     const int32_t* d_tokens, const int32_t* d_parents, const int32_t* d_node_start, const void* d_draft, int draft_type,
+                     int64_t draft_stride, int draft_count, const int32_t* d_draft_rows, int distinct, int32_t* d_ids, float* d_logprobs,
+                     pa_stream_t stream);
+
+/* Pages handed out on the GPU (device_pages.cu), for steps whose lengths only the GPU knows; the host's way is KVTileCache::register_tile
+ * (kv_cache/kv_tile_cache.cpp:65-98).  Table row b holds pages for its first d_held[b] tiles, of every head; the d_state[0] free pages are the
+ * first of d_free [total_pages].  d_state [4]: free pages, calls that were refused, and a word that every call leaves at zero.
+ *
+ * pa_take_pages: room for rows d_start[b] .. d_start[b + 1] - 1 behind the first d_lengths[b] tokens of sequence (and table row) b: tiles from
+ *   d_held[b] to ceil((length + rows) / tile_size) get pages from the end of the free list, sequence by sequence, tile by tile, head by head.
+ *   Where the pages or the table do not suffice the call is refused as a whole: no page is handed out and d_state[1] grows by one.
+ *   d_row_seq, d_positions [rows] (-1: a row of no sequence) and d_slots [rows][num_heads]: page * tile_size + position % tile_size, or -1 where
+ *   there is no page.
+ * pa_release_pages: the tiles of sequence b from ceil(d_lengths[b] / tile_size) on give back their pages, in the reverse of that order (so that
+ *   releasing what was just taken undoes it), and their entries become -1.
+ * Up to 16384 sequences (more: PA_ERR_UNSUPPORTED); total_pages * tile_size < 2^31. */
+int pa_take_pages(int32_t* d_table, int num_beams, int num_heads, int num_tiles, int tile_size, int total_pages, int32_t* d_free, int32_t* d_held,
+                  int32_t* d_state, const int32_t* d_lengths, const int32_t* d_start, int num_seqs, int rows, int32_t* d_row_seq,
+                  int32_t* d_positions, int32_t* d_slots, pa_stream_t stream);
+int pa_release_pages(int32_t* d_table, int num_beams, int num_heads, int num_tiles, int tile_size, int total_pages, int32_t* d_free, int32_t* d_held,
+                     int32_t* d_state, const int32_t* d_lengths, int num_seqs, pa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,7 +5,7 @@
 The .so lands next to csrc/ (git-ignored).
 
 --core builds libpa_b200_core.so from the CORE sources only: the page table, the small decoder ops with the fp32 linear
-layer, sampling with its logit rules, drafted trees' arrays, and the ragged-batch sequence ops (norm / token shift / recurrence, differential and latent attention,
+layer, sampling with its logit rules and draws, pages handed out on the GPU, drafted trees' arrays, and the ragged-batch sequence ops (norm / token shift / recurrence, differential and latent attention,
 routed experts, masked softmax attention, matrix-state recurrences).  It is what the config-driven models need; a first run in a fresh checkout compiles this and no more.
 """
 import glob
@@ -18,7 +18,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libpa_b200.so")
 OUT_CORE = os.path.join(HERE, "libpa_b200_core.so")
-CORE = ("page_table.cu", "decoder_ops.cu", "linear_tf32x3.cu", "sampling.cu", "logit_rules.cu", "draft_tree.cu", "seq_ops.cu", "diff_attention.cu",
+CORE = ("page_table.cu", "decoder_ops.cu", "linear_tf32x3.cu", "sampling.cu", "logit_rules.cu", "draw_tokens.cu", "device_pages.cu", "draft_tree.cu", "seq_ops.cu", "diff_attention.cu",
         "latent_attention.cu", "masked_attention.cu", "attention_tc.cu", "masked_decode.cu", "latent_decode.cu", "recurrence_ops.cu", "moe_ops.cu", "moe_tc.cu")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 

@@ -12,6 +12,7 @@ from .int8_quant import (batch_dequantize, batch_minmax_scale, batch_quantize, c
                          compute_minmax_scale, dequantize_from_int8, dnnl_matmul_int8, quantize_to_int8)
 from .kv_tile_cache import KVTileCache  # noqa: F401
 from .page_table import PageTable  # noqa: F401
+from .device_pages import DevicePages  # noqa: F401
 from . import sampling  # noqa: F401
 from .draft_tree import Accepted, DraftTree, TreeCaches, lookup_drafts, paged_tree_attention, tree_accept  # noqa: F401
 

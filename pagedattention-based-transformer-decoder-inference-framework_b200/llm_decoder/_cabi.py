@@ -20,6 +20,14 @@ _lib = None
 
 _vp, _i32, _i64, _f32, _f64, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double, C.c_size_t
 
+
+
+class DrawRules(C.Structure):
+    """pa_draw_rules."""
+    _fields_ = [("row_seq", _vp), ("num_seqs", _i32), ("temperatures", _vp), ("top_ks", _vp), ("top_ps", _vp), ("min_ps", _vp),
+                ("temperature", _f32), ("top_k", _i32), ("top_p", _f32), ("min_p", _f32)]
+
+
 _DECODE_COMMON = [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp]
 
 _SIGS = {
@@ -243,6 +251,12 @@ _SIGS = {
     "pa_draft_trees": ([_vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp], _i32),
     "pa_tree_accept": ([_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, C.POINTER(_vp),
                         _vp, _vp, _vp, _vp, _vp], _i32),
+    # sampling with drafted tokens (draw_tokens.cu), pages handed out on the GPU (device_pages.cu)
+    "pa_truncated_softmax": ([_vp, _i32, _i64, _i32, _i32, C.POINTER(DrawRules), _vp, _i64, _vp], _i32),
+    "pa_draw_tokens": ([_vp, _i32, _i64, _i32, _i32, C.POINTER(DrawRules), _vp, _i32, _vp, _vp, _vp], _i32),
+    "pa_verify_drafts": ([_vp, _i32, _i64, _i32, _i32, C.POINTER(DrawRules), _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _vp, _i32, _vp, _vp, _vp], _i32),
+    "pa_take_pages": ([_vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp], _i32),
+    "pa_release_pages": ([_vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp], _i32),
     "pa_causal_conv": ([_vp, _i64, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i64, _i32, _vp], _i32),
 }
 

@@ -110,6 +110,28 @@ class KVTileCache:
             self._reset_allocator()
             self.page_table_.clear()
 
+    # ---- pages handed out on the GPU (no reference code) ---------------------------------
+    def pages_on_device(self):
+        """A DevicePages for this cache's table and free pages (and those of the caches that share them): pages are taken and released on the
+        GPU from now on, and register_tile, release_beam, fork_beam and the others raise until its to_host().  No page may be shared."""
+        from .device_pages import DevicePages
+        with self.mutex_:
+            if self._page_refs:
+                raise RuntimeError("KVTileCache.pages_on_device: pages are shared by several beams")
+            pages = DevicePages(self.page_table_, self.total_pages_, self.tile_size_, free=self._free)
+            pages._cache = self
+        return pages
+
+    def pages_of_host(self, free):
+        """DevicePages.to_host: the table's entries are this side's again, oldest first by tile, and `free` the free pages."""
+        pt = self.page_table_
+        with self.mutex_:
+            table = pt.host_table_.reshape(pt.num_beams_, pt.num_heads_, pt.num_tiles_)
+            self.tile_to_page_map_.clear()
+            for t, b, h in np.argwhere((table >= 0).transpose(2, 0, 1)).tolist():
+                self.tile_to_page_map_[(b, h, t)] = int(table[b, h, t])
+            self._free[:] = free
+
     # ---- kv_tile_cache.cpp:52-62 (device addresses) ------------------------------------
     def _page_offset_bytes(self, page_id):
         assert 0 <= page_id < self.total_pages_, "page_id out of range"
@@ -124,6 +146,7 @@ class KVTileCache:
 
     # ---- kv_tile_cache.cpp:65-98 -------------------------------------------------------
     def register_tile(self, beam_id, head_id, tile_id):
+        self.page_table_.on_host("KVTileCache.register_tile")
         with self.mutex_:
             key = (int(beam_id), int(head_id), int(tile_id))
             page = self.tile_to_page_map_.get(key)
@@ -144,6 +167,7 @@ class KVTileCache:
         pages -- goes through register_tile and fails or evicts as it does."""
         beam_id, t0, t1 = int(beam_id), int(t0), int(t1)
         pt = self.page_table_
+        pt.on_host("KVTileCache.register_range")
         H, T = pt.num_heads_, pt.num_tiles_
         n = (t1 - t0) * H
         if n <= 0:
@@ -176,6 +200,7 @@ class KVTileCache:
         at the next flush, on the device; pages return to the free list (a page still shared with another row only
         loses this reference).  Returns the number of tiles released."""
         beam_id = int(beam_id)
+        self.page_table_.on_host("KVTileCache.release_beam")
         with self.mutex_:
             m, pt, refs, free = self.tile_to_page_map_, self.page_table_, self._refs(), self._free
             keys = [k for k in m if k[0] == beam_id]
@@ -194,6 +219,7 @@ class KVTileCache:
         return len(keys)
 
     def free_pages(self):
+        self.page_table_.on_host("KVTileCache.free_pages")
         return len(self._free)
 
     def append_rows(self, src, k_off, v_off, row_slot, row_pos):
@@ -264,6 +290,7 @@ class KVTileCache:
 
     def save_tiles_cpu_format(self, path):
         pt = self.page_table_
+        pt.on_host("KVTileCache.save_tiles_cpu_format")
         pt.flush()
         flat = np.nonzero((pt.host_table_ >= 0) & (pt.host_table_ < self.total_pages_))[0]
         pages = pt.host_table_[flat]
@@ -285,6 +312,7 @@ class KVTileCache:
     def load_tiles_cpu_format(self, path):
         """Tiles of the file are (re)mapped to pages (fresh pages from the free list for unmapped tiles)
         and their K/V bytes uploaded in one batched scatter."""
+        self.page_table_.on_host("KVTileCache.load_tiles_cpu_format")
         nb = self.tile_payload_bytes()
         try:
             with open(path, "rb") as f:
@@ -326,9 +354,12 @@ class KVTileCache:
         return count
 
     # ---- hot path: append (get_write_ptr + row write, hpp:29-34) -------------------------
-    def append(self, new_k, new_v, positions, beam_ids=None):
+    def append(self, new_k, new_v, positions=None, beam_ids=None, slots=None):
         """new_k/new_v: [R, H, D] device tensors (f16 or f32; bf16 for bf16 pools), or page-locked host tensors (uploaded on the copy
-        stream, attention.HostPipe); positions: [R] int32 device."""
+        stream, attention.HostPipe); positions: [R] int32 device.  slots: instead of positions (and beam_ids), the rows' places in the
+        pools, [R, H] int32 device as DevicePages.take gives them; rows at -1 go nowhere."""
+        if (positions is None) == (slots is None) or (slots is not None and beam_ids is not None):
+            raise ValueError("KVTileCache.append: positions, or slots")
         pt = self.page_table_
         table = pt.device_data()
         releases = []
@@ -345,8 +376,16 @@ class KVTileCache:
         assert new_k.is_contiguous() and new_v.is_contiguous() and new_k.shape == new_v.shape
         assert new_k.shape[1] == pt.num_heads_ and new_k.shape[2] == self.head_dim_
         lib = _cabi.lib()
-        common = (table.data_ptr(), pt.num_beams_, pt.num_heads_, pt.num_tiles_, self.total_pages_,
-                  self.tile_size_, self.head_dim_, new_k.data_ptr(), new_v.data_ptr(),
+        if slots is None:
+            places = (table.data_ptr(), pt.num_beams_, pt.num_heads_, pt.num_tiles_, self.total_pages_, self.tile_size_)
+        else:       # a table of their own: pages of one row, of which every new row has its first
+            if slots.shape != (R, pt.num_heads_) or slots.dtype != torch.int32 or slots.device != table.device or not slots.is_contiguous():
+                raise ValueError(f"KVTileCache.append: slots are int32 [{R}, {pt.num_heads_}] on {table.device}")
+            if R == 0:
+                return
+            places = (slots.data_ptr(), R, pt.num_heads_, 1, self.total_pages_ * self.tile_size_, 1)
+            positions = torch.zeros(R, dtype=torch.int32, device=table.device)
+        common = (*places, self.head_dim_, new_k.data_ptr(), new_v.data_ptr(),
                   _cabi.ptr(beam_ids), positions.data_ptr(), R, _cabi.stream())
         with _cabi.on_device(table.device):
             if self.dtype == "f32":
@@ -377,6 +416,7 @@ class KVTileCache:
         pt = self.page_table_
         nt = pt.num_tiles_ if num_tiles is None else int(num_tiles)
         refs = self._refs()
+        pt.on_host("KVTileCache.fork_beam")
         with self.mutex_:
             for h in range(pt.num_heads_):
                 for t in range(nt):
@@ -414,6 +454,7 @@ class KVTileCache:
         `beam_ids`) are HOST integer sequences: page management is host logic, as in the reference
         (kv_tile_cache.cpp:65-98)."""
         pt = self.page_table_
+        pt.on_host("KVTileCache.append_cow")
         pos_h = [int(p) for p in positions]
         rows = list(range(len(pos_h))) if beam_ids is None else [int(b) for b in beam_ids]
         refs = self._refs()

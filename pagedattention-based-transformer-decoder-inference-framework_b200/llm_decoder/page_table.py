@@ -22,6 +22,12 @@ class PageTable:
         self.host_table_ = np.empty(0, dtype=np.int32)
         self._pending = {}
         self._device = torch.device(device) if device is not None else None
+        self.device_pages_ = None       # a DevicePages, while it is the one that changes the table
+
+    def on_host(self, what):
+        """Raises while a DevicePages hands out the table's pages: the host does not know them."""
+        if self.device_pages_ is not None:
+            raise RuntimeError(f"{what}: the table's pages are handed out on the GPU (DevicePages.to_host gives them back)")
 
     # page_table.cpp:14-26
     def init(self, num_beams, num_heads, num_tiles):
@@ -33,6 +39,7 @@ class PageTable:
         self.d_table_ = torch.empty(self.total_entries_, dtype=torch.int32, device=dev)
         self.host_table_ = np.full(self.total_entries_, -1, dtype=np.int32)
         self._pending.clear()
+        self.device_pages_ = None
         self._clear_device()
 
     def _clear_device(self):
@@ -45,6 +52,7 @@ class PageTable:
         if self.d_table_ is not None:
             self.host_table_.fill(-1)
             self._pending.clear()
+            self.device_pages_ = None
             self._clear_device()
 
     # page_table.hpp:39-42
@@ -53,6 +61,7 @@ class PageTable:
 
     # page_table.cpp:49-53 (assert on range, as the reference)
     def assign(self, beam_id, head_id, tile_id, page_id):
+        self.on_host("PageTable.assign")
         idx = self.index(beam_id, head_id, tile_id)
         assert 0 <= idx < self.total_entries_, "PageTable.assign: index out of range"
         self.host_table_[idx] = page_id
@@ -60,6 +69,7 @@ class PageTable:
 
     def assign_many(self, flat_idx, pages):
         """Vectorised assign: flat_idx / pages int arrays (host)."""
+        self.on_host("PageTable.assign_many")
         flat_idx = np.asarray(flat_idx, dtype=np.int64)
         pages = np.asarray(pages, dtype=np.int32)
         assert flat_idx.min(initial=0) >= 0 and flat_idx.max(initial=-1) < self.total_entries_
@@ -76,6 +86,7 @@ class PageTable:
     # page_table.cpp:64-67 (the reference edits only the host mirror; here the device
     # entry is cleared at the next flush as well)
     def remove(self, beam_id, head_id, tile_id):
+        self.on_host("PageTable.remove")
         idx = self.index(beam_id, head_id, tile_id)
         self.host_table_[idx] = -1
         self._pending[idx] = -1
@@ -96,6 +107,7 @@ class PageTable:
 
     # page_table.hpp:44-49 -- host-visible form of the device lookup
     def lookup(self, beam_id, head_id, tile_id):
+        self.on_host("PageTable.lookup")
         idx = self.index(beam_id, head_id, tile_id)
         if idx < 0 or idx >= self.total_entries_:
             return -1
@@ -123,11 +135,13 @@ class PageTable:
 
     # page_table.cpp:59-62
     def sync_to_gpu(self):
+        self.on_host("PageTable.sync_to_gpu")
         self._pending.clear()
         self.d_table_.copy_(torch.from_numpy(self.host_table_), non_blocking=False)
 
     def load_host_table(self, table):
         """Replace the whole map from a host array [num_beams, num_heads, num_tiles]."""
+        self.on_host("PageTable.load_host_table")
         table = np.ascontiguousarray(table, dtype=np.int32).reshape(-1)
         assert table.size == self.total_entries_
         self.host_table_[:] = table

@@ -1,6 +1,10 @@
 """Device-side sampling over vocabulary logits: the reference's CPU filters
 (attention_cpu/softmax_lut.cpp:203-256) and its GPU sketch (attention/top_k_top_p_filter.cuh:55-111)
-as three kernels of libpa_b200.so.  Tensors are CUDA float32 [rows, vocab]."""
+as three kernels of libpa_b200.so (`sample`: tensors are CUDA float32 [rows, vocab]); rules of a batch's requests (adjust_logits); and, for requests
+with temperatures and truncations of their own, the distribution that is drawn from, draws from it by given numbers and drafted tokens kept or
+replaced (truncated_softmax, draw_tokens, verify_drafts)."""
+import ctypes
+
 import torch
 
 from . import _cabi
@@ -193,3 +197,122 @@ def adjusted_argmax(logits, history=None, history_start=None, repetition=1.0, pr
     ids = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
     _rules(logits, None, ids, history, history_start, repetition, presence, frequency, bias, allowed, allowed_rows, row_seq, tree)
     return ids
+
+
+def _draw_rules(logits, temperature, top_k, top_p, min_p, row_seq, tree):
+    """(arguments of the logits, pa_draw_rules by reference, what must live until the call) of a call over logits."""
+    dev, at, kind = logits.device, logits.get_device(), _LOGIT_TYPES.get(logits.dtype)
+    if logits.dim() != 2 or kind is None or not logits.is_cuda:
+        raise ValueError("logits: [rows, vocab] of float32, float16 or bfloat16 on the GPU")
+    (rows, V), (stride, one) = logits.shape, logits.stride()
+    if V == 0 or (rows and ((V > 1 and one != 1) or (rows > 1 and stride < V))):
+        raise ValueError("logits: a vocabulary, and rows of consecutive elements that do not overlap")
+    if rows and V * logits.element_size() > _MOST_ROW_BYTES:
+        raise ValueError(f"logits: rows of at most {_MOST_ROW_BYTES} bytes")
+
+    def of(x, dtype, what, n):
+        if x.dtype is not dtype or x.get_device() != at or x.dim() != 1 or not x.is_contiguous() or (n is not None and x.numel() != n):
+            raise ValueError(f"{what}: a contiguous {dtype} vector{'' if n is None else f' of {n}'} on {dev}")
+        return x.data_ptr()
+    seqs, rules = rows, _cabi.DrawRules()
+    if tree is not None:
+        if tree.rows != rows or tree.device != dev or row_seq is not None:
+            raise ValueError("tree: one with a node for every row, on the logits' device (and then no row_seq)")
+        seqs, rules.row_seq = tree.num_seqs, tree.row_seq.data_ptr()
+    elif row_seq is not None:
+        rules.row_seq = of(row_seq, torch.int32, "row_seq", rows)
+        seqs = None             # as many as the rules say
+    for x, what, dtype in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                           (min_p, "min_p", torch.float32)):
+        if isinstance(x, torch.Tensor):
+            setattr(rules, what + "s", of(x, dtype, what, seqs))
+            seqs = x.numel()
+        else:
+            x = int(x) if dtype is torch.int32 else float(x)
+            if not x >= 0 or (what == "min_p" and x > 1) or (what == "top_k" and x >= 2 ** 31):
+                raise ValueError(f"{what}: not below 0{', at most 1' if what == 'min_p' else ''}")
+            setattr(rules, what, x)
+    rules.num_seqs = (2 ** 31 - 1) if seqs is None else seqs        # (values alone: whatever sequences the rows name)
+    return (logits.data_ptr(), kind, stride if rows > 1 else V, rows, V, ctypes.byref(rules))
+
+
+_MOST_ROW_BYTES = 1500000               # what the shared memory of a cluster of eight CTAs holds
+
+
+def truncated_softmax(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, row_seq=None, tree=None, out=None):
+    """The distribution that the next token of every row of logits [rows, vocab] is drawn from, float32 [rows, vocab] (pa_truncated_softmax).
+    With w = exp((x - max x) / temperature) a token stays if fewer than top_k are above it, if the w above it, of those that stay so far, sum up
+    to less than top_p of theirs, and if its w is at least min_p; p = w / (sum of what stays).  The largest always stays, tokens of one value stay or go
+    together; a row of -inf alone gives zeros.  (apply_topk_topp_filter is the reference's filter: of equal tokens the later go first, top_p counts
+    before top_k, and nothing is divided again.)
+
+    temperature, top_k, top_p, min_p: a number, or a tensor per sequence (float32; top_k int32).  temperature 0: the lowest index of the
+    largest alone; top_k 0, top_p 1, min_p 0 leave nothing out.  row_seq: the sequence of every row (None: row r is sequence r); tree: the rows are the
+    nodes of a DraftTree.  out: float32, rows of consecutive elements, no memory of the logits."""
+    if out is None:
+        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != torch.float32 or out.device != logits.device or \
+            (out.numel() and out.shape[1] > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
+        raise ValueError("out: float32 of the logits' shape and device, rows of consecutive elements")
+    args = _draw_rules(logits, temperature, top_k, top_p, min_p, row_seq, tree)
+    if args[3]:
+        with _cabi.on_device(logits.device):
+            _cabi.check(_cabi.lib().pa_truncated_softmax(*args, out.data_ptr(), out.stride(0) if args[3] > 1 else args[4], _cabi.stream_on(logits.device)),
+                        "pa_truncated_softmax")
+    return out
+
+
+def draw_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, row_seq=None, tree=None, logprobs=False):
+    """Tokens drawn by the numbers `uniform` (float32 in [0, 1), [rows] or [rows, n]) from the distributions of truncated_softmax: int32 of uniform's
+    shape (pa_draw_tokens).  The first token up to which the probabilities exceed the number; of n numbers a row each draws from what the ones
+    before it left (n different tokens); -1 where nothing is left.  logprobs=True: (ids, log p of them, float32, -inf for -1)."""
+    rows = logits.shape[0]
+    if uniform.dim() not in (1, 2) or uniform.shape[0] != rows or uniform.dtype is not torch.float32 or uniform.device != logits.device or \
+            not uniform.is_contiguous():
+        raise ValueError(f"uniform: contiguous float32 [{rows}] or [{rows}, n] on {logits.device}")
+    ids = torch.empty(uniform.shape, dtype=torch.int32, device=logits.device)
+    logs = torch.empty(uniform.shape, dtype=torch.float32, device=logits.device) if logprobs else None
+    args = _draw_rules(logits, temperature, top_k, top_p, min_p, row_seq, tree)
+    if ids.numel():
+        with _cabi.on_device(logits.device):
+            _cabi.check(_cabi.lib().pa_draw_tokens(*args, uniform.data_ptr(), ids.numel() // rows, ids.data_ptr(), _cabi.ptr(logs),
+                                                   _cabi.stream_on(logits.device)), "pa_draw_tokens")
+    return (ids, logs) if logprobs else ids
+
+
+def verify_drafts(logits, tree, uniform, draft_probs, draft_rows=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, distinct=False,
+                  logprobs=False):
+    """What a step over a DraftTree (with tokens) gives at every node, int32 [rows] (pa_verify_drafts), where the children of a node were drawn by
+    chance from a draft model: the token of a child, or another one, such that the tokens along the path that tree_accept takes by these ids are distributed
+    as if they had been drawn one by one from truncated_softmax(logits, ...).
+
+    draft_probs: [n, vocab] of float32, float16 or bfloat16, rows of consecutive elements; row draft_rows[r] (int32, None: r) is what the children
+    of node r were drawn from, in order, each from all of it, or with distinct=True from what the ones before it left (draw_tokens with n numbers).
+    draft_rows[r] outside [0, n): children that were not drawn by chance (lookup_drafts); the id is drawn as by draw_tokens.
+    uniform: float32 [rows, 2] in [0, 1): for the test of the node itself, and for the draw at it.  The rules are those of truncated_softmax,
+    per sequence of the tree.  logprobs=True: (ids, log p of them)."""
+    rows, V, dev = *logits.shape, logits.device
+    if tree.tokens is None:
+        raise ValueError("tree: one with tokens")
+    kind = _LOGIT_TYPES.get(draft_probs.dtype)
+    if kind is None or draft_probs.dim() != 2 or draft_probs.shape[1] != V or draft_probs.device != dev or \
+            (draft_probs.numel() and ((V > 1 and draft_probs.stride(1) != 1) or (draft_probs.shape[0] > 1 and draft_probs.stride(0) < V))):
+        raise ValueError(f"draft_probs: [n, {V}] of float32, float16 or bfloat16 on {dev}, rows of consecutive elements")
+    if draft_rows is None:
+        if draft_probs.shape[0] != rows:
+            raise ValueError(f"draft_probs: a row for each of the {rows} nodes, or draft_rows")
+    elif draft_rows.dtype is not torch.int32 or draft_rows.shape != (rows,) or draft_rows.device != dev or not draft_rows.is_contiguous():
+        raise ValueError(f"draft_rows: a contiguous int32 vector of {rows} on {dev}")
+    if uniform.dtype is not torch.float32 or uniform.shape != (rows, 2) or uniform.device != dev or not uniform.is_contiguous():
+        raise ValueError(f"uniform: contiguous float32 [{rows}, 2] on {dev}")
+    ids = torch.empty(rows, dtype=torch.int32, device=dev)
+    logs = torch.empty(rows, dtype=torch.float32, device=dev) if logprobs else None
+    args = _draw_rules(logits, temperature, top_k, top_p, min_p, None, tree)
+    n = draft_probs.shape[0]
+    if rows:
+        with _cabi.on_device(dev):
+            _cabi.check(_cabi.lib().pa_verify_drafts(
+                *args, uniform.data_ptr(), tree.tokens.data_ptr(), tree.parents.data_ptr(), tree.node_start.data_ptr(), draft_probs.data_ptr() if n else None,
+                kind, draft_probs.stride(0) if n > 1 else V, n, _cabi.ptr(draft_rows), int(distinct), ids.data_ptr(), _cabi.ptr(logs),
+                _cabi.stream_on(dev)), "pa_verify_drafts")
+    return (ids, logs) if logprobs else ids

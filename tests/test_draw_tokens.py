@@ -1,0 +1,363 @@
+"""truncated_softmax, draw_tokens and verify_drafts against their definitions in float64, row by row.
+
+Bounds.  A weight is off by 1.3e-12 of itself (the polynomial's end; 64-bit rounding is far below), so that a border of the cumulative sums is off by
+at most 2.6e-12 of the sum: an id is right where its number lies within 4e-12 of the id's own stretch.  A probability is rounded once to a float
+(2^-24), next to 2.6e-12 and, where it is below the normal floats, half of the smallest one; a log probability likewise, on
+top of 2.6e-12 of its argument."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+EPS = 4e-12
+
+
+def kept_weights(x, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, most=np.inf):
+    """Weights of one row by the definition, 0 where a rule leaves the token out."""
+    x = np.where(np.isnan(x), -np.inf, np.minimum(x.astype(np.float64), most))
+    w = np.zeros(len(x))
+    if x.max() == -np.inf:
+        return w
+    if not temperature > 0:
+        w[int(np.argmax(x))] = 1.0
+        return w
+    with np.errstate(invalid="ignore", over="ignore"):
+        w = np.where(x == -np.inf, 0.0, np.exp((x - x.max()) / np.float64(temperature)))
+    alive = x > -np.inf
+    values, group, size = np.unique(x, return_inverse=True, return_counts=True)
+    above = np.concatenate([np.cumsum(size[::-1])[::-1][1:], [0]])[group]
+    if 0 < top_k < len(x):
+        alive &= above < top_k
+    if top_p < 1:
+        mass = np.bincount(group, np.where(alive, w, 0.0), len(values))
+        before = np.concatenate([np.cumsum(mass[::-1])[::-1][1:], [0.0]])[group]
+        alive &= (before < np.float64(top_p) * mass.sum()) | (x == x.max())
+    alive &= (w >= min(min_p, 1.0)) if min_p > 0 else True
+    return np.where(alive, w, 0.0)
+
+
+def is_drawn(w, token, number):
+    """Whether `number` (in [0, 1)) draws the token, up to the bound."""
+    if w.sum() == 0:
+        return token == -1
+    cum = np.cumsum(w)
+    target, eps = np.float64(number) * cum[-1], EPS * cum[-1]
+    return 0 <= token < len(w) and w[token] > 0 and cum[token] - w[token] - eps <= target < cum[token] + eps
+
+
+def near_float(got, want):
+    return np.all(np.abs(got - want) <= np.abs(want) * (2.0 ** -24 + 3e-12) + 2.0 ** -150)
+
+
+class Case:
+    """Logits on the GPU as rows of a wider, odd allocation, and what each row's request asks for."""
+
+    def __init__(self, seed, kind, rows, V, rules="mixed", pad=0, shift=0, spread=3.0, odd=False):
+        rng = np.random.default_rng(seed)
+        x = rng.standard_normal((rows, V)) * spread
+        if odd:             # masks, infinities, not-a-numbers, lowest values, ties
+            x[rng.random((rows, V)) < 0.3] = -np.inf
+            x[rng.random((rows, V)) < 0.02] = np.nan
+            x[::5][rng.random((len(x[::5]), V)) < 0.02] = np.inf
+            x[1::5] = np.round(x[1::5])
+            x[2::5] = -np.inf
+            x[3::5][rng.random((len(x[3::5]), V)) < 0.5] = float(torch.finfo(TYPES[kind]).min)
+            if rows > 6:
+                x[6] = float(torch.finfo(TYPES[kind]).min)
+        store = torch.from_numpy(x.astype(np.float32)).to(TYPES[kind])
+        wide = torch.full((rows * (V + pad) + shift,), float("nan"), dtype=TYPES[kind]).cuda()
+        self.dev = wide[shift:].view(rows, V + pad)[:, :V]
+        self.dev.copy_(store)
+        self.x, self.rows, self.V, self.most = store.float().numpy(), rows, V, float(torch.finfo(TYPES[kind]).max)
+        u = rng.random((4, rows)).astype(np.float32)
+        on = rng.random((4, rows)) < 0.6
+        if rules == "mixed":
+            self.rules = dict(temperature=np.where(on[0], 0.2 + 2 * u[0], np.where(u[0] < 0.3, 0, 1)).astype(np.float32),
+                              top_k=np.where(on[1], 1 + (u[1] ** 2 * 1.2 * V).astype(np.int32), 0).astype(np.int32),
+                              top_p=np.where(on[2], u[2], 1).astype(np.float32), min_p=np.where(on[3], u[3] ** 4, 0).astype(np.float32))
+            self.kw = {k: torch.from_numpy(v).cuda() for k, v in self.rules.items()}
+        else:
+            self.kw = rules
+            self.rules = {k: np.full(rows, v, dtype=np.int32 if k == "top_k" else np.float32) for k, v in rules.items()}
+        self.numbers = rng.random((rows, 8)).astype(np.float32)
+
+    def weights(self, r, seq=None):
+        return kept_weights(self.x[r], most=self.most, **{k: v[r if seq is None else seq] for k, v in self.rules.items()})
+
+
+CASES = [(0, "f32", 9, 1000, "mixed", 3, 1), (1, "f32", 3, 50257, "mixed", 0, 0), (2, "bf16", 12, 1003, "mixed", 1, 3), (3, "f16", 12, 4097, "mixed", 0, 5),
+         (4, "f32", 5, 1, "mixed", 2, 1), (5, "f32", 40, 2, "mixed", 0, 0), (6, "bf16", 40, 7, "mixed", 0, 1), (7, "f32", 21, 33, "mixed", 1, 0),
+         (8, "f32", 2, 128000, dict(top_p=0.9), 0, 0), (9, "bf16", 2, 128001, dict(top_k=50, top_p=0.95), 0, 1), (10, "f32", 3, 20000, dict(), 5, 2),
+         (11, "f32", 2, 375000, dict(top_p=0.999, temperature=2.0), 0, 0), (12, "f16", 160, 3000, "mixed", 0, 0), (13, "f32", 300, 517, "mixed", 0, 0),
+         (14, "f32", 4, 9000, dict(top_k=8999), 0, 0), (15, "f32", 4, 9000, dict(temperature=1e-30, top_p=0.5), 0, 3), (16, "f32", 4, 9000, dict(temperature=math.inf, top_p=0.4), 0, 0),
+         (17, "bf16", 4, 9000, dict(top_p=0.0), 0, 0), (18, "f32", 4, 9000, dict(min_p=1.0), 0, 0), (19, "f32", 6, 30000, dict(top_p=0.9999999), 1, 0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("odd", [False, True])
+@pytest.mark.parametrize("spread", [3.0, 0.01, 30.0])
+@pytest.mark.parametrize("seed,kind,rows,V,rules,pad,shift", CASES)
+def test_probabilities_and_draws(seed, kind, rows, V, rules, pad, shift, spread, odd):
+    from llm_decoder import sampling
+    c = Case(seed, kind, rows, V, rules, pad, shift, spread, odd)
+    probs = sampling.truncated_softmax(c.dev, **c.kw).double().cpu().numpy()
+    one, logs = sampling.draw_tokens(c.dev, torch.from_numpy(c.numbers[:, 0].copy()).cuda(), logprobs=True, **c.kw)
+    some, more = sampling.draw_tokens(c.dev, torch.from_numpy(c.numbers).cuda(), logprobs=True, **c.kw)
+    one, logs, some, more = (t.cpu().numpy() for t in (one, logs, some, more))
+    assert probs.shape == (rows, V) and one.shape == (rows,) and some.shape == more.shape == (rows, 8)
+    for r in range(rows):
+        w = c.weights(r)
+        p = w / w.sum() if w.sum() else w
+        assert np.array_equal(probs[r] > 0, p.astype(np.float32) > 0) and near_float(probs[r], p)
+        assert is_drawn(w, one[r], c.numbers[r, 0])
+        for i, t in enumerate(some[r]):
+            assert is_drawn(w, t, c.numbers[r, i]), (r, i)
+            lp = math.log(p[t]) if t >= 0 else -math.inf
+            assert more[r, i] == lp or abs(more[r, i] - lp) <= abs(lp) * 2.0 ** -24 + 3e-12
+            if t >= 0:
+                w = w.copy()
+                w[t] = 0
+        assert some[r, 0] == one[r] and more[r, 0] == logs[r]
+
+
+@pytest.mark.gpu
+def test_numbers_at_the_ends():
+    """0 draws the first token that stays, what is not below 1 the last one, what is below 0 or no number the first."""
+    from llm_decoder import sampling
+    x = torch.full((6, 700), -math.inf, device="cuda")
+    x[:, 5], x[:, 30], x[:, 600] = 0.0, 1.0, 0.5
+    u = torch.tensor([0.0, 1.0 - 2.0 ** -24, 1.0, 7.0, -3.0, math.nan], device="cuda")
+    assert sampling.draw_tokens(x, u).tolist() == [5, 600, 600, 600, 5, 5]
+    ids, logs = sampling.draw_tokens(x[:1], torch.zeros(1, 5, device="cuda"), logprobs=True)
+    assert ids.tolist() == [[5, 30, 600, -1, -1]] and logs[0, 3:].tolist() == [-math.inf] * 2
+    assert sampling.draw_tokens(x, u, temperature=0.0).tolist() == [30] * 6
+    assert sampling.draw_tokens(x[:1], torch.zeros(1, 2, device="cuda"), temperature=0.0).tolist() == [[30, -1]]
+
+
+@pytest.mark.gpu
+def test_rows_by_sequence_and_other_streams():
+    """Rows name their sequences (or none: nothing is left out), calls run on the stream that is current, captured calls follow their inputs."""
+    from llm_decoder import DraftTree, sampling
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(5, 999, device="cuda", generator=g)
+    k = torch.tensor([1, 3], dtype=torch.int32, device="cuda")
+    row_seq = torch.tensor([1, 0, 1, 2, -1], dtype=torch.int32, device="cuda")
+    kept = (sampling.truncated_softmax(x, top_k=k, row_seq=row_seq) > 0).sum(1).tolist()
+    assert kept == [3, 1, 3, 999, 999]
+    assert (sampling.truncated_softmax(x, top_k=2, row_seq=row_seq) > 0).sum(1).tolist()[:4] == [2, 2, 2, 2]
+    tree = DraftTree([[-1, 0], [], [-1, 0, 0]], device="cuda")
+    kept = (sampling.truncated_softmax(x, top_k=torch.tensor([4, 5, 6], dtype=torch.int32, device="cuda"), tree=tree) > 0).sum(1).tolist()
+    assert kept == [4, 4, 6, 6, 6]
+    u = torch.rand(5, device="cuda", generator=g)
+    want = sampling.draw_tokens(x, u, top_p=0.8)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = sampling.draw_tokens(x, u, top_p=0.8)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ids = sampling.draw_tokens(x, u, top_p=0.8)
+        probs = sampling.truncated_softmax(x, top_p=0.8)
+    x.copy_(torch.randn(5, 999, device="cuda", generator=g))
+    graph.replay()
+    assert torch.equal(ids, sampling.draw_tokens(x, u, top_p=0.8)) and torch.equal(probs, sampling.truncated_softmax(x, top_p=0.8))
+    out = torch.zeros(5, 1203, device="cuda")
+    sampling.truncated_softmax(x, top_p=0.8, out=out[:, 2:1001])
+    assert torch.equal(out[:, 2:1001], probs) and not out[:, :2].any() and not out[:, 1001:].any()
+
+
+# ------------------------------------------------------------------------------------------------------------ verification
+def verified(w, children, tokens, q, numbers, draws, distinct):
+    """(kept child's token, or None; the weights that are drawn from; whether every test is clear of the bound) at one node."""
+    p = w / w.sum()
+    left, gone, clear = p, [], True
+    for c in children:
+        t = tokens[c]
+        if not 0 <= t < len(w):
+            continue
+        was = q.copy()
+        if distinct and gone:
+            was[gone] = 0
+            was = was / max(1 - q[gone].sum(), 1e-18)
+        clear &= abs(numbers[c] * was[t] - left[t]) > 1e-9 * (was[t] + left[t]) or was[t] == left[t] == 0
+        if numbers[c] * was[t] < left[t]:
+            return t, p, clear
+        rest = np.maximum(left - was, 0)
+        gone.append(t)
+        left = rest / rest.sum() if rest.sum() > 1e-300 else np.zeros_like(rest)
+    return None, (left if left.sum() else p), clear
+
+
+def tree_of(rng, n, most):
+    parents, children = [-1], [0]
+    for i in range(1, n):
+        p = int(rng.choice([j for j in range(i) if children[j] < most]))
+        parents.append(p)
+        children[p] += 1
+        children.append(0)
+    return parents
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("distinct", [False, True])
+@pytest.mark.parametrize("seed,kind,draft,sizes,V,most,rules,pad", [
+    (0, "f32", "f32", [6], 50257, 1, dict(top_p=0.9), 0), (1, "bf16", "bf16", [5, 0, 9, 1], 1003, 3, "mixed", 1), (2, "f16", "f32", [12, 7], 4097, 4, dict(), 3),
+    (3, "f32", "f16", [40] * 4, 300, 5, "mixed", 0), (4, "f32", "f32", [30, 30], 8, 6, dict(), 1), (5, "bf16", "f32", [3] * 60, 2000, 2, dict(temperature=0.7), 0),
+    (6, "f32", "bf16", [200], 64, 20, dict(top_k=20), 0), (7, "f32", "f32", [8, 8], 128000, 2, "mixed", 0), (8, "f32", "f32", [5], 40, 4, dict(temperature=0.0), 0)])
+def test_verification(seed, kind, draft, sizes, V, most, rules, pad, distinct):
+    from llm_decoder import DraftTree, sampling
+    rng = np.random.default_rng(seed)
+    parents = [tree_of(rng, n, min(most, V - 1)) if n else [] for n in sizes]
+    R = sum(sizes)
+    c = Case(seed, kind, R, V, rules, pad)
+    seq = [b for b, n in enumerate(sizes) for _ in range(n)]
+    first = np.concatenate([[0], np.cumsum(sizes)])
+    near = c.x.astype(np.float64) + rng.standard_normal((R, V)) * 0.8
+    q = np.exp(near - near.max(1, keepdims=True))
+    q /= q.sum(1, keepdims=True)
+    qd = torch.from_numpy(q.astype(np.float32)).to(TYPES[draft])
+    q = qd.double().numpy()
+    kids = [[int(first[b]) + i for i, p in enumerate(parents[b]) if p == r - first[b]] for r, b in enumerate(seq)]
+    tokens = rng.integers(0, V, R)
+    for r in range(R):
+        if kids[r]:
+            pool = q[r] / q[r].sum()
+            some = rng.choice(V, len(kids[r]), replace=not distinct or np.count_nonzero(pool) < len(kids[r]), p=pool)
+            tokens[kids[r]] = some
+    if R > 20:
+        tokens[R - 1] = V + 3           # no token of the vocabulary
+    # every second node's distribution at another place, some nodes' children not by chance
+    rank = np.array([r if rng.random() < 0.9 else rng.choice([-1, R + 5]) for r in range(R)], dtype=np.int32)
+    order = rng.permutation(R)
+    where = np.empty(R, dtype=np.int32)
+    where[order] = np.arange(R)
+    rows = np.where((rank >= 0) & (rank < R), where[np.clip(rank, 0, R - 1)], rank).astype(np.int32)
+    numbers = rng.random((R, 2)).astype(np.float32)
+    tree = DraftTree(parents, [tokens[first[b]:first[b + 1]].tolist() for b in range(len(sizes))], "cuda")
+    wide = torch.full((R, V + pad), float("nan"), dtype=qd.dtype).cuda()
+    wide[:, :V] = qd[torch.from_numpy(order)].cuda()
+    kw = {k: (v[:len(sizes)].contiguous() if isinstance(v, torch.Tensor) else v) for k, v in c.kw.items()}
+    ids, logs = sampling.verify_drafts(c.dev, tree, torch.from_numpy(numbers).cuda(), wide[:, :V], draft_rows=torch.from_numpy(rows).cuda(), distinct=distinct,
+                                       logprobs=True, **kw)
+    again = sampling.verify_drafts(c.dev, tree, torch.from_numpy(numbers).cuda(), wide[:, :V], draft_rows=torch.from_numpy(rows).cuda(), distinct=distinct, **kw)
+    assert torch.equal(ids, again)
+    plain = sampling.draw_tokens(c.dev, torch.from_numpy(numbers[:, 1].copy()).cuda(), tree=tree, **kw).cpu().numpy()
+    ids, logs, unclear = ids.cpu().numpy(), logs.cpu().numpy(), 0
+    for r in range(R):
+        w = c.weights(r, seq[r])
+        chance = 0 <= rank[r] < R
+        token, rest, clear = verified(w, kids[r] if chance else [], tokens, q[r], numbers[:, 0], numbers[:, 1], distinct)
+        if not clear:
+            unclear += 1
+            continue
+        if token is not None:
+            assert ids[r] == token
+        else:               # what is left may be small: its sums are off by the bound of what it was
+            cum, at = np.cumsum(rest), ids[r]
+            target, eps = numbers[r, 1] * cum[-1], 1e-9 * cum[-1]
+            assert rest[at] > -eps and cum[at] - rest[at] - eps <= target < cum[at] + eps
+        if not chance or not kids[r]:
+            assert ids[r] == plain[r]
+        lp = math.log(w[ids[r]] / w.sum())
+        assert abs(logs[r] - lp) <= abs(lp) * 2.0 ** -24 + 3e-12
+    assert unclear <= R // 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("distinct,most", [(False, 1), (False, 3), (True, 3)])
+def test_ids_are_distributed_as_the_model(distinct, most):
+    """40000 sequences with one root, whose children are drawn from q: the roots' ids follow p.  A share of 40000 draws is off by more than six of its
+    deviations once in 5e8."""
+    from llm_decoder import DraftTree, sampling
+    n, V = 40000, 9
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal(V).astype(np.float32) * 1.5
+    q = rng.dirichlet(np.ones(V)).astype(np.float32)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    logits = torch.from_numpy(np.log(q)).cuda().expand(n, V).contiguous()
+    kids = sampling.draw_tokens(logits, torch.rand(n, most, device="cuda", generator=g)) if distinct else \
+        torch.stack([sampling.draw_tokens(logits, torch.rand(n, device="cuda", generator=g)) for _ in range(most)], 1)
+    kids = kids.cpu().numpy()
+    if distinct:
+        assert all(len(set(k)) == most for k in kids.tolist())
+    tree = DraftTree([[-1] + [0] * most] * n, [[0, *k] for k in kids.tolist()], "cuda")
+    target = torch.from_numpy(x).cuda().expand(tree.rows, V).contiguous()
+    rows = torch.full((tree.rows,), -1, dtype=torch.int32, device="cuda")
+    rows[::most + 1] = 0
+    ids = sampling.verify_drafts(target, tree, torch.rand(tree.rows, 2, device="cuda", generator=g), torch.from_numpy(q).cuda()[None], draft_rows=rows,
+                                 distinct=distinct, top_k=7)[::most + 1]
+    w = kept_weights(x, top_k=7)
+    p = w / w.sum()
+    share = np.bincount(ids.cpu().numpy(), minlength=V) / n
+    assert np.all(np.abs(share - p) <= 6 * np.sqrt(p * (1 - p) / n)) and np.all(share[p == 0] == 0)
+
+
+# ---------------------------------------------------------------------------------------------------------------- refusals
+def test_refused_on_the_host():
+    from llm_decoder import _cabi, sampling
+    x = torch.zeros(3, 10)
+    for call in (lambda: sampling.truncated_softmax(x), lambda: sampling.draw_tokens(x, torch.zeros(3))):
+        with pytest.raises(ValueError):
+            call()
+    lib, ref = _cabi.lib(), __import__("ctypes").byref
+    rules = _cabi.DrawRules(num_seqs=4, temperature=1.0, top_p=1.0)
+    assert lib.pa_truncated_softmax(None, 0, 8, 4, 8, ref(rules), 0x1000, 8, None) == -1
+    assert lib.pa_truncated_softmax(0x1000, 0, 7, 4, 8, ref(rules), 0x9000, 8, None) == -1
+    assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, ref(rules), 0x9000, 7, None) == -1
+    assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, ref(rules), 0x1040, 8, None) == -1          # overlaps
+    assert lib.pa_truncated_softmax(0x1002, 0, 8, 4, 8, ref(rules), 0x9000, 8, None) == -1          # no address of a float
+    assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, None, 0x9000, 8, None) == -1
+    assert lib.pa_truncated_softmax(0x1000, 0, 8, 0, 8, ref(rules), None, 8, None) == 0
+    assert lib.pa_truncated_softmax(0x1000, 3, 8, 4, 8, ref(rules), 0x9000, 8, None) == -2
+    assert lib.pa_draw_tokens(0x1000, 0, 8, 4, 8, ref(rules), None, 1, 0x9000, None, None) == -1
+    assert lib.pa_draw_tokens(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, 0, 0x9000, None, None) == -1
+    assert lib.pa_draw_tokens(0x1000, 0, 8, 4, 0, ref(rules), 0x8000, 1, 0x9000, None, None) == -1
+    tree = (0x2000, 0x3000, 0x4000)
+    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 0x5000, 0, 8, 4, None, 0, 0x9000, None, None) == -1      # no row_seq
+    rules.row_seq = 0x6000
+    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 0x5000, 0, 8, 3, None, 0, 0x9000, None, None) == -1      # rows without one
+    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 0x5000, 0, 7, 4, None, 0, 0x9000, None, None) == -1
+    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 0x5000, 3, 8, 4, None, 0, 0x9000, None, None) == -2
+
+
+@pytest.mark.gpu
+def test_refused_tensors():
+    from llm_decoder import DraftTree, sampling
+    x, u = torch.zeros(3, 10, device="cuda"), torch.zeros(3, device="cuda")
+    f, i = torch.float32, torch.int32
+    of = lambda n, t: torch.ones(n, dtype=t, device="cuda")  # noqa: E731
+    tree = DraftTree([[-1, 0], [-1]], [[1, 2], [3]], "cuda")
+    bad = [dict(temperature=-1.0), dict(top_k=-1), dict(top_p=float("nan")), dict(min_p=1.5), dict(temperature=of(2, f)), dict(top_k=of(3, f)),
+           dict(top_p=of(3, f).cpu()), dict(row_seq=of(2, i)), dict(row_seq=of(3, f)), dict(tree=DraftTree([[-1]], device="cuda")), dict(tree=tree, row_seq=of(3, i)),
+           dict(temperature=of(2, f), top_p=of(3, f), row_seq=of(3, i))]
+    for kw in bad:
+        for call in (sampling.truncated_softmax, lambda x, **kw: sampling.draw_tokens(x, u, **kw)):
+            with pytest.raises(ValueError):
+                call(x, **kw)
+    for logits in (x.double(), x[0], x.t(), torch.zeros(2, 3, 4, device="cuda"), torch.zeros(1, 400000, device="cuda"), torch.zeros(1, 10, device="cuda").expand(3, 10)):
+        with pytest.raises(ValueError):
+            sampling.truncated_softmax(logits)
+    for numbers in (u.double(), u[:2], u.cpu(), torch.zeros(3, 2, 2, device="cuda"), torch.zeros(3, 4, device="cuda")[:, :2]):
+        with pytest.raises(ValueError):
+            sampling.draw_tokens(x, numbers)
+    for out in (x.half(), x[:2], torch.zeros(10, 3, device="cuda").t()):
+        with pytest.raises(ValueError):
+            sampling.truncated_softmax(x, out=out)
+    with pytest.raises(Exception):
+        sampling.truncated_softmax(x, out=x)
+    pair, q = torch.zeros(3, 2, device="cuda"), torch.full((3, 10), 0.1, device="cuda")
+    assert sampling.verify_drafts(x, tree, pair, q).shape == (3,)
+    for args in ((x, DraftTree([[-1, 0], [-1]], device="cuda"), pair, q), (x, tree, u, q), (x, tree, pair, q[:2]), (x, tree, pair, q[:, :9]), (x, tree, pair, q.double()),
+                 (x, tree, pair, q.cpu()), (x[:2], tree, pair, q)):
+        with pytest.raises(ValueError):
+            sampling.verify_drafts(*args)
+    for rows in (of(2, i), of(3, f), of(3, i).cpu()):
+        with pytest.raises(ValueError):
+            sampling.verify_drafts(x, tree, pair, q, draft_rows=rows)
+    empty = torch.zeros(0, 10, device="cuda")
+    assert sampling.truncated_softmax(empty).shape == (0, 10) and sampling.draw_tokens(empty, torch.zeros(0, device="cuda")).shape == (0,)
+    assert sampling.draw_tokens(x, torch.zeros(3, 0, device="cuda")).shape == (3, 0)
