@@ -1131,9 +1131,9 @@ typedef struct {
     const int32_t* d_top_k;
     const float* d_top_p;
     const float* d_min_p;
-    float temperature;
+    double temperature;
     int top_k;
-    float top_p, min_p;
+    double top_p, min_p;
 } pa_draw_rules;
 int pa_truncated_softmax(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, float* d_probs,
                          int64_t probs_stride, pa_stream_t stream);

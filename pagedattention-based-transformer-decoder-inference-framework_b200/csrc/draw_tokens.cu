@@ -43,7 +43,7 @@ struct Args {
     const int32_t* row_seq;
     const float *temperature, *top_p, *min_p;               // per sequence; null: the value beside it
     const int32_t* top_k;
-    float temperature1, top_p1, min_p1;
+    double temperature1, top_p1, min_p1;
     int top_k1;
     float* probs;                                           // [rows][vocab], rows probs_stride apart
     int64_t probs_stride;
@@ -428,13 +428,13 @@ struct Piece {
     __device__ void rules() {
         const int b = a.row_seq ? a.row_seq[row] : row;
         const bool known = (unsigned)b < (unsigned)a.num_seqs;
-        const float t = !known ? 1.f : a.temperature ? a.temperature[b] : a.temperature1, m = !known ? 0.f : a.min_p ? a.min_p[b] : a.min_p1;
-        const float p = !known ? 1.f : a.top_p ? a.top_p[b] : a.top_p1;
+        const double t = !known ? 1.0 : a.temperature ? (double)a.temperature[b] : a.temperature1;
+        const double p = !known ? 1.0 : a.top_p ? (double)a.top_p[b] : a.top_p1, m = !known ? 0.0 : a.min_p ? (double)a.min_p[b] : a.min_p1;
         const int k = !known ? 0 : a.top_k ? a.top_k[b] : a.top_k1;
         only = -1;
         border = -INFINITY;
-        min_p = m > 0.f ? fminf(m, 1.f) : 0.f;
-        if (!(t > 0.f)) {
+        min_p = m > 0.0 ? fmin(m, 1.0) : 0.0;
+        if (!(t > 0.0)) {
             int v = INT_MAX;
             words([&](float x, int j) { if (x == top && lo + j < v && x > -INFINITY) v = lo + j; });
             v = over_block(v, sh.ipart, Min());
@@ -444,9 +444,9 @@ struct Piece {
             scale = 0.0;
             return;
         }
-        scale = 1.4426950408889634074 / (double)t;
+        scale = 1.4426950408889634074 / t;
         if (k > 0 && k < a.vocab) border = find<false>((double)k, -INFINITY);
-        if (p < 1.f) border = find<true>((double)fmaxf(p, 0.f), border);
+        if (p < 1.0) border = find<true>(fmax(p, 0.0), border);
     }
 
     // ---- sums of f(x, slot) over the parts of the piece; the whole row's

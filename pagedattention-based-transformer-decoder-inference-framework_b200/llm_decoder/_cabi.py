@@ -25,7 +25,7 @@ _vp, _i32, _i64, _f32, _f64, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.
 class DrawRules(C.Structure):
     """pa_draw_rules."""
     _fields_ = [("row_seq", _vp), ("num_seqs", _i32), ("temperatures", _vp), ("top_ks", _vp), ("top_ps", _vp), ("min_ps", _vp),
-                ("temperature", _f32), ("top_k", _i32), ("top_p", _f32), ("min_p", _f32)]
+                ("temperature", _f64), ("top_k", _i32), ("top_p", _f64), ("min_p", _f64)]
 
 
 _DECODE_COMMON = [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp]

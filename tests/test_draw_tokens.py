@@ -80,7 +80,7 @@ class Case:
             self.kw = {k: torch.from_numpy(v).cuda() for k, v in self.rules.items()}
         else:
             self.kw = rules
-            self.rules = {k: np.full(rows, v, dtype=np.int32 if k == "top_k" else np.float32) for k, v in rules.items()}
+            self.rules = {k: np.full(rows, v, dtype=np.int32 if k == "top_k" else np.float64) for k, v in rules.items()}
         self.numbers = rng.random((rows, 8)).astype(np.float32)
 
     def weights(self, r, seq=None):
