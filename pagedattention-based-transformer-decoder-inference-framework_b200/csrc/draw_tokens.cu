@@ -31,8 +31,10 @@
 namespace pa {
 namespace drawn {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 2048, kPer = kBins / kThreads, kList = 1024, kMostRanks = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 2048, kPer = kBins / kThreads, kList = 256, kFew = 256, kMostRanks = 8, kMostStrips = 64;
+static_assert(kFew <= kThreads && kPer % 4 == 0, "a thread for each of few, whole words of steps");
 constexpr uint32_t kAll = 0xffffffffu;
+constexpr float kLowest = -3.402823466e38f;
 enum Mode { PROBS, DRAW, VERIFY };
 
 struct Args {
@@ -40,6 +42,8 @@ struct Args {
     int64_t stride;
     int rows, vocab, ranks, num_seqs;
     size_t data_bytes;                                      // shared memory of a CTA's piece of the row
+    int count_shift;                                        // a step's word: tokens above it, their parts of a step below
+    float parts;                                            // of a step (0: none are kept)
     const int32_t* row_seq;
     const float *temperature, *top_p, *min_p;               // per sequence; null: the value beside it
     const int32_t* top_k;
@@ -59,18 +63,13 @@ struct Args {
 
 template <typename T> __device__ __forceinline__ float widen(T v) { return to_f32<T>(v); }
 template <> __device__ __forceinline__ float widen<__half>(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T narrow(float v) { return from_f32<T>(v); }
+template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
+// the largest number of a type, and how many low bits of it as a float say nothing
 template <typename T> struct Limit;
-template <> struct Limit<float> { static constexpr float most = 3.402823466e38f; };
-template <> struct Limit<__half> { static constexpr float most = 65504.f; };
-template <> struct Limit<bf16_t> { static constexpr float most = 3.38953139e38f; };
-
-// NaN as -inf, +inf as the largest value, -0 as 0
-template <typename T> __device__ __forceinline__ float clean(T v) {
-    return fminf(fmaxf(widen<T>(v), -INFINITY), Limit<T>::most) + 0.f;
-}
-
-template <typename T> __device__ __forceinline__ T nothing() { return from_f32<T>(-INFINITY); }
-template <> __device__ __forceinline__ __half nothing<__half>() { return __ushort_as_half(0xfc00); }
+template <> struct Limit<float> { static constexpr float most = 3.402823466e38f; static constexpr int spare = 0; };
+template <> struct Limit<__half> { static constexpr float most = 65504.f; static constexpr int spare = 13; };
+template <> struct Limit<bf16_t> { static constexpr float most = 3.38953139e38f; static constexpr int spare = 16; };
 
 template <typename T> struct __align__(16) Word {
     static constexpr int N = 16 / (int)sizeof(T);
@@ -78,32 +77,37 @@ template <typename T> struct __align__(16) Word {
 };
 
 // the same place in the shared memory of another CTA of the cluster
-template <typename T> __device__ __forceinline__ const T* peer(const T* p, int rank) {
+template <typename T> __device__ __forceinline__ T* peer(T* p, int rank) {
     uint64_t r;
     asm("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
-    return reinterpret_cast<const T*>(r);
+    return reinterpret_cast<T*>(r);
 }
 
-// ordered as the numbers (no NaN, no -0)
+// ordered as the numbers (no NaN; -0 as 0)
 __device__ __forceinline__ uint32_t key_of(float x) {
-    const uint32_t u = __float_as_uint(x);
+    const uint32_t u = __float_as_uint(x + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-struct Add { template <typename V> __device__ V operator()(V a, V b) const { return a + b; } };
-struct Max { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct Add {
+    template <typename V> __device__ V operator()(V a, V b) const { return a + b; }
+    template <typename V> __device__ static V none() { return 0; }
+};
+struct Max {
+    __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+    template <typename V> __device__ static V none() { return -INFINITY; }
+};
 struct Min {
     __device__ float operator()(float a, float b) const { return fminf(a, b); }
     __device__ int operator()(int a, int b) const { return min(a, b); }
+    template <typename V> __device__ static V none() { return std::is_same<V, int>::value ? (V)INT_MAX : (V)INFINITY; }
 };
 
-// 2^y for y <= 0, by all lanes of a warp, lane j of which holds 2^(j/32) in `table`.  Below 2^-1022: 0.
+// 2^y by all lanes of a warp, lane j of which holds 2^(j/32) in `table`: for y of -1022 to 0; others give some number
 __device__ __forceinline__ double exp2_64(double y, double table) {
     constexpr double magic = 211106232532992.0;             // 1.5 x 2^47: sums end at multiples of 1/32
     constexpr double c1 = 0.69314718055994530942, c2 = 0.24022650695910071233, c3 = 0.05550410866482157995, c4 = 0.00961812910762847716;    // ln 2 ^ k / k!
-    const bool some = y > -1022.0;
-    y = some ? y : 0.0;
     const double at = y + magic;
     const int n = __double2loint(at);
     const double r = y - (at - magic);
@@ -112,24 +116,37 @@ __device__ __forceinline__ double exp2_64(double y, double table) {
     p = fma(r, p, c1);
     p = fma(r, p, 1.0);
     p *= __shfl_sync(kAll, table, n & 31);
-    p = __hiloint2double(__double2hiint(p) + (n >> 5 << 20), __double2loint(p));
-    return some ? p : 0.0;
+    return __hiloint2double(__double2hiint(p) + (n >> 5 << 20), __double2loint(p));
 }
 
+struct Near { float x; int slot; };
+struct Verdict {                    // of the cluster's first CTA
+    float up, lo;                   // what is at or above `up` is summed, what is at or above `lo` listed
+    float r_lo, r_hi, border;
+    double above, limit;
+    int above_n, done, halve, ruled;
+};
+
 struct Shared {                     // beside the piece of the row
-    uint4 hist[kBins / 4];
-    float list[kList];
+    union {
+        uint4 hist[kBins / 4];
+        double few_w[kFew];
+        int32_t child[PA_TREE_MOST_NODES];
+    };
+    Near list[kList];
+    float few[kFew];
     double seg[kWarps];             // weights of the warps' parts of the piece, in the row's order
+    double strip[kMostStrips];      // of one part's strips
     double part[kWarps], part2[kWarps];
     float fpart[kWarps];
     int ipart[kWarps];
-    int b_lo, b_hi, b_first, above, listed, children;
+    int b_lo, b_hi, b_first, to_n, listed, children, hit;
     // what the other CTAs of the cluster read
+    Verdict verdict;
     float x_top, x_lo, x_hi, x_up;
     int x_first, x_listed;
     double x_all, x_above, x_total[2];
 };
-static_assert(kList >= PA_TREE_MOST_NODES, "a node's children take the place of the list");
 
 template <typename T, typename Q, int MODE>
 struct Piece {
@@ -140,8 +157,8 @@ struct Piece {
     const int tid, warp, lane, rank, row;
     int lo, used, strips, s0, s1;   // slots that are used, strips of 32 words; this warp's are s0 .. s1 - 1
     float top, border;              // the largest; the least value that is kept
-    double scale, table, min_p;
-    int only;                       // the one token that is kept, or -1
+    double scale, base, table;      // w = 2^(x scale + base)
+    int only;                       // temperature 0: the one token that is kept, else -1
     int turn = 0;                   // of x_total
 
     __device__ Piece(const Args& args, Shared& shared, T* piece) :
@@ -154,43 +171,76 @@ struct Piece {
         if (lane == 0) parts[warp] = v;
         __syncthreads();
         v = parts[0];
+#pragma unroll
         for (int w = 1; w < kWarps; ++w) v = op(v, parts[w]);
         __syncthreads();
         return v;
     }
-    template <typename V, typename Op> __device__ V over_cluster(const V* place, Op op) {     // between two cluster_sync
-        V v = *peer(place, 0);
-        for (int c = 1; c < a.ranks; ++c) v = op(v, *peer(place, c));
-        return v;
+    // what the CTAs of the cluster have in a place: all on their way at once (between two cluster_sync)
+    template <typename V> __device__ __forceinline__ void of_all(V* place, V (&v)[kMostRanks], V none) {
+#pragma unroll
+        for (int c = 0; c < kMostRanks; ++c) v[c] = *peer(place, min(c, a.ranks - 1));
+#pragma unroll
+        for (int c = 1; c < kMostRanks; ++c)
+            if (c >= a.ranks) v[c] = none;
+    }
+    template <typename V, typename Op> __device__ __forceinline__ V over_cluster(V* place, Op op) {
+        V v[kMostRanks];
+        of_all(place, v, Op::template none<V>());
+#pragma unroll
+        for (int c = 1; c < kMostRanks; ++c) v[0] = op(v[0], v[c]);
+        return v[0];
     }
     __device__ __forceinline__ double warp_sum64(double v) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
         return v;
     }
-    __device__ __forceinline__ float at(int slot) const { return sizeof(T) == 4 ? widen<T>(data[slot]) : clean<T>(data[slot]); }
+    __device__ __forceinline__ float at(int slot) const { return widen<T>(data[slot]); }
 
     // ---- weights, by all lanes of a warp
-    __device__ __forceinline__ double weight(float x) const { return exp2_64(((double)x - (double)top) * scale, table); }
-    __device__ __forceinline__ double kept(float x, int v) const {
-        if (only >= 0) return v == only && x > -INFINITY ? 1.0 : 0.0;
-        const bool in = x >= border && x > -INFINITY;
+    __device__ __forceinline__ double weight(float x) const { return exp2_64(fma((double)x, scale, base), table); }
+    __device__ __forceinline__ double kept(float x) const {
+        const bool in = x >= border;
         if (!__any_sync(kAll, in)) return 0.0;
         const double w = weight(x);
-        return in && w >= min_p ? w : 0.0;
+        return in ? w : 0.0;
     }
 
-    // f(x, slot) for the warp's tokens: all lanes together, word by word or (row order of lanes) token by token
+    // f(x, slot) for the warp's tokens, all lanes together
     template <typename F> __device__ __forceinline__ void words(F f) const {
         for (int s = s0; s < s1; ++s) {
             const int j = s * STRIP + lane * N;
             const Word<T> w = *reinterpret_cast<const Word<T>*>(data + j);
 #pragma unroll
-            for (int e = 0; e < N; ++e) f(sizeof(T) == 4 ? widen<T>(w.v[e]) : clean<T>(w.v[e]), j + e);
+            for (int e = 0; e < N; ++e) f(widen<T>(w.v[e]), j + e);
         }
     }
+    // the weights of what is at or above `least` in a strip, or of lanes on neighbouring tokens (n of them)
+    __device__ __forceinline__ double strip_sum(int s, float least) const {
+        const Word<T> w = *reinterpret_cast<const Word<T>*>(data + s * STRIP + lane * N);
+        float x[N], m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            x[e] = widen<T>(w.v[e]);
+            m = fmaxf(m, x[e]);
+        }
+        if (!__any_sync(kAll, m >= least)) return 0.0;
+        double sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const double v = weight(x[e]);
+            sum += x[e] >= least ? v : 0.0;
+        }
+        return sum;
+    }
+    __device__ double kept_sum() {
+        double sum = 0.0;
+        for (int s = s0; s < s1; ++s) sum += strip_sum(s, border);
+        return join(sum);
+    }
 
-    // ---- the piece into shared memory, and the row's largest
+    // ---- the piece into shared memory, and the row's largest (NaN is never the larger, and never at or above anything)
     __device__ void load() {
         const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.stride;
         const int V = a.vocab, first = min(V, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));     // tokens before the first whole word
@@ -202,27 +252,28 @@ struct Piece {
         s0 = strips * warp / kWarps;
         s1 = strips * (warp + 1) / kWarps;
         float m = -INFINITY;
-        const Word<T>* src = reinterpret_cast<const Word<T>*>(x + first) + w0;
-        Word<T>* dst = reinterpret_cast<Word<T>*>(data) + head;
-#pragma unroll 4
-        for (int i = tid; i < w1 - w0; i += kThreads) {
-            const uint4 raw = ldg_stream_128(src + i);
-            Word<T> w = *reinterpret_cast<const Word<T>*>(&raw);
+        const uint4* src = reinterpret_cast<const uint4*>(x + first) + w0;
+        uint4* dst = reinterpret_cast<uint4*>(data) + head;
+        constexpr int D = 8;                    // words on their way per thread
+        for (int i = tid; i < w1 - w0; i += D * kThreads) {
+            uint4 raw[D];
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const float f = clean<T>(w.v[e]);
-                m = fmaxf(m, f);
-                if constexpr (sizeof(T) == 4) w.v[e] = f;
-            }
-            dst[i] = w;
+            for (int d = 0; d < D; ++d)
+                if (i + d * kThreads < w1 - w0) raw[d] = ldg_stream_128(src + i + d * kThreads);
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+                if (i + d * kThreads < w1 - w0) {
+                    dst[i + d * kThreads] = raw[d];
+                    const Word<T> w = *reinterpret_cast<const Word<T>*>(&raw[d]);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) m = fmaxf(m, widen<T>(w.v[e]));
+                }
         }
         auto edge = [&](int j) {                // token by token; what is not of the piece is -inf
             const int v = lo + j;
-            const bool mine = v >= 0 && v < V && j < used;
-            const float f = mine ? clean<T>(x[v]) : -INFINITY;
-            m = fmaxf(m, f);
-            if constexpr (sizeof(T) == 4) data[j] = f;
-            else data[j] = mine ? x[v] : nothing<T>();
+            const T t = v >= 0 && v < V && j < used ? x[v] : narrow<T>(-INFINITY);
+            data[j] = t;
+            m = fmaxf(m, widen<T>(t));
         };
         if (head && tid < N) edge(tid);
         for (int j = used - tail * N + tid; j < strips * STRIP; j += kThreads) edge(j);
@@ -230,234 +281,452 @@ struct Piece {
         if (tid == 0) sh.x_top = m;
         cluster_sync();
         top = over_cluster(&sh.x_top, Max());
+        if (top == INFINITY) {                  // as the type's largest
+            for (int j = tid; j < strips * STRIP; j += kThreads)
+                if (at(j) == INFINITY) data[j] = narrow<T>(Limit<T>::most);
+            top = Limit<T>::most;
+            __syncthreads();
+        }
     }
 
-    // ---- the least value that is kept of those from `least` on: with MASS the weights above it are below `share` of all, else fewer than
-    // `share` tokens are above it.  R = [lo_x, hi_x] holds it; the first value in R is kept in any case.
-    template <bool MASS> __device__ float find(double share, float least) {
-        float lo_x = least, hi_x = top;
-        double above_w = 0.0, limit = share;
-        int above_n = 0;
-        bool listed = false, halve = false;
-        const float step = (float)(scale * 64.0);
-        for (int level = 0; level < 128; ++level) {
-            const uint32_t k_hi = key_of(hi_x), range = level ? k_hi - key_of(lo_x) : 0u;
-            const int bits = 32 - __clz(range), shift = bits > 11 ? bits - 11 : 0;
-            auto bin = [&](float x) {
-                return level ? (int)((k_hi - key_of(x)) >> shift) : max(0, min(kBins - 1, (int)((top - x) * step)));
-            };
-            auto each = [&](auto f) {               // f(x) for all, or those that were listed
-                if (!listed) words([&](float x, int) { f(x); });
-                else for (int i = 0; i < sh.listed; i += kThreads) f(i + tid < sh.listed ? sh.list[i + tid] : -INFINITY);
-            };
-            auto in = [&](float x) { return x >= lo_x && x <= hi_x && x > -INFINITY; };
-            int from = 0, to = 0;                   // R's steps that may hold the border
-            if (halve) {                            // the bounds did not help: by halves, whose weights are summed exactly
-                from = to = 1;
-                cluster_sync();                     // the last sums have been read
-            } else {
-                for (int i = tid; i < kBins / 4; i += kThreads) sh.hist[i] = make_uint4(0, 0, 0, 0);
-                if (tid == 0) {
-                    sh.b_lo = sh.b_hi = -1;
-                    sh.b_first = kBins;
+    // ---- where the border is, as far as the counts tell (by the first CTA): the steps of R that may hold it
+    // bounds(b, n, parts, least, most): the weights that the n tokens of step b have at least and at most
+    template <bool MASS, typename B> __device__ void weigh(double share, bool first, const Verdict& r, int& from, int& to, B bounds) {
+        uint32_t n[kPer], parts[kPer];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) n[e] = parts[e] = 0;
+#pragma unroll
+        for (int e = 0; e < kPer; e += 4) {
+            uint4 h[kMostRanks];
+            of_all(sh.hist + tid * (kPer / 4) + e / 4, h, make_uint4(0, 0, 0, 0));
+#pragma unroll
+            for (int c = 0; c < kMostRanks; ++c) {
+                const uint32_t w[4] = {h[c].x, h[c].y, h[c].z, h[c].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    n[e + k] += w[k] >> a.count_shift;
+                    parts[e + k] += w[k] & ((1u << a.count_shift) - 1u);
                 }
+            }
+        }
+        const double limit = MASS && first ? share * over_cluster(&sh.x_all, Add()) : r.limit;
+        if (tid == 0) {
+            sh.b_lo = sh.b_hi = -1;
+            sh.b_first = kBins;
+        }
+        double least_w[kPer], most_w[kPer], least = 0.0, most = 0.0;
+        int count = 0;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            count += n[e];
+            if (!MASS) continue;
+            bounds(tid * kPer + e, n[e], parts[e], least_w[e], most_w[e]);
+            least += least_w[e];
+            most += most_w[e];
+        }
+        int count_to = count;
+        double least_to = least, most_to = most;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int p = __shfl_up_sync(kAll, count_to, o);
+            const double q = MASS ? __shfl_up_sync(kAll, least_to, o) : 0.0, s = MASS ? __shfl_up_sync(kAll, most_to, o) : 0.0;
+            if (lane >= o) {
+                count_to += p;
+                least_to += q;
+                most_to += s;
+            }
+        }
+        if (lane == 31) {
+            sh.ipart[warp] = count_to;
+            sh.part[warp] = least_to;
+            sh.part2[warp] = most_to;
+        }
+        __syncthreads();
+        count_to -= count;
+        least_to -= least;
+        most_to -= most;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+            if (w < warp) {
+                count_to += sh.ipart[w];
+                least_to += sh.part[w];
+                most_to += sh.part2[w];
+            }
+        const int before = count_to;
+        int b_first = kBins, b_lo = -1, b_hi = -1;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            const int b = tid * kPer + e;
+            if (n[e]) {
+                b_first = min(b_first, b);
+                if (MASS ? r.above + most_to < limit : r.above_n + count_to < limit) b_lo = b;
+                if (MASS ? r.above + least_to < limit : r.above_n + count_to < limit) b_hi = b;
+            }
+            count_to += n[e];
+            if (MASS) {
+                least_to += least_w[e];
+                most_to += most_w[e];
+            }
+        }
+        if (b_first < kBins) atomicMin(&sh.b_first, b_first);
+        if (b_lo >= 0) atomicMax(&sh.b_lo, b_lo);
+        if (b_hi >= 0) atomicMax(&sh.b_hi, b_hi);
+        __syncthreads();
+        from = max(sh.b_lo, sh.b_first);
+        to = max(sh.b_hi, from);
+        int m = before;
+        if (from / kPer == tid) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                if (tid * kPer + e < from) m += n[e];
+            sh.verdict.above_n = r.above_n + m;
+            sh.verdict.limit = limit;
+        }
+        if (!MASS && to / kPer == tid) {            // tokens up to the last of them
+            m = before;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                if (tid * kPer + e <= to) m += n[e];
+            sh.to_n = r.above_n + m;
+        }
+        __syncthreads();
+    }
+
+    // the least float whose step is below b (the steps fall while the floats grow), by a warp: 31 of them are tried at a time
+    template <typename F> __device__ float edge_of(int b, F place) const {
+        if (b <= 0) return INFINITY;
+        uint64_t l = key_of(kLowest), h = key_of(top);          // place(h) = 0 < b; the answer is in [l, h]
+        while (l < h) {
+            const uint64_t d = (h - l + 31) / 32, k = min(l + d * lane, h);
+            const uint32_t yes = __ballot_sync(kAll, place(of_key((uint32_t)k)) < b);
+            const int i = __ffs(yes) - 1;                        // the first that is
+            if (i == 0) return of_key((uint32_t)l);
+            const uint64_t was = l;
+            if (i > 0) {
+                l = min(was + d * (i - 1) + 1, h);
+                h = min(was + d * i, h);
+            } else {
+                l = min(was + d * 31 + 1, h);
+            }
+        }
+        return of_key((uint32_t)h);
+    }
+
+    // the few tokens that the CTAs have listed, in this one (the first)
+    __device__ void gather(int n) {
+        int m[kMostRanks];
+        of_all(&sh.x_listed, m, 0);
+        int c = 0, i = tid;
+#pragma unroll
+        for (int k = 0; k < kMostRanks - 1; ++k)
+            if (c == k && i >= m[k]) {
+                i -= m[k];
+                c = k + 1;
+            }
+        if (tid < n) sh.few[tid] = peer(sh.list + i, c)->x;
+        else if (tid < kFew) sh.few[tid] = -INFINITY;
+        __syncthreads();
+    }
+    // the border among n few tokens, each of which sums (or counts) what is above it: of those at or above `least`
+    template <bool MASS> __device__ float among(int n, float least, double above, int above_n, double limit) {
+        const float x = tid < n ? sh.few[tid] : -INFINITY;
+        double sum[4] = {above, 0.0, 0.0, 0.0};
+        int count = above_n;
+        if (warp * 32 < n)
+            for (int i = 0; i < n; i += 4) {
+                const float4 y = *reinterpret_cast<const float4*>(sh.few + i);
+                const float u[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (MASS) sum[e] += u[e] > x ? sh.few_w[i + e] : 0.0;
+                    else count += u[e] > x;
+                }
+            }
+        const bool in = x >= least && tid < n && (MASS ? sum[0] + sum[1] + (sum[2] + sum[3]) < limit : count < limit);
+        const float low = over_block(in ? x : INFINITY, sh.fpart, Min()), most = over_block(x, sh.fpart, Max());
+        return fminf(low, most);                    // the largest is kept in any case
+    }
+    // their weights; the sum of those at or above `least`
+    __device__ double weights_of_few(int n, float least) {
+        const float x = tid < n ? sh.few[tid] : -INFINITY;
+        double w = weight(x);
+        w = x >= least ? w : 0.0;
+        sh.few_w[tid] = w;
+        return over_block(w, sh.part, Add());
+    }
+
+    // ---- the border: the least value that is kept of those from `least` on.  With MASS the weights above it are below `share` of all, else fewer
+    // than `share` tokens are above it; the largest is kept in any case.  Where few are counted, these are also cut to share p of their weights
+    // (p below 1).  Returns the value from which on sh.seg has summed all (asked for by `sums`, or MASS), the rest of it with what is listed;
+    // infinity: all are listed; NaN: neither.
+    template <bool MASS> __device__ float find(double share, float least, bool sums, double p, bool& ruled) {
+        Verdict r;                              // R = [r_lo, r_hi] holds the border, `above` and above_n are above R
+        r.r_lo = least;
+        r.r_hi = top;
+        r.above = 0.0;
+        r.above_n = 0;
+        r.limit = share;
+        r.halve = 0;
+        const float step = (float)(scale * 64.0), parts = a.parts;
+        // steps of 1/64 in log2 w to begin with, rounded to the nearest; by floats where these would be too coarse or too fine, and afterwards
+        bool first = true, by_logs = scale > 1e-6 && scale < 1e6;
+        for (int level = 0; level < 128; ++level) {
+            const uint32_t k_hi = key_of(r.r_hi) >> Limit<T>::spare, range = k_hi - (key_of(r.r_lo) >> Limit<T>::spare);
+            const int bits = 32 - __clz(range), shift = bits > 11 ? bits - 11 : 0;
+            auto by_log = [&](float x) { return fminf((top - x) * step, kBins - 1.f); };
+            auto place = [&](float x) -> int {
+                if (by_logs) return __float_as_int(by_log(x) + 8388608.f) & (kBins - 1);
+                return (int)((k_hi - (key_of(x) >> Limit<T>::spare)) >> shift) & (kBins - 1);
+            };
+            if (!r.halve) {
+                for (int i = tid; i < kBins / 4; i += kThreads) sh.hist[i] = make_uint4(0, 0, 0, 0);
                 __syncthreads();
                 double all = 0.0;
-                uint32_t* hist = reinterpret_cast<uint32_t*>(sh.hist);
-                each([&](float x) {
-                    const bool here = in(x);
-                    if (here) atomicAdd(hist + bin(x), 1u);
-                    if (MASS && level == 0 && __any_sync(kAll, here)) {
-                        const double w = weight(x);
-                        all += here ? w : 0.0;
+                const uint32_t hist = smem_u32(sh.hist), one = 1u << a.count_shift;
+                for (int s = s0; s < s1; ++s) {
+                    const Word<T> w = *reinterpret_cast<const Word<T>*>(data + s * STRIP + lane * N);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const float x = widen<T>(w.v[e]);
+                        const bool here = x >= r.r_lo && x <= r.r_hi;
+                        uint32_t at = hist, add = one;
+                        if (by_logs) {
+                            const float d = by_log(x), up = d + 8388608.f;
+                            at += (__float_as_uint(up) & (kBins - 1)) * 4;
+                            if (MASS) add += __float_as_uint(fmaf(d - (up - 8388608.f), parts, 8388608.f + 0.5f * parts)) & 0x7fffffu;
+                        } else {
+                            at += place(x) * 4;
+                        }
+                        if (here) asm volatile("red.shared.add.u32 [%0], %1;" ::"r"(at), "r"(add) : "memory");
+                        if (MASS && first) {
+                            const double v = weight(x);
+                            all += here ? v : 0.0;
+                        }
                     }
-                });
-                if (MASS && level == 0) {
+                }
+                if (MASS && first) {
                     all = over_block(all, sh.part, Add());
                     if (tid == 0) sh.x_all = all;
                 }
                 cluster_sync();
-                if (MASS && level == 0) limit = share * over_cluster(&sh.x_all, Add());
-                // four steps a thread: how many tokens, and between what bounds their weights are; then of all steps above
-                uint32_t n[kPer] = {0, 0, 0, 0};
-                for (int c = 0; c < a.ranks; ++c) {
-                    const uint4 h = *peer(sh.hist + tid, c);
-                    n[0] += h.x; n[1] += h.y; n[2] += h.z; n[3] += h.w;
-                }
-                double least_w[kPer], most_w[kPer], least_sum = 0.0, most_sum = 0.0;
-                int count = 0;
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    const int b = tid * kPer + e;
-                    count += n[e];
-                    if (!MASS) continue;
-                    if (level == 0) {               // (rounding of (top - x) * step: 2048 x 2^-22 of a step)
-                        most_w[e] = n[e] * (double)exp2f(-b / 64.f) * (1.0 + 1e-5);
-                        least_w[e] = b == kBins - 1 ? 0.0 : n[e] * (double)exp2f(-(b + 1) / 64.f) * (1.0 - 1e-5);
-                    } else {
+                if (rank == 0) {
+                    int from, to;
+                    // d of a step's tokens: b + what their parts say, within half a part; w = 2^(-d/64) falls by at most a 6e-5th of itself more than
+                    // evenly between the ends of a step, and (top - x) step is rounded by 2048 x 2^-22 of a step
+                    auto by_step = [&](int b, uint32_t n, uint32_t q, double& l, double& m) {
+                        const float mean = parts > 0.f && n ? ((float)q / (float)n - 0.5f * parts) / parts : 0.f, half = parts > 0.f ? 0.5f / parts : 0.5f;
+                        m = n * (double)exp2f((half - mean - b) / 64.f) * (1.0 + 8e-5);
+                        l = b == kBins - 1 ? 0.0 : n * (double)exp2f((-half - mean - b) / 64.f) * (1.0 - 2e-5);
+                    };
+                    auto by_float = [&](int b, uint32_t n, uint32_t, double& l, double& m) {
                         const uint64_t k0 = min((uint64_t)b << shift, (uint64_t)range), k1 = min(((uint64_t)(b + 1) << shift) - 1, (uint64_t)range);
-                        most_w[e] = n[e] * weight(of_key(k_hi - (uint32_t)k0)) * (shift ? 1.0 + 1e-11 : 1.0);
-                        least_w[e] = n[e] * weight(of_key(k_hi - (uint32_t)k1)) * (shift ? 1.0 - 1e-11 : 1.0);
+                        const double w0 = weight(of_spared(k_hi - (uint32_t)k0)), w1 = weight(of_spared(k_hi - (uint32_t)k1));
+                        m = n * w0 * (shift ? 1.0 + 1e-10 : 1.0);
+                        l = n * w1 * (shift ? 1.0 - 1e-10 : 1.0);
+                    };
+                    if (by_logs) weigh<MASS>(share, first, r, from, to, by_step);
+                    else weigh<MASS>(share, first, r, from, to, by_float);
+                    const bool all_few = !MASS && first && sh.to_n <= kFew;         // all that can be kept are few: listed, not summed
+                    if (by_logs) {
+                        if (warp == 0) {
+                            const float e = all_few ? INFINITY : edge_of(from, place);
+                            if (lane == 0) sh.verdict.up = e;
+                        } else if (warp == 1) {
+                            const float e = to == kBins - 1 ? r.r_lo : fmaxf(edge_of(to + 1, place), r.r_lo);
+                            if (lane == 0) sh.verdict.lo = e;
+                        }
+                    } else if (tid == 0) {
+                        const uint64_t k = (uint64_t)(to + 1) << shift;
+                        sh.verdict.up = all_few ? INFINITY : from == 0 ? above_of(r.r_hi) : of_spared(k_hi - (uint32_t)(((uint64_t)from << shift) - 1));
+                        sh.verdict.lo = k > range ? r.r_lo : fmaxf(of_spared(k_hi - (uint32_t)k + 1), r.r_lo);
                     }
-                    most_sum += most_w[e];
-                    least_sum += least_w[e];
+                    if (all_few && tid == 0) sh.verdict.above_n = 0;
                 }
-                int count_to = count;
-                double least_to = least_sum, most_to = most_sum;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int p = __shfl_up_sync(kAll, count_to, o);
-                    const double q = MASS ? __shfl_up_sync(kAll, least_to, o) : 0.0, s = MASS ? __shfl_up_sync(kAll, most_to, o) : 0.0;
-                    if (lane >= o) {
-                        count_to += p;
-                        least_to += q;
-                        most_to += s;
-                    }
-                }
-                if (lane == 31) {
-                    sh.ipart[warp] = count_to;
-                    sh.part[warp] = least_to;
-                    sh.part2[warp] = most_to;
-                }
-                __syncthreads();
-                count_to -= count;
-                least_to -= least_sum;
-                most_to -= most_sum;
-                for (int w = 0; w < warp; ++w) {
-                    count_to += sh.ipart[w];
-                    least_to += sh.part[w];
-                    most_to += sh.part2[w];
-                }
-                const int before = count_to;
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    const int b = tid * kPer + e;
-                    if (n[e]) {
-                        atomicMin(&sh.b_first, b);
-                        if (MASS ? above_w + most_to < limit : above_n + count_to < limit) atomicMax(&sh.b_lo, b);
-                        if (MASS ? above_w + least_to < limit : above_n + count_to < limit) atomicMax(&sh.b_hi, b);
-                    }
-                    count_to += n[e];
-                    if (MASS) {
-                        least_to += least_w[e];
-                        most_to += most_w[e];
-                    }
-                }
-                __syncthreads();
-                from = max(sh.b_lo, sh.b_first);
-                to = max(sh.b_hi, from);
-                if (from / kPer == tid) {
-                    int m = before;
-#pragma unroll
-                    for (int e = 0; e < kPer; ++e)
-                        if (tid * kPer + e < from) m += n[e];
-                    sh.above = m;
-                }
-                __syncthreads();
-                above_n += sh.above;
-                if (level && shift == 0 && from == to) {
-                    lo_x = of_key(k_hi - (uint32_t)from);
-                    break;
+            } else {                                        // the bounds did not help: by halves, whose weights are summed
+                cluster_sync();                             // the last verdict has been read
+                if (rank == 0 && tid == 0) {
+                    sh.verdict.up = of_spared(k_hi - range / 2);
+                    sh.verdict.lo = r.r_lo;
+                    sh.verdict.above_n = r.above_n;
+                    sh.verdict.limit = r.limit;
                 }
             }
-            // what is above those steps, summed; the ends of what is in them, and a list of it
-            const uint32_t half = key_of(lo_x) + range / 2;
-            auto place = [&](float x) { return halve ? (key_of(x) > half ? 0 : 1) : bin(x); };
+            cluster_sync();
+            const float up = peer(&sh.verdict, 0)->up, near = peer(&sh.verdict, 0)->lo;
+            r.limit = peer(&sh.verdict, 0)->limit;
+            const int above_n = peer(&sh.verdict, 0)->above_n;
+            // ---- what is above those steps, summed; what is in them, listed
+            if (tid == 0) sh.listed = 0;
+            __syncthreads();
             double sum = 0.0;
             float least_x = INFINITY, most_x = -INFINITY, least_up = INFINITY;
-            const bool listing = !listed && !halve;
-            if (listing) {
-                if (tid == 0) sh.listed = 0;
-                __syncthreads();
-            }
-            each([&](float x) {
-                const bool here = in(x);
-                const int b = here ? place(x) : kBins;
-                const bool up = b < from, near = b >= from && b <= to;
-                if (MASS && __any_sync(kAll, up)) {
-                    const double w = weight(x);
-                    sum += up ? w : 0.0;
-                    if (up) least_up = fminf(least_up, x);
+            for (int s = s0; s < s1; ++s) {
+                const int j = s * STRIP + lane * N;
+                const Word<T> w = *reinterpret_cast<const Word<T>*>(data + j);
+                float x[N], m = -INFINITY;
+                uint32_t mine = 0;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    x[e] = widen<T>(w.v[e]);
+                    m = fmaxf(m, x[e]);
                 }
-                if (near) {
-                    least_x = fminf(least_x, x);
-                    most_x = fmaxf(most_x, x);
+                if (!__any_sync(kAll, m >= near)) continue;
+#pragma unroll
+                for (int e = 0; e < N; ++e) mine |= (uint32_t)(x[e] >= near && !(x[e] >= up)) << e;
+                if ((MASS || sums) && __any_sync(kAll, m >= up)) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const double v = weight(x[e]);
+                        sum += x[e] >= up ? v : 0.0;
+                        if (r.halve && x[e] >= up && x[e] <= r.r_hi) least_up = fminf(least_up, x[e]);
+                    }
                 }
-                if (listing && __any_sync(kAll, near)) {
-                    const uint32_t who = __ballot_sync(kAll, near);
+                if (__any_sync(kAll, mine != 0)) {
                     int at = 0;
-                    if (lane == 0) at = atomicAdd(&sh.listed, __popc(who));
-                    at = __shfl_sync(kAll, at, 0) + __popc(who & ((1u << lane) - 1u));
-                    if (near && at < kList) sh.list[at] = x;
+                    if (mine) at = atomicAdd(&sh.listed, __popc(mine));
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (mine >> e & 1u) {
+                            least_x = fminf(least_x, x[e]);
+                            most_x = fmaxf(most_x, x[e]);
+                            if (at < kList) sh.list[at] = Near{x[e], j + e};
+                            ++at;
+                        }
                 }
-            });
-            if (MASS) sum = over_block(sum, sh.part, Add());
+            }
+            sum = warp_sum64(sum);
+            if (lane == 0) sh.seg[warp] = sum;
             least_x = over_block(least_x, sh.fpart, Min());
             most_x = over_block(most_x, sh.fpart, Max());
-            if (halve) least_up = over_block(least_up, sh.fpart, Min());
+            if (r.halve) least_up = over_block(least_up, sh.fpart, Min());
             if (tid == 0) {
-                sh.x_above = sum;
+                double t = 0.0;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) t += sh.seg[w];
+                sh.x_above = t;
                 sh.x_lo = least_x;
                 sh.x_hi = most_x;
                 sh.x_up = least_up;
                 sh.x_listed = sh.listed;
             }
             cluster_sync();
-            const double more = MASS ? over_cluster(&sh.x_above, Add()) : 0.0;
-            const float lo_was = lo_x, hi_was = hi_x;
-            if (halve && above_w + more >= limit) {         // the border is in the upper half
-                lo_x = over_cluster(&sh.x_up, Min());
-            } else {
-                above_w += more;
-                lo_x = over_cluster(&sh.x_lo, Min());
-                hi_x = over_cluster(&sh.x_hi, Max());
-                if (listing) {
-                    listed = true;
-                    for (int c = 0; c < a.ranks; ++c) listed = listed && *peer(&sh.x_listed, c) <= kList;
+            // ---- few are left, or all alike: the border; else once more
+            if (rank == 0) {
+                int listed[kMostRanks], n = 0, most = 0;
+                of_all(&sh.x_listed, listed, 0);
+#pragma unroll
+                for (int c = 0; c < kMostRanks; ++c) {
+                    n += listed[c];
+                    most = max(most, listed[c]);
+                }
+                const double above = MASS ? over_cluster(&sh.x_above, Add()) : 0.0;
+                const float l = over_cluster(&sh.x_lo, Min()), h = over_cluster(&sh.x_hi, Max()), u = r.halve ? over_cluster(&sh.x_up, Min()) : 0.f;
+                const bool upper = MASS && r.halve && above >= r.limit;          // the border is in the upper half
+                const bool few = !upper && n <= kFew && most <= kList, rules_too = !MASS && up == INFINITY && few;
+                float found = l;
+                if (few && (l < h || rules_too)) {
+                    gather(n);
+                    if (MASS) weights_of_few(n, -INFINITY);
+                    found = among<MASS>(n, -INFINITY, above, above_n, r.limit);
+                    if (rules_too && p < 1.0) {
+                        const double all = weights_of_few(n, found);
+                        found = among<true>(n, found, 0.0, 0, p * all);
+                    }
+                }
+                if (tid == 0) {
+                    Verdict& v = sh.verdict;
+                    v.border = found;
+                    v.done = !upper && (few || l == h);
+                    v.ruled = rules_too;
+                    v.r_lo = upper ? u : l;
+                    v.r_hi = upper ? r.r_hi : h;
+                    v.above = upper ? r.above : above;
+                    v.above_n = above_n;
+                    v.halve = MASS && !by_logs && !r.halve && !v.done &&
+                              key_of(v.r_hi) - key_of(v.r_lo) > (key_of(r.r_hi) - key_of(r.r_lo)) / 2;
                 }
             }
-            if (lo_x == hi_x) break;
-            // (the first count goes by steps of log2 w, the ones after it by those of floats)
-            halve = MASS && level > 0 && !halve && key_of(hi_x) - key_of(lo_x) > (key_of(hi_was) - key_of(lo_was)) / 2;
+            cluster_sync();
+            const Verdict v = *peer(&sh.verdict, 0);
+            border = v.border;
+            ruled = v.ruled;
+            if (v.done) {
+                if (!(MASS || sums || up == INFINITY)) return NAN;
+                return sh.listed > kList ? NAN : up;
+            }
+            r.r_lo = v.r_lo;
+            r.r_hi = v.r_hi;
+            r.above = v.above;
+            r.above_n = v.above_n;
+            r.halve = v.halve;
+            by_logs = first = false;
         }
-        cluster_sync();                 // nobody reads what comes next in its place
-        return lo_x;
+        return NAN;
     }
+    // the listed tokens that are kept, to the parts that they are in
+    __device__ void add_listed() {
+        double more = 0.0;
+        for (int i = 0; i < sh.listed; i += 32) {
+            const Near one = i + lane < sh.listed ? sh.list[i + lane] : Near{-INFINITY, 0};
+            const bool mine = one.x >= border && one.slot >= s0 * STRIP && one.slot < s1 * STRIP;
+            if (__any_sync(kAll, mine)) {
+                const double w = weight(one.x);
+                more += mine ? w : 0.0;
+            }
+        }
+        more = warp_sum64(more);
+        if (lane == 0) sh.seg[warp] += more;
+    }
+    __device__ __forceinline__ float of_spared(uint32_t k) const {             // the least float of a key without its spare bits
+        const uint32_t full = k << Limit<T>::spare;
+        // (negative numbers have ones in their spare bits as keys)
+        return of_key(full & 0x80000000u ? full : full | ((1u << Limit<T>::spare) - 1u));
+    }
+    __device__ __forceinline__ float above_of(float x) const { return of_key(key_of(x) + 1u); }
 
-    // ---- the rules of the row's sequence
-    __device__ void rules() {
+    // ---- the rules of the row's sequence: the border, and the sums of what is kept.  The total
+    __device__ double rules() {
         const int b = a.row_seq ? a.row_seq[row] : row;
         const bool known = (unsigned)b < (unsigned)a.num_seqs;
         const double t = !known ? 1.0 : a.temperature ? (double)a.temperature[b] : a.temperature1;
         const double p = !known ? 1.0 : a.top_p ? (double)a.top_p[b] : a.top_p1, m = !known ? 0.0 : a.min_p ? (double)a.min_p[b] : a.min_p1;
         const int k = !known ? 0 : a.top_k ? a.top_k[b] : a.top_k1;
         only = -1;
-        border = -INFINITY;
-        min_p = m > 0.0 ? fmin(m, 1.0) : 0.0;
         if (!(t > 0.0)) {
             int v = INT_MAX;
-            words([&](float x, int j) { if (x == top && lo + j < v && x > -INFINITY) v = lo + j; });
+            words([&](float x, int j) { if (x == top) v = min(v, lo + j); });
             v = over_block(v, sh.ipart, Min());
             if (tid == 0) sh.x_first = v;
             cluster_sync();
             only = over_cluster(&sh.x_first, Min());
-            scale = 0.0;
-            return;
+            words([&](float x, int j) { if (x == top && lo + j != only) data[j] = narrow<T>(-INFINITY); });
+            __syncwarp();
+            border = top;
+            scale = base = 0.0;
+            return kept_sum();
         }
         scale = 1.4426950408889634074 / t;
-        if (k > 0 && k < a.vocab) border = find<false>((double)k, -INFINITY);
-        if (p < 1.0) border = find<true>(fmax(p, 0.0), border);
+        base = -(double)top * scale;
+        border = at_least((double)top - 1021.0 / scale);                // what has no weight in 64 bits
+        const float least = !(m > 0.0) ? kLowest : m >= 1.0 ? (t < INFINITY ? top : kLowest) : at_least((double)top + t * log(m));      // w >= m
+        float from = NAN;
+        bool ruled = false;
+        if (k > 0 && k < a.vocab) from = find<false>((double)k, border, !(p < 1.0), p, ruled);
+        if (p < 1.0 && !ruled) from = find<true>(fmax(p, 0.0), border, true, 1.0, ruled);
+        border = fmaxf(border, least);
+        if (!(from >= border)) return kept_sum();       // no sums, or of more than is kept
+        add_listed();
+        return joined();
     }
+    __device__ __forceinline__ float at_least(double x) const { return x >= (double)kLowest ? __double2float_ru(x) : kLowest; }
 
-    // ---- sums of f(x, slot) over the parts of the piece; the whole row's
-    template <typename F> __device__ double sums(F f) {
-        double sum = 0.0;
-        words([&](float x, int j) { sum += f(x, j); });
-        return join(sum);
-    }
+    // ---- the parts' sums, and the whole row's
     __device__ double join(double sum) {
         sum = warp_sum64(sum);
         if (lane == 0) sh.seg[warp] = sum;
+        return joined();
+    }
+    __device__ double joined() {
         __syncthreads();
         publish();
         cluster_sync();
@@ -472,70 +741,112 @@ struct Piece {
         }
     }
 
-    // ---- the first token up to which the sums of f exceed `target`, where it is in this CTA's piece: found by its first warp; -1 elsewhere
+    // ---- the first token up to which the sums of f(slot) exceed `target`, as a slot of the CTA whose piece has it; -1 in the others
     template <typename F> __device__ int search(double target, F f) {
-        double run = 0.0, mine = 0.0;
+        double t[kMostRanks], run = 0.0, mine = 0.0;
+        of_all(&sh.x_total[turn], t, 0.0);
         int owner = -1;
-        for (int c = 0; c < a.ranks; ++c) {
-            const double t = *peer(&sh.x_total[turn], c);
-            if (t > 0.0 && (owner < 0 || run <= target)) {       // the first that exceeds, else the last that has anything
+        bool open = true;
+#pragma unroll
+        for (int c = 0; c < kMostRanks; ++c) {              // the first that exceeds it, else (by rounding) the last that has anything
+            if (open && t[c] > 0.0) {
                 owner = c;
                 mine = run;
-                if (run + t > target) break;
+                open = !(run + t[c] > target);
             }
-            run += t;
+            run += t[c];
         }
-        if (owner != rank || warp != 0) return -1;
+        if (owner != rank) return -1;
         run = mine;
-        int part = -1;
+        int part = 0;
+        open = true;
+#pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            if (sh.seg[w] > 0.0) {
+            if (open && sh.seg[w] > 0.0) {
                 part = w;
                 mine = run;
-                if (run + sh.seg[w] > target) break;
+                open = !(run + sh.seg[w] > target);
             }
             run += sh.seg[w];
         }
-        run = mine;
-        const int e0 = strips * part / kWarps, e1 = strips * (part + 1) / kWarps;
-        int last = -1;
-        for (int s = e0; s < e1; ++s) {
-            const int j = s * STRIP + lane * N;
+        const int e0 = strips * part / kWarps, n = strips * (part + 1) / kWarps - e0;       // at most kMostStrips
+        for (int i = warp; i < n; i += kWarps) {
+            double sum = 0.0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum += f((e0 + i) * STRIP + lane * N + e);
+            sum = warp_sum64(sum);
+            if (lane == 0) sh.strip[i] = sum;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            run = mine;
+            int at = 0;
+            open = true;
+            for (int i = 0; i < n; ++i) {
+                const double w = sh.strip[i];
+                if (open && w > 0.0) {
+                    at = i;
+                    mine = run;
+                    open = !(run + w > target);
+                }
+                run += w;
+            }
+            const int j = (e0 + at) * STRIP + lane * N;
             double w[N], to = 0.0;
 #pragma unroll
-            for (int e = 0; e < N; ++e) to += w[e] = f(at(j + e), j + e);
+            for (int e = 0; e < N; ++e) to += w[e] = f(j + e);
             const double own = to;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const double q = __shfl_up_sync(kAll, to, o);
                 if (lane >= o) to += q;
             }
-            double cum = run + to - own;
-            int hit = -1, some = -1;
+            double cum = mine + to - own;
+            int hit = -1, last = -1;
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 cum += w[e];
-                if (w[e] > 0.0) some = j + e;
-                if (hit < 0 && w[e] > 0.0 && cum > target) hit = j + e;
+                if (w[e] > 0.0) {
+                    last = j + e;
+                    if (hit < 0 && cum > target) hit = j + e;
+                }
             }
             const uint32_t who = __ballot_sync(kAll, hit >= 0);
-            if (who) return __shfl_sync(kAll, hit, __ffs(who) - 1);
-            last = max(last, __reduce_max_sync(kAll, some));
-            run += __shfl_sync(kAll, to, 31);
+            hit = who ? __shfl_sync(kAll, hit, __ffs(who) - 1) : __reduce_max_sync(kAll, last);
+            if (lane == 0) sh.hit = hit;
         }
-        return last;
+        __syncthreads();
+        return sh.hit;
     }
 
     // ---- what the modes do
     __device__ void probs() {
-        const double total = top > -INFINITY ? sums([&](float x, int j) { return kept(x, lo + j); }) : 0.0, share = total > 0.0 ? 1.0 / total : 0.0;
+        const double total = top > -INFINITY ? rules() : 0.0, share = total > 0.0 ? 1.0 / total : 0.0;
+        if (!(total > 0.0)) border = INFINITY;
         float* out = a.probs + (int64_t)row * a.probs_stride + lo;
         for (int s = s0; s < s1; ++s) {
+            const int j = s * STRIP + lane;                 // lanes on neighbouring tokens, as they are written
+            float x[N], m = -INFINITY, y[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const int j = s * STRIP + e * 32 + lane, v = lo + j;        // lanes on neighbouring tokens, as they are written
-                const double w = share > 0.0 ? kept(at(j), v) : 0.0;
-                if (v >= 0 && v < a.vocab && j < used) out[j] = (float)(w * share);
+                x[e] = at(j + e * 32);
+                m = fmaxf(m, x[e]);
+                y[e] = 0.f;
+            }
+            if (__any_sync(kAll, m >= border)) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const double w = weight(x[e]);
+                    y[e] = x[e] >= border ? (float)(w * share) : 0.f;
+                }
+            }
+            if (lo + s * STRIP >= 0 && (s + 1) * STRIP <= used && lo + (s + 1) * STRIP <= a.vocab) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) out[j + e * 32] = y[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (lo + j + e * 32 >= 0 && lo + j + e * 32 < a.vocab && j + e * 32 < used) out[j + e * 32] = y[e];
             }
         }
     }
@@ -545,8 +856,8 @@ struct Piece {
             if (rank == 0 && tid < 32) for (int i = lane; i < a.count; i += 32) put(i, -1, 0.0);
             return;
         }
-        auto f = [&](float x, int j) { return kept(x, lo + j); };
-        const double whole = sums(f);
+        auto f = [&](int j) { return kept(at(j)); };
+        const double whole = rules();
         double total = whole;
         for (int i = 0; i < a.count; ++i) {
             if (i) total = over_cluster(&sh.x_total[turn], Add());
@@ -556,23 +867,21 @@ struct Piece {
             }
             const float u = a.uniform[(int64_t)row * a.count + i];
             const int j = search((u > 0.f ? (double)u : 0.0) * total, f);
-            if (j >= 0) {
-                const double w = f(at(j), j);
+            if (j >= 0 && warp == 0) {
+                const double w = kept(at(j));
                 if (lane == 0) put(i, lo + j, w / whole);
             }
             if (i + 1 == a.count) break;
             if (j >= 0) {                           // it leaves: its warp's part is summed anew
-                __syncwarp();
-                if (lane == 0) data[j] = nothing<T>();
-                __syncwarp();
-                int part = 0;
-                while (strips * (part + 1) / kWarps <= j / STRIP) ++part;
-                double sum = 0.0;
-                for (int s = strips * part / kWarps; s < strips * (part + 1) / kWarps; ++s)
-#pragma unroll
-                    for (int e = 0; e < N; ++e) sum += f(at(s * STRIP + lane * N + e), s * STRIP + lane * N + e);
-                sum = warp_sum64(sum);
-                if (lane == 0) sh.seg[part] = sum;
+                __syncthreads();
+                if (tid == 0) data[j] = narrow<T>(-INFINITY);
+                __syncthreads();
+                if (j >= s0 * STRIP && j < s1 * STRIP) {
+                    double sum = 0.0;
+                    for (int s = s0; s < s1; ++s) sum += strip_sum(s, border);
+                    sum = warp_sum64(sum);
+                    if (lane == 0) sh.seg[warp] = sum;
+                }
             }
             __syncthreads();
             publish();
@@ -590,11 +899,9 @@ struct Piece {
             if (rank == 0 && tid == 0) put(0, -1, 0.0);
             return;
         }
-        auto whole = [&](float xv, int j) { return kept(xv, lo + j); };
-        const double total = sums(whole);
+        const double total = rules();
         const int b = a.row_seq[row], which = a.draft_rows ? a.draft_rows[row] : row;
         const bool drafted = (unsigned)which < (unsigned)a.draft_count && (unsigned)b < (unsigned)a.num_seqs;
-        int32_t* child = reinterpret_cast<int32_t*>(sh.list);
         if (warp == 0) {
             int n = 0;
             if (drafted) {
@@ -603,7 +910,7 @@ struct Piece {
                     const bool mine = r + lane < r1 && a.parents[r + lane] == row - r0;
                     const uint32_t who = __ballot_sync(kAll, mine);
                     const int at = n + __popc(who & ((1u << lane) - 1u));
-                    if (mine && at < PA_TREE_MOST_NODES) child[at] = r + lane;
+                    if (mine && at < PA_TREE_MOST_NODES) sh.child[at] = r + lane;
                     n += __popc(who);
                 }
             }
@@ -613,14 +920,11 @@ struct Piece {
         const Q* q = drafted ? static_cast<const Q*>(a.draft) + (int64_t)which * a.draft_stride : nullptr;
         const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.stride;
         double taken = 0.0, S = total, gone = 0.0;
-        auto rest = [&](float xv, int j) {          // what refused children have left of a token
-            const double w = kept(xv, lo + j);
-            return w > 0.0 ? fmax(w - taken * (double)widen<Q>(q[lo + j]), 0.0) : 0.0;
-        };
         for (int i = 0; i < sh.children; ++i) {
-            const int r = child[i], c = a.tokens[r];
+            const int r = sh.child[i], c = a.tokens[r];
             if ((unsigned)c >= (unsigned)a.vocab) continue;
-            const double w = kept(clean<T>(x[c]), c), qc = (double)widen<Q>(q[c]);
+            const float xc = widen<T>(x[c]);
+            const double w = kept(only >= 0 && c != only ? -INFINITY : fminf(xc, xc == xc ? Limit<T>::most : -INFINITY)), qc = (double)widen<Q>(q[c]);
             if ((double)a.uniform[2 * (int64_t)r] * qc * S < fmax(w - taken * qc, 0.0) * (1.0 - gone)) {
                 if (rank == 0 && tid == 0) put(0, c, w / total);
                 return;
@@ -628,32 +932,44 @@ struct Piece {
             taken += S / fmax(1.0 - gone, 1e-18);
             if (a.distinct) gone += qc;
             double sum = 0.0;
-            for (int s = s0; s < s1; ++s)
+            for (int s = s0; s < s1; ++s) {
+                const int j = s * STRIP + lane;     // lanes on neighbouring tokens, as q lies
+                float xs[N], qs[N], m = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < N; ++e) {       // lanes on neighbouring tokens, as q lies
-                    const int j = s * STRIP + e * 32 + lane;
-                    sum += rest(at(j), j);
+                for (int e = 0; e < N; ++e) {
+                    xs[e] = at(j + e * 32);
+                    m = fmaxf(m, xs[e]);
                 }
+                if (!__any_sync(kAll, m >= border)) continue;
+#pragma unroll
+                for (int e = 0; e < N; ++e) qs[e] = xs[e] >= border ? widen<Q>(q[lo + j + e * 32]) : 0.f;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const double v = weight(xs[e]) - taken * (double)qs[e];
+                    sum += xs[e] >= border && v > 0.0 ? v : 0.0;
+                }
+            }
             S = join(sum);
         }
         const bool left = taken > 0.0 && S > 0.0;
-        if (taken > 0.0 && !left) S = sums(whole);  // nothing is left by rounding, or where q is no distribution
+        if (taken > 0.0 && !left) S = kept_sum();   // nothing is left by rounding, or where q is no distribution
         const float u = a.uniform[2 * (int64_t)row + 1];
-        const double target = (u > 0.f ? (double)u : 0.0) * S;
-        const int j = left ? search(target, rest) : search(target, whole);
-        if (j >= 0) {
-            const double w = whole(at(j), j);
+        const int j = search((u > 0.f ? (double)u : 0.0) * S, [&](int slot) {
+            const double w = kept(at(slot));
+            return left && w > 0.0 ? fmax(w - taken * (double)widen<Q>(q[lo + slot]), 0.0) : w;
+        });
+        if (j >= 0 && warp == 0) {
+            const double w = kept(at(j));
             if (lane == 0) put(0, lo + j, w / total);
         }
     }
 };
 
-template <typename T, typename Q, int MODE> __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant__ Args a) {
+template <typename T, typename Q, int MODE> __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(16) uint8_t smem[];
     Piece<T, Q, MODE> p(a, *reinterpret_cast<Shared*>(smem + a.data_bytes), reinterpret_cast<T*>(smem));
     p.table = exp2((threadIdx.x & 31) / 32.0);
     p.load();
-    if (p.top > -INFINITY) p.rules();
     if constexpr (MODE == PROBS) p.probs();
     else if constexpr (MODE == DRAW) p.draw();
     else p.verify();
@@ -668,6 +984,10 @@ template <typename T, typename Q, int MODE> static int launch(Args a, cudaStream
     a.ranks = 1;
     while (a.ranks < kMostRanks && (bytes(a.ranks) > 56 * 1024 || (a.rows * a.ranks * 2 <= device_info().sm_count && a.vocab / a.ranks >= 4096))) a.ranks *= 2;
     a.data_bytes = bytes(a.ranks);
+    int counts = 1;                     // bits for a CTA's tokens; parts of a step, whose sums must fit beside them
+    while (((size_t)1 << counts) <= a.data_bytes / sizeof(T)) ++counts;
+    a.count_shift = 32 - counts;
+    a.parts = 2 * counts < 32 ? (float)(1 << (32 - 2 * counts < 8 ? 32 - 2 * counts : 8)) : 0.f;
     if (a.data_bytes > most || (int64_t)a.rows * a.ranks > INT_MAX) return PA_ERR_UNSUPPORTED;
     const size_t smem = a.data_bytes + sizeof(Shared);
     const cudaError_t e = allow_dynamic_smem<draw_kernel<T, Q, MODE>>(smem);
