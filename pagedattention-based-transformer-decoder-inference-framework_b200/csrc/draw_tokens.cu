@@ -31,10 +31,10 @@
 namespace pa {
 namespace drawn {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 2048, kPer = kBins / kThreads, kList = 256, kFew = 256, kMostRanks = 8, kMostStrips = 64;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kPer = kBins / kThreads, kList = 256, kMany = 1024, kFew = 256, kMostRanks = 8, kMostStrips = 64;
 static_assert(kFew <= kThreads && kPer % 4 == 0, "a thread for each of few, whole words of steps");
 constexpr uint32_t kAll = 0xffffffffu;
-constexpr float kLowest = -3.402823466e38f;
+constexpr float kLowest = -3.402823466e38f, kSteps = 32.f;      // steps of log2 w
 enum Mode { PROBS, DRAW, VERIFY };
 
 struct Args {
@@ -130,22 +130,26 @@ struct Verdict {                    // of the cluster's first CTA
 struct Shared {                     // beside the piece of the row
     union {
         uint4 hist[kBins / 4];
-        double few_w[kFew];
+        float many[kMany];          // tokens that all CTAs have listed
         int32_t child[PA_TREE_MOST_NODES];
     };
     Near list[kList];
+    union {
+        double few_w[kFew];
+        uint32_t fine[kThreads];
+    };
     float few[kFew];
     double seg[kWarps];             // weights of the warps' parts of the piece, in the row's order
     double strip[kMostStrips];      // of one part's strips
     double part[kWarps], part2[kWarps];
-    float fpart[kWarps];
+    float fpart[kWarps], fpart2[kWarps], fpart3[kWarps];
     int ipart[kWarps];
-    int b_lo, b_hi, b_first, to_n, listed, children, hit;
+    int b_lo, b_hi, b_first, before_n, to_n, listed, children, hit;
     // what the other CTAs of the cluster read
     Verdict verdict;
     float x_top, x_lo, x_hi, x_up;
     int x_first, x_listed;
-    double x_all, x_above, x_total[2];
+    double x_below, x_above, x_total[2];
 };
 
 template <typename T, typename Q, int MODE>
@@ -160,6 +164,7 @@ struct Piece {
     double scale, base, table;      // w = 2^(x scale + base)
     int only;                       // temperature 0: the one token that is kept, else -1
     int turn = 0;                   // of x_total
+    bool left = false;              // has arrived at the last barrier
 
     __device__ Piece(const Args& args, Shared& shared, T* piece) :
         a(args), sh(shared), data(piece), tid(threadIdx.x), warp(threadIdx.x >> 5), lane(threadIdx.x & 31), rank((int)cluster_ctarank()),
@@ -289,38 +294,25 @@ struct Piece {
         }
     }
 
-    // ---- where the border is, as far as the counts tell (by the first CTA): the steps of R that may hold it
-    // bounds(b, n, parts, least, most): the weights that the n tokens of step b have at least and at most
-    template <bool MASS, typename B> __device__ void weigh(double share, bool first, const Verdict& r, int& from, int& to, B bounds) {
-        uint32_t n[kPer], parts[kPer];
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) n[e] = parts[e] = 0;
-#pragma unroll
-        for (int e = 0; e < kPer; e += 4) {
-            uint4 h[kMostRanks];
-            of_all(sh.hist + tid * (kPer / 4) + e / 4, h, make_uint4(0, 0, 0, 0));
-#pragma unroll
-            for (int c = 0; c < kMostRanks; ++c) {
-                const uint32_t w[4] = {h[c].x, h[c].y, h[c].z, h[c].w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    n[e + k] += w[k] >> a.count_shift;
-                    parts[e + k] += w[k] & ((1u << a.count_shift) - 1u);
-                }
-            }
-        }
-        const double limit = MASS && first ? share * over_cluster(&sh.x_all, Add()) : r.limit;
+    // ---- where the border is, as far as counts tell: the steps that may hold it, of PER a thread.  counted(b): (tokens, parts); bounds(b, n, parts,
+    // least, most): the weights that they have at least and at most; above, above_n: what is above the first step.  The border is where what is above it
+    // reaches `limit`, or with `whole` that share of all.  Leaves the tokens above `from` in before_n, those up to `to` in to_n.
+    template <bool MASS, int PER, typename C, typename B>
+    __device__ void weigh(bool whole, double limit, double above, int above_n, int& from, int& to, C counted, B bounds) {
+        uint32_t n[PER];
+        double least_w[PER], most_w[PER], least = 0.0, most = 0.0;
+        int count = 0;
+        uint32_t parts[PER];
+        counted(n, parts);
         if (tid == 0) {
             sh.b_lo = sh.b_hi = -1;
-            sh.b_first = kBins;
+            sh.b_first = INT_MAX;
         }
-        double least_w[kPer], most_w[kPer], least = 0.0, most = 0.0;
-        int count = 0;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
+        for (int e = 0; e < PER; ++e) {
             count += n[e];
             if (!MASS) continue;
-            bounds(tid * kPer + e, n[e], parts[e], least_w[e], most_w[e]);
+            bounds(tid * PER + e, n[e], parts[e], least_w[e], most_w[e]);
             least += least_w[e];
             most += most_w[e];
         }
@@ -342,25 +334,33 @@ struct Piece {
             sh.part2[warp] = most_to;
         }
         __syncthreads();
-        count_to -= count;
-        least_to -= least;
-        most_to -= most;
+        count_to += above_n - count;
+        least_to += above - least;
+        most_to += above - most;
+        double limit_least = limit, limit_most = limit, least_all = 0.0, most_all = 0.0;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w)
+        for (int w = 0; w < kWarps; ++w) {
             if (w < warp) {
                 count_to += sh.ipart[w];
                 least_to += sh.part[w];
                 most_to += sh.part2[w];
             }
+            least_all += sh.part[w];
+            most_all += sh.part2[w];
+        }
+        if (MASS && whole) {
+            limit_least *= least_all;
+            limit_most *= most_all;
+        }
         const int before = count_to;
-        int b_first = kBins, b_lo = -1, b_hi = -1;
+        int b_first = INT_MAX, b_lo = -1, b_hi = -1;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            const int b = tid * kPer + e;
+        for (int e = 0; e < PER; ++e) {
+            const int b = tid * PER + e;
             if (n[e]) {
                 b_first = min(b_first, b);
-                if (MASS ? r.above + most_to < limit : r.above_n + count_to < limit) b_lo = b;
-                if (MASS ? r.above + least_to < limit : r.above_n + count_to < limit) b_hi = b;
+                if (MASS ? most_to < limit_least : count_to < limit) b_lo = b;
+                if (MASS ? least_to < limit_most : count_to < limit) b_hi = b;
             }
             count_to += n[e];
             if (MASS) {
@@ -368,27 +368,20 @@ struct Piece {
                 most_to += most_w[e];
             }
         }
-        if (b_first < kBins) atomicMin(&sh.b_first, b_first);
+        if (b_first < INT_MAX) atomicMin(&sh.b_first, b_first);
         if (b_lo >= 0) atomicMax(&sh.b_lo, b_lo);
         if (b_hi >= 0) atomicMax(&sh.b_hi, b_hi);
         __syncthreads();
-        from = max(sh.b_lo, sh.b_first);
+        from = max(sh.b_lo, sh.b_first);            // the first that has any holds the largest, which is kept
         to = max(sh.b_hi, from);
-        int m = before;
-        if (from / kPer == tid) {
+        int m = before, m_to = before;
 #pragma unroll
-            for (int e = 0; e < kPer; ++e)
-                if (tid * kPer + e < from) m += n[e];
-            sh.verdict.above_n = r.above_n + m;
-            sh.verdict.limit = limit;
+        for (int e = 0; e < PER; ++e) {
+            if (tid * PER + e < from) m += n[e];
+            if (tid * PER + e <= to) m_to += n[e];
         }
-        if (!MASS && to / kPer == tid) {            // tokens up to the last of them
-            m = before;
-#pragma unroll
-            for (int e = 0; e < kPer; ++e)
-                if (tid * kPer + e <= to) m += n[e];
-            sh.to_n = r.above_n + m;
-        }
+        if (from / PER == tid) sh.before_n = m;
+        if (to / PER == tid) sh.to_n = m_to;
         __syncthreads();
     }
 
@@ -412,20 +405,27 @@ struct Piece {
         return of_key((uint32_t)h);
     }
 
-    // the few tokens that the CTAs have listed, in this one (the first)
-    __device__ void gather(int n) {
-        int m[kMostRanks];
-        of_all(&sh.x_listed, m, 0);
-        int c = 0, i = tid;
+    // the n tokens that the CTAs have listed, in this one (the first)
+    __device__ void gather(int n, const int (&m)[kMostRanks]) {
+        for (int t = tid; t < n; t += kThreads) {
+            int c = 0, i = t;
 #pragma unroll
-        for (int k = 0; k < kMostRanks - 1; ++k)
-            if (c == k && i >= m[k]) {
-                i -= m[k];
-                c = k + 1;
-            }
-        if (tid < n) sh.few[tid] = peer(sh.list + i, c)->x;
-        else if (tid < kFew) sh.few[tid] = -INFINITY;
+            for (int k = 0; k < kMostRanks - 1; ++k)
+                if (c == k && i >= m[k]) {
+                    i -= m[k];
+                    c = k + 1;
+                }
+            sh.many[t] = peer(sh.list + i, c)->x;
+        }
         __syncthreads();
+    }
+    // the weights of n few tokens; the sum of those at or above `least`
+    __device__ double weights_of_few(int n, float least) {
+        const float x = tid < n ? sh.few[tid] : -INFINITY;
+        double w = weight(x);
+        w = tid < n && x >= least ? w : 0.0;
+        sh.few_w[tid] = w;
+        return over_block(w, sh.part, Add());
     }
     // the border among n few tokens, each of which sums (or counts) what is above it: of those at or above `least`
     template <bool MASS> __device__ float among(int n, float least, double above, int above_n, double limit) {
@@ -446,13 +446,67 @@ struct Piece {
         const float low = over_block(in ? x : INFINITY, sh.fpart, Min()), most = over_block(x, sh.fpart, Max());
         return fminf(low, most);                    // the largest is kept in any case
     }
-    // their weights; the sum of those at or above `least`
-    __device__ double weights_of_few(int n, float least) {
-        const float x = tid < n ? sh.few[tid] : -INFINITY;
-        double w = weight(x);
-        w = x >= least ? w : 0.0;
-        sh.few_w[tid] = w;
-        return over_block(w, sh.part, Add());
+    // the border among up to kMany tokens, [l, h]: by a finer count, if they are not few; NaN: they are not, nor will they be
+    template <bool MASS> __device__ float select(int n, float l, float h, double above, int above_n, double limit, int& few) {
+        for (int round = 0; round < 5; ++round) {
+            few = 0;
+            if (l == h) return l;
+            if (n <= kFew || round) {
+                if (tid == 0) sh.hit = 0;
+                __syncthreads();
+                for (int t = tid; t < n; t += kThreads) {
+                    const float x = sh.many[t];
+                    if (x >= l && x <= h) {
+                        const int at = atomicAdd(&sh.hit, 1);
+                        if (at < kFew) sh.few[at] = x;
+                    }
+                }
+                __syncthreads();
+                few = sh.hit;
+                if (few <= kFew) {
+                    for (int t = few + tid; t < kFew; t += kThreads) sh.few[t] = -INFINITY;
+                    __syncthreads();
+                    if (MASS) weights_of_few(few, l);
+                    return among<MASS>(few, l, above, above_n, limit);
+                }
+            }
+            const uint32_t k_hi = key_of(h), range = k_hi - key_of(l);
+            const int bits = 32 - __clz(range), shift = bits > 8 ? bits - 8 : 0;
+            sh.fine[tid] = 0;
+            __syncthreads();
+            for (int t = tid; t < n; t += kThreads) {
+                const float x = sh.many[t];
+                if (x >= l && x <= h) atomicAdd(&sh.fine[(k_hi - key_of(x)) >> shift], 1u);
+            }
+            __syncthreads();
+            int from, to;
+            weigh<MASS, 1>(false, limit, above, above_n, from, to,
+                           [&](uint32_t (&c)[1], uint32_t (&q)[1]) { c[0] = sh.fine[tid]; q[0] = 0; },
+                           [&](int b, uint32_t c, uint32_t, double& least, double& most) {
+                               const uint64_t k0 = min((uint64_t)b << shift, (uint64_t)range), k1 = min(((uint64_t)(b + 1) << shift) - 1, (uint64_t)range);
+                               most = c * weight(of_key(k_hi - (uint32_t)k0)) * (1.0 + 1e-10);
+                               least = c * weight(of_key(k_hi - (uint32_t)k1)) * (1.0 - 1e-10);
+                           });
+            above_n = sh.before_n;
+            double sum = 0.0;
+            float low = INFINITY, high = -INFINITY;
+            for (int t0 = 0; t0 < n; t0 += kThreads) {
+                const float x = t0 + tid < n ? sh.many[t0 + tid] : NAN;
+                const int b = x >= l && x <= h ? (int)((k_hi - key_of(x)) >> shift) : INT_MAX;
+                if (MASS) {
+                    const double w = weight(x);
+                    sum += b < from ? w : 0.0;
+                }
+                if (b >= from && b <= to) {
+                    low = fminf(low, x);
+                    high = fmaxf(high, x);
+                }
+            }
+            if (MASS) above += over_block(sum, sh.part, Add());
+            l = over_block(low, sh.fpart, Min());
+            h = over_block(high, sh.fpart, Max());
+        }
+        return NAN;
     }
 
     // ---- the border: the least value that is kept of those from `least` on.  With MASS the weights above it are below `share` of all, else fewer
@@ -467,12 +521,12 @@ struct Piece {
         r.above_n = 0;
         r.limit = share;
         r.halve = 0;
-        const float step = (float)(scale * 64.0), parts = a.parts;
-        // steps of 1/64 in log2 w to begin with, rounded to the nearest; by floats where these would be too coarse or too fine, and afterwards
+        const float step = (float)(scale * kSteps), parts = a.parts;
+        // steps of 1/32 in log2 w to begin with, rounded to the nearest; by floats where these would be too coarse or too fine, and afterwards
         bool first = true, by_logs = scale > 1e-6 && scale < 1e6;
         for (int level = 0; level < 128; ++level) {
             const uint32_t k_hi = key_of(r.r_hi) >> Limit<T>::spare, range = k_hi - (key_of(r.r_lo) >> Limit<T>::spare);
-            const int bits = 32 - __clz(range), shift = bits > 11 ? bits - 11 : 0;
+            const int bits = 32 - __clz(range), shift = bits > 10 ? bits - 10 : 0;
             auto by_log = [&](float x) { return fminf((top - x) * step, kBins - 1.f); };
             auto place = [&](float x) -> int {
                 if (by_logs) return __float_as_int(by_log(x) + 8388608.f) & (kBins - 1);
@@ -481,14 +535,12 @@ struct Piece {
             if (!r.halve) {
                 for (int i = tid; i < kBins / 4; i += kThreads) sh.hist[i] = make_uint4(0, 0, 0, 0);
                 __syncthreads();
-                double all = 0.0;
                 const uint32_t hist = smem_u32(sh.hist), one = 1u << a.count_shift;
                 for (int s = s0; s < s1; ++s) {
                     const Word<T> w = *reinterpret_cast<const Word<T>*>(data + s * STRIP + lane * N);
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
                         const float x = widen<T>(w.v[e]);
-                        const bool here = x >= r.r_lo && x <= r.r_hi;
                         uint32_t at = hist, add = one;
                         if (by_logs) {
                             const float d = by_log(x), up = d + 8388608.f;
@@ -497,26 +549,34 @@ struct Piece {
                         } else {
                             at += place(x) * 4;
                         }
-                        if (here) asm volatile("red.shared.add.u32 [%0], %1;" ::"r"(at), "r"(add) : "memory");
-                        if (MASS && first) {
-                            const double v = weight(x);
-                            all += here ? v : 0.0;
-                        }
+                        if (x >= r.r_lo && x <= r.r_hi) asm volatile("red.shared.add.u32 [%0], %1;" ::"r"(at), "r"(add) : "memory");
                     }
-                }
-                if (MASS && first) {
-                    all = over_block(all, sh.part, Add());
-                    if (tid == 0) sh.x_all = all;
                 }
                 cluster_sync();
                 if (rank == 0) {
                     int from, to;
-                    // d of a step's tokens: b + what their parts say, within half a part; w = 2^(-d/64) falls by at most a 6e-5th of itself more than
-                    // evenly between the ends of a step, and (top - x) step is rounded by 2048 x 2^-22 of a step
+                    auto counted = [&](uint32_t (&n)[kPer], uint32_t (&q)[kPer]) {
+                        uint4 h[kMostRanks];
+                        of_all(sh.hist + tid, h, make_uint4(0, 0, 0, 0));
+#pragma unroll
+                        for (int e = 0; e < kPer; ++e) n[e] = q[e] = 0;
+#pragma unroll
+                        for (int c = 0; c < kMostRanks; ++c) {
+                            const uint32_t w[4] = {h[c].x, h[c].y, h[c].z, h[c].w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                n[k] += w[k] >> a.count_shift;
+                                q[k] += w[k] & (one - 1u);
+                            }
+                        }
+                    };
+                    // d of a step's tokens: b + what their parts say, within half a part; w = 2^(-d/32) falls by at most a 6e-5th of itself more than
+                    // evenly between the ends of a step, and (top - x) step is rounded by 1024 x 2^-22 of a step
+                    const float half = parts > 0.f ? 0.5f / parts : 0.5f;
                     auto by_step = [&](int b, uint32_t n, uint32_t q, double& l, double& m) {
-                        const float mean = parts > 0.f && n ? ((float)q / (float)n - 0.5f * parts) / parts : 0.f, half = parts > 0.f ? 0.5f / parts : 0.5f;
-                        m = n * (double)exp2f((half - mean - b) / 64.f) * (1.0 + 8e-5);
-                        l = b == kBins - 1 ? 0.0 : n * (double)exp2f((-half - mean - b) / 64.f) * (1.0 - 2e-5);
+                        const float mean = parts > 0.f && n ? (__fdividef((float)q, (float)n) - 0.5f * parts) * (2.f * half) : 0.f;
+                        m = n * (double)exp2f((half - mean - b) * (1.f / kSteps)) * (1.0 + 8e-5);
+                        l = b == kBins - 1 ? 0.0 : n * (double)exp2f((-half - mean - b) * (1.f / kSteps)) * (1.0 - 2e-5);
                     };
                     auto by_float = [&](int b, uint32_t n, uint32_t, double& l, double& m) {
                         const uint64_t k0 = min((uint64_t)b << shift, (uint64_t)range), k1 = min(((uint64_t)(b + 1) << shift) - 1, (uint64_t)range);
@@ -524,8 +584,8 @@ struct Piece {
                         m = n * w0 * (shift ? 1.0 + 1e-10 : 1.0);
                         l = n * w1 * (shift ? 1.0 - 1e-10 : 1.0);
                     };
-                    if (by_logs) weigh<MASS>(share, first, r, from, to, by_step);
-                    else weigh<MASS>(share, first, r, from, to, by_float);
+                    if (by_logs) weigh<MASS, kPer>(first, r.limit, r.above, r.above_n, from, to, counted, by_step);
+                    else weigh<MASS, kPer>(first, r.limit, r.above, r.above_n, from, to, counted, by_float);
                     const bool all_few = !MASS && first && sh.to_n <= kFew;         // all that can be kept are few: listed, not summed
                     if (by_logs) {
                         if (warp == 0) {
@@ -540,7 +600,7 @@ struct Piece {
                         sh.verdict.up = all_few ? INFINITY : from == 0 ? above_of(r.r_hi) : of_spared(k_hi - (uint32_t)(((uint64_t)from << shift) - 1));
                         sh.verdict.lo = k > range ? r.r_lo : fmaxf(of_spared(k_hi - (uint32_t)k + 1), r.r_lo);
                     }
-                    if (all_few && tid == 0) sh.verdict.above_n = 0;
+                    if (tid == 0) sh.verdict.above_n = all_few ? 0 : sh.before_n;
                 }
             } else {                                        // the bounds did not help: by halves, whose weights are summed
                 cluster_sync();                             // the last verdict has been read
@@ -548,18 +608,17 @@ struct Piece {
                     sh.verdict.up = of_spared(k_hi - range / 2);
                     sh.verdict.lo = r.r_lo;
                     sh.verdict.above_n = r.above_n;
-                    sh.verdict.limit = r.limit;
                 }
             }
             cluster_sync();
             const float up = peer(&sh.verdict, 0)->up, near = peer(&sh.verdict, 0)->lo;
-            r.limit = peer(&sh.verdict, 0)->limit;
             const int above_n = peer(&sh.verdict, 0)->above_n;
-            // ---- what is above those steps, summed; what is in them, listed
+            // ---- what is above those steps, summed (with what is not, the first time: a share is of all); what is in them, listed
             if (tid == 0) sh.listed = 0;
             __syncthreads();
-            double sum = 0.0;
+            double sum = 0.0, below = 0.0;
             float least_x = INFINITY, most_x = -INFINITY, least_up = INFINITY;
+            const float floor = MASS && first ? least : near;
             for (int s = s0; s < s1; ++s) {
                 const int j = s * STRIP + lane * N;
                 const Word<T> w = *reinterpret_cast<const Word<T>*>(data + j);
@@ -570,10 +629,15 @@ struct Piece {
                     x[e] = widen<T>(w.v[e]);
                     m = fmaxf(m, x[e]);
                 }
-                if (!__any_sync(kAll, m >= near)) continue;
+                if (!__any_sync(kAll, m >= floor)) continue;
+                if (MASS && first) {
 #pragma unroll
-                for (int e = 0; e < N; ++e) mine |= (uint32_t)(x[e] >= near && !(x[e] >= up)) << e;
-                if ((MASS || sums) && __any_sync(kAll, m >= up)) {
+                    for (int e = 0; e < N; ++e) {
+                        const double v = weight(x[e]);
+                        sum += x[e] >= up ? v : 0.0;
+                        below += x[e] >= floor && !(x[e] >= up) ? v : 0.0;
+                    }
+                } else if ((MASS || sums) && __any_sync(kAll, m >= up)) {
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
                         const double v = weight(x[e]);
@@ -581,9 +645,10 @@ struct Piece {
                         if (r.halve && x[e] >= up && x[e] <= r.r_hi) least_up = fminf(least_up, x[e]);
                     }
                 }
-                if (__any_sync(kAll, mine != 0)) {
-                    int at = 0;
-                    if (mine) at = atomicAdd(&sh.listed, __popc(mine));
+#pragma unroll
+                for (int e = 0; e < N; ++e) mine |= (uint32_t)(x[e] >= near && !(x[e] >= up)) << e;
+                if (mine) {
+                    int at = atomicAdd(&sh.listed, __popc(mine));
 #pragma unroll
                     for (int e = 0; e < N; ++e)
                         if (mine >> e & 1u) {
@@ -593,24 +658,43 @@ struct Piece {
                             ++at;
                         }
                 }
+                __syncwarp();
             }
             sum = warp_sum64(sum);
-            if (lane == 0) sh.seg[warp] = sum;
-            least_x = over_block(least_x, sh.fpart, Min());
-            most_x = over_block(most_x, sh.fpart, Max());
-            if (r.halve) least_up = over_block(least_up, sh.fpart, Min());
-            if (tid == 0) {
-                double t = 0.0;
+            if (MASS && first) below = warp_sum64(below);
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) t += sh.seg[w];
-                sh.x_above = t;
+            for (int o = 16; o > 0; o >>= 1) {
+                least_x = fminf(least_x, __shfl_xor_sync(kAll, least_x, o));
+                most_x = fmaxf(most_x, __shfl_xor_sync(kAll, most_x, o));
+                if (r.halve) least_up = fminf(least_up, __shfl_xor_sync(kAll, least_up, o));
+            }
+            if (lane == 0) {
+                sh.seg[warp] = sum;
+                sh.part[warp] = below;
+                sh.fpart[warp] = least_x;
+                sh.fpart2[warp] = most_x;
+                sh.fpart3[warp] = least_up;
+            }
+            __syncthreads();
+            if (tid == 0) {
+                sum = below = 0.0;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    sum += sh.seg[w];
+                    below += sh.part[w];
+                    least_x = fminf(least_x, sh.fpart[w]);
+                    most_x = fmaxf(most_x, sh.fpart2[w]);
+                    least_up = fminf(least_up, sh.fpart3[w]);
+                }
+                sh.x_above = sum;
+                sh.x_below = below;
                 sh.x_lo = least_x;
                 sh.x_hi = most_x;
                 sh.x_up = least_up;
                 sh.x_listed = sh.listed;
             }
             cluster_sync();
-            // ---- few are left, or all alike: the border; else once more
+            // ---- not many are left, or all alike: the border; else once more
             if (rank == 0) {
                 int listed[kMostRanks], n = 0, most = 0;
                 of_all(&sh.x_listed, listed, 0);
@@ -620,15 +704,21 @@ struct Piece {
                     most = max(most, listed[c]);
                 }
                 const double above = MASS ? over_cluster(&sh.x_above, Add()) : 0.0;
+                const double limit = MASS && first ? share * (above + over_cluster(&sh.x_below, Add())) : r.limit;
                 const float l = over_cluster(&sh.x_lo, Min()), h = over_cluster(&sh.x_hi, Max()), u = r.halve ? over_cluster(&sh.x_up, Min()) : 0.f;
-                const bool upper = MASS && r.halve && above >= r.limit;          // the border is in the upper half
-                const bool few = !upper && n <= kFew && most <= kList, rules_too = !MASS && up == INFINITY && few;
-                float found = l;
-                if (few && (l < h || rules_too)) {
-                    gather(n);
-                    if (MASS) weights_of_few(n, -INFINITY);
-                    found = among<MASS>(n, -INFINITY, above, above_n, r.limit);
+                const bool upper = MASS && r.halve && above >= limit;            // the border is in the upper half
+                const bool many = !upper && n <= kMany && most <= kList, rules_too = !MASS && up == INFINITY && many && n <= kFew;
+                float found = NAN;
+                if (l == h && !upper && !rules_too) found = l;
+                else if (many) {
+                    int few;
+                    gather(n, listed);
+                    found = select<MASS>(n, l, h, above, above_n, limit, few);
                     if (rules_too && p < 1.0) {
+                        if (few == 0) {                     // (all alike)
+                            sh.few[tid] = tid < n ? sh.many[tid] : -INFINITY;
+                            __syncthreads();
+                        }
                         const double all = weights_of_few(n, found);
                         found = among<true>(n, found, 0.0, 0, p * all);
                     }
@@ -636,12 +726,13 @@ struct Piece {
                 if (tid == 0) {
                     Verdict& v = sh.verdict;
                     v.border = found;
-                    v.done = !upper && (few || l == h);
+                    v.done = found == found;
                     v.ruled = rules_too;
                     v.r_lo = upper ? u : l;
                     v.r_hi = upper ? r.r_hi : h;
                     v.above = upper ? r.above : above;
                     v.above_n = above_n;
+                    v.limit = limit;
                     v.halve = MASS && !by_logs && !r.halve && !v.done &&
                               key_of(v.r_hi) - key_of(v.r_lo) > (key_of(r.r_hi) - key_of(r.r_lo)) / 2;
                 }
@@ -658,6 +749,7 @@ struct Piece {
             r.r_hi = v.r_hi;
             r.above = v.above;
             r.above_n = v.above_n;
+            r.limit = v.limit;
             r.halve = v.halve;
             by_logs = first = false;
         }
@@ -742,9 +834,13 @@ struct Piece {
     }
 
     // ---- the first token up to which the sums of f(slot) exceed `target`, as a slot of the CTA whose piece has it; -1 in the others
-    template <typename F> __device__ int search(double target, F f) {
+    template <typename F> __device__ int search(double target, bool last, F f) {
         double t[kMostRanks], run = 0.0, mine = 0.0;
         of_all(&sh.x_total[turn], t, 0.0);
+        if (last) {             // nothing of the others is read any more
+            cluster_arrive();
+            left = true;
+        }
         int owner = -1;
         bool open = true;
 #pragma unroll
@@ -802,17 +898,17 @@ struct Piece {
                 if (lane >= o) to += q;
             }
             double cum = mine + to - own;
-            int hit = -1, last = -1;
+            int hit = -1, end = -1;
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 cum += w[e];
                 if (w[e] > 0.0) {
-                    last = j + e;
+                    end = j + e;
                     if (hit < 0 && cum > target) hit = j + e;
                 }
             }
             const uint32_t who = __ballot_sync(kAll, hit >= 0);
-            hit = who ? __shfl_sync(kAll, hit, __ffs(who) - 1) : __reduce_max_sync(kAll, last);
+            hit = who ? __shfl_sync(kAll, hit, __ffs(who) - 1) : __reduce_max_sync(kAll, end);
             if (lane == 0) sh.hit = hit;
         }
         __syncthreads();
@@ -866,7 +962,7 @@ struct Piece {
                 continue;                           // (so will all the others be)
             }
             const float u = a.uniform[(int64_t)row * a.count + i];
-            const int j = search((u > 0.f ? (double)u : 0.0) * total, f);
+            const int j = search((u > 0.f ? (double)u : 0.0) * total, i + 1 == a.count, f);
             if (j >= 0 && warp == 0) {
                 const double w = kept(at(j));
                 if (lane == 0) put(i, lo + j, w / whole);
@@ -951,12 +1047,12 @@ struct Piece {
             }
             S = join(sum);
         }
-        const bool left = taken > 0.0 && S > 0.0;
-        if (taken > 0.0 && !left) S = kept_sum();   // nothing is left by rounding, or where q is no distribution
+        const bool some = taken > 0.0 && S > 0.0;
+        if (taken > 0.0 && !some) S = kept_sum();   // nothing is left by rounding, or where q is no distribution
         const float u = a.uniform[2 * (int64_t)row + 1];
-        const int j = search((u > 0.f ? (double)u : 0.0) * S, [&](int slot) {
+        const int j = search((u > 0.f ? (double)u : 0.0) * S, true, [&](int slot) {
             const double w = kept(at(slot));
-            return left && w > 0.0 ? fmax(w - taken * (double)widen<Q>(q[lo + slot]), 0.0) : w;
+            return some && w > 0.0 ? fmax(w - taken * (double)widen<Q>(q[lo + slot]), 0.0) : w;
         });
         if (j >= 0 && warp == 0) {
             const double w = kept(at(j));
@@ -973,7 +1069,8 @@ template <typename T, typename Q, int MODE> __global__ void __launch_bounds__(kT
     if constexpr (MODE == PROBS) p.probs();
     else if constexpr (MODE == DRAW) p.draw();
     else p.verify();
-    cluster_sync();                     // no CTA leaves while others read its shared memory
+    if (!p.left) cluster_arrive();      // no CTA leaves while others read its shared memory
+    cluster_wait();
 }
 
 template <typename T, typename Q, int MODE> static int launch(Args a, cudaStream_t st) {
