@@ -1065,6 +1065,7 @@ int pa_conv_append_in_words(int units, int columns, int num_items, int64_t rows)
 #define PA_TYPE_BF16 2
 #define PA_TYPE_I8 3
 #define PA_TREE_MOST_NODES 1024
+#define PA_DRAW_MOST_ROW_BYTES 1500000
 size_t pa_tree_attention_workspace_bytes(int rows, int num_seqs, int most_nodes, int heads, int kv_heads, int head_dim);
 int pa_tree_attention(const void* d_q, int64_t q_stride, int q_type, void* d_out, const void* d_k_pool, const void* d_v_pool,
                       const float* d_k_scales, const float* d_v_scales, int kv_type, const int32_t* d_table, int num_beams, int kv_heads,
@@ -1109,15 +1110,16 @@ int pa_tree_accept(const int32_t* d_ids, const int32_t* d_tokens, const int32_t*
  *     a token stays if fewer than top_k tokens are above it (top_k <= 0: all do), if the w above it, of those that stay so far, sum up to
  *     less than top_p of theirs (top_p not below 1: all do), and if its w is at least min_p; the largest always stays, tokens of one
  *     value stay or go together;       p = w / (sum of the w that stay)
- * Weights and sums are in 64 bits.  Vocabularies up to 1.5 million bytes of logits a row (more: PA_ERR_UNSUPPORTED).
+ * Weights and sums are in 64 bits.  Vocabularies up to PA_DRAW_MOST_ROW_BYTES of logits a row (more: PA_ERR_UNSUPPORTED).  The workspace, on 16
+ * bytes, holds what the kernels of a call leave each other; it needs no values before a call.
  *
  * pa_truncated_softmax: p as floats [rows][vocab], rows probs_stride apart (zeros where every logit is -inf), in memory that the logits do not
  *   share (PA_ERR_INVALID_ARG).
  * pa_draw_tokens: d_ids[r][i] = the first v up to which the sum of p, without the tokens d_ids[r][0 .. i - 1], exceeds
  *   d_uniform[r][i] times all of it (numbers below 0 and NaN as 0; from 1 on: the last token that stays); -1 where no token is left.
  *   d_logprobs (NULL: not wanted): log p of it, -inf for -1.
- * pa_verify_drafts: rows are nodes of drafted trees (pa_draft_trees; d_node_start [num_seqs + 1], d_row_seq not NULL).  The children of node r, in
- *   order, were drawn from q = row d_draft_rows[r] (NULL: r) of d_draft (of draft_type, rows draft_stride apart): each from all of it, or
+ * pa_verify_drafts: rows are nodes of drafted trees (pa_draft_trees; d_node_start [num_seqs + 1], d_row_seq not NULL).  The children of node r (at most
+ *   most_children of any node), in order, were drawn from q = row d_draft_rows[r] (NULL: r) of d_draft (of draft_type, rows draft_stride apart): each from all of it, or
  *   with `distinct` from what the ones before it left.  One after the other a child c is kept, where d_uniform[c][0] q(c) S < max(p(c) -
  *   a q(c), 0) (1 - Q), or refused (a += S / (1 - Q), S = sum max(p - a q, 0), with `distinct` Q += q(c); from a = 0, S = 1, Q = 0).
  *   d_ids[r]: the token of the child that is kept, else one drawn by d_uniform[r][1] from max(p - a q, 0) (from p, where nothing is left of it);
@@ -1135,14 +1137,15 @@ typedef struct {
     int top_k;
     double top_p, min_p;
 } pa_draw_rules;
+size_t pa_draw_workspace_bytes(int type, int rows, int vocab);
 int pa_truncated_softmax(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, float* d_probs,
-                         int64_t probs_stride, pa_stream_t stream);
+                         int64_t probs_stride, void* d_workspace, size_t workspace_bytes, pa_stream_t stream);
 int pa_draw_tokens(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, const float* d_uniform, int count,
-                   int32_t* d_ids, float* d_logprobs, pa_stream_t stream);
+                   int32_t* d_ids, float* d_logprobs, void* d_workspace, size_t workspace_bytes, pa_stream_t stream);
 int pa_verify_drafts(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, const float* d_uniform,
-                     const int32_t* d_tokens, const int32_t* d_parents, const int32_t* d_node_start, const void* d_draft, int draft_type,
+                     const int32_t* d_tokens, const int32_t* d_parents, const int32_t* d_node_start, int most_children, const void* d_draft, int draft_type,
                      int64_t draft_stride, int draft_count, const int32_t* d_draft_rows, int distinct, int32_t* d_ids, float* d_logprobs,
-                     pa_stream_t stream);
+                     void* d_workspace, size_t workspace_bytes, pa_stream_t stream);
 
 /* Pages handed out on the GPU (device_pages.cu), for steps whose lengths only the GPU knows; the host's way is KVTileCache::register_tile
  * (kv_cache/kv_tile_cache.cpp:65-98).  Table row b holds pages for its first d_held[b] tiles, of every head; the d_state[0] free pages are the

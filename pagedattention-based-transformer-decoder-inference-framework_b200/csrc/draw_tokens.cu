@@ -17,9 +17,15 @@
 // thousand.  2^y is 2^(j/32), from a table that the warp's lanes hold, times a polynomial of the fourth degree of the rest |r| <= 1/64 (Taylor's,
 // error (r ln 2)^5 / 5! <= 1.3e-12): nine operations in 64 bits, of which an SM does 64 a cycle.
 //
-// A row is shared by a cluster of CTAs, whose shared memory holds it: logits come from memory once.  The least value that is kept is found
-// without sorting: tokens are counted by 2048 steps of 1/64 in log2 w; with the bounds of the steps' weights the counts tell within some per cent where
-// the border is; what is above is summed exactly, what is near is listed and counted again by finer steps, of floats in the end.
+// Rows are read in chunks of up to 64 strips (8192 tokens) by CTAs that know nothing of each other, from memory once and from L2 once more:
+//   count   (where a rule needs it) every chunk's largest logit, and its tokens by 1024 steps of 1/32 in log2 w
+//   range   (a CTA a row) the least value that is kept lies in one or two of these steps: found from bounds of their weights, without sorting
+//   sum     the weights of what is above those steps, in 64 bits, and a list of what is in them
+//   finish  (a cluster of CTAs a row) the border among the listed tokens, the sums of the chunks, the tokens that the numbers draw; verification
+//   write   probabilities
+// Rows that this does not settle (more tokens than the lists hold, of logits that lie closer than a step; temperatures far from 1) are searched by
+// finish itself, by finer steps.
+#include <algorithm>
 #include <climits>
 #include <type_traits>
 
@@ -31,19 +37,47 @@
 namespace pa {
 namespace drawn {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kPer = kBins / kThreads, kList = 256, kMany = 1024, kFew = 256, kMostRanks = 8, kMostStrips = 64;
-static_assert(kFew <= kThreads && kPer % 4 == 0, "a thread for each of few, whole words of steps");
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kPer = kBins / kThreads, kList = 256, kMany = 2048, kFew = 256, kMostRanks = 8;
+constexpr int kWords = 8, kMostChunkStrips = kWords * kWarps, kMostStrips = 512, kMostChunks = 512, kGroup = 8192;       // a group of rows has so many chunks
+static_assert(kFew == kThreads && kPer == 4, "a thread for each of few; a word of steps a thread");
+constexpr int kCountShift = 18;             // a step's word: a chunk's tokens (up to 8192) from here on, the sum of their parts below
 constexpr uint32_t kAll = 0xffffffffu;
-constexpr float kLowest = -3.402823466e38f, kSteps = 32.f;      // steps of log2 w
+constexpr float kLowest = -3.402823466e38f, kSteps = 32.f, kLogitSteps = 32.f;      // steps of log2 w, or of a logit where these are smaller
+constexpr int kParts = 16;                                      // of a step, by which its tokens' mean is known
+constexpr float kMagic = 12582912.f;                            // 1.5 x 2^23: sums end at whole numbers
 enum Mode { PROBS, DRAW, VERIFY };
+
+struct Near { float x; int token; };
+struct Chunk {
+    double above, whole;            // sums of the weights at or above `up`, and of all
+    float top, lo, hi;              // the largest logit; the ends of what is listed
+    int listed, first;              // how many, the lowest of them
+    int spare_;
+};
+struct Row {                        // what range and finish leave
+    float top, up, lo, border;      // (up may be no number: nothing is at or above it)
+    float floor;                    // what has a weight in 64 bits
+    int above_n, settled, only, all;
+    double scale, share;
+};
+
+struct Rest {                       // a node whose last child was refused
+    double taken, out, total;       // a, Q, the sum of the kept
+    int child, open;                // the next child; whether the rest is to be summed
+};
 
 struct Args {
     const void* logits;
     int64_t stride;
     int rows, vocab, ranks, num_seqs;
-    size_t data_bytes;                                      // shared memory of a CTA's piece of the row
-    int count_shift;                                        // a step's word: tokens above it, their parts of a step below
-    float parts;                                            // of a step (0: none are kept)
+    int row0, chunks, chunk_strips;                         // of the group of rows; chunks of a row, strips of a chunk
+    int ranked;                                             // whether a rule may need an order (top_k, top_p, min_p)
+    uint32_t* hist;                                         // workspace: [chunks of the group][kBins]
+    Near* list;                                             // [chunks][kList]
+    Chunk* chunk;
+    Row* row;
+    Rest* rest;
+    double* rest_sum;                                       // [chunks]
     const int32_t* row_seq;
     const float *temperature, *top_p, *min_p;               // per sequence; null: the value beside it
     const int32_t* top_k;
@@ -94,6 +128,7 @@ struct Add {
     template <typename V> __device__ V operator()(V a, V b) const { return a + b; }
     template <typename V> __device__ static V none() { return 0; }
 };
+struct Most { __device__ int operator()(int a, int b) const { return max(a, b); } };
 struct Max {
     __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
     template <typename V> __device__ static V none() { return -INFINITY; }
@@ -104,73 +139,125 @@ struct Min {
     template <typename V> __device__ static V none() { return std::is_same<V, int>::value ? (V)INT_MAX : (V)INFINITY; }
 };
 
+__device__ const double kTable[32] = {     // 2^(j/32)
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+};
+__constant__ double kPoly[4] = {0.69314718055994530942, 0.24022650695910071233, 0.05550410866482157995, 0.00961812910762847716};        // ln 2 ^ k / k!
 // 2^y by all lanes of a warp, lane j of which holds 2^(j/32) in `table`: for y of -1022 to 0; others give some number
 __device__ __forceinline__ double exp2_64(double y, double table) {
     constexpr double magic = 211106232532992.0;             // 1.5 x 2^47: sums end at multiples of 1/32
-    constexpr double c1 = 0.69314718055994530942, c2 = 0.24022650695910071233, c3 = 0.05550410866482157995, c4 = 0.00961812910762847716;    // ln 2 ^ k / k!
     const double at = y + magic;
     const int n = __double2loint(at);
     const double r = y - (at - magic);
-    double p = fma(r, c4, c3);
-    p = fma(r, p, c2);
-    p = fma(r, p, c1);
+    double p = fma(r, kPoly[3], kPoly[2]);
+    p = fma(r, p, kPoly[1]);
+    p = fma(r, p, kPoly[0]);
     p = fma(r, p, 1.0);
-    p *= __shfl_sync(kAll, table, n & 31);
-    return __hiloint2double(__double2hiint(p) + (n >> 5 << 20), __double2loint(p));
+    p *= __shfl_sync(kAll, table, n);           // (of which the low five bits count)
+    return __hiloint2double(__double2hiint(p) + (n >> 5) * 1048576, __double2loint(p));
 }
 
-struct Near { float x; int slot; };
-struct Verdict {                    // of the cluster's first CTA
-    float up, lo;                   // what is at or above `up` is summed, what is at or above `lo` listed
-    float r_lo, r_hi, border;
-    double above, limit;
-    int above_n, done, halve, ruled;
-};
 
-struct Shared {                     // beside the piece of the row
-    union {
-        uint4 hist[kBins / 4];
-        float many[kMany];          // tokens that all CTAs have listed
-        int32_t child[PA_TREE_MOST_NODES];
-    };
-    Near list[kList];
-    union {
-        double few_w[kFew];
-        uint32_t fine[kThreads];
-    };
-    float few[kFew];
-    double seg[kWarps];             // weights of the warps' parts of the piece, in the row's order
-    double strip[kMostStrips];      // of one part's strips
-    double part[kWarps], part2[kWarps];
-    float fpart[kWarps], fpart2[kWarps], fpart3[kWarps];
-    int ipart[kWarps];
-    int b_lo, b_hi, b_first, before_n, to_n, listed, children, hit;
-    // what the other CTAs of the cluster read
-    Verdict verdict;
-    float x_top, x_lo, x_hi, x_up;
-    int x_first, x_listed;
-    double x_below, x_above, x_total[2];
-};
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-template <typename T, typename Q, int MODE>
-struct Piece {
+// the rules of a row's sequence
+struct Rules {
+    double t, p, m, scale;
+    float fine;                     // parts of a logit
+    int k;
+    __device__ Rules(const Args& a, int row) {
+        const int b = a.row_seq ? a.row_seq[row] : row;
+        const bool known = (unsigned)b < (unsigned)a.num_seqs;
+        t = !known ? 1.0 : a.temperature ? (double)a.temperature[b] : a.temperature1;
+        p = !known ? 1.0 : a.top_p ? (double)a.top_p[b] : a.top_p1;
+        m = !known ? 0.0 : a.min_p ? (double)a.min_p[b] : a.min_p1;
+        k = !known ? 0 : a.top_k ? a.top_k[b] : a.top_k1;
+        if (k >= a.vocab || k < 0) k = 0;
+        scale = greedy() ? 0.0 : 1.4426950408889634074 / t;
+        fine = fmaxf((float)(scale * kSteps), kLogitSteps) * kParts;
+    }
+    __device__ bool greedy() const { return !(t > 0.0); }
+    __device__ bool counts() const { return (k > 0 || p < 1.0) && !greedy() && scale > 1e-6 && scale < 1e6; }
+    __device__ static float at_least(double x) { return x >= (double)kLowest ? __double2float_ru(x) : kLowest; }
+    // from where on a token has a weight in 64 bits, and one of at least m
+    __device__ float floor(float top) const { return at_least((double)top - 1021.0 / scale); }
+    __device__ float least(float top) const {
+        return !(m > 0.0) ? kLowest : m >= 1.0 ? (t < INFINITY ? top : kLowest) : at_least((double)top + t * log(m));
+    }
+};
+// Steps on a grid that all chunks share, each of kParts: the bits of a float that is the nearest part above kMagic, so that differences of bits are
+// differences of parts (up to 2^22 of them; what lies further down differs by more).  `first` ends the step of the largest.
+__device__ __forceinline__ uint32_t on_grid(float x, float fine) { return __float_as_uint(fmaf(x, fine, kMagic)); }
+__device__ __forceinline__ uint32_t below(uint32_t first, float x, float fine) { return min(first - on_grid(x, fine), (uint32_t)(kBins * kParts - 1)); }
+
+// a row as strips of 32 words of 16 bytes from the word that it begins in; what is outside it is -inf
+template <typename T> struct View {
     static constexpr int N = Word<T>::N, STRIP = 32 * N;
-    const Args& a;
-    Shared& sh;
-    T* const data;                  // slot j is token lo + j; what is outside the row is -inf
-    const int tid, warp, lane, rank, row;
-    int lo, used, strips, s0, s1;   // slots that are used, strips of 32 words; this warp's are s0 .. s1 - 1
-    float top, border;              // the largest; the least value that is kept
-    double scale, base, table;      // w = 2^(x scale + base)
-    int only;                       // temperature 0: the one token that is kept, else -1
-    int turn = 0;                   // of x_total
-    bool left = false;              // has arrived at the last barrier
+    const T* x;
+    int V, off, strips;
+    __device__ View(const Args& a, int row) : x(static_cast<const T*>(a.logits) + (int64_t)row * a.stride), V(a.vocab) {
+        off = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+        strips = (V + off + STRIP - 1) / STRIP;
+    }
+    __device__ __forceinline__ int token(int s, int lane) const { return s * STRIP + lane * N - off; }         // the first of a lane's word
+    // whether n strips are whole (for all lanes alike: loads that wait on no branch of their own are on their way together)
+    __device__ __forceinline__ bool whole(int s, int n) const { return token(s, 0) >= 0 && token(s + n, 0) <= V; }
+    __device__ __forceinline__ Word<T> load_whole(int s, int lane) const {
+        const uint4 raw = ldg_stream_128(x + token(s, lane));
+        return *reinterpret_cast<const Word<T>*>(&raw);
+    }
+    __device__ __forceinline__ Word<T> load(int s, int lane) const {
+        const int v = token(s, lane);
+        Word<T> w;
+        if (whole(s, 1)) w = load_whole(s, lane);
+        else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) w.v[e] = v + e >= 0 && v + e < V ? x[v + e] : narrow<T>(-INFINITY);
+        }
+        return w;
+    }
+    // f(word, strip, first token of the lane's word) for the strips from s on, `step` apart, several on their way at once
+    template <int SOME, typename F> __device__ __forceinline__ void each(int s, int s1, int step, int lane, F f) const {
+        for (; s < s1; s += SOME * step) {
+            Word<T> w[SOME];
+            if (s + (SOME - 1) * step < s1 && whole(s, (SOME - 1) * step + 1)) {
+#pragma unroll
+                for (int k = 0; k < SOME; ++k) w[k] = load_whole(s + k * step, lane);
+            } else {
+#pragma unroll
+                for (int k = 0; k < SOME; ++k)
+                    if (s + k * step < s1) w[k] = load(s + k * step, lane);
+            }
+#pragma unroll
+            for (int k = 0; k < SOME; ++k)
+                if (s + k * step < s1) f(w[k], s + k * step, token(s + k * step, lane));
+        }
+    }
+    __device__ __forceinline__ float at(int v) const { return v >= 0 && v < V ? widen<T>(x[v]) : -INFINITY; }
+};
+// +inf as the type's largest (NaN never is at or above anything, what is made of it does not count)
+template <typename T> __device__ __forceinline__ float finite(float x) { return fminf(x, Limit<T>::most); }
 
-    __device__ Piece(const Args& args, Shared& shared, T* piece) :
-        a(args), sh(shared), data(piece), tid(threadIdx.x), warp(threadIdx.x >> 5), lane(threadIdx.x & 31), rank((int)cluster_ctarank()),
-        row((int)(blockIdx.x / args.ranks)) {}
-
-    template <typename V, typename Op> __device__ V over_block(V v, V* parts, Op op) {
+// what a block of kThreads does together
+struct Block {
+    const int tid, warp, lane;
+    double table;                   // 2^(lane / 32)
+    double scale = 0.0, base = 0.0; // w = 2^(x scale + base)
+    __device__ Block() : tid(threadIdx.x), warp(threadIdx.x >> 5), lane(threadIdx.x & 31) { table = kTable[threadIdx.x & 31]; }
+    __device__ __forceinline__ void relative_to(float top, double s) {
+        scale = s;
+        base = -(double)top * s;
+    }
+    template <typename T> __device__ __forceinline__ double weight(float x) const { return exp2_64(fma((double)finite<T>(x), scale, base), table); }
+    template <typename V, typename Op> __device__ V over(V v, V* parts, Op op) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kAll, v, o));
         if (lane == 0) parts[warp] = v;
@@ -181,118 +268,97 @@ struct Piece {
         __syncthreads();
         return v;
     }
-    // what the CTAs of the cluster have in a place: all on their way at once (between two cluster_sync)
-    template <typename V> __device__ __forceinline__ void of_all(V* place, V (&v)[kMostRanks], V none) {
-#pragma unroll
-        for (int c = 0; c < kMostRanks; ++c) v[c] = *peer(place, min(c, a.ranks - 1));
-#pragma unroll
-        for (int c = 1; c < kMostRanks; ++c)
-            if (c >= a.ranks) v[c] = none;
-    }
-    template <typename V, typename Op> __device__ __forceinline__ V over_cluster(V* place, Op op) {
-        V v[kMostRanks];
-        of_all(place, v, Op::template none<V>());
-#pragma unroll
-        for (int c = 1; c < kMostRanks; ++c) v[0] = op(v[0], v[c]);
-        return v[0];
-    }
-    __device__ __forceinline__ double warp_sum64(double v) {
+    __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
         return v;
     }
-    __device__ __forceinline__ float at(int slot) const { return widen<T>(data[slot]); }
+};
 
-    // ---- weights, by all lanes of a warp
-    __device__ __forceinline__ double weight(float x) const { return exp2_64(fma((double)x, scale, base), table); }
-    __device__ __forceinline__ double kept(float x) const {
-        const bool in = x >= border;
-        if (!__any_sync(kAll, in)) return 0.0;
-        const double w = weight(x);
-        return in ? w : 0.0;
+// a chunk's words, all on their way at once, into shared memory, where each is its thread's own; the largest that the thread has
+template <typename T> __device__ __forceinline__ float load_chunk(const View<T>& view, int s0, int s1, int warp, int lane, Word<T>* words) {
+    constexpr int N = Word<T>::N;
+    const T* from = view.x + view.token(s0 + warp, lane);
+    Word<T>* to = words + warp * 32 + lane;
+    if (view.whole(s0, s1 - s0)) {
+#pragma unroll 4
+        for (int s = s0 + warp; s < s1; s += kWarps, from += kWarps * View<T>::STRIP, to += kWarps * 32)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+    } else {
+        for (int s = s0 + warp; s < s1; s += kWarps) words[(s - s0) * 32 + lane] = view.load(s, lane);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    float m = -INFINITY;
+#pragma unroll 2
+    for (int s = s0 + warp; s < s1; s += kWarps) {
+        const Word<T> w = words[(s - s0) * 32 + lane];
+#pragma unroll
+        for (int e = 0; e < N; ++e) m = fmaxf(m, widen<T>(w.v[e]));
+    }
+    return m;
+}
+// sum += v where x is at or above `least`; mask |= bit where it is at or above `lo` and not that
+__device__ __forceinline__ void add_from(double& sum, double v, float x, float least) {
+    asm("{\n\t.reg .pred p;\n\tsetp.ge.f32 p, %1, %2;\n\t@p add.rn.f64 %0, %0, %3;\n\t}" : "+d"(sum) : "f"(x), "f"(least), "d"(v));
+}
+__device__ __forceinline__ void add_and_mark(double& sum, double v, float x, float least, float lo, uint32_t& mask, uint32_t bit) {
+    asm("{\n\t.reg .pred p, q;\n\tsetp.ge.f32 p, %2, %3;\n\tsetp.ge.and.f32 q, %2, %4, !p;\n\t@p add.rn.f64 %0, %0, %5;\n\t@q or.b32 %1, %1, %6;\n\t}"
+        : "+d"(sum), "+r"(mask) : "f"(x), "f"(least), "f"(lo), "d"(v), "r"(bit));
+}
 
-    // f(x, slot) for the warp's tokens, all lanes together
-    template <typename F> __device__ __forceinline__ void words(F f) const {
-        for (int s = s0; s < s1; ++s) {
-            const int j = s * STRIP + lane * N;
-            const Word<T> w = *reinterpret_cast<const Word<T>*>(data + j);
-#pragma unroll
-            for (int e = 0; e < N; ++e) f(widen<T>(w.v[e]), j + e);
-        }
+// ------------------------------------------------------------------------------------------------------------------- count
+template <typename T> __global__ void __launch_bounds__(kThreads, 6) count_kernel(const __grid_constant__ Args a) {
+    constexpr int N = Word<T>::N;
+    __shared__ Word<T> s_words[kMostChunkStrips * 4 / N * 32];
+    __shared__ uint4 s_hist[kBins / 4];
+    __shared__ float s_part[kWarps], s_fine;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, local = blockIdx.x / a.chunks, c = blockIdx.x - local * a.chunks, row = a.row0 + local;
+    let_next_start();
+    const View<T> view(a, row);
+    if (tid == 0) {                     // (one thread: its divisions take as long as a word of every other)
+        const Rules r(a, row);
+        s_fine = r.counts() ? r.fine : 0.f;
     }
-    // the weights of what is at or above `least` in a strip, or of lanes on neighbouring tokens (n of them)
-    __device__ __forceinline__ double strip_sum(int s, float least) const {
-        const Word<T> w = *reinterpret_cast<const Word<T>*>(data + s * STRIP + lane * N);
-        float x[N], m = -INFINITY;
+    const int s0 = c * a.chunk_strips, s1 = min(s0 + a.chunk_strips, view.strips);
+    s_hist[tid] = make_uint4(0, 0, 0, 0);
+    const float m0 = load_chunk<T>(view, s0, s1, warp, lane, s_words);
+    float m = m0;
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+    if (lane == 0) s_part[warp] = m;
+    __syncthreads();
+    m = s_part[0];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            x[e] = widen<T>(w.v[e]);
-            m = fmaxf(m, x[e]);
-        }
-        if (!__any_sync(kAll, m >= least)) return 0.0;
-        double sum = 0.0;
+    for (int i = 1; i < kWarps; ++i) m = fmaxf(m, s_part[i]);
+    m = finite<T>(m);
+    const float fine = s_fine;
+    if (fine > 0.f && m > -INFINITY) {
+        const uint32_t first = on_grid(m, fine) | (kParts - 1), one = 1u << kCountShift, hist = smem_u32(s_hist);
+#pragma unroll 2
+        for (int s = s0 + warp; s < s1; s += kWarps) {
+            const Word<T> w = s_words[(s - s0) * 32 + lane];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const double v = weight(x[e]);
-            sum += x[e] >= least ? v : 0.0;
+            for (int e = 0; e < N; ++e) {
+                const float x = widen<T>(w.v[e]);
+                const uint32_t d = below(first, x, fine);
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.gt.f32 p, %2, %3;\n\t@p red.shared.add.u32 [%0], %1;\n\t}"
+                             ::"r"(hist + (d / kParts) * 4), "r"(one | (d % kParts)), "f"(x), "f"(-INFINITY) : "memory");
+            }
         }
-        return sum;
+        __syncthreads();
+        reinterpret_cast<uint4*>(a.hist + (int64_t)blockIdx.x * kBins)[tid] = s_hist[tid];
     }
-    __device__ double kept_sum() {
-        double sum = 0.0;
-        for (int s = s0; s < s1; ++s) sum += strip_sum(s, border);
-        return join(sum);
-    }
+    if (tid == 0) a.chunk[blockIdx.x].top = m;
+}
 
-    // ---- the piece into shared memory, and the row's largest (NaN is never the larger, and never at or above anything)
-    __device__ void load() {
-        const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.stride;
-        const int V = a.vocab, first = min(V, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));     // tokens before the first whole word
-        const int whole = (V - first) / N, w0 = (int)((int64_t)whole * rank / a.ranks), w1 = (int)((int64_t)whole * (rank + 1) / a.ranks);
-        const int head = rank == 0 && first > 0, tail = rank == a.ranks - 1 && first + whole * N < V;
-        used = (w1 - w0 + head + tail) * N;
-        lo = first + (w0 - head) * N;
-        strips = (used + STRIP - 1) / STRIP;
-        s0 = strips * warp / kWarps;
-        s1 = strips * (warp + 1) / kWarps;
-        float m = -INFINITY;
-        const uint4* src = reinterpret_cast<const uint4*>(x + first) + w0;
-        uint4* dst = reinterpret_cast<uint4*>(data) + head;
-        constexpr int D = 8;                    // words on their way per thread
-        for (int i = tid; i < w1 - w0; i += D * kThreads) {
-            uint4 raw[D];
-#pragma unroll
-            for (int d = 0; d < D; ++d)
-                if (i + d * kThreads < w1 - w0) raw[d] = ldg_stream_128(src + i + d * kThreads);
-#pragma unroll
-            for (int d = 0; d < D; ++d)
-                if (i + d * kThreads < w1 - w0) {
-                    dst[i + d * kThreads] = raw[d];
-                    const Word<T> w = *reinterpret_cast<const Word<T>*>(&raw[d]);
-#pragma unroll
-                    for (int e = 0; e < N; ++e) m = fmaxf(m, widen<T>(w.v[e]));
-                }
-        }
-        auto edge = [&](int j) {                // token by token; what is not of the piece is -inf
-            const int v = lo + j;
-            const T t = v >= 0 && v < V && j < used ? x[v] : narrow<T>(-INFINITY);
-            data[j] = t;
-            m = fmaxf(m, widen<T>(t));
-        };
-        if (head && tid < N) edge(tid);
-        for (int j = used - tail * N + tid; j < strips * STRIP; j += kThreads) edge(j);
-        m = over_block(m, sh.fpart, Max());     // (its barriers also publish the piece)
-        if (tid == 0) sh.x_top = m;
-        cluster_sync();
-        top = over_cluster(&sh.x_top, Max());
-        if (top == INFINITY) {                  // as the type's largest
-            for (int j = tid; j < strips * STRIP; j += kThreads)
-                if (at(j) == INFINITY) data[j] = narrow<T>(Limit<T>::most);
-            top = Limit<T>::most;
-            __syncthreads();
-        }
-    }
+// ------------------------------------------------------------------------------------------------------------------- range
+struct WeighShared {
+    double part[kWarps], part2[kWarps];
+    float fpart[kWarps];
+    int ipart[kWarps], b_lo, b_hi, b_first, before_n, to_n;
+};
+struct Weigher : Block {
+    WeighShared& sh;
+    __device__ Weigher(WeighShared& s) : sh(s) {}
 
     // ---- where the border is, as far as counts tell: the steps that may hold it, of PER a thread.  counted(b): (tokens, parts); bounds(b, n, parts,
     // least, most): the weights that they have at least and at most; above, above_n: what is above the first step.  The border is where what is above it
@@ -385,9 +451,10 @@ struct Piece {
         __syncthreads();
     }
 
+
     // the least float whose step is below b (the steps fall while the floats grow), by a warp: 31 of them are tried at a time
-    template <typename F> __device__ float edge_of(int b, F place) const {
-        if (b <= 0) return INFINITY;
+    template <typename F> __device__ float edge_of(int b, float top, F place) const {
+        if (b <= 0) return NAN;                     // nothing is at or above it, nor infinity
         uint64_t l = key_of(kLowest), h = key_of(top);          // place(h) = 0 < b; the answer is in [l, h]
         while (l < h) {
             const uint64_t d = (h - l + 31) / 32, k = min(l + d * lane, h);
@@ -405,27 +472,369 @@ struct Piece {
         return of_key((uint32_t)h);
     }
 
-    // the n tokens that the CTAs have listed, in this one (the first)
-    __device__ void gather(int n, const int (&m)[kMostRanks]) {
-        for (int t = tid; t < n; t += kThreads) {
-            int c = 0, i = t;
+};
+
+template <typename T> __global__ void __launch_bounds__(kThreads) range_kernel(const __grid_constant__ Args a) {
+    __shared__ uint32_t s_n[kBins], s_q[kBins];
+    __shared__ WeighShared sh;
+    __shared__ float s_top[kWarps], s_edge[2], s_tops[kMostChunks];
+    Weigher b(sh);
+    const int local = blockIdx.x, row = a.row0 + local, tid = b.tid;
+    let_next_start();
+    const Rules r(a, row);
+    for (int i = tid; i < kBins; i += kThreads) s_n[i] = s_q[i] = 0;
+    wait_for_last();
+    const Chunk* chunk = a.chunk + (int64_t)local * a.chunks;
+    float top = -INFINITY;
+    for (int c = tid; c < a.chunks; c += kThreads) top = fmaxf(top, s_tops[c] = chunk[c].top);
+    top = b.over(top, s_top, Max());
+    Row out{};
+    out.top = top;
+    out.settled = 1;
+    out.only = -1;
+    b.relative_to(top, r.scale);
+    const float floor = r.greedy() ? top : r.floor(top), least = r.greedy() ? top : r.least(top);
+    out.up = out.lo = fmaxf(floor, least);              // nothing but min_p
+    if (r.greedy()) out.up = NAN;
+    const float t0 = top * r.fine;
+    if (top > -INFINITY && (r.k > 0 || r.p < 1.0) && !r.greedy()) {
+        if (!r.counts() || !(fabsf(t0) < 2097152.f)) out.settled = 0;
+        else {
+            const uint32_t g0 = on_grid(top, r.fine) | (kParts - 1), one = 1u << kCountShift;
+            const float log2_w = (float)(r.scale / r.fine), end = __uint_as_float(g0) - kMagic - t0, err = 0.5f + (fabsf(t0) + kBins * kParts) * 1.3e-7f;
+            constexpr int SOME = 8;                     // chunks whose words are on their way at once
+            for (int c0 = 0; c0 < a.chunks; c0 += SOME) {
+                uint32_t h[SOME][kPer];
+                int off[SOME];
 #pragma unroll
-            for (int k = 0; k < kMostRanks - 1; ++k)
-                if (c == k && i >= m[k]) {
-                    i -= m[k];
-                    c = k + 1;
+                for (int k = 0; k < SOME; ++k) {
+                    const float m = c0 + k < a.chunks ? s_tops[c0 + k] : -INFINITY;
+                    off[k] = (int)(min(g0 - (on_grid(m, r.fine) | (kParts - 1)), (uint32_t)(kBins * kParts - 1)) / kParts);
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i)
+                        h[k][i] = m > -INFINITY ? __ldcg(a.hist + ((int64_t)local * a.chunks + c0 + k) * kBins + tid + i * kThreads) : 0u;
                 }
-            sh.many[t] = peer(sh.list + i, c)->x;
+#pragma unroll
+                for (int k = 0; k < SOME; ++k)
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i)
+                        if (h[k][i]) {
+                            const int at = min(tid + i * kThreads + off[k], kBins - 1);
+                            atomicAdd(s_n + at, h[k][i] >> kCountShift);
+                            atomicAdd(s_q + at, h[k][i] & (one - 1u));
+                        }
+            }
+            __syncthreads();
+            auto counted = [&](uint32_t (&n)[kPer], uint32_t (&q)[kPer]) {
+#pragma unroll
+                for (int i = 0; i < kPer; i += 4) {
+                    const uint4 u = reinterpret_cast<const uint4*>(s_n)[tid * (kPer / 4) + i / 4], v = reinterpret_cast<const uint4*>(s_q)[tid * (kPer / 4) + i / 4];
+                    n[i] = u.x; n[i + 1] = u.y; n[i + 2] = u.z; n[i + 3] = u.w;
+                    q[i] = v.x; q[i + 1] = v.y; q[i + 2] = v.z; q[i + 3] = v.w;
+                }
+            };
+            // a token lies by d parts below the end of the first step, on the mean as many as the parts say, within half of one and the rounding of
+            // its product (err); w falls by at most a 6e-5th of itself more than evenly between the ends of a step
+            auto bounds = [&](int i, uint32_t n, uint32_t q, double& l, double& m) {
+                const float mean = end - i * kParts - (n ? __fdividef((float)q, (float)n) : 0.f);
+                m = n * (double)exp2f((mean + err) * log2_w) * (1.0 + 8e-5);
+                l = i == kBins - 1 ? 0.0 : n * (double)exp2f((mean - err) * log2_w) * (1.0 - 2e-5);
+            };
+            auto place = [&](float x) { return (int)(below(g0, x, r.fine) / kParts); };
+            int from = 0, to = 0;
+            bool few = false;
+            if (r.k > 0) {
+                b.weigh<false, kPer>(false, (double)r.k, 0.0, 0, from, to, counted, bounds);
+                few = sh.to_n <= kFew;                  // all that can be kept are few: listed, not summed
+                if (!few && r.p < 1.0) out.settled = 0; // (a share of many: of those from a border that is not known yet)
+            } else {
+                b.weigh<true, kPer>(true, r.p, 0.0, 0, from, to, counted, bounds);
+            }
+            if (b.warp < 2) {
+                const float e = b.warp == 0 ? (few ? NAN : b.edge_of(from, top, place)) : (to == kBins - 1 ? floor : b.edge_of(to + 1, top, place));
+                if (b.lane == 0) s_edge[b.warp] = e;
+            }
+            __syncthreads();
+            out.up = s_edge[0];
+            out.lo = fmaxf(s_edge[1], floor);
+            out.above_n = few ? 0 : sh.before_n;
+            if (least >= out.up) out.up = out.lo = least;           // min_p keeps less: its border is the border
         }
-        __syncthreads();
     }
+    out.all = out.settled && !r.greedy() && r.p < 1.0 && !(r.k > 0) && !(out.lo >= out.up);
+    out.floor = floor;
+    out.scale = r.scale;
+    if (tid == 0) a.row[local] = out;
+}
+
+// --------------------------------------------------------------------------------------------------------------------- sum
+template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(const __grid_constant__ Args a) {
+    constexpr int N = Word<T>::N;
+    __shared__ Word<T> s_words[kMostChunkStrips * 4 / N * 32];
+    __shared__ Near s_list[kList];
+    __shared__ double s_above[kWarps], s_whole[kWarps];
+    __shared__ float s_lo[kWarps], s_hi[kWarps], s_top[kWarps];
+    __shared__ int s_listed, s_first;
+    Block b;
+    const int tid = b.tid, warp = b.warp, lane = b.lane, local = blockIdx.x / a.chunks, c = blockIdx.x - local * a.chunks, row = a.row0 + local;
+    let_next_start();
+    const View<T> view(a, row);
+    __shared__ Row s_row;
+    const int s0 = c * a.chunk_strips, s1 = min(s0 + a.chunk_strips, view.strips);
+    if (tid == 0) {
+        s_listed = 0;
+        s_first = INT_MAX;
+        if (a.ranked) {
+            wait_for_last();
+            s_row = a.row[local];
+            if (!s_row.settled) s_row.up = s_row.lo = NAN;
+        }
+    }
+    const float mine_top = load_chunk<T>(view, s0, s1, warp, lane, s_words);
+    if (!a.ranked) {                    // temperatures alone: relative to the chunk's own largest
+        const float m = finite<T>(b.over(mine_top, s_top, Max()));
+        if (tid == 0) {
+            const Rules r(a, row);
+            s_row.top = m;
+            s_row.scale = r.scale;
+            s_row.floor = s_row.up = s_row.lo = r.floor(m);
+            if (r.greedy()) s_row.up = NAN, s_row.lo = m;
+            s_row.all = 0;
+        }
+    }
+    __syncthreads();
+    const float up = s_row.up, lo = s_row.lo, top = s_row.top, floor = s_row.all ? s_row.floor : lo;
+    const bool all = s_row.all, lists = !(lo >= up);    // also what is below; whether any is listed
+    b.relative_to(top, s_row.scale);
+    double above = 0.0, whole = 0.0;
+    float least_x = INFINITY, most_x = -INFINITY;
+    if (top > -INFINITY) {
+        for (int s = s0 + warp; s < s1; s += kWarps) {
+            const Word<T> w = s_words[(s - s0) * 32 + lane];
+            float x[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = widen<T>(w.v[e]);
+            uint32_t mine = 0;
+            if (all) {                  // (no infinity: range has left such rows to finish; what has no weight, or is no number: 2^-1021)
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const double v = exp2_64(fma((double)fmaxf(x[e], floor), b.scale, b.base), b.table);
+                    whole += v;
+                    add_and_mark(above, v, x[e], up, lo, mine, 1u << e);
+                }
+            } else {
+                float m = x[0];
+#pragma unroll
+                for (int e = 1; e < N; ++e) m = fmaxf(m, x[e]);
+                if (!__any_sync(kAll, m >= floor)) continue;
+                if (up == up && __any_sync(kAll, m >= up)) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) add_and_mark(above, b.weight<T>(x[e]), x[e], up, lo, mine, 1u << e);
+                } else if (lists) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) mine |= (uint32_t)(x[e] >= lo && !(x[e] >= up)) << e;
+                }
+            }
+            if (!lists) continue;
+            if (mine) {
+                int at = atomicAdd(&s_listed, __popc(mine));
+                const int v = view.token(s, lane);
+                atomicMin(&s_first, v + __ffs(mine) - 1);
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (mine >> e & 1u) {
+                        const float y = finite<T>(x[e]);
+                        least_x = fminf(least_x, y);
+                        most_x = fmaxf(most_x, y);
+                        if (at < kList) s_list[at] = Near{y, v + e};
+                        ++at;
+                    }
+            }
+            __syncwarp();
+        }
+    }
+    above = b.warp_sum(above);
+    if (all) whole = b.warp_sum(whole);
+    if (lists)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            least_x = fminf(least_x, __shfl_xor_sync(kAll, least_x, o));
+            most_x = fmaxf(most_x, __shfl_xor_sync(kAll, most_x, o));
+        }
+    if (lane == 0) {
+        s_above[warp] = above;
+        s_whole[warp] = whole;
+        s_lo[warp] = least_x;
+        s_hi[warp] = most_x;
+    }
+    __syncthreads();
+    const int listed = s_listed;
+    if (tid < min(listed, kList)) a.list[(int64_t)blockIdx.x * kList + tid] = s_list[tid];
+    if (tid == 0) {
+        Chunk out{};
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            out.above += s_above[i];
+            out.whole += s_whole[i];
+            least_x = fminf(least_x, s_lo[i]);
+            most_x = fmaxf(most_x, s_hi[i]);
+        }
+        out.top = top;
+        out.lo = least_x;
+        out.hi = most_x;
+        out.listed = listed;
+        out.first = s_first;
+        a.chunk[blockIdx.x] = out;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------ finish
+template <typename Q> __device__ __forceinline__ const Q* draft_row(const Args& a, int row) {       // (of a node that has one)
+    return static_cast<const Q*>(a.draft) + (int64_t)(a.draft_rows ? a.draft_rows[row] : row) * a.draft_stride;
+}
+
+struct Verdict {                    // of the cluster's first CTA
+    float up, lo;                   // what is at or above `up` is summed, what is at or above `lo` listed
+    float r_lo, r_hi, border, top;
+    double above, limit, total;
+    int above_n, done, halve, only, settled;
+};
+
+struct Shared : WeighShared {
+    union {
+        uint4 hist[kBins / 4];
+        float many[kMany];          // listed tokens of the row
+        int32_t child[PA_TREE_MOST_NODES];
+    };
+    union {
+        Near list[kList];
+        double strip[kMostStrips];  // sums of a part's strips
+    };
+    union {
+        double few_w[kFew];
+        uint32_t fine[kThreads];
+    };
+    float few[kFew];
+    double chunk[kMostChunks];      // sums of the chunks, in the row's order
+    int first[kMostChunks + 1];     // listed tokens of the chunks before
+    double seg[kWarps];             // or of the warps' parts of this CTA's share of the row
+    float fpart2[kWarps], fpart3[kWarps];
+    int listed, children, hit;
+    // what the other CTAs of the cluster read
+    Verdict verdict;
+    float x_lo, x_hi, x_up;
+    int x_listed;
+    double x_below, x_above, x_total[2];
+};
+
+template <typename T, typename Q, int MODE>
+struct Finish : Weigher {
+    static constexpr int N = Word<T>::N, STRIP = 32 * N;
+    const Args& a;
+    Shared& sh;
+    const int rank, local, row;
+    const View<T> view;
+    uint32_t* const gone;           // a bit per token that was drawn (where several are drawn)
+    int s0, s1;                     // strips of this warp's part
+    float top, border;              // the largest; the least value that is kept
+    int only = -1;                  // temperature 0: the one token that is kept
+    int turn = 0;                   // of x_total
+    bool by_chunks = true;          // the sums are the chunks', in the first CTA
+    bool left = false;              // has arrived at the last barrier
+
+    __device__ Finish(const Args& args, Shared& shared, uint32_t* bits) :
+        Weigher(shared), a(args), sh(shared), rank((int)cluster_ctarank()), local((int)(blockIdx.x / args.ranks)), row(args.row0 + local), view(args, row), gone(bits) {
+        const int parts = a.ranks * kWarps, part = rank * kWarps + warp;
+        s0 = (int)((int64_t)view.strips * part / parts);
+        s1 = (int)((int64_t)view.strips * (part + 1) / parts);
+    }
+
+    // what the CTAs of the cluster have in a place: all on their way at once (between two cluster_sync)
+    template <typename V> __device__ __forceinline__ void of_all(V* place, V (&v)[kMostRanks], V none) {
+#pragma unroll
+        for (int c = 0; c < kMostRanks; ++c) v[c] = *peer(place, min(c, a.ranks - 1));
+#pragma unroll
+        for (int c = 1; c < kMostRanks; ++c)
+            if (c >= a.ranks) v[c] = none;
+    }
+    template <typename V, typename Op> __device__ __forceinline__ V over_cluster(V* place, Op op) {
+        V v[kMostRanks];
+        of_all(place, v, Op::template none<V>());
+#pragma unroll
+        for (int c = 1; c < kMostRanks; ++c) v[0] = op(v[0], v[c]);
+        return v[0];
+    }
+
+    // ---- weights, by all lanes of a warp
+    __device__ __forceinline__ double weight(float x) const { return Block::weight<T>(x); }
+    __device__ __forceinline__ double kept(float x, int v) const {
+        bool in = x >= border && (only < 0 || v == only);
+        if (gone && in) in = !(gone[v >> 5] >> (v & 31) & 1u);
+        if (!__any_sync(kAll, in)) return 0.0;
+        const double w = weight(x);
+        return in ? w : 0.0;
+    }
+    // the weights of a word's tokens, v and on
+    __device__ __forceinline__ void kept_of(const Word<T>& x, int v, double (&w)[N]) const {
+        uint32_t in = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) in |= (uint32_t)(widen<T>(x.v[e]) >= border) << e;
+        if (only >= 0) in &= only >= v && only < v + N ? 1u << (only - v) : 0u;
+        if (gone && in)
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (in >> e & 1u) in &= ~((gone[(v + e) >> 5] >> ((v + e) & 31) & 1u) << e);
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = 0.0;
+        if (!__any_sync(kAll, in != 0)) return;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const double u = weight(widen<T>(x.v[e]));
+            w[e] = in >> e & 1u ? u : 0.0;
+        }
+    }
+    __device__ __forceinline__ double word_sum(const Word<T>& x, int v) const {
+        double w[N], sum = 0.0;
+        kept_of(x, v, w);
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum += w[e];
+        return sum;
+    }
+    __device__ double kept_sum() {
+        double sum = 0.0;
+        view.template each<4>(s0, s1, 1, lane, [&](const Word<T>& x, int, int v) { sum += word_sum(x, v); });
+        return join(sum);
+    }
+    // ---- the parts' sums, and the whole row's
+    __device__ double join(double sum) {
+        sum = warp_sum(sum);
+        if (lane == 0) sh.seg[warp] = sum;
+        return joined();
+    }
+    __device__ double joined() {
+        by_chunks = false;
+        __syncthreads();
+        publish();
+        cluster_sync();
+        return over_cluster(&sh.x_total[turn], Add());
+    }
+    __device__ void publish() {
+        turn ^= 1;              // two places in turn: others may still read the last one
+        if (tid == 0) {
+            double t = 0.0;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) t += sh.seg[w];
+            sh.x_total[turn] = t;
+        }
+    }
+
     // the weights of n few tokens; the sum of those at or above `least`
     __device__ double weights_of_few(int n, float least) {
         const float x = tid < n ? sh.few[tid] : -INFINITY;
         double w = weight(x);
         w = tid < n && x >= least ? w : 0.0;
         sh.few_w[tid] = w;
-        return over_block(w, sh.part, Add());
+        return over(w, sh.part, Add());
     }
     // the border among n few tokens, each of which sums (or counts) what is above it: of those at or above `least`
     template <bool MASS> __device__ float among(int n, float least, double above, int above_n, double limit) {
@@ -443,7 +852,7 @@ struct Piece {
                 }
             }
         const bool in = x >= least && tid < n && (MASS ? sum[0] + sum[1] + (sum[2] + sum[3]) < limit : count < limit);
-        const float low = over_block(in ? x : INFINITY, sh.fpart, Min()), most = over_block(x, sh.fpart, Max());
+        const float low = over(in ? x : INFINITY, sh.fpart, Min()), most = over(x, sh.fpart, Max());
         return fminf(low, most);                    // the largest is kept in any case
     }
     // the border among up to kMany tokens, [l, h]: by a finer count, if they are not few; NaN: they are not, nor will they be
@@ -502,113 +911,70 @@ struct Piece {
                     high = fmaxf(high, x);
                 }
             }
-            if (MASS) above += over_block(sum, sh.part, Add());
-            l = over_block(low, sh.fpart, Min());
-            h = over_block(high, sh.fpart, Max());
+            if (MASS) above += over(sum, sh.part, Add());
+            l = over(low, sh.fpart, Min());
+            h = over(high, sh.fpart, Max());
         }
         return NAN;
     }
 
     // ---- the border: the least value that is kept of those from `least` on.  With MASS the weights above it are below `share` of all, else fewer
-    // than `share` tokens are above it; the largest is kept in any case.  Where few are counted, these are also cut to share p of their weights
-    // (p below 1).  Returns the value from which on sh.seg has summed all (asked for by `sums`, or MASS), the rest of it with what is listed;
-    // infinity: all are listed; NaN: neither.
-    template <bool MASS> __device__ float find(double share, float least, bool sums, double p, bool& ruled) {
-        Verdict r;                              // R = [r_lo, r_hi] holds the border, `above` and above_n are above R
+    // than `share` tokens are above it; the largest is kept in any case.  By steps of floats, 1024 at a time; what is above those that may hold it
+    // is summed exactly.  Returns the value from which on sh.seg has summed all (asked for by `sums`, or MASS), the rest of it with what is listed;
+    // NaN: it has not.
+    template <bool MASS> __device__ float find(double share, float least, bool sums) {
+        Verdict r{};                            // R = [r_lo, r_hi] holds the border, `above` and above_n are above R
         r.r_lo = least;
         r.r_hi = top;
-        r.above = 0.0;
-        r.above_n = 0;
         r.limit = share;
-        r.halve = 0;
-        const float step = (float)(scale * kSteps), parts = a.parts;
-        // steps of 1/32 in log2 w to begin with, rounded to the nearest; by floats where these would be too coarse or too fine, and afterwards
-        bool first = true, by_logs = scale > 1e-6 && scale < 1e6;
+        bool first = true;
         for (int level = 0; level < 128; ++level) {
             const uint32_t k_hi = key_of(r.r_hi) >> Limit<T>::spare, range = k_hi - (key_of(r.r_lo) >> Limit<T>::spare);
             const int bits = 32 - __clz(range), shift = bits > 10 ? bits - 10 : 0;
-            auto by_log = [&](float x) { return fminf((top - x) * step, kBins - 1.f); };
-            auto place = [&](float x) -> int {
-                if (by_logs) return __float_as_int(by_log(x) + 8388608.f) & (kBins - 1);
-                return (int)((k_hi - (key_of(x) >> Limit<T>::spare)) >> shift) & (kBins - 1);
-            };
+            cluster_sync();                     // the last verdict, and this CTA's counts, have been read
             if (!r.halve) {
-                for (int i = tid; i < kBins / 4; i += kThreads) sh.hist[i] = make_uint4(0, 0, 0, 0);
+                sh.hist[tid] = make_uint4(0, 0, 0, 0);
                 __syncthreads();
-                const uint32_t hist = smem_u32(sh.hist), one = 1u << a.count_shift;
+                const uint32_t hist = smem_u32(sh.hist);
                 for (int s = s0; s < s1; ++s) {
-                    const Word<T> w = *reinterpret_cast<const Word<T>*>(data + s * STRIP + lane * N);
+                    const Word<T> w = view.load(s, lane);
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
-                        const float x = widen<T>(w.v[e]);
-                        uint32_t at = hist, add = one;
-                        if (by_logs) {
-                            const float d = by_log(x), up = d + 8388608.f;
-                            at += (__float_as_uint(up) & (kBins - 1)) * 4;
-                            if (MASS) add += __float_as_uint(fmaf(d - (up - 8388608.f), parts, 8388608.f + 0.5f * parts)) & 0x7fffffu;
-                        } else {
-                            at += place(x) * 4;
-                        }
-                        if (x >= r.r_lo && x <= r.r_hi) asm volatile("red.shared.add.u32 [%0], %1;" ::"r"(at), "r"(add) : "memory");
+                        const float x = finite<T>(widen<T>(w.v[e]));
+                        const uint32_t b = ((k_hi - (key_of(x) >> Limit<T>::spare)) >> shift) & (kBins - 1);
+                        if (widen<T>(w.v[e]) >= r.r_lo && x <= r.r_hi) asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(hist + 4 * b) : "memory");
                     }
                 }
                 cluster_sync();
                 if (rank == 0) {
                     int from, to;
-                    auto counted = [&](uint32_t (&n)[kPer], uint32_t (&q)[kPer]) {
+                    auto counted = [&](uint32_t (&n)[4], uint32_t (&q)[4]) {
                         uint4 h[kMostRanks];
                         of_all(sh.hist + tid, h, make_uint4(0, 0, 0, 0));
 #pragma unroll
-                        for (int e = 0; e < kPer; ++e) n[e] = q[e] = 0;
-#pragma unroll
-                        for (int c = 0; c < kMostRanks; ++c) {
-                            const uint32_t w[4] = {h[c].x, h[c].y, h[c].z, h[c].w};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                n[k] += w[k] >> a.count_shift;
-                                q[k] += w[k] & (one - 1u);
-                            }
+                        for (int c = 1; c < kMostRanks; ++c) {
+                            h[0].x += h[c].x; h[0].y += h[c].y; h[0].z += h[c].z; h[0].w += h[c].w;
                         }
+                        n[0] = h[0].x; n[1] = h[0].y; n[2] = h[0].z; n[3] = h[0].w;
+                        q[0] = q[1] = q[2] = q[3] = 0;
                     };
-                    // d of a step's tokens: b + what their parts say, within half a part; w = 2^(-d/32) falls by at most a 6e-5th of itself more than
-                    // evenly between the ends of a step, and (top - x) step is rounded by 1024 x 2^-22 of a step
-                    const float half = parts > 0.f ? 0.5f / parts : 0.5f;
-                    auto by_step = [&](int b, uint32_t n, uint32_t q, double& l, double& m) {
-                        const float mean = parts > 0.f && n ? (__fdividef((float)q, (float)n) - 0.5f * parts) * (2.f * half) : 0.f;
-                        m = n * (double)exp2f((half - mean - b) * (1.f / kSteps)) * (1.0 + 8e-5);
-                        l = b == kBins - 1 ? 0.0 : n * (double)exp2f((-half - mean - b) * (1.f / kSteps)) * (1.0 - 2e-5);
-                    };
-                    auto by_float = [&](int b, uint32_t n, uint32_t, double& l, double& m) {
+                    auto bounds = [&](int b, uint32_t n, uint32_t, double& l, double& m) {
                         const uint64_t k0 = min((uint64_t)b << shift, (uint64_t)range), k1 = min(((uint64_t)(b + 1) << shift) - 1, (uint64_t)range);
-                        const double w0 = weight(of_spared(k_hi - (uint32_t)k0)), w1 = weight(of_spared(k_hi - (uint32_t)k1));
-                        m = n * w0 * (shift ? 1.0 + 1e-10 : 1.0);
-                        l = n * w1 * (shift ? 1.0 - 1e-10 : 1.0);
+                        m = n * weight(of_spared(k_hi - (uint32_t)k0)) * (1.0 + 1e-10);
+                        l = n * weight(of_spared(k_hi - (uint32_t)k1)) * (1.0 - 1e-10);
                     };
-                    if (by_logs) weigh<MASS, kPer>(first, r.limit, r.above, r.above_n, from, to, counted, by_step);
-                    else weigh<MASS, kPer>(first, r.limit, r.above, r.above_n, from, to, counted, by_float);
-                    const bool all_few = !MASS && first && sh.to_n <= kFew;         // all that can be kept are few: listed, not summed
-                    if (by_logs) {
-                        if (warp == 0) {
-                            const float e = all_few ? INFINITY : edge_of(from, place);
-                            if (lane == 0) sh.verdict.up = e;
-                        } else if (warp == 1) {
-                            const float e = to == kBins - 1 ? r.r_lo : fmaxf(edge_of(to + 1, place), r.r_lo);
-                            if (lane == 0) sh.verdict.lo = e;
-                        }
-                    } else if (tid == 0) {
+                    weigh<MASS, 4>(first, r.limit, r.above, r.above_n, from, to, counted, bounds);
+                    if (tid == 0) {
                         const uint64_t k = (uint64_t)(to + 1) << shift;
-                        sh.verdict.up = all_few ? INFINITY : from == 0 ? above_of(r.r_hi) : of_spared(k_hi - (uint32_t)(((uint64_t)from << shift) - 1));
+                        sh.verdict.up = from == 0 ? (r.r_hi < Limit<T>::most ? of_key(key_of(r.r_hi) + 1u) : NAN) : of_spared(k_hi - (uint32_t)(((uint64_t)from << shift) - 1));
                         sh.verdict.lo = k > range ? r.r_lo : fmaxf(of_spared(k_hi - (uint32_t)k + 1), r.r_lo);
+                        sh.verdict.above_n = sh.before_n;
                     }
-                    if (tid == 0) sh.verdict.above_n = all_few ? 0 : sh.before_n;
                 }
-            } else {                                        // the bounds did not help: by halves, whose weights are summed
-                cluster_sync();                             // the last verdict has been read
-                if (rank == 0 && tid == 0) {
-                    sh.verdict.up = of_spared(k_hi - range / 2);
-                    sh.verdict.lo = r.r_lo;
-                    sh.verdict.above_n = r.above_n;
-                }
+            } else if (rank == 0 && tid == 0) {             // the bounds did not help: by halves, whose weights are summed
+                sh.verdict.up = of_spared(k_hi - range / 2);
+                sh.verdict.lo = r.r_lo;
+                sh.verdict.above_n = r.above_n;
             }
             cluster_sync();
             const float up = peer(&sh.verdict, 0)->up, near = peer(&sh.verdict, 0)->lo;
@@ -620,8 +986,8 @@ struct Piece {
             float least_x = INFINITY, most_x = -INFINITY, least_up = INFINITY;
             const float floor = MASS && first ? least : near;
             for (int s = s0; s < s1; ++s) {
-                const int j = s * STRIP + lane * N;
-                const Word<T> w = *reinterpret_cast<const Word<T>*>(data + j);
+                const Word<T> w = view.load(s, lane);
+                const int v = view.token(s, lane);
                 float x[N], m = -INFINITY;
                 uint32_t mine = 0;
 #pragma unroll
@@ -630,18 +996,12 @@ struct Piece {
                     m = fmaxf(m, x[e]);
                 }
                 if (!__any_sync(kAll, m >= floor)) continue;
-                if (MASS && first) {
+                if ((MASS && first) || ((MASS || sums) && __any_sync(kAll, m >= up))) {
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
-                        const double v = weight(x[e]);
-                        sum += x[e] >= up ? v : 0.0;
-                        below += x[e] >= floor && !(x[e] >= up) ? v : 0.0;
-                    }
-                } else if ((MASS || sums) && __any_sync(kAll, m >= up)) {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const double v = weight(x[e]);
-                        sum += x[e] >= up ? v : 0.0;
+                        const double u = weight(x[e]);
+                        sum += x[e] >= up ? u : 0.0;
+                        if (MASS && first) below += x[e] >= floor && !(x[e] >= up) ? u : 0.0;
                         if (r.halve && x[e] >= up && x[e] <= r.r_hi) least_up = fminf(least_up, x[e]);
                     }
                 }
@@ -652,21 +1012,22 @@ struct Piece {
 #pragma unroll
                     for (int e = 0; e < N; ++e)
                         if (mine >> e & 1u) {
-                            least_x = fminf(least_x, x[e]);
-                            most_x = fmaxf(most_x, x[e]);
-                            if (at < kList) sh.list[at] = Near{x[e], j + e};
+                            const float y = finite<T>(x[e]);
+                            least_x = fminf(least_x, y);
+                            most_x = fmaxf(most_x, y);
+                            if (at < kList) sh.list[at] = Near{y, v + e};
                             ++at;
                         }
                 }
                 __syncwarp();
             }
-            sum = warp_sum64(sum);
-            if (MASS && first) below = warp_sum64(below);
+            sum = warp_sum(sum);
+            below = warp_sum(below);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
                 least_x = fminf(least_x, __shfl_xor_sync(kAll, least_x, o));
                 most_x = fmaxf(most_x, __shfl_xor_sync(kAll, most_x, o));
-                if (r.halve) least_up = fminf(least_up, __shfl_xor_sync(kAll, least_up, o));
+                least_up = fminf(least_up, __shfl_xor_sync(kAll, least_up, o));
             }
             if (lane == 0) {
                 sh.seg[warp] = sum;
@@ -705,192 +1066,295 @@ struct Piece {
                 }
                 const double above = MASS ? over_cluster(&sh.x_above, Add()) : 0.0;
                 const double limit = MASS && first ? share * (above + over_cluster(&sh.x_below, Add())) : r.limit;
-                const float l = over_cluster(&sh.x_lo, Min()), h = over_cluster(&sh.x_hi, Max()), u = r.halve ? over_cluster(&sh.x_up, Min()) : 0.f;
+                const float l = over_cluster(&sh.x_lo, Min()), h = over_cluster(&sh.x_hi, Max()), u = over_cluster(&sh.x_up, Min());
                 const bool upper = MASS && r.halve && above >= limit;            // the border is in the upper half
-                const bool many = !upper && n <= kMany && most <= kList, rules_too = !MASS && up == INFINITY && many && n <= kFew;
                 float found = NAN;
-                if (l == h && !upper && !rules_too) found = l;
-                else if (many) {
-                    int few;
-                    gather(n, listed);
-                    found = select<MASS>(n, l, h, above, above_n, limit, few);
-                    if (rules_too && p < 1.0) {
-                        if (few == 0) {                     // (all alike)
-                            sh.few[tid] = tid < n ? sh.many[tid] : -INFINITY;
-                            __syncthreads();
-                        }
-                        const double all = weights_of_few(n, found);
-                        found = among<true>(n, found, 0.0, 0, p * all);
+                if (l == h && !upper) found = l;
+                else if (!upper && n <= kMany && most <= kList) {
+                    int few, from = 0;
+#pragma unroll
+                    for (int c = 0; c < kMostRanks; ++c) {
+                        if (tid < listed[c]) sh.many[from + tid] = peer(sh.list + tid, min(c, a.ranks - 1))->x;
+                        from += listed[c];
                     }
+                    __syncthreads();
+                    found = select<MASS>(n, l, h, above, above_n, limit, few);
                 }
                 if (tid == 0) {
                     Verdict& v = sh.verdict;
                     v.border = found;
                     v.done = found == found;
-                    v.ruled = rules_too;
                     v.r_lo = upper ? u : l;
                     v.r_hi = upper ? r.r_hi : h;
                     v.above = upper ? r.above : above;
                     v.above_n = above_n;
                     v.limit = limit;
-                    v.halve = MASS && !by_logs && !r.halve && !v.done &&
-                              key_of(v.r_hi) - key_of(v.r_lo) > (key_of(r.r_hi) - key_of(r.r_lo)) / 2;
+                    v.halve = MASS && !r.halve && !v.done && key_of(v.r_hi) - key_of(v.r_lo) > (key_of(r.r_hi) - key_of(r.r_lo)) / 2;
                 }
             }
             cluster_sync();
-            const Verdict v = *peer(&sh.verdict, 0);
-            border = v.border;
-            ruled = v.ruled;
-            if (v.done) {
-                if (!(MASS || sums || up == INFINITY)) return NAN;
-                return sh.listed > kList ? NAN : up;
-            }
-            r.r_lo = v.r_lo;
-            r.r_hi = v.r_hi;
-            r.above = v.above;
-            r.above_n = v.above_n;
-            r.limit = v.limit;
-            r.halve = v.halve;
-            by_logs = first = false;
+            r = *peer(&sh.verdict, 0);
+            border = r.border;
+            if (r.done) return (MASS || sums) && sh.listed <= kList ? up : NAN;
+            first = false;
         }
         return NAN;
     }
+    __device__ __forceinline__ float of_spared(uint32_t k) const {             // the least float of a key without its spare bits
+        const uint32_t full = k << Limit<T>::spare;
+        return of_key(full & 0x80000000u ? full : full | ((1u << Limit<T>::spare) - 1u));      // (negative numbers have ones there as keys)
+    }
     // the listed tokens that are kept, to the parts that they are in
     __device__ void add_listed() {
+        const int v0 = view.token(s0, 0), v1 = view.token(s1, 0);
         double more = 0.0;
         for (int i = 0; i < sh.listed; i += 32) {
             const Near one = i + lane < sh.listed ? sh.list[i + lane] : Near{-INFINITY, 0};
-            const bool mine = one.x >= border && one.slot >= s0 * STRIP && one.slot < s1 * STRIP;
+            const bool mine = one.x >= border && one.token >= v0 && one.token < v1;
             if (__any_sync(kAll, mine)) {
                 const double w = weight(one.x);
                 more += mine ? w : 0.0;
             }
         }
-        more = warp_sum64(more);
+        more = warp_sum(more);
         if (lane == 0) sh.seg[warp] += more;
     }
-    __device__ __forceinline__ float of_spared(uint32_t k) const {             // the least float of a key without its spare bits
-        const uint32_t full = k << Limit<T>::spare;
-        // (negative numbers have ones in their spare bits as keys)
-        return of_key(full & 0x80000000u ? full : full | ((1u << Limit<T>::spare) - 1u));
-    }
-    __device__ __forceinline__ float above_of(float x) const { return of_key(key_of(x) + 1u); }
-
-    // ---- the rules of the row's sequence: the border, and the sums of what is kept.  The total
+    // ---- the border and the sums: from what the kernels before have left, or, where that does not settle it, from the row
     __device__ double rules() {
-        const int b = a.row_seq ? a.row_seq[row] : row;
-        const bool known = (unsigned)b < (unsigned)a.num_seqs;
-        const double t = !known ? 1.0 : a.temperature ? (double)a.temperature[b] : a.temperature1;
-        const double p = !known ? 1.0 : a.top_p ? (double)a.top_p[b] : a.top_p1, m = !known ? 0.0 : a.min_p ? (double)a.min_p[b] : a.min_p1;
-        const int k = !known ? 0 : a.top_k ? a.top_k[b] : a.top_k1;
-        only = -1;
-        if (!(t > 0.0)) {
-            int v = INT_MAX;
-            words([&](float x, int j) { if (x == top) v = min(v, lo + j); });
-            v = over_block(v, sh.ipart, Min());
-            if (tid == 0) sh.x_first = v;
-            cluster_sync();
-            only = over_cluster(&sh.x_first, Min());
-            words([&](float x, int j) { if (x == top && lo + j != only) data[j] = narrow<T>(-INFINITY); });
-            __syncwarp();
-            border = top;
-            scale = base = 0.0;
-            return kept_sum();
-        }
-        scale = 1.4426950408889634074 / t;
-        base = -(double)top * scale;
-        border = at_least((double)top - 1021.0 / scale);                // what has no weight in 64 bits
-        const float least = !(m > 0.0) ? kLowest : m >= 1.0 ? (t < INFINITY ? top : kLowest) : at_least((double)top + t * log(m));      // w >= m
+        const Rules r(a, row);
+        wait_for_last();
+        if (rank == 0) settle(r);
+        cluster_sync();
+        const Verdict v = *peer(&sh.verdict, 0);
+        top = v.top;
+        border = v.border;
+        only = v.only;
+        relative_to(top, r.scale);
+        if (!(top > -INFINITY) || v.settled) return v.total;
+        border = r.floor(top);
         float from = NAN;
-        bool ruled = false;
-        if (k > 0 && k < a.vocab) from = find<false>((double)k, border, !(p < 1.0), p, ruled);
-        if (p < 1.0 && !ruled) from = find<true>(fmax(p, 0.0), border, true, 1.0, ruled);
-        border = fmaxf(border, least);
+        if (r.k > 0) from = find<false>((double)r.k, border, !(r.p < 1.0));
+        if (r.p < 1.0) from = find<true>(fmax(r.p, 0.0), border, true);
+        border = fmaxf(border, r.least(top));
         if (!(from >= border)) return kept_sum();       // no sums, or of more than is kept
         add_listed();
         return joined();
     }
-    __device__ __forceinline__ float at_least(double x) const { return x >= (double)kLowest ? __double2float_ru(x) : kLowest; }
-
-    // ---- the parts' sums, and the whole row's
-    __device__ double join(double sum) {
-        sum = warp_sum64(sum);
-        if (lane == 0) sh.seg[warp] = sum;
-        return joined();
-    }
-    __device__ double joined() {
+    // (by the first CTA)
+    __device__ void settle(const Rules& r) {
+        const Chunk* chunk = a.chunk + (int64_t)local * a.chunks;
+        const Near* list = a.list + (int64_t)local * a.chunks * kList;
+        Row in{};
+        if (a.ranked) in = a.row[local];
+        float m = -INFINITY, l = INFINITY, h = -INFINITY;
+        int n = 0, most = 0, first = INT_MAX;
+        double above = 0.0, all = 0.0;
+        for (int c = tid; c < a.chunks; c += kThreads) {
+            const Chunk one = chunk[c];
+            m = fmaxf(m, one.top);
+            l = fminf(l, one.lo);
+            h = fmaxf(h, one.hi);
+            n += one.listed;
+            most = max(most, one.listed);
+            above += one.above;
+            all += one.whole;
+            sh.chunk[c] = one.above;
+            sh.first[c] = one.listed;
+        }
+        m = over(m, sh.fpart, Max());
+        top = m;
+        relative_to(top, r.scale);
+        double total = 0.0;
+        float found = INFINITY;
+        bool settled = true;
+        if (!(m > -INFINITY)) {
+            // every logit is -inf: nothing is kept
+        } else if (r.greedy()) {                        // the lowest of the largest
+            for (int c = tid; c < a.chunks; c += kThreads)
+                if (chunk[c].top == m && chunk[c].listed) first = min(first, chunk[c].first);
+            first = over(first, sh.ipart, Min());
+            for (int c = tid; c < a.chunks; c += kThreads) {
+                const int v = (c * a.chunk_strips) * STRIP - view.off;
+                sh.chunk[c] = first >= v && first < v + a.chunk_strips * STRIP ? 1.0 : 0.0;
+            }
+            found = m;
+            total = 1.0;
+        } else if (!a.ranked) {
+            found = r.floor(m);
+            for (int c0 = 0; c0 < a.chunks; c0 += kThreads) {       // from the chunk's largest to the row's
+                const float t = c0 + tid < a.chunks ? chunk[c0 + tid].top : m;
+                const double w = t >= found ? weight(t) : 0.0;
+                if (c0 + tid < a.chunks) total += sh.chunk[c0 + tid] *= w;
+            }
+            total = over(total, sh.part, Add());
+        } else if (!in.settled) {
+            settled = false;
+        } else {
+            n = over(n, sh.ipart, Add());
+            most = over(most, sh.ipart, Most());
+            l = over(l, sh.fpart, Min());
+            h = over(h, sh.fpart, Max());
+            above = over(above, sh.part, Add());
+            all = over(all, sh.part, Add());
+            const float least = r.least(m);
+            if (n == 0) found = in.up;                  // only min_p: all of it is summed
+            else {
+                const bool both = r.k > 0 && r.p < 1.0;          // (a count, of which all are listed; a share of it comes next)
+                if (l == h) found = l;
+                else if (n <= kMany && most <= kList) {
+                    starts();
+                    for (int i = tid; i < n; i += kThreads) {
+                        int c = 0, end = a.chunks - 1;          // the last chunk that begins at or before it
+                        while (c < end) {
+                            const int mid = (c + end + 1) >> 1;
+                            if (sh.first[mid] <= i) c = mid;
+                            else end = mid - 1;
+                        }
+                        sh.many[i] = list[c * kList + i - sh.first[c]].x;
+                    }
+                    __syncthreads();
+                    int some;
+                    if (r.k > 0) found = select<false>(n, l, h, 0.0, in.above_n, (double)r.k, some);
+                    else found = select<true>(n, l, h, above, 0, r.p * all, some);
+                    if (both && found == found) {
+                        const double counted = weights_of_few(n, found);
+                        found = among<true>(n, found, 0.0, 0, r.p * counted);
+                    }
+                } else found = NAN;
+                found = fmaxf(found, found == found ? least : found);
+            }
+            settled = found == found;
+            if (settled) {                              // what is listed and kept, to its chunk
+                if (l == h) {                           // (all alike)
+                    const double w = weight(l);
+                    for (int c = tid; c < a.chunks; c += kThreads)
+                        if (found <= l) sh.chunk[c] += chunk[c].listed * w;
+                } else if (n > 0) {
+                    for (int c = warp; c < a.chunks; c += kWarps) {
+                        double sum = 0.0;
+                        for (int i = sh.first[c]; i < sh.first[c + 1]; i += 32) {
+                            const float x = i + lane < sh.first[c + 1] ? sh.many[i + lane] : -INFINITY;
+                            if (__any_sync(kAll, x >= found)) {
+                                const double w = weight(x);
+                                sum += x >= found ? w : 0.0;
+                            }
+                        }
+                        sum = warp_sum(sum);
+                        if (lane == 0) sh.chunk[c] += sum;
+                    }
+                }
+                __syncthreads();
+                for (int c = tid; c < a.chunks; c += kThreads) total += sh.chunk[c];
+                total = over(total, sh.part, Add());
+            }
+        }
         __syncthreads();
-        publish();
-        cluster_sync();
-        return over_cluster(&sh.x_total[turn], Add());
-    }
-    __device__ void publish() {
-        turn ^= 1;              // two places in turn: others may still read the last one
         if (tid == 0) {
-            double t = 0.0;
-            for (int w = 0; w < kWarps; ++w) t += sh.seg[w];
-            sh.x_total[turn] = t;
+            Verdict& v = sh.verdict;
+            v.top = m;
+            v.border = found;
+            v.only = r.greedy() && m > -INFINITY ? first : -1;
+            v.total = total;
+            v.settled = settled;
         }
     }
+    // sh.first: from the chunks' numbers of listed tokens to where they begin
+    __device__ void starts() {
+        __syncthreads();
+        if (warp == 0) {
+            constexpr int EACH = kMostChunks / 32;
+            int n[EACH], sum = 0;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                const int c = lane * EACH + e;
+                n[e] = c < a.chunks ? sh.first[c] : 0;
+                sum += n[e];
+            }
+            int to = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int p = __shfl_up_sync(kAll, to, o);
+                if (lane >= o) to += p;
+            }
+            to -= sum;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                const int c = lane * EACH + e;
+                if (c <= a.chunks) sh.first[c] = to;
+                to += n[e];
+            }
+            if (lane == 31 && a.chunks == kMostChunks) sh.first[kMostChunks] = to;
+        }
+        __syncthreads();
+    }
 
-    // ---- the first token up to which the sums of f(slot) exceed `target`, as a slot of the CTA whose piece has it; -1 in the others
-    template <typename F> __device__ int search(double target, bool last, F f) {
-        double t[kMostRanks], run = 0.0, mine = 0.0;
-        of_all(&sh.x_total[turn], t, 0.0);
-        if (last) {             // nothing of the others is read any more
+    // ---- the first token up to which the sums of f(x, token) exceed `target`; -1 in the CTAs that it is not in.  `part` is where it is
+    // (f of a word's tokens: their weights)
+    template <typename F> __device__ int search(double target, bool last, int& part, F f) {
+        double run = 0.0, mine = 0.0;
+        bool open = true;               // the first that exceeds it, else (by rounding) the last that has anything
+        int owner = by_chunks ? 0 : -1;
+        if (!by_chunks) {
+            double t[kMostRanks];
+            of_all(&sh.x_total[turn], t, 0.0);
+#pragma unroll
+            for (int c = 0; c < kMostRanks; ++c) {
+                if (open && t[c] > 0.0) {
+                    owner = c;
+                    mine = run;
+                    open = !(run + t[c] > target);
+                }
+                run += t[c];
+            }
+        }
+        if (last && a.ranks > 1) {      // nothing of the others is read any more
             cluster_arrive();
             left = true;
         }
-        int owner = -1;
-        bool open = true;
-#pragma unroll
-        for (int c = 0; c < kMostRanks; ++c) {              // the first that exceeds it, else (by rounding) the last that has anything
-            if (open && t[c] > 0.0) {
-                owner = c;
-                mine = run;
-                open = !(run + t[c] > target);
-            }
-            run += t[c];
-        }
         if (owner != rank) return -1;
         run = mine;
-        int part = 0;
+        part = 0;
         open = true;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (open && sh.seg[w] > 0.0) {
-                part = w;
+        const int parts = by_chunks ? a.chunks : kWarps;
+        for (int c = 0; c < parts; ++c) {
+            const double t = by_chunks ? sh.chunk[c] : sh.seg[c];
+            if (open && t > 0.0) {
+                part = c;
                 mine = run;
-                open = !(run + sh.seg[w] > target);
+                open = !(run + t > target);
             }
-            run += sh.seg[w];
+            run += t;
         }
-        const int e0 = strips * part / kWarps, n = strips * (part + 1) / kWarps - e0;       // at most kMostStrips
-        for (int i = warp; i < n; i += kWarps) {
-            double sum = 0.0;
+        const int of = rank * kWarps + part, all = a.ranks * kWarps;
+        const int e0 = by_chunks ? part * a.chunk_strips : (int)((int64_t)view.strips * of / all);
+        const int n = (by_chunks ? min(e0 + a.chunk_strips, view.strips) : (int)((int64_t)view.strips * (of + 1) / all)) - e0;
+        view.template each<4>(e0 + warp, e0 + n, kWarps, lane, [&](const Word<T>& x, int s, int v) {
+            double w[N], sum = 0.0;
+            f(x, v, w);
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum += f((e0 + i) * STRIP + lane * N + e);
-            sum = warp_sum64(sum);
-            if (lane == 0) sh.strip[i] = sum;
-        }
+            for (int e = 0; e < N; ++e) sum += w[e];
+            sum = warp_sum(sum);
+            if (lane == 0) sh.strip[s - e0] = sum;
+        });
         __syncthreads();
         if (warp == 0) {
             run = mine;
             int at = 0;
             open = true;
             for (int i = 0; i < n; ++i) {
-                const double w = sh.strip[i];
-                if (open && w > 0.0) {
+                const double t = sh.strip[i];
+                if (open && t > 0.0) {
                     at = i;
                     mine = run;
-                    open = !(run + w > target);
+                    open = !(run + t > target);
                 }
-                run += w;
+                run += t;
             }
-            const int j = (e0 + at) * STRIP + lane * N;
+            const int v = view.token(e0 + at, lane);
             double w[N], to = 0.0;
+            f(view.load(e0 + at, lane), v, w);
 #pragma unroll
-            for (int e = 0; e < N; ++e) to += w[e] = f(j + e);
+            for (int e = 0; e < N; ++e) to += w[e];
             const double own = to;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -903,8 +1367,8 @@ struct Piece {
             for (int e = 0; e < N; ++e) {
                 cum += w[e];
                 if (w[e] > 0.0) {
-                    end = j + e;
-                    if (hit < 0 && cum > target) hit = j + e;
+                    end = v + e;
+                    if (hit < 0 && cum > target) hit = v + e;
                 }
             }
             const uint32_t who = __ballot_sync(kAll, hit >= 0);
@@ -917,71 +1381,55 @@ struct Piece {
 
     // ---- what the modes do
     __device__ void probs() {
-        const double total = top > -INFINITY ? rules() : 0.0, share = total > 0.0 ? 1.0 / total : 0.0;
-        if (!(total > 0.0)) border = INFINITY;
-        float* out = a.probs + (int64_t)row * a.probs_stride + lo;
-        for (int s = s0; s < s1; ++s) {
-            const int j = s * STRIP + lane;                 // lanes on neighbouring tokens, as they are written
-            float x[N], m = -INFINITY, y[N];
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                x[e] = at(j + e * 32);
-                m = fmaxf(m, x[e]);
-                y[e] = 0.f;
-            }
-            if (__any_sync(kAll, m >= border)) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const double w = weight(x[e]);
-                    y[e] = x[e] >= border ? (float)(w * share) : 0.f;
-                }
-            }
-            if (lo + s * STRIP >= 0 && (s + 1) * STRIP <= used && lo + (s + 1) * STRIP <= a.vocab) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) out[j + e * 32] = y[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (lo + j + e * 32 >= 0 && lo + j + e * 32 < a.vocab && j + e * 32 < used) out[j + e * 32] = y[e];
-            }
+        const double total = rules();
+        if (rank == 0 && tid == 0) {
+            Row& out = a.row[local];
+            out.top = top;
+            out.border = total > 0.0 ? border : INFINITY;
+            out.only = only;
+            out.share = total > 0.0 ? 1.0 / total : 0.0;
         }
     }
 
     __device__ void draw() {
-        if (!(top > -INFINITY)) {
-            if (rank == 0 && tid < 32) for (int i = lane; i < a.count; i += 32) put(i, -1, 0.0);
-            return;
-        }
-        auto f = [&](int j) { return kept(at(j)); };
         const double whole = rules();
+        if (by_chunks && rank != 0) return;
         double total = whole;
+        auto f = [&](const Word<T>& x, int v, double (&w)[N]) { kept_of(x, v, w); };
         for (int i = 0; i < a.count; ++i) {
-            if (i) total = over_cluster(&sh.x_total[turn], Add());
             if (!(total > 0.0)) {
                 if (rank == 0 && tid == 0) put(i, -1, 0.0);
                 continue;                           // (so will all the others be)
             }
             const float u = a.uniform[(int64_t)row * a.count + i];
-            const int j = search((u > 0.f ? (double)u : 0.0) * total, i + 1 == a.count, f);
-            if (j >= 0 && warp == 0) {
-                const double w = kept(at(j));
-                if (lane == 0) put(i, lo + j, w / whole);
+            int part = 0;
+            const int v = search((u > 0.f ? (double)u : 0.0) * total, !by_chunks && i + 1 == a.count, part, f);
+            if (v >= 0 && warp == 0) {
+                const double w = kept(view.at(v), v);
+                if (lane == 0) put(i, v, w / whole);
             }
             if (i + 1 == a.count) break;
-            if (j >= 0) {                           // it leaves: its warp's part is summed anew
+            if (v >= 0) {                           // it leaves: its part is summed anew
                 __syncthreads();
-                if (tid == 0) data[j] = narrow<T>(-INFINITY);
+                if (tid == 0) gone[v >> 5] |= 1u << (v & 31);
                 __syncthreads();
-                if (j >= s0 * STRIP && j < s1 * STRIP) {
-                    double sum = 0.0;
-                    for (int s = s0; s < s1; ++s) sum += strip_sum(s, border);
-                    sum = warp_sum64(sum);
-                    if (lane == 0) sh.seg[warp] = sum;
-                }
+                const int of = rank * kWarps + part, all = a.ranks * kWarps;
+                const int e0 = by_chunks ? part * a.chunk_strips : (int)((int64_t)view.strips * of / all);
+                const int e1 = by_chunks ? min(e0 + a.chunk_strips, view.strips) : (int)((int64_t)view.strips * (of + 1) / all);
+                double sum = 0.0;
+                view.template each<4>(e0 + warp, e1, kWarps, lane, [&](const Word<T>& x, int, int t) { sum += word_sum(x, t); });
+                sum = over(sum, sh.part, Add());
+                if (tid == 0) (by_chunks ? sh.chunk[part] : sh.seg[part]) = sum;
             }
             __syncthreads();
-            publish();
-            cluster_sync();
+            if (by_chunks) {
+                total = 0.0;
+                for (int c = 0; c < a.chunks; ++c) total += sh.chunk[c];
+            } else {
+                publish();
+                cluster_sync();
+                total = over_cluster(&sh.x_total[turn], Add());
+            }
         }
     }
     __device__ void put(int i, int id, double p) {
@@ -989,15 +1437,12 @@ struct Piece {
         if (a.logprobs) a.logprobs[(int64_t)row * a.count + i] = id < 0 ? -INFINITY : (float)log(p);
     }
 
-    // (in weights: p, S and a times the sum of the kept)
-    __device__ void verify() {
-        if (!(top > -INFINITY)) {
-            if (rank == 0 && tid == 0) put(0, -1, 0.0);
-            return;
-        }
-        const double total = rules();
+    // ---- verification, in weights: p, S and a times the sum of the kept.  A node's tests go on until a child is kept, or refused: then what it
+    // leaves is summed by chunks (rest_kernel) before the next one
+    __device__ void children() {
         const int b = a.row_seq[row], which = a.draft_rows ? a.draft_rows[row] : row;
         const bool drafted = (unsigned)which < (unsigned)a.draft_count && (unsigned)b < (unsigned)a.num_seqs;
+        __syncthreads();
         if (warp == 0) {
             int n = 0;
             if (drafted) {
@@ -1013,59 +1458,94 @@ struct Piece {
             if (lane == 0) sh.children = min(n, PA_TREE_MOST_NODES);
         }
         __syncthreads();
-        const Q* q = drafted ? static_cast<const Q*>(a.draft) + (int64_t)which * a.draft_stride : nullptr;
-        const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.stride;
-        double taken = 0.0, S = total, gone = 0.0;
-        for (int i = 0; i < sh.children; ++i) {
+    }
+    // true: the node's id is given, or a refused child's rest has to be summed (a.rest)
+    __device__ bool tests(Rest st, double S) {
+        const Q* q = draft_row<Q>(a, row);
+        for (int i = st.child; i < sh.children; ++i) {
             const int r = sh.child[i], c = a.tokens[r];
             if ((unsigned)c >= (unsigned)a.vocab) continue;
-            const float xc = widen<T>(x[c]);
-            const double w = kept(only >= 0 && c != only ? -INFINITY : fminf(xc, xc == xc ? Limit<T>::most : -INFINITY)), qc = (double)widen<Q>(q[c]);
-            if ((double)a.uniform[2 * (int64_t)r] * qc * S < fmax(w - taken * qc, 0.0) * (1.0 - gone)) {
-                if (rank == 0 && tid == 0) put(0, c, w / total);
-                return;
+            const double w = kept(view.at(c), c), qc = (double)widen<Q>(q[c]);
+            if ((double)a.uniform[2 * (int64_t)r] * qc * S < fmax(w - st.taken * qc, 0.0) * (1.0 - st.out)) {
+                if (rank == 0 && tid == 0) put(0, c, w / st.total);
+                return true;
             }
-            taken += S / fmax(1.0 - gone, 1e-18);
-            if (a.distinct) gone += qc;
-            double sum = 0.0;
-            for (int s = s0; s < s1; ++s) {
-                const int j = s * STRIP + lane;     // lanes on neighbouring tokens, as q lies
-                float xs[N], qs[N], m = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    xs[e] = at(j + e * 32);
-                    m = fmaxf(m, xs[e]);
-                }
-                if (!__any_sync(kAll, m >= border)) continue;
-#pragma unroll
-                for (int e = 0; e < N; ++e) qs[e] = xs[e] >= border ? widen<Q>(q[lo + j + e * 32]) : 0.f;
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const double v = weight(xs[e]) - taken * (double)qs[e];
-                    sum += xs[e] >= border && v > 0.0 ? v : 0.0;
-                }
+            st.taken += S / fmax(1.0 - st.out, 1e-18);
+            if (a.distinct) st.out += qc;
+            if (S > 0.0) {
+                st.child = i + 1;
+                st.open = 1;
+                if (rank == 0 && tid == 0) a.rest[local] = st;
+                return true;
             }
-            S = join(sum);
         }
-        const bool some = taken > 0.0 && S > 0.0;
-        if (taken > 0.0 && !some) S = kept_sum();   // nothing is left by rounding, or where q is no distribution
+        return false;
+    }
+    __device__ void draw_from(double S, double taken, double total) {
+        const Q* q = draft_row<Q>(a, row);
         const float u = a.uniform[2 * (int64_t)row + 1];
-        const int j = search((u > 0.f ? (double)u : 0.0) * S, true, [&](int slot) {
-            const double w = kept(at(slot));
-            return some && w > 0.0 ? fmax(w - taken * (double)widen<Q>(q[lo + slot]), 0.0) : w;
+        int part;
+        const int v = search((u > 0.f ? (double)u : 0.0) * S, true, part, [&](const Word<T>& x, int token, double (&w)[N]) {
+            kept_of(x, token, w);
+            if (taken > 0.0)
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (w[e] > 0.0) w[e] = fmax(w[e] - taken * (double)widen<Q>(q[token + e]), 0.0);
         });
-        if (j >= 0 && warp == 0) {
-            const double w = kept(at(j));
-            if (lane == 0) put(0, lo + j, w / total);
+        if (v >= 0 && warp == 0) {
+            const double w = kept(view.at(v), v);
+            if (lane == 0) put(0, v, w / total);
         }
+    }
+    __device__ void verify() {
+        const double total = rules();
+        Rest st{};
+        st.total = total;
+        if (rank == 0 && tid == 0) {
+            Row& out = a.row[local];
+            out.top = top;
+            out.border = border;
+            out.only = only;
+            out.scale = scale;
+            a.rest[local] = st;
+            if (!(total > 0.0)) put(0, -1, 0.0);
+        }
+        if (!(total > 0.0)) return;
+        children();
+        if (!tests(st, total)) draw_from(total, 0.0, total);
+    }
+    __device__ void go_on() {
+        wait_for_last();
+        Rest st = a.rest[local];
+        if (!st.open) return;
+        __syncthreads();
+        st.open = 0;
+        if (tid == 0) a.rest[local] = st;
+        const Row in = a.row[local];
+        top = in.top;
+        border = in.border;
+        only = in.only;
+        relative_to(top, in.scale);
+        const double* sums = a.rest_sum + (int64_t)local * a.chunks;
+        double S = 0.0;
+        for (int c = tid; c < a.chunks; c += kThreads) S += sh.chunk[c] = sums[c];
+        S = over(S, sh.part, Add());
+        children();
+        if (S > 0.0 && tests(st, S)) return;
+        if (S > 0.0) draw_from(S, st.taken, st.total);
+        else draw_from(kept_sum(), 0.0, st.total);          // nothing is left by rounding, or where q is no distribution: p
     }
 };
 
-template <typename T, typename Q, int MODE> __global__ void __launch_bounds__(kThreads, 3) draw_kernel(const __grid_constant__ Args a) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    Piece<T, Q, MODE> p(a, *reinterpret_cast<Shared*>(smem + a.data_bytes), reinterpret_cast<T*>(smem));
-    p.table = exp2((threadIdx.x & 31) / 32.0);
-    p.load();
+template <typename T, typename Q, int MODE> __global__ void __launch_bounds__(kThreads) finish_kernel(const __grid_constant__ Args a) {
+    __shared__ Shared sh;
+    extern __shared__ uint32_t bits[];
+    if (MODE == DRAW && a.count > 1) {
+        for (int i = threadIdx.x; i < (a.vocab + 31) / 32; i += kThreads) bits[i] = 0;
+        __syncthreads();
+    }
+    let_next_start();
+    Finish<T, Q, MODE> p(a, sh, MODE == DRAW && a.count > 1 ? bits : nullptr);
     if constexpr (MODE == PROBS) p.probs();
     else if constexpr (MODE == DRAW) p.draw();
     else p.verify();
@@ -1073,47 +1553,217 @@ template <typename T, typename Q, int MODE> __global__ void __launch_bounds__(kT
     cluster_wait();
 }
 
-template <typename T, typename Q, int MODE> static int launch(Args a, cudaStream_t st) {
-    constexpr int N = Word<T>::N;
-    // the fewest CTAs whose pieces leave room for three on an SM, more while rows are few
-    auto bytes = [&](int ranks) { return (((size_t)a.vocab / N / ranks + 3 + 31) / 32) * 512; };
-    const size_t most = device_info().max_smem_optin - sizeof(Shared) - 1024;
-    a.ranks = 1;
-    while (a.ranks < kMostRanks && (bytes(a.ranks) > 56 * 1024 || (a.rows * a.ranks * 2 <= device_info().sm_count && a.vocab / a.ranks >= 4096))) a.ranks *= 2;
-    a.data_bytes = bytes(a.ranks);
-    int counts = 1;                     // bits for a CTA's tokens; parts of a step, whose sums must fit beside them
-    while (((size_t)1 << counts) <= a.data_bytes / sizeof(T)) ++counts;
-    a.count_shift = 32 - counts;
-    a.parts = 2 * counts < 32 ? (float)(1 << (32 - 2 * counts < 8 ? 32 - 2 * counts : 8)) : 0.f;
-    if (a.data_bytes > most || (int64_t)a.rows * a.ranks > INT_MAX) return PA_ERR_UNSUPPORTED;
-    const size_t smem = a.data_bytes + sizeof(Shared);
-    const cudaError_t e = allow_dynamic_smem<draw_kernel<T, Q, MODE>>(smem);
-    if (e != cudaSuccess) return (int)e;
+// -------------------------------------------------------------------------------------------------------------------- rest
+// What refused children have left of a chunk: max(w - taken q, 0).  Words of the logits, and of q where it lies alike, several on their way at once
+template <typename T, typename Q> __global__ void __launch_bounds__(kThreads, 3) rest_kernel(const __grid_constant__ Args a) {
+    constexpr int N = Word<T>::N, QN = 16 / (int)sizeof(Q), SOME = sizeof(T) < 4 ? 2 : 4;
+    __shared__ double s_part[kWarps];
+    Block b;
+    const int local = blockIdx.x / a.chunks, c = blockIdx.x - local * a.chunks, row = a.row0 + local, lane = b.lane;
+    let_next_start();
+    wait_for_last();
+    const Rest st = a.rest[local];
+    if (!st.open) return;
+    const View<T> view(a, row);
+    const Row r = a.row[local];
+    b.relative_to(r.top, r.scale);
+    const Q* q = draft_row<Q>(a, row);
+    const int s0 = c * a.chunk_strips, s1 = min(s0 + a.chunk_strips, view.strips);
+    const bool alike = ((uintptr_t)(q - view.off) & 15) == 0;
+    double sum = 0.0;
+    auto add = [&](const Word<T>& x, int v, const float (&y)[N]) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < N; ++e) m = fmaxf(m, widen<T>(x.v[e]));
+        if (!__any_sync(kAll, m >= r.border)) return;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float z = widen<T>(x.v[e]);
+            const double u = b.weight<T>(z) - st.taken * (double)y[e];
+            if (z >= r.border && (r.only < 0 || v + e == r.only) && u > 0.0) sum += u;
+        }
+    };
+    for (int s = s0 + b.warp; s < s1; s += SOME * kWarps) {
+        if (alike && s + (SOME - 1) * kWarps < s1 && view.whole(s, (SOME - 1) * kWarps + 1)) {
+            Word<T> x[SOME];
+            float y[SOME][N];
+#pragma unroll
+            for (int k = 0; k < SOME; ++k) x[k] = view.load_whole(s + k * kWarps, lane);
+#pragma unroll
+            for (int k = 0; k < SOME; ++k) {
+                const int v = view.token(s + k * kWarps, lane);
+                if constexpr (QN <= N) {
+#pragma unroll
+                    for (int e = 0; e < N; e += QN) {
+                        const uint4 raw = ldg_stream_128(q + v + e);
+#pragma unroll
+                        for (int i = 0; i < QN; ++i) y[k][e + i] = widen<Q>(reinterpret_cast<const Q*>(&raw)[i]);
+                    }
+                } else {                            // (eight of q to a word of its own, four of the logits)
+                    const uint2 raw = ldg_stream_64(q + v);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) y[k][i] = widen<Q>(reinterpret_cast<const Q*>(&raw)[i]);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < SOME; ++k) add(x[k], view.token(s + k * kWarps, lane), y[k]);
+        } else {
+            for (int k = 0; k < SOME && s + k * kWarps < s1; ++k) {
+                const int v = view.token(s + k * kWarps, lane);
+                float y[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) y[e] = v + e >= 0 && v + e < view.V ? widen<Q>(q[v + e]) : 0.f;
+                add(view.load(s + k * kWarps, lane), v, y);
+            }
+        }
+    }
+    sum = b.over(sum, s_part, Add());
+    if (b.tid == 0) a.rest_sum[blockIdx.x] = sum;
+}
+
+// Where a node's tests go on after that
+template <typename T, typename Q> __global__ void __launch_bounds__(kThreads) go_on_kernel(const __grid_constant__ Args a) {
+    __shared__ Shared sh;
+    let_next_start();
+    Finish<T, Q, VERIFY> p(a, sh, nullptr);
+    p.go_on();
+}
+
+// ------------------------------------------------------------------------------------------------------------------- write
+template <typename T> __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__ Args a) {
+    constexpr int N = Word<T>::N, STRIP = 32 * N;
+    Block b;
+    const int local = blockIdx.x / a.chunks, c = blockIdx.x - local * a.chunks, row = a.row0 + local;
+    const View<T> view(a, row);
+    const Rules rules(a, row);
+    const int s0 = c * a.chunk_strips, s1 = min(s0 + a.chunk_strips, view.strips);
+    wait_for_last();
+    const Row r = a.row[local];
+    b.relative_to(r.top, rules.scale);
+    float* out = a.probs + (int64_t)row * a.probs_stride;
+#pragma unroll 2
+    for (int s = s0 + b.warp; s < s1; s += kWarps) {
+        const int v = s * STRIP + b.lane - view.off;                // lanes on neighbouring tokens, as they are written
+        float x[N], y[N], m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            x[e] = view.at(v + e * 32);
+            if (r.only >= 0 && v + e * 32 != r.only) x[e] = -INFINITY;
+            m = fmaxf(m, x[e]);
+            y[e] = 0.f;
+        }
+        if (__any_sync(kAll, m >= r.border))
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const double w = b.weight<T>(x[e]);
+                y[e] = x[e] >= r.border ? (float)(w * r.share) : 0.f;
+            }
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (v + e * 32 >= 0 && v + e * 32 < a.vocab) out[v + e * 32] = y[e];
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------ launch
+// Chunks of 8192 tokens, smaller ones while there are not two for every SM
+struct Cut {
+    int chunks, chunk_strips, group;        // of a row; rows that go together
+};
+static Cut cut_of(int type, int rows, int vocab) {
+    const int words = type == PA_TYPE_F32 ? 4 : 8, strips = (vocab + words - 1 + 32 * words - 1) / (32 * words);        // of a row that begins inside a word
+    Cut c;
+    c.chunk_strips = type == PA_TYPE_F32 ? 64 : 32;
+    auto chunks = [&] { return (strips + c.chunk_strips - 1) / c.chunk_strips; };
+    while (c.chunk_strips > (type == PA_TYPE_F32 ? 32 : 16) && (int64_t)rows * chunks() < device_info().sm_count) c.chunk_strips /= 2;
+    c.chunks = chunks();
+    c.group = std::min(rows, std::max(1, kGroup / c.chunks));
+    return c;
+}
+static size_t row_bytes(const Cut& c) { return (size_t)c.chunks * (kBins * 4 + kList * sizeof(Near) + sizeof(Chunk) + sizeof(double)) + sizeof(Row) + sizeof(Rest); }
+
+template <auto Kernel> static cudaError_t start(const Args& a, unsigned ctas, unsigned cluster, size_t smem, bool first, cudaStream_t st) {
+    const cudaError_t e = smem ? allow_dynamic_smem<Kernel>(smem) : cudaSuccess;
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.rows * a.ranks));
+    cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)a.ranks;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (cluster) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = cluster;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (!first) {                   // the first kernel begins when all before it have ended, the others while theirs does
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
     cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, draw_kernel<T, Q, MODE>, a);
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, Kernel, a);
 }
 
-template <int MODE> static int launch(const Args& a, int type, int draft_type, cudaStream_t st) {
+template <typename T, typename Q, int MODE> static int launch(Args a, int type, int most_children, void* workspace, cudaStream_t st) {
+    const Cut c = cut_of(type, a.rows, a.vocab);
+    if ((size_t)a.vocab * sizeof(T) > PA_DRAW_MOST_ROW_BYTES) return PA_ERR_UNSUPPORTED;
+    a.chunks = c.chunks;
+    a.chunk_strips = c.chunk_strips;
+    a.ranked = a.top_k || a.top_k1 > 0 || a.top_p || a.top_p1 < 1.0 || a.min_p || a.min_p1 > 0.0;
+    a.ranks = 1;
+    while (a.ranks < kMostRanks && (int64_t)a.rows * a.ranks <= device_info().sm_count) a.ranks *= 2;
+    uint8_t* at = static_cast<uint8_t*>(workspace);
+    const size_t n = (size_t)c.group * c.chunks;
+    a.hist = reinterpret_cast<uint32_t*>(at);
+    at += n * kBins * 4;
+    a.list = reinterpret_cast<Near*>(at);
+    at += n * kList * sizeof(Near);
+    a.chunk = reinterpret_cast<Chunk*>(at);
+    at += n * sizeof(Chunk);
+    a.rest_sum = reinterpret_cast<double*>(at);
+    at += n * sizeof(double);
+    a.rest = reinterpret_cast<Rest*>(at);
+    at += c.group * sizeof(Rest);
+    a.row = reinterpret_cast<Row*>(at);
+    const int rows = a.rows;
+    for (int r = 0; r < rows; r += c.group) {
+        a.row0 = r;
+        const unsigned some = (unsigned)std::min(c.group, rows - r), ctas = some * (unsigned)c.chunks;
+        cudaError_t e = cudaSuccess;
+        if (a.ranked) {
+            e = start<count_kernel<T>>(a, ctas, 0, 0, true, st);
+            if (e == cudaSuccess) e = start<range_kernel<T>>(a, some, 0, 0, false, st);
+        }
+        if (e == cudaSuccess) e = start<sum_kernel<T>>(a, ctas, 0, 0, !a.ranked, st);
+        if (e == cudaSuccess) e = start<finish_kernel<T, Q, MODE>>(a, some * a.ranks, a.ranks, MODE == DRAW && a.count > 1 ? (size_t)(a.vocab + 31) / 32 * 4 : 0, false, st);
+        if (e == cudaSuccess && MODE == PROBS) e = start<write_kernel<T>>(a, ctas, 0, 0, false, st);
+        if constexpr (MODE == VERIFY) {
+            Args one = a;
+            one.ranks = 1;
+            for (int i = 0; i < most_children && e == cudaSuccess; ++i) {
+                e = start<rest_kernel<T, Q>>(one, ctas, 0, 0, false, st);
+                if (e == cudaSuccess) e = start<go_on_kernel<T, Q>>(one, some, 0, 0, false, st);
+            }
+        }
+        if (e != cudaSuccess) return (int)e;
+    }
+    return PA_OK;
+}
+
+template <int MODE> static int launch(const Args& a, int type, int draft_type, int most_children, void* workspace, cudaStream_t st) {
     if constexpr (MODE == VERIFY) {
         auto of = [&](auto t) {
             typedef decltype(t) T;
-            return draft_type == PA_TYPE_F32 ? launch<T, float, MODE>(a, st) : draft_type == PA_TYPE_F16 ? launch<T, __half, MODE>(a, st) :
-                   draft_type == PA_TYPE_BF16 ? launch<T, bf16_t, MODE>(a, st) : PA_ERR_UNSUPPORTED;
+            return draft_type == PA_TYPE_F32 ? launch<T, float, MODE>(a, type, most_children, workspace, st) : draft_type == PA_TYPE_F16 ? launch<T, __half, MODE>(a, type, most_children, workspace, st) :
+                   draft_type == PA_TYPE_BF16 ? launch<T, bf16_t, MODE>(a, type, most_children, workspace, st) : PA_ERR_UNSUPPORTED;
         };
         return type == PA_TYPE_F32 ? of(float()) : type == PA_TYPE_F16 ? of(__half()) : type == PA_TYPE_BF16 ? of(bf16_t()) : PA_ERR_UNSUPPORTED;
     } else {
-        return type == PA_TYPE_F32 ? launch<float, float, MODE>(a, st) : type == PA_TYPE_F16 ? launch<__half, float, MODE>(a, st) :
-               type == PA_TYPE_BF16 ? launch<bf16_t, float, MODE>(a, st) : PA_ERR_UNSUPPORTED;
+        return type == PA_TYPE_F32 ? launch<float, float, MODE>(a, type, most_children, workspace, st) : type == PA_TYPE_F16 ? launch<__half, float, MODE>(a, type, most_children, workspace, st) :
+               type == PA_TYPE_BF16 ? launch<bf16_t, float, MODE>(a, type, most_children, workspace, st) : PA_ERR_UNSUPPORTED;
     }
 }
 
@@ -1125,6 +1775,7 @@ static Args args(const void* logits, int64_t stride, int rows, int vocab, const 
     a.temperature1 = rules->temperature; a.top_k1 = rules->top_k; a.top_p1 = rules->top_p; a.min_p1 = rules->min_p;
     return a;
 }
+static bool holds(const void* workspace, size_t bytes, size_t need) { return workspace && (uintptr_t)workspace % 16 == 0 && bytes >= need; }
 static bool usable(const void* logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules) {
     return rows >= 0 && vocab > 0 && stride >= vocab && rules && rules->num_seqs >= 0 && (rows == 0 || logits) &&
            (uintptr_t)logits % (type == PA_TYPE_F32 ? 4 : 2) == 0;
@@ -1135,8 +1786,14 @@ static bool usable(const void* logits, int type, int64_t stride, int rows, int v
 
 using namespace pa;
 
+PA_API size_t pa_draw_workspace_bytes(int type, int rows, int vocab) {
+    if (rows <= 0 || vocab <= 0 || type < PA_TYPE_F32 || type > PA_TYPE_BF16) return 0;
+    const drawn::Cut c = drawn::cut_of(type, rows, vocab);
+    return drawn::row_bytes(c) * c.group;
+}
+
 PA_API int pa_truncated_softmax(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, float* d_probs,
-                                int64_t probs_stride, pa_stream_t stream) {
+                                int64_t probs_stride, void* d_workspace, size_t workspace_bytes, pa_stream_t stream) {
     using namespace pa::drawn;
     PA_CHECK_ARG(usable(d_logits, type, stride, rows, vocab, rules) && probs_stride >= vocab);
     if (rows == 0) return PA_OK;
@@ -1146,31 +1803,34 @@ PA_API int pa_truncated_softmax(const void* d_logits, int type, int64_t stride, 
     PA_CHECK_ARG(in >= out_end || out >= in_end);
     Args a = args(d_logits, stride, rows, vocab, rules);
     a.probs = d_probs; a.probs_stride = probs_stride;
-    return launch<PROBS>(a, type, 0, as_stream(stream));
+    if (!holds(d_workspace, workspace_bytes, pa_draw_workspace_bytes(type, rows, vocab))) return PA_ERR_WORKSPACE;
+    return launch<PROBS>(a, type, 0, 0, d_workspace, as_stream(stream));
 }
 
 PA_API int pa_draw_tokens(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, const float* d_uniform,
-                          int count, int32_t* d_ids, float* d_logprobs, pa_stream_t stream) {
+                          int count, int32_t* d_ids, float* d_logprobs, void* d_workspace, size_t workspace_bytes, pa_stream_t stream) {
     using namespace pa::drawn;
     PA_CHECK_ARG(usable(d_logits, type, stride, rows, vocab, rules) && count > 0);
     if (rows == 0) return PA_OK;
     PA_CHECK_ARG(d_uniform && d_ids);
     Args a = args(d_logits, stride, rows, vocab, rules);
     a.uniform = d_uniform; a.count = count; a.ids = d_ids; a.logprobs = d_logprobs;
-    return launch<DRAW>(a, type, 0, as_stream(stream));
+    if (!holds(d_workspace, workspace_bytes, pa_draw_workspace_bytes(type, rows, vocab))) return PA_ERR_WORKSPACE;
+    return launch<DRAW>(a, type, 0, 0, d_workspace, as_stream(stream));
 }
 
 PA_API int pa_verify_drafts(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, const float* d_uniform,
-                            const int32_t* d_tokens, const int32_t* d_parents, const int32_t* d_node_start, const void* d_draft, int draft_type,
+                            const int32_t* d_tokens, const int32_t* d_parents, const int32_t* d_node_start, int most_children, const void* d_draft, int draft_type,
                             int64_t draft_stride, int draft_count, const int32_t* d_draft_rows, int distinct, int32_t* d_ids, float* d_logprobs,
-                            pa_stream_t stream) {
+                            void* d_workspace, size_t workspace_bytes, pa_stream_t stream) {
     using namespace pa::drawn;
-    PA_CHECK_ARG(usable(d_logits, type, stride, rows, vocab, rules) && draft_count >= 0 && (draft_count == 0 || (d_draft && draft_stride >= vocab)));
+    PA_CHECK_ARG(usable(d_logits, type, stride, rows, vocab, rules) && draft_count >= 0 && most_children >= 0 && most_children < PA_TREE_MOST_NODES && (draft_count == 0 || (d_draft && draft_stride >= vocab)));
     if (rows == 0) return PA_OK;
     PA_CHECK_ARG(d_uniform && d_ids && d_tokens && d_parents && d_node_start && rules->d_row_seq && (d_draft_rows || draft_count >= rows));
     Args a = args(d_logits, stride, rows, vocab, rules);
     a.uniform = d_uniform; a.count = 1; a.ids = d_ids; a.logprobs = d_logprobs;
     a.tokens = d_tokens; a.parents = d_parents; a.node_start = d_node_start; a.draft = d_draft; a.draft_stride = draft_stride;
     a.draft_count = draft_count; a.draft_rows = d_draft_rows; a.distinct = distinct;
-    return launch<VERIFY>(a, type, draft_type, as_stream(stream));
+    if (!holds(d_workspace, workspace_bytes, pa_draw_workspace_bytes(type, rows, vocab))) return PA_ERR_WORKSPACE;
+    return launch<VERIFY>(a, type, draft_type, most_children, d_workspace, as_stream(stream));
 }

@@ -62,7 +62,16 @@ class DraftTree:
         self.row_seq, self.parents, self.depths, self.nodes = parts[:4]
         self.tokens = None if tokens is None else parts[4]
         self.mask = parts[-1].view(R, words)
+        self._parents, self._branches = flat, None
         self._space = {}                # (heads, kv heads, D) -> bytes of workspace that pa_tree_attention wants for this tree
+
+    @property
+    def branches(self):
+        "Children of the node that has the most."
+        if self._branches is None:
+            up = self._parents + np.repeat(np.cumsum(self.sizes) - self.sizes, self.sizes).astype(np.int64) if self.rows else self._parents
+            self._branches = int(np.bincount(up[self._parents >= 0]).max(initial=0))
+        return self._branches
 
     def positions(self, ctx_lens):
         """Where the nodes' K/V rows go in the caches (`KVTileCache.append`): behind the context, in node order."""

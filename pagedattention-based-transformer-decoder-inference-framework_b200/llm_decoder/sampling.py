@@ -236,7 +236,20 @@ def _draw_rules(logits, temperature, top_k, top_p, min_p, row_seq, tree):
     return (logits.data_ptr(), kind, stride if rows > 1 else V, rows, V, ctypes.byref(rules))
 
 
-_MOST_ROW_BYTES = 1500000               # what the shared memory of a cluster of eight CTAs holds
+_MOST_ROW_BYTES = 1500000               # PA_DRAW_MOST_ROW_BYTES
+_draw_spaces = _cabi.PerThread()        # workspaces of the calls below
+
+
+def _draw_space(args, dev, stream):
+    """(address, bytes) of a workspace for a call over these logits on a stream, and the tensor."""
+    need = _cabi.lib().pa_draw_workspace_bytes(args[1], args[3], args[4])
+    if _cabi.capturing(stream):         # a graph has a workspace of its own: its replays may run beside other calls
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    else:
+        ws = _draw_spaces.of.get((dev.index, stream))
+        if ws is None or ws.numel() < need:
+            ws = _draw_spaces.of[(dev.index, stream)] = torch.empty(need, dtype=torch.uint8, device=dev)
+    return ws.data_ptr(), need, ws
 
 
 def truncated_softmax(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, row_seq=None, tree=None, out=None):
@@ -257,7 +270,9 @@ def truncated_softmax(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ro
     args = _draw_rules(logits, temperature, top_k, top_p, min_p, row_seq, tree)
     if args[3]:
         with _cabi.on_device(logits.device):
-            _cabi.check(_cabi.lib().pa_truncated_softmax(*args, out.data_ptr(), out.stride(0) if args[3] > 1 else args[4], _cabi.stream_on(logits.device)),
+            stream = _cabi.stream_on(logits.device)
+            at, need, ws = _draw_space(args, logits.device, stream)
+            _cabi.check(_cabi.lib().pa_truncated_softmax(*args, out.data_ptr(), out.stride(0) if args[3] > 1 else args[4], at, need, stream),
                         "pa_truncated_softmax")
     return out
 
@@ -275,8 +290,10 @@ def draw_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
     args = _draw_rules(logits, temperature, top_k, top_p, min_p, row_seq, tree)
     if ids.numel():
         with _cabi.on_device(logits.device):
-            _cabi.check(_cabi.lib().pa_draw_tokens(*args, uniform.data_ptr(), ids.numel() // rows, ids.data_ptr(), _cabi.ptr(logs),
-                                                   _cabi.stream_on(logits.device)), "pa_draw_tokens")
+            stream = _cabi.stream_on(logits.device)
+            at, need, ws = _draw_space(args, logits.device, stream)
+            _cabi.check(_cabi.lib().pa_draw_tokens(*args, uniform.data_ptr(), ids.numel() // rows, ids.data_ptr(), _cabi.ptr(logs), at, need, stream),
+                        "pa_draw_tokens")
     return (ids, logs) if logprobs else ids
 
 
@@ -311,8 +328,11 @@ def verify_drafts(logits, tree, uniform, draft_probs, draft_rows=None, temperatu
     n = draft_probs.shape[0]
     if rows:
         with _cabi.on_device(dev):
+            stream = _cabi.stream_on(dev)
+            at, need, ws = _draw_space(args, dev, stream)
             _cabi.check(_cabi.lib().pa_verify_drafts(
-                *args, uniform.data_ptr(), tree.tokens.data_ptr(), tree.parents.data_ptr(), tree.node_start.data_ptr(), draft_probs.data_ptr() if n else None,
+                *args, uniform.data_ptr(), tree.tokens.data_ptr(), tree.parents.data_ptr(), tree.node_start.data_ptr(), tree.branches,
+                draft_probs.data_ptr() if n else None,
                 kind, draft_probs.stride(0) if n > 1 else V, n, _cabi.ptr(draft_rows), int(distinct), ids.data_ptr(), _cabi.ptr(logs),
-                _cabi.stream_on(dev)), "pa_verify_drafts")
+                at, need, stream), "pa_verify_drafts")
     return (ids, logs) if logprobs else ids

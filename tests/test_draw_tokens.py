@@ -304,24 +304,27 @@ def test_refused_on_the_host():
         with pytest.raises(ValueError):
             call()
     lib, ref = _cabi.lib(), __import__("ctypes").byref
-    rules = _cabi.DrawRules(num_seqs=4, temperature=1.0, top_p=1.0)
-    assert lib.pa_truncated_softmax(None, 0, 8, 4, 8, ref(rules), 0x1000, 8, None) == -1
-    assert lib.pa_truncated_softmax(0x1000, 0, 7, 4, 8, ref(rules), 0x9000, 8, None) == -1
-    assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, ref(rules), 0x9000, 7, None) == -1
-    assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, ref(rules), 0x1040, 8, None) == -1          # overlaps
-    assert lib.pa_truncated_softmax(0x1002, 0, 8, 4, 8, ref(rules), 0x9000, 8, None) == -1          # no address of a float
-    assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, None, 0x9000, 8, None) == -1
-    assert lib.pa_truncated_softmax(0x1000, 0, 8, 0, 8, ref(rules), None, 8, None) == 0
-    assert lib.pa_truncated_softmax(0x1000, 3, 8, 4, 8, ref(rules), 0x9000, 8, None) == -2
-    assert lib.pa_draw_tokens(0x1000, 0, 8, 4, 8, ref(rules), None, 1, 0x9000, None, None) == -1
-    assert lib.pa_draw_tokens(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, 0, 0x9000, None, None) == -1
-    assert lib.pa_draw_tokens(0x1000, 0, 8, 4, 0, ref(rules), 0x8000, 1, 0x9000, None, None) == -1
+    rules, ws = _cabi.DrawRules(num_seqs=4, temperature=1.0, top_p=1.0), (0x10000, 1 << 30)
+    assert lib.pa_draw_workspace_bytes(0, 4, 8) > 0 and lib.pa_draw_workspace_bytes(0, 0, 8) == lib.pa_draw_workspace_bytes(3, 4, 8) == 0
+    assert lib.pa_truncated_softmax(None, 0, 8, 4, 8, ref(rules), 0x1000, 8, *ws, None) == -1
+    assert lib.pa_truncated_softmax(0x1000, 0, 7, 4, 8, ref(rules), 0x9000, 8, *ws, None) == -1
+    assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, ref(rules), 0x9000, 7, *ws, None) == -1
+    assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, ref(rules), 0x1040, 8, *ws, None) == -1          # overlaps
+    assert lib.pa_truncated_softmax(0x1002, 0, 8, 4, 8, ref(rules), 0x9000, 8, *ws, None) == -1          # no address of a float
+    assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, None, 0x9000, 8, *ws, None) == -1
+    assert lib.pa_truncated_softmax(0x1000, 0, 8, 0, 8, ref(rules), None, 8, *ws, None) == 0
+    assert lib.pa_truncated_softmax(0x1000, 3, 8, 4, 8, ref(rules), 0x9000, 8, *ws, None) == -2
+    assert lib.pa_draw_tokens(0x1000, 0, 8, 4, 8, ref(rules), None, 1, 0x9000, None, *ws, None) == -1
+    assert lib.pa_draw_tokens(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, 0, 0x9000, None, *ws, None) == -1
+    assert lib.pa_draw_tokens(0x1000, 0, 8, 4, 0, ref(rules), 0x8000, 1, 0x9000, None, *ws, None) == -1
+    assert lib.pa_draw_tokens(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, 1, 0x9000, None, 0x10000, 8, None) == -3
+    assert lib.pa_draw_tokens(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, 1, 0x9000, None, None, 1 << 30, None) == -3
     tree = (0x2000, 0x3000, 0x4000)
-    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 0x5000, 0, 8, 4, None, 0, 0x9000, None, None) == -1      # no row_seq
+    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 2, 0x5000, 0, 8, 4, None, 0, 0x9000, None, *ws, None) == -1      # no row_seq
     rules.row_seq = 0x6000
-    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 0x5000, 0, 8, 3, None, 0, 0x9000, None, None) == -1      # rows without one
-    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 0x5000, 0, 7, 4, None, 0, 0x9000, None, None) == -1
-    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 0x5000, 3, 8, 4, None, 0, 0x9000, None, None) == -2
+    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 2, 0x5000, 0, 8, 3, None, 0, 0x9000, None, *ws, None) == -1      # rows without one
+    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 2, 0x5000, 0, 7, 4, None, 0, 0x9000, None, *ws, None) == -1
+    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 2, 0x5000, 3, 8, 4, None, 0, 0x9000, None, *ws, None) == -2
 
 
 @pytest.mark.gpu
