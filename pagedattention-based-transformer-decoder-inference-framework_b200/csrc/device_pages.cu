@@ -77,20 +77,8 @@ template <bool TAKE> __global__ void __launch_bounds__(kThreads) pages_kernel(co
     const int entries = fits ? (int)all : 0;
     if (tid == 0) first[a.seqs] = fits ? (int)s_run : 0;
     __syncthreads();
-    if (tid == 0) {
-        __threadfence();
-        s_last = atomicAdd(a.state + READ, 1) == (int)gridDim.x - 1;
-    }
-    __syncthreads();
-    if (s_last) {                                       // all have read what changes now
-        if (fits)
-            for (int b = tid; b < a.seqs; b += kThreads) a.held[b] = TAKE ? wanted(a, b, from[b]) : from[b];
-        if (tid == 0) {
-            a.state[READ] = 0;
-            if (fits) a.state[FREE] = count + (TAKE ? -entries : entries);
-            else a.state[REFUSED] += 1;
-        }
-    }
+    // (all of this CTA's threads have what they read; who comes last changes it, when its own share is done)
+    if (tid == 0) s_last = atomicAdd(a.state + READ, 1) == (int)gridDim.x - 1;
     auto sequence = [&](const int32_t* starts, int at) {        // the last sequence that begins at or before `at`
         int lo = 0, hi = a.seqs - 1;
         while (lo < hi) {
@@ -115,37 +103,57 @@ template <bool TAKE> __global__ void __launch_bounds__(kThreads) pages_kernel(co
             }
         }
     }
-    if (!TAKE) return;
-    // ---- the rows, some at a time: their sequences and positions, then their slots
-    __shared__ int r_pos[kRows], r_seq[kRows];
-    for (int r0 = blockIdx.x * kRows; r0 < a.rows; r0 += gridDim.x * kRows) {
-        const int n = min(kRows, a.rows - r0);
-        __syncthreads();
-        if (tid < n) {
-            const int r = r0 + tid, b = sequence(a.start, r);
-            const bool in = a.seqs > 0 && r >= a.start[b] && r < a.start[b + 1];
-            const int pos = in ? max(a.lengths[b], 0) + r - a.start[b] : -1;
-            a.row_seq[r] = r_seq[tid] = in ? b : -1;
-            a.positions[r] = r_pos[tid] = pos;
-        }
-        __syncthreads();
-        for (int i = tid; i < n * a.heads; i += kThreads) {
-            const int r = i / a.heads, h = i - r * a.heads, b = r_seq[r], pos = r_pos[r], t = pos / a.tile;
-            int page = -1;
-            if (pos >= 0 && t < a.tiles) {
-                const bool fresh = fits && t >= from[b] && t < from[b] + first[b + 1] - first[b];
-                page = fresh ? a.free[count - 1 - ((int64_t)(first[b] + t - from[b]) * a.heads + h)] : a.table[((int64_t)b * a.heads + h) * a.tiles + t];
+    // ---- the rows, some at a time: their sequences, tiles and places in these, then their slots
+    if (TAKE) {
+        __shared__ int r_tile[kRows], r_at[kRows], r_seq[kRows];
+        const int dh = kThreads % a.heads, dr = kThreads / a.heads;
+        for (int r0 = blockIdx.x * kRows; r0 < a.rows; r0 += gridDim.x * kRows) {
+            const int n = min(kRows, a.rows - r0);
+            __syncthreads();
+            if (tid < n) {
+                const int r = r0 + tid, b = sequence(a.start, r), s0 = a.start[b];
+                const bool in = r >= s0 && r < a.start[b + 1];
+                const int pos = in ? max(a.lengths[b], 0) + r - s0 : -1, t = pos / a.tile;
+                a.row_seq[r] = in ? b : -1;
+                a.positions[r] = pos;
+                r_seq[tid] = b;
+                r_tile[tid] = pos >= 0 && t < a.tiles ? t : -1;
+                r_at[tid] = pos - t * a.tile;
             }
-            a.slots[(int64_t)r0 * a.heads + i] = page < 0 || page >= a.total ? -1 : page * a.tile + pos % a.tile;
+            __syncthreads();
+            int r = tid / a.heads, h = tid - r * a.heads;
+            for (int i = tid; i < n * a.heads; i += kThreads) {
+                const int b = r_seq[r], t = r_tile[r], own = t - from[b];
+                int page = -1;
+                if (t >= 0)
+                    page = fits && own >= 0 && own < first[b + 1] - first[b] ? a.free[count - 1 - ((int64_t)(first[b] + own) * a.heads + h)]
+                                                                            : a.table[((int64_t)b * a.heads + h) * a.tiles + t];
+                a.slots[(int64_t)r0 * a.heads + i] = (unsigned)page < (unsigned)a.total ? page * a.tile + r_at[r] : -1;
+                h += dh;
+                r += dr;
+                if (h >= a.heads) {
+                    h -= a.heads;
+                    ++r;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (s_last) {
+        if (fits)
+            for (int b = tid; b < a.seqs; b += kThreads) a.held[b] = TAKE ? wanted(a, b, from[b]) : from[b];
+        if (tid == 0) {
+            a.state[READ] = 0;
+            if (fits) a.state[FREE] = count + (TAKE ? -entries : entries);
+            else a.state[REFUSED] += 1;
         }
     }
 }
 
-template <bool TAKE> static int launch(const Args& a, int64_t work, cudaStream_t st) {
+template <bool TAKE> static int launch(const Args& a, int64_t ctas, int64_t most, cudaStream_t st) {
     const size_t smem = (size_t)(2 * a.seqs + 1) * 4;
     const cudaError_t e = allow_dynamic_smem<pages_kernel<TAKE>>(smem);
     if (e != cudaSuccess) return (int)e;
-    const int64_t ctas = (work + 4 * kThreads - 1) / (4 * kThreads), most = 4 * (int64_t)device_info().sm_count;
     pages_kernel<TAKE><<<(unsigned)(ctas < 1 ? 1 : ctas > most ? most : ctas), kThreads, smem, st>>>(a);
     PA_RETURN_LAUNCH_STATUS();
 }
@@ -168,7 +176,7 @@ PA_API int pa_take_pages(int32_t* d_table, int num_beams, int num_heads, int num
     PA_CHECK_ARG(usable(a) && rows >= 0 && num_seqs <= num_beams && (num_seqs == 0 || d_start) && (rows == 0 || (num_seqs > 0 && d_row_seq && d_positions && d_slots)));
     if (num_seqs == 0) return PA_OK;
     if (num_seqs > kMostSeqs) return PA_ERR_UNSUPPORTED;
-    return launch<true>(a, (int64_t)rows * num_heads, as_stream(stream));
+    return launch<true>(a, ((int64_t)rows * num_heads + 4 * kThreads - 1) / (4 * kThreads), 4 * (int64_t)device_info().sm_count, as_stream(stream));
 }
 
 PA_API int pa_release_pages(int32_t* d_table, int num_beams, int num_heads, int num_tiles, int tile_size, int total_pages, int32_t* d_free, int32_t* d_held,
@@ -178,6 +186,6 @@ PA_API int pa_release_pages(int32_t* d_table, int num_beams, int num_heads, int 
     PA_CHECK_ARG(usable(a) && num_seqs <= num_beams);
     if (num_seqs == 0) return PA_OK;
     if (num_seqs > kMostSeqs) return PA_ERR_UNSUPPORTED;
-    // (how much goes back the host does not know: as many CTAs as a few drafted rows of every sequence keep busy)
-    return launch<false>(a, (int64_t)num_seqs * num_heads * 4, as_stream(stream));
+    // (how much goes back the host does not know: as many CTAs as a whole table keeps busy)
+    return launch<false>(a, (int64_t)num_seqs * num_heads * num_tiles / (16 * kThreads), device_info().sm_count, as_stream(stream));
 }

@@ -297,15 +297,6 @@ template <typename T> __device__ __forceinline__ float load_chunk(const View<T>&
     }
     return m;
 }
-// sum += v where x is at or above `least`; mask |= bit where it is at or above `lo` and not that
-__device__ __forceinline__ void add_from(double& sum, double v, float x, float least) {
-    asm("{\n\t.reg .pred p;\n\tsetp.ge.f32 p, %1, %2;\n\t@p add.rn.f64 %0, %0, %3;\n\t}" : "+d"(sum) : "f"(x), "f"(least), "d"(v));
-}
-__device__ __forceinline__ void add_and_mark(double& sum, double v, float x, float least, float lo, uint32_t& mask, uint32_t bit) {
-    asm("{\n\t.reg .pred p, q;\n\tsetp.ge.f32 p, %2, %3;\n\tsetp.ge.and.f32 q, %2, %4, !p;\n\t@p add.rn.f64 %0, %0, %5;\n\t@q or.b32 %1, %1, %6;\n\t}"
-        : "+d"(sum), "+r"(mask) : "f"(x), "f"(least), "f"(lo), "d"(v), "r"(bit));
-}
-
 // ------------------------------------------------------------------------------------------------------------------- count
 template <typename T> __global__ void __launch_bounds__(kThreads, 6) count_kernel(const __grid_constant__ Args a) {
     constexpr int N = Word<T>::N;
@@ -604,7 +595,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(
     }
     __syncthreads();
     const float up = s_row.up, lo = s_row.lo, top = s_row.top, floor = s_row.all ? s_row.floor : lo;
-    const bool all = s_row.all, lists = !(lo >= up);    // also what is below; whether any is listed
+    const bool all = s_row.all, lists = !(lo >= up), plain = up == s_row.floor && (top - up) * s_row.scale > 900.0;        // also what is below; whether any is listed; whether all is above
     b.relative_to(top, s_row.scale);
     double above = 0.0, whole = 0.0;
     float least_x = INFINITY, most_x = -INFINITY;
@@ -615,12 +606,18 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(
 #pragma unroll
             for (int e = 0; e < N; ++e) x[e] = widen<T>(w.v[e]);
             uint32_t mine = 0;
-            if (all) {                  // (no infinity: range has left such rows to finish; what has no weight, or is no number: 2^-1021)
+            if (plain) {                // (what has no weight, or is no number, as 2^-900 or less)
+#pragma unroll
+                for (int e = 0; e < N; ++e) above += b.weight<T>(fmaxf(x[e], floor));
+                continue;
+            }
+            if (all) {                  // (no infinity: range has left such rows to finish)
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
                     const double v = exp2_64(fma((double)fmaxf(x[e], floor), b.scale, b.base), b.table);
                     whole += v;
-                    add_and_mark(above, v, x[e], up, lo, mine, 1u << e);
+                    above += x[e] >= up ? v : 0.0;
+                    mine |= (uint32_t)(x[e] >= lo && !(x[e] >= up)) << e;
                 }
             } else {
                 float m = x[0];
@@ -629,8 +626,12 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(
                 if (!__any_sync(kAll, m >= floor)) continue;
                 if (up == up && __any_sync(kAll, m >= up)) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) add_and_mark(above, b.weight<T>(x[e]), x[e], up, lo, mine, 1u << e);
-                } else if (lists) {
+                    for (int e = 0; e < N; ++e) {
+                        const double v = b.weight<T>(x[e]);
+                        above += x[e] >= up ? v : 0.0;
+                    }
+                }
+                if (lists) {
 #pragma unroll
                     for (int e = 0; e < N; ++e) mine |= (uint32_t)(x[e] >= lo && !(x[e] >= up)) << e;
                 }

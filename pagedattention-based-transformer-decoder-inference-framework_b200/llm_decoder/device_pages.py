@@ -59,6 +59,9 @@ class DevicePages:
         host[0], host[4:4 + B], host[4 + B:4 + B + len(free)] = len(free), held, free
         self._state, self._held, self._free = to_device(torch.from_numpy(host), self.device).clone().split_with_sizes([4, B, total_pages])
         pt.device_pages_ = self
+        self._common = (pt.d_table_.data_ptr(), B, pt.num_heads_, pt.num_tiles_, tile_size, total_pages, self._free.data_ptr(), self._held.data_ptr(),
+                        self._state.data_ptr())
+        self._most, self._take, self._release = min(B, MOST_SEQS), _cabi.lib().pa_take_pages, _cabi.lib().pa_release_pages
 
     def _mine(self, what):
         if self.table.device_pages_ is not self:
@@ -73,14 +76,9 @@ class DevicePages:
 
     def _sizes(self, lengths, what):
         lengths = self._vector(lengths, None, "lengths")
-        if lengths.numel() > min(self.table.num_beams_, MOST_SEQS):
-            raise ValueError(f"DevicePages.{what}: at most {min(self.table.num_beams_, MOST_SEQS)} sequences")
+        if lengths.numel() > self._most:
+            raise ValueError(f"DevicePages.{what}: at most {self._most} sequences")
         return lengths
-
-    def _common(self):
-        pt = self.table
-        return (pt.d_table_.data_ptr(), pt.num_beams_, pt.num_heads_, pt.num_tiles_, self.tile_size, self.total_pages, self._free.data_ptr(),
-                self._held.data_ptr(), self._state.data_ptr())
 
     def take(self, lengths, start, rows):
         """Room for new rows start[b] .. start[b + 1] - 1 (`rows` of them in all) behind the first lengths[b] tokens of table row b, for all b below
@@ -95,7 +93,7 @@ class DevicePages:
             raise ValueError("DevicePages.take: rows of the sequences")
         with _cabi.on_device(self.device):
             row_seq, positions, slots = torch.empty(rows * (H + 2), dtype=torch.int32, device=self.device).split_with_sizes((rows, rows, rows * H))
-            _cabi.check(_cabi.lib().pa_take_pages(*self._common(), lengths.data_ptr(), start.data_ptr(), B, rows, row_seq.data_ptr(),
+            _cabi.check(self._take(*self._common, lengths.data_ptr(), start.data_ptr(), B, rows, row_seq.data_ptr(),
                                                   positions.data_ptr(), slots.data_ptr(), _cabi.stream_on(self.device)), "pa_take_pages")
         return NewRows(row_seq, positions, slots.view(rows, H))
 
@@ -105,7 +103,7 @@ class DevicePages:
         self._mine("release")
         lengths = self._sizes(lengths, "release")
         with _cabi.on_device(self.device):
-            _cabi.check(_cabi.lib().pa_release_pages(*self._common(), lengths.data_ptr(), lengths.numel(), _cabi.stream_on(self.device)),
+            _cabi.check(self._release(*self._common, lengths.data_ptr(), lengths.numel(), _cabi.stream_on(self.device)),
                         "pa_release_pages")
 
     def free_pages(self):
