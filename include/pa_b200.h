@@ -1137,7 +1137,7 @@ typedef struct {
     int top_k;
     double top_p, min_p;
 } pa_draw_rules;
-size_t pa_draw_workspace_bytes(int type, int rows, int vocab);
+size_t pa_draw_workspace_bytes(int type, int rows, int vocab, int most_children /* 0 but for pa_verify_drafts */);
 int pa_truncated_softmax(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, float* d_probs,
                          int64_t probs_stride, void* d_workspace, size_t workspace_bytes, pa_stream_t stream);
 int pa_draw_tokens(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, const float* d_uniform, int count,

@@ -63,14 +63,14 @@ struct Row {                        // what range and finish leave
 
 struct Rest {                       // a node whose last child was refused
     double taken, out, total;       // a, Q, the sum of the kept
-    int child, open;                // the next child; whether the rest is to be summed
+    int child;                      // the next one
 };
 
 struct Args {
     const void* logits;
     int64_t stride;
     int rows, vocab, ranks, num_seqs;
-    int row0, chunks, chunk_strips;                         // of the group of rows; chunks of a row, strips of a chunk
+    int row0, group, chunks, chunk_strips;                  // of the group of rows; chunks of a row, strips of a chunk
     int ranked;                                             // whether a rule may need an order (top_k, top_p, min_p)
     uint32_t* hist;                                         // workspace: [chunks of the group][kBins]
     Near* list;                                             // [chunks][kList]
@@ -78,6 +78,8 @@ struct Args {
     Row* row;
     Rest* rest;
     double* rest_sum;                                       // [chunks]
+    int32_t *open, *opened;                                 // of every round, how many rows are open, and which
+    int round;
     const int32_t* row_seq;
     const float *temperature, *top_p, *min_p;               // per sequence; null: the value beside it
     const int32_t* top_k;
@@ -575,6 +577,10 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(
     if (tid == 0) {
         s_listed = 0;
         s_first = INT_MAX;
+        if (blockIdx.x == 0 && a.open) {
+            if (!a.ranked) wait_for_last();
+            for (int i = 0; i <= a.round; ++i) a.open[i] = 0;           // (here: how many rounds there may be)
+        }
         if (a.ranked) {
             wait_for_last();
             s_row = a.row[local];
@@ -743,8 +749,8 @@ struct Finish : Weigher {
     bool by_chunks = true;          // the sums are the chunks', in the first CTA
     bool left = false;              // has arrived at the last barrier
 
-    __device__ Finish(const Args& args, Shared& shared, uint32_t* bits) :
-        Weigher(shared), a(args), sh(shared), rank((int)cluster_ctarank()), local((int)(blockIdx.x / args.ranks)), row(args.row0 + local), view(args, row), gone(bits) {
+    __device__ Finish(const Args& args, Shared& shared, uint32_t* bits, int of_group) :
+        Weigher(shared), a(args), sh(shared), rank((int)cluster_ctarank()), local(of_group), row(args.row0 + local), view(args, row), gone(bits) {
         const int parts = a.ranks * kWarps, part = rank * kWarps + warp;
         s0 = (int)((int64_t)view.strips * part / parts);
         s1 = (int)((int64_t)view.strips * (part + 1) / parts);
@@ -1289,6 +1295,35 @@ struct Finish : Weigher {
         __syncthreads();
     }
 
+    // by a warp: the first of n sums up to which they exceed `target` (else, by rounding, the last that is anything), and what is before it
+    __device__ __forceinline__ int locate(const double* t, int n, double target, double& before) const {
+        const int each = (n + 31) / 32, i0 = min(lane * each, n), i1 = min(i0 + each, n);
+        double own = 0.0;
+        for (int i = i0; i < i1; ++i) own += t[i];
+        double to = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double q = __shfl_up_sync(kAll, to, o);
+            if (lane >= o) to += q;
+        }
+        const double from = before + (to - own);
+        int hit = -1;
+        double run = from, at = from;
+        bool open = true;
+        for (int i = i0; i < i1; ++i) {
+            if (open && t[i] > 0.0) {
+                hit = i;
+                at = run;
+                open = !(run + t[i] > target);
+            }
+            run += t[i];
+        }
+        const uint32_t over = __ballot_sync(kAll, !open), some = __ballot_sync(kAll, hit >= 0);
+        const int who = over ? __ffs(over) - 1 : some ? 31 - __clz(some) : 0;
+        before = __shfl_sync(kAll, at, who);
+        return max(__shfl_sync(kAll, hit, who), 0);
+    }
+
     // ---- the first token up to which the sums of f(x, token) exceed `target`; -1 in the CTAs that it is not in.  `part` is where it is
     // (f of a word's tokens: their weights)
     template <typename F> __device__ int search(double target, bool last, int& part, F f) {
@@ -1313,19 +1348,7 @@ struct Finish : Weigher {
             left = true;
         }
         if (owner != rank) return -1;
-        run = mine;
-        part = 0;
-        open = true;
-        const int parts = by_chunks ? a.chunks : kWarps;
-        for (int c = 0; c < parts; ++c) {
-            const double t = by_chunks ? sh.chunk[c] : sh.seg[c];
-            if (open && t > 0.0) {
-                part = c;
-                mine = run;
-                open = !(run + t > target);
-            }
-            run += t;
-        }
+        part = locate(by_chunks ? sh.chunk : sh.seg, by_chunks ? a.chunks : kWarps, target, mine);
         const int of = rank * kWarps + part, all = a.ranks * kWarps;
         const int e0 = by_chunks ? part * a.chunk_strips : (int)((int64_t)view.strips * of / all);
         const int n = (by_chunks ? min(e0 + a.chunk_strips, view.strips) : (int)((int64_t)view.strips * (of + 1) / all)) - e0;
@@ -1339,18 +1362,7 @@ struct Finish : Weigher {
         });
         __syncthreads();
         if (warp == 0) {
-            run = mine;
-            int at = 0;
-            open = true;
-            for (int i = 0; i < n; ++i) {
-                const double t = sh.strip[i];
-                if (open && t > 0.0) {
-                    at = i;
-                    mine = run;
-                    open = !(run + t > target);
-                }
-                run += t;
-            }
+            const int at = locate(sh.strip, n, target, mine);
             const int v = view.token(e0 + at, lane);
             double w[N], to = 0.0;
             f(view.load(e0 + at, lane), v, w);
@@ -1417,15 +1429,22 @@ struct Finish : Weigher {
                 const int of = rank * kWarps + part, all = a.ranks * kWarps;
                 const int e0 = by_chunks ? part * a.chunk_strips : (int)((int64_t)view.strips * of / all);
                 const int e1 = by_chunks ? min(e0 + a.chunk_strips, view.strips) : (int)((int64_t)view.strips * (of + 1) / all);
+                const int own = (v + view.off) / STRIP;         // its strip has changed
+                if (warp == 0) {
+                    const double t = warp_sum(word_sum(view.load(own, lane), view.token(own, lane)));
+                    if (lane == 0) sh.strip[own - e0] = t;
+                }
+                __syncthreads();
                 double sum = 0.0;
-                view.template each<4>(e0 + warp, e1, kWarps, lane, [&](const Word<T>& x, int, int t) { sum += word_sum(x, t); });
+                for (int s = tid; s < e1 - e0; s += kThreads) sum += sh.strip[s];
                 sum = over(sum, sh.part, Add());
                 if (tid == 0) (by_chunks ? sh.chunk[part] : sh.seg[part]) = sum;
             }
             __syncthreads();
             if (by_chunks) {
                 total = 0.0;
-                for (int c = 0; c < a.chunks; ++c) total += sh.chunk[c];
+                for (int c = tid; c < a.chunks; c += kThreads) total += sh.chunk[c];
+                total = over(total, sh.part, Add());
             } else {
                 publish();
                 cluster_sync();
@@ -1475,8 +1494,10 @@ struct Finish : Weigher {
             if (a.distinct) st.out += qc;
             if (S > 0.0) {
                 st.child = i + 1;
-                st.open = 1;
-                if (rank == 0 && tid == 0) a.rest[local] = st;
+                if (rank == 0 && tid == 0) {
+                    a.rest[local] = st;
+                    a.opened[(int64_t)a.round * a.group + atomicAdd(a.open + a.round, 1)] = local;      // (their order changes nothing)
+                }
                 return true;
             }
         }
@@ -1487,11 +1508,17 @@ struct Finish : Weigher {
         const float u = a.uniform[2 * (int64_t)row + 1];
         int part;
         const int v = search((u > 0.f ? (double)u : 0.0) * S, true, part, [&](const Word<T>& x, int token, double (&w)[N]) {
+            float y[N];
+            if (taken > 0.0)            // (of places outside the row, whose weights are 0, any)
+#pragma unroll
+                for (int e = 0; e < N; ++e) y[e] = widen<Q>(q[min(max(token + e, 0), view.V - 1)]);
             kept_of(x, token, w);
             if (taken > 0.0)
 #pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (w[e] > 0.0) w[e] = fmax(w[e] - taken * (double)widen<Q>(q[token + e]), 0.0);
+                for (int e = 0; e < N; ++e) {
+                    const double u = w[e] - taken * (double)y[e];
+                    w[e] = u > 0.0 ? u : 0.0;
+                }
         });
         if (v >= 0 && warp == 0) {
             const double w = kept(view.at(v), v);
@@ -1508,7 +1535,6 @@ struct Finish : Weigher {
             out.border = border;
             out.only = only;
             out.scale = scale;
-            a.rest[local] = st;
             if (!(total > 0.0)) put(0, -1, 0.0);
         }
         if (!(total > 0.0)) return;
@@ -1516,12 +1542,7 @@ struct Finish : Weigher {
         if (!tests(st, total)) draw_from(total, 0.0, total);
     }
     __device__ void go_on() {
-        wait_for_last();
-        Rest st = a.rest[local];
-        if (!st.open) return;
-        __syncthreads();
-        st.open = 0;
-        if (tid == 0) a.rest[local] = st;
+        const Rest st = a.rest[local];
         const Row in = a.row[local];
         top = in.top;
         border = in.border;
@@ -1546,7 +1567,7 @@ template <typename T, typename Q, int MODE> __global__ void __launch_bounds__(kT
         __syncthreads();
     }
     let_next_start();
-    Finish<T, Q, MODE> p(a, sh, MODE == DRAW && a.count > 1 ? bits : nullptr);
+    Finish<T, Q, MODE> p(a, sh, MODE == DRAW && a.count > 1 ? bits : nullptr, (int)(blockIdx.x / a.ranks));
     if constexpr (MODE == PROBS) p.probs();
     else if constexpr (MODE == DRAW) p.draw();
     else p.verify();
@@ -1560,11 +1581,13 @@ template <typename T, typename Q> __global__ void __launch_bounds__(kThreads, 3)
     constexpr int N = Word<T>::N, QN = 16 / (int)sizeof(Q), SOME = sizeof(T) < 4 ? 2 : 4;
     __shared__ double s_part[kWarps];
     Block b;
-    const int local = blockIdx.x / a.chunks, c = blockIdx.x - local * a.chunks, row = a.row0 + local, lane = b.lane;
+    const int lane = b.lane;
     let_next_start();
     wait_for_last();
+    const int all = a.open[a.round - 1] * a.chunks;
+    for (int i = blockIdx.x; i < all; i += gridDim.x) {
+    const int local = a.opened[(int64_t)(a.round - 1) * a.group + i / a.chunks], c = i % a.chunks, row = a.row0 + local;
     const Rest st = a.rest[local];
-    if (!st.open) return;
     const View<T> view(a, row);
     const Row r = a.row[local];
     b.relative_to(r.top, r.scale);
@@ -1619,14 +1642,18 @@ template <typename T, typename Q> __global__ void __launch_bounds__(kThreads, 3)
         }
     }
     sum = b.over(sum, s_part, Add());
-    if (b.tid == 0) a.rest_sum[blockIdx.x] = sum;
+    if (b.tid == 0) a.rest_sum[(int64_t)local * a.chunks + c] = sum;
+    }
 }
 
 // Where a node's tests go on after that
 template <typename T, typename Q> __global__ void __launch_bounds__(kThreads) go_on_kernel(const __grid_constant__ Args a) {
     __shared__ Shared sh;
     let_next_start();
-    Finish<T, Q, VERIFY> p(a, sh, nullptr);
+    wait_for_last();
+    const int i = blockIdx.x;           // of the rows that are open, which a list has
+    if (i >= a.open[a.round - 1]) return;
+    Finish<T, Q, VERIFY> p(a, sh, nullptr, a.opened[(int64_t)(a.round - 1) * a.group + i]);
     p.go_on();
 }
 
@@ -1681,6 +1708,7 @@ static Cut cut_of(int type, int rows, int vocab) {
     return c;
 }
 static size_t row_bytes(const Cut& c) { return (size_t)c.chunks * (kBins * 4 + kList * sizeof(Near) + sizeof(Chunk) + sizeof(double)) + sizeof(Row) + sizeof(Rest); }
+static size_t round_bytes(const Cut& c) { return ((size_t)c.group + 1) * 4; }
 
 template <auto Kernel> static cudaError_t start(const Args& a, unsigned ctas, unsigned cluster, size_t smem, bool first, cudaStream_t st) {
     const cudaError_t e = smem ? allow_dynamic_smem<Kernel>(smem) : cudaSuccess;
@@ -1729,6 +1757,13 @@ template <typename T, typename Q, int MODE> static int launch(Args a, int type, 
     a.rest = reinterpret_cast<Rest*>(at);
     at += c.group * sizeof(Rest);
     a.row = reinterpret_cast<Row*>(at);
+    at += c.group * sizeof(Row);
+    if (MODE == VERIFY) {
+        a.open = reinterpret_cast<int32_t*>(at);
+        a.opened = a.open + most_children + 1;
+    }
+    a.group = c.group;
+    a.round = most_children;
     const int rows = a.rows;
     for (int r = 0; r < rows; r += c.group) {
         a.row0 = r;
@@ -1739,14 +1774,16 @@ template <typename T, typename Q, int MODE> static int launch(Args a, int type, 
             if (e == cudaSuccess) e = start<range_kernel<T>>(a, some, 0, 0, false, st);
         }
         if (e == cudaSuccess) e = start<sum_kernel<T>>(a, ctas, 0, 0, !a.ranked, st);
-        if (e == cudaSuccess) e = start<finish_kernel<T, Q, MODE>>(a, some * a.ranks, a.ranks, MODE == DRAW && a.count > 1 ? (size_t)(a.vocab + 31) / 32 * 4 : 0, false, st);
+        Args f = a;
+        f.round = 0;
+        if (e == cudaSuccess) e = start<finish_kernel<T, Q, MODE>>(f, some * a.ranks, a.ranks, MODE == DRAW && a.count > 1 ? (size_t)(a.vocab + 31) / 32 * 4 : 0, false, st);
         if (e == cudaSuccess && MODE == PROBS) e = start<write_kernel<T>>(a, ctas, 0, 0, false, st);
         if constexpr (MODE == VERIFY) {
-            Args one = a;
-            one.ranks = 1;
-            for (int i = 0; i < most_children && e == cudaSuccess; ++i) {
-                e = start<rest_kernel<T, Q>>(one, ctas, 0, 0, false, st);
-                if (e == cudaSuccess) e = start<go_on_kernel<T, Q>>(one, some, 0, 0, false, st);
+            f.ranks = 1;                // (few nodes come so far)
+            const unsigned sms = (unsigned)std::max(1, device_info().sm_count);
+            for (f.round = 1; f.round <= most_children && e == cudaSuccess; ++f.round) {
+                e = start<rest_kernel<T, Q>>(f, std::min(ctas, 16 * sms), 0, 0, false, st);
+                if (e == cudaSuccess) e = start<go_on_kernel<T, Q>>(f, some, 0, 0, false, st);
             }
         }
         if (e != cudaSuccess) return (int)e;
@@ -1787,10 +1824,10 @@ static bool usable(const void* logits, int type, int64_t stride, int rows, int v
 
 using namespace pa;
 
-PA_API size_t pa_draw_workspace_bytes(int type, int rows, int vocab) {
-    if (rows <= 0 || vocab <= 0 || type < PA_TYPE_F32 || type > PA_TYPE_BF16) return 0;
+PA_API size_t pa_draw_workspace_bytes(int type, int rows, int vocab, int most_children) {
+    if (rows <= 0 || vocab <= 0 || most_children < 0 || type < PA_TYPE_F32 || type > PA_TYPE_BF16) return 0;
     const drawn::Cut c = drawn::cut_of(type, rows, vocab);
-    return drawn::row_bytes(c) * c.group;
+    return drawn::row_bytes(c) * c.group + drawn::round_bytes(c) * ((size_t)most_children + 1);
 }
 
 PA_API int pa_truncated_softmax(const void* d_logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules, float* d_probs,
@@ -1804,7 +1841,7 @@ PA_API int pa_truncated_softmax(const void* d_logits, int type, int64_t stride, 
     PA_CHECK_ARG(in >= out_end || out >= in_end);
     Args a = args(d_logits, stride, rows, vocab, rules);
     a.probs = d_probs; a.probs_stride = probs_stride;
-    if (!holds(d_workspace, workspace_bytes, pa_draw_workspace_bytes(type, rows, vocab))) return PA_ERR_WORKSPACE;
+    if (!holds(d_workspace, workspace_bytes, pa_draw_workspace_bytes(type, rows, vocab, 0))) return PA_ERR_WORKSPACE;
     return launch<PROBS>(a, type, 0, 0, d_workspace, as_stream(stream));
 }
 
@@ -1816,7 +1853,7 @@ PA_API int pa_draw_tokens(const void* d_logits, int type, int64_t stride, int ro
     PA_CHECK_ARG(d_uniform && d_ids);
     Args a = args(d_logits, stride, rows, vocab, rules);
     a.uniform = d_uniform; a.count = count; a.ids = d_ids; a.logprobs = d_logprobs;
-    if (!holds(d_workspace, workspace_bytes, pa_draw_workspace_bytes(type, rows, vocab))) return PA_ERR_WORKSPACE;
+    if (!holds(d_workspace, workspace_bytes, pa_draw_workspace_bytes(type, rows, vocab, 0))) return PA_ERR_WORKSPACE;
     return launch<DRAW>(a, type, 0, 0, d_workspace, as_stream(stream));
 }
 
@@ -1832,6 +1869,6 @@ PA_API int pa_verify_drafts(const void* d_logits, int type, int64_t stride, int 
     a.uniform = d_uniform; a.count = 1; a.ids = d_ids; a.logprobs = d_logprobs;
     a.tokens = d_tokens; a.parents = d_parents; a.node_start = d_node_start; a.draft = d_draft; a.draft_stride = draft_stride;
     a.draft_count = draft_count; a.draft_rows = d_draft_rows; a.distinct = distinct;
-    if (!holds(d_workspace, workspace_bytes, pa_draw_workspace_bytes(type, rows, vocab))) return PA_ERR_WORKSPACE;
+    if (!holds(d_workspace, workspace_bytes, pa_draw_workspace_bytes(type, rows, vocab, most_children))) return PA_ERR_WORKSPACE;
     return launch<VERIFY>(a, type, draft_type, most_children, d_workspace, as_stream(stream));
 }

@@ -252,7 +252,7 @@ _SIGS = {
     "pa_tree_accept": ([_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, C.POINTER(_vp),
                         _vp, _vp, _vp, _vp, _vp], _i32),
     # sampling with drafted tokens (draw_tokens.cu), pages handed out on the GPU (device_pages.cu)
-    "pa_draw_workspace_bytes": ([_i32, _i32, _i32], _sz),
+    "pa_draw_workspace_bytes": ([_i32, _i32, _i32, _i32], _sz),
     "pa_truncated_softmax": ([_vp, _i32, _i64, _i32, _i32, C.POINTER(DrawRules), _vp, _i64, _vp, _sz, _vp], _i32),
     "pa_draw_tokens": ([_vp, _i32, _i64, _i32, _i32, C.POINTER(DrawRules), _vp, _i32, _vp, _vp, _vp, _sz, _vp], _i32),
     "pa_verify_drafts": ([_vp, _i32, _i64, _i32, _i32, C.POINTER(DrawRules), _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _sz,

@@ -240,9 +240,9 @@ _MOST_ROW_BYTES = 1500000               # PA_DRAW_MOST_ROW_BYTES
 _draw_spaces = _cabi.PerThread()        # workspaces of the calls below
 
 
-def _draw_space(args, dev, stream):
+def _draw_space(args, dev, stream, children=0):
     """(address, bytes) of a workspace for a call over these logits on a stream, and the tensor."""
-    need = _cabi.lib().pa_draw_workspace_bytes(args[1], args[3], args[4])
+    need = _cabi.lib().pa_draw_workspace_bytes(args[1], args[3], args[4], children)
     if _cabi.capturing(stream):         # a graph has a workspace of its own: its replays may run beside other calls
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
     else:
@@ -329,7 +329,7 @@ def verify_drafts(logits, tree, uniform, draft_probs, draft_rows=None, temperatu
     if rows:
         with _cabi.on_device(dev):
             stream = _cabi.stream_on(dev)
-            at, need, ws = _draw_space(args, dev, stream)
+            at, need, ws = _draw_space(args, dev, stream, tree.branches)
             _cabi.check(_cabi.lib().pa_verify_drafts(
                 *args, uniform.data_ptr(), tree.tokens.data_ptr(), tree.parents.data_ptr(), tree.node_start.data_ptr(), tree.branches,
                 draft_probs.data_ptr() if n else None,

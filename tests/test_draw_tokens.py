@@ -305,7 +305,7 @@ def test_refused_on_the_host():
             call()
     lib, ref = _cabi.lib(), __import__("ctypes").byref
     rules, ws = _cabi.DrawRules(num_seqs=4, temperature=1.0, top_p=1.0), (0x10000, 1 << 30)
-    assert lib.pa_draw_workspace_bytes(0, 4, 8) > 0 and lib.pa_draw_workspace_bytes(0, 0, 8) == lib.pa_draw_workspace_bytes(3, 4, 8) == 0
+    assert lib.pa_draw_workspace_bytes(0, 4, 8, 0) > 0 and lib.pa_draw_workspace_bytes(0, 0, 8, 0) == lib.pa_draw_workspace_bytes(3, 4, 8, 0) == 0
     assert lib.pa_truncated_softmax(None, 0, 8, 4, 8, ref(rules), 0x1000, 8, *ws, None) == -1
     assert lib.pa_truncated_softmax(0x1000, 0, 7, 4, 8, ref(rules), 0x9000, 8, *ws, None) == -1
     assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, ref(rules), 0x9000, 7, *ws, None) == -1
