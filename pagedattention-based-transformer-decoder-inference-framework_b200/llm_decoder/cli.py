@@ -3,10 +3,12 @@
     python -m llm_decoder.cli generate --model DIR --prompt 5,17,3 [--prompt ...] --max-new-tokens 16
                                        [--dtype bfloat16|float32] [--temperature T --top-k K --top-p P --seed S]
                                        [--drafts N --repetition-penalty R --presence-penalty P --frequency-penalty F]
+                                       [--sample --temperature T --top-k K --top-p P --min-p M --seed S]
     python -m llm_decoder.cli trace    --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N   (bin/trace_run)
 
 --drafts and the penalties are for CUDADecoder and INT8Decoder, greedily: up to N guesses of the next tokens, looked up in the sequence
-itself, are verified in every step (decoders.generate_drafted).
+itself, are verified in every step (decoders.generate_drafted).  --sample, for these too: tokens are drawn by chance, with --drafts or without,
+from the distribution that temperature, top k, top p and min p leave.
 
 `trace` replays a schedule from standard input, one JSON object per line:
     {"step": 0, "entries": [{"id": "a", "tokens": [5, 17, 3], "want": [0, 2]}], "end": []}
@@ -89,11 +91,17 @@ def generate_main(argv=None):
     ap.add_argument("--repetition-penalty", type=float, default=1.0)
     ap.add_argument("--presence-penalty", type=float, default=0.0)
     ap.add_argument("--frequency-penalty", type=float, default=0.0)
+    ap.add_argument("--sample", action="store_true")
+    ap.add_argument("--min-p", type=float, default=0.0)
     a = ap.parse_args(argv)
     rules = dict(repetition=a.repetition_penalty, presence=a.presence_penalty, frequency=a.frequency_penalty)
-    drafted = a.drafts != 0 or rules != dict(repetition=1.0, presence=0.0, frequency=0.0)
-    if drafted and (a.temperature != 1.0 or a.top_k > 0 or a.top_p < 1.0):
-        ap.error("--drafts and the penalties go with greedy generation")
+    drafted = a.sample or a.drafts != 0 or rules != dict(repetition=1.0, presence=0.0, frequency=0.0)
+    if drafted and not a.sample and (a.temperature != 1.0 or a.top_k > 0 or a.top_p < 1.0):
+        ap.error("--drafts and the penalties go with greedy generation, or with --sample")
+    if a.min_p != 0.0 and not a.sample:
+        ap.error("--min-p goes with --sample")
+    if a.sample:
+        rules.update(temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, min_p=a.min_p, seed=a.seed)
     _ensure_library()
     from .registry import load_model
     prompts = [[int(t) for t in p.split(",") if t.strip()] for p in a.prompt]

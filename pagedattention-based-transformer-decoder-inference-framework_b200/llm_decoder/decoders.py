@@ -101,7 +101,10 @@ class _DecoderBase:
 
     def __init__(self, num_layers, num_heads, head_dim, hidden_dim, vocab_size, max_seq_len, *, device=None,
                  tile_size=16, batch_size=1, attn_temperature=1.0, use_overlap=None, use_cuda_graph=True,
-                 use_prefill=True):
+                 use_prefill=True, kv_tokens=None):
+        """kv_tokens: the K/V pools hold so many tokens, for all sequences together (each rounded up to whole tiles), and hand out their
+        pages on the GPU as the sequences grow (DevicePages), instead of max_seq_len tokens for every sequence; a call that finds too few
+        raises.  forward_tokens alone does not look: `pages.check()`."""
         if min(num_layers, num_heads, head_dim, hidden_dim, vocab_size, max_seq_len) <= 0:
             raise ValueError("decoder dimensions must be positive")
         if hidden_dim != num_heads * head_dim:
@@ -113,6 +116,9 @@ class _DecoderBase:
         self.hidden_dim_, self.vocab_size_, self.max_seq_len_ = hidden_dim, vocab_size, max_seq_len
         self.inter_dim_ = hidden_dim * 4  # decoder_block.hpp:28
         self.tile_size_ = tile_size
+        if kv_tokens is not None and kv_tokens <= 0:
+            raise ValueError("kv_tokens must be positive")
+        self.kv_tokens, self.pages = kv_tokens, None
         self.attn_temperature = float(attn_temperature)  # AttentionCUDA::forward default (attention_config.hpp:19)
         self.use_overlap = use_overlap
         self.use_cuda_graph = use_cuda_graph
@@ -134,12 +140,20 @@ class _DecoderBase:
         nt = (self.max_seq_len_ + self.tile_size_ - 1) // self.tile_size_
         self._batch, self._num_tiles = B, nt
         table = np.arange(B * H * nt, dtype=np.int32).reshape(B, H, nt)
-        self.kv_caches = []
+        few = None if self.kv_tokens is None else H * min(B * nt, -(-self.kv_tokens // self.tile_size_))
+        self.kv_caches, self.pages = [], None
         for _ in range(self.num_layers_):
             kvc = KVTileCache(self.KV_DTYPE, device=dev)
-            kvc.init(B * H * nt, self.tile_size_, D)
-            kvc.configure_table(B, H, nt)
-            kvc.page_table_.load_host_table(table)
+            kvc.init(B * H * nt if few is None else few, self.tile_size_, D)
+            if few is None:
+                kvc.configure_table(B, H, nt)
+                kvc.page_table_.load_host_table(table)
+            elif self.pages is None:            # one table for all layers, whose pages the GPU hands out
+                kvc.configure_table(B, H, nt)
+                self.pages = kvc.pages_on_device()
+                self._starts = torch.arange(B + 1, dtype=torch.int32, device=dev)       # a row for each sequence
+            else:
+                kvc.share_pages(self.kv_caches[0])
             self.kv_caches.append(kvc)
         f32 = dict(dtype=torch.float32, device=dev)
         self.ids = torch.zeros(B, dtype=torch.int32, device=dev)
@@ -153,9 +167,11 @@ class _DecoderBase:
         self._step_warm = 0  # a new batch size gets one eager step before capture (lazy buffers, GEMM scratch)
 
     def reset(self):
-        """Forget all cached context (positions back to 0; pages keep their assignment)."""
+        """Forget all cached context (positions back to 0; pages keep their assignment, or, with kv_tokens, go back)."""
         self.positions.zero_()
         self.ctx_lens.fill_(1)
+        if self.pages is not None:
+            self.pages.release(self.positions)
 
     # ------------------------------------------------------------------ device step
     def _chk(self, st, what):
@@ -270,6 +286,8 @@ class _DecoderBase:
     def _step(self):
         """One decode step for the B tokens in self.ids at self.positions; writes the greedy next
         ids back into self.ids and advances positions.  Device work only (CUDA-graph capturable)."""
+        if self.pages is not None:
+            self.pages.take(self.positions, self._starts, self._batch)
         self._layers(self.bufs, self.ids, self.positions, self.ctx_lens, None, self._ws)
         self._head(self.bufs.x)
         self._chk(self._lib.pa_advance_positions(self.positions.data_ptr(), self.ctx_lens.data_ptr(), self._batch,
@@ -290,6 +308,8 @@ class _DecoderBase:
         beam = torch.arange(B, dtype=torch.int32, device=dev).repeat_interleave(n)
         ws = torch.empty(self._lib.pa_decode_workspace_bytes(R, self.num_heads_, self.head_dim_, self._num_tiles,
                                                              self.tile_size_), dtype=torch.uint8, device=dev)
+        if self.pages is not None:
+            self.pages.take(torch.zeros_like(self.positions), self._starts * n, R)
         self._layers(bf, prompt.reshape(-1).contiguous(), positions, ctx, beam, ws, prefill_shape=(B, n))
         if head:
             self._head(bf.x.view(B, n, self.hidden_dim_)[:, n - 1, :].contiguous())
@@ -375,10 +395,12 @@ class _DecoderBase:
                 if i + 1 < max_len:
                     self._step_or_replay()
             gen_host = gen.t().cpu().tolist()  # the only synchronisation of the call
+            if self.pages is not None:
+                self.pages.check()
         return [list(p) + g for p, g in zip(prompts, gen_host)]
 
     def generate_drafted(self, prompts, max_len, drafts=16, branches=2, draft=None, repetition=1.0, presence=0.0, frequency=0.0,
-                         bias=None, allowed=None):
+                         bias=None, allowed=None, temperature=None, top_k=0, top_p=1.0, min_p=0.0, seed=None, distinct=False):
         """generate_batch's greedy tokens in fewer steps: every step runs the pending token of each sequence and up to `drafts` guesses
         of what follows it, and keeps the guesses that the model itself would have given (draft_tree.py).  What the guesses are
         changes the number of steps (`drafted_steps_` afterwards) and not the tokens, up to ties within the rounding of the logits.
@@ -386,7 +408,14 @@ class _DecoderBase:
         draft(tokens, most, depth) -> (parents, tokens) of a sequence's tree, at most `most` nodes in paths of at most `depth`, whose node 0 is
         the last of `tokens`; the default looks for what followed when the last tokens came up before (lookup_drafts).
         repetition, presence, frequency: sampling.adjust_logits' penalties for tokens of the prompt and those generated (a number, or one
-        per sequence); bias: (tokens, values, start [sequences + 1]); allowed: a mask [sequences, words] of int32, both as there."""
+        per sequence); bias: (tokens, values, start [sequences + 1]); allowed: a mask [sequences, words] of int32, both as there.
+
+        temperature: tokens are drawn by chance, from sampling.truncated_softmax's distribution with temperature, top_k, top_p and min_p (a number,
+        or one per sequence; the temperature counts as generate's does).  The i-th token of a sequence is drawn by a number that `seed` gives it,
+        so that guesses do not change the tokens here either.  A `draft` that draws its guesses by chance from a model of its own returns
+        (parents, tokens, probs): probs [nodes, vocab] on the device, row i of which is what the children of node i were drawn from, in order (with
+        distinct=True each from what the ones before it left; of nodes without children anything).  They are kept or replaced by
+        sampling.verify_drafts: the tokens then depend on the guesses, their distribution does not."""
         B, n = len(prompts), len(prompts[0]) if prompts else 0
         if n == 0 or any(len(p) != n for p in prompts):
             raise ValueError("prompts must be non-empty and of equal length")
@@ -397,6 +426,8 @@ class _DecoderBase:
         if max_len <= 0:
             return [list(p) for p in prompts]
         given, draft = draft, draft or (lambda tokens, most, depth: lookup_drafts(tokens, most, depth, branches))
+        if temperature is None and (top_k, top_p, min_p) != (0, 1.0, 0.0):
+            raise ValueError("top_k, top_p and min_p go with a temperature")
         self._setup_batch(B)
         self.reset()
         self._sampling = None
@@ -411,13 +442,23 @@ class _DecoderBase:
             if allowed is not None:
                 allowed = on_device(allowed, torch.int32)
             plain = all(isinstance(x, (int, float)) for x in per_seq) and (*per_seq,) == (1, 0, 0)
+            if temperature is not None:
+                of = lambda x, dtype: x if isinstance(x, (int, float)) else on_device(x, dtype)  # noqa: E731
+                chance = dict(temperature=of(temperature, torch.float32), top_k=of(top_k, torch.int32), top_p=of(top_p, torch.float32),
+                              min_p=of(min_p, torch.float32))
+                if not self.ARGMAX_DIVIDE:      # logits times the temperature
+                    t = chance["temperature"]
+                    chance["temperature"] = 1.0 / t if isinstance(t, torch.Tensor) or t else float("inf")
+                gen = torch.Generator(device=dev)
+                gen.manual_seed(0 if seed is None else int(seed))
+                numbers = torch.rand((B, max_len), device=dev, generator=gen)
             seqs = [np.asarray(p, dtype=np.int32) for p in prompts]
             if n > 1:       # all but the last token of a prompt, which is the first pending one
                 self._prefill(to_device(torch.from_numpy(np.stack(seqs)[:, :-1].copy()), dev), head=False)
             ctx = torch.full((B,), n - 1, dtype=torch.int32, device=dev)
             caches, bufs = TreeCaches(self.kv_caches), None
             while any(len(s) < n + max_len for s in seqs):
-                parents, tokens = [], []
+                parents, tokens, probs = [], [], []
                 for s in seqs:
                     left, room = n + max_len - len(s), self.max_seq_len_ - len(s) + 1        # tokens to come; rows that the cache takes
                     if left == 0:
@@ -425,7 +466,11 @@ class _DecoderBase:
                     elif left == 1 or drafts == 0:
                         p, t = [-1], s[-1:]
                     else:
-                        p, t = draft(s, min(1 + drafts, room), left)
+                        p, t, *q = draft(s, min(1 + drafts, room), left)
+                        if len(q) == 1 and temperature is not None and isinstance(q[0], torch.Tensor) and q[0].shape == (len(p), self.vocab_size_):
+                            probs.append((len(parents), q[0]))
+                        elif q:
+                            raise ValueError("draft: probabilities [nodes, vocab] on the device, and a temperature")
                         if not 1 <= len(p) <= min(1 + drafts, room) or len(t) != len(p) or int(t[0]) != int(s[-1]):
                             raise ValueError("draft: between one and `most` nodes, the first of them the sequence's last token")
                         if given and longest_path(p) > left:
@@ -436,20 +481,46 @@ class _DecoderBase:
                 if bufs is None or bufs.R < tree.rows:
                     bufs = _Bufs(max(tree.rows, B * (1 + drafts)), self.hidden_dim_, self.inter_dim_, dev)
                 bf = bufs.first(tree.rows)
+                if self.pages is not None:
+                    self.pages.take(ctx, tree.node_start, tree.rows)
                 self._layers(bf, tree.tokens, tree.positions(ctx), ctx, tree.row_seq, None, tree=tree)
                 history = start = None
                 if not plain:       # the tokens before the pending one; a node's path counts by itself
                     history = to_device(torch.from_numpy(np.concatenate([s[:-1] for s in seqs] + [np.zeros(1, np.int32)])), dev)
                     start = to_device(torch.from_numpy(np.cumsum([0] + [len(s) - 1 for s in seqs], dtype=np.int32)), dev)
-                ids = sampling.adjusted_argmax(self._node_logits(bf), history, start, *per_seq, bias=bias, allowed=allowed,
-                                               allowed_rows=None if allowed is None else tree.row_seq, tree=tree)
+                logits, kw = self._node_logits(bf), dict(bias=bias, allowed=allowed, allowed_rows=None if allowed is None else tree.row_seq, tree=tree)
+                if temperature is None:
+                    ids = sampling.adjusted_argmax(logits, history, start, *per_seq, **kw)
+                else:
+                    if not plain or bias is not None or allowed is not None:
+                        sampling.adjust_logits(logits, history, start, *per_seq, out=logits, **kw)
+                    which = (ctx[tree.row_seq] + tree.depths - (n - 1)).clamp_(max=max_len - 1)      # of the sequence's tokens: the one behind a node
+                    u = numbers[tree.row_seq.long(), which.long()]
+                    if not probs:
+                        ids = sampling.draw_tokens(logits, u, tree=tree, **chance)
+                    else:
+                        rows, at = np.full(tree.rows, -1, dtype=np.int32), 0
+                        first = np.cumsum([0] + tree.sizes)
+                        for b, q in probs:
+                            rows[first[b]:first[b + 1]] = np.arange(at, at + len(q))
+                            at += len(q)
+                        tests = torch.rand(tree.rows, device=dev, generator=gen)
+                        q = probs[0][1].contiguous() if len(probs) == 1 else torch.cat([q for _b, q in probs])
+                        ids = sampling.verify_drafts(logits, tree, torch.stack((tests, u), 1), q, to_device(torch.from_numpy(rows), dev),
+                                                     distinct=distinct, **chance)
                 done = tree_accept(ids, tree, caches, ctx)
                 ctx = done.ctx_lens
+                if self.pages is not None:
+                    self.pages.release(ctx)
                 got = torch.cat((done.counts[:, None], done.tokens), 1).cpu().numpy()       # the step's synchronisation
+                if temperature is not None and any((g[1:1 + g[0]] < 0).any() for g in got):
+                    raise RuntimeError("no token is allowed: nothing to draw from")
                 seqs = [np.concatenate((s, g[1:1 + g[0]]))[:n + max_len] for s, g in zip(seqs, got)]
                 self.drafted_steps_ += 1
             if _cabi.lost_waits() != lost:      # asked before tokens are handed out
                 raise RuntimeError("a kernel gave up on a wait: logits of this call are not valid")
+            if self.pages is not None:
+                self.pages.check()
             self.positions.copy_(ctx)
             self.ctx_lens.copy_(ctx + 1)
             self.ids.copy_(to_device(torch.from_numpy(np.array([s[-1] for s in seqs], dtype=np.int32)), dev))
