@@ -37,7 +37,7 @@
 namespace pa {
 namespace drawn {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kPer = kBins / kThreads, kList = 256, kMany = 2048, kFew = 256, kMostRanks = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kPer = kBins / kThreads, kList = 1024, kMany = 2048, kFew = 256, kOwn = 256, kMostRanks = 8;
 constexpr int kWords = 8, kMostChunkStrips = kWords * kWarps, kMostStrips = 512, kMostChunks = 512, kGroup = 8192;       // a group of rows has so many chunks
 static_assert(kFew == kThreads && kPer == 4, "a thread for each of few; a word of steps a thread");
 constexpr int kCountShift = 18;             // a step's word: a chunk's tokens (up to 8192) from here on, the sum of their parts below
@@ -676,7 +676,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(
     }
     __syncthreads();
     const int listed = s_listed;
-    if (tid < min(listed, kList)) a.list[(int64_t)blockIdx.x * kList + tid] = s_list[tid];
+    for (int i = tid; i < min(listed, kList); i += kThreads) a.list[(int64_t)blockIdx.x * kList + i] = s_list[i];
     if (tid == 0) {
         Chunk out{};
 #pragma unroll
@@ -714,7 +714,7 @@ struct Shared : WeighShared {
         int32_t child[PA_TREE_MOST_NODES];
     };
     union {
-        Near list[kList];
+        Near list[kOwn];
         double strip[kMostStrips];  // sums of a part's strips
     };
     union {
@@ -943,15 +943,14 @@ struct Finish : Weigher {
                 sh.hist[tid] = make_uint4(0, 0, 0, 0);
                 __syncthreads();
                 const uint32_t hist = smem_u32(sh.hist);
-                for (int s = s0; s < s1; ++s) {
-                    const Word<T> w = view.load(s, lane);
+                view.template each<4>(s0, s1, 1, lane, [&](const Word<T>& w, int, int) {
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
                         const float x = finite<T>(widen<T>(w.v[e]));
                         const uint32_t b = ((k_hi - (key_of(x) >> Limit<T>::spare)) >> shift) & (kBins - 1);
                         if (widen<T>(w.v[e]) >= r.r_lo && x <= r.r_hi) asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(hist + 4 * b) : "memory");
                     }
-                }
+                });
                 cluster_sync();
                 if (rank == 0) {
                     int from, to;
@@ -992,9 +991,7 @@ struct Finish : Weigher {
             double sum = 0.0, below = 0.0;
             float least_x = INFINITY, most_x = -INFINITY, least_up = INFINITY;
             const float floor = MASS && first ? least : near;
-            for (int s = s0; s < s1; ++s) {
-                const Word<T> w = view.load(s, lane);
-                const int v = view.token(s, lane);
+            view.template each<4>(s0, s1, 1, lane, [&](const Word<T>& w, int, int v) {
                 float x[N], m = -INFINITY;
                 uint32_t mine = 0;
 #pragma unroll
@@ -1002,7 +999,7 @@ struct Finish : Weigher {
                     x[e] = widen<T>(w.v[e]);
                     m = fmaxf(m, x[e]);
                 }
-                if (!__any_sync(kAll, m >= floor)) continue;
+                if (!__any_sync(kAll, m >= floor)) return;
                 if ((MASS && first) || ((MASS || sums) && __any_sync(kAll, m >= up))) {
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
@@ -1022,12 +1019,12 @@ struct Finish : Weigher {
                             const float y = finite<T>(x[e]);
                             least_x = fminf(least_x, y);
                             most_x = fmaxf(most_x, y);
-                            if (at < kList) sh.list[at] = Near{y, v + e};
+                            if (at < kOwn) sh.list[at] = Near{y, v + e};
                             ++at;
                         }
                 }
                 __syncwarp();
-            }
+            });
             sum = warp_sum(sum);
             below = warp_sum(below);
 #pragma unroll
@@ -1077,7 +1074,7 @@ struct Finish : Weigher {
                 const bool upper = MASS && r.halve && above >= limit;            // the border is in the upper half
                 float found = NAN;
                 if (l == h && !upper) found = l;
-                else if (!upper && n <= kMany && most <= kList) {
+                else if (!upper && n <= kMany && most <= kOwn) {
                     int few, from = 0;
 #pragma unroll
                     for (int c = 0; c < kMostRanks; ++c) {
@@ -1102,7 +1099,7 @@ struct Finish : Weigher {
             cluster_sync();
             r = *peer(&sh.verdict, 0);
             border = r.border;
-            if (r.done) return (MASS || sums) && sh.listed <= kList ? up : NAN;
+            if (r.done) return (MASS || sums) && sh.listed <= kOwn ? up : NAN;
             first = false;
         }
         return NAN;
@@ -1208,21 +1205,31 @@ struct Finish : Weigher {
             else {
                 const bool both = r.k > 0 && r.p < 1.0;          // (a count, of which all are listed; a share of it comes next)
                 if (l == h) found = l;
-                else if (n <= kMany && most <= kList) {
+                else if (most <= kList) {
                     starts();
-                    for (int i = tid; i < n; i += kThreads) {
-                        int c = 0, end = a.chunks - 1;          // the last chunk that begins at or before it
+                    auto listed = [&](int i) {                  // the i-th listed token
+                        int c = 0, end = a.chunks - 1;          // in the last chunk that begins at or before it
                         while (c < end) {
                             const int mid = (c + end + 1) >> 1;
                             if (sh.first[mid] <= i) c = mid;
                             else end = mid - 1;
                         }
-                        sh.many[i] = list[c * kList + i - sh.first[c]].x;
+                        return list[c * kList + i - sh.first[c]].x;
+                    };
+                    const double limit = r.k > 0 ? (double)r.k : r.p * all;
+                    int count = n, above_n = in.above_n, some;
+                    float low = l, high = h;
+                    if (n <= kMany) {
+                        for (int i = tid; i < n; i += kThreads) sh.many[i] = listed(i);
+                        __syncthreads();
+                    } else if (r.k > 0) {
+                        count = narrow_listed<false>(n, low, high, above, above_n, limit, listed);
+                    } else {
+                        count = narrow_listed<true>(n, low, high, above, above_n, limit, listed);
                     }
-                    __syncthreads();
-                    int some;
-                    if (r.k > 0) found = select<false>(n, l, h, 0.0, in.above_n, (double)r.k, some);
-                    else found = select<true>(n, l, h, above, 0, r.p * all, some);
+                    if (count > kMany) found = NAN;
+                    else if (r.k > 0) found = select<false>(count, low, high, 0.0, above_n, limit, some);
+                    else found = select<true>(count, low, high, above, 0, limit, some);
                     if (both && found == found) {
                         const double counted = weights_of_few(n, found);
                         found = among<true>(n, found, 0.0, 0, r.p * counted);
@@ -1240,7 +1247,7 @@ struct Finish : Weigher {
                     for (int c = warp; c < a.chunks; c += kWarps) {
                         double sum = 0.0;
                         for (int i = sh.first[c]; i < sh.first[c + 1]; i += 32) {
-                            const float x = i + lane < sh.first[c + 1] ? sh.many[i + lane] : -INFINITY;
+                            const float x = i + lane >= sh.first[c + 1] ? -INFINITY : n <= kMany ? sh.many[i + lane] : list[c * kList + i + lane - sh.first[c]].x;
                             if (__any_sync(kAll, x >= found)) {
                                 const double w = weight(x);
                                 sum += x >= found ? w : 0.0;
@@ -1264,6 +1271,51 @@ struct Finish : Weigher {
             v.total = total;
             v.settled = settled;
         }
+    }
+    // Of n listed tokens, [l, h], more than select takes: counted by 1024 steps of floats; those of the steps that may hold the border go to sh.many.
+    // How many these are; [l, h], above and above_n become theirs
+    template <bool MASS, typename F> __device__ int narrow_listed(int n, float& l, float& h, double& above, int& above_n, double limit, F listed) {
+        const uint32_t k_hi = key_of(h), range = k_hi - key_of(l);
+        const int bits = 32 - __clz(range), shift = bits > 10 ? bits - 10 : 0;
+        sh.hist[tid] = make_uint4(0, 0, 0, 0);
+        if (tid == 0) sh.hit = 0;
+        __syncthreads();
+        uint32_t* hist = reinterpret_cast<uint32_t*>(sh.hist);
+        for (int i = tid; i < n; i += kThreads) atomicAdd(hist + ((k_hi - key_of(listed(i))) >> shift), 1u);
+        __syncthreads();
+        int from, to;
+        weigh<MASS, kPer>(false, limit, above, above_n, from, to,
+                          [&](uint32_t (&c)[kPer], uint32_t (&q)[kPer]) {
+                              const uint4 u = sh.hist[tid];
+                              c[0] = u.x; c[1] = u.y; c[2] = u.z; c[3] = u.w;
+                              q[0] = q[1] = q[2] = q[3] = 0;
+                          },
+                          [&](int b, uint32_t c, uint32_t, double& least, double& most) {
+                              const uint64_t k0 = min((uint64_t)b << shift, (uint64_t)range), k1 = min(((uint64_t)(b + 1) << shift) - 1, (uint64_t)range);
+                              most = c * weight(of_key(k_hi - (uint32_t)k0)) * (1.0 + 1e-10);
+                              least = c * weight(of_key(k_hi - (uint32_t)k1)) * (1.0 - 1e-10);
+                          });
+        above_n = sh.before_n;
+        double sum = 0.0;
+        float low = INFINITY, high = -INFINITY;
+        for (int i0 = 0; i0 < n; i0 += kThreads) {
+            const float x = i0 + tid < n ? listed(i0 + tid) : NAN;
+            const int b = x == x ? (int)((k_hi - key_of(x)) >> shift) : INT_MAX;
+            if (MASS) {
+                const double w = weight(x);
+                sum += b < from ? w : 0.0;
+            }
+            if (b >= from && b <= to) {
+                low = fminf(low, x);
+                high = fmaxf(high, x);
+                const int at = atomicAdd(&sh.hit, 1);
+                if (at < kMany) sh.many[at] = x;        // (the counts there have been read)
+            }
+        }
+        if (MASS) above += over(sum, sh.part, Add());
+        l = over(low, sh.fpart, Min());
+        h = over(high, sh.fpart, Max());
+        return sh.hit;
     }
     // sh.first: from the chunks' numbers of listed tokens to where they begin
     __device__ void starts() {
