@@ -736,7 +736,7 @@ struct Shared : WeighShared {
 
 template <typename T, typename Q, int MODE>
 struct Finish : Weigher {
-    static constexpr int N = Word<T>::N, STRIP = 32 * N;
+    static constexpr int N = Word<T>::N, STRIP = 32 * N, FEW = N > 4 ? 2 : 4;           // (strips on their way at once)
     const Args& a;
     Shared& sh;
     const int rank, local, row;
@@ -809,7 +809,7 @@ struct Finish : Weigher {
     }
     __device__ double kept_sum() {
         double sum = 0.0;
-        view.template each<4>(s0, s1, 1, lane, [&](const Word<T>& x, int, int v) { sum += word_sum(x, v); });
+        view.template each<FEW>(s0, s1, 1, lane, [&](const Word<T>& x, int, int v) { sum += word_sum(x, v); });
         return join(sum);
     }
     // ---- the parts' sums, and the whole row's
@@ -943,7 +943,7 @@ struct Finish : Weigher {
                 sh.hist[tid] = make_uint4(0, 0, 0, 0);
                 __syncthreads();
                 const uint32_t hist = smem_u32(sh.hist);
-                view.template each<4>(s0, s1, 1, lane, [&](const Word<T>& w, int, int) {
+                view.template each<FEW>(s0, s1, 1, lane, [&](const Word<T>& w, int, int) {
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
                         const float x = finite<T>(widen<T>(w.v[e]));
@@ -991,7 +991,7 @@ struct Finish : Weigher {
             double sum = 0.0, below = 0.0;
             float least_x = INFINITY, most_x = -INFINITY, least_up = INFINITY;
             const float floor = MASS && first ? least : near;
-            view.template each<4>(s0, s1, 1, lane, [&](const Word<T>& w, int, int v) {
+            view.template each<FEW>(s0, s1, 1, lane, [&](const Word<T>& w, int, int v) {
                 float x[N], m = -INFINITY;
                 uint32_t mine = 0;
 #pragma unroll
@@ -1404,7 +1404,7 @@ struct Finish : Weigher {
         const int of = rank * kWarps + part, all = a.ranks * kWarps;
         const int e0 = by_chunks ? part * a.chunk_strips : (int)((int64_t)view.strips * of / all);
         const int n = (by_chunks ? min(e0 + a.chunk_strips, view.strips) : (int)((int64_t)view.strips * (of + 1) / all)) - e0;
-        view.template each<4>(e0 + warp, e0 + n, kWarps, lane, [&](const Word<T>& x, int s, int v) {
+        view.template each<FEW>(e0 + warp, e0 + n, kWarps, lane, [&](const Word<T>& x, int s, int v) {
             double w[N], sum = 0.0;
             f(x, v, w);
 #pragma unroll
@@ -1611,7 +1611,7 @@ struct Finish : Weigher {
     }
 };
 
-template <typename T, typename Q, int MODE> __global__ void __launch_bounds__(kThreads) finish_kernel(const __grid_constant__ Args a) {
+template <typename T, typename Q, int MODE> __global__ void __launch_bounds__(kThreads, 2) finish_kernel(const __grid_constant__ Args a) {
     __shared__ Shared sh;
     extern __shared__ uint32_t bits[];
     if (MODE == DRAW && a.count > 1) {
@@ -1699,7 +1699,7 @@ template <typename T, typename Q> __global__ void __launch_bounds__(kThreads, 3)
 }
 
 // Where a node's tests go on after that
-template <typename T, typename Q> __global__ void __launch_bounds__(kThreads) go_on_kernel(const __grid_constant__ Args a) {
+template <typename T, typename Q> __global__ void __launch_bounds__(kThreads, 2) go_on_kernel(const __grid_constant__ Args a) {
     __shared__ Shared sh;
     let_next_start();
     wait_for_last();
