@@ -91,6 +91,7 @@ template <bool TAKE> __global__ void __launch_bounds__(kThreads) pages_kernel(co
     // ---- the table: neighbouring threads on neighbouring tiles of a head
     if (entries) {
         const int64_t step = (int64_t)gridDim.x * kThreads;
+#pragma unroll 2
         for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < entries; i += step) {
             const int b = sequence(first, (int)(i / a.heads)), base = first[b], n = first[b + 1] - base;
             const int own = (int)(i - (int64_t)base * a.heads), h = own / n, t = own - h * n;
@@ -103,37 +104,38 @@ template <bool TAKE> __global__ void __launch_bounds__(kThreads) pages_kernel(co
             }
         }
     }
-    // ---- the rows, some at a time: their sequences, tiles and places in these, then their slots
+    // ---- the rows, some at a time: their sequences, where their pages stand and their places in these; then their slots, a thread for a head of
+    // some neighbouring rows, which looks up a page once for the rows of a tile
     if (TAKE) {
-        __shared__ int r_tile[kRows], r_at[kRows], r_seq[kRows];
-        const int dh = kThreads % a.heads, dr = kThreads / a.heads;
+        __shared__ int64_t r_page[kRows];           // in the table, or counted down from -1 in the free list
+        __shared__ int r_at[kRows];                 // (-1: no page)
+        const int groups = max(1, kThreads / a.heads), each = (kRows + groups - 1) / groups, g = tid / a.heads, h0 = tid - g * a.heads;
         for (int r0 = blockIdx.x * kRows; r0 < a.rows; r0 += gridDim.x * kRows) {
             const int n = min(kRows, a.rows - r0);
             __syncthreads();
             if (tid < n) {
                 const int r = r0 + tid, b = sequence(a.start, r), s0 = a.start[b];
                 const bool in = r >= s0 && r < a.start[b + 1];
-                const int pos = in ? max(a.lengths[b], 0) + r - s0 : -1, t = pos / a.tile;
+                const int pos = in ? max(a.lengths[b], 0) + r - s0 : -1, t = pos / a.tile, own = t - from[b];
                 a.row_seq[r] = in ? b : -1;
                 a.positions[r] = pos;
-                r_seq[tid] = b;
-                r_tile[tid] = pos >= 0 && t < a.tiles ? t : -1;
-                r_at[tid] = pos - t * a.tile;
+                r_at[tid] = pos >= 0 && t < a.tiles ? pos - t * a.tile : -1;
+                r_page[tid] = fits && own >= 0 && own < first[b + 1] - first[b] ? -(int64_t)(count - 1 - (first[b] + own) * a.heads) - 1 : (int64_t)b * a.heads * a.tiles + t;
             }
             __syncthreads();
-            int r = tid / a.heads, h = tid - r * a.heads;
-            for (int i = tid; i < n * a.heads; i += kThreads) {
-                const int b = r_seq[r], t = r_tile[r], own = t - from[b];
+            if (g >= groups) continue;
+            for (int h = h0; h < a.heads; h += kThreads) {
+                int64_t last = LLONG_MIN;
                 int page = -1;
-                if (t >= 0)
-                    page = fits && own >= 0 && own < first[b + 1] - first[b] ? a.free[count - 1 - ((int64_t)(first[b] + own) * a.heads + h)]
-                                                                            : a.table[((int64_t)b * a.heads + h) * a.tiles + t];
-                a.slots[(int64_t)r0 * a.heads + i] = (unsigned)page < (unsigned)a.total ? page * a.tile + r_at[r] : -1;
-                h += dh;
-                r += dr;
-                if (h >= a.heads) {
-                    h -= a.heads;
-                    ++r;
+                int32_t* out = a.slots + ((int64_t)r0 + g * each) * a.heads + h;
+                for (int r = g * each; r < min(n, (g + 1) * each); ++r, out += a.heads) {
+                    const int at = r_at[r];
+                    if (at >= 0 && r_page[r] != last) {
+                        last = r_page[r];
+                        page = last < 0 ? a.free[-(last + 1) - h] : a.table[last + (int64_t)h * a.tiles];
+                        if ((unsigned)page >= (unsigned)a.total) page = -1;
+                    }
+                    *out = at >= 0 && page >= 0 ? page * a.tile + at : -1;
                 }
             }
         }
@@ -187,5 +189,5 @@ PA_API int pa_release_pages(int32_t* d_table, int num_beams, int num_heads, int 
     if (num_seqs == 0) return PA_OK;
     if (num_seqs > kMostSeqs) return PA_ERR_UNSUPPORTED;
     // (how much goes back the host does not know: as many CTAs as a whole table keeps busy)
-    return launch<false>(a, (int64_t)num_seqs * num_heads * num_tiles / (16 * kThreads), device_info().sm_count, as_stream(stream));
+    return launch<false>(a, (int64_t)num_seqs * num_heads * num_tiles / (8 * kThreads), 3 * (int64_t)device_info().sm_count, as_stream(stream));
 }
