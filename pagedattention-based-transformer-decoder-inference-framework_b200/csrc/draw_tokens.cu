@@ -52,7 +52,6 @@ struct Chunk {
     double above, whole;            // sums of the weights at or above `up`, and of all
     float top, lo, hi;              // the largest logit; the ends of what is listed
     int listed, first;              // how many, the lowest of them
-    int spare_;
 };
 struct Row {                        // what range and finish leave
     float top, up, lo, border;      // (up may be no number: nothing is at or above it)
@@ -165,7 +164,6 @@ __device__ __forceinline__ double exp2_64(double y, double table) {
     p *= __shfl_sync(kAll, table, n);           // (of which the low five bits count)
     return __hiloint2double(__double2hiint(p) + (n >> 5) * 1048576, __double2loint(p));
 }
-
 
 __device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -444,7 +442,6 @@ struct Weigher : Block {
         __syncthreads();
     }
 
-
     // the least float whose step is below b (the steps fall while the floats grow), by a warp: 31 of them are tried at a time
     template <typename F> __device__ float edge_of(int b, float top, F place) const {
         if (b <= 0) return NAN;                     // nothing is at or above it, nor infinity
@@ -464,7 +461,6 @@ struct Weigher : Block {
         }
         return of_key((uint32_t)h);
     }
-
 };
 
 template <typename T> __global__ void __launch_bounds__(kThreads) range_kernel(const __grid_constant__ Args a) {
@@ -605,7 +601,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(
     b.relative_to(top, s_row.scale);
     double above = 0.0, whole = 0.0;
     float least_x = INFINITY, most_x = -INFINITY;
-    if (top > -INFINITY) {
+    // (a warp without a token that has a weight sums nothing: below, what has none counts as a little)
+    if (top > -INFINITY && !(plain && !__any_sync(kAll, mine_top >= floor))) {
         for (int s = s0 + warp; s < s1; s += kWarps) {
             const Word<T> w = s_words[(s - s0) * 32 + lane];
             float x[N];
@@ -1187,7 +1184,7 @@ struct Finish : Weigher {
             found = r.floor(m);
             for (int c0 = 0; c0 < a.chunks; c0 += kThreads) {       // from the chunk's largest to the row's
                 const float t = c0 + tid < a.chunks ? chunk[c0 + tid].top : m;
-                const double w = t >= found ? weight(t) : 0.0;
+                const double u = weight(fmaxf(t, found)), w = t >= found ? u : 0.0;         // (by all lanes: weights need a warp)
                 if (c0 + tid < a.chunks) total += sh.chunk[c0 + tid] *= w;
             }
             total = over(total, sh.part, Add());
@@ -1538,7 +1535,7 @@ struct Finish : Weigher {
             const int r = sh.child[i], c = a.tokens[r];
             if ((unsigned)c >= (unsigned)a.vocab) continue;
             const double w = kept(view.at(c), c), qc = (double)widen<Q>(q[c]);
-            if ((double)a.uniform[2 * (int64_t)r] * qc * S < fmax(w - st.taken * qc, 0.0) * (1.0 - st.out)) {
+            if ((double)a.uniform[2 * (int64_t)r] * qc * S < fmax(fma(-st.taken, qc, w), 0.0) * (1.0 - st.out)) {
                 if (rank == 0 && tid == 0) put(0, c, w / st.total);
                 return true;
             }
@@ -1568,7 +1565,7 @@ struct Finish : Weigher {
             if (taken > 0.0)
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    const double u = w[e] - taken * (double)y[e];
+                    const double u = fma(-taken, (double)y[e], w[e]);
                     w[e] = u > 0.0 ? u : 0.0;
                 }
         });
@@ -1638,63 +1635,63 @@ template <typename T, typename Q> __global__ void __launch_bounds__(kThreads, 3)
     wait_for_last();
     const int all = a.open[a.round - 1] * a.chunks;
     for (int i = blockIdx.x; i < all; i += gridDim.x) {
-    const int local = a.opened[(int64_t)(a.round - 1) * a.group + i / a.chunks], c = i % a.chunks, row = a.row0 + local;
-    const Rest st = a.rest[local];
-    const View<T> view(a, row);
-    const Row r = a.row[local];
-    b.relative_to(r.top, r.scale);
-    const Q* q = draft_row<Q>(a, row);
-    const int s0 = c * a.chunk_strips, s1 = min(s0 + a.chunk_strips, view.strips);
-    const bool alike = ((uintptr_t)(q - view.off) & 15) == 0;
-    double sum = 0.0;
-    auto add = [&](const Word<T>& x, int v, const float (&y)[N]) {
-        float m = -INFINITY;
+        const int local = a.opened[(int64_t)(a.round - 1) * a.group + i / a.chunks], c = i % a.chunks, row = a.row0 + local;
+        const Rest st = a.rest[local];
+        const View<T> view(a, row);
+        const Row r = a.row[local];
+        b.relative_to(r.top, r.scale);
+        const Q* q = draft_row<Q>(a, row);
+        const int s0 = c * a.chunk_strips, s1 = min(s0 + a.chunk_strips, view.strips);
+        const bool alike = ((uintptr_t)(q - view.off) & 15) == 0;
+        double sum = 0.0;
+        auto add = [&](const Word<T>& x, int v, const float (&y)[N]) {
+            float m = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < N; ++e) m = fmaxf(m, widen<T>(x.v[e]));
-        if (!__any_sync(kAll, m >= r.border)) return;
+            for (int e = 0; e < N; ++e) m = fmaxf(m, widen<T>(x.v[e]));
+            if (!__any_sync(kAll, m >= r.border)) return;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float z = widen<T>(x.v[e]);
-            const double u = b.weight<T>(z) - st.taken * (double)y[e];
-            if (z >= r.border && (r.only < 0 || v + e == r.only) && u > 0.0) sum += u;
-        }
-    };
-    for (int s = s0 + b.warp; s < s1; s += SOME * kWarps) {
-        if (alike && s + (SOME - 1) * kWarps < s1 && view.whole(s, (SOME - 1) * kWarps + 1)) {
-            Word<T> x[SOME];
-            float y[SOME][N];
+            for (int e = 0; e < N; ++e) {
+                const float z = widen<T>(x.v[e]);
+                const double u = fma(-st.taken, (double)y[e], b.weight<T>(z));         // (rounded alike wherever it is taken)
+                if (z >= r.border && (r.only < 0 || v + e == r.only) && u > 0.0) sum += u;
+            }
+        };
+        for (int s = s0 + b.warp; s < s1; s += SOME * kWarps) {
+            if (alike && s + (SOME - 1) * kWarps < s1 && view.whole(s, (SOME - 1) * kWarps + 1)) {
+                Word<T> x[SOME];
+                float y[SOME][N];
 #pragma unroll
-            for (int k = 0; k < SOME; ++k) x[k] = view.load_whole(s + k * kWarps, lane);
+                for (int k = 0; k < SOME; ++k) x[k] = view.load_whole(s + k * kWarps, lane);
 #pragma unroll
-            for (int k = 0; k < SOME; ++k) {
-                const int v = view.token(s + k * kWarps, lane);
-                if constexpr (QN <= N) {
+                for (int k = 0; k < SOME; ++k) {
+                    const int v = view.token(s + k * kWarps, lane);
+                    if constexpr (QN <= N) {
 #pragma unroll
-                    for (int e = 0; e < N; e += QN) {
-                        const uint4 raw = ldg_stream_128(q + v + e);
+                        for (int e = 0; e < N; e += QN) {
+                            const uint4 raw = ldg_stream_128(q + v + e);
 #pragma unroll
-                        for (int i = 0; i < QN; ++i) y[k][e + i] = widen<Q>(reinterpret_cast<const Q*>(&raw)[i]);
+                            for (int i = 0; i < QN; ++i) y[k][e + i] = widen<Q>(reinterpret_cast<const Q*>(&raw)[i]);
+                        }
+                    } else {                            // (eight of q to a word of its own, four of the logits)
+                        const uint2 raw = ldg_stream_64(q + v);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) y[k][i] = widen<Q>(reinterpret_cast<const Q*>(&raw)[i]);
                     }
-                } else {                            // (eight of q to a word of its own, four of the logits)
-                    const uint2 raw = ldg_stream_64(q + v);
+                }
 #pragma unroll
-                    for (int i = 0; i < N; ++i) y[k][i] = widen<Q>(reinterpret_cast<const Q*>(&raw)[i]);
+                for (int k = 0; k < SOME; ++k) add(x[k], view.token(s + k * kWarps, lane), y[k]);
+            } else {
+                for (int k = 0; k < SOME && s + k * kWarps < s1; ++k) {
+                    const int v = view.token(s + k * kWarps, lane);
+                    float y[N];
+#pragma unroll
+                    for (int e = 0; e < N; ++e) y[e] = v + e >= 0 && v + e < view.V ? widen<Q>(q[v + e]) : 0.f;
+                    add(view.load(s + k * kWarps, lane), v, y);
                 }
             }
-#pragma unroll
-            for (int k = 0; k < SOME; ++k) add(x[k], view.token(s + k * kWarps, lane), y[k]);
-        } else {
-            for (int k = 0; k < SOME && s + k * kWarps < s1; ++k) {
-                const int v = view.token(s + k * kWarps, lane);
-                float y[N];
-#pragma unroll
-                for (int e = 0; e < N; ++e) y[e] = v + e >= 0 && v + e < view.V ? widen<Q>(q[v + e]) : 0.f;
-                add(view.load(s + k * kWarps, lane), v, y);
-            }
         }
-    }
-    sum = b.over(sum, s_part, Add());
-    if (b.tid == 0) a.rest_sum[(int64_t)local * a.chunks + c] = sum;
+        sum = b.over(sum, s_part, Add());
+        if (b.tid == 0) a.rest_sum[(int64_t)local * a.chunks + c] = sum;
     }
 }
 
@@ -1789,8 +1786,8 @@ template <auto Kernel> static cudaError_t start(const Args& a, unsigned ctas, un
 }
 
 template <typename T, typename Q, int MODE> static int launch(Args a, int type, int most_children, void* workspace, cudaStream_t st) {
-    const Cut c = cut_of(type, a.rows, a.vocab);
     if ((size_t)a.vocab * sizeof(T) > PA_DRAW_MOST_ROW_BYTES) return PA_ERR_UNSUPPORTED;
+    const Cut c = cut_of(type, a.rows, a.vocab);
     a.chunks = c.chunks;
     a.chunk_strips = c.chunk_strips;
     a.ranked = a.top_k || a.top_k1 > 0 || a.top_p || a.top_p1 < 1.0 || a.min_p || a.min_p1 > 0.0;
@@ -1878,6 +1875,7 @@ using namespace pa;
 
 PA_API size_t pa_draw_workspace_bytes(int type, int rows, int vocab, int most_children) {
     if (rows <= 0 || vocab <= 0 || most_children < 0 || type < PA_TYPE_F32 || type > PA_TYPE_BF16) return 0;
+    if ((size_t)vocab * (type == PA_TYPE_F32 ? 4 : 2) > PA_DRAW_MOST_ROW_BYTES) return 0;
     const drawn::Cut c = drawn::cut_of(type, rows, vocab);
     return drawn::row_bytes(c) * c.group + drawn::round_bytes(c) * ((size_t)most_children + 1);
 }
@@ -1914,7 +1912,7 @@ PA_API int pa_verify_drafts(const void* d_logits, int type, int64_t stride, int 
                             int64_t draft_stride, int draft_count, const int32_t* d_draft_rows, int distinct, int32_t* d_ids, float* d_logprobs,
                             void* d_workspace, size_t workspace_bytes, pa_stream_t stream) {
     using namespace pa::drawn;
-    PA_CHECK_ARG(usable(d_logits, type, stride, rows, vocab, rules) && draft_count >= 0 && most_children >= 0 && most_children < PA_TREE_MOST_NODES && (draft_count == 0 || (d_draft && draft_stride >= vocab)));
+    PA_CHECK_ARG(usable(d_logits, type, stride, rows, vocab, rules) && draft_count >= 0 && most_children >= 0 && most_children < PA_TREE_MOST_NODES && (draft_count == 0 || (d_draft && draft_stride >= vocab && (uintptr_t)d_draft % (draft_type == PA_TYPE_F32 ? 4 : 2) == 0)));
     if (rows == 0) return PA_OK;
     PA_CHECK_ARG(d_uniform && d_ids && d_tokens && d_parents && d_node_start && rules->d_row_seq && (d_draft_rows || draft_count >= rows));
     Args a = args(d_logits, stride, rows, vocab, rules);

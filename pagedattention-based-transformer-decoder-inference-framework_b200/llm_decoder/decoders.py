@@ -172,6 +172,7 @@ class _DecoderBase:
         self.ctx_lens.fill_(1)
         if self.pages is not None:
             self.pages.release(self.positions)
+            self.pages.forget()
 
     # ------------------------------------------------------------------ device step
     def _chk(self, st, what):

@@ -41,16 +41,18 @@ class DevicePages:
         if not (mapped == (np.arange(pt.num_tiles_) < held[:, None])[:, None]).all():
             raise ValueError("DevicePages: a row's first tiles have pages, of every head alike")
         used = table[mapped]
-        if len(np.unique(used)) != len(used) or (len(used) and used.max() >= total_pages):
+        taken = np.zeros(total_pages, dtype=bool)           # marks, not a sort: pools have many pages
+        if len(used) and used.max() < total_pages:
+            taken[used] = True
+        if np.count_nonzero(taken) != len(used):
             raise ValueError("DevicePages: pages of the pool, none of them twice")
         if free is None:
-            rest = np.ones(total_pages, dtype=bool)
-            rest[used] = False
-            free = np.flatnonzero(rest)[::-1]
+            free = np.flatnonzero(~taken)[::-1]
         else:
             free = np.asarray(free.cpu() if isinstance(free, torch.Tensor) else free)
-            every = np.concatenate([free, used])
-            if len(np.unique(every)) != len(every) or (len(free) and not 0 <= free.min() <= free.max() < total_pages):
+            if len(free) and 0 <= free.min() <= free.max() < total_pages:
+                taken[free] = True
+            if np.count_nonzero(taken) != len(used) + len(free):
                 raise ValueError("DevicePages: free pages are pages of the pool, none of them twice or in the table")
         self.table, self.total_pages, self.tile_size = pt, total_pages, tile_size
         self.device, self._cache = pt.d_table_.device, None
@@ -116,6 +118,10 @@ class DevicePages:
         if refused:
             self._state[1] = 0
             raise RuntimeError(f"DevicePages: {refused} steps found too few pages (or tiles), their rows have no place")
+
+    def forget(self):
+        """Calls that found too few pages so far count no longer."""
+        self._state[1:2].zero_()
 
     def to_host(self):
         """The table and the free pages are the host's again.  Synchronises."""

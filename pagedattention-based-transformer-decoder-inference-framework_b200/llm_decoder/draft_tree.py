@@ -67,7 +67,7 @@ class DraftTree:
 
     @property
     def branches(self):
-        "Children of the node that has the most."
+        """Children of the node that has the most."""
         if self._branches is None:
             up = self._parents + np.repeat(np.cumsum(self.sizes) - self.sizes, self.sizes).astype(np.int64) if self.rows else self._parents
             self._branches = int(np.bincount(up[self._parents >= 0]).max(initial=0))

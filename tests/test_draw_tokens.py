@@ -137,6 +137,21 @@ def test_numbers_at_the_ends():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_masks_that_leave_a_few(kind):
+    """Rows of many chunks of which a mask leaves three tokens, with rules per sequence that leave nothing out: these, and then none."""
+    from llm_decoder import sampling
+    x = torch.full((3, 60000), -math.inf, device="cuda", dtype=TYPES[kind])
+    for r, kept in enumerate(([5, 30, 600], [100, 30000, 59999], [41000, 41001, 50000])):
+        x[r, kept] = torch.tensor([0.0, 1.0, 0.5], device="cuda", dtype=TYPES[kind])
+    zero, u = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(3, 5, device="cuda")
+    for kw in (dict(), dict(top_k=zero), dict(min_p=zero.float()), dict(top_k=zero, top_p=zero.float() + 1, temperature=zero.float() + 0.01)):
+        ids = sampling.draw_tokens(x, u, **kw)
+        assert [sorted(i[:3]) for i in ids.tolist()] == [[5, 30, 600], [100, 30000, 59999], [41000, 41001, 50000]] and (ids[:, 3:] == -1).all()
+        assert sampling.draw_tokens(x, u[:, 0] + 1, **kw).tolist() == [600, 59999, 50000]
+
+
+@pytest.mark.gpu
 def test_rows_by_sequence_and_other_streams():
     """Rows name their sequences (or none: nothing is left out), calls run on the stream that is current, captured calls follow their inputs."""
     from llm_decoder import DraftTree, sampling
@@ -325,6 +340,9 @@ def test_refused_on_the_host():
     assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 2, 0x5000, 0, 8, 3, None, 0, 0x9000, None, *ws, None) == -1      # rows without one
     assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 2, 0x5000, 0, 7, 4, None, 0, 0x9000, None, *ws, None) == -1
     assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 2, 0x5000, 3, 8, 4, None, 0, 0x9000, None, *ws, None) == -2
+    assert lib.pa_verify_drafts(0x1000, 0, 8, 4, 8, ref(rules), 0x8000, *tree, 2, 0x5002, 0, 8, 4, None, 0, 0x9000, None, *ws, None) == -1      # no address of a float
+    assert lib.pa_draw_workspace_bytes(0, 1, 375001, 0) == lib.pa_draw_workspace_bytes(1, 1, 2 ** 31 - 1, 0) == 0
+    assert lib.pa_draw_tokens(0x1000, 0, 375001, 1, 375001, ref(rules), 0x8000, 1, 0x9000, None, *ws, None) == -2
 
 
 @pytest.mark.gpu
