@@ -78,7 +78,11 @@ template <bool TAKE> __global__ void __launch_bounds__(kThreads) pages_kernel(co
     if (tid == 0) first[a.seqs] = fits ? (int)s_run : 0;
     __syncthreads();
     // (all of this CTA's threads have what they read; who comes last changes it, when its own share is done)
-    if (tid == 0) s_last = atomicAdd(a.state + READ, 1) == (int)gridDim.x - 1;
+    if (tid == 0) {
+        int arrived = 0;
+        if (gridDim.x > 1) asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(arrived) : "l"(a.state + READ) : "memory");
+        s_last = arrived == (int)gridDim.x - 1;
+    }
     auto sequence = [&](const int32_t* starts, int at) {        // the last sequence that begins at or before `at`
         int lo = 0, hi = a.seqs - 1;
         while (lo < hi) {
