@@ -464,7 +464,7 @@ struct Weigher : Block {
 };
 
 template <typename T> __global__ void __launch_bounds__(kThreads) range_kernel(const __grid_constant__ Args a) {
-    __shared__ uint32_t s_n[kBins], s_q[kBins];
+    __shared__ __align__(16) uint32_t s_n[kBins], s_q[kBins];       // (read four at a time)
     __shared__ WeighShared sh;
     __shared__ float s_top[kWarps], s_edge[2], s_tops[kMostChunks];
     Weigher b(sh);
@@ -718,7 +718,7 @@ struct Shared : WeighShared {
         double few_w[kFew];
         uint32_t fine[kThreads];
     };
-    float few[kFew];
+    alignas(16) float few[kFew];
     double chunk[kMostChunks];      // sums of the chunks, in the row's order
     int first[kMostChunks + 1];     // listed tokens of the chunks before
     double seg[kWarps];             // or of the warps' parts of this CTA's share of the row
