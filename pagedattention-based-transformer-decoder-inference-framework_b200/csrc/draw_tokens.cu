@@ -152,7 +152,7 @@ __device__ const double kTable[32] = {     // 2^(j/32)
 };
 __constant__ double kPoly[4] = {0.69314718055994530942, 0.24022650695910071233, 0.05550410866482157995, 0.00961812910762847716};        // ln 2 ^ k / k!
 // 2^y by all lanes of a warp, lane j of which holds 2^(j/32) in `table`: for y of -1022 to 0; others give some number
-__device__ __forceinline__ double exp2_64(double y, double table) {
+template <typename F> __device__ __forceinline__ double exp2_by(double y, F table) {
     constexpr double magic = 211106232532992.0;             // 1.5 x 2^47: sums end at multiples of 1/32
     const double at = y + magic;
     const int n = __double2loint(at);
@@ -161,8 +161,11 @@ __device__ __forceinline__ double exp2_64(double y, double table) {
     p = fma(r, p, kPoly[1]);
     p = fma(r, p, kPoly[0]);
     p = fma(r, p, 1.0);
-    p *= __shfl_sync(kAll, table, n);           // (of which the low five bits count)
+    p *= table(n);
     return __hiloint2double(__double2hiint(p) + (n >> 5) * 1048576, __double2loint(p));
+}
+__device__ __forceinline__ double exp2_64(double y, double table) {
+    return exp2_by(y, [&](int n) { return __shfl_sync(kAll, table, n); });        // (of which the low five bits count)
 }
 
 __device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -569,6 +572,9 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(
     let_next_start();
     const View<T> view(a, row);
     __shared__ Row s_row;
+    __shared__ double s_table[32];
+    if (tid < 32) s_table[tid] = b.table;
+    auto exp2_s = [&](double y) { return exp2_by(y, [&](int n) { return s_table[n & 31]; }); };
     const int s0 = c * a.chunk_strips, s1 = min(s0 + a.chunk_strips, view.strips);
     if (tid == 0) {
         s_listed = 0;
@@ -611,13 +617,13 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(
             uint32_t mine = 0;
             if (plain) {                // (what has no weight, or is no number, as 2^-900 or less)
 #pragma unroll
-                for (int e = 0; e < N; ++e) above += b.weight<T>(fmaxf(x[e], floor));
+                for (int e = 0; e < N; ++e) above += exp2_s(fma((double)finite<T>(fmaxf(x[e], floor)), b.scale, b.base));
                 continue;
             }
             if (all) {                  // (no infinity: range has left such rows to finish)
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    const double v = exp2_64(fma((double)fmaxf(x[e], floor), b.scale, b.base), b.table);
+                    const double v = exp2_s(fma((double)fmaxf(x[e], floor), b.scale, b.base));
                     whole += v;
                     above += x[e] >= up ? v : 0.0;
                     mine |= (uint32_t)(x[e] >= lo && !(x[e] >= up)) << e;
