@@ -14,8 +14,10 @@
 //
 // Ids have to be those of the definition: a cumulative sum that is off by e draws another token for a share of e of the numbers at each of
 // up to V borders, so that weights and sums are in 64 bits (an error of 1e-12: one draw in 10^7 of 128000 tokens); floats would be off in one of a
-// thousand.  2^y is 2^(j/32), from a table that the warp's lanes hold, times a polynomial of the fourth degree of the rest |r| <= 1/64 (Taylor's,
-// error (r ln 2)^5 / 5! <= 1.3e-12): nine operations in 64 bits, of which an SM does 64 a cycle.
+// thousand.  2^y is 2^(j/32), from a table of which every lane of a warp holds one, times a polynomial of the fourth degree of the rest |r| <= 1/64
+// (Taylor's, error (r ln 2)^5 / 5! <= 1.3e-12): nine operations in 64 bits, of which an SM does 64 a cycle.  With the conversion of the logit and
+// the table's word a weight takes 9.4 cycles of an SM for 32 tokens (8.2 with the table in shared memory, which is better where all of a row is
+// summed; 10.3 with the conversion by whole numbers): 35 us for 256 rows of 128000, against 20 for reading them.
 //
 // Rows are read in chunks of up to 64 strips (8192 tokens) by CTAs that know nothing of each other, from memory once and from L2 once more:
 //   count   (where a rule needs it) every chunk's largest logit, and its tokens by 1024 steps of 1/32 in log2 w
@@ -23,8 +25,12 @@
 //   sum     the weights of what is above those steps, in 64 bits, and a list of what is in them
 //   finish  (a cluster of CTAs a row) the border among the listed tokens, the sums of the chunks, the tokens that the numbers draw; verification
 //   write   probabilities
-// Rows that this does not settle (more tokens than the lists hold, of logits that lie closer than a step; temperatures far from 1) are searched by
-// finish itself, by finer steps.
+// Rows that this does not settle (more tokens than the lists hold, of logits that lie closer than a step; temperatures far from 1; a share of what
+// a top_k of more than kFew leaves) are searched by finish itself, by finer steps: some 50 us more a row.
+//
+// 256 rows of 128000 float logits, rules of their own, replayed: 103 us (the first form, a cluster of CTAs a row that read it four times: 352; one that
+// kept it in shared memory: 152, better below 64 rows (one row 25 us against 33), but an SM waits there while one CTA of the cluster
+// looks for the border).  Each kernel begins while the one before ends (programmatic launches), which hides their 4 us each.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -301,6 +307,8 @@ template <typename T> __device__ __forceinline__ float load_chunk(const View<T>&
     return m;
 }
 // ------------------------------------------------------------------------------------------------------------------- count
+// Bound by shared memory's additions, then by memory: 256 x 128000 floats in 32 us (4.1 TB/s), 57 % of the issue slots.  A warp's additions to one word
+// go one after the other, so that steps are fine enough (1/32) for a warp's logits to fall into different ones; a step's tokens and parts go in one word.
 template <typename T> __global__ void __launch_bounds__(kThreads, 6) count_kernel(const __grid_constant__ Args a) {
     constexpr int N = Word<T>::N;
     __shared__ Word<T> s_words[kMostChunkStrips * 4 / N * 32];
@@ -466,6 +474,9 @@ struct Weigher : Block {
     }
 };
 
+// A chain of dependent steps in one CTA a row (chunks' counts, two scans, the searches for the steps' ends): 15 us for 256 rows, 7 for one.  By the
+// last of the row's CTAs in count instead of a kernel of its own it is slower (124 us against 103 for the whole call: nothing of it is done ahead, and
+// count has 40 registers).
 template <typename T> __global__ void __launch_bounds__(kThreads) range_kernel(const __grid_constant__ Args a) {
     __shared__ __align__(16) uint32_t s_n[kBins], s_q[kBins];       // (read four at a time)
     __shared__ WeighShared sh;
@@ -560,6 +571,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads) range_kernel(c
 }
 
 // --------------------------------------------------------------------------------------------------------------------- sum
+// Bound by arithmetic in 64 bits where all of a row is summed (a share is asked for, or temperatures alone), else by reading: 41 us for 256 rows with rules of
+// their own, 62 for 384 of 16-bit logits.  Words of which nothing is kept are passed over by whole warps.
 template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(const __grid_constant__ Args a) {
     constexpr int N = Word<T>::N;
     __shared__ Word<T> s_words[kMostChunkStrips * 4 / N * 32];
@@ -1614,6 +1627,7 @@ struct Finish : Weigher {
     }
 };
 
+// Again dependent steps: 27 us for 256 rows, 10 for one.  Two CTAs an SM (191 registers without the bound: one; 112 us against 103 for the whole call)
 template <typename T, typename Q, int MODE> __global__ void __launch_bounds__(kThreads, 2) finish_kernel(const __grid_constant__ Args a) {
     __shared__ Shared sh;
     extern __shared__ uint32_t bits[];
@@ -1631,7 +1645,9 @@ template <typename T, typename Q, int MODE> __global__ void __launch_bounds__(kT
 }
 
 // -------------------------------------------------------------------------------------------------------------------- rest
-// What refused children have left of a chunk: max(w - taken q, 0).  Words of the logits, and of q where it lies alike, several on their way at once
+// What refused children have left of a chunk: max(w - taken q, 0).  Words of the logits, and of q where it lies alike, several on their way at once.  A launch
+// for every child that a node may have, of the rows whose last test has failed: 64 chains of six, 16-bit, 39 us (by the CTA that
+// tests, a row took 60 to 100); without such a row 3
 template <typename T, typename Q> __global__ void __launch_bounds__(kThreads, 3) rest_kernel(const __grid_constant__ Args a) {
     constexpr int N = Word<T>::N, QN = 16 / (int)sizeof(Q), SOME = sizeof(T) < 4 ? 2 : 4;
     __shared__ double s_part[kWarps];
@@ -1713,6 +1729,7 @@ template <typename T, typename Q> __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // ------------------------------------------------------------------------------------------------------------------- write
+// 64 x 50257: 15 us, for 13 MB from L2 and as many written; weights are formed anew, which costs less than keeping them in 64 bits
 template <typename T> __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__ Args a) {
     constexpr int N = Word<T>::N, STRIP = 32 * N;
     Block b;
@@ -1748,7 +1765,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) write_kernel(c
 }
 
 // ------------------------------------------------------------------------------------------------------------------ launch
-// Chunks of 8192 tokens, smaller ones while there are not two for every SM
+// Chunks of 8192 tokens, of 4096 where there are fewer of these than SMs (16 rows of 50257 are 112 or 208 CTAs)
 struct Cut {
     int chunks, chunk_strips, group;        // of a row; rows that go together
 };
