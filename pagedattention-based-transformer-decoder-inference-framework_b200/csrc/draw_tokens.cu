@@ -157,21 +157,24 @@ __device__ const double kTable[32] = {     // 2^(j/32)
     1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
 };
 __constant__ double kPoly[4] = {0.69314718055994530942, 0.24022650695910071233, 0.05550410866482157995, 0.00961812910762847716};        // ln 2 ^ k / k!
-// 2^y by all lanes of a warp, lane j of which holds 2^(j/32) in `table`: for y of -1022 to 0; others give some number
-template <typename F> __device__ __forceinline__ double exp2_by(double y, F table) {
+// 2^y = p s for y of -1022 to 0 (others give some numbers): s = 2^(n/32), from table(n) = 2^(j/32) less j 2^-5 in its exponent's place, j = the low five
+// bits of n, so that n can be added there as it is
+template <typename F> __device__ __forceinline__ double2 exp2_parts(double y, F table) {
     constexpr double magic = 211106232532992.0;             // 1.5 x 2^47: sums end at multiples of 1/32
     const double at = y + magic;
     const int n = __double2loint(at);
-    const double r = y - (at - magic);
+    const double r = y - (at - magic), t = table(n);
     double p = fma(r, kPoly[3], kPoly[2]);
     p = fma(r, p, kPoly[1]);
     p = fma(r, p, kPoly[0]);
     p = fma(r, p, 1.0);
-    p *= table(n);
-    return __hiloint2double(__double2hiint(p) + (n >> 5) * 1048576, __double2loint(p));
+    return make_double2(p, __hiloint2double((int)((unsigned)__double2hiint(t) + ((unsigned)n << 15)), __double2loint(t)));
 }
+__device__ __forceinline__ double table_entry(int j) { return __hiloint2double(__double2hiint(kTable[j]) - (j << 15), __double2loint(kTable[j])); }
+// by all lanes of a warp, lane j of which holds entry j
 __device__ __forceinline__ double exp2_64(double y, double table) {
-    return exp2_by(y, [&](int n) { return __shfl_sync(kAll, table, n); });        // (of which the low five bits count)
+    const double2 w = exp2_parts(y, [&](int n) { return __shfl_sync(kAll, table, n); });
+    return w.x * w.y;
 }
 
 __device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -258,9 +261,9 @@ template <typename T> __device__ __forceinline__ float finite(float x) { return 
 // what a block of kThreads does together
 struct Block {
     const int tid, warp, lane;
-    double table;                   // 2^(lane / 32)
+    double table;                   // the lane's entry
     double scale = 0.0, base = 0.0; // w = 2^(x scale + base)
-    __device__ Block() : tid(threadIdx.x), warp(threadIdx.x >> 5), lane(threadIdx.x & 31) { table = kTable[threadIdx.x & 31]; }
+    __device__ Block() : tid(threadIdx.x), warp(threadIdx.x >> 5), lane(threadIdx.x & 31) { table = table_entry(threadIdx.x & 31); }
     __device__ __forceinline__ void relative_to(float top, double s) {
         scale = s;
         base = -(double)top * s;
@@ -587,7 +590,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(
     __shared__ Row s_row;
     __shared__ double s_table[32];
     if (tid < 32) s_table[tid] = b.table;
-    auto exp2_s = [&](double y) { return exp2_by(y, [&](int n) { return s_table[n & 31]; }); };
+    auto exp2_s = [&](float x) { return exp2_parts(fma((double)x, b.scale, b.base), [&](int n) { return s_table[n & 31]; }); };
     const int s0 = c * a.chunk_strips, s1 = min(s0 + a.chunk_strips, view.strips);
     if (tid == 0) {
         s_listed = 0;
@@ -630,13 +633,17 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(
             uint32_t mine = 0;
             if (plain) {                // (what has no weight, or is no number, as 2^-900 or less)
 #pragma unroll
-                for (int e = 0; e < N; ++e) above += exp2_s(fma((double)finite<T>(fmaxf(x[e], floor)), b.scale, b.base));
+                for (int e = 0; e < N; ++e) {
+                    const double2 v = exp2_s(finite<T>(fmaxf(x[e], floor)));
+                    above = fma(v.x, v.y, above);
+                }
                 continue;
             }
             if (all) {                  // (no infinity: range has left such rows to finish)
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    const double v = exp2_s(fma((double)fmaxf(x[e], floor), b.scale, b.base));
+                    const double2 u = exp2_s(fmaxf(x[e], floor));
+                    const double v = u.x * u.y;
                     whole += v;
                     above += x[e] >= up ? v : 0.0;
                     mine |= (uint32_t)(x[e] >= lo && !(x[e] >= up)) << e;
