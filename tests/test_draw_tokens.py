@@ -382,3 +382,43 @@ def test_refused_tensors():
     empty = torch.zeros(0, 10, device="cuda")
     assert sampling.truncated_softmax(empty).shape == (0, 10) and sampling.draw_tokens(empty, torch.zeros(0, device="cuda")).shape == (0,)
     assert sampling.draw_tokens(x, torch.zeros(3, 0, device="cuda")).shape == (3, 0)
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once():
+    """Calls of several host threads on streams of their own, and captured calls that are replayed beside each other, give what each gives alone."""
+    import threading
+
+    from llm_decoder import sampling
+    g = torch.Generator(device="cuda").manual_seed(11)
+    cases = [(torch.randn(n, v, device="cuda", generator=g) * 2, torch.rand(n, 2, device="cuda", generator=g), kw)
+             for n, v, kw in ((70, 30011, dict(top_p=0.9)), (3, 128000, dict(top_k=300)), (150, 9000, dict(temperature=0.5)), (33, 50257, dict(top_k=40, top_p=0.8)))]
+    want = [(sampling.draw_tokens(x, u, **kw), sampling.truncated_softmax(x, **kw)) for x, u, kw in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        x, u, kw = cases[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                ids, probs = sampling.draw_tokens(x, u, **kw), sampling.truncated_softmax(x, **kw)
+                if not torch.equal(ids, want[i][0]) or not torch.equal(probs, want[i][1]):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    graphs, got, streams = [], [], [torch.cuda.Stream() for _ in range(4)]
+    for x, u, kw in cases:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append((sampling.draw_tokens(x, u, **kw), sampling.truncated_softmax(x, **kw)))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
