@@ -26,10 +26,10 @@
 //   finish  (a cluster of CTAs a row) the border among the listed tokens, the sums of the chunks, the tokens that the numbers draw; verification
 //   write   probabilities
 // Rows that this does not settle (more tokens than the lists hold, of logits that lie closer than a step; temperatures far from 1; a share of what
-// a top_k of more than kFew leaves) are searched by finish itself, by finer steps: some 50 us more a row.
+// a top_k of more than kFew leaves) are searched by finish itself, by finer steps: 30 us more for one row of 128000, 1 to 1.4 a row for 256.
 //
 // 256 rows of 128000 float logits, rules of their own, replayed: 103 us (the first form, a cluster of CTAs a row that read it four times: 352; one that
-// kept it in shared memory: 152, better below 64 rows (one row 25 us against 33), but an SM waits there while one CTA of the cluster
+// kept it in shared memory: 152, better below 64 rows (one row 25 us against 31), but an SM waits there while one CTA of the cluster
 // looks for the border).  Each kernel begins while the one before ends (programmatic launches), which hides their 4 us each.
 #include <algorithm>
 #include <climits>
@@ -477,23 +477,27 @@ struct Weigher : Block {
     }
 };
 
-// A chain of dependent steps in one CTA a row (chunks' counts, two scans, the searches for the steps' ends): 15 us for 256 rows, 7 for one.  By the
-// last of the row's CTAs in count instead of a kernel of its own it is slower (124 us against 103 for the whole call: nothing of it is done ahead, and
-// count has 40 registers).
-template <typename T> __global__ void __launch_bounds__(kThreads) range_kernel(const __grid_constant__ Args a) {
-    __shared__ __align__(16) uint32_t s_n[kBins], s_q[kBins];       // (read four at a time)
-    __shared__ WeighShared sh;
-    __shared__ float s_top[kWarps], s_edge[2], s_tops[kMostChunks];
+// A chain of dependent steps in one CTA a row (chunks' counts, two scans, the searches for the steps' ends): 15 us for 256 rows, 7 for one.  A kernel of its
+// own, or, for few rows, the beginning of sum.  By the last of the row's CTAs in count it is slower (124 us against 103 for the whole call: nothing of
+// it is done ahead, and count has 40 registers).
+struct Steps {
+    alignas(16) uint32_t n[kBins];      // (read four at a time)
+    alignas(16) uint32_t q[kBins];
+};
+struct RangeShared : WeighShared {
+    float top[kWarps], edge[2], tops[kMostChunks];
+};
+// by all threads of a CTA, when count has ended
+__device__ __forceinline__ Row range_of(const Args& a, int local, const Rules& r, Steps& steps, RangeShared& sh) {
     Weigher b(sh);
-    const int local = blockIdx.x, row = a.row0 + local, tid = b.tid;
-    let_next_start();
-    const Rules r(a, row);
+    const int tid = b.tid;
+    uint32_t *const s_n = steps.n, *const s_q = steps.q;
+    float *const s_tops = sh.tops, *const s_edge = sh.edge;
     for (int i = tid; i < kBins; i += kThreads) s_n[i] = s_q[i] = 0;
-    wait_for_last();
     const Chunk* chunk = a.chunk + (int64_t)local * a.chunks;
     float top = -INFINITY;
-    for (int c = tid; c < a.chunks; c += kThreads) top = fmaxf(top, s_tops[c] = chunk[c].top);
-    top = b.over(top, s_top, Max());
+    for (int c = tid; c < a.chunks; c += kThreads) top = fmaxf(top, s_tops[c] = __ldcg(&chunk[c].top));
+    top = b.over(top, sh.top, Max());
     Row out{};
     out.top = top;
     out.settled = 1;
@@ -570,16 +574,29 @@ template <typename T> __global__ void __launch_bounds__(kThreads) range_kernel(c
     out.all = out.settled && !r.greedy() && r.p < 1.0 && !(r.k > 0) && !(out.lo >= out.up);
     out.floor = floor;
     out.scale = r.scale;
-    if (tid == 0) a.row[local] = out;
+    return out;
+}
+template <typename T> __global__ void __launch_bounds__(kThreads) range_kernel(const __grid_constant__ Args a) {
+    __shared__ Steps steps;
+    __shared__ RangeShared sh;
+    let_next_start();
+    const Rules r(a, a.row0 + (int)blockIdx.x);
+    wait_for_last();
+    const Row out = range_of(a, blockIdx.x, r, steps, sh);
+    if (threadIdx.x == 0) a.row[blockIdx.x] = out;
 }
 
 // --------------------------------------------------------------------------------------------------------------------- sum
-// Bound by arithmetic in 64 bits where all of a row is summed (a share is asked for, or temperatures alone), else by reading: 41 us for 256 rows with rules of
-// their own, 62 for 384 of 16-bit logits.  Words of which nothing is kept are passed over by whole warps.
-template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(const __grid_constant__ Args a) {
+// Bound by instructions (60 % of the issue slots, 18 to 36 % of the 64-bit pipe) where all of a row is summed (a share is asked for, or temperatures alone), else by reading: 40 us for
+// 256 rows with rules of their own, 58 for 384 of 16-bit logits.  Words of which nothing is kept are passed over by whole warps.
+template <typename T, bool RANGES> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(const __grid_constant__ Args a) {
     constexpr int N = Word<T>::N;
     __shared__ Word<T> s_words[kMostChunkStrips * 4 / N * 32];
-    __shared__ Near s_list[kList];
+    __shared__ union {
+        Near list[kList];
+        Steps steps;
+    } s_near;
+    Near* const s_list = s_near.list;
     __shared__ double s_above[kWarps], s_whole[kWarps];
     __shared__ float s_lo[kWarps], s_hi[kWarps], s_top[kWarps];
     __shared__ int s_listed, s_first;
@@ -596,16 +613,26 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(
         s_listed = 0;
         s_first = INT_MAX;
         if (blockIdx.x == 0 && a.open) {
-            if (!a.ranked) wait_for_last();
             for (int i = 0; i <= a.round; ++i) a.open[i] = 0;           // (here: how many rounds there may be)
         }
-        if (a.ranked) {
+        if (a.ranked && !RANGES) {
             wait_for_last();
             s_row = a.row[local];
             if (!s_row.settled) s_row.up = s_row.lo = NAN;
         }
     }
     const float mine_top = load_chunk<T>(view, s0, s1, warp, lane, s_words);
+    if constexpr (RANGES) {             // every CTA for itself
+        __shared__ RangeShared sh;
+        const Rules r(a, row);
+        wait_for_last();
+        Row out = range_of(a, local, r, s_near.steps, sh);
+        if (tid == 0) {
+            if (c == 0) a.row[local] = out;
+            if (!out.settled) out.up = out.lo = NAN;
+            s_row = out;
+        }
+    }
     if (!a.ranked) {                    // temperatures alone: relative to the chunk's own largest
         const float m = finite<T>(b.over(mine_top, s_top, Max()));
         if (tid == 0) {
@@ -709,12 +736,18 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) sum_kernel(
             least_x = fminf(least_x, s_lo[i]);
             most_x = fmaxf(most_x, s_hi[i]);
         }
-        out.top = top;
         out.lo = least_x;
         out.hi = most_x;
         out.listed = listed;
         out.first = s_first;
-        a.chunk[blockIdx.x] = out;
+        Chunk* const to = a.chunk + blockIdx.x;
+        if (!a.ranked) to->top = top;           // (else count's, which the row's other CTAs may still read)
+        to->above = out.above;
+        to->whole = out.whole;
+        to->lo = out.lo;
+        to->hi = out.hi;
+        to->listed = out.listed;
+        to->first = out.first;
     }
 }
 
@@ -1848,11 +1881,14 @@ template <typename T, typename Q, int MODE> static int launch(Args a, int type, 
         a.row0 = r;
         const unsigned some = (unsigned)std::min(c.group, rows - r), ctas = some * (unsigned)c.chunks;
         cudaError_t e = cudaSuccess;
+        // up to two CTAs for an SM: each finds its row's range by itself, a launch less, and nothing else would run there meanwhile (one row of 50257, 13
+        // CTAs: 32.9 -> 30.9 us; 33 x 32001 half, 264 CTAs: 31.8 -> 30; where there are more it takes longer: 64 x 50257, 448 CTAs: 50.9 -> 53.1)
+        const bool at_once = a.ranked && ctas <= 2u * (unsigned)std::max(0, device_info().sm_count);
         if (a.ranked) {
             e = start<count_kernel<T>>(a, ctas, 0, 0, true, st);
-            if (e == cudaSuccess) e = start<range_kernel<T>>(a, some, 0, 0, false, st);
+            if (e == cudaSuccess && !at_once) e = start<range_kernel<T>>(a, some, 0, 0, false, st);
         }
-        if (e == cudaSuccess) e = start<sum_kernel<T>>(a, ctas, 0, 0, !a.ranked, st);
+        if (e == cudaSuccess) e = at_once ? start<sum_kernel<T, true>>(a, ctas, 0, 0, false, st) : start<sum_kernel<T, false>>(a, ctas, 0, 0, !a.ranked, st);
         Args f = a;
         f.round = 0;
         if (e == cudaSuccess) e = start<finish_kernel<T, Q, MODE>>(f, some * a.ranks, a.ranks, MODE == DRAW && a.count > 1 ? (size_t)(a.vocab + 31) / 32 * 4 : 0, false, st);
