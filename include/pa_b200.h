@@ -1110,7 +1110,7 @@ int pa_tree_accept(const int32_t* d_ids, const int32_t* d_tokens, const int32_t*
  *     a token stays if fewer than top_k tokens are above it (top_k <= 0: all do), if the w above it, of those that stay so far, sum up to
  *     less than top_p of theirs (top_p not below 1: all do), and if its w is at least min_p; the largest always stays, tokens of one
  *     value stay or go together;       p = w / (sum of the w that stay)
- * Weights and sums are in 64 bits.  Vocabularies up to PA_DRAW_MOST_ROW_BYTES of logits a row (more: PA_ERR_UNSUPPORTED).  The workspace, on 16
+ * Weights and sums are in 64 bits.  Up to 2^30 rows; vocabularies up to PA_DRAW_MOST_ROW_BYTES of logits a row (more: PA_ERR_UNSUPPORTED).  The workspace, on 16
  * bytes, holds what the kernels of a call leave each other; it needs no values before a call.
  *
  * pa_truncated_softmax: p as floats [rows][vocab], rows probs_stride apart (zeros where every logit is -inf), in memory that the logits do not
@@ -1158,7 +1158,7 @@ int pa_verify_drafts(const void* d_logits, int type, int64_t stride, int rows, i
  *   there is no page.
  * pa_release_pages: the tiles of sequence b from ceil(d_lengths[b] / tile_size) on give back their pages, in the reverse of that order (so that
  *   releasing what was just taken undoes it), and their entries become -1.
- * Up to 16384 sequences (more: PA_ERR_UNSUPPORTED); total_pages * tile_size < 2^31. */
+ * Up to 16384 sequences (more: PA_ERR_UNSUPPORTED) and 2^30 rows; total_pages * tile_size < 2^31. */
 int pa_take_pages(int32_t* d_table, int num_beams, int num_heads, int num_tiles, int tile_size, int total_pages, int32_t* d_free, int32_t* d_held,
                   int32_t* d_state, const int32_t* d_lengths, const int32_t* d_start, int num_seqs, int rows, int32_t* d_row_seq,
                   int32_t* d_positions, int32_t* d_slots, pa_stream_t stream);

@@ -18,7 +18,7 @@
 namespace pa {
 namespace pages {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kMostSeqs = 16384, kRows = 64;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kMostSeqs = 16384, kRows = 64, kMostRows = 1 << 30;
 
 struct Args {
     int32_t* table;             // [beams][heads][tiles]
@@ -181,7 +181,7 @@ PA_API int pa_take_pages(int32_t* d_table, int num_beams, int num_heads, int num
                          int32_t* d_positions, int32_t* d_slots, pa_stream_t stream) {
     using namespace pa::pages;
     const Args a{d_table, d_free, d_held, d_state, d_lengths, d_start, num_seqs, rows, num_heads, num_tiles, tile_size, total_pages, d_row_seq, d_positions, d_slots};
-    PA_CHECK_ARG(usable(a) && rows >= 0 && num_seqs <= num_beams && (num_seqs == 0 || d_start) && (rows == 0 || (num_seqs > 0 && d_row_seq && d_positions && d_slots)));
+    PA_CHECK_ARG(usable(a) && rows >= 0 && rows <= kMostRows && num_seqs <= num_beams && (num_seqs == 0 || d_start) && (rows == 0 || (num_seqs > 0 && d_row_seq && d_positions && d_slots)));
     if (num_seqs == 0) return PA_OK;
     if (num_seqs > kMostSeqs) return PA_ERR_UNSUPPORTED;
     return launch<true>(a, ((int64_t)rows * num_heads + 4 * kThreads - 1) / (4 * kThreads), 4 * (int64_t)device_info().sm_count, as_stream(stream));

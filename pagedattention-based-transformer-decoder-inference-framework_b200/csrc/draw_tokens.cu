@@ -46,6 +46,7 @@ namespace drawn {
 constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kPer = kBins / kThreads, kList = 1024, kMany = 2048, kFew = 256, kOwn = 256, kMostRanks = 8;
 constexpr int kWords = 8, kMostChunkStrips = kWords * kWarps, kMostStrips = 512, kMostChunks = 512, kGroup = 8192;       // a group of rows has so many chunks
 static_assert(kFew == kThreads && kPer == 4, "a thread for each of few; a word of steps a thread");
+constexpr int kMostRows = 1 << 30;          // (so that a row's number and a little more fit 31 bits)
 constexpr int kCountShift = 18;             // a step's word: a chunk's tokens (up to 8192) from here on, the sum of their parts below
 constexpr uint32_t kAll = 0xffffffffu;
 constexpr float kLowest = -3.402823466e38f, kSteps = 32.f, kLogitSteps = 32.f;      // steps of log2 w, or of a logit where these are smaller
@@ -1930,7 +1931,7 @@ static Args args(const void* logits, int64_t stride, int rows, int vocab, const 
 }
 static bool holds(const void* workspace, size_t bytes, size_t need) { return workspace && (uintptr_t)workspace % 16 == 0 && bytes >= need; }
 static bool usable(const void* logits, int type, int64_t stride, int rows, int vocab, const pa_draw_rules* rules) {
-    return rows >= 0 && vocab > 0 && stride >= vocab && rules && rules->num_seqs >= 0 && (rows == 0 || logits) &&
+    return rows >= 0 && rows <= kMostRows && vocab > 0 && stride >= vocab && rules && rules->num_seqs >= 0 && (rows == 0 || logits) &&
            (uintptr_t)logits % (type == PA_TYPE_F32 ? 4 : 2) == 0;
 }
 

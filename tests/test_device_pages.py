@@ -195,6 +195,7 @@ def test_refused_on_the_host():
     assert lib.pa_take_pages(*good, 0x5000, 0x6000, 3, 1, 0x7000, 0x8000, 0x9000, None) == -1             # more sequences than table rows
     assert lib.pa_take_pages(*good, 0x5000, None, 2, 1, 0x7000, 0x8000, 0x9000, None) == -1
     assert lib.pa_take_pages(*good, 0x5000, 0x6000, 2, 1, 0x7000, None, 0x9000, None) == -1
+    assert lib.pa_take_pages(*good, 0x5000, 0x6000, 2, 2 ** 30 + 1, 0x7000, 0x8000, 0x9000, None) == -1
     assert lib.pa_take_pages(*good, 0x5000, 0x6000, 0, 1, 0x7000, 0x8000, 0x9000, None) == -1
     assert lib.pa_take_pages(*good, 0x5000, 0x6000, 0, 0, None, None, None, None) == 0
     assert lib.pa_take_pages(None, *good[1:], 0x5000, 0x6000, 2, 1, 0x7000, 0x8000, 0x9000, None) == -1

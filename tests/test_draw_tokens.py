@@ -324,6 +324,7 @@ def test_refused_on_the_host():
     assert lib.pa_truncated_softmax(None, 0, 8, 4, 8, ref(rules), 0x1000, 8, *ws, None) == -1
     assert lib.pa_truncated_softmax(0x1000, 0, 7, 4, 8, ref(rules), 0x9000, 8, *ws, None) == -1
     assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, ref(rules), 0x9000, 7, *ws, None) == -1
+    assert lib.pa_draw_tokens(0x1000, 0, 8, 2 ** 30 + 1, 8, ref(rules), 0x8000, 1, 0x9000, None, *ws, None) == -1
     assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, ref(rules), 0x1040, 8, *ws, None) == -1          # overlaps
     assert lib.pa_truncated_softmax(0x1002, 0, 8, 4, 8, ref(rules), 0x9000, 8, *ws, None) == -1          # no address of a float
     assert lib.pa_truncated_softmax(0x1000, 0, 8, 4, 8, None, 0x9000, 8, *ws, None) == -1
