@@ -1118,7 +1118,7 @@ int pa_tree_accept(const int32_t* d_ids, const int32_t* d_tokens, const int32_t*
  * pa_draw_tokens: d_ids[r][i] = the first v up to which the sum of p, without the tokens d_ids[r][0 .. i - 1], exceeds
  *   d_uniform[r][i] times all of it (numbers below 0 and NaN as 0; from 1 on: the last token that stays); -1 where no token is left.
  *   d_logprobs (NULL: not wanted): log p of it, -inf for -1.
- * pa_verify_drafts: rows are nodes of drafted trees (pa_draft_trees; d_node_start [num_seqs + 1], d_row_seq not NULL).  The children of node r (at most
+ * pa_verify_drafts: rows are nodes of drafted trees (pa_draft_trees; d_node_start [num_seqs + 1], d_row_seq not NULL).  The children of node r (the first
  *   most_children of any node), in order, were drawn from q = row d_draft_rows[r] (NULL: r) of d_draft (of draft_type, rows draft_stride apart): each from all of it, or
  *   with `distinct` from what the ones before it left.  One after the other a child c is kept, where d_uniform[c][0] q(c) S < max(p(c) -
  *   a q(c), 0) (1 - Q), or refused (a += S / (1 - Q), S = sum max(p - a q, 0), with `distinct` Q += q(c); from a = 0, S = 1, Q = 0).

@@ -100,7 +100,7 @@ struct Args {
     const int32_t *tokens, *parents, *node_start, *draft_rows;      // nodes of drafted trees
     const void* draft;
     int64_t draft_stride;
-    int draft_count, distinct;
+    int draft_count, distinct, most_children;
 };
 
 template <typename T> __device__ __forceinline__ float widen(T v) { return to_f32<T>(v); }
@@ -1584,7 +1584,7 @@ struct Finish : Weigher {
                     n += __popc(who);
                 }
             }
-            if (lane == 0) sh.children = min(n, PA_TREE_MOST_NODES);
+            if (lane == 0) sh.children = min(n, a.most_children);       // (of more there would be no round)
         }
         __syncthreads();
     }
@@ -1876,7 +1876,7 @@ template <typename T, typename Q, int MODE> static int launch(Args a, int type, 
         a.opened = a.open + most_children + 1;
     }
     a.group = c.group;
-    a.round = most_children;
+    a.round = a.most_children = most_children;
     const int rows = a.rows;
     for (int r = 0; r < rows; r += c.group) {
         a.row0 = r;

@@ -386,6 +386,28 @@ def test_refused_tensors():
 
 
 @pytest.mark.gpu
+def test_more_children_than_said():
+    """Children beyond the number that the call was told count as not there."""
+    from llm_decoder import DraftTree, _cabi, sampling
+    g = torch.Generator(device="cuda").manual_seed(4)
+    n, V = 200, 50
+    x, q = torch.randn(3 * n, V, device="cuda", generator=g), torch.rand(3 * n, V, device="cuda", generator=g)
+    q /= q.sum(1, keepdim=True)
+    u, tokens = torch.rand(3 * n, 2, device="cuda", generator=g), np.random.default_rng(1).integers(0, V, (n, 2)).tolist()
+    tree = DraftTree([[-1, 0, 0]] * n, [[0, *t] for t in tokens], "cuda")
+    ids, ws = torch.full((3 * n,), -7, dtype=torch.int32, device="cuda"), torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    rules = _cabi.DrawRules(num_seqs=n, temperature=1.0, top_p=1.0)
+    rules.row_seq = tree.row_seq.data_ptr()
+    _cabi.check(_cabi.lib().pa_verify_drafts(x.data_ptr(), 0, V, 3 * n, V, __import__("ctypes").byref(rules), u.data_ptr(), tree.tokens.data_ptr(), tree.parents.data_ptr(),
+                                             tree.node_start.data_ptr(), 1, q.data_ptr(), 0, V, 3 * n, None, 0, ids.data_ptr(), None, ws.data_ptr(), ws.numel(),
+                                             _cabi.stream()), "pa_verify_drafts")
+    keep = torch.arange(3 * n, device="cuda").view(n, 3)[:, :2].reshape(-1)
+    fewer = DraftTree([[-1, 0]] * n, [[0, t[0]] for t in tokens], "cuda")
+    want = sampling.verify_drafts(x[keep].contiguous(), fewer, u[keep].contiguous(), q[keep].contiguous())
+    assert torch.equal(ids[keep], want) and int(ids.min()) >= 0
+
+
+@pytest.mark.gpu
 def test_two_calls_at_once():
     """Calls of several host threads on streams of their own, and captured calls that are replayed beside each other, give what each gives alone."""
     import threading
