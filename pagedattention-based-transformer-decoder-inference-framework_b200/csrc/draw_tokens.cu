@@ -1372,7 +1372,9 @@ struct Finish : Weigher {
         if (MASS) above += over(sum, sh.part, Add());
         l = over(low, sh.fpart, Min());
         h = over(high, sh.fpart, Max());
-        return sh.hit;
+        const int some = sh.hit;
+        __syncthreads();                            // (select counts there anew)
+        return some;
     }
     // sh.first: from the chunks' numbers of listed tokens to where they begin
     __device__ void starts() {

@@ -445,3 +445,40 @@ def test_two_calls_at_once():
                 graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+# ---------------------------------------------------------------------------------- rows with thousands of tokens next to the border
+def steps_of(x, temperature):
+    """Which step of 1/32 (of log2 w, or of a logit where these are smaller) every token of a row lies in, counted from the largest."""
+    fine = np.float32(max(1.4426950408889634 / temperature * 32, 32.0)) * np.float32(16)
+    part = np.rint(x.astype(np.float64) * np.float64(fine)).astype(np.int64)
+    return ((part.max() | 15) - part) // 16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed,kind,V,spread,rules", [
+    (0, "f32", 128000, 0.3, dict(top_p=0.9)), (1, "f32", 128000, 0.4, dict(top_p=0.7, temperature=0.8)), (2, "f32", 250001, 0.9, dict(top_p=0.88, temperature=2.0)),
+    (3, "f32", 300001, 1.5, dict(top_p=0.9, temperature=1.5)), (4, "f32", 128000, 0.5, dict(top_k=60000)), (5, "f32", 200003, 0.6, dict(top_k=90000, min_p=0.001)),
+    (6, "f32", 128000, 0.3, dict(top_k=64000)), (7, "f16", 128000, 0.3, dict(top_p=0.9)), (8, "f16", 250001, 0.7, dict(top_k=100000)),
+    (9, "bf16", 160000, 0.35, dict(top_p=0.85)), (10, "bf16", 128000, 0.5, dict(top_k=70000))])
+def test_many_tokens_next_to_the_border(seed, kind, V, spread, rules):
+    """More than 2048 tokens of a row in the border's step, at most 1024 of any 8192 neighbours: narrowed down among themselves, counted or weighed, and
+    summed from their list.  The same each time."""
+    from llm_decoder import sampling
+    c = Case(seed, kind, 3, V, rules, spread=spread)
+    u = torch.from_numpy(c.numbers[:, 0].copy()).cuda()
+    t = c.rules.get("temperature", np.ones(3))
+    probs, (ids, logs) = sampling.truncated_softmax(c.dev, **rules), sampling.draw_tokens(c.dev, u, logprobs=True, **rules)
+    for _ in range(20):
+        again = sampling.draw_tokens(c.dev, u, logprobs=True, **rules)
+        assert torch.equal(again[0], ids) and torch.equal(again[1], logs) and torch.equal(sampling.truncated_softmax(c.dev, **rules), probs)
+    probs, ids = probs.double().cpu().numpy(), ids.tolist()
+    for r in range(3):
+        w, step = c.weights(r), steps_of(c.x[r], t[r])
+        near = step == step[w > 0].max()
+        assert near.sum() > 2048
+        for s in (near, np.isin(step, step[w > 0].max() + np.array([-1, 0, 1]))):
+            assert max(s[i:i + 8192].sum() for i in range(0, V, 1024)) <= 1024
+        p = w / w.sum()
+        assert np.array_equal(probs[r] > 0, p > 0) and near_float(probs[r], p)
+        assert is_drawn(w, ids[r], c.numbers[r, 0])
