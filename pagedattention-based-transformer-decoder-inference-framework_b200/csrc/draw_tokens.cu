@@ -43,7 +43,7 @@
 namespace pa {
 namespace drawn {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kPer = kBins / kThreads, kList = 1024, kMany = 2048, kFew = 256, kOwn = 256, kMostRanks = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kPer = kBins / kThreads, kList = 1024, kMany = 2048, kFew = 256, kOwn = 256, kMostRanks = 8, kElsewhere = -2;
 constexpr int kWords = 8, kMostChunkStrips = kWords * kWarps, kMostStrips = 512, kMostChunks = 512, kGroup = 8192;       // a group of rows has so many chunks
 static_assert(kFew == kThreads && kPer == 4, "a thread for each of few; a word of steps a thread");
 constexpr int kMostRows = 1 << 30;          // (so that a row's number and a little more fit 31 bits)
@@ -1435,12 +1435,12 @@ struct Finish : Weigher {
         return max(__shfl_sync(kAll, hit, who), 0);
     }
 
-    // ---- the first token up to which the sums of f(x, token) exceed `target`; -1 in the CTAs that it is not in.  `part` is where it is
+    // ---- the first token up to which the sums of f(x, token) exceed `target` (-1: none has any), or kElsewhere in the CTAs that it is not in.  `part` is where it is
     // (f of a word's tokens: their weights)
     template <typename F> __device__ int search(double target, bool last, int& part, F f) {
         double run = 0.0, mine = 0.0;
         bool open = true;               // the first that exceeds it, else (by rounding) the last that has anything
-        int owner = by_chunks ? 0 : -1;
+        int owner = 0;
         if (!by_chunks) {
             double t[kMostRanks];
             of_all(&sh.x_total[turn], t, 0.0);
@@ -1458,7 +1458,7 @@ struct Finish : Weigher {
             cluster_arrive();
             left = true;
         }
-        if (owner != rank) return -1;
+        if (owner != rank) return kElsewhere;
         part = locate(by_chunks ? sh.chunk : sh.seg, by_chunks ? a.chunks : kWarps, target, mine);
         const int of = rank * kWarps + part, all = a.ranks * kWarps;
         const int e0 = by_chunks ? part * a.chunk_strips : (int)((int64_t)view.strips * of / all);
@@ -1528,7 +1528,7 @@ struct Finish : Weigher {
             const float u = a.uniform[(int64_t)row * a.count + i];
             int part = 0;
             const int v = search((u > 0.f ? (double)u : 0.0) * total, !by_chunks && i + 1 == a.count, part, f);
-            if (v >= 0 && warp == 0) {
+            if (v != kElsewhere && warp == 0) {
                 const double w = kept(view.at(v), v);
                 if (lane == 0) put(i, v, w / whole);
             }
@@ -1631,7 +1631,7 @@ struct Finish : Weigher {
                     w[e] = u > 0.0 ? u : 0.0;
                 }
         });
-        if (v >= 0 && warp == 0) {
+        if (v != kElsewhere && warp == 0) {
             const double w = kept(view.at(v), v);
             if (lane == 0) put(0, v, w / total);
         }

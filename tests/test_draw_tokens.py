@@ -482,3 +482,36 @@ def test_many_tokens_next_to_the_border(seed, kind, V, spread, rules):
         p = w / w.sum()
         assert np.array_equal(probs[r] > 0, p > 0) and near_float(probs[r], p)
         assert is_drawn(w, ids[r], c.numbers[r, 0])
+
+
+# -------------------------------------------------------------------------------------------------------- temperatures next to 0
+SMALL = [1e-3, 1e-6, 1e-8, 1e-10, 1e-12, 1e-14, 1e-16, 1e-17, 1e-18, 1e-20, 1e-22, 1e-24, 1e-40, 1e-310, 5e-324]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("top_p", [1.0, 0.9])
+@pytest.mark.parametrize("at", [3.3, 28.7, -1e10])
+def test_every_id_is_written(at, top_p):
+    """Ids in memory that holds something else before the call are tokens or -1 after it."""
+    import ctypes
+
+    from llm_decoder import DraftTree, _cabi
+    V, rows = 9001, 12
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(rows, V, device="cuda", generator=g) + at - 3.3
+    x[::2, 77] = at + 1
+    q = torch.softmax(x + torch.randn(rows, V, device="cuda", generator=g), 1)
+    u, ws = torch.rand(rows, 3, device="cuda", generator=g), torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    tree = DraftTree([[-1, 0, 0, 1]] * 3, [[0, 77, 5, 9]] * 3, "cuda")
+    lib = _cabi.lib()
+    for t in SMALL:
+        ids, one = (torch.full(s, -7, dtype=torch.int32, device="cuda") for s in ((rows, 3), (rows,)))
+        rules = _cabi.DrawRules(num_seqs=rows, temperature=t, top_p=top_p)
+        _cabi.check(lib.pa_draw_tokens(x.data_ptr(), 0, V, rows, V, ctypes.byref(rules), u.data_ptr(), 3, ids.data_ptr(), None, ws.data_ptr(), ws.numel(),
+                                       _cabi.stream()), "pa_draw_tokens")
+        rules.row_seq = tree.row_seq.data_ptr()
+        _cabi.check(lib.pa_verify_drafts(x.data_ptr(), 0, V, rows, V, ctypes.byref(rules), u.data_ptr(), tree.tokens.data_ptr(), tree.parents.data_ptr(),
+                                         tree.node_start.data_ptr(), 2, q.data_ptr(), 0, V, rows, None, 0, one.data_ptr(), None, ws.data_ptr(), ws.numel(),
+                                         _cabi.stream()), "pa_verify_drafts")
+        for got in (ids, one):
+            assert int(got.min()) >= -1 and int(got.max()) < V, t
