@@ -158,13 +158,14 @@ __device__ const double kTable[32] = {     // 2^(j/32)
     1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
 };
 __constant__ double kPoly[4] = {0.69314718055994530942, 0.24022650695910071233, 0.05550410866482157995, 0.00961812910762847716};        // ln 2 ^ k / k!
-// 2^y = p s for y of -1022 to 0 (others give some numbers): s = 2^(n/32), from table(n) = 2^(j/32) less j 2^-5 in its exponent's place, j = the low five
-// bits of n, so that n can be added there as it is
-template <typename F> __device__ __forceinline__ double2 exp2_parts(double y, F table) {
+// 2^y = p s for y = d scale of -1022 to 0 (others give some numbers): s = 2^(n/32), from table(n) = 2^(j/32) less j 2^-5 in its exponent's place, j = the
+// low five bits of n, so that n can be added there as it is.  The largest logit is taken away before the scaling (d is exact, or off by 2^-53 of itself): a
+// difference of two products would be off by 2^-53 of the larger, which small temperatures and large logits make more than all of y
+template <typename F> __device__ __forceinline__ double2 exp2_parts(double d, double scale, F table) {
     constexpr double magic = 211106232532992.0;             // 1.5 x 2^47: sums end at multiples of 1/32
-    const double at = y + magic;
+    const double at = fma(d, scale, magic);
     const int n = __double2loint(at);
-    const double r = y - (at - magic), t = table(n);
+    const double r = fma(d, scale, magic - at), t = table(n);
     double p = fma(r, kPoly[3], kPoly[2]);
     p = fma(r, p, kPoly[1]);
     p = fma(r, p, kPoly[0]);
@@ -173,8 +174,8 @@ template <typename F> __device__ __forceinline__ double2 exp2_parts(double y, F 
 }
 __device__ __forceinline__ double table_entry(int j) { return __hiloint2double(__double2hiint(kTable[j]) - (j << 15), __double2loint(kTable[j])); }
 // by all lanes of a warp, lane j of which holds entry j
-__device__ __forceinline__ double exp2_64(double y, double table) {
-    const double2 w = exp2_parts(y, [&](int n) { return __shfl_sync(kAll, table, n); });
+__device__ __forceinline__ double exp2_64(double d, double scale, double table) {
+    const double2 w = exp2_parts(d, scale, [&](int n) { return __shfl_sync(kAll, table, n); });
     return w.x * w.y;
 }
 
@@ -194,7 +195,7 @@ struct Rules {
         m = !known ? 0.0 : a.min_p ? (double)a.min_p[b] : a.min_p1;
         k = !known ? 0 : a.top_k ? a.top_k[b] : a.top_k1;
         if (k >= a.vocab || k < 0) k = 0;
-        scale = greedy() ? 0.0 : 1.4426950408889634074 / t;
+        scale = greedy() ? 0.0 : fmin(1.4426950408889634074 / t, 1e300);        // (a number, that 0 times it is 0: floats differ by 1e-45 or not at all)
         fine = fmaxf((float)(scale * kSteps), kLogitSteps) * kParts;
     }
     __device__ bool greedy() const { return !(t > 0.0); }
@@ -263,13 +264,13 @@ template <typename T> __device__ __forceinline__ float finite(float x) { return 
 struct Block {
     const int tid, warp, lane;
     double table;                   // the lane's entry
-    double scale = 0.0, base = 0.0; // w = 2^(x scale + base)
+    double scale = 0.0, largest = 0.0;      // w = 2^((x - largest) scale)
     __device__ Block() : tid(threadIdx.x), warp(threadIdx.x >> 5), lane(threadIdx.x & 31) { table = table_entry(threadIdx.x & 31); }
     __device__ __forceinline__ void relative_to(float top, double s) {
         scale = s;
-        base = -(double)top * s;
+        largest = top;
     }
-    template <typename T> __device__ __forceinline__ double weight(float x) const { return exp2_64(fma((double)finite<T>(x), scale, base), table); }
+    template <typename T> __device__ __forceinline__ double weight(float x) const { return exp2_64((double)finite<T>(x) - largest, scale, table); }
     template <typename V, typename Op> __device__ V over(V v, V* parts, Op op) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kAll, v, o));
@@ -608,7 +609,7 @@ template <typename T, bool RANGES> __global__ void __launch_bounds__(kThreads, 4
     __shared__ Row s_row;
     __shared__ double s_table[32];
     if (tid < 32) s_table[tid] = b.table;
-    auto exp2_s = [&](float x) { return exp2_parts(fma((double)x, b.scale, b.base), [&](int n) { return s_table[n & 31]; }); };
+    auto exp2_s = [&](float x) { return exp2_parts((double)x - b.largest, b.scale, [&](int n) { return s_table[n & 31]; }); };
     const int s0 = c * a.chunk_strips, s1 = min(s0 + a.chunk_strips, view.strips);
     if (tid == 0) {
         s_listed = 0;

@@ -515,3 +515,62 @@ def test_every_id_is_written(at, top_p):
                                          _cabi.stream()), "pa_verify_drafts")
         for got in (ids, one):
             assert int(got.min()) >= -1 and int(got.max()) < V, t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rules", [dict(), dict(top_p=0.9), dict(top_k=5), dict(min_p=0.2), dict(top_k=400, top_p=0.7)])
+@pytest.mark.parametrize("kind,at", [("f32", 3.3), ("f32", 28.7), ("f32", 1e4), ("f32", -1e10), ("f32", 1e20), ("f32", -3e38), ("bf16", 28.7), ("bf16", 1e20),
+                                     ("f16", -1e4)])
+def test_small_temperatures_and_large_logits(kind, at, rules):
+    """Weights are those of the differences from the largest logit, however small the temperature or large the logits: as numbers and per sequence, with rules
+    and without.  (Where what is left weighs less than 2^-960 of all, a float64 of the definition has no full precision: not looked at.)"""
+    from llm_decoder import DraftTree, sampling
+    rows, V = 6, 20001
+    c = Case(17, kind, rows, V, dict(rules), 1, 1)
+    x = torch.from_numpy(c.x) / 3 * (3 if abs(at) < 100 else abs(at) * (1e-6 if kind == "f32" else 0.01)) + at
+    c.dev.copy_(x.clamp(-c.most, c.most).to(TYPES[kind]))
+    c.x = c.dev.float().cpu().numpy()
+    u = torch.from_numpy(c.numbers[:, :3].copy()).cuda()
+    q = np.full((rows, V), 0.5 / V)
+    q[:, 11] += 0.25
+    q[np.arange(rows), np.argmax(c.x, 1)] += 0.25
+    qd = torch.from_numpy(q.astype(np.float32)).cuda()
+    q = qd.double().cpu().numpy()
+    parents, tokens = [-1, 0, 0, 1, 1, 2], [0, 11, int(np.argmax(c.x[0])), int(np.argmax(c.x[1])), 11, 300]
+    tree, kids = DraftTree([parents], [tokens], "cuda"), [[1, 2], [3, 4], [5], [], [], []]
+    pair = torch.from_numpy(c.numbers[:, 3:5].copy()).cuda()
+    some = [1.0, abs(at) * 1e-6, abs(at) * 1e-8, *SMALL]
+    for form in ("number", "each"):
+        temperatures = [float(np.float32(t)) for t in some if np.float32(t) > 0] if form == "each" else some
+        for i, t in enumerate(temperatures):
+            each = np.full(rows, t)
+            kw = dict(rules, temperature=t)
+            if form == "each":
+                each = np.roll(np.array(temperatures), -i)[:rows].astype(np.float32)
+                kw["temperature"] = torch.from_numpy(each).cuda()
+            c.rules["temperature"] = each
+            probs = sampling.truncated_softmax(c.dev, **kw).double().cpu().numpy()
+            ids, logs = (y.cpu().numpy() for y in sampling.draw_tokens(c.dev, u, logprobs=True, **kw))
+            for r in range(rows):
+                w = c.weights(r)
+                p = w / w.sum()
+                assert near_float(probs[r], p), (t, r)
+                for k, token in enumerate(ids[r]):
+                    if w.sum() < 2.0 ** -960 * p.max():
+                        break
+                    assert is_drawn(w, token, c.numbers[r, k]), (t, r, k)
+                    assert abs(logs[r, k] - math.log(p[token])) <= abs(math.log(p[token])) * 2.0 ** -24 + 3e-12
+                    w = w.copy()
+                    w[token] = 0
+            if form == "each":
+                kw["temperature"] = kw["temperature"][:1].contiguous()
+            got = sampling.verify_drafts(c.dev, tree, pair, qd, **kw).tolist()
+            for r in range(rows):
+                w = kept_weights(c.x[r], most=c.most, temperature=each[0], **rules)
+                token, rest, clear = verified(w, kids[r], tokens, q[r], c.numbers[:, 3], c.numbers[:, 4], False)
+                if clear and token is not None:
+                    assert got[r] == token, (t, r)
+                elif clear:
+                    at_id, cum = got[r], np.cumsum(rest)
+                    target, eps = np.float64(c.numbers[r, 4]) * cum[-1], 1e-9 * cum[-1]
+                    assert rest[at_id] > 0 and cum[at_id] - rest[at_id] - eps <= target < cum[at_id] + eps, (t, r)
