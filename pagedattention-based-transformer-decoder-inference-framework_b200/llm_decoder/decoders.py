@@ -458,6 +458,12 @@ class _DecoderBase:
                 self._prefill(to_device(torch.from_numpy(np.stack(seqs)[:, :-1].copy()), dev), head=False)
             ctx = torch.full((B,), n - 1, dtype=torch.int32, device=dev)
             caches, bufs = TreeCaches(self.kv_caches), None
+
+            def sound():        # asked before tokens are handed out, or found missing
+                if _cabi.lost_waits() != lost:
+                    raise RuntimeError("a kernel gave up on a wait: logits of this call are not valid")
+                if self.pages is not None:
+                    self.pages.check()
             while any(len(s) < n + max_len for s in seqs):
                 parents, tokens, probs = [], [], []
                 for s in seqs:
@@ -515,13 +521,11 @@ class _DecoderBase:
                     self.pages.release(ctx)
                 got = torch.cat((done.counts[:, None], done.tokens), 1).cpu().numpy()       # the step's synchronisation
                 if temperature is not None and any((g[1:1 + g[0]] < 0).any() for g in got):
+                    sound()
                     raise RuntimeError("no token is allowed: nothing to draw from")
                 seqs = [np.concatenate((s, g[1:1 + g[0]]))[:n + max_len] for s, g in zip(seqs, got)]
                 self.drafted_steps_ += 1
-            if _cabi.lost_waits() != lost:      # asked before tokens are handed out
-                raise RuntimeError("a kernel gave up on a wait: logits of this call are not valid")
-            if self.pages is not None:
-                self.pages.check()
+            sound()
             self.positions.copy_(ctx)
             self.ctx_lens.copy_(ctx + 1)
             self.ids.copy_(to_device(torch.from_numpy(np.array([s[-1] for s in seqs], dtype=np.int32)), dev))

@@ -200,3 +200,21 @@ def test_the_command_samples(tmp_path, capsys, cls):
     assert run("--sample", "--drafts", "8", "--temperature", "0.8", "--top-k", "20", "--top-p", "0.9", "--min-p", "0.01", "--seed", "6") == want
     with pytest.raises(SystemExit):
         run("--min-p", "0.1")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", ["CUDADecoder", "INT8Decoder"])
+def test_what_is_wrong_is_what_is_raised(tmp_path, monkeypatch, cls):
+    """Logits from which nothing can be drawn, in a call that found too few pages or whose kernels gave up on a wait: that is what the error says, and "no token"
+    only where neither happened."""
+    from llm_decoder import _cabi
+    dec = decoder(cls, tmp_path, 7, 97, 2, 64, batch_size=2, kv_tokens=64)
+    nothing = np.zeros((2, 4), dtype=np.int32)
+    for n, what in ((50, "too few pages"), (5, "no token is allowed")):
+        with pytest.raises(RuntimeError, match=what):
+            dec.generate_drafted([[3] * n, [4] * n], 20, temperature=0.8, allowed=nothing)
+    assert len(dec.generate_drafted([[3] * 5, [4] * 5], 6, temperature=0.8)[0]) == 11
+    counts = iter(range(9))
+    monkeypatch.setattr(_cabi, "lost_waits", lambda: next(counts))
+    with pytest.raises(RuntimeError, match="gave up on a wait"):
+        dec.generate_drafted([[3] * 5, [4] * 5], 20, temperature=0.8, allowed=nothing)
