@@ -1591,7 +1591,7 @@ struct Finish : Weigher {
         }
         __syncthreads();
     }
-    // true: the node's id is given, or a refused child's rest has to be summed (a.rest)
+    // true: the node's id is given, or a refused child's rest has to be summed (a.rest); false: no child is left
     __device__ bool tests(Rest st, double S) {
         const Q* q = draft_row<Q>(a, row);
         for (int i = st.child; i < sh.children; ++i) {
@@ -1604,14 +1604,12 @@ struct Finish : Weigher {
             }
             st.taken += S / fmax(1.0 - st.out, 1e-18);
             if (a.distinct) st.out += qc;
-            if (S > 0.0) {
-                st.child = i + 1;
-                if (rank == 0 && tid == 0) {
-                    a.rest[local] = st;
-                    a.opened[(int64_t)a.round * a.group + atomicAdd(a.open + a.round, 1)] = local;      // (their order changes nothing)
-                }
-                return true;
+            st.child = i + 1;
+            if (rank == 0 && tid == 0) {
+                a.rest[local] = st;
+                a.opened[(int64_t)a.round * a.group + atomicAdd(a.open + a.round, 1)] = local;      // (their order changes nothing)
             }
+            return true;
         }
         return false;
     }
