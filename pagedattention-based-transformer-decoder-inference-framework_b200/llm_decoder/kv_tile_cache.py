@@ -76,6 +76,7 @@ class KVTileCache:
         one registration per tile serve both, each with rows of its own."""
         if (self.total_pages_, self.tile_size_) != (owner.total_pages_, owner.tile_size_):
             raise ValueError("KVTileCache.share_pages: the pools differ in pages or tile size")
+        self.page_table_.on_host("KVTileCache.share_pages")
         self.page_table_, self.tile_to_page_map_, self._free = owner.page_table_, owner.tile_to_page_map_, owner._free
         self._page_refs, self.mutex_ = owner._page_refs, owner.mutex_
 
@@ -96,6 +97,7 @@ class KVTileCache:
         """Use caller-provided pools [total_pages, tile_size, head_dim] (no copy)."""
         assert key_buffer.shape == value_buffer.shape and key_buffer.is_contiguous() and value_buffer.is_contiguous()
         assert key_buffer.dtype == _DTYPES[self.dtype]
+        self.page_table_.on_host("KVTileCache.adopt_buffers")
         self.total_pages_, self.tile_size_, self.head_dim_ = key_buffer.shape
         self.value_dim_ = self.head_dim_
         self.key_buffer_, self.value_buffer_ = key_buffer, value_buffer

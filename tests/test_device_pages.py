@@ -204,3 +204,21 @@ def test_refused_on_the_host():
     assert lib.pa_release_pages(*good, 0x5000, 3, None) == -1
     assert lib.pa_release_pages(*good, None, 2, None) == -1
     assert lib.pa_release_pages(*good, None, 0, None) == 0
+
+
+def test_pools_do_not_change_under_pages_on_the_gpu():
+    """While a DevicePages hands out a cache's pages, the cache takes no other buffers and no other cache's pages: to_host would give its free list pages of the
+    pool it had, or write the other cache's."""
+    import llm_decoder as ld
+    a, b = ld.KVTileCache("f16"), ld.KVTileCache("f16")
+    pool = torch.zeros(4, 16, 64, dtype=torch.float16)
+    for kv in (a, b):
+        kv.adopt_buffers(pool, pool)
+    a.page_table_.device_pages_ = object()
+    free, table = a._free, a.page_table_
+    for call in (lambda: a.adopt_buffers(pool[:2], pool[:2]), lambda: a.share_pages(b)):
+        with pytest.raises(RuntimeError, match="to_host"):
+            call()
+    assert a.total_pages_ == 4 and a._free is free and a.page_table_ is table
+    b.share_pages(a)            # (the other way: one set of pages, handed out on the GPU)
+    assert b.page_table_ is table
