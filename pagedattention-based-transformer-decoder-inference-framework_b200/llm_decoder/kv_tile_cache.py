@@ -76,7 +76,8 @@ class KVTileCache:
         one registration per tile serve both, each with rows of its own."""
         if (self.total_pages_, self.tile_size_) != (owner.total_pages_, owner.tile_size_):
             raise ValueError("KVTileCache.share_pages: the pools differ in pages or tile size")
-        self.page_table_.on_host("KVTileCache.share_pages")
+        if self.page_table_ is not owner.page_table_:
+            self.page_table_.on_host("KVTileCache.share_pages")
         self.page_table_, self.tile_to_page_map_, self._free = owner.page_table_, owner.tile_to_page_map_, owner._free
         self._page_refs, self.mutex_ = owner._page_refs, owner.mutex_
 
