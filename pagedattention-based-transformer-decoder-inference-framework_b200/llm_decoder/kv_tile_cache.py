@@ -388,9 +388,9 @@ class KVTileCache:
                 return
             places = (slots.data_ptr(), R, pt.num_heads_, 1, self.total_pages_ * self.tile_size_, 1)
             positions = torch.zeros(R, dtype=torch.int32, device=table.device)
-        common = (*places, self.head_dim_, new_k.data_ptr(), new_v.data_ptr(),
-                  _cabi.ptr(beam_ids), positions.data_ptr(), R, _cabi.stream())
         with _cabi.on_device(table.device):
+            common = (*places, self.head_dim_, new_k.data_ptr(), new_v.data_ptr(),
+                      _cabi.ptr(beam_ids), positions.data_ptr(), R, _cabi.stream())
             if self.dtype == "f32":
                 assert new_k.dtype == torch.float32
                 st = lib.pa_kv_append_f32(self.key_buffer_.data_ptr(), self.value_buffer_.data_ptr(), *common)

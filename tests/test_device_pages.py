@@ -223,3 +223,34 @@ def test_pools_do_not_change_under_pages_on_the_gpu():
     for _ in range(2):
         b.share_pages(a)        # (the other way: one set of pages, handed out on the GPU)
         assert b.page_table_ is table
+
+
+def test_rows_go_to_the_stream_of_their_device(monkeypatch):
+    """append and what it allocates belong to the pools' device, whichever is current: the stream is asked for where that device is."""
+    import contextlib
+
+    from llm_decoder import KVTileCache, _cabi
+
+    class OnGpu(torch.Tensor):          # (nothing is launched here)
+        is_cuda = property(lambda self: True)
+    here, asked = [], []
+
+    @contextlib.contextmanager
+    def on_device(device):
+        here.append(device)
+        yield
+        here.pop()
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: 0
+    monkeypatch.setattr(_cabi, "on_device", on_device)
+    monkeypatch.setattr(_cabi, "stream", lambda: asked.append(bool(here)) or 0)
+    monkeypatch.setattr(_cabi, "lib", lambda: Library())
+    kv, k = KVTileCache("f16"), torch.zeros(3, 2, 64, dtype=torch.float16).as_subclass(OnGpu)
+    kv.adopt_buffers(torch.zeros(4, 16, 64, dtype=torch.float16), torch.zeros(4, 16, 64, dtype=torch.float16))
+    monkeypatch.setattr(kv.page_table_, "num_heads_", 2)
+    monkeypatch.setattr(kv.page_table_, "d_table_", torch.zeros(8, dtype=torch.int32))
+    kv.append(k, k, torch.zeros(3, dtype=torch.int32))
+    kv.append(k, k, slots=torch.zeros(3, 2, dtype=torch.int32))
+    assert asked == [True, True]
