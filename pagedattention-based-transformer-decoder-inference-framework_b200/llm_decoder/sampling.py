@@ -199,12 +199,18 @@ def adjusted_argmax(logits, history=None, history_start=None, repetition=1.0, pr
     return ids
 
 
+def _matrix(logits):
+    if logits.dim() != 2:
+        raise ValueError("logits: [rows, vocab]")
+    return logits.shape
+
+
 def _draw_rules(logits, temperature, top_k, top_p, min_p, row_seq, tree):
     """(arguments of the logits, pa_draw_rules by reference, what must live until the call) of a call over logits."""
     dev, at, kind = logits.device, logits.get_device(), _LOGIT_TYPES.get(logits.dtype)
-    if logits.dim() != 2 or kind is None or not logits.is_cuda:
+    (rows, V), (stride, one) = _matrix(logits), logits.stride()
+    if kind is None or not logits.is_cuda:
         raise ValueError("logits: [rows, vocab] of float32, float16 or bfloat16 on the GPU")
-    (rows, V), (stride, one) = logits.shape, logits.stride()
     if V == 0 or (rows and ((V > 1 and one != 1) or (rows > 1 and stride < V))):
         raise ValueError("logits: a vocabulary, and rows of consecutive elements that do not overlap")
     if rows and V * logits.element_size() > _MOST_ROW_BYTES:
@@ -262,9 +268,10 @@ def truncated_softmax(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ro
     temperature, top_k, top_p, min_p: a number, or a tensor per sequence (float32; top_k int32).  temperature 0: the lowest index of the
     largest alone; top_k 0, top_p 1, min_p 0 leave nothing out.  row_seq: the sequence of every row (None: row r is sequence r); tree: the rows are the
     nodes of a DraftTree.  out: float32, rows of consecutive elements, no memory of the logits."""
+    shape = _matrix(logits)
     if out is None:
-        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
-    elif out.shape != logits.shape or out.dtype != torch.float32 or out.device != logits.device or \
+        out = torch.empty(shape, dtype=torch.float32, device=logits.device)
+    elif out.shape != shape or out.dtype != torch.float32 or out.device != logits.device or \
             (out.numel() and out.shape[1] > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
         raise ValueError("out: float32 of the logits' shape and device, rows of consecutive elements")
     args = _draw_rules(logits, temperature, top_k, top_p, min_p, row_seq, tree)
@@ -281,7 +288,7 @@ def draw_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
     """Tokens drawn by the numbers `uniform` (float32 in [0, 1), [rows] or [rows, n]) from the distributions of truncated_softmax: int32 of uniform's
     shape (pa_draw_tokens).  The first token up to which the probabilities exceed the number; of n numbers a row each draws from what the ones
     before it left (n different tokens); -1 where nothing is left.  logprobs=True: (ids, log p of them, float32, -inf for -1)."""
-    rows = logits.shape[0]
+    rows = _matrix(logits)[0]
     if uniform.dim() not in (1, 2) or uniform.shape[0] != rows or uniform.dtype is not torch.float32 or uniform.device != logits.device or \
             not uniform.is_contiguous():
         raise ValueError(f"uniform: contiguous float32 [{rows}] or [{rows}, n] on {logits.device}")
@@ -308,7 +315,7 @@ def verify_drafts(logits, tree, uniform, draft_probs, draft_rows=None, temperatu
     draft_rows[r] outside [0, n): children that were not drawn by chance (lookup_drafts); the id is drawn as by draw_tokens.
     uniform: float32 [rows, 2] in [0, 1): for the test of the node itself, and for the draw at it.  The rules are those of truncated_softmax,
     per sequence of the tree.  logprobs=True: (ids, log p of them)."""
-    rows, V, dev = *logits.shape, logits.device
+    rows, V, dev = *_matrix(logits), logits.device
     if tree.tokens is None:
         raise ValueError("tree: one with tokens")
     kind = _LOGIT_TYPES.get(draft_probs.dtype)

@@ -574,3 +574,14 @@ def test_small_temperatures_and_large_logits(kind, at, rules):
                     at_id, cum = got[r], np.cumsum(rest)
                     target, eps = np.float64(c.numbers[r, 4]) * cum[-1], 1e-9 * cum[-1]
                     assert rest[at_id] > 0 and cum[at_id] - rest[at_id] - eps <= target < cum[at_id] + eps, (t, r)
+
+
+def test_logits_of_no_rows_are_refused():
+    """Logits that are no matrix raise what other wrong arguments raise, with `out` and without."""
+    from llm_decoder import sampling
+    for shape in ((10,), (), (2, 3, 4)):
+        x = torch.zeros(shape)
+        for call in (lambda: sampling.truncated_softmax(x), lambda: sampling.truncated_softmax(x, out=torch.zeros(shape)), lambda: sampling.draw_tokens(x, torch.zeros(10)),
+                     lambda: sampling.verify_drafts(x, None, torch.zeros(10, 2), torch.zeros(10, 10))):
+            with pytest.raises(ValueError):
+                call()
