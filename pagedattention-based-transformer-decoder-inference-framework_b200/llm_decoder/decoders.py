@@ -33,6 +33,7 @@ synchronisation); the steady-state step is captured in a CUDA graph.
 import copy
 import json
 import os
+from numbers import Real
 
 import numpy as np
 import torch
@@ -437,14 +438,14 @@ class _DecoderBase:
             lost = _cabi.lost_waits()
             def on_device(x, dtype):
                 return x if isinstance(x, torch.Tensor) else to_device(torch.as_tensor(np.asarray(x), dtype=dtype), dev)
-            per_seq = [x if isinstance(x, (int, float)) else on_device(x, torch.float32) for x in (repetition, presence, frequency)]
+            per_seq = [x if isinstance(x, Real) else on_device(x, torch.float32) for x in (repetition, presence, frequency)]
             if bias is not None:
                 bias = [on_device(x, t) for x, t in zip(bias, (torch.int32, torch.float32, torch.int32))]
             if allowed is not None:
                 allowed = on_device(allowed, torch.int32)
-            plain = all(isinstance(x, (int, float)) for x in per_seq) and (*per_seq,) == (1, 0, 0)
+            plain = all(isinstance(x, Real) for x in per_seq) and (*per_seq,) == (1, 0, 0)
             if temperature is not None:
-                of = lambda x, dtype: x if isinstance(x, (int, float)) else on_device(x, dtype)  # noqa: E731
+                of = lambda x, dtype: x if isinstance(x, Real) else on_device(x, dtype)  # noqa: E731
                 chance = dict(temperature=of(temperature, torch.float32), top_k=of(top_k, torch.int32), top_p=of(top_p, torch.float32),
                               min_p=of(min_p, torch.float32))
                 if not self.ARGMAX_DIVIDE:      # logits times the temperature

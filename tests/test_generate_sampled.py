@@ -218,3 +218,14 @@ def test_what_is_wrong_is_what_is_raised(tmp_path, monkeypatch, cls):
     monkeypatch.setattr(_cabi, "lost_waits", lambda: next(counts))
     with pytest.raises(RuntimeError, match="gave up on a wait"):
         dec.generate_drafted([[3] * 5, [4] * 5], 20, temperature=0.8, allowed=nothing)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", ["CUDADecoder", "INT8Decoder"])
+def test_numbers_of_numpy_are_numbers(tmp_path, cls):
+    """Rules given as numpy's scalars, and per sequence, draw what they draw as Python's numbers."""
+    dec = decoder(cls, tmp_path, 7, 97, 2, 64, batch_size=2)
+    prompts, rules = [[3, 5, 7], [2, 4, 6]], dict(temperature=0.75, top_k=20, top_p=0.875, min_p=0.0625, repetition=1.25)
+    want = dec.generate_drafted(prompts, 20, seed=2, **rules)
+    assert dec.generate_drafted(prompts, 20, seed=2, **{k: (np.int64 if k == "top_k" else np.float32)(v) for k, v in rules.items()}) == want
+    assert dec.generate_drafted(prompts, 20, seed=2, **{k: [v, v] for k, v in rules.items()}) == want
