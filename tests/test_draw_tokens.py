@@ -585,3 +585,44 @@ def test_logits_of_no_rows_are_refused():
                      lambda: sampling.verify_drafts(x, None, torch.zeros(10, 2), torch.zeros(10, 10))):
             with pytest.raises(ValueError):
                 call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("distinct", [False, True])
+@pytest.mark.parametrize("seed,kind,V,rules", [(0, "f32", 5001, dict(top_k=30)), (1, "bf16", 20000, dict(top_p=0.8, temperature=1.3)), (2, "f16", 300, dict(min_p=0.05)),
+                                               (3, "f32", 60001, dict(top_k=400, top_p=0.9)), (4, "f32", 12, dict())])
+def test_replacements_are_what_refused_children_leave(seed, kind, V, rules, distinct):
+    """Where every child is refused, the id has weight by the rules and in what the children have left: none that the rules leave out, and none of which
+    the draft gave more than the model does."""
+    from llm_decoder import DraftTree, sampling
+    rng = np.random.default_rng(seed)
+    B, kids = 40, 3
+    c = Case(seed, kind, B * (kids + 1), V, rules)
+    roots = np.arange(B) * (kids + 1)
+    q, tokens = np.zeros((B, V)), np.zeros((B, kids + 1), dtype=np.int64)
+    for b, r in enumerate(roots):       # drafts that like what the model likes less: many children are refused
+        w = c.weights(r)
+        some = rng.permutation(V)[:min(V, 6)]
+        q[b, some] = rng.random(len(some)) + 0.1
+        q[b, rng.choice(np.flatnonzero(w > 0), 3)] += rng.random(3)
+        q[b] /= q[b].sum()
+        tokens[b, 1:] = rng.choice(V, kids, replace=False, p=q[b])
+    qd = torch.from_numpy(q.astype(np.float32)).cuda()
+    q = qd.double().cpu().numpy()
+    rows = torch.full((len(c.x),), -1, dtype=torch.int32)
+    rows[::kids + 1] = torch.arange(B, dtype=torch.int32)
+    numbers = np.concatenate([rng.random((len(c.x), 1)) ** 0.25, rng.random((len(c.x), 1))], 1).astype(np.float32)
+    tree = DraftTree([[-1, 0, 0, 0]] * B, tokens.tolist(), "cuda")
+    ids = sampling.verify_drafts(c.dev, tree, torch.from_numpy(numbers).cuda(), qd, draft_rows=rows.cuda(), distinct=distinct, **rules).tolist()
+    replaced = 0
+    for b, r in enumerate(roots):
+        w = c.weights(r)
+        token, rest, clear = verified(w, list(range(r + 1, r + kids + 1)), tokens.reshape(-1), q[b], numbers[:, 0], numbers[:, 1], distinct)
+        if clear and token is None:
+            replaced += 1
+            cum, at = np.cumsum(rest), ids[r]
+            target, eps = numbers[r, 1] * cum[-1], 1e-9 * cum[-1]
+            assert w[at] > 0 and rest[at] > 0 and cum[at] - rest[at] - eps <= target < cum[at] + eps
+        elif clear:
+            assert ids[r] == token
+    assert replaced >= B // 4

@@ -229,3 +229,39 @@ def test_numbers_of_numpy_are_numbers(tmp_path, cls):
     want = dec.generate_drafted(prompts, 20, seed=2, **rules)
     assert dec.generate_drafted(prompts, 20, seed=2, **{k: (np.int64 if k == "top_k" else np.float32)(v) for k, v in rules.items()}) == want
     assert dec.generate_drafted(prompts, 20, seed=2, **{k: [v, v] for k, v in rules.items()}) == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", ["CUDADecoder", "INT8Decoder"])
+@pytest.mark.parametrize("rules", [dict(temperature=0.7), dict(temperature=1.3, top_p=0.8), dict(temperature=1.0, top_k=9, min_p=0.02)])
+def test_tokens_are_those_of_the_logits_of_their_step(tmp_path, monkeypatch, cls, rules):
+    """Every node's id is drawn by its number from the very logits of its row, to the draws' own bound, and the tokens of a sequence are the ids along the paths
+    that were taken, each drawn by the number of its place."""
+    from test_draw_tokens import is_drawn
+
+    from llm_decoder import sampling
+    dec, n, more, seed = decoder(cls, tmp_path, 5, 97, 2, 64, batch_size=2), 6, 30, 11
+    plain, calls = sampling.draw_tokens, []
+
+    def draw_tokens(logits, u, tree, **kw):
+        ids = plain(logits, u, tree=tree, **kw)
+        calls.append((logits.float().cpu().numpy(), u.cpu().numpy(), kw, tree, ids.cpu().numpy()))
+        return ids
+    monkeypatch.setattr(sampling, "draw_tokens", draw_tokens)
+    prompts = np.random.default_rng(3).integers(0, 97, (2, n)).tolist()
+    got = dec.generate_drafted(prompts, more, drafts=10, branches=3, seed=seed, **rules)
+    given, at = numbers_of(seed, 2, more), [n, n]
+    for logits, u, kw, tree, ids in calls:
+        for row, number, token in zip(logits, u, ids):
+            w = kept_weights(row, **kw)
+            assert is_drawn(w, token, number)
+        first = np.concatenate([[0], np.cumsum(tree.sizes)])
+        parents, tokens = tree.parents.cpu().numpy(), tree.tokens.cpu().numpy()
+        for b in range(2):
+            node = 0 if tree.sizes[b] else None
+            while node is not None and at[b] < n + more:
+                r = first[b] + node
+                assert u[r] == given[b, at[b] - n] and got[b][at[b]] == ids[r]
+                at[b] += 1
+                node = next((k for k in range(node + 1, tree.sizes[b]) if parents[first[b] + k] == node and tokens[first[b] + k] == ids[r]), None)
+    assert at == [n + more] * 2
