@@ -1024,8 +1024,9 @@ struct Finish : Weigher {
                     };
                     auto bounds = [&](int b, uint32_t n, uint32_t, double& l, double& m) {
                         const uint64_t k0 = min((uint64_t)b << shift, (uint64_t)range), k1 = min(((uint64_t)(b + 1) << shift) - 1, (uint64_t)range);
-                        m = n * weight(of_spared(k_hi - (uint32_t)k0)) * (1.0 + 1e-10);
-                        l = n * weight(of_spared(k_hi - (uint32_t)k1)) * (1.0 - 1e-10);
+                        // (the least value need not be one of the type, whose next one below has no weight in 64 bits, nor any number for it)
+                        m = n * weight(fmaxf(of_spared(k_hi - (uint32_t)k0), r.r_lo)) * (1.0 + 1e-10);
+                        l = n * weight(fmaxf(of_spared(k_hi - (uint32_t)k1), r.r_lo)) * (1.0 - 1e-10);
                     };
                     weigh<MASS, 4>(first, r.limit, r.above, r.above_n, from, to, counted, bounds);
                     if (tid == 0) {

@@ -626,3 +626,28 @@ def test_replacements_are_what_refused_children_leave(seed, kind, V, rules, dist
         elif clear:
             assert ids[r] == token
     assert replaced >= B // 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("top_p", [0.3, 0.9, 0.99])
+@pytest.mark.parametrize("kind,at,V", [("f16", 1000, 300), ("f16", 1000, 30001), ("f16", -1000, 5000), ("f16", 30000, 7), ("f16", -60000, 20000), ("bf16", 100, 30001),
+                                       ("bf16", 1000, 9000), ("bf16", -1e4, 500), ("bf16", 1e6, 40000), ("f32", 1e6, 9000)])
+def test_coarse_logits_far_from_zero(kind, at, V, top_p):
+    """Logits with a common offset, next to which their type has few values: a share of them is that of the definition where the least value with a weight is
+    none of the type.  Temperatures from half a step of the type to 30 of them."""
+    from llm_decoder import sampling
+    rows = 40
+    step = 2.0 ** (math.floor(math.log2(abs(at))) + 1) * {"f32": 2.0 ** -23, "f16": 2.0 ** -10, "bf16": 2.0 ** -7}[kind] / 2
+    c = Case(23, kind, rows, V, dict(top_p=top_p))
+    g = torch.from_numpy(np.random.default_rng(2).standard_normal((rows, V)) * step * 2 + at)
+    c.dev.copy_(g.clamp(-c.most, c.most).float().to(TYPES[kind]))
+    c.x = c.dev.float().cpu().numpy()
+    c.rules["temperature"] = np.exp(np.linspace(math.log(step / 2), math.log(step * 30), rows)).astype(np.float32)
+    kw = dict(top_p=top_p, temperature=torch.from_numpy(c.rules["temperature"]).cuda())
+    probs = sampling.truncated_softmax(c.dev, **kw).double().cpu().numpy()
+    ids = sampling.draw_tokens(c.dev, torch.from_numpy(c.numbers[:, 0].copy()).cuda(), **kw).tolist()
+    for r in range(rows):
+        w = c.weights(r)
+        p = w / w.sum()
+        assert np.array_equal(probs[r] > 0, p > 0) and near_float(probs[r], p), r
+        assert is_drawn(w, ids[r], c.numbers[r, 0]), r
