@@ -651,3 +651,14 @@ def test_coarse_logits_far_from_zero(kind, at, V, top_p):
         p = w / w.sum()
         assert np.array_equal(probs[r] > 0, p > 0) and near_float(probs[r], p), r
         assert is_drawn(w, ids[r], c.numbers[r, 0]), r
+
+
+def test_limits_are_those_of_the_library():
+    """Where Python refuses, the library does."""
+    from llm_decoder import _cabi, device_pages, sampling
+    lib, most = _cabi.lib(), sampling._MOST_ROW_BYTES
+    for kind, size in ((0, 4), (1, 2), (2, 2)):
+        assert lib.pa_draw_workspace_bytes(kind, 1, most // size, 0) > 0 and lib.pa_draw_workspace_bytes(kind, 1, most // size + 1, 0) == 0
+    n = device_pages.MOST_SEQS + 1
+    table = (0x1000, n, 2, 4, 16, 8, 0x2000, 0x3000, 0x4000)
+    assert lib.pa_take_pages(*table, 0x5000, 0x6000, n, 1, 0x7000, 0x8000, 0x9000, None) == lib.pa_release_pages(*table, 0x5000, n, None) == -2
