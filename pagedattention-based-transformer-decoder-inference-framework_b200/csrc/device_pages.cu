@@ -8,8 +8,8 @@
 // Integers and few bytes: the floor is a launch and two dependent trips to memory.  Every CTA sums the sequences' tiles by itself (a scan in shared
 // memory), because waiting for another CTA's sums would take as long; then the CTAs share the table's entries and the rows.  Nobody writes what
 // others still read: counts and held tiles change by the CTA that is the last to have read them (an ordered count, 2 us where there are several).
-// Replayed, a take and the release that undoes it: one sequence and 8 rows 8 us; 128 of 8192 tokens and 4096 rows 14; 32 prompts, 135000 rows of 32 heads 25
-// (of which 4.4 for writing the slots): there the slots' addresses, a thread for a head of neighbouring rows (35 with a thread a slot).
+// Replayed, a take and the release that undoes it: one sequence and 8 rows 8 us; 128 of up to 8192 tokens and 2614 rows 14; 32 prompts, 164435 rows of 32
+// heads 25 (4.4 is the floor of all bytes, 3.2 of it the slots): there the slots' addresses, a thread for a head of neighbouring rows (35 with a thread a slot).
 #include <climits>
 
 #include "dynamic_smem.cuh"

@@ -19,16 +19,19 @@
 // the table's word a weight takes 9.4 cycles of an SM for 32 tokens (8.2 with the table in shared memory, which is better where all of a row is
 // summed; 10.3 with the conversion by whole numbers): 35 us for 256 rows of 128000, against 20 for reading them.
 //
-// Rows are read in chunks of up to 64 strips (8192 tokens) by CTAs that know nothing of each other, from memory once and from L2 once more:
+// Rows are read in chunks of up to 64 strips (8192 tokens) by CTAs that know nothing of each other, from memory once and, as far as L2 holds them
+// (256 rows of 128000 floats, 131 MB, are more than that), from there once more:
 //   count   (where a rule needs it) every chunk's largest logit, and its tokens by 1024 steps of 1/32 in log2 w
 //   range   (a CTA a row) the least value that is kept lies in one or two of these steps: found from bounds of their weights, without sorting
 //   sum     the weights of what is above those steps, in 64 bits, and a list of what is in them
 //   finish  (a cluster of CTAs a row) the border among the listed tokens, the sums of the chunks, the tokens that the numbers draw; verification
 //   write   probabilities
-// Rows that this does not settle (more tokens than the lists hold, of logits that lie closer than a step; temperatures far from 1; a share of what
-// a top_k of more than kFew leaves) are searched by finish itself, by finer steps: 30 us more for one row of 128000, 1 to 1.4 a row for 256.
+// Rows that this does not settle are searched by finish itself, by finer steps: 30 us more for one row of 128000, 1 to 1.4 a row for 256.  These are rows
+// with more tokens next to the border than the lists hold (logits that lie closer than a step); a share of what a top_k of more than kFew leaves; and
+// rows whose largest logit lies outside the grid of the steps, which is one of x itself, so that chunks need not know it: |top| of 2840 T (4096 where T
+// is above 1.4) and more, infinity too, and T outside 1.4e-6 to 1.4e6.
 //
-// 256 rows of 128000 float logits, rules of their own, replayed: 103 us (the first form, a cluster of CTAs a row that read it four times: 352; one that
+// 256 rows of 128000 float logits, rules of their own, replayed: 102 us (the first form, a cluster of CTAs a row that read it four times: 352; one that
 // kept it in shared memory: 152, better below 64 rows (one row 25 us against 31), but an SM waits there while one CTA of the cluster
 // looks for the border).  Each kernel begins while the one before ends (programmatic launches), which hides their 4 us each.
 #include <algorithm>
