@@ -559,7 +559,7 @@ def test_small_temperatures_and_large_logits(kind, at, rules):
                     if w.sum() < 2.0 ** -960 * p.max():
                         break
                     assert is_drawn(w, token, c.numbers[r, k]), (t, r, k)
-                    assert abs(logs[r, k] - math.log(p[token])) <= abs(math.log(p[token])) * 2.0 ** -24 + 3e-12
+                    assert abs(float(logs[r, k]) - math.log(p[token])) <= abs(math.log(p[token])) * 2.0 ** -24 + 3e-12
                     w = w.copy()
                     w[token] = 0
             if form == "each":
