@@ -71,6 +71,8 @@ class DevicePages:
 
     def _vector(self, x, n, what):
         if not isinstance(x, torch.Tensor):
+            if _cabi.capturing(_cabi.stream_on(self.device)):       # (a replay would copy what the staging buffer holds by then)
+                raise RuntimeError(f"{what}: a tensor on {self.device} while a graph is captured")
             x = to_device(torch.as_tensor(np.asarray(x), dtype=torch.int32), self.device)
         if x.dtype is not torch.int32 or x.dim() != 1 or (n is not None and x.numel() != n) or x.device != self.device or not x.is_contiguous():
             raise ValueError(f"{what}: a contiguous int32 vector{'' if n is None else f' of {n}'} on {self.device}")
@@ -85,7 +87,7 @@ class DevicePages:
     def take(self, lengths, start, rows):
         """Room for new rows start[b] .. start[b + 1] - 1 (`rows` of them in all) behind the first lengths[b] tokens of table row b, for all b below
         len(lengths): tiles that they need and that have no page get one (pa_take_pages).  lengths, start: int32 device tensors, or
-        sequences of ints.  NewRows(row_seq [rows], positions [rows], slots [rows, heads]); a slot is a row of the pool, or -1 where there
+        sequences of ints (not while a graph is captured).  NewRows(row_seq [rows], positions [rows], slots [rows, heads]); a slot is a row of the pool, or -1 where there
         is no page: too few pages, or more tokens than the table has tiles for, and the call hands out none (`check`)."""
         self._mine("take")
         lengths = self._sizes(lengths, "take")

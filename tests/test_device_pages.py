@@ -254,3 +254,22 @@ def test_rows_go_to_the_stream_of_their_device(monkeypatch):
     kv.append(k, k, torch.zeros(3, dtype=torch.int32))
     kv.append(k, k, slots=torch.zeros(3, 2, dtype=torch.int32))
     assert asked == [True, True]
+
+
+@pytest.mark.gpu
+def test_captured_calls_take_tensors():
+    """Numbers of the host are copied once, by way of a buffer that others use next: a captured call is refused them, and what was captured before replays."""
+    import llm_decoder as ld
+    pt = ld.PageTable()
+    pt.init(2, 2, 4)
+    pages = ld.DevicePages(pt, 16, 16)
+    lengths, start = torch.tensor([20, 0], dtype=torch.int32, device="cuda"), start_of([3, 4])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: pages.take([20, 0], start, 7), lambda: pages.take(lengths, [0, 3, 7], 7), lambda: pages.release([20, 0])):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+        new = pages.take(lengths, start, 7)
+    graph.replay()
+    assert new.positions.tolist() == [20, 21, 22, 0, 1, 2, 3] and pages.free_pages() == 16 - 2 * 3
+    assert pages.take([20, 0], [0, 3, 7], 7).slots.tolist() == new.slots.tolist()
