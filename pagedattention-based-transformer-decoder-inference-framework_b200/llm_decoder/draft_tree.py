@@ -122,6 +122,8 @@ _workspaces = _cabi.PerThread()         # of pa_tree_attention: one for the cach
 
 def _vector(x, n, device, what):
     if not isinstance(x, torch.Tensor):
+        if device.type == "cuda" and _cabi.capturing(_cabi.stream_on(device)):       # (a replay would copy what the staging buffer holds by then)
+            raise RuntimeError(f"{what}: a tensor on {device} while a graph is captured")
         x = to_device(torch.as_tensor(np.asarray(x), dtype=torch.int32), device)
     if x.dtype is not torch.int32 or x.shape != (n,) or x.device != device or not x.is_contiguous():
         raise ValueError(f"{what}: a contiguous int32 vector of {n} on {device}")
@@ -132,7 +134,7 @@ def paged_tree_attention(q, kv_cache, tree, ctx_lens, temperature=1.0, beam_ids=
     """Attention of the nodes of `tree` over the pages of `kv_cache` (pa_tree_attention): q [rows, heads, D] (rows may be a view of a
     wider projection); row r of sequence b sees the first ctx_lens[b] cached tokens and, of the nodes behind them, those of its mask.
     heads is a multiple of the cache's heads.  beam_ids: table row per sequence (None: b).  ctx_lens, beam_ids: int32 device tensors,
-    or sequences of ints.  out: [rows, heads, D] like q, contiguous.
+    or sequences of ints (not while a graph is captured).  out: [rows, heads, D] like q, contiguous.
 
     Up to 1024 sequences, heads of 64 or 128, pages of 16 rows (or multiples) that are not float; what is beyond goes through the general kernel, some
     forty times as slow where contexts are long.  Partial results are kept in a workspace per host thread and stream."""

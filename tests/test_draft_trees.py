@@ -368,3 +368,28 @@ def test_accept_without_caches_and_refusals():
         ld.TreeCaches(kv)
     nothing = ld.tree_accept(ids[:0], ld.DraftTree([[], []], [[], []], device="cuda"), [], [3, 8])
     assert nothing.counts.tolist() == [0, 0] and nothing.ctx_lens.tolist() == [3, 8] and nothing.tokens.shape == (2, 0)
+
+
+@pytest.mark.gpu
+def test_captured_calls_take_tensors():
+    """Numbers of the host come by way of a staging buffer that the next calls write: a captured call is refused them."""
+    import llm_decoder as ld
+    kv = ld.KVTileCache("f16")
+    kv.init(8, 16, 64)
+    kv.configure_table(1, 2, 4)
+    kv.register_range(0, 0, 1)
+    tree, q = ld.DraftTree([[-1, 0]], [[5, 6]], "cuda:0"), torch.randn(2, 2, 64, device="cuda")
+    ids, ctx = torch.tensor([6, 7], dtype=torch.int32, device="cuda"), torch.tensor([3], dtype=torch.int32, device="cuda")
+    caches = ld.TreeCaches([kv])
+    want = ld.tree_accept(ids, tree, caches, [3]).ctx_lens.tolist()
+    ld.paged_tree_attention(q, kv, tree, [3])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: ld.paged_tree_attention(q, kv, tree, [3]), lambda: ld.paged_tree_attention(q, kv, tree, ctx, beam_ids=[0]),
+                     lambda: ld.tree_accept(ids, tree, caches, [3]), lambda: ld.tree_accept([6, 7], tree, caches, ctx)):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+        done = ld.tree_accept(ids, tree, caches, ctx)
+    graph.replay()
+    assert done.ctx_lens.tolist() == want == [5]
