@@ -87,8 +87,8 @@ class DevicePages:
     def take(self, lengths, start, rows):
         """Room for new rows start[b] .. start[b + 1] - 1 (`rows` of them in all) behind the first lengths[b] tokens of table row b, for all b below
         len(lengths): tiles that they need and that have no page get one (pa_take_pages).  lengths, start: int32 device tensors, or
-        sequences of ints (not while a graph is captured).  NewRows(row_seq [rows], positions [rows], slots [rows, heads]); a slot is a row of the pool, or -1 where there
-        is no page: too few pages, or more tokens than the table has tiles for, and the call hands out none (`check`)."""
+        sequences of ints (not while a graph is captured).  NewRows(row_seq [rows], positions [rows], slots [rows, heads]); a slot is a row of the
+        pool, or -1 where there is no page: too few pages, or more tokens than the table has tiles for, and the call hands out none (`check`)."""
         self._mine("take")
         lengths = self._sizes(lengths, "take")
         B, rows, H = lengths.numel(), int(rows), self.table.num_heads_
